@@ -36,6 +36,7 @@ __all__ = [
     "LatentSpec", "latent_append", "latent_attention", "latent_gather", "latent_prefill", "latent_queries",
     "Decay", "linear_attention", "low_rank", "token_mix",
     "Act", "ScoreMods", "HeadRecurrence", "ShortConv", "head_recurrence", "gated_group_norm", "short_conv",
+    "QuantizedPages",
     "KernelLibraryError", "device_status", "raise_on_device_error", "native_available", "launch_count",
     "reset_launch_count",
 ]
@@ -647,7 +648,10 @@ def rope_kv_append(
 
     qkv is bf16 ``[T, W]`` or fp32 split-K partials ``[S, T, W]``.  Cache layout
     ``[num_blocks, nkv, block_size, head_dim]``; slot = block * block_size + offset
-    (negative slot = do not store)."""
+    (negative slot = do not store).  `QuantizedPages` in the place of both caches keep keys and values in 8 bits."""
+    if _quantized(k_cache, v_cache):
+        return quantized_kv.rope_kv_append(qkv, positions, slots, cos_sin, k_cache, v_cache, nq, nkv, head_dim, bias=bias,
+                                           q_norm_w=q_norm_w, k_norm_w=k_norm_w, norm_eps=norm_eps, q_out=q_out)
     partial = qkv.dtype == torch.float32
     T = qkv.shape[-2]
     W = (nq + 2 * nkv) * head_dim
@@ -905,6 +909,10 @@ def _mods_ref(mods: Optional[ScoreMods]):
     return ctypes.byref(mods.arg()) if mods else None
 
 
+def _quantized(k_cache, v_cache) -> bool:
+    return isinstance(k_cache, QuantizedPages) or isinstance(v_cache, QuantizedPages)
+
+
 def _gather_kv(cache: torch.Tensor, table_row: torch.Tensor, ctx: int) -> torch.Tensor:
     """[ctx, nkv, D] view of one sequence's cached K or V (reference path)."""
     bs = cache.shape[2]
@@ -988,7 +996,11 @@ def paged_attn_decode(
     """Decode attention over the paged cache.  q ``[B * q_len, nq * D]`` (the q_len
     newest tokens of each sequence, already appended to the cache);
     context_lens counts them.  Causal among the new tokens; window > 0: a query sees itself and the window - 1 tokens
-    before it; chunk > 0: only the positions of its own chunk of that many; mods: see `ScoreMods`."""
+    before it; chunk > 0: only the positions of its own chunk of that many; mods: see `ScoreMods`.  The caches may be
+    `QuantizedPages` (without mods)."""
+    if _quantized(k_cache, v_cache):
+        return quantized_kv.paged_attn_decode(q, k_cache, v_cache, block_table, context_lens, scale, q_len=q_len, window=window, chunk=chunk,
+                                              sinks=sinks, mods=mods, num_splits=num_splits, scratch=scratch, out=out)
     nkv, bs, D = k_cache.shape[1], k_cache.shape[2], k_cache.shape[3]
     B = block_table.shape[0]
     nq = q.shape[-1] // D
@@ -1073,7 +1085,11 @@ def rope_attn_decode(
 
     qkv_partials is the fp32 split-K output ``[S, B, (nq + 2 nkv) * D]`` of the fused QKV projection.  The kernel
     sums it, adds the bias, applies QK-norm and RoPE, stores the new key and value at ``slots`` and attends over the
-    cache pages plus the new token.  Returns ``[B, nq * D]`` bf16."""
+    cache pages plus the new token.  Returns ``[B, nq * D]`` bf16.  With `QuantizedPages` the new token takes part as it is kept there."""
+    if _quantized(k_cache, v_cache):
+        return quantized_kv.rope_attn_decode(qkv_partials, positions, slots, cos_sin, k_cache, v_cache, block_table, context_lens, scale,
+                                             nq, nkv, bias=bias, q_norm_w=q_norm_w, k_norm_w=k_norm_w, norm_eps=norm_eps, window=window,
+                                             sinks=sinks, num_splits=num_splits, scratch=scratch, out=out)
     D = k_cache.shape[3]
     B = block_table.shape[0]
     if out is None:
@@ -1130,7 +1146,11 @@ def flash_attn_prefill(
     """Blockwise prefill attention.  q ``[total_q, nq * D]`` packs the new tokens of
     all sequences (sequence b owns rows q_start[b] .. q_start[b] + q_lens[b]); K/V
     of the whole context (cached prefix + new tokens) are read from the paged
-    cache.  Query i of a sequence sits at position context_len - q_len + i.  mods: see `ScoreMods`."""
+    cache.  Query i of a sequence sits at position context_len - q_len + i.  mods: see `ScoreMods`.  The
+    caches may be `QuantizedPages` (without mods)."""
+    if _quantized(k_cache, v_cache):
+        return quantized_kv.flash_attn_prefill(q, k_cache, v_cache, block_table, q_start, q_lens, context_lens, scale, max_q_len=max_q_len,
+                                               causal=causal, window=window, chunk=chunk, sinks=sinks, mods=mods, out=out)
     nkv, bs, D = k_cache.shape[1], k_cache.shape[2], k_cache.shape[3]
     B = block_table.shape[0]
     total_q = q.shape[0]
@@ -1439,6 +1459,8 @@ from .mixers import (Act, Branch, MapsSpec, Norm, Proj, activation, gate_heads, 
 from .latent_attention import (LatentSpec, latent_append, latent_attention, latent_gather,  # noqa: E402,F401
                                latent_prefill, latent_queries)
 from .linear_attention import Decay, linear_attention, low_rank, token_mix  # noqa: E402,F401
+from . import quantized_kv  # noqa: E402
+from .quantized_kv import QuantizedPages  # noqa: E402
 from .head_recurrence import (HeadRecurrence, ShortConv, gated_group_norm, head_recurrence,  # noqa: E402,F401
                               short_conv)
 

@@ -44,7 +44,8 @@ NVCC_FLAGS = [
 # GEMM epilogue and the attention softmax want; the normalisation and sampling
 # files keep IEEE division and sqrt.
 NO_FAST_MATH = {"sampling.cu", "elementwise.cu", "decode_layer.cu", "gated_residual.cu", "recurrent.cu", "attn_maps.cu",
-                "gemm_simt.cu", "gemm_f32_split.cu", "linear_attn.cu", "latent_attn.cu", "head_recurrence.cu", "post_residual.cu"}
+                "gemm_simt.cu", "gemm_f32_split.cu", "linear_attn.cu", "latent_attn.cu", "head_recurrence.cu", "post_residual.cu",
+                "append_q8.cu"}
 
 
 # what a single-GPU decoder of models/hybrid.py launches

@@ -1,0 +1,349 @@
+"""Keys and values kept in 8 bits: the pages, and the operators that write and read them.
+
+A page of 32 tokens of one kv head is e4m3 values ``[32, dim]`` and one power of two per token.  A head's row x is kept as
+``e4m3(x / 2^e)`` (nearest, ties to even) and e, the smallest whole number with ``max|x| <= 448 * 2^e``, between -64 and 64: rows
+beyond 448 * 2^64 saturate, and what is below 2^-74 becomes zero.  A row that holds a value which is not finite stands for NaN as a whole
+(scale NaN, values 0), so that a NaN in a masked place has no way into a sum.
+
+One scale per token and head, because tokens are appended one at a time: a scale that several tokens shared would have to be
+guessed, or change what is stored already.  A power of two, because e4m3 is a floating type: another factor would keep no more
+bits, and this one is undone without a rounding.
+
+The values are rounded once, from sums, norms and rotations in 64 bits, so that a token has the same bytes whichever kernel, or the
+reference on the CPU, writes them.
+
+These functions are reached through `rope_kv_append`, `paged_attn_decode`, `rope_attn_decode`, `flash_attn_prefill` and
+`packed_attention`, which take a `QuantizedPages` wherever they take a cache tensor.  No file of the reference corresponds to
+them (its cache is dense and bf16, examples/models/qwen3/qwen3.py:52-71).
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+
+PAGE = 32
+LOG2_MIN, LOG2_MAX = -64, 64
+DIMS = (64, 128)
+
+
+class QuantizedPages:
+    """Keys or values of one layer: e4m3 `values` [blocks, kv heads, 32, dim] and power-of-two `scales` [blocks, kv heads, 32]
+    (torch.float8_e8m0fnu), both contiguous and on one device."""
+    __slots__ = ("values", "scales", "shape", "device", "is_cuda")
+
+    def __init__(self, values: torch.Tensor, scales: torch.Tensor):
+        if values.dtype is not torch.float8_e4m3fn or scales.dtype is not torch.float8_e8m0fnu:
+            raise TypeError("QuantizedPages wants float8_e4m3fn values and float8_e8m0fnu scales")
+        if values.dim() != 4 or values.shape[2] != PAGE or scales.shape != values.shape[:3]:
+            raise ValueError("QuantizedPages wants values [blocks, kv heads, 32, dim] and scales [blocks, kv heads, 32]")
+        if values.shape[3] not in DIMS:
+            raise ValueError("QuantizedPages has heads of 64 or 128 columns")
+        if not values.is_contiguous() or not scales.is_contiguous() or values.device != scales.device:
+            raise ValueError("QuantizedPages wants contiguous tensors on one device")
+        if (values.data_ptr() | scales.data_ptr()) & 15:
+            raise ValueError("QuantizedPages wants tensors that start on 16 bytes")
+        self.values, self.scales = values, scales
+        self.shape, self.device, self.is_cuda = values.shape, values.device, values.is_cuda
+
+    @classmethod
+    def new(cls, num_blocks: int, kv_heads: int, dim: int, device="cpu") -> "QuantizedPages":
+        """Pages of zeros."""
+        values = torch.zeros((num_blocks, kv_heads, PAGE, dim), dtype=torch.uint8, device=device)
+        scales = torch.full((num_blocks, kv_heads, PAGE), 127, dtype=torch.uint8, device=device)
+        return cls(values.view(torch.float8_e4m3fn), scales.view(torch.float8_e8m0fnu))
+
+    @property
+    def nbytes(self) -> int:
+        return self.values.numel() + self.scales.numel()
+
+    def dequantize(self, blocks: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The values that the pages (of the given blocks) stand for, fp32 [blocks, kv heads, 32, dim]."""
+        v, s = self.values.view(torch.uint8), self.scales.view(torch.uint8)
+        if blocks is not None:
+            v, s = v[blocks], s[blocks]
+        return v.view(torch.float8_e4m3fn).float() * s.view(torch.float8_e8m0fnu).float()[..., None]
+
+
+# --------------------------------------------------------------------------- reference on the CPU
+def _pow2(e: torch.Tensor) -> torch.Tensor:
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
+def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(e4m3 values, scales) of rows [..., dim], computed in 64 bits."""
+    x = x.double()
+    fine = x.isfinite().all(-1)
+    x = torch.where(fine[..., None], x, 0.0)
+    m, e = torch.frexp(x.abs().amax(-1))                          # 448 is 0.875 * 2^9
+    e = torch.where(m == 0, LOG2_MIN, e - 9 + (m > 0.875).int()).clamp(LOG2_MIN, LOG2_MAX)
+    y = x * _pow2(-e)[..., None]
+    step = _pow2((torch.frexp(y)[1] - 1).clamp(min=-6) - 3)
+    y = (torch.round(y / step) * step).clamp(-448.0, 448.0)
+    scales = torch.where(fine, e + 127, 255).to(torch.uint8)
+    return y.float().to(torch.float8_e4m3fn), scales.view(torch.float8_e8m0fnu)
+
+
+def _ref_append(qkv, positions, slots, cos_sin, k_pages, v_pages, nq, nkv, dim, bias, q_norm_w, k_norm_w, eps, q_out):
+    T = qkv.shape[-2]
+    x = qkv.double()
+    x = x.reshape(-1, T, x.shape[-1]).sum(0) if qkv.dtype == torch.float32 else x
+    if bias is not None:
+        x = x + bias.double()
+    x = x.reshape(T, nq + 2 * nkv, dim)
+
+    def turn(t, w):
+        if w is not None:
+            t = t / torch.sqrt(t.square().mean(-1, keepdim=True) + eps) * w.to(t.dtype)
+        if cos_sin is not None:
+            cs = cos_sin[positions.long().clamp(0, cos_sin.shape[0] - 1)].to(t.dtype)[:, None]
+            h = dim // 2
+            t = torch.cat([t[..., :h] * cs[..., :h] - t[..., h:] * cs[..., h:], t[..., h:] * cs[..., :h] + t[..., :h] * cs[..., h:]], -1)
+        return t
+
+    q_out.copy_(turn(x[:, :nq].float(), q_norm_w).reshape(q_out.shape))
+    if slots is not None:
+        at = slots.long()
+        on = (at >= 0) & (at < k_pages.shape[0] * PAGE)
+        at = at[on]
+        for pages, rows in ((k_pages, turn(x[:, nq:nq + nkv], k_norm_w)), (v_pages, x[:, nq + nkv:])):
+            values, scales = quantize_rows(rows[on])
+            pages.values.view(torch.uint8)[at // PAGE, :, at % PAGE] = values.view(torch.uint8)
+            pages.scales.view(torch.uint8)[at // PAGE, :, at % PAGE] = scales.view(torch.uint8)
+    return q_out
+
+
+def _ref_rows(pages: QuantizedPages, table_row: torch.Tensor, ctx: int) -> torch.Tensor:
+    """[ctx, kv heads, dim] of one sequence; blocks outside the pool read as zeros."""
+    blocks = table_row[:(ctx + PAGE - 1) // PAGE].long()
+    inside = (blocks >= 0) & (blocks < pages.shape[0])
+    x = pages.dequantize(torch.where(inside, blocks, 0)).masked_fill(~inside[:, None, None, None], 0.0)
+    return x.permute(0, 2, 1, 3).reshape(-1, pages.shape[1], pages.shape[3])[:ctx]
+
+
+def _ref_attend(q, k_pages, v_pages, table_row, ctx, scale, pos0, causal, window, chunk, sinks):
+    """q [n, nq, dim] fp32 at positions pos0, pos0 + 1, ... of one sequence -> the same shape."""
+    n, nq, dim = q.shape
+    if ctx <= 0:
+        return torch.zeros_like(q)
+    k, v = _ref_rows(k_pages, table_row, ctx), _ref_rows(v_pages, table_row, ctx)
+    group = nq // k.shape[1]
+    lost = v.isnan().any(-1)
+    s = torch.einsum("qhd,khd->hqk", q, k.repeat_interleave(group, 1)) * scale
+    s = s.masked_fill(lost.T.repeat_interleave(group, 0)[:, None], float("nan"))
+    at, pos = torch.arange(ctx), pos0 + torch.arange(n)[:, None]
+    seen = at <= pos if causal else torch.ones((n, ctx), dtype=torch.bool)
+    if window > 0:
+        seen = seen & (at > pos - window)
+    if chunk > 0:
+        seen = seen & (at >= pos - pos % chunk)
+    s = s.masked_fill(~seen, float("-inf"))
+    top = s.amax(-1, keepdim=True)
+    if sinks is not None:
+        top = torch.maximum(top, sinks.float()[:, None, None])
+    top = torch.where(top == float("-inf"), 0.0, top)
+    p = torch.exp(s - top)
+    total = p.sum(-1, keepdim=True)
+    if sinks is not None:
+        total = total + torch.exp(sinks.float()[:, None, None] - top)
+    o = torch.einsum("hqk,khd->hqd", p, v.masked_fill(lost[..., None], 0.0).repeat_interleave(group, 1))
+    return torch.where(total == 0, 0.0, o / total).transpose(0, 1)
+
+
+# --------------------------------------------------------------------------- checks of arguments
+def _pair(k_cache, v_cache) -> Tuple[int, int, int]:
+    """(blocks, kv heads, dim) of a layer's pages."""
+    if type(k_cache) is not QuantizedPages or type(v_cache) is not QuantizedPages:
+        raise TypeError("keys and values are both QuantizedPages, or neither is")
+    if k_cache.shape != v_cache.shape or k_cache.device != v_cache.device:
+        raise ValueError("keys and values want pages of one shape on one device")
+    return k_cache.shape[0], k_cache.shape[1], k_cache.shape[3]
+
+
+def _want(t: Optional[torch.Tensor], name: str, dtype, shape, device, optional: bool = False) -> None:
+    if t is None:
+        if not optional:
+            raise ValueError(f"{name} is missing")
+        return
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} wants {dtype}, not {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name} has the shape {tuple(t.shape)}, not {tuple(shape)}")
+    if t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} wants to be contiguous and on {device}")
+
+
+def _check_device(pages: QuantizedPages) -> bool:
+    """Whether the kernels run (CUDA); they are launched on the current device's current stream."""
+    if not pages.is_cuda:
+        return False
+    if pages.device.index != torch._C._cuda_getDevice():
+        raise ValueError("the pages are on another device than the current one")
+    _lib.ensure_init()
+    return True
+
+
+def _check_heads(nq: int, nkv: int) -> None:
+    if nq < 1 or nkv < 1 or nq % nkv:
+        raise ValueError("query heads are a multiple of the kv heads")
+
+
+def _check_table(block_table, context_lens, device) -> int:
+    if block_table.dim() != 2 or block_table.shape[1] < 1:
+        raise ValueError("block_table wants [sequences, blocks]")
+    if block_table.dtype is not torch.int32:
+        raise TypeError(f"block_table wants torch.int32, not {block_table.dtype}")
+    if block_table.device != device or block_table.stride(1) != 1:
+        raise ValueError(f"block_table wants neighbouring columns and to be on {device}")
+    B = block_table.shape[0]
+    _want(context_lens, "context_lens", torch.int32, (B,), device)
+    return B
+
+
+def _check_qkv(qkv, positions, slots, cos_sin, k_cache, nq, nkv, head_dim, bias, q_norm_w, k_norm_w) -> int:
+    dev, T, W = k_cache.device, qkv.shape[-2], (nq + 2 * nkv) * head_dim
+    _check_heads(nq, nkv)
+    if nkv != k_cache.shape[1] or head_dim != k_cache.shape[3]:
+        raise ValueError("the pages have other kv heads than the projection")
+    if qkv.dtype not in (torch.float32, torch.bfloat16) or qkv.dim() not in ((2, 3) if qkv.dtype is torch.float32 else (2,)):
+        raise TypeError("qkv is bf16 [T, W] or fp32 partial sums [S, T, W]")
+    if qkv.shape[-1] != W or qkv.shape[0] < 1 <= T:
+        raise ValueError(f"qkv has {qkv.shape[-1]} columns, not {W}")
+    if qkv.device != dev or qkv.stride(-1) != 1 or qkv.stride(-2) != W:
+        raise ValueError(f"qkv wants rows that follow one another, on {dev}")
+    _want(positions, "positions", torch.int32, (T,), dev, optional=cos_sin is None)
+    _want(slots, "slots", torch.int32, (T,), dev, optional=True)
+    if cos_sin is not None:
+        _want(cos_sin, "cos_sin", torch.float32, (cos_sin.shape[0], head_dim), dev)
+        if not cos_sin.shape[0]:
+            raise ValueError("cos_sin has no rows")
+    _want(bias, "bias", torch.bfloat16, (W,), dev, optional=True)
+    _want(q_norm_w, "q_norm_w", torch.bfloat16, (head_dim,), dev, optional=True)
+    _want(k_norm_w, "k_norm_w", torch.bfloat16, (head_dim,), dev, optional=True)
+    return T
+
+
+def _check_masks(mods, window: int, chunk: int, sinks, nq: int, device) -> None:
+    if mods:
+        raise ValueError("attention over QuantizedPages takes no score modifications")
+    if window < 0 or chunk < 0:
+        raise ValueError("window and chunk are not negative")
+    _want(sinks, "sinks", torch.float32, (nq,), device, optional=True)
+
+
+def _result(out: Optional[torch.Tensor], shape, device) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=torch.bfloat16, device=device)
+    _want(out, "out", torch.bfloat16, shape, device)
+    return out
+
+
+def _p(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+# --------------------------------------------------------------------------- operators
+def rope_kv_append(qkv, positions, slots, cos_sin, k_cache, v_cache, nq, nkv, head_dim, *, bias=None, q_norm_w=None, k_norm_w=None,
+                   norm_eps=1e-6, q_out=None) -> torch.Tensor:
+    """`ops.rope_kv_append` onto quantised pages: norms and rotations are rounded once, at the end.  A slot that is negative or
+    outside the pages stores nothing; two tokens of a call have different slots."""
+    blocks = _pair(k_cache, v_cache)[0]
+    T = _check_qkv(qkv, positions, slots, cos_sin, k_cache, nq, nkv, head_dim, bias, q_norm_w, k_norm_w)
+    q_out = _result(q_out, (T, nq * head_dim), k_cache.device)
+    if not _check_device(k_cache):
+        return _ref_append(qkv, positions, slots, cos_sin, k_cache, v_cache, nq, nkv, head_dim, bias, q_norm_w, k_norm_w, norm_eps, q_out)
+    partial = qkv.dtype is torch.float32
+    splits, stride = (qkv.shape[0], qkv.stride(0)) if qkv.dim() == 3 else (1, 0)
+    at = qkv.data_ptr()
+    rc = _lib.lib().nkb_q8_append(
+        None if partial else at, at if partial else None, splits, stride, _p(bias), _p(positions), _p(slots), _p(cos_sin), _p(q_norm_w),
+        _p(k_norm_w), float(norm_eps), q_out.data_ptr(), k_cache.values.data_ptr(), k_cache.scales.data_ptr(), v_cache.values.data_ptr(),
+        v_cache.scales.data_ptr(), T, nq, nkv, head_dim, 0 if cos_sin is None else cos_sin.shape[0], blocks, _stream())
+    _lib.check(rc, "nkb_q8_append")
+    _count_launch()
+    return q_out
+
+
+def paged_attn_decode(q, k_cache, v_cache, block_table, context_lens, scale, *, q_len=1, window=0, chunk=0, sinks=None, mods=None,
+                      num_splits=0, scratch=None, out=None) -> torch.Tensor:
+    """`ops.paged_attn_decode` over quantised pages."""
+    blocks, nkv, D = _pair(k_cache, v_cache)
+    dev = k_cache.device
+    B = _check_table(block_table, context_lens, dev)
+    nq = q.shape[-1] // D
+    _check_heads(nq, nkv)
+    _check_masks(mods, window, chunk, sinks, nq, dev)
+    if q_len < 1:
+        raise ValueError("q_len is at least one")
+    _want(q, "q", torch.bfloat16, (B * q_len, nq * D), dev)
+    out = _result(out, q.shape, dev)
+    if not B:
+        return out
+    if not _check_device(k_cache):
+        qf, res = q.float().reshape(B, q_len, nq, D), out.view(B, q_len, nq, D)
+        for b in range(B):
+            ctx = min(int(context_lens[b]), block_table.shape[1] * PAGE)
+            res[b] = _ref_attend(qf[b], k_cache, v_cache, block_table[b], ctx, scale, ctx - q_len, True, window, chunk, sinks)
+        return out
+    rc = _lib.lib().nkb_q8_attn_simple(
+        q.data_ptr(), k_cache.values.data_ptr(), k_cache.scales.data_ptr(), v_cache.values.data_ptr(), v_cache.scales.data_ptr(),
+        block_table.data_ptr(), None, None, context_lens.data_ptr(), out.data_ptr(), B, B * q_len, q_len, nq, nkv, D, blocks,
+        block_table.shape[1], block_table.stride(0), float(scale), 1, int(window), int(chunk), _p(sinks), _stream())
+    _lib.check(rc, "nkb_q8_attn_simple")
+    _count_launch()
+    return out
+
+
+def rope_attn_decode(qkv_partials, positions, slots, cos_sin, k_cache, v_cache, block_table, context_lens, scale, nq, nkv, *, bias=None,
+                     q_norm_w=None, k_norm_w=None, norm_eps=1e-6, window=0, sinks=None, num_splits=0, scratch=None,
+                     out=None) -> torch.Tensor:
+    """`ops.rope_attn_decode` over quantised pages.  The new token takes part as it is kept, in 8 bits, so that a step has the
+    result of `rope_kv_append` and `paged_attn_decode`."""
+    _pair(k_cache, v_cache)
+    if qkv_partials.dtype is not torch.float32 or qkv_partials.shape[-2] != block_table.shape[0]:
+        raise ValueError("rope_attn_decode wants fp32 partials [S, B, W], one token per sequence")
+    q = rope_kv_append(qkv_partials, positions, slots, cos_sin, k_cache, v_cache, nq, nkv, k_cache.shape[3], bias=bias, q_norm_w=q_norm_w,
+                       k_norm_w=k_norm_w, norm_eps=norm_eps)
+    return paged_attn_decode(q, k_cache, v_cache, block_table, context_lens, scale, window=window, sinks=sinks, num_splits=num_splits,
+                             scratch=scratch, out=out)
+
+
+def flash_attn_prefill(q, k_cache, v_cache, block_table, q_start, q_lens, context_lens, scale, *, max_q_len, causal=True, window=0,
+                       chunk=0, sinks=None, mods=None, out=None) -> torch.Tensor:
+    """`ops.flash_attn_prefill` over quantised pages.  Rows of q that belong to no sequence are left as they are in `out`."""
+    blocks, nkv, D = _pair(k_cache, v_cache)
+    dev = k_cache.device
+    B = _check_table(block_table, context_lens, dev)
+    nq = q.shape[-1] // D
+    _check_heads(nq, nkv)
+    _check_masks(mods, window, chunk, sinks, nq, dev)
+    _want(q, "q", torch.bfloat16, (q.shape[0], nq * D), dev)
+    _want(q_start, "q_start", torch.int32, (B,), dev)
+    _want(q_lens, "q_lens", torch.int32, (B,), dev)
+    out = _result(out, q.shape, dev)
+    if not B or not q.shape[0]:
+        return out
+    if max_q_len < 1:
+        raise ValueError("max_q_len is at least one")
+    if not _check_device(k_cache):
+        qf, res = q.float().reshape(-1, nq, D), out.view(-1, nq, D)
+        for b in range(B):
+            n, at, ctx = int(q_lens[b]), int(q_start[b]), min(int(context_lens[b]), block_table.shape[1] * PAGE)
+            if n > 0:
+                res[at:at + n] = _ref_attend(qf[at:at + n], k_cache, v_cache, block_table[b], ctx, scale, ctx - n, causal, window, chunk,
+                                             sinks)
+        return out
+    rc = _lib.lib().nkb_q8_attn_simple(
+        q.data_ptr(), k_cache.values.data_ptr(), k_cache.scales.data_ptr(), v_cache.values.data_ptr(), v_cache.scales.data_ptr(),
+        block_table.data_ptr(), q_start.data_ptr(), q_lens.data_ptr(), context_lens.data_ptr(), out.data_ptr(), B, q.shape[0],
+        int(max_q_len), nq, nkv, D, blocks, block_table.shape[1], block_table.stride(0), float(scale), 1 if causal else 0, int(window),
+        int(chunk), _p(sinks), _stream())
+    _lib.check(rc, "nkb_q8_attn_simple")
+    _count_launch()
+    return out
+
+
+from . import _count_launch, _stream  # noqa: E402  (defined above the import of this module)
