@@ -17,6 +17,8 @@ int encode_tmap_bf16_2d(CUtensorMap* m, const void* ptr, uint64_t inner, uint64_
                         uint32_t box_inner, uint32_t box_outer);
 int encode_tmap_bf16(CUtensorMap* m, const void* ptr, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
                      const uint32_t* box);
+int encode_tmap_u8(CUtensorMap* m, const void* ptr, int rank, const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
+                   int swizzle);
 int* status_word();
 struct GemmArgs;
 void mark_bulk(GemmArgs& a);   // gemm_tcgen05.cu: enables the bulk-copy epilogue when the output is 16-byte aligned
@@ -159,6 +161,11 @@ int nkb_q8_attn_simple(const void* q, const void* k_values, const void* k_scales
                        const int* block_table, const int* q_start, const int* q_lens, const int* context_lens, void* out, int batch,
                        int total_q, int max_q_len, int nq, int nkv, int head_dim, int num_blocks, int table_width, long long table_stride,
                        float scale, int causal, int window, int chunk, const float* sinks, void* stream);
+long long nkb_q8_attn_decode_scratch_floats(int batch, int nkv, int head_dim, int group, int num_splits);
+int nkb_q8_attn_decode(const void* q, const void* k_values, const void* k_scales, const void* v_values, const void* v_scales,
+                       const int* block_table, const int* context_lens, void* out, float* scratch, int batch, int q_len, int nq, int nkv,
+                       int head_dim, int num_blocks, int table_width, long long table_stride, float scale, int window, int chunk,
+                       const float* sinks, int num_splits, void* stream);
 int nkb_decode_advance(int* context_lens, const int* block_table, int* positions, int* slots, int batch, int q_len,
                        int max_blocks, int block_size, void* stream);
 // Positions and cache slots of the tokens of a packed step (sequences one behind another without gaps, each with its row of the table).

@@ -28,13 +28,13 @@
 // and prefix sharing are new here.
 #include "common.cuh"
 #include "mma_frag.cuh"
+#include "page_plan.cuh"
 #include "attn_maps.h"
 #include "api.h"
 #include <math.h>
 
 namespace nkb {
 
-constexpr int kPage = 32;
 constexpr int kDecStages = 3;
 // The scratch buffer starts with the arrival counters (one per sequence x kv head, at most this many), the
 // split partials follow.  Counters must be zero before the first call and are reset by the merging CTA.
@@ -72,6 +72,7 @@ struct DecodeParams {
   int qkv_splits, max_pos;
   int qkv_pairs;             // partials may be read two at a time
   NkbScoreMods mods;         // MODS only (not fused)
+  __device__ __forceinline__ int context(int b) const { return context_lens[b]; }
 };
 
 // Rows of the fused QKV output of one token, two heads at a time, in two steps so that a warp has the loads of all of them in flight:
@@ -202,71 +203,6 @@ __device__ __forceinline__ float modified_score(float s, const DecodeParams& p, 
   }
   if (p.mods.dist_a) s = fmaf(-dist_a, __log2f(fmaf(dist_b, float(dist), 1.f)), s);
   return s;
-}
-
-// MODS: scores are capped, lose a term that grows with the distance, or the first tokens stay visible outside the window.
-// Pages a sequence of ctx tokens has to be read (fused: all tokens but the new one), `kept` of them first tokens' ahead of the window's.
-template <bool MODS>
-__device__ __forceinline__ int pages_of(const DecodeParams& p, int ctx, int& page_lo, int& kept) {
-  const int first_tok = nkb_first_visible(max(ctx - p.q_len, 0), p.window, p.chunk);
-  page_lo = first_tok / kPage;
-  const int page_hi = ((p.qkv_partials ? ctx - 1 : ctx) + kPage - 1) / kPage;
-  kept = MODS ? min((p.mods.keep_first + kPage - 1) / kPage, page_lo) : 0;
-  return kept + max(page_hi - page_lo, 0);
-}
-
-// Divides the pages of all sequences among `units` CTAs: every CTA of a kv head takes up to `per` pages of one sequence, per the
-// same for all, so that long sequences get more CTAs and all of them end together.  (Divided into equal numbers of CTAs per sequence, a
-// batch waits for its longest one: 7 sequences of 3500 to 7000 tokens 38.5 us, 33.7 here; one of 32000 36 and 30.)  At least `least`
-// pages each, because partial results cost a merge: one sequence of 203 tokens in single pages 15.5 us, as a whole 6.2.
-// units >= 2 * batch; returns false for a CTA without work.  One warp's lanes agree on everything.
-struct PagePlan {
-  int b, split, splits, per;
-};
-template <bool MODS>
-__device__ __forceinline__ bool plan_pages(const DecodeParams& p, int unit, int least, int lane, PagePlan& o) {
-  constexpr uint32_t kAll = 0xffffffffu;
-  int lo, kept, total = 0, mine = 0;
-  for (int i = lane; i < p.batch; i += 32) {
-    const int n = pages_of<MODS>(p, p.context_lens[i], lo, kept);
-    total += n;
-    if (i < 32) mine = n;
-  }
-  total = __reduce_add_sync(kAll, total);
-  // lane i tries first + first * i / 31 pages; the last one, twice the mean, always does: sum ceil(n / per) <= total / per + batch
-  const int first = max((total + p.units - 1) / p.units, least), per_i = first + (first * lane + 30) / 31;
-  const float inv = 1.f / float(per_i);
-  float count = 0.f;
-  for (int i0 = 0; i0 < p.batch; i0 += 32) {
-    if (i0 > 0) mine = i0 + lane < p.batch ? pages_of<MODS>(p, p.context_lens[i0 + lane], lo, kept) : 0;
-    const int m = min(p.batch - i0, 32);
-    for (int i = 0; i < m; ++i)          // (n - 1/2) / per lies half a part off any whole number, far beyond the rounding
-      count += fmaxf(ceilf((float(__shfl_sync(kAll, mine, i)) - 0.5f) * inv), 1.f);
-  }
-  const uint32_t fits = __ballot_sync(kAll, count <= float(p.units)) | 0x80000000u;
-  o.per = __shfl_sync(kAll, per_i, __ffs(fits) - 1);
-  int base = 0;                          // units of the sequences before i0
-  for (int i0 = 0; i0 < p.batch; i0 += 32) {
-    const bool in = i0 + lane < p.batch;
-    const int n = in ? pages_of<MODS>(p, p.context_lens[i0 + lane], lo, kept) : 0;
-    const int want = in ? max((n + o.per - 1) / o.per, 1) : 0;
-    int end = want;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int x = __shfl_up_sync(kAll, end, d);
-      if (lane >= d) end += x;
-    }
-    const uint32_t past = __ballot_sync(kAll, in && unit < base + end);
-    if (past) {
-      const int at = __ffs(past) - 1;
-      o.b = i0 + at;
-      o.splits = __shfl_sync(kAll, want, at);
-      o.split = unit - base - (__shfl_sync(kAll, end, at) - o.splits);
-      return true;
-    }
-    base += __shfl_sync(kAll, end, 31);
-  }
-  return false;
 }
 
 // Warps of a CTA beside those that stream pages: they take their share of the new token's rows (fused mode) and of the merge, for which
@@ -719,15 +655,6 @@ static int launch_decode(const CUtensorMap& tk, const CUtensorMap& tv, const Dec
   const dim3 grid = p.units ? dim3(p.units, p.nkv, 1) : dim3(1, p.nkv, p.batch);
   return launch_pdl(paged_attn_decode_kernel<D, kDecWarps, MODS>, grid, dim3((kDecWarps + dec_helpers<D, kDecWarps>()) * 32), size_t(smem),
                     s, tk, tv, p);
-}
-
-// Units of the page plan: num_splits per sequence, rounded up to one wave of one CTA per SM, or of two (the scratch, which is sized for nq
-// heads, has room for num_splits * group per sequence).
-static int plan_units(int batch, int nkv, int group, int num_splits) {
-  if (num_splits <= 1) return 0;
-  const int asked = batch * num_splits, one = num_sms() / nkv, two = 2 * num_sms() / nkv;
-  const int wave = asked <= one ? one : (asked <= two ? two : asked);
-  return wave < asked * group ? wave : asked * group;
 }
 
 // Warps per CTA: every warp streams its own pages through a private 3-stage ring (48 KB at D = 128), so an SM

@@ -24,10 +24,8 @@ static EncodeTiledFn get_encode_fn() {
   return fn;
 }
 
-// bf16 tensor map with 128-byte swizzle; dims/box are innermost-first,
-// strides_bytes has rank-1 entries (dimension 0 is contiguous).
-int encode_tmap_bf16(CUtensorMap* m, const void* ptr, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
-                     const uint32_t* box) {
+static int encode_tmap(CUtensorMap* m, CUtensorMapDataType type, CUtensorMapSwizzle swizzle, const void* ptr, int rank,
+                       const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box) {
   EncodeTiledFn fn = get_encode_fn();
   if (!fn || rank < 1 || rank > 5) return -1;
   cuuint64_t d[5], s[5];
@@ -38,10 +36,24 @@ int encode_tmap_bf16(CUtensorMap* m, const void* ptr, int rank, const uint64_t* 
     e[i] = 1;
     if (i + 1 < rank) s[i] = strides_bytes[i];
   }
-  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, cuuint32_t(rank), const_cast<void*>(ptr), d, s, b, e,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = fn(m, type, cuuint32_t(rank), const_cast<void*>(ptr), d, s, b, e, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : int(r);
+}
+
+// bf16 tensor map with 128-byte swizzle; dims/box are innermost-first,
+// strides_bytes has rank-1 entries (dimension 0 is contiguous).
+int encode_tmap_bf16(CUtensorMap* m, const void* ptr, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
+                     const uint32_t* box) {
+  return encode_tmap(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_SWIZZLE_128B, ptr, rank, dims, strides_bytes, box);
+}
+
+// The same of bytes; swizzle: 128, 64 or 0 bytes.
+int encode_tmap_u8(CUtensorMap* m, const void* ptr, int rank, const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
+                   int swizzle) {
+  return encode_tmap(m, CU_TENSOR_MAP_DATA_TYPE_UINT8,
+                     swizzle == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : (swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE),
+                     ptr, rank, dims, strides_bytes, box);
 }
 
 int encode_tmap_bf16_2d(CUtensorMap* m, const void* ptr, uint64_t inner, uint64_t outer, uint64_t ld_elems,

@@ -245,6 +245,30 @@ def _p(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
+COUNTERS = 16384                     # words of the scratch of decode attention that count arrivals
+_SCRATCH = {}
+
+
+def _scratch(device: torch.device, floats: int) -> torch.Tensor:
+    """Partial results of divided sequences, behind arrival counters that are zero between calls: one per device and stream.  A graph
+    that is captured gets its own, cleared whenever it runs: it may run beside other graphs, and ahead of the call that would have
+    cleared a shared one."""
+    if torch.cuda.is_current_stream_capturing():
+        buf = torch.empty((floats,), dtype=torch.float32, device=device)
+        buf[:COUNTERS].zero_()
+        return buf
+    key = (device.index, _stream())
+    buf = _SCRATCH.get(key)
+    if buf is None or buf.numel() < floats:
+        buf = _SCRATCH[key] = torch.zeros((floats,), dtype=torch.float32, device=device)
+    return buf
+
+
+def _pick_splits(ctas: int, max_pages: int, sms: int = 148) -> int:
+    """Parts that decode attention makes of a sequence on average."""
+    return 1 if ctas >= sms else max(min(sms // ctas, max(max_pages // 8, 1), 16), 1)
+
+
 # --------------------------------------------------------------------------- operators
 def rope_kv_append(qkv, positions, slots, cos_sin, k_cache, v_cache, nq, nkv, head_dim, *, bias=None, q_norm_w=None, k_norm_w=None,
                    norm_eps=1e-6, q_out=None) -> torch.Tensor:
@@ -288,11 +312,25 @@ def paged_attn_decode(q, k_cache, v_cache, block_table, context_lens, scale, *, 
             ctx = min(int(context_lens[b]), block_table.shape[1] * PAGE)
             res[b] = _ref_attend(qf[b], k_cache, v_cache, block_table[b], ctx, scale, ctx - q_len, True, window, chunk, sinks)
         return out
-    rc = _lib.lib().nkb_q8_attn_simple(
+    group = nq // nkv
+    if q_len * group > 16:          # more rows than a fragment of the decode kernel has
+        q_start = torch.arange(0, B * q_len, q_len, device=dev, dtype=torch.int32)
+        return flash_attn_prefill(q, k_cache, v_cache, block_table, q_start, torch.full_like(q_start, q_len), context_lens, scale,
+                                  max_q_len=q_len, window=window, chunk=chunk, sinks=sinks, out=out)
+    L = _lib.lib()
+    if num_splits <= 0:
+        num_splits = _pick_splits(B * nkv, block_table.shape[1])
+    if num_splits > 1:
+        need = L.nkb_q8_attn_decode_scratch_floats(B, nkv, D, group, num_splits)
+        if scratch is None:
+            scratch = _scratch(dev, need)
+        elif scratch.dtype is not torch.float32 or scratch.numel() < need or scratch.device != dev or not scratch.is_contiguous():
+            raise ValueError(f"scratch wants {need} contiguous fp32 values on {dev}, the first {COUNTERS} zero before the first call")
+    rc = L.nkb_q8_attn_decode(
         q.data_ptr(), k_cache.values.data_ptr(), k_cache.scales.data_ptr(), v_cache.values.data_ptr(), v_cache.scales.data_ptr(),
-        block_table.data_ptr(), None, None, context_lens.data_ptr(), out.data_ptr(), B, B * q_len, q_len, nq, nkv, D, blocks,
-        block_table.shape[1], block_table.stride(0), float(scale), 1, int(window), int(chunk), _p(sinks), _stream())
-    _lib.check(rc, "nkb_q8_attn_simple")
+        block_table.data_ptr(), context_lens.data_ptr(), out.data_ptr(), _p(scratch), B, q_len, nq, nkv, D, blocks,
+        block_table.shape[1], block_table.stride(0), float(scale), int(window), int(chunk), _p(sinks), num_splits, _stream())
+    _lib.check(rc, "nkb_q8_attn_decode")
     _count_launch()
     return out
 
