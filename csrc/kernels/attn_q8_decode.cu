@@ -6,14 +6,16 @@
 // 2^{t_j - M}, M near the largest t so far, multiply the values as they are kept, and 2^{-v_j} takes a weight back to the denominator.  So
 // values of any size meet weights that f16 holds: a weight below 2^-30 of the largest contribution is all that rounds to nothing.
 //
-// The op is bound by the bytes of the pages, half of a bf16 cache's, and next by the instructions per byte: four bytes are two
-// conversions to f16 (exact; e4m3 has no matrix instruction with 16-bit queries) and one (V: two) bytes permutation.  Queries are f16 too, each
-// row brought below 2^15 by a power of two, which loses nothing that 32-bit sums would keep.  Fragments come from shared memory with
-// ldmatrix in units of two bytes: a lane then holds four neighbouring columns of a key, which the queries are permuted to match, and of a
-// value pairs of neighbouring columns, which a byte permutation turns into pairs of tokens.
+// The op is bound by the bytes of the pages, half of a bf16 cache's, and next by what a warp does per page.  Four bytes are two
+// conversions to f16 (exact; e4m3 has no matrix instruction with 16-bit queries).  Keys and columns of values are the 16-row side of the
+// products, query rows the side of eight: S^T = K Q^T, O^T = V^T P^T, so that a group of up to eight rows costs half the products and a
+// lane half the exponentials that rows padded to sixteen would.  Queries are f16 too, each row brought below 2^15 by a power of two, which
+// loses nothing that 32-bit sums would keep.  Fragments come from shared memory with ldmatrix in units of two bytes: a lane then holds
+// four neighbouring columns of a key, which the queries are permuted to match, and of a value pairs of neighbouring columns, which a byte
+// permutation turns into pairs of tokens.
 //
 // The grid, the page plan and the merge are those of decode attention over bf16 pages (attn_decode.cu); a page is half as large, so
-// an SM holds the rings of eight warps.
+// an SM holds the rings of twice as many warps.
 #include "api.h"
 #include "kv_quant.cuh"
 #include "mma_frag.cuh"
@@ -24,7 +26,9 @@
 namespace nkb {
 
 constexpr int kQ8Stages = 3;
-constexpr int kQ8SmWarps = 8;          // warps whose rings an SM holds
+// warps whose rings an SM holds
+template <int D>
+constexpr int kQ8SmWarps = 1024 / D;
 constexpr int kQ8Counters = 16384;     // the scratch starts with as many arrival counters
 constexpr float kQ8Lift = 6.f;         // log2 of the weight at M; t may grow by kQ8Grow above M before M follows: f16 ends at 2^16
 constexpr float kQ8Grow = 8.f;
@@ -56,6 +60,12 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// the transpose of an 8 x 8 matrix of 16-bit values that the warp holds
+__device__ __forceinline__ uint32_t transposed_8x8(uint32_t v) {
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;" : "+r"(v));
+  return v;
+}
+
 // Byte of a 16-byte piece in a [32][D] page, as the load's swizzle places it: 128-byte rows piece ^ row, 64-byte rows piece ^ row / 2
 template <int D>
 __device__ __forceinline__ uint32_t q8_piece(int row, int piece) {
@@ -65,13 +75,15 @@ __device__ __forceinline__ uint32_t q8_piece(int row, int piece) {
 template <int D, int W>
 struct DecodeQ8Smem {
   static constexpr int kMat = kPage * D, kStage = 2 * kMat, kScales = 256;       // K and V scales, on 128 bytes each
-  static constexpr int kRings = W * kQ8Stages * kStage, kScaleAt = kRings, kFactorAt = kScaleAt + W * kQ8Stages * kScales;
-  static constexpr int kBytes = kFactorAt + W * 3 * kPage * 4 + 1024;
-  static_assert(kRings >= W * (16 * D + 32) * 4, "merge space must fit in the rings");
+  static constexpr int kRings = W * kQ8Stages * kStage, kScaleAt = kRings;
+  static constexpr int kBytes = kScaleAt + W * kQ8Stages * kScales + 1024;
+  static constexpr int kPitch = D + 8;                                           // floats between the rows of merged results
+  static_assert(kRings >= W * (16 * kPitch + 32) * 4, "merge space must fit in the rings");
 };
 
-template <int D, int W>
-__global__ void __launch_bounds__(W * 32, kQ8SmWarps / W)
+// NT: query rows of a kv head in eights
+template <int D, int W, int NT>
+__global__ void __launch_bounds__(W * 32, kQ8SmWarps<D> / W)
 attn_q8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                       const __grid_constant__ CUtensorMap tmKS, const __grid_constant__ CUtensorMap tmVS, const DecodeQ8Params p) {
   using L = DecodeQ8Smem<D, W>;
@@ -107,7 +119,6 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
 
   uint8_t* my_ring = smem + warp * kQ8Stages * L::kStage;
   uint8_t* my_scales = smem + L::kScaleAt + warp * kQ8Stages * L::kScales;
-  float* my_factors = reinterpret_cast<float*>(smem + L::kFactorAt) + warp * 3 * kPage;
   const uint64_t policy = l2_evict_first();
   // A block outside the pool lies outside the tensor maps, which read zeros there.
   auto issue = [&](int blk, int stage) {
@@ -131,45 +142,52 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
   for (int s = 0; s < kQ8Stages; ++s)
     if (p0 + warp + s * W < p1) issue(blks[s], s);
 
-  // ---- query fragments (the first pages are on their way): four neighbouring columns per lane and step, as the keys come
-  uint32_t qf[D / 16][4];
-  float rs0, rs1;                        // raw score -> exponent of two, without the key's factor
-  {
-    const __nv_bfloat16* q0 = p.q + (((long long)b * p.q_len + g / p.group) * p.nq + kvh * p.group + g % p.group) * D + 4 * t;
-    const __nv_bfloat16* q1 = p.q + (((long long)b * p.q_len + (g + 8) / p.group) * p.nq + kvh * p.group + (g + 8) % p.group) * D + 4 * t;
-    auto load_row = [&](const __nv_bfloat16* src, bool on, float& rs, int half) {
-      uint2 v[D / 16];
-      float mx = 0.f;
+  // ---- query fragments (the first pages are on their way): lane (g, t) has columns 16 ks + 4 t ... of row g, as the keys come.
+  // rs: raw score -> exponent of two, without the key's factor, of rows 2 t and 2 t + 1
+  uint32_t qf[NT][D / 16][2];
+  float rs[NT][2];
+  int pos[NT][2], low[NT][2];            // last and first visible position
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        v[ks] = on ? *reinterpret_cast<const uint2*>(src + 16 * ks) : make_uint2(0u, 0u);
-        const float2 a = unpack_bf16x2(v[ks].x), c = unpack_bf16x2(v[ks].y);
-        mx = fmaxf(fmaxf(fmaxf(mx, fabsf(a.x)), fmaxf(fabsf(a.y), fabsf(c.x))), fabsf(c.y));
-      }
-      mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, 2));
-      const int e = max((__float_as_int(mx) >> 23) - 127, -100);
-      const float up = exp2_int(14 - e);
-      rs = p.scale_log2 * exp2_int(min(e - 14, 127));
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = nt * 8 + g;
+    const __nv_bfloat16* src = p.q + (((long long)b * p.q_len + r / p.group) * p.nq + kvh * p.group + r % p.group) * D + 4 * t;
+    uint2 v[D / 16];
+    float mx = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        const float2 a = unpack_bf16x2(v[ks].x), c = unpack_bf16x2(v[ks].y);
-        qf[ks][half] = pack_f16x2(a.x * up, a.y * up);
-        qf[ks][2 + half] = pack_f16x2(c.x * up, c.y * up);
-      }
-    };
-    load_row(q0, g < rows, rs0, 0);
-    load_row(q1, g + 8 < rows, rs1, 1);
+    for (int ks = 0; ks < D / 16; ++ks) {
+      v[ks] = r < rows ? *reinterpret_cast<const uint2*>(src + 16 * ks) : make_uint2(0u, 0u);
+      const float2 x = unpack_bf16x2(v[ks].x), y = unpack_bf16x2(v[ks].y);
+      mx = fmaxf(fmaxf(fmaxf(mx, fabsf(x.x)), fmaxf(fabsf(x.y), fabsf(y.x))), fabsf(y.y));
+    }
+    mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, 2));
+    const int e = max((__float_as_int(mx) >> 23) - 127, -100);
+    const float up = exp2_int(14 - e), down = p.scale_log2 * exp2_int(e - 14);
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      const float2 x = unpack_bf16x2(v[ks].x), y = unpack_bf16x2(v[ks].y);
+      qf[nt][ks][0] = pack_f16x2(x.x * up, x.y * up);
+      qf[nt][ks][1] = pack_f16x2(y.x * up, y.y * up);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      rs[nt][i] = __shfl_sync(kAll, down, (2 * t + i) * 4);
+      const int row = nt * 8 + 2 * t + i;
+      pos[nt][i] = ctx - p.q_len + (row < rows ? row / p.group : 0);
+      low[nt][i] = nkb_first_visible(pos[nt][i], p.window, p.chunk);
+    }
   }
-  // last and first visible position of the rows this lane has, and of all rows
-  const int pos0 = ctx - p.q_len + (g < rows ? g / p.group : 0), pos1 = ctx - p.q_len + (g + 8 < rows ? (g + 8) / p.group : 0);
-  const int low0 = nkb_first_visible(pos0, p.window, p.chunk), low1 = nkb_first_visible(pos1, p.window, p.chunk);
-  const int all_hi = ctx - p.q_len, all_lo = nkb_first_visible(ctx - 1, p.window, p.chunk);
+  const int all_hi = ctx - p.q_len, all_lo = nkb_first_visible(ctx - 1, p.window, p.chunk);      // what every row sees
 
-  float o[D / 8][4];
+  // lane (g, t): rows 2 t, 2 t + 1 of columns 16 c + 2 g, 16 c + 2 g + 1
+  float o[NT][D / 16][4], m[NT][2], l[NT][2];
 #pragma unroll
-  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) o[nt][c][0] = o[nt][c][1] = o[nt][c][2] = o[nt][c][3] = 0.f;
+    m[nt][0] = m[nt][1] = -INFINITY;
+    l[nt][0] = l[nt][1] = 0.f;
+  }
 
   int stage = 0;
   uint32_t phase = 0;
@@ -179,101 +197,112 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
     const bool ok = mbar_wait(&bars[warp][stage], phase, &abort_flag, p.status, ERR_WAIT_SMEM_FULL);
     if (!__all_sync(kAll, ok)) break;
     const uint32_t kbase = smem_u32(my_ring + stage * L::kStage), vbase = kbase + L::kMat;
-    {
-      // lane = token: its factors, for the lanes that hold its scores
-      const int kb = my_scales[stage * L::kScales + lane], vb = my_scales[stage * L::kScales + 128 + lane];
-      const float ve = float(q8_log2_of(vb));
-      my_factors[lane] = q8_factor_of(kb);
-      my_factors[kPage + lane] = vb == 255 ? __int_as_float(0x7fc00000) : ve;
-      my_factors[2 * kPage + lane] = exp2_int(-q8_log2_of(vb));
-    }
-    __syncwarp();
+    // lane = token: its factors, for the lanes that hold its scores
+    const int kb = my_scales[stage * L::kScales + lane], vb = my_scales[stage * L::kScales + 128 + lane];
+    const int v_log2 = q8_log2_of(vb);
+    const float my_kf = q8_factor_of(kb), my_ve = vb == 255 ? __int_as_float(0x7fc00000) : float(v_log2), my_back = exp2_int(-v_log2);
 
-    float s[4][4];
+    // S^T: keys 16 mt + g and + 8, rows 2 t and 2 t + 1
+    float s[2][NT][4];
 #pragma unroll
-    for (int nt = 0; nt < 4; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+    for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
-    for (int kp = 0; kp < D / 64; ++kp) {
+      for (int nt = 0; nt < NT; ++nt) s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.f;
+    }
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt) {
-        uint32_t r[4];
-        ldsm_x4(kbase + q8_piece<D>(nt * 8 + (lane & 7), 4 * kp + (lane >> 3)), r[0], r[1], r[2], r[3]);
+    for (int c2 = 0; c2 < D / 32; ++c2) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          mma_16816_f16(s[nt], qf[4 * kp + i], e4m3x2_to_f16x2(uint16_t(r[i])), e4m3x2_to_f16x2(uint16_t(r[i] >> 16)));
+      for (int mt = 0; mt < 2; ++mt) {
+        uint32_t r[4];                   // two pieces of keys 0 to 7 and of 8 to 15
+        ldsm_x4(kbase + q8_piece<D>(mt * 16 + (lane & 15), 2 * c2 + (lane >> 4)), r[0], r[1], r[2], r[3]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t a[4] = {e4m3x2_to_f16x2(uint16_t(r[2 * i])), e4m3x2_to_f16x2(uint16_t(r[2 * i + 1])),
+                                 e4m3x2_to_f16x2(uint16_t(r[2 * i] >> 16)), e4m3x2_to_f16x2(uint16_t(r[2 * i + 1] >> 16))};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_16816_f16(s[mt][nt], a, qf[nt][2 * c2 + i][0], qf[nt][2 * c2 + i][1]);
+        }
       }
     }
     // t = s + v, the mask only where a page crosses an edge
     const int tok0 = pg * kPage;
     const bool edge = tok0 + kPage - 1 > all_hi || tok0 < all_lo;
-    float mx0 = -INFINITY, mx1 = -INFINITY;
-    float back[4][2];
+    float mx[NT][2], back[2][2];
+    bool grow = false;
 #pragma unroll
-    for (int nt = 0; nt < 4; ++nt) {
-      const float2 kf = *reinterpret_cast<const float2*>(my_factors + nt * 8 + 2 * t);
-      const float2 ve = *reinterpret_cast<const float2*>(my_factors + kPage + nt * 8 + 2 * t);
-      const float2 bk = *reinterpret_cast<const float2*>(my_factors + 2 * kPage + nt * 8 + 2 * t);
-      back[nt][0] = bk.x;
-      back[nt][1] = bk.y;
+    for (int nt = 0; nt < NT; ++nt) mx[nt][0] = mx[nt][1] = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float v0 = fmaf(s[nt][e] * rs0, e ? kf.y : kf.x, e ? ve.y : ve.x);
-        float v1 = fmaf(s[nt][2 + e] * rs1, e ? kf.y : kf.x, e ? ve.y : ve.x);
-        if (edge) {
-          const int tok = tok0 + nt * 8 + 2 * t + e;
-          if (tok > pos0 || tok < low0) v0 = -INFINITY;
-          if (tok > pos1 || tok < low1) v1 = -INFINITY;
+    for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int key = mt * 16 + h * 8 + g;
+        const float kf = __shfl_sync(kAll, my_kf, key), ve = __shfl_sync(kAll, my_ve, key);
+        back[mt][h] = __shfl_sync(kAll, my_back, key);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float x = fmaf(s[mt][nt][2 * h + i] * rs[nt][i], kf, ve);
+            if (edge && (tok0 + key > pos[nt][i] || tok0 + key < low[nt][i])) x = -INFINITY;
+            s[mt][nt][2 * h + i] = x;
+            mx[nt][i] = fmaxf(mx[nt][i], x);
+          }
         }
-        s[nt][e] = v0;
-        s[nt][2 + e] = v1;
-        mx0 = fmaxf(mx0, v0);
-        mx1 = fmaxf(mx1, v1);
       }
     }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) grow = grow || mx[nt][0] > m[nt][0] + kQ8Grow || mx[nt][1] > m[nt][1] + kQ8Grow;
     // M follows the largest t when that has grown by more than kQ8Grow
-    if (__any_sync(kAll, mx0 > m0 + kQ8Grow || mx1 > m1 + kQ8Grow)) {
-      mx0 = fmaxf(mx0, __shfl_xor_sync(kAll, mx0, 1));
-      mx0 = fmaxf(mx0, __shfl_xor_sync(kAll, mx0, 2));
-      mx1 = fmaxf(mx1, __shfl_xor_sync(kAll, mx1, 1));
-      mx1 = fmaxf(mx1, __shfl_xor_sync(kAll, mx1, 2));
-      const float mn0 = fmaxf(m0, mx0), mn1 = fmaxf(m1, mx1);
-      const float a0 = m0 == -INFINITY ? 0.f : exp2f(m0 - mn0), a1 = m1 == -INFINITY ? 0.f : exp2f(m1 - mn1);
-      m0 = mn0;
-      m1 = mn1;
-      l0 *= a0;
-      l1 *= a1;
+    if (__any_sync(kAll, grow)) {
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        o[i][0] *= a0; o[i][1] *= a0;
-        o[i][2] *= a1; o[i][3] *= a1;
+      for (int nt = 0; nt < NT; ++nt) {
+        float keep[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float x = mx[nt][i];
+          x = fmaxf(x, __shfl_xor_sync(kAll, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(kAll, x, 8));
+          x = fmaxf(fmaxf(x, __shfl_xor_sync(kAll, x, 16)), m[nt][i]);
+          keep[i] = m[nt][i] == x ? 1.f : exp2f(m[nt][i] - x);
+          m[nt][i] = x;
+          l[nt][i] *= keep[i];
+        }
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+          o[nt][c][0] *= keep[0]; o[nt][c][1] *= keep[1];
+          o[nt][c][2] *= keep[0]; o[nt][c][3] *= keep[1];
+        }
       }
     }
-    const float base0 = (m0 == -INFINITY ? 0.f : m0) - kQ8Lift, base1 = (m1 == -INFINITY ? 0.f : m1) - kQ8Lift;
+    uint32_t pb[2][NT][2];               // P^T: row g, tokens 2 t and 2 t + 1 of each eight
 #pragma unroll
-    for (int nt = 0; nt < 4; ++nt) {
+    for (int nt = 0; nt < NT; ++nt) {
+      const float base0 = (m[nt][0] == -INFINITY ? 0.f : m[nt][0]) - kQ8Lift, base1 = (m[nt][1] == -INFINITY ? 0.f : m[nt][1]) - kQ8Lift;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        s[nt][e] = exp2f(s[nt][e] - base0);
-        s[nt][2 + e] = exp2f(s[nt][2 + e] - base1);
-        l0 = fmaf(s[nt][e], back[nt][e], l0);
-        l1 = fmaf(s[nt][2 + e], back[nt][e], l1);
+      for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float w0 = exp2f(s[mt][nt][2 * h] - base0), w1 = exp2f(s[mt][nt][2 * h + 1] - base1);
+          l[nt][0] = fmaf(w0, back[mt][h], l[nt][0]);
+          l[nt][1] = fmaf(w1, back[mt][h], l[nt][1]);
+          pb[mt][nt][h] = transposed_8x8(pack_f16x2(w0, w1));
+        }
       }
     }
-    // O += P V
+    // O^T += V^T P^T
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const uint32_t pa[4] = {pack_f16x2(s[2 * j][0], s[2 * j][1]), pack_f16x2(s[2 * j][2], s[2 * j][3]),
-                              pack_f16x2(s[2 * j + 1][0], s[2 * j + 1][1]), pack_f16x2(s[2 * j + 1][2], s[2 * j + 1][3])};
+    for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
-      for (int cp = 0; cp < D / 32; ++cp) {
-        uint32_t r[4];
-        ldsm_x4_t(vbase + q8_piece<D>(16 * j + ((lane >> 3) & 1) * 8 + (lane & 7), 2 * cp + (lane >> 4)), r[0], r[1], r[2], r[3]);
+      for (int c2 = 0; c2 < D / 32; ++c2) {
+        uint32_t r[4];                   // tokens 0 to 7 and 8 to 15 of two pieces
+        ldsm_x4_t(vbase + q8_piece<D>(mt * 16 + (lane & 15), 2 * c2 + (lane >> 4)), r[0], r[1], r[2], r[3]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = __byte_perm(r[i], 0u, 0x3120);     // pairs of tokens: column 2g below, 2g + 1 above
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t lo = __byte_perm(r[2 * i], 0u, 0x3120), hi = __byte_perm(r[2 * i + 1], 0u, 0x3120);   // pairs of tokens
+          const uint32_t a[4] = {e4m3x2_to_f16x2(uint16_t(lo)), e4m3x2_to_f16x2(uint16_t(lo >> 16)),
+                                 e4m3x2_to_f16x2(uint16_t(hi)), e4m3x2_to_f16x2(uint16_t(hi >> 16))};
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          mma_16816_f16(o[4 * cp + 2 * c], pa, e4m3x2_to_f16x2(uint16_t(r[2 * c])), e4m3x2_to_f16x2(uint16_t(r[2 * c + 1])));
-          mma_16816_f16(o[4 * cp + 2 * c + 1], pa, e4m3x2_to_f16x2(uint16_t(r[2 * c] >> 16)), e4m3x2_to_f16x2(uint16_t(r[2 * c + 1] >> 16)));
+          for (int nt = 0; nt < NT; ++nt) mma_16816_f16(o[nt][2 * c2 + i], a, pb[mt][nt][0], pb[mt][nt][1]);
         }
       }
     }
@@ -281,30 +310,38 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
     if (next < p1) issue(next_blk, stage);
     if (++stage == kQ8Stages) { stage = 0; phase ^= 1u; }
   }
-  l0 += __shfl_xor_sync(kAll, l0, 1);
-  l0 += __shfl_xor_sync(kAll, l0, 2);
-  l1 += __shfl_xor_sync(kAll, l1, 1);
-  l1 += __shfl_xor_sync(kAll, l1, 2);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) l[nt][i] += __shfl_xor_sync(kAll, l[nt][i], x);
+    }
+  }
 
   if (abort_flag) {
     for (int i = 0; i < 200; ++i) __nanosleep(1000);
   }
   __syncthreads();  // every load consumed: the rings are merge space now
 
-  float* mo = reinterpret_cast<float*>(smem);             // [warp][16][D]
-  float* mm = mo + W * 16 * D;                            // [warp][16]
+  float* mo = reinterpret_cast<float*>(smem);             // [warp][16][pitch]
+  float* mm = mo + W * 16 * L::kPitch;                    // [warp][16]
   float* ml = mm + W * 16;
 #pragma unroll
-  for (int c = 0; c < D / 16; ++c) {
-    // column 16 c + 4 t + i: even ones in one tile, odd ones in the next
-    if (g < rows)
-      *reinterpret_cast<float4*>(mo + (warp * 16 + g) * D + 16 * c + 4 * t) = make_float4(o[2 * c][0], o[2 * c + 1][0], o[2 * c][1], o[2 * c + 1][1]);
-    if (g + 8 < rows)
-      *reinterpret_cast<float4*>(mo + (warp * 16 + g + 8) * D + 16 * c + 4 * t) = make_float4(o[2 * c][2], o[2 * c + 1][2], o[2 * c][3], o[2 * c + 1][3]);
-  }
-  if (t == 0) {
-    mm[warp * 16 + g] = m0; mm[warp * 16 + g + 8] = m1;
-    ml[warp * 16 + g] = l0; ml[warp * 16 + g + 8] = l1;
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = nt * 8 + 2 * t + i;
+      if (row < rows) {
+        float* dst = mo + (warp * 16 + row) * L::kPitch + 2 * g;
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) *reinterpret_cast<float2*>(dst + 16 * c) = make_float2(o[nt][c][i], o[nt][c][2 + i]);
+      }
+      if (g == 0) {
+        mm[warp * 16 + row] = m[nt][i];
+        ml[warp * 16 + row] = l[nt][i];
+      }
+    }
   }
   __syncthreads();
   // o and l carry 2^(lift - M); merged values 2^(lift - mf)
@@ -331,7 +368,7 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       const float mw = mm[w * 16 + r], sc = mw == -INFINITY && mf != -INFINITY ? 0.f : exp2f(mw == mf ? 0.f : mw - mf);
-      const float4 x = *reinterpret_cast<const float4*>(mo + (w * 16 + r) * D + d);
+      const float4 x = *reinterpret_cast<const float4*>(mo + (w * 16 + r) * L::kPitch + d);
       acc.x += sc * x.x; acc.y += sc * x.y; acc.z += sc * x.z; acc.w += sc * x.w;
       l += sc * ml[w * 16 + r];
     }
@@ -395,28 +432,29 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
   }
 }
 
-template <int D, int W>
+template <int D, int W, int NT>
 static int launch_decode_q8(const CUtensorMap (&m)[4], const DecodeQ8Params& p, cudaStream_t s) {
   using L = DecodeQ8Smem<D, W>;
   static bool attr_set[64] = {false};    // the attribute is per device
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
   if (!attr_set[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(attn_q8_decode_kernel<D, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+    const cudaError_t e = cudaFuncSetAttribute(attn_q8_decode_kernel<D, W, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
     if (e != cudaSuccess) return int(e);
     attr_set[dev] = true;
   }
   const dim3 grid = p.units ? dim3(p.units, p.nkv, 1) : dim3(1, p.nkv, p.batch);
-  return launch_pdl(attn_q8_decode_kernel<D, W>, grid, dim3(W * 32), size_t(L::kBytes), s, m[0], m[1], m[2], m[3], p);
+  return launch_pdl(attn_q8_decode_kernel<D, W, NT>, grid, dim3(W * 32), size_t(L::kBytes), s, m[0], m[1], m[2], m[3], p);
 }
 
-template <int D>
+template <int D, int NT>
 static int dispatch_decode_q8(const CUtensorMap (&m)[4], const DecodeQ8Params& p, cudaStream_t s) {
+  constexpr int most = kQ8SmWarps<D>;
   const long long ctas = (long long)(p.units ? p.units : p.batch) * p.nkv, sms = num_sms();
-  if (ctas <= sms) return launch_decode_q8<D, 8>(m, p, s);
-  if (ctas <= 2 * sms) return launch_decode_q8<D, 4>(m, p, s);
-  if (ctas <= 4 * sms) return launch_decode_q8<D, 2>(m, p, s);
-  return launch_decode_q8<D, 1>(m, p, s);
+  if (ctas <= sms) return launch_decode_q8<D, most, NT>(m, p, s);
+  if (ctas <= 2 * sms) return launch_decode_q8<D, most / 2, NT>(m, p, s);
+  if (ctas <= 4 * sms) return launch_decode_q8<D, most / 4, NT>(m, p, s);
+  return launch_decode_q8<D, most / 8, NT>(m, p, s);
 }
 
 // Tensor maps of K and V pages and of their scales
@@ -467,7 +505,8 @@ extern "C" int nkb_q8_attn_decode(const void* q, const void* k_values, const voi
   CUtensorMap m[4];
   if (int rc = q8_maps(m, {k_values, v_values, k_scales, v_scales}, head_dim, nkv, num_blocks)) return rc;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (head_dim == 128) return dispatch_decode_q8<128>(m, p, s);
-  if (head_dim == 64) return dispatch_decode_q8<64>(m, p, s);
+  const bool eight = q_len * p.group <= 8;
+  if (head_dim == 128) return eight ? dispatch_decode_q8<128, 1>(m, p, s) : dispatch_decode_q8<128, 2>(m, p, s);
+  if (head_dim == 64) return eight ? dispatch_decode_q8<64, 1>(m, p, s) : dispatch_decode_q8<64, 2>(m, p, s);
   return -2;
 }
