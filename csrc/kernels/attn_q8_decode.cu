@@ -50,8 +50,7 @@ struct DecodeQ8Params {
 };
 
 __device__ __forceinline__ void mma_16816_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -202,6 +201,20 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
     const int v_log2 = q8_log2_of(vb);
     const float my_kf = q8_factor_of(kb), my_ve = vb == 255 ? __int_as_float(0x7fc00000) : float(v_log2), my_back = exp2_int(-v_log2);
 
+    // fragments of the page ahead of their use, a wait for shared memory each otherwise
+    uint32_t kr[D / 32][2][4], vr[2][D / 32][4];         // pieces 2 c and 2 c + 1 of tokens 0 to 7 and 8 to 15 of each sixteen
+#pragma unroll
+    for (int c2 = 0; c2 < D / 32; ++c2) {
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+        ldsm_x4(kbase + q8_piece<D>(mt * 16 + (lane & 15), 2 * c2 + (lane >> 4)), kr[c2][mt][0], kr[c2][mt][1], kr[c2][mt][2], kr[c2][mt][3]);
+    }
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+      for (int c2 = 0; c2 < D / 32; ++c2)
+        ldsm_x4_t(vbase + q8_piece<D>(mt * 16 + (lane & 15), 2 * c2 + (lane >> 4)), vr[mt][c2][0], vr[mt][c2][1], vr[mt][c2][2], vr[mt][c2][3]);
+    }
     // S^T: keys 16 mt + g and + 8, rows 2 t and 2 t + 1
     float s[2][NT][4];
 #pragma unroll
@@ -213,8 +226,7 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
     for (int c2 = 0; c2 < D / 32; ++c2) {
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
-        uint32_t r[4];                   // two pieces of keys 0 to 7 and of 8 to 15
-        ldsm_x4(kbase + q8_piece<D>(mt * 16 + (lane & 15), 2 * c2 + (lane >> 4)), r[0], r[1], r[2], r[3]);
+        const uint32_t(&r)[4] = kr[c2][mt];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const uint32_t a[4] = {e4m3x2_to_f16x2(uint16_t(r[2 * i])), e4m3x2_to_f16x2(uint16_t(r[2 * i + 1])),
@@ -230,8 +242,6 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
     float mx[NT][2], back[2][2];
     bool grow = false;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) mx[nt][0] = mx[nt][1] = -INFINITY;
-#pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -242,13 +252,28 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            float x = fmaf(s[mt][nt][2 * h + i] * rs[nt][i], kf, ve);
-            if (edge && (tok0 + key > pos[nt][i] || tok0 + key < low[nt][i])) x = -INFINITY;
-            s[mt][nt][2 * h + i] = x;
-            mx[nt][i] = fmaxf(mx[nt][i], x);
+            s[mt][nt][2 * h + i] = fmaf(s[mt][nt][2 * h + i] * rs[nt][i], kf, ve);
           }
         }
       }
+    }
+    if (edge) {
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int tok = tok0 + mt * 16 + (e >> 1) * 8 + g;
+            if (tok > pos[nt][e & 1] || tok < low[nt][e & 1]) s[mt][nt][e] = -INFINITY;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) mx[nt][i] = fmaxf(fmax3(s[0][nt][i], s[0][nt][2 + i], s[1][nt][i]), s[1][nt][2 + i]);
     }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) grow = grow || mx[nt][0] > m[nt][0] + kQ8Grow || mx[nt][1] > m[nt][1] + kQ8Grow;
@@ -294,8 +319,7 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
     for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
       for (int c2 = 0; c2 < D / 32; ++c2) {
-        uint32_t r[4];                   // tokens 0 to 7 and 8 to 15 of two pieces
-        ldsm_x4_t(vbase + q8_piece<D>(mt * 16 + (lane & 15), 2 * c2 + (lane >> 4)), r[0], r[1], r[2], r[3]);
+        const uint32_t(&r)[4] = vr[mt][c2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const uint32_t lo = __byte_perm(r[2 * i], 0u, 0x3120), hi = __byte_perm(r[2 * i + 1], 0u, 0x3120);   // pairs of tokens
