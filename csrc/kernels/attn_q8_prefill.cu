@@ -1,0 +1,617 @@
+// Attention of packed prompts over 8-bit pages (kv_quant.cuh) on tcgen05.
+//
+//   o_i = sum_j 2^{s_ij + v_j} v8_j / sum_j 2^{s_ij},    s_ij = (scale / ln 2) 2^{k_j} (q_i . k8_j)
+//
+// The structure is that of prefill attention over bf16 pages (attn_prefill.cu: two 128-row query tiles in ping-pong, one MMA issuer each,
+// S and O in tensor memory, one softmax thread per row, turns with the exponentials), with what 8 bits change:
+//
+//   warps 0-3    convert: a warp takes one page of every 128-token tile from global memory (a tile ahead, in registers), makes it f16
+//                in the swizzled layout that the MMA reads and brings the tokens to the tile's largest scale, 2^K for keys and 2^V
+//                for values, on the way
+//   warps 4-11   softmax
+//   warps 12, 13 issue tcgen05.mma (14 and 15 idle)
+//
+// f16 holds an e4m3 value times 2^-22 and up exactly or nearly (from 2^6 down, behind the tile's largest), so the products see what is
+// kept.  A tile's exponents are two numbers that enter where one number did before: 2^K in the multiplier of the scores, V in the exponent
+// of the weights, 2^-V where the weights are summed.  Nothing is added per score.  There is no MMA of 16-bit queries with e4m3 keys, and keys
+// in two parts on the 8-bit MMA would double the products.
+//
+// Rows of a query tile are (token, head of the group): short prompts fill tiles, and a tile's rows end close to one another.  Queries become
+// f16 as they are loaded, each row scaled below 2^15 by a power of two.
+//
+// 128 exponentials per row bound the loop (2048 cycles per 256 x 128 scores, as many as its MMAs at 128 columns), so conversion has warps
+// of its own, with the registers that the softmax leaves: 80 and 176 a thread.
+#include "api.h"
+#include "kv_quant.cuh"
+#include "attn_maps.h"
+#include <cuda_fp16.h>
+#include <math.h>
+
+namespace nkb {
+
+constexpr int kP8Tile = 128;             // query rows of an MMA tile, tokens of a K or V tile
+constexpr int kP8Threads = 512;
+constexpr int kP8Regs = 128;             // a thread's registers at launch; 2 * 128 * (80 + 176) is all of them
+constexpr int kP8Slots = 8;              // tiles whose exponents are kept: more than converters can be ahead of the softmax
+constexpr float kP8Grow = 8.f;           // log2 of the growth of a row's maximum that makes O follow
+constexpr float kP8Lift = 6.f;           // log2 of a weight at the maximum, and of a value at the tile's largest scale
+
+struct PrefillQ8Params {
+  const __nv_bfloat16* q;
+  const uint8_t *k_values, *k_scales, *v_values, *v_scales;
+  const int *block_table, *q_start, *q_lens, *context_lens;
+  __nv_bfloat16* out;
+  const float* sinks;
+  int* status;
+  int total_q, nq, nkv, group, num_blocks, table_width, causal, window, chunk;
+  long long table_stride;
+  float scale_log2;
+};
+
+struct PrefillQ8Ctrl {
+  uint64_t q_full[2];
+  uint64_t kv_full[4], kv_empty[4];
+  uint64_t e_full[kP8Slots];
+  uint64_t s_full[2], s_empty[2], p_full[2], o_full[2];
+  uint64_t turn[2][4];
+  int e_k[kP8Slots], e_v[kP8Slots];
+  uint32_t tmem_base;
+  int abort;
+};
+
+// (inlined: a call would not allow the register split)
+__device__ __forceinline__ bool p8_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  return mbar_wait(bar, parity, abort_flag, status, code);
+}
+
+// Tiles [lo, hi) that a query tile attends to, and its rows
+struct P8Range {
+  int lo, hi, rows;
+};
+__device__ __forceinline__ P8Range p8_range(const PrefillQ8Params& p, int row0, int all_rows, int q_len, int ctx) {
+  P8Range r{0, 0, 0};
+  if (row0 >= all_rows) return r;
+  r.rows = min(kP8Tile, all_rows - row0);
+  const int first = ctx - q_len + row0 / p.group, last = ctx - q_len + (row0 + r.rows - 1) / p.group;
+  r.hi = (max(ctx, 0) + kP8Tile - 1) / kP8Tile;
+  if (p.causal) r.hi = min(r.hi, (max(last, -1) + kP8Tile) / kP8Tile);
+  r.lo = nkb_first_visible(first, p.window, p.chunk) / kP8Tile;
+  if (r.hi < r.lo) r.hi = r.lo;
+  return r;
+}
+
+template <int D>
+struct PrefillQ8Smem {
+  static constexpr int NH = D / 64;                       // 128-byte halves of a row
+  static constexpr int kHalf = kP8Tile * 128;             // [128 rows][64 f16], swizzled
+  static constexpr int kTile = NH * kHalf;                // Q, K or V tile
+  static constexpr int kP = 2 * kHalf;                    // weights [128][128]
+  static constexpr int kStages = D == 64 ? 4 : 3;
+  static constexpr int kBytes = 2 * kTile + kStages * kTile + 2 * kP + int(sizeof(PrefillQ8Ctrl)) + 1024;
+  static_assert(kBytes <= 232448, "shared memory of a CTA");
+};
+
+// 2^d as a pair of f16, 0 below what f16 has
+__device__ __forceinline__ uint32_t f16x2_pow2(int d) {
+  const uint32_t h = d >= -14 ? uint32_t(d + 15) << 10 : (d >= -24 ? 1u << (d + 24) : 0u);
+  return h | (h << 16);
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t p8_pack_f16x2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ void st_shared_16(uint32_t at, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+// Instruction descriptor for kind::f16 with f16 inputs and fp32 accumulation
+__host__ __device__ constexpr uint32_t p8_idesc(int m, int n, int b_mn_major) {
+  return (1u << 4) | (uint32_t(b_mn_major) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const PrefillQ8Params p) {
+  using L = PrefillQ8Smem<D>;
+  constexpr int NH = L::NH, kHalf = L::kHalf, kStages = L::kStages;
+  constexpr uint32_t kAll = 0xffffffffu, kTmemCols = 512, kSCol = 0, kOCol = 256;
+  const int qt = gridDim.x - 1 - blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;      // the longest rows start first
+  griddep_wait();
+  griddep_launch();
+  const int q_len = p.q_lens[b], all_rows = q_len * p.group;
+  if (qt * 2 * kP8Tile >= all_rows) return;
+  const int ctx = min(p.context_lens[b], p.table_width * kQ8Page);
+  const P8Range tr0 = p8_range(p, qt * 2 * kP8Tile, all_rows, q_len, ctx), tr1 = p8_range(p, (qt * 2 + 1) * kP8Tile, all_rows, q_len, ctx);
+  const bool two = tr1.rows > 0;
+  const int u_lo = tr0.lo, u_hi = two ? max(tr0.hi, tr1.hi) : tr0.hi, n_union = u_hi - u_lo;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* q_s = smem;
+  uint8_t* kv_s = q_s + 2 * L::kTile;
+  uint8_t* p_s = kv_s + kStages * L::kTile;
+  PrefillQ8Ctrl* ctrl = reinterpret_cast<PrefillQ8Ctrl*>(p_s + 2 * L::kP);
+  const int warp = warp_idx_uniform(), lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&ctrl->kv_full[i], 4);                    // one arrival from each converting warp
+      mbar_init(&ctrl->kv_empty[i], two ? 2 : 1);         // one from each query tile's issuer
+    }
+    for (int i = 0; i < kP8Slots; ++i) mbar_init(&ctrl->e_full[i], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&ctrl->q_full[i], 4);
+      mbar_init(&ctrl->s_full[i], 1);
+      mbar_init(&ctrl->s_empty[i], 4);
+      mbar_init(&ctrl->p_full[i], 4);
+      mbar_init(&ctrl->o_full[i], 1);
+      for (int q = 0; q < 4; ++q) mbar_init(&ctrl->turn[i][q], 1);
+    }
+    ctrl->abort = 0;
+    mbar_fence_init();
+    fence_proxy_async();
+  }
+  if (warp == 12) {
+    tmem_alloc(&ctrl->tmem_base, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = __shfl_sync(kAll, ctrl->tmem_base, 0);
+  volatile int* abort_flag = &ctrl->abort;
+
+  if (warp < 4) {
+    // ---------------------------------------------------------------- conversion
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    constexpr int kRows = 512 / D, kSteps = kQ8Page / kRows;       // tokens per sixteen-byte load of the warp, loads per page
+    constexpr int kLanes = D / 16;                                 // lanes that share a token
+    const int piece = lane % kLanes, row_of = lane / kLanes;
+    const int* table = p.block_table + b * p.table_stride;
+    // tokens that some row sees
+    const int first = ctx - q_len + qt * 2 * kP8Tile / p.group;
+    const int vis_lo = nkb_first_visible(first, p.window, p.chunk);
+    const int vis_hi = p.causal ? min(ctx, ctx - q_len + (min((qt + 1) * 2 * kP8Tile, all_rows) - 1) / p.group + 1) : ctx;
+    auto table_of = [&](int x) {                                   // block of page lane / 8 of walk position x; -1: none
+      const int page = (u_lo + x) * 4 + (lane >> 3);
+      const int blk = x < n_union && page * kQ8Page < ctx ? table[page] : -1;
+      return blk >= 0 && blk < p.num_blocks ? blk : -1;
+    };
+    auto scales_of = [&](const uint8_t* at, int blk) {             // scale bytes of tokens 4 lane .. 4 lane + 3 of the tile
+      return blk >= 0 ? *reinterpret_cast<const uint32_t*>(at + ((long long)blk * p.nkv + kvh) * kQ8Page + (lane & 7) * 4) : 0x7f7f7f7fu;
+    };
+    uint4 cur[kSteps];
+    struct Page {                                                  // this warp's page of a tile: where it lies, its rows [lo, hi) that are seen
+      const uint8_t* at;
+      int lo, hi;
+    };
+    auto page_of = [&](const uint8_t* at, int blk, int x) {
+      const int tok = (u_lo + x) * kP8Tile + warp * kQ8Page + row_of;
+      return Page{at + ((long long)max(blk, 0) * p.nkv + kvh) * (kQ8Page * D) + lane * 16, vis_lo - tok, blk >= 0 ? vis_hi - tok : -kQ8Page};
+    };
+    auto load = [&](const Page& g, int i) {                        // 512 bytes of it
+      cur[i] = i * kRows >= g.lo && i * kRows < g.hi ? __ldg(reinterpret_cast<const uint4*>(g.at + i * 512)) : make_uint4(0u, 0u, 0u, 0u);
+    };
+    // order of the tiles: K(0), then K(u + 1), V(u), as the issuers take them
+    int blk_x = table_of(0), blk_n = table_of(1);                  // blocks of the K tile at hand and of the next
+    uint32_t kb = scales_of(p.k_scales, blk_x), vb = scales_of(p.v_scales, blk_x);
+    uint32_t kb_n = 0, vb_n = 0;
+    int my_v = 0;                                                  // this warp's block of the V tile at hand
+    uint32_t v_fac = 0, v_fac_n = 0;                               // factors of token `lane` of its page
+    int my_k = __shfl_sync(kAll, blk_x, warp * 8);
+    {
+      const Page g = page_of(p.k_values, my_k, 0);
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) load(g, i);
+    }
+    // where the lane's two chunks of a row go: where eight lanes have one row (D = 128), those of its second half store the odd chunk first,
+    // so that all banks are used
+    const int odd = NH == 2 ? piece >> 2 : 0;
+    const uint32_t to0 = smem_u32(kv_s) + (piece >> 2) * kHalf + (warp * kQ8Page + row_of) * 128 + ((((piece & 3) * 2 + odd) ^ row_of) << 4);
+    int seq = 0;
+    bool live = n_union > 0;
+    // converts `cur` into ring stage seq % kStages while it loads the next item
+    auto convert = [&](uint32_t fac, const uint8_t* next_at, int next_blk, int next_x) {
+      const int st = seq % kStages;
+      const uint32_t ph = uint32_t(seq / kStages) & 1u;
+      ++seq;
+      const bool ok = p8_wait(&ctrl->kv_empty[st], ph ^ 1u, abort_flag, p.status, ERR_WAIT_SMEM_EMPTY);
+      if (!__all_sync(kAll, ok)) {
+        live = false;
+        return;
+      }
+      const Page g = page_of(next_at ? next_at : p.k_values, next_at ? next_blk : -1, next_x);
+      const uint32_t to = to0 + st * L::kTile;
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        const uint4 v = cur[i];
+        load(g, i);
+        const uint32_t f = __shfl_sync(kAll, fac, i * kRows + row_of);
+        const uint4 lo = make_uint4(hmul2(e4m3x2_to_f16x2(uint16_t(v.x)), f), hmul2(e4m3x2_to_f16x2(uint16_t(v.x >> 16)), f),
+                                    hmul2(e4m3x2_to_f16x2(uint16_t(v.y)), f), hmul2(e4m3x2_to_f16x2(uint16_t(v.y >> 16)), f));
+        const uint4 hi = make_uint4(hmul2(e4m3x2_to_f16x2(uint16_t(v.z)), f), hmul2(e4m3x2_to_f16x2(uint16_t(v.z >> 16)), f),
+                                    hmul2(e4m3x2_to_f16x2(uint16_t(v.w)), f), hmul2(e4m3x2_to_f16x2(uint16_t(v.w >> 16)), f));
+        // rows four on: bit 2 of the swizzle
+        const uint32_t at = (to ^ (kRows == 4 && (i & 1) ? 64u : 0u)) + i * kRows * 128;
+        st_shared_16(at, odd ? hi : lo);
+        st_shared_16(at ^ 16u, odd ? lo : hi);
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctrl->kv_full[st]);
+    };
+    // a K tile: exponents of the tile, factors of this warp's tokens of K and (for later) V
+    auto do_k = [&](int x, const uint8_t* next_at, int next_blk, int next_x) {
+      int ek = kQ8MinLog2, ev = kQ8MinLog2;
+      const int tok0 = (u_lo + x) * kP8Tile + lane * 4;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int k = (kb >> (8 * j)) & 255, v = (vb >> (8 * j)) & 255;
+        const bool on = tok0 + j < vis_hi && tok0 + j >= vis_lo && k != 255 && v != 255;
+        ek = max(ek, on ? q8_log2_of(k) : kQ8MinLog2);
+        ev = max(ev, on ? q8_log2_of(v) : kQ8MinLog2);
+      }
+      ek = __reduce_max_sync(kAll, ek);
+      ev = __reduce_max_sync(kAll, ev);
+      const int at = warp * 8 + (lane >> 2), sh = 8 * (lane & 3);
+      const int k = (__shfl_sync(kAll, kb, at) >> sh) & 255, v = (__shfl_sync(kAll, vb, at) >> sh) & 255;
+      const int tok = (u_lo + x) * kP8Tile + warp * kQ8Page + lane;
+      const bool seen = tok < vis_hi && tok >= vis_lo, none = k == 255 || v == 255;      // none: the row stands for NaN, its scores too
+      const uint32_t fac = !seen ? 0u : (none ? 0x7fff7fffu : f16x2_pow2(q8_log2_of(k) - ek + int(kP8Lift)));
+      v_fac_n = !seen || none ? 0u : f16x2_pow2(q8_log2_of(v) - ev + int(kP8Lift));
+      if (warp == 0 && lane == 0) {
+        ctrl->e_k[x % kP8Slots] = ek;
+        ctrl->e_v[x % kP8Slots] = ev;
+        mbar_arrive(&ctrl->e_full[x % kP8Slots]);
+      }
+      convert(fac, next_at, next_blk, next_x);
+    };
+    if (live) {
+      kb_n = scales_of(p.k_scales, blk_n);
+      vb_n = scales_of(p.v_scales, blk_n);
+      my_v = my_k;
+      my_k = __shfl_sync(kAll, blk_n, warp * 8);
+      const bool more = n_union > 1;
+      do_k(0, more ? p.k_values : p.v_values, more ? my_k : my_v, more ? 1 : 0);
+      v_fac = v_fac_n;
+    }
+#pragma unroll 1
+    for (int u = 0; u < n_union && live; ++u) {
+      // at hand: K(u + 1) if there is one, else V(u)
+      if (u + 1 < n_union) {
+        const int blk_2 = table_of(u + 2);
+        kb = kb_n;
+        vb = vb_n;
+        do_k(u + 1, p.v_values, my_v, u);
+        if (!live) break;
+        kb_n = scales_of(p.k_scales, blk_2);
+        vb_n = scales_of(p.v_scales, blk_2);
+        const int my_k1 = my_k;
+        my_k = __shfl_sync(kAll, blk_2, warp * 8);
+        const bool k_next = u + 2 < n_union;                       // then V(u + 1) comes behind K(u + 2)
+        convert(v_fac, k_next ? p.k_values : p.v_values, k_next ? my_k : my_k1, k_next ? u + 2 : u + 1);
+        my_v = my_k1;
+        v_fac = v_fac_n;
+      } else {
+        convert(v_fac, nullptr, 0, 0);
+      }
+    }
+  } else if (warp >= 12) {
+    // ---------------------------------------------------------------- MMA issuers, one per query tile (see attn_prefill.cu)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    constexpr uint32_t idesc_qk = p8_idesc(128, kP8Tile, 0), idesc_pv = p8_idesc(128, D, 1);
+    const int t = warp - 12;
+    if (t < 2 && (t == 0 || two) && elect_one()) {
+      const P8Range tr = t == 0 ? tr0 : tr1;
+      const int a_lo = tr.lo - u_lo, a_hi = tr.hi - u_lo;
+      const uint32_t q_lo = uint32_t(make_smem_desc_sw128(smem_u32(q_s + t * L::kTile), 0, 1024));
+      const uint32_t kv_lo = uint32_t(make_smem_desc_sw128(smem_u32(kv_s), 0, 1024));
+      const uint32_t p_lo = uint32_t(make_smem_desc_sw128(smem_u32(p_s + t * L::kP), 0, 1024));
+      const uint64_t hk = uint64_t(uint32_t(make_smem_desc_sw128(0, 0, 1024) >> 32)) << 32;
+      const uint32_t lbo_v = (uint32_t(kHalf) >> 4) << 16;
+      const uint32_t s_tmem = tmem_base + kSCol + t * 128, o_tmem = tmem_base + kOCol + t * 128;
+      bool ok = p8_wait(&ctrl->q_full[t], 0, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
+      int seq = 0;
+      auto do_k = [&](int x) {
+        if (x >= n_union || !ok) return;
+        const int item = seq++, st = item % kStages;
+        ok = p8_wait(&ctrl->kv_full[st], uint32_t(item / kStages) & 1u, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
+        if (!ok) return;
+        if (x >= a_lo && x < a_hi) {
+          ok = p8_wait(&ctrl->s_empty[t], (uint32_t(x - a_lo) & 1u) ^ 1u, abort_flag, p.status, ERR_WAIT_TMEM_EMPTY);
+          if (!ok) return;
+          tc_fence_after();
+          const uint32_t kvd = kv_lo + uint32_t(st * L::kTile >> 4);
+#pragma unroll
+          for (int h = 0; h < NH; ++h) {
+            uint64_t da[4], db[4];
+#pragma unroll
+            for (int k4 = 0; k4 < 4; ++k4) {
+              da[k4] = hk | (q_lo + uint32_t(h * (kHalf >> 4) + k4 * 2));
+              db[k4] = hk | (kvd + uint32_t(h * (kHalf >> 4) + k4 * 2));
+            }
+            umma4_ss(s_tmem, da, db, idesc_qk, h > 0 ? 1u : 0u);
+          }
+          umma_commit(&ctrl->s_full[t]);
+        }
+        umma_commit(&ctrl->kv_empty[st]);
+      };
+      auto do_v = [&](int x) {
+        if (!ok) return;
+        const int item = seq++, st = item % kStages;
+        ok = p8_wait(&ctrl->kv_full[st], uint32_t(item / kStages) & 1u, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
+        if (!ok) return;
+        if (x >= a_lo && x < a_hi) {
+          ok = p8_wait(&ctrl->p_full[t], uint32_t(x - a_lo) & 1u, abort_flag, p.status, ERR_WAIT_SOFTMAX);
+          if (!ok) return;
+          tc_fence_after();
+          const uint32_t kvd = kv_lo + uint32_t(st * L::kTile >> 4);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint64_t da[4], db[4];
+#pragma unroll
+            for (int k4 = 0; k4 < 4; ++k4) {
+              db[k4] = hk | ((kvd + uint32_t((h * 4 + k4) * 128)) | lbo_v);
+              da[k4] = hk | (p_lo + uint32_t(h * (kHalf >> 4) + k4 * 2));
+            }
+            umma4_ss(o_tmem, da, db, idesc_pv, (x > a_lo || h > 0) ? 1u : 0u);
+          }
+          umma_commit(&ctrl->o_full[t]);
+        }
+        umma_commit(&ctrl->kv_empty[st]);
+      };
+      do_k(0);
+#pragma unroll 1
+      for (int u = 0; u < n_union && ok; ++u) {
+        do_k(u + 1);
+        do_v(u);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- softmax, one thread per row
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+    const int t = (warp - 4) >> 2, quad = warp & 3;
+    const P8Range tr = t == 0 ? tr0 : tr1;
+    const int r = quad * 32 + lane, row = (qt * 2 + t) * kP8Tile + r;      // row of (token, head) pairs
+    const int token = row / p.group, head = kvh * p.group + row % p.group;
+    const long long q_row = (long long)p.q_start[b] + token;
+    const bool mine = r < tr.rows && q_row >= 0 && q_row < p.total_q;
+    const uint32_t lane_off = uint32_t(quad * 32) << 16;
+    const uint32_t s_addr = tmem_base + lane_off + kSCol + t * 128, o_addr = tmem_base + lane_off + kOCol + t * 128;
+    uint8_t* my_p = p_s + t * L::kP + r * 128;
+    float raw_log2 = 0.f;                                                  // raw score -> exponent of two, without 2^K
+    if (tr.rows > 0) {
+      uint4 v[D / 8];
+      const uint4* src = reinterpret_cast<const uint4*>(p.q + (q_row * p.nq + head) * D);
+      float mx = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) v[i] = mine ? src[i] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = unpack_bf16x2(w[j]);
+          mx = fmax3(mx, fabsf(f.x), fabsf(f.y));
+        }
+      }
+      const int e = max((__float_as_int(mx) >> 23) - 127, -100);
+      const float up = exp2_int(14 - e);
+      raw_log2 = p.scale_log2 * exp2_int(e - 14);
+      uint8_t* dst = q_s + t * L::kTile + r * 128;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+        uint32_t h[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = unpack_bf16x2(w[j]);
+          h[j] = p8_pack_f16x2(f.x * up, f.y * up);
+        }
+        *reinterpret_cast<uint4*>(dst + (i >> 3) * kHalf + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctrl->q_full[t]);
+    }
+    const int n_tiles = tr.hi - tr.lo, n_other = t == 0 ? (two ? tr1.hi - tr1.lo : 0) : tr0.hi - tr0.lo;
+    const int q_pos = ctx - q_len + token, hi_pos = p.causal ? min(ctx - 1, q_pos) : ctx - 1;
+    const int lo_pos = nkb_first_visible(q_pos, p.window, p.chunk);
+    float m = -INFINITY, l = 0.f;
+    bool alive = true;
+    for (int it = 0; it < n_tiles; ++it) {
+      const int x = tr.lo - u_lo + it, kv0 = (tr.lo + it) * kP8Tile;
+      bool ok = p8_wait(&ctrl->e_full[x % kP8Slots], uint32_t(x / kP8Slots) & 1u, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
+      ok = ok && p8_wait(&ctrl->s_full[t], uint32_t(it) & 1u, abort_flag, p.status, ERR_WAIT_TMEM_FULL);
+      if (!__all_sync(kAll, ok)) { alive = false; break; }
+      const int e_k = *(volatile int*)&ctrl->e_k[x % kP8Slots], e_v = *(volatile int*)&ctrl->e_v[x % kP8Slots];
+      const float to_log2 = raw_log2 * exp2_int(e_k - int(kP8Lift)), add = float(e_v);
+      tc_fence_after();
+      uint32_t v[kP8Tile];
+#pragma unroll
+      for (int c = 0; c < kP8Tile / 32; ++c) tmem_ld_32x32(s_addr + c * 32, reinterpret_cast<uint32_t(&)[32]>(v[c * 32]));
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctrl->s_empty[t]);      // the scores (and the tile's exponents) are in registers
+      const bool edge = kv0 + kP8Tile - 1 > hi_pos || kv0 < lo_pos;
+      if (__any_sync(kAll, edge)) {
+        const int hi_rel = hi_pos - kv0, lo_rel = lo_pos - kv0;
+#pragma unroll
+        for (int i = 0; i < kP8Tile; ++i)
+          if (i > hi_rel || i < lo_rel) v[i] = 0xff800000u;
+      }
+      float mx4[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx4[i] = fmaxf(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+#pragma unroll
+      for (int i = 8; i < kP8Tile; i += 2) mx4[(i >> 1) & 3] = fmax3(mx4[(i >> 1) & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+      const float mx = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), to_log2, add);
+      bool p_free = it == 0;
+      if (it == 0) {
+        m = mx;
+      } else {
+        const bool grow = mx > m + kP8Grow;
+        if (__any_sync(kAll, grow)) {
+          ok = p8_wait(&ctrl->o_full[t], uint32_t(it - 1) & 1u, abort_flag, p.status, ERR_WAIT_TMEM_FULL);
+          if (!__all_sync(kAll, ok)) { alive = false; break; }
+          p_free = true;
+          tc_fence_after();
+          const float alpha = grow ? exp2f(m - mx) : 1.f;
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32(o_addr + c * 32, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st_32x32(o_addr + c * 32, o);
+          }
+          tmem_st_wait();
+          l *= alpha;
+          if (grow) m = mx;
+        }
+      }
+      const float less = add + kP8Lift - (m == -INFINITY ? 0.f : m);
+      const float2 sc2 = make_float2(to_log2, to_log2), nb2 = make_float2(less, less);
+      float2 sum2[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum2[i] = make_float2(0.f, 0.f);
+      if (!p_free) {
+        ok = p8_wait(&ctrl->o_full[t], uint32_t(it - 1) & 1u, abort_flag, p.status, ERR_WAIT_TMEM_FULL);
+        if (!__all_sync(kAll, ok)) { alive = false; break; }
+      }
+      // turns with the exponentials: tile 0 (it), tile 1 (it), tile 0 (it + 1), ...
+      if (t == 0 ? (it >= 1 && it - 1 < n_other) : (it < n_other)) {
+        ok = p8_wait(&ctrl->turn[t][quad], uint32_t(t == 0 ? it - 1 : it) & 1u, abort_flag, p.status, ERR_WAIT_SOFTMAX);
+        if (!__all_sync(kAll, ok)) { alive = false; break; }
+      }
+#pragma unroll
+      for (int c = 0; c < kP8Tile / 32; ++c) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int k = c * 32 + 2 * i;
+          const float2 y = ffma2(make_float2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), sc2, nb2);
+          const float2 e = make_float2(exp2f(y.x), exp2f(y.y));
+          sum2[i & 3] = fadd2(sum2[i & 3], e);
+          pk[i] = p8_pack_f16x2(e.x, e.y);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<uint4*>(my_p + (c >> 1) * kHalf + ((((c & 1) * 4 + q) ^ (r & 7)) << 4)) =
+              make_uint4(pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctrl->turn[1 - t][quad]);
+      fence_proxy_async();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctrl->p_full[t]);
+      const float2 s4 = fadd2(fadd2(sum2[0], sum2[1]), fadd2(sum2[2], sum2[3]));
+      l = fmaf(s4.x + s4.y, exp2_int(-e_v), l);
+    }
+    // ---- O / l
+    if (tr.rows > 0) {
+      bool have_o = false;
+      if (alive && n_tiles > 0) {
+        const bool ok = p8_wait(&ctrl->o_full[t], uint32_t(n_tiles - 1) & 1u, abort_flag, p.status, ERR_WAIT_TMEM_FULL);
+        have_o = __all_sync(kAll, ok);
+        if (have_o) tc_fence_after();
+      }
+      float osc = exp2f(-kP8Lift);                        // what values are larger by
+      if (p.sinks) {
+        const float sk = p.sinks[mine ? head : 0] * 1.4426950408889634f, m2 = fmaxf(m, sk), keep = m == -INFINITY ? 0.f : exp2f(m - m2);
+        osc *= keep;
+        l = l * keep + exp2f(sk - m2 + kP8Lift);
+      }
+      const float inv = l == 0.f ? 0.f : osc / l;
+      __nv_bfloat16* dst = p.out + (q_row * p.nq + head) * D;
+      const bool store = mine && !*abort_flag;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        if (have_o) {
+          tmem_ld_32x32(o_addr + c * 32, o);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0u;
+        }
+        if (store) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            uint4 w;
+            w.x = pack_bf16x2(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
+            w.y = pack_bf16x2(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
+            w.z = pack_bf16x2(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
+            w.w = pack_bf16x2(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
+            *reinterpret_cast<uint4*>(dst + c * 32 + i) = w;
+          }
+        }
+      }
+    }
+  }
+
+  if (*abort_flag) {
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, kTmemCols);
+  }
+}
+
+template <int D>
+static int launch_prefill_q8(const PrefillQ8Params& p, int batch, int max_q_len, cudaStream_t s) {
+  using L = PrefillQ8Smem<D>;
+  static bool attr_set[64] = {false};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
+  if (!attr_set[dev]) {
+    // the register split would wait for registers that a smaller launch does not have
+    cudaFuncAttributes a;
+    if (cudaError_t e = cudaFuncGetAttributes(&a, attn_q8_prefill_kernel<D>)) return int(e);
+    if (a.numRegs != kP8Regs) return -3;
+    if (cudaError_t e = cudaFuncSetAttribute(attn_q8_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes)) return int(e);
+    attr_set[dev] = true;
+  }
+  const long long tiles = ((long long)max_q_len * p.group + 2 * kP8Tile - 1) / (2 * kP8Tile);
+  if (tiles > 0x7fffffffll) return -2;
+  return launch_pdl(attn_q8_prefill_kernel<D>, dim3(unsigned(tiles), p.nkv, batch), dim3(kP8Threads), size_t(L::kBytes), s, p);
+}
+
+}  // namespace nkb
+
+using namespace nkb;
+
+extern "C" int nkb_q8_attn_prefill(const void* q, const void* k_values, const void* k_scales, const void* v_values, const void* v_scales,
+                                   const int* block_table, const int* q_start, const int* q_lens, const int* context_lens, void* out,
+                                   int batch, int total_q, int max_q_len, int nq, int nkv, int head_dim, int num_blocks, int table_width,
+                                   long long table_stride, float scale, int causal, int window, int chunk, const float* sinks,
+                                   void* stream) {
+  if (batch <= 0 || total_q <= 0) return 0;
+  if (batch > 65535 || nkv > 65535 || nkv < 1 || nq % nkv || max_q_len < 1) return -2;
+  if (!status_word() && nkb_init() != 0) return -1;
+  PrefillQ8Params p{};
+  p.q = (const __nv_bfloat16*)q;
+  p.k_values = (const uint8_t*)k_values; p.k_scales = (const uint8_t*)k_scales;
+  p.v_values = (const uint8_t*)v_values; p.v_scales = (const uint8_t*)v_scales;
+  p.block_table = block_table; p.q_start = q_start; p.q_lens = q_lens; p.context_lens = context_lens;
+  p.out = (__nv_bfloat16*)out;
+  p.sinks = sinks;
+  p.status = status_word();
+  p.total_q = total_q; p.nq = nq; p.nkv = nkv; p.group = nq / nkv; p.num_blocks = num_blocks; p.table_width = table_width;
+  p.causal = causal; p.window = window; p.chunk = chunk;
+  p.table_stride = table_stride;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (head_dim == 128) return launch_prefill_q8<128>(p, batch, max_q_len, s);
+  if (head_dim == 64) return launch_prefill_q8<64>(p, batch, max_q_len, s);
+  return -2;
+}

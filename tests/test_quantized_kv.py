@@ -59,7 +59,9 @@ def oracle_attend(q, k, v, scale, pos, causal=True, window=0, chunk=0, sinks=Non
 
     Tolerance: the result is rounded to bf16 (2^-8 of it); weights to f16 (2^-11 each), exponentials by the special-function unit and
     sums in 32 bits (2^-19), and scores in 32 bits, where a tensor core cuts each of the up to eight partial sums behind 2^-22 of what
-    it holds: 2^-19 of sum |q k|, which moves a weight by that much of itself, and the sum of weights too."""
+    it holds: 2^-19 of sum |q k|, which moves a weight by that much of itself, and the sum of weights too.  f16's steps end at 2^-24:
+    with the largest weight at 2^6 or above, a weight is off by up to 2^-31 of the largest besides (which takes a value's scale in, so
+    that it may be that of the largest value), for every token."""
     n = k.shape[0]
     at = torch.arange(n)
     seen = at <= pos if causal else torch.ones(n, dtype=torch.bool)
@@ -79,7 +81,7 @@ def oracle_attend(q, k, v, scale, pos, causal=True, window=0, chunk=0, sinks=Non
     p = p / total
     o = p @ v
     moved = 2.0 ** -19 * float((k.abs() @ q.abs()).max()) * scale
-    return o, 2.0 ** -8 * o.abs() + (p @ v.abs()) * (2.0 ** -11 + 2.0 ** -19 + 2 * moved) + 1e-30
+    return o, 2.0 ** -8 * o.abs() + (p @ v.abs()) * (2.0 ** -11 + 2.0 ** -19 + 2 * moved) + n * 2.0 ** -30 * float(v.abs().max()) + 1e-30
 
 
 def check_attention(out, q, k_pages, v_pages, table, spans, scale, nq, group, sinks=None, **masks):
