@@ -5,9 +5,9 @@
 // The structure is that of prefill attention over bf16 pages (attn_prefill.cu: two 128-row query tiles in ping-pong, one MMA issuer each,
 // S and O in tensor memory, one softmax thread per row, turns with the exponentials), with what 8 bits change:
 //
-//   warps 0-3    convert: a warp takes one page of every 128-token tile from global memory (a tile ahead, in registers), makes it f16
-//                in the swizzled layout that the MMA reads and brings the tokens to the tile's largest scale, 2^K for keys and 2^V
-//                for values, on the way
+//   warps 0-3    convert: a warp takes one page of every 128-token tile (bulk copies into a ring of its own, ahead), makes it f16 in the
+//                swizzled layout that the MMA reads and brings the tokens to the tile's largest scale, 2^K for keys and 2^V for
+//                values, on the way
 //   warps 4-11   softmax
 //   warps 12, 13 issue tcgen05.mma (14 and 15 idle)
 //
@@ -20,7 +20,7 @@
 // f16 as they are loaded, each row scaled below 2^15 by a power of two.
 //
 // 128 exponentials per row bound the loop (2048 cycles per 256 x 128 scores, as many as its MMAs at 128 columns), so conversion has warps
-// of its own, with the registers that the softmax leaves: 80 and 176 a thread.
+// of its own, with the registers that the softmax leaves: 72 and 184 a thread.
 #include "api.h"
 #include "kv_quant.cuh"
 #include "attn_maps.h"
@@ -31,7 +31,7 @@ namespace nkb {
 
 constexpr int kP8Tile = 128;             // query rows of an MMA tile, tokens of a K or V tile
 constexpr int kP8Threads = 512;
-constexpr int kP8Regs = 128;             // a thread's registers at launch; 2 * 128 * (80 + 176) is all of them
+constexpr int kP8Regs = 128;             // a thread's registers at launch; 2 * 128 * (72 + 184) is all of them
 constexpr int kP8Slots = 8;              // tiles whose exponents are kept: more than converters can be ahead of the softmax
 constexpr float kP8Grow = 8.f;           // log2 of the growth of a row's maximum that makes O follow
 constexpr float kP8Lift = 6.f;           // log2 of a weight at the maximum, and of a value at the tile's largest scale
@@ -50,6 +50,7 @@ struct PrefillQ8Params {
 
 struct PrefillQ8Ctrl {
   uint64_t q_full[2];
+  uint64_t raw_full[4][4];               // [stage][warp]
   uint64_t kv_full[4], kv_empty[4];
   uint64_t e_full[kP8Slots];
   uint64_t s_full[2], s_empty[2], p_full[2], o_full[2];
@@ -86,8 +87,9 @@ struct PrefillQ8Smem {
   static constexpr int kHalf = kP8Tile * 128;             // [128 rows][64 f16], swizzled
   static constexpr int kTile = NH * kHalf;                // Q, K or V tile
   static constexpr int kP = 2 * kHalf;                    // weights [128][128]
-  static constexpr int kStages = D == 64 ? 4 : 3;
-  static constexpr int kBytes = 2 * kTile + kStages * kTile + 2 * kP + int(sizeof(PrefillQ8Ctrl)) + 1024;
+  static constexpr int kStages = D == 64 ? 4 : 2;         // of the f16 ring, and of every warp's ring of pages
+  static constexpr int kPageBytes = kQ8Page * D;
+  static constexpr int kBytes = 2 * kTile + kStages * (kTile + 4 * kPageBytes) + 2 * kP + int(sizeof(PrefillQ8Ctrl)) + 1024;
   static_assert(kBytes <= 232448, "shared memory of a CTA");
 };
 
@@ -132,11 +134,13 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* q_s = smem;
   uint8_t* kv_s = q_s + 2 * L::kTile;
-  uint8_t* p_s = kv_s + kStages * L::kTile;
+  uint8_t* raw_s = kv_s + kStages * L::kTile;
+  uint8_t* p_s = raw_s + kStages * 4 * L::kPageBytes;
   PrefillQ8Ctrl* ctrl = reinterpret_cast<PrefillQ8Ctrl*>(p_s + 2 * L::kP);
   const int warp = warp_idx_uniform(), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
+      for (int w = 0; w < 4; ++w) mbar_init(&ctrl->raw_full[i][w], 1);
       mbar_init(&ctrl->kv_full[i], 4);                    // one arrival from each converting warp
       mbar_init(&ctrl->kv_empty[i], two ? 2 : 1);         // one from each query tile's issuer
     }
@@ -165,7 +169,7 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
 
   if (warp < 4) {
     // ---------------------------------------------------------------- conversion
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     constexpr int kRows = 512 / D, kSteps = kQ8Page / kRows;       // tokens per sixteen-byte load of the warp, loads per page
     constexpr int kLanes = D / 16;                                 // lanes that share a token
     const int piece = lane % kLanes, row_of = lane / kLanes;
@@ -174,76 +178,81 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
     const int first = ctx - q_len + qt * 2 * kP8Tile / p.group;
     const int vis_lo = nkb_first_visible(first, p.window, p.chunk);
     const int vis_hi = p.causal ? min(ctx, ctx - q_len + (min((qt + 1) * 2 * kP8Tile, all_rows) - 1) / p.group + 1) : ctx;
-    auto table_of = [&](int x) {                                   // block of page lane / 8 of walk position x; -1: none
-      const int page = (u_lo + x) * 4 + (lane >> 3);
+    auto block_at = [&](int x, int page_of_tile) {                 // block of a page of walk position x; -1: none
+      const int page = (u_lo + x) * 4 + page_of_tile;
       const int blk = x < n_union && page * kQ8Page < ctx ? table[page] : -1;
       return blk >= 0 && blk < p.num_blocks ? blk : -1;
     };
     auto scales_of = [&](const uint8_t* at, int blk) {             // scale bytes of tokens 4 lane .. 4 lane + 3 of the tile
       return blk >= 0 ? *reinterpret_cast<const uint32_t*>(at + ((long long)blk * p.nkv + kvh) * kQ8Page + (lane & 7) * 4) : 0x7f7f7f7fu;
     };
-    uint4 cur[kSteps];
-    struct Page {                                                  // this warp's page of a tile: where it lies, its rows [lo, hi) that are seen
-      const uint8_t* at;
-      int lo, hi;
+    // Items in the order the issuers take them: K(0), then K(u + 1), V(u).  This warp's blocks of 32 tiles at a time, lane by lane, and of
+    // the 32 behind them.
+    const int items = 2 * n_union;
+    int base = 0, blks = block_at(lane, warp), blks_n = block_at(32 + lane, warp);
+    auto my_block = [&](int x) { return __shfl_sync(kAll, x - base < 32 ? blks : blks_n, x & 31); };
+    auto is_v = [&](int i) { return i > 0 && ((i & 1) == 0 || i == items - 1); };
+    auto tile_of = [&](int i) { return i == 0 ? 0 : ((i & 1) == 0 ? i / 2 - 1 : min((i + 1) / 2, n_union - 1)); };
+    uint8_t* my_raw = raw_s + warp * L::kPageBytes;
+    auto fetch = [&](int i) {
+      if (i >= items) return;
+      const int blk = my_block(tile_of(i)), st = i % kStages;
+      if (lane == 0) {
+        uint64_t* bar = &ctrl->raw_full[st][warp];
+        if (blk >= 0) {
+          mbar_expect_tx(bar, L::kPageBytes);
+          bulk_load_1d(my_raw + st * 4 * L::kPageBytes, (is_v(i) ? p.v_values : p.k_values) + ((long long)blk * p.nkv + kvh) * L::kPageBytes,
+                       L::kPageBytes, bar);
+        } else {
+          mbar_arrive(bar);
+        }
+      }
     };
-    auto page_of = [&](const uint8_t* at, int blk, int x) {
-      const int tok = (u_lo + x) * kP8Tile + warp * kQ8Page + row_of;
-      return Page{at + ((long long)max(blk, 0) * p.nkv + kvh) * (kQ8Page * D) + lane * 16, vis_lo - tok, blk >= 0 ? vis_hi - tok : -kQ8Page};
-    };
-    auto load = [&](const Page& g, int i) {                        // 512 bytes of it
-      cur[i] = i * kRows >= g.lo && i * kRows < g.hi ? __ldg(reinterpret_cast<const uint4*>(g.at + i * 512)) : make_uint4(0u, 0u, 0u, 0u);
-    };
-    // order of the tiles: K(0), then K(u + 1), V(u), as the issuers take them
-    int blk_x = table_of(0), blk_n = table_of(1);                  // blocks of the K tile at hand and of the next
-    uint32_t kb = scales_of(p.k_scales, blk_x), vb = scales_of(p.v_scales, blk_x);
-    uint32_t kb_n = 0, vb_n = 0;
-    int my_v = 0;                                                  // this warp's block of the V tile at hand
-    uint32_t v_fac = 0, v_fac_n = 0;                               // factors of token `lane` of its page
-    int my_k = __shfl_sync(kAll, blk_x, warp * 8);
-    {
-      const Page g = page_of(p.k_values, my_k, 0);
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) load(g, i);
-    }
+#pragma unroll 1
+    for (int i = 0; i < kStages; ++i) fetch(i);
+    const int blk_0 = block_at(0, lane >> 3), blk_1 = block_at(1, lane >> 3);
+    uint32_t kb = scales_of(p.k_scales, blk_0), vb = scales_of(p.v_scales, blk_0);
+    uint32_t kb_n = scales_of(p.k_scales, blk_1), vb_n = scales_of(p.v_scales, blk_1);     // of the next tile
+    uint32_t v_fac = 0, v_fac_n = 0;                               // factors of token `lane` of this warp's page of V
     // where the lane's two chunks of a row go: where eight lanes have one row (D = 128), those of its second half store the odd chunk first,
     // so that all banks are used
     const int odd = NH == 2 ? piece >> 2 : 0;
     const uint32_t to0 = smem_u32(kv_s) + (piece >> 2) * kHalf + (warp * kQ8Page + row_of) * 128 + ((((piece & 3) * 2 + odd) ^ row_of) << 4);
-    int seq = 0;
-    bool live = n_union > 0;
-    // converts `cur` into ring stage seq % kStages while it loads the next item
-    auto convert = [&](uint32_t fac, const uint8_t* next_at, int next_blk, int next_x) {
-      const int st = seq % kStages;
-      const uint32_t ph = uint32_t(seq / kStages) & 1u;
-      ++seq;
-      const bool ok = p8_wait(&ctrl->kv_empty[st], ph ^ 1u, abort_flag, p.status, ERR_WAIT_SMEM_EMPTY);
+    bool live = true;
+    auto convert = [&](int i, uint32_t fac) {
+      const int st = i % kStages, x = tile_of(i);
+      const uint32_t ph = uint32_t(i / kStages) & 1u;
+      bool ok = p8_wait(&ctrl->raw_full[st][warp], ph, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
+      ok = ok && p8_wait(&ctrl->kv_empty[st], ph ^ 1u, abort_flag, p.status, ERR_WAIT_SMEM_EMPTY);
       if (!__all_sync(kAll, ok)) {
         live = false;
         return;
       }
-      const Page g = page_of(next_at ? next_at : p.k_values, next_at ? next_blk : -1, next_x);
+      const int tok = (u_lo + x) * kP8Tile + warp * kQ8Page + row_of, lo = vis_lo - tok, hi = my_block(x) >= 0 ? vis_hi - tok : -kQ8Page;
+      const uint8_t* from = my_raw + st * 4 * L::kPageBytes + lane * 16;
       const uint32_t to = to0 + st * L::kTile;
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        const uint4 v = cur[i];
-        load(g, i);
-        const uint32_t f = __shfl_sync(kAll, fac, i * kRows + row_of);
-        const uint4 lo = make_uint4(hmul2(e4m3x2_to_f16x2(uint16_t(v.x)), f), hmul2(e4m3x2_to_f16x2(uint16_t(v.x >> 16)), f),
-                                    hmul2(e4m3x2_to_f16x2(uint16_t(v.y)), f), hmul2(e4m3x2_to_f16x2(uint16_t(v.y >> 16)), f));
-        const uint4 hi = make_uint4(hmul2(e4m3x2_to_f16x2(uint16_t(v.z)), f), hmul2(e4m3x2_to_f16x2(uint16_t(v.z >> 16)), f),
-                                    hmul2(e4m3x2_to_f16x2(uint16_t(v.w)), f), hmul2(e4m3x2_to_f16x2(uint16_t(v.w >> 16)), f));
+      for (int j = 0; j < kSteps; ++j) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(from + j * 512);
+        const bool seen = j * kRows >= lo && j * kRows < hi;       // what no row sees may be anything
+        const uint4 v = seen ? raw : make_uint4(0u, 0u, 0u, 0u);
+        const uint32_t f = __shfl_sync(kAll, fac, j * kRows + row_of);
+        const uint4 a = make_uint4(hmul2(e4m3x2_to_f16x2(uint16_t(v.x)), f), hmul2(e4m3x2_to_f16x2(uint16_t(v.x >> 16)), f),
+                                   hmul2(e4m3x2_to_f16x2(uint16_t(v.y)), f), hmul2(e4m3x2_to_f16x2(uint16_t(v.y >> 16)), f));
+        const uint4 c = make_uint4(hmul2(e4m3x2_to_f16x2(uint16_t(v.z)), f), hmul2(e4m3x2_to_f16x2(uint16_t(v.z >> 16)), f),
+                                   hmul2(e4m3x2_to_f16x2(uint16_t(v.w)), f), hmul2(e4m3x2_to_f16x2(uint16_t(v.w >> 16)), f));
         // rows four on: bit 2 of the swizzle
-        const uint32_t at = (to ^ (kRows == 4 && (i & 1) ? 64u : 0u)) + i * kRows * 128;
-        st_shared_16(at, odd ? hi : lo);
-        st_shared_16(at ^ 16u, odd ? lo : hi);
+        const uint32_t at = (to ^ (kRows == 4 && (j & 1) ? 64u : 0u)) + j * kRows * 128;
+        st_shared_16(at, odd ? c : a);
+        st_shared_16(at ^ 16u, odd ? a : c);
       }
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&ctrl->kv_full[st]);
+      fetch(i + kStages);
     };
     // a K tile: exponents of the tile, factors of this warp's tokens of K and (for later) V
-    auto do_k = [&](int x, const uint8_t* next_at, int next_blk, int next_x) {
+    auto do_k = [&](int i, int x) {
       int ek = kQ8MinLog2, ev = kQ8MinLog2;
       const int tok0 = (u_lo + x) * kP8Tile + lane * 4;
 #pragma unroll
@@ -266,41 +275,34 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
         ctrl->e_v[x % kP8Slots] = ev;
         mbar_arrive(&ctrl->e_full[x % kP8Slots]);
       }
-      convert(fac, next_at, next_blk, next_x);
+      convert(i, fac);
     };
-    if (live) {
-      kb_n = scales_of(p.k_scales, blk_n);
-      vb_n = scales_of(p.v_scales, blk_n);
-      my_v = my_k;
-      my_k = __shfl_sync(kAll, blk_n, warp * 8);
-      const bool more = n_union > 1;
-      do_k(0, more ? p.k_values : p.v_values, more ? my_k : my_v, more ? 1 : 0);
+    if (n_union > 0) {
+      do_k(0, 0);
       v_fac = v_fac_n;
     }
 #pragma unroll 1
     for (int u = 0; u < n_union && live; ++u) {
-      // at hand: K(u + 1) if there is one, else V(u)
+      if (u == base + 32) {
+        base += 32;
+        blks = blks_n;
+        blks_n = block_at(base + 32 + lane, warp);
+      }
       if (u + 1 < n_union) {
-        const int blk_2 = table_of(u + 2);
+        const int blk_2 = block_at(u + 2, lane >> 3);
         kb = kb_n;
         vb = vb_n;
-        do_k(u + 1, p.v_values, my_v, u);
+        do_k(2 * u + 1, u + 1);
         if (!live) break;
         kb_n = scales_of(p.k_scales, blk_2);
         vb_n = scales_of(p.v_scales, blk_2);
-        const int my_k1 = my_k;
-        my_k = __shfl_sync(kAll, blk_2, warp * 8);
-        const bool k_next = u + 2 < n_union;                       // then V(u + 1) comes behind K(u + 2)
-        convert(v_fac, k_next ? p.k_values : p.v_values, k_next ? my_k : my_k1, k_next ? u + 2 : u + 1);
-        my_v = my_k1;
-        v_fac = v_fac_n;
-      } else {
-        convert(v_fac, nullptr, 0, 0);
       }
+      convert(u + 1 < n_union ? 2 * u + 2 : 2 * u + 1, v_fac);
+      v_fac = v_fac_n;
     }
   } else if (warp >= 12) {
     // ---------------------------------------------------------------- MMA issuers, one per query tile (see attn_prefill.cu)
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     constexpr uint32_t idesc_qk = p8_idesc(128, kP8Tile, 0), idesc_pv = p8_idesc(128, D, 1);
     const int t = warp - 12;
     if (t < 2 && (t == 0 || two) && elect_one()) {
@@ -372,7 +374,7 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- softmax, one thread per row
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
     const int t = (warp - 4) >> 2, quad = warp & 3;
     const P8Range tr = t == 0 ? tr0 : tr1;
     const int r = quad * 32 + lane, row = (qt * 2 + t) * kP8Tile + r;      // row of (token, head) pairs
