@@ -60,9 +60,19 @@ struct PrefillQ8Ctrl {
   int abort;
 };
 
-// (inlined: a call would not allow the register split)
+// Bounded barrier wait of a few instructions: the kernel has two dozen of them beside its unrolled loops, and a call would not allow the
+// register split.  A try waits for some time by itself; so many tries are seconds.
+constexpr uint32_t kP8Tries = 1u << 22;
 __device__ __forceinline__ bool p8_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
-  return mbar_wait(bar, parity, abort_flag, status, code);
+  uint32_t left = kP8Tries;
+  while (!mbar_try_wait(bar, parity)) {
+    if ((--left & 255u) == 0 && (left == 0 || *abort_flag)) {
+      *abort_flag = 1;
+      atomicCAS(status, 0, code | (blockIdx.x << 8));
+      return false;
+    }
+  }
+  return true;
 }
 
 // Tiles [lo, hi) that a query tile attends to, and its rows
@@ -210,16 +220,16 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
     };
 #pragma unroll 1
     for (int i = 0; i < kStages; ++i) fetch(i);
-    const int blk_0 = block_at(0, lane >> 3), blk_1 = block_at(1, lane >> 3);
-    uint32_t kb = scales_of(p.k_scales, blk_0), vb = scales_of(p.v_scales, blk_0);
-    uint32_t kb_n = scales_of(p.k_scales, blk_1), vb_n = scales_of(p.v_scales, blk_1);     // of the next tile
+    int blk_k = block_at(0, lane >> 3), blk_kn = block_at(1, lane >> 3);                     // of the tile at hand and of the next
+    uint32_t kb = scales_of(p.k_scales, blk_k), vb = scales_of(p.v_scales, blk_k);
+    uint32_t kb_n = scales_of(p.k_scales, blk_kn), vb_n = scales_of(p.v_scales, blk_kn);
     uint32_t v_fac = 0, v_fac_n = 0;                               // factors of token `lane` of this warp's page of V
     // where the lane's two chunks of a row go: where eight lanes have one row (D = 128), those of its second half store the odd chunk first,
     // so that all banks are used
     const int odd = NH == 2 ? piece >> 2 : 0;
     const uint32_t to0 = smem_u32(kv_s) + (piece >> 2) * kHalf + (warp * kQ8Page + row_of) * 128 + ((((piece & 3) * 2 + odd) ^ row_of) << 4);
     bool live = true;
-    auto convert = [&](int i, uint32_t fac) {
+    auto convert = [&](int i, uint32_t fac, bool whole) {
       const int st = i % kStages, x = tile_of(i);
       const uint32_t ph = uint32_t(i / kStages) & 1u;
       bool ok = p8_wait(&ctrl->raw_full[st][warp], ph, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
@@ -231,20 +241,33 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
       const int tok = (u_lo + x) * kP8Tile + warp * kQ8Page + row_of, lo = vis_lo - tok, hi = my_block(x) >= 0 ? vis_hi - tok : -kQ8Page;
       const uint8_t* from = my_raw + st * 4 * L::kPageBytes + lane * 16;
       const uint32_t to = to0 + st * L::kTile;
+      // four loads at a time, then their stores (a load behind a store would wait for it)
+      constexpr int kAhead = 4;
 #pragma unroll
-      for (int j = 0; j < kSteps; ++j) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(from + j * 512);
-        const bool seen = j * kRows >= lo && j * kRows < hi;       // what no row sees may be anything
-        const uint4 v = seen ? raw : make_uint4(0u, 0u, 0u, 0u);
-        const uint32_t f = __shfl_sync(kAll, fac, j * kRows + row_of);
-        const uint4 a = make_uint4(hmul2(e4m3x2_to_f16x2(uint16_t(v.x)), f), hmul2(e4m3x2_to_f16x2(uint16_t(v.x >> 16)), f),
-                                   hmul2(e4m3x2_to_f16x2(uint16_t(v.y)), f), hmul2(e4m3x2_to_f16x2(uint16_t(v.y >> 16)), f));
-        const uint4 c = make_uint4(hmul2(e4m3x2_to_f16x2(uint16_t(v.z)), f), hmul2(e4m3x2_to_f16x2(uint16_t(v.z >> 16)), f),
-                                   hmul2(e4m3x2_to_f16x2(uint16_t(v.w)), f), hmul2(e4m3x2_to_f16x2(uint16_t(v.w >> 16)), f));
-        // rows four on: bit 2 of the swizzle
-        const uint32_t at = (to ^ (kRows == 4 && (j & 1) ? 64u : 0u)) + j * kRows * 128;
-        st_shared_16(at, odd ? c : a);
-        st_shared_16(at ^ 16u, odd ? a : c);
+      for (int j0 = 0; j0 < kSteps; j0 += kAhead) {
+        uint4 raw[kAhead];
+        uint32_t f[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) raw[j] = *reinterpret_cast<const uint4*>(from + (j0 + j) * 512);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) f[j] = __shfl_sync(kAll, fac, (j0 + j) * kRows + row_of);
+        if (!whole) {                                              // what no row sees may be anything
+#pragma unroll
+          for (int j = 0; j < kAhead; ++j)
+            if ((j0 + j) * kRows < lo || (j0 + j) * kRows >= hi) raw[j] = make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+          const uint4 v = raw[j];
+          const uint4 a = make_uint4(hmul2(e4m3x2_to_f16x2(uint16_t(v.x)), f[j]), hmul2(e4m3x2_to_f16x2(uint16_t(v.x >> 16)), f[j]),
+                                     hmul2(e4m3x2_to_f16x2(uint16_t(v.y)), f[j]), hmul2(e4m3x2_to_f16x2(uint16_t(v.y >> 16)), f[j]));
+          const uint4 c = make_uint4(hmul2(e4m3x2_to_f16x2(uint16_t(v.z)), f[j]), hmul2(e4m3x2_to_f16x2(uint16_t(v.z >> 16)), f[j]),
+                                     hmul2(e4m3x2_to_f16x2(uint16_t(v.w)), f[j]), hmul2(e4m3x2_to_f16x2(uint16_t(v.w >> 16)), f[j]));
+          // rows four on: bit 2 of the swizzle
+          const uint32_t at = (to ^ (kRows == 4 && (j & 1) ? 64u : 0u)) + (j0 + j) * kRows * 128;
+          st_shared_16(at, odd ? c : a);
+          st_shared_16(at ^ 16u, odd ? a : c);
+        }
       }
       fence_proxy_async();
       __syncwarp();
@@ -252,34 +275,47 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
       fetch(i + kStages);
     };
     // a K tile: exponents of the tile, factors of this warp's tokens of K and (for later) V
+    bool whole = false, whole_n = false;                           // all tokens of the V tile at hand, and of the next, are seen and are numbers
     auto do_k = [&](int i, int x) {
-      int ek = kQ8MinLog2, ev = kQ8MinLog2;
-      const int tok0 = (u_lo + x) * kP8Tile + lane * 4;
+      const int tile0 = (u_lo + x) * kP8Tile;
+      // a byte is between 63 and 191 where it is a scale: bits 6 and 7 both set are a NaN
+      const bool odd_one = ((kb & (kb << 1)) | (vb & (vb << 1))) & 0x80808080u;
+      whole_n = tile0 >= vis_lo && tile0 + kP8Tile <= vis_hi && !__any_sync(kAll, odd_one || blk_k < 0);
+      uint32_t k4 = kb, v4 = vb;
+      if (!whole_n) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int k = (kb >> (8 * j)) & 255, v = (vb >> (8 * j)) & 255;
-        const bool on = tok0 + j < vis_hi && tok0 + j >= vis_lo && k != 255 && v != 255;
-        ek = max(ek, on ? q8_log2_of(k) : kQ8MinLog2);
-        ev = max(ev, on ? q8_log2_of(v) : kQ8MinLog2);
+        for (int j = 0; j < 4; ++j) {
+          const int tok = tile0 + lane * 4 + j;
+          if (tok >= vis_hi || tok < vis_lo || ((kb >> (8 * j)) & 255) == 255 || ((vb >> (8 * j)) & 255) == 255) {
+            k4 &= ~(255u << (8 * j));
+            v4 &= ~(255u << (8 * j));
+          }
+        }
       }
-      ek = __reduce_max_sync(kAll, ek);
-      ev = __reduce_max_sync(kAll, ev);
+      const uint32_t k2 = __vmaxu2(k4 & 0x00ff00ffu, (k4 >> 8) & 0x00ff00ffu), v2 = __vmaxu2(v4 & 0x00ff00ffu, (v4 >> 8) & 0x00ff00ffu);
+      const int ek = q8_log2_of(int(__reduce_max_sync(kAll, max(k2 & 0xffffu, k2 >> 16))));
+      const int ev = q8_log2_of(int(__reduce_max_sync(kAll, max(v2 & 0xffffu, v2 >> 16))));
       const int at = warp * 8 + (lane >> 2), sh = 8 * (lane & 3);
       const int k = (__shfl_sync(kAll, kb, at) >> sh) & 255, v = (__shfl_sync(kAll, vb, at) >> sh) & 255;
-      const int tok = (u_lo + x) * kP8Tile + warp * kQ8Page + lane;
-      const bool seen = tok < vis_hi && tok >= vis_lo, none = k == 255 || v == 255;      // none: the row stands for NaN, its scores too
-      const uint32_t fac = !seen ? 0u : (none ? 0x7fff7fffu : f16x2_pow2(q8_log2_of(k) - ek + int(kP8Lift)));
-      v_fac_n = !seen || none ? 0u : f16x2_pow2(q8_log2_of(v) - ev + int(kP8Lift));
+      uint32_t fac = f16x2_pow2(q8_log2_of(k) - ek + int(kP8Lift));
+      v_fac_n = f16x2_pow2(q8_log2_of(v) - ev + int(kP8Lift));
+      if (!whole_n) {
+        const int tok = tile0 + warp * kQ8Page + lane;
+        const bool seen = tok < vis_hi && tok >= vis_lo, none = k == 255 || v == 255;    // none: the row stands for NaN, its scores too
+        fac = !seen ? 0u : (none ? 0x7fff7fffu : fac);
+        v_fac_n = !seen || none ? 0u : v_fac_n;
+      }
       if (warp == 0 && lane == 0) {
         ctrl->e_k[x % kP8Slots] = ek;
         ctrl->e_v[x % kP8Slots] = ev;
         mbar_arrive(&ctrl->e_full[x % kP8Slots]);
       }
-      convert(i, fac);
+      convert(i, fac, whole_n);
     };
     if (n_union > 0) {
       do_k(0, 0);
       v_fac = v_fac_n;
+      whole = whole_n;
     }
 #pragma unroll 1
     for (int u = 0; u < n_union && live; ++u) {
@@ -292,13 +328,16 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
         const int blk_2 = block_at(u + 2, lane >> 3);
         kb = kb_n;
         vb = vb_n;
+        blk_k = blk_kn;
         do_k(2 * u + 1, u + 1);
         if (!live) break;
+        blk_kn = blk_2;
         kb_n = scales_of(p.k_scales, blk_2);
         vb_n = scales_of(p.v_scales, blk_2);
       }
-      convert(u + 1 < n_union ? 2 * u + 2 : 2 * u + 1, v_fac);
+      convert(u + 1 < n_union ? 2 * u + 2 : 2 * u + 1, v_fac, whole);
       v_fac = v_fac_n;
+      whole = whole_n;
     }
   } else if (warp >= 12) {
     // ---------------------------------------------------------------- MMA issuers, one per query tile (see attn_prefill.cu)
