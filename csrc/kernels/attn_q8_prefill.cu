@@ -5,11 +5,12 @@
 // The structure is that of prefill attention over bf16 pages (attn_prefill.cu: two 128-row query tiles in ping-pong, one MMA issuer each,
 // S and O in tensor memory, one softmax thread per row, turns with the exponentials), with what 8 bits change:
 //
-//   warps 0-3    convert: a warp takes one page of every 128-token tile (bulk copies into a ring of its own, ahead), makes it f16 in the
-//                swizzled layout that the MMA reads and brings the tokens to the tile's largest scale, 2^K for keys and 2^V for
-//                values, on the way
+//   warps 0-3    convert: a warp makes its page of every 128-token tile f16 in the swizzled layout that the MMA reads, and brings the
+//                tokens to the tile's largest scale, 2^K for keys and 2^V for values, on the way
 //   warps 4-11   softmax
-//   warps 12, 13 issue tcgen05.mma (14 and 15 idle)
+//   warps 12, 13 issue tcgen05.mma
+//   warp 14      reads the scales of the tiles to come and finds K and V
+//   warp 15      fetches the pages, by bulk copies
 //
 // f16 holds an e4m3 value times 2^-22 and up exactly or nearly (from 2^6 down, behind the tile's largest), so the products see what is
 // kept.  A tile's exponents are two numbers that enter where one number did before: 2^K in the multiplier of the scores, V in the exponent
@@ -32,7 +33,8 @@ namespace nkb {
 constexpr int kP8Tile = 128;             // query rows of an MMA tile, tokens of a K or V tile
 constexpr int kP8Threads = 512;
 constexpr int kP8Regs = 128;             // a thread's registers at launch; 2 * 128 * (72 + 184) is all of them
-constexpr int kP8Slots = 8;              // tiles whose exponents are kept: more than converters can be ahead of the softmax
+constexpr int kP8Slots = 8;              // tiles whose scales are kept
+constexpr int kP8Lead = 4;               // tiles that warp 14 is ahead of the conversion of V at most
 constexpr float kP8Grow = 8.f;           // log2 of the growth of a row's maximum that makes O follow
 constexpr float kP8Lift = 6.f;           // log2 of a weight at the maximum, and of a value at the tile's largest scale
 
@@ -50,12 +52,13 @@ struct PrefillQ8Params {
 
 struct PrefillQ8Ctrl {
   uint64_t q_full[2];
-  uint64_t raw_full[4][4];               // [stage][warp]
-  uint64_t kv_full[4], kv_empty[4];
-  uint64_t e_full[kP8Slots];
+  uint64_t raw_full[4], raw_empty[4], kv_full[4], kv_empty[4];
+  uint64_t e_full[kP8Slots], e_empty[kP8Slots];
   uint64_t s_full[2], s_empty[2], p_full[2], o_full[2];
   uint64_t turn[2][4];
   int e_k[kP8Slots], e_v[kP8Slots];
+  int pages[kP8Slots];                   // bits 0 to 3: the page is there; 4: all tokens of the tile are seen and are numbers
+  uint8_t bytes[kP8Slots][2][kP8Tile];   // scales of K and of V
   uint32_t tmem_base;
   int abort;
 };
@@ -99,7 +102,7 @@ struct PrefillQ8Smem {
   static constexpr int kP = 2 * kHalf;                    // weights [128][128]
   static constexpr int kStages = D == 64 ? 4 : 2;         // of the f16 ring, and of every warp's ring of pages
   static constexpr int kPageBytes = kQ8Page * D;
-  static constexpr int kBytes = 2 * kTile + kStages * (kTile + 4 * kPageBytes) + 2 * kP + int(sizeof(PrefillQ8Ctrl)) + 1024;
+  static constexpr int kBytes = 2 * kTile + kStages * (kTile + 4 * kPageBytes) + 2 * kP + int(sizeof(PrefillQ8Ctrl));
   static_assert(kBytes <= 232448, "shared memory of a CTA");
 };
 
@@ -140,21 +143,28 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
   const bool two = tr1.rows > 0;
   const int u_lo = tr0.lo, u_hi = two ? max(tr0.hi, tr1.hi) : tr0.hi, n_union = u_hi - u_lo;
 
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* q_s = smem;
+  extern __shared__ __align__(1024) uint8_t p8_smem[];    // the swizzle wants it on 1024 bytes, and there is no static memory ahead of it
+  uint8_t* q_s = p8_smem;
   uint8_t* kv_s = q_s + 2 * L::kTile;
   uint8_t* raw_s = kv_s + kStages * L::kTile;
   uint8_t* p_s = raw_s + kStages * 4 * L::kPageBytes;
   PrefillQ8Ctrl* ctrl = reinterpret_cast<PrefillQ8Ctrl*>(p_s + 2 * L::kP);
   const int warp = warp_idx_uniform(), lane = threadIdx.x & 31;
+  if (smem_u32(p8_smem) & 1023) {
+    if (threadIdx.x == 0) atomicCAS(p.status, 0, ERR_BAD_ARGUMENT);
+    return;
+  }
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
-      for (int w = 0; w < 4; ++w) mbar_init(&ctrl->raw_full[i][w], 1);
+      mbar_init(&ctrl->raw_full[i], 4);                   // one arrival for each page
+      mbar_init(&ctrl->raw_empty[i], 4);                  // one from each converting warp, as below
       mbar_init(&ctrl->kv_full[i], 4);                    // one arrival from each converting warp
       mbar_init(&ctrl->kv_empty[i], two ? 2 : 1);         // one from each query tile's issuer
     }
-    for (int i = 0; i < kP8Slots; ++i) mbar_init(&ctrl->e_full[i], 1);
+    for (int i = 0; i < kP8Slots; ++i) {
+      mbar_init(&ctrl->e_full[i], 1);
+      mbar_init(&ctrl->e_empty[i], 4);
+    }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ctrl->q_full[i], 4);
       mbar_init(&ctrl->s_full[i], 1);
@@ -176,6 +186,18 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
   tc_fence_after();
   const uint32_t tmem_base = __shfl_sync(kAll, ctrl->tmem_base, 0);
   volatile int* abort_flag = &ctrl->abort;
+  // Ring items in the order the issuers take them: K(0), then K(u + 1), V(u)
+  const int items = 2 * n_union;
+  const auto is_v = [&](int i) { return i > 0 && ((i & 1) == 0 || i == items - 1); };
+  const auto tile_of = [&](int i) { return i == 0 ? 0 : ((i & 1) == 0 ? i / 2 - 1 : min((i + 1) / 2, n_union - 1)); };
+  // tokens that some row sees
+  const int vis_lo = nkb_first_visible(ctx - q_len + qt * 2 * kP8Tile / p.group, p.window, p.chunk);
+  const int vis_hi = p.causal ? min(ctx, ctx - q_len + (min((qt + 1) * 2 * kP8Tile, all_rows) - 1) / p.group + 1) : ctx;
+  const auto block_at = [&](int x, int page_of_tile) {    // block of a page of walk position x; -1: none
+    const int page = (u_lo + x) * 4 + page_of_tile;
+    const int blk = x < n_union && page * kQ8Page < ctx ? p.block_table[b * p.table_stride + page] : -1;
+    return blk >= 0 && blk < p.num_blocks ? blk : -1;
+  };
 
   if (warp < 4) {
     // ---------------------------------------------------------------- conversion
@@ -183,165 +205,147 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
     constexpr int kRows = 512 / D, kSteps = kQ8Page / kRows;       // tokens per sixteen-byte load of the warp, loads per page
     constexpr int kLanes = D / 16;                                 // lanes that share a token
     const int piece = lane % kLanes, row_of = lane / kLanes;
-    const int* table = p.block_table + b * p.table_stride;
-    // tokens that some row sees
-    const int first = ctx - q_len + qt * 2 * kP8Tile / p.group;
-    const int vis_lo = nkb_first_visible(first, p.window, p.chunk);
-    const int vis_hi = p.causal ? min(ctx, ctx - q_len + (min((qt + 1) * 2 * kP8Tile, all_rows) - 1) / p.group + 1) : ctx;
-    auto block_at = [&](int x, int page_of_tile) {                 // block of a page of walk position x; -1: none
-      const int page = (u_lo + x) * 4 + page_of_tile;
-      const int blk = x < n_union && page * kQ8Page < ctx ? table[page] : -1;
-      return blk >= 0 && blk < p.num_blocks ? blk : -1;
-    };
-    auto scales_of = [&](const uint8_t* at, int blk) {             // scale bytes of tokens 4 lane .. 4 lane + 3 of the tile
-      return blk >= 0 ? *reinterpret_cast<const uint32_t*>(at + ((long long)blk * p.nkv + kvh) * kQ8Page + (lane & 7) * 4) : 0x7f7f7f7fu;
-    };
-    // Items in the order the issuers take them: K(0), then K(u + 1), V(u).  This warp's blocks of 32 tiles at a time, lane by lane, and of
-    // the 32 behind them.
-    const int items = 2 * n_union;
-    int base = 0, blks = block_at(lane, warp), blks_n = block_at(32 + lane, warp);
-    auto my_block = [&](int x) { return __shfl_sync(kAll, x - base < 32 ? blks : blks_n, x & 31); };
-    auto is_v = [&](int i) { return i > 0 && ((i & 1) == 0 || i == items - 1); };
-    auto tile_of = [&](int i) { return i == 0 ? 0 : ((i & 1) == 0 ? i / 2 - 1 : min((i + 1) / 2, n_union - 1)); };
-    uint8_t* my_raw = raw_s + warp * L::kPageBytes;
-    auto fetch = [&](int i) {
-      if (i >= items) return;
-      const int blk = my_block(tile_of(i)), st = i % kStages;
-      if (lane == 0) {
-        uint64_t* bar = &ctrl->raw_full[st][warp];
-        if (blk >= 0) {
-          mbar_expect_tx(bar, L::kPageBytes);
-          bulk_load_1d(my_raw + st * 4 * L::kPageBytes, (is_v(i) ? p.v_values : p.k_values) + ((long long)blk * p.nkv + kvh) * L::kPageBytes,
-                       L::kPageBytes, bar);
-        } else {
-          mbar_arrive(bar);
-        }
-      }
-    };
-#pragma unroll 1
-    for (int i = 0; i < kStages; ++i) fetch(i);
-    int blk_k = block_at(0, lane >> 3), blk_kn = block_at(1, lane >> 3);                     // of the tile at hand and of the next
-    uint32_t kb = scales_of(p.k_scales, blk_k), vb = scales_of(p.v_scales, blk_k);
-    uint32_t kb_n = scales_of(p.k_scales, blk_kn), vb_n = scales_of(p.v_scales, blk_kn);
-    uint32_t v_fac = 0, v_fac_n = 0;                               // factors of token `lane` of this warp's page of V
-    // where the lane's two chunks of a row go: where eight lanes have one row (D = 128), those of its second half store the odd chunk first,
-    // so that all banks are used
+    // where the lane's two chunks of a row go: where eight lanes have one row (D = 128), those of its second half take their eight-byte halves
+    // the other way round, so that all banks are used
     const int odd = NH == 2 ? piece >> 2 : 0;
     const uint32_t to0 = smem_u32(kv_s) + (piece >> 2) * kHalf + (warp * kQ8Page + row_of) * 128 + ((((piece & 3) * 2 + odd) ^ row_of) << 4);
-    bool live = true;
-    auto convert = [&](int i, uint32_t fac, bool whole) {
-      const int st = i % kStages, x = tile_of(i);
+    const uint8_t* from0 = raw_s + warp * L::kPageBytes + lane * 16 + odd * 8;
+#pragma unroll 1
+    for (int i = 0; i < items; ++i) {
+      const bool v_item = is_v(i);
+      const int st = i % kStages, x = tile_of(i), slot = x % kP8Slots;
       const uint32_t ph = uint32_t(i / kStages) & 1u;
-      bool ok = p8_wait(&ctrl->raw_full[st][warp], ph, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
+      bool ok = v_item || p8_wait(&ctrl->e_full[slot], uint32_t(x / kP8Slots) & 1u, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
+      ok = ok && p8_wait(&ctrl->raw_full[st], ph, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
       ok = ok && p8_wait(&ctrl->kv_empty[st], ph ^ 1u, abort_flag, p.status, ERR_WAIT_SMEM_EMPTY);
-      if (!__all_sync(kAll, ok)) {
-        live = false;
-        return;
+      if (!__all_sync(kAll, ok)) break;
+      // factor of token `lane` of the page
+      const int pages = ctrl->pages[slot], byte = ctrl->bytes[slot][v_item][warp * kQ8Page + lane];
+      const bool whole = pages & 16;
+      uint32_t fac = f16x2_pow2(q8_log2_of(byte) - (v_item ? ctrl->e_v[slot] : ctrl->e_k[slot]) + int(kP8Lift));
+      const int tok0 = (u_lo + x) * kP8Tile + warp * kQ8Page;
+      if (!whole) {
+        // NaN, K's or V's, is one of the scores: a row that does not see the token must not meet it in a product
+        const bool none = byte == 255 || ctrl->bytes[slot][!v_item][warp * kQ8Page + lane] == 255;
+        if (none) fac = v_item ? 0u : 0x7fff7fffu;
+        if (tok0 + lane < vis_lo || tok0 + lane >= vis_hi) fac = 0u;
       }
-      const int tok = (u_lo + x) * kP8Tile + warp * kQ8Page + row_of, lo = vis_lo - tok, hi = my_block(x) >= 0 ? vis_hi - tok : -kQ8Page;
-      const uint8_t* from = my_raw + st * 4 * L::kPageBytes + lane * 16;
+      const int lo = vis_lo - tok0 - row_of, hi = (pages >> warp) & 1 ? vis_hi - tok0 - row_of : -kQ8Page;
+      const uint8_t* from = from0 + st * 4 * L::kPageBytes;
       const uint32_t to = to0 + st * L::kTile;
       // four loads at a time, then their stores (a load behind a store would wait for it)
       constexpr int kAhead = 4;
 #pragma unroll
       for (int j0 = 0; j0 < kSteps; j0 += kAhead) {
-        uint4 raw[kAhead];
+        uint2 ra[kAhead], rc[kAhead];
         uint32_t f[kAhead];
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) raw[j] = *reinterpret_cast<const uint4*>(from + (j0 + j) * 512);
+        for (int j = 0; j < kAhead; ++j) {
+          const uint8_t* at = from + (j0 + j) * 512;
+          ra[j] = *reinterpret_cast<const uint2*>(at);
+          rc[j] = *reinterpret_cast<const uint2*>(odd ? at - 8 : at + 8);
+        }
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) f[j] = __shfl_sync(kAll, fac, (j0 + j) * kRows + row_of);
         if (!whole) {                                              // what no row sees may be anything
 #pragma unroll
           for (int j = 0; j < kAhead; ++j)
-            if ((j0 + j) * kRows < lo || (j0 + j) * kRows >= hi) raw[j] = make_uint4(0u, 0u, 0u, 0u);
+            if ((j0 + j) * kRows < lo || (j0 + j) * kRows >= hi) ra[j] = rc[j] = make_uint2(0u, 0u);
         }
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
-          const uint4 v = raw[j];
-          const uint4 a = make_uint4(hmul2(e4m3x2_to_f16x2(uint16_t(v.x)), f[j]), hmul2(e4m3x2_to_f16x2(uint16_t(v.x >> 16)), f[j]),
-                                     hmul2(e4m3x2_to_f16x2(uint16_t(v.y)), f[j]), hmul2(e4m3x2_to_f16x2(uint16_t(v.y >> 16)), f[j]));
-          const uint4 c = make_uint4(hmul2(e4m3x2_to_f16x2(uint16_t(v.z)), f[j]), hmul2(e4m3x2_to_f16x2(uint16_t(v.z >> 16)), f[j]),
-                                     hmul2(e4m3x2_to_f16x2(uint16_t(v.w)), f[j]), hmul2(e4m3x2_to_f16x2(uint16_t(v.w >> 16)), f[j]));
+          const uint4 a = make_uint4(hmul2(e4m3x2_to_f16x2(uint16_t(ra[j].x)), f[j]), hmul2(e4m3x2_to_f16x2(uint16_t(ra[j].x >> 16)), f[j]),
+                                     hmul2(e4m3x2_to_f16x2(uint16_t(ra[j].y)), f[j]), hmul2(e4m3x2_to_f16x2(uint16_t(ra[j].y >> 16)), f[j]));
+          const uint4 c = make_uint4(hmul2(e4m3x2_to_f16x2(uint16_t(rc[j].x)), f[j]), hmul2(e4m3x2_to_f16x2(uint16_t(rc[j].x >> 16)), f[j]),
+                                     hmul2(e4m3x2_to_f16x2(uint16_t(rc[j].y)), f[j]), hmul2(e4m3x2_to_f16x2(uint16_t(rc[j].y >> 16)), f[j]));
           // rows four on: bit 2 of the swizzle
           const uint32_t at = (to ^ (kRows == 4 && (j & 1) ? 64u : 0u)) + (j0 + j) * kRows * 128;
-          st_shared_16(at, odd ? c : a);
-          st_shared_16(at ^ 16u, odd ? a : c);
+          st_shared_16(at, a);
+          st_shared_16(at ^ 16u, c);
         }
       }
       fence_proxy_async();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ctrl->kv_full[st]);
-      fetch(i + kStages);
-    };
-    // a K tile: exponents of the tile, factors of this warp's tokens of K and (for later) V
-    bool whole = false, whole_n = false;                           // all tokens of the V tile at hand, and of the next, are seen and are numbers
-    auto do_k = [&](int i, int x) {
-      const int tile0 = (u_lo + x) * kP8Tile;
-      // a byte is between 63 and 191 where it is a scale: bits 6 and 7 both set are a NaN
-      const bool odd_one = ((kb & (kb << 1)) | (vb & (vb << 1))) & 0x80808080u;
-      whole_n = tile0 >= vis_lo && tile0 + kP8Tile <= vis_hi && !__any_sync(kAll, odd_one || blk_k < 0);
-      uint32_t k4 = kb, v4 = vb;
-      if (!whole_n) {
+      if (lane == 0) {
+        mbar_arrive(&ctrl->kv_full[st]);
+        mbar_arrive(&ctrl->raw_empty[st]);
+        if (v_item) mbar_arrive(&ctrl->e_empty[slot]);
+      }
+    }
+  } else if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 15) {
+      // -------------------------------------------------------------- pages: lanes 0 to 3 a page of the item each
+      int blk = lane < 4 ? block_at(0, lane) : -1;
+#pragma unroll 1
+      for (int i = 0; i < items; ++i) {
+        const int st = i % kStages;
+        const int next = i + 1 < items && lane < 4 ? block_at(tile_of(i + 1), lane) : -1;
+        const bool ok = p8_wait(&ctrl->raw_empty[st], (uint32_t(i / kStages) & 1u) ^ 1u, abort_flag, p.status, ERR_WAIT_SMEM_EMPTY);
+        if (!__all_sync(kAll, ok)) break;
+        if (lane < 4) {
+          uint64_t* bar = &ctrl->raw_full[st];
+          if (blk >= 0) {
+            mbar_expect_tx(bar, L::kPageBytes);
+            bulk_load_1d(raw_s + (st * 4 + lane) * L::kPageBytes,
+                         (is_v(i) ? p.v_values : p.k_values) + ((long long)blk * p.nkv + kvh) * L::kPageBytes, L::kPageBytes, bar);
+          } else {
+            mbar_arrive(bar);
+          }
+        }
+        __syncwarp();
+        blk = next;
+      }
+    } else if (warp == 14) {
+      // -------------------------------------------------------------- scales: a lane has tokens 4 lane .. 4 lane + 3 of a tile
+      auto scales_of = [&](const uint8_t* at, int blk) {
+        return blk >= 0 ? *reinterpret_cast<const uint32_t*>(at + ((long long)blk * p.nkv + kvh) * kQ8Page + (lane & 7) * 4) : 0x7f7f7f7fu;
+      };
+      int blk = block_at(0, lane >> 3), blk_n = block_at(1, lane >> 3);
+      uint32_t kb = scales_of(p.k_scales, blk), vb = scales_of(p.v_scales, blk);
+#pragma unroll 1
+      for (int x = 0; x < n_union; ++x) {
+        const uint32_t kb_n = scales_of(p.k_scales, blk_n), vb_n = scales_of(p.v_scales, blk_n);
+        const int blk_2 = block_at(x + 2, lane >> 3), slot = x % kP8Slots, tile0 = (u_lo + x) * kP8Tile;
+        // Tile x - 8 had this slot.  Its V, and with it the softmax of the tile, is behind the V of tile x - 4, which is converted after
+        // V(x - 6) has been used.
+        if (x >= kP8Lead) {
+          const bool ok = p8_wait(&ctrl->e_empty[(x - kP8Lead) % kP8Slots], uint32_t((x - kP8Lead) / kP8Slots) & 1u, abort_flag, p.status,
+                                  ERR_WAIT_SMEM_EMPTY);
+          if (!__all_sync(kAll, ok)) break;
+        }
+        uint32_t k4 = kb, v4 = vb;
+        bool all = blk >= 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int tok = tile0 + lane * 4 + j;
           if (tok >= vis_hi || tok < vis_lo || ((kb >> (8 * j)) & 255) == 255 || ((vb >> (8 * j)) & 255) == 255) {
-            k4 &= ~(255u << (8 * j));
+            k4 &= ~(255u << (8 * j));                     // such a token has no say in the tile's scale
             v4 &= ~(255u << (8 * j));
+            all = false;
           }
         }
-      }
-      const uint32_t k2 = __vmaxu2(k4 & 0x00ff00ffu, (k4 >> 8) & 0x00ff00ffu), v2 = __vmaxu2(v4 & 0x00ff00ffu, (v4 >> 8) & 0x00ff00ffu);
-      const int ek = q8_log2_of(int(__reduce_max_sync(kAll, max(k2 & 0xffffu, k2 >> 16))));
-      const int ev = q8_log2_of(int(__reduce_max_sync(kAll, max(v2 & 0xffffu, v2 >> 16))));
-      const int at = warp * 8 + (lane >> 2), sh = 8 * (lane & 3);
-      const int k = (__shfl_sync(kAll, kb, at) >> sh) & 255, v = (__shfl_sync(kAll, vb, at) >> sh) & 255;
-      uint32_t fac = f16x2_pow2(q8_log2_of(k) - ek + int(kP8Lift));
-      v_fac_n = f16x2_pow2(q8_log2_of(v) - ev + int(kP8Lift));
-      if (!whole_n) {
-        const int tok = tile0 + warp * kQ8Page + lane;
-        const bool seen = tok < vis_hi && tok >= vis_lo, none = k == 255 || v == 255;    // none: the row stands for NaN, its scores too
-        fac = !seen ? 0u : (none ? 0x7fff7fffu : fac);
-        v_fac_n = !seen || none ? 0u : v_fac_n;
-      }
-      if (warp == 0 && lane == 0) {
-        ctrl->e_k[x % kP8Slots] = ek;
-        ctrl->e_v[x % kP8Slots] = ev;
-        mbar_arrive(&ctrl->e_full[x % kP8Slots]);
-      }
-      convert(i, fac, whole_n);
-    };
-    if (n_union > 0) {
-      do_k(0, 0);
-      v_fac = v_fac_n;
-      whole = whole_n;
-    }
-#pragma unroll 1
-    for (int u = 0; u < n_union && live; ++u) {
-      if (u == base + 32) {
-        base += 32;
-        blks = blks_n;
-        blks_n = block_at(base + 32 + lane, warp);
-      }
-      if (u + 1 < n_union) {
-        const int blk_2 = block_at(u + 2, lane >> 3);
+        const uint32_t k2 = __vmaxu2(k4 & 0x00ff00ffu, (k4 >> 8) & 0x00ff00ffu), v2 = __vmaxu2(v4 & 0x00ff00ffu, (v4 >> 8) & 0x00ff00ffu);
+        const int ek = q8_log2_of(int(__reduce_max_sync(kAll, max(k2 & 0xffffu, k2 >> 16))));
+        const int ev = q8_log2_of(int(__reduce_max_sync(kAll, max(v2 & 0xffffu, v2 >> 16))));
+        const uint32_t there = __ballot_sync(kAll, blk >= 0);
+        const bool whole = __all_sync(kAll, all);
+        *reinterpret_cast<uint32_t*>(&ctrl->bytes[slot][0][lane * 4]) = kb;
+        *reinterpret_cast<uint32_t*>(&ctrl->bytes[slot][1][lane * 4]) = vb;
+        if (lane == 0) {
+          ctrl->e_k[slot] = ek;
+          ctrl->e_v[slot] = ev;
+          ctrl->pages[slot] = int((there & 1) | ((there >> 7) & 2) | ((there >> 14) & 4) | ((there >> 21) & 8)) | (whole ? 16 : 0);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctrl->e_full[slot]);
         kb = kb_n;
         vb = vb_n;
-        blk_k = blk_kn;
-        do_k(2 * u + 1, u + 1);
-        if (!live) break;
-        blk_kn = blk_2;
-        kb_n = scales_of(p.k_scales, blk_2);
-        vb_n = scales_of(p.v_scales, blk_2);
+        blk = blk_n;
+        blk_n = blk_2;
       }
-      convert(u + 1 < n_union ? 2 * u + 2 : 2 * u + 1, v_fac, whole);
-      v_fac = v_fac_n;
-      whole = whole_n;
     }
-  } else if (warp >= 12) {
     // ---------------------------------------------------------------- MMA issuers, one per query tile (see attn_prefill.cu)
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     constexpr uint32_t idesc_qk = p8_idesc(128, kP8Tile, 0), idesc_pv = p8_idesc(128, D, 1);
     const int t = warp - 12;
     if (t < 2 && (t == 0 || two) && elect_one()) {
