@@ -160,7 +160,8 @@ int nkb_q8_append(const void* qkv_bf16, const float* qkv_partials, int splits, l
 int nkb_q8_attn_prefill(const void* q, const void* k_values, const void* k_scales, const void* v_values, const void* v_scales,
                        const int* block_table, const int* q_start, const int* q_lens, const int* context_lens, void* out, int batch,
                        int total_q, int max_q_len, int nq, int nkv, int head_dim, int num_blocks, int table_width, long long table_stride,
-                       float scale, int causal, int window, int chunk, const float* sinks, void* stream);
+                       float scale, int causal, int window, int chunk, const float* sinks,
+                       unsigned int* sched, void* stream);
 long long nkb_q8_attn_decode_scratch_floats(int batch, int nkv, int head_dim, int group, int num_splits);
 int nkb_q8_attn_decode(const void* q, const void* k_values, const void* k_scales, const void* v_values, const void* v_scales,
                        const int* block_table, const int* context_lens, void* out, float* scratch, int batch, int q_len, int nq, int nkv,

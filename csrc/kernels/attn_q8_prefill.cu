@@ -26,6 +26,7 @@
 #include "kv_quant.cuh"
 #include "attn_maps.h"
 #include <cuda_fp16.h>
+#include <limits.h>
 #include <math.h>
 
 namespace nkb {
@@ -45,17 +46,35 @@ struct PrefillQ8Params {
   __nv_bfloat16* out;
   const float* sinks;
   int* status;
-  int total_q, nq, nkv, group, num_blocks, table_width, causal, window, chunk;
+  int batch, total_q, nq, nkv, group, num_blocks, table_width, causal, window, chunk;
+  int q_blocks;                          // 256-row blocks of the longest sequence
   long long table_stride;
   float scale_log2;
+  unsigned int* sched;                   // [0] works taken, [1] CTAs done; zero between calls
 };
+
+// Piece of work of a CTA: 256 rows of a sequence's kv head
+struct P8Range {                         // tiles [lo, hi) that a query tile attends to, and its rows
+  int lo, hi, rows;
+};
+struct P8Work {
+  int b, kvh, q_len, ctx, row0;          // b < 0: none
+  int u_lo, n_union;                     // tiles that either query tile attends to
+  P8Range tr0, tr1;
+  // tiles whose exponentials the two take turns with
+  __device__ __forceinline__ int paired() const { return tr1.rows > 0 ? min(tr0.hi - tr0.lo, tr1.hi - tr1.lo) : 0; }
+};
+constexpr int kP8Works = 3;              // works ahead of their use
+constexpr int kP8Readers = 15;           // warps 0 to 14 read them
 
 struct PrefillQ8Ctrl {
   uint64_t q_full[2];
   uint64_t raw_full[4], raw_empty[4], kv_full[4], kv_empty[4];
   uint64_t e_full[kP8Slots], e_empty[kP8Slots];
-  uint64_t s_full[2], s_empty[2], p_full[2], o_full[2];
+  uint64_t s_full[2], s_empty[2], p_full[2], o_full[2], o_empty[2];
   uint64_t turn[2][4];
+  uint64_t w_full[kP8Works], w_empty[kP8Works];
+  P8Work works[kP8Works];
   int e_k[kP8Slots], e_v[kP8Slots];
   int pages[kP8Slots];                   // bits 0 to 3: the page is there; 4: all tokens of the tile are seen and are numbers
   uint8_t bytes[kP8Slots][2][kP8Tile];   // scales of K and of V
@@ -78,10 +97,6 @@ __device__ __forceinline__ bool p8_wait(uint64_t* bar, uint32_t parity, volatile
   return true;
 }
 
-// Tiles [lo, hi) that a query tile attends to, and its rows
-struct P8Range {
-  int lo, hi, rows;
-};
 __device__ __forceinline__ P8Range p8_range(const PrefillQ8Params& p, int row0, int all_rows, int q_len, int ctx) {
   P8Range r{0, 0, 0};
   if (row0 >= all_rows) return r;
@@ -93,6 +108,47 @@ __device__ __forceinline__ P8Range p8_range(const PrefillQ8Params& p, int row0, 
   if (r.hi < r.lo) r.hi = r.lo;
   return r;
 }
+// Rows row0 .. of sequence b and kv head kvh; false: there are none
+__device__ __forceinline__ bool p8_work(const PrefillQ8Params& p, int b, int kvh, int row0, P8Work& o) {
+  o.b = b;
+  o.kvh = kvh;
+  o.row0 = row0;
+  o.q_len = p.q_lens[b];
+  o.ctx = min(p.context_lens[b], p.table_width * kQ8Page);
+  if (row0 >= (long long)o.q_len * p.group) return false;
+  const int all_rows = o.q_len * p.group;
+  o.tr0 = p8_range(p, row0, all_rows, o.q_len, o.ctx);
+  o.tr1 = p8_range(p, row0 + kP8Tile, all_rows, o.q_len, o.ctx);
+  o.u_lo = o.tr0.lo;
+  o.n_union = (o.tr1.rows > 0 ? max(o.tr0.hi, o.tr1.hi) : o.tr0.hi) - o.u_lo;
+  return true;
+}
+// The next work for a warp or (one = true) a single thread; n counts them.  False: there are no more, or the wait has run out.
+__device__ __forceinline__ bool p8_next(PrefillQ8Ctrl* ctrl, uint32_t& n, P8Work& k, bool one, int* status) {
+  const uint32_t slot = n % kP8Works;
+  bool ok = p8_wait(&ctrl->w_full[slot], n / kP8Works & 1u, &ctrl->abort, status, ERR_WAIT_SMEM_FULL);
+  if (!one) ok = __all_sync(0xffffffffu, ok);
+  if (!ok) return false;
+  k = ctrl->works[slot];
+  ++n;
+  if (!one) __syncwarp();
+  if (one || (threadIdx.x & 31) == 0) mbar_arrive(&ctrl->w_empty[slot]);
+  return k.b >= 0;
+}
+// Tokens [lo, hi) that some row of the work sees
+__device__ __forceinline__ void p8_seen(const PrefillQ8Params& p, const P8Work& k, int& lo, int& hi) {
+  lo = nkb_first_visible(k.ctx - k.q_len + k.row0 / p.group, p.window, p.chunk);
+  hi = p.causal ? min(k.ctx, k.ctx - k.q_len + (min(k.row0 + 2 * kP8Tile, k.q_len * p.group) - 1) / p.group + 1) : k.ctx;
+}
+// Block of a page of walk position x; -1: none
+__device__ __forceinline__ int p8_block(const PrefillQ8Params& p, const P8Work& k, int x, int page_of_tile) {
+  const int page = (k.u_lo + x) * 4 + page_of_tile;
+  const int blk = x < k.n_union && page * kQ8Page < k.ctx ? p.block_table[k.b * p.table_stride + page] : -1;
+  return blk >= 0 && blk < p.num_blocks ? blk : -1;
+}
+// Ring items of a work in the order the issuers take them: K(0), then K(u + 1), V(u)
+__device__ __forceinline__ bool p8_is_v(int i, int items) { return i > 0 && ((i & 1) == 0 || i == items - 1); }
+__device__ __forceinline__ int p8_tile(int i, int items) { return i == 0 ? 0 : ((i & 1) == 0 ? i / 2 - 1 : min((i + 1) / 2, items / 2 - 1)); }
 
 template <int D>
 struct PrefillQ8Smem {
@@ -133,16 +189,6 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
   using L = PrefillQ8Smem<D>;
   constexpr int NH = L::NH, kHalf = L::kHalf, kStages = L::kStages;
   constexpr uint32_t kAll = 0xffffffffu, kTmemCols = 512, kSCol = 0, kOCol = 256;
-  const int qt = gridDim.x - 1 - blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;      // the longest rows start first
-  griddep_wait();
-  griddep_launch();
-  const int q_len = p.q_lens[b], all_rows = q_len * p.group;
-  if (qt * 2 * kP8Tile >= all_rows) return;
-  const int ctx = min(p.context_lens[b], p.table_width * kQ8Page);
-  const P8Range tr0 = p8_range(p, qt * 2 * kP8Tile, all_rows, q_len, ctx), tr1 = p8_range(p, (qt * 2 + 1) * kP8Tile, all_rows, q_len, ctx);
-  const bool two = tr1.rows > 0;
-  const int u_lo = tr0.lo, u_hi = two ? max(tr0.hi, tr1.hi) : tr0.hi, n_union = u_hi - u_lo;
-
   extern __shared__ __align__(1024) uint8_t p8_smem[];    // the swizzle wants it on 1024 bytes, and there is no static memory ahead of it
   uint8_t* q_s = p8_smem;
   uint8_t* kv_s = q_s + 2 * L::kTile;
@@ -159,7 +205,11 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
       mbar_init(&ctrl->raw_full[i], 4);                   // one arrival for each page
       mbar_init(&ctrl->raw_empty[i], 4);                  // one from each converting warp, as below
       mbar_init(&ctrl->kv_full[i], 4);                    // one arrival from each converting warp
-      mbar_init(&ctrl->kv_empty[i], two ? 2 : 1);         // one from each query tile's issuer
+      mbar_init(&ctrl->kv_empty[i], 2);                   // one from each query tile's issuer
+    }
+    for (int i = 0; i < kP8Works; ++i) {
+      mbar_init(&ctrl->w_full[i], 1);
+      mbar_init(&ctrl->w_empty[i], kP8Readers);
     }
     for (int i = 0; i < kP8Slots; ++i) {
       mbar_init(&ctrl->e_full[i], 1);
@@ -171,6 +221,7 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
       mbar_init(&ctrl->s_empty[i], 4);
       mbar_init(&ctrl->p_full[i], 4);
       mbar_init(&ctrl->o_full[i], 1);
+      mbar_init(&ctrl->o_empty[i], 4);
       for (int q = 0; q < 4; ++q) mbar_init(&ctrl->turn[i][q], 1);
     }
     ctrl->abort = 0;
@@ -186,18 +237,8 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
   tc_fence_after();
   const uint32_t tmem_base = __shfl_sync(kAll, ctrl->tmem_base, 0);
   volatile int* abort_flag = &ctrl->abort;
-  // Ring items in the order the issuers take them: K(0), then K(u + 1), V(u)
-  const int items = 2 * n_union;
-  const auto is_v = [&](int i) { return i > 0 && ((i & 1) == 0 || i == items - 1); };
-  const auto tile_of = [&](int i) { return i == 0 ? 0 : ((i & 1) == 0 ? i / 2 - 1 : min((i + 1) / 2, n_union - 1)); };
-  // tokens that some row sees
-  const int vis_lo = nkb_first_visible(ctx - q_len + qt * 2 * kP8Tile / p.group, p.window, p.chunk);
-  const int vis_hi = p.causal ? min(ctx, ctx - q_len + (min((qt + 1) * 2 * kP8Tile, all_rows) - 1) / p.group + 1) : ctx;
-  const auto block_at = [&](int x, int page_of_tile) {    // block of a page of walk position x; -1: none
-    const int page = (u_lo + x) * 4 + page_of_tile;
-    const int blk = x < n_union && page * kQ8Page < ctx ? p.block_table[b * p.table_stride + page] : -1;
-    return blk >= 0 && blk < p.num_blocks ? blk : -1;
-  };
+  griddep_wait();
+  griddep_launch();
 
   if (warp < 4) {
     // ---------------------------------------------------------------- conversion
@@ -210,20 +251,32 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
     const int odd = NH == 2 ? piece >> 2 : 0;
     const uint32_t to0 = smem_u32(kv_s) + (piece >> 2) * kHalf + (warp * kQ8Page + row_of) * 128 + ((((piece & 3) * 2 + odd) ^ row_of) << 4);
     const uint8_t* from0 = raw_s + warp * L::kPageBytes + lane * 16 + odd * 8;
+    uint32_t item0 = 0, tiles0 = 0;                                // ring items and tiles of the works before
+    uint32_t n_works = 0;
+    bool alive = true;
+    P8Work k;
+#pragma unroll 1
+    while (alive && p8_next(ctrl, n_works, k, false, p.status)) {
+    int vis_lo, vis_hi;
+    p8_seen(p, k, vis_lo, vis_hi);
+    const int items = 2 * k.n_union;
 #pragma unroll 1
     for (int i = 0; i < items; ++i) {
-      const bool v_item = is_v(i);
-      const int st = i % kStages, x = tile_of(i), slot = x % kP8Slots;
-      const uint32_t ph = uint32_t(i / kStages) & 1u;
-      bool ok = v_item || p8_wait(&ctrl->e_full[slot], uint32_t(x / kP8Slots) & 1u, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
+      const bool v_item = p8_is_v(i, items);
+      const int x = p8_tile(i, items), st = (item0 + i) % kStages, slot = (tiles0 + x) % kP8Slots;
+      const uint32_t ph = (item0 + i) / kStages & 1u;
+      bool ok = v_item || p8_wait(&ctrl->e_full[slot], (tiles0 + x) / kP8Slots & 1u, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
       ok = ok && p8_wait(&ctrl->raw_full[st], ph, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
       ok = ok && p8_wait(&ctrl->kv_empty[st], ph ^ 1u, abort_flag, p.status, ERR_WAIT_SMEM_EMPTY);
-      if (!__all_sync(kAll, ok)) break;
+      if (!__all_sync(kAll, ok)) {
+        alive = false;
+        break;
+      }
       // factor of token `lane` of the page
       const int pages = ctrl->pages[slot], byte = ctrl->bytes[slot][v_item][warp * kQ8Page + lane];
       const bool whole = pages & 16;
       uint32_t fac = f16x2_pow2(q8_log2_of(byte) - (v_item ? ctrl->e_v[slot] : ctrl->e_k[slot]) + int(kP8Lift));
-      const int tok0 = (u_lo + x) * kP8Tile + warp * kQ8Page;
+      const int tok0 = (k.u_lo + x) * kP8Tile + warp * kQ8Page;
       if (!whole) {
         // NaN, K's or V's, is one of the scores: a row that does not see the token must not meet it in a product
         const bool none = byte == 255 || ctrl->bytes[slot][!v_item][warp * kQ8Page + lane] == 255;
@@ -272,100 +325,165 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
         if (v_item) mbar_arrive(&ctrl->e_empty[slot]);
       }
     }
+    item0 += items;
+    tiles0 += k.n_union;
+    }
   } else if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 15) {
       // -------------------------------------------------------------- pages: lanes 0 to 3 a page of the item each
-      int blk = lane < 4 ? block_at(0, lane) : -1;
+      // and the works, taken from a counter of the grid: the last rows of all sequences first, those with the longest contexts ahead
+      const int across = p.nkv * p.batch;
+      int order = lane;                                   // (up to 32 sequences) the sequence of rank `lane`
+      if (p.batch <= 32) {
+        const int ctx = lane < p.batch ? p.context_lens[lane] : INT_MIN;
+        int rank = 0;
+        for (int j = 0; j < 32; ++j) {
+          const int c = __shfl_sync(kAll, ctx, j);
+          rank += c > ctx || (c == ctx && j < lane);
+        }
+        for (int j = 0; j < 32; ++j)
+          if (__shfl_sync(kAll, rank, j) == lane) order = j;
+      }
+      auto take = [&]() {
+        unsigned int w = 0;
+        if (lane == 0) w = atomicAdd(p.sched, 1u);
+        return w;
+      };
+      uint32_t item0 = 0, n_works = 0;
+      unsigned int taken = take();
+      bool alive = true;
+      P8Work k;
 #pragma unroll 1
-      for (int i = 0; i < items; ++i) {
-        const int st = i % kStages;
-        const int next = i + 1 < items && lane < 4 ? block_at(tile_of(i + 1), lane) : -1;
-        const bool ok = p8_wait(&ctrl->raw_empty[st], (uint32_t(i / kStages) & 1u) ^ 1u, abort_flag, p.status, ERR_WAIT_SMEM_EMPTY);
-        if (!__all_sync(kAll, ok)) break;
-        if (lane < 4) {
-          uint64_t* bar = &ctrl->raw_full[st];
-          if (blk >= 0) {
-            mbar_expect_tx(bar, L::kPageBytes);
-            bulk_load_1d(raw_s + (st * 4 + lane) * L::kPageBytes,
-                         (is_v(i) ? p.v_values : p.k_values) + ((long long)blk * p.nkv + kvh) * L::kPageBytes, L::kPageBytes, bar);
-          } else {
-            mbar_arrive(bar);
+      while (alive) {
+        const unsigned int w = __shfl_sync(kAll, taken, 0), level = w / across;
+        k.b = -1;
+        k.n_union = 0;
+        if (level < unsigned(p.q_blocks)) {
+          const int rest = int(w % across), b = rest / p.nkv;
+          if (!p8_work(p, p.batch <= 32 ? __shfl_sync(kAll, order, b & 31) : b, rest % p.nkv, (p.q_blocks - 1 - int(level)) * 2 * kP8Tile, k)) {
+            taken = take();
+            continue;
           }
         }
+        const bool free_slot = p8_wait(&ctrl->w_empty[n_works % kP8Works], (n_works / kP8Works & 1u) ^ 1u, abort_flag, p.status, ERR_WAIT_SMEM_EMPTY);
+        if (!__all_sync(kAll, free_slot)) break;
+        if (lane == 0) {
+          ctrl->works[n_works % kP8Works] = k;
+          mbar_arrive(&ctrl->w_full[n_works % kP8Works]);
+        }
         __syncwarp();
-        blk = next;
+        ++n_works;
+        if (k.b < 0) break;
+        const int items = 2 * k.n_union;
+        int blk = lane < 4 ? p8_block(p, k, 0, lane) : -1;
+#pragma unroll 1
+        for (int i = 0; i < items; ++i, ++item0) {
+          if (i == max(items - 3, 0)) taken = take();     // late, so that works go to who is free, and early enough to be there
+          const int st = item0 % kStages;
+          const int next = i + 1 < items && lane < 4 ? p8_block(p, k, p8_tile(i + 1, items), lane) : -1;
+          const bool ok = p8_wait(&ctrl->raw_empty[st], (item0 / kStages & 1u) ^ 1u, abort_flag, p.status, ERR_WAIT_SMEM_EMPTY);
+          if (!__all_sync(kAll, ok)) {
+            alive = false;
+            break;
+          }
+          if (lane < 4) {
+            uint64_t* bar = &ctrl->raw_full[st];
+            if (blk >= 0) {
+              mbar_expect_tx(bar, L::kPageBytes);
+              bulk_load_1d(raw_s + (st * 4 + lane) * L::kPageBytes,
+                           (p8_is_v(i, items) ? p.v_values : p.k_values) + ((long long)blk * p.nkv + k.kvh) * L::kPageBytes, L::kPageBytes, bar);
+            } else {
+              mbar_arrive(bar);
+            }
+          }
+          __syncwarp();
+          blk = next;
+        }
+        if (items == 0) taken = take();
       }
     } else if (warp == 14) {
       // -------------------------------------------------------------- scales: a lane has tokens 4 lane .. 4 lane + 3 of a tile
-      auto scales_of = [&](const uint8_t* at, int blk) {
-        return blk >= 0 ? *reinterpret_cast<const uint32_t*>(at + ((long long)blk * p.nkv + kvh) * kQ8Page + (lane & 7) * 4) : 0x7f7f7f7fu;
-      };
-      int blk = block_at(0, lane >> 3), blk_n = block_at(1, lane >> 3);
-      uint32_t kb = scales_of(p.k_scales, blk), vb = scales_of(p.v_scales, blk);
+      uint32_t tiles0 = 0, n_works = 0;
+      bool alive = true;
+      P8Work k;
 #pragma unroll 1
-      for (int x = 0; x < n_union; ++x) {
-        const uint32_t kb_n = scales_of(p.k_scales, blk_n), vb_n = scales_of(p.v_scales, blk_n);
-        const int blk_2 = block_at(x + 2, lane >> 3), slot = x % kP8Slots, tile0 = (u_lo + x) * kP8Tile;
-        // Tile x - 8 had this slot.  Its V, and with it the softmax of the tile, is behind the V of tile x - 4, which is converted after
-        // V(x - 6) has been used.
-        if (x >= kP8Lead) {
-          const bool ok = p8_wait(&ctrl->e_empty[(x - kP8Lead) % kP8Slots], uint32_t((x - kP8Lead) / kP8Slots) & 1u, abort_flag, p.status,
-                                  ERR_WAIT_SMEM_EMPTY);
-          if (!__all_sync(kAll, ok)) break;
-        }
-        uint32_t k4 = kb, v4 = vb;
-        bool all = blk >= 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int tok = tile0 + lane * 4 + j;
-          if (tok >= vis_hi || tok < vis_lo || ((kb >> (8 * j)) & 255) == 255 || ((vb >> (8 * j)) & 255) == 255) {
-            k4 &= ~(255u << (8 * j));                     // such a token has no say in the tile's scale
-            v4 &= ~(255u << (8 * j));
-            all = false;
+      while (alive && p8_next(ctrl, n_works, k, false, p.status)) {
+        auto scales_of = [&](const uint8_t* at, int blk) {
+          return blk >= 0 ? *reinterpret_cast<const uint32_t*>(at + ((long long)blk * p.nkv + k.kvh) * kQ8Page + (lane & 7) * 4) : 0x7f7f7f7fu;
+        };
+        int vis_lo, vis_hi;
+        p8_seen(p, k, vis_lo, vis_hi);
+        int blk = p8_block(p, k, 0, lane >> 3), blk_n = p8_block(p, k, 1, lane >> 3);
+        uint32_t kb = scales_of(p.k_scales, blk), vb = scales_of(p.v_scales, blk);
+#pragma unroll 1
+        for (int x = 0; x < k.n_union; ++x, ++tiles0) {
+          const uint32_t kb_n = scales_of(p.k_scales, blk_n), vb_n = scales_of(p.v_scales, blk_n);
+          const int blk_2 = p8_block(p, k, x + 2, lane >> 3), slot = tiles0 % kP8Slots, tile0 = (k.u_lo + x) * kP8Tile;
+          // The tile eight before had this slot.  Its V, and with it its softmax, is behind the V of four tiles before, which is converted
+          // after that of six before has been used.
+          if (tiles0 >= kP8Lead) {
+            const uint32_t past = tiles0 - kP8Lead;
+            const bool ok = p8_wait(&ctrl->e_empty[past % kP8Slots], past / kP8Slots & 1u, abort_flag, p.status, ERR_WAIT_SMEM_EMPTY);
+            if (!__all_sync(kAll, ok)) {
+              alive = false;
+              break;
+            }
           }
+          uint32_t k4 = kb, v4 = vb;
+          bool all = blk >= 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int tok = tile0 + lane * 4 + j;
+            if (tok >= vis_hi || tok < vis_lo || ((kb >> (8 * j)) & 255) == 255 || ((vb >> (8 * j)) & 255) == 255) {
+              k4 &= ~(255u << (8 * j));                   // such a token has no say in the tile's scale
+              v4 &= ~(255u << (8 * j));
+              all = false;
+            }
+          }
+          const uint32_t k2 = __vmaxu2(k4 & 0x00ff00ffu, (k4 >> 8) & 0x00ff00ffu), v2 = __vmaxu2(v4 & 0x00ff00ffu, (v4 >> 8) & 0x00ff00ffu);
+          const int ek = q8_log2_of(int(__reduce_max_sync(kAll, max(k2 & 0xffffu, k2 >> 16))));
+          const int ev = q8_log2_of(int(__reduce_max_sync(kAll, max(v2 & 0xffffu, v2 >> 16))));
+          const uint32_t there = __ballot_sync(kAll, blk >= 0);
+          const bool whole = __all_sync(kAll, all);
+          *reinterpret_cast<uint32_t*>(&ctrl->bytes[slot][0][lane * 4]) = kb;
+          *reinterpret_cast<uint32_t*>(&ctrl->bytes[slot][1][lane * 4]) = vb;
+          if (lane == 0) {
+            ctrl->e_k[slot] = ek;
+            ctrl->e_v[slot] = ev;
+            ctrl->pages[slot] = int((there & 1) | ((there >> 7) & 2) | ((there >> 14) & 4) | ((there >> 21) & 8)) | (whole ? 16 : 0);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctrl->e_full[slot]);
+          kb = kb_n;
+          vb = vb_n;
+          blk = blk_n;
+          blk_n = blk_2;
         }
-        const uint32_t k2 = __vmaxu2(k4 & 0x00ff00ffu, (k4 >> 8) & 0x00ff00ffu), v2 = __vmaxu2(v4 & 0x00ff00ffu, (v4 >> 8) & 0x00ff00ffu);
-        const int ek = q8_log2_of(int(__reduce_max_sync(kAll, max(k2 & 0xffffu, k2 >> 16))));
-        const int ev = q8_log2_of(int(__reduce_max_sync(kAll, max(v2 & 0xffffu, v2 >> 16))));
-        const uint32_t there = __ballot_sync(kAll, blk >= 0);
-        const bool whole = __all_sync(kAll, all);
-        *reinterpret_cast<uint32_t*>(&ctrl->bytes[slot][0][lane * 4]) = kb;
-        *reinterpret_cast<uint32_t*>(&ctrl->bytes[slot][1][lane * 4]) = vb;
-        if (lane == 0) {
-          ctrl->e_k[slot] = ek;
-          ctrl->e_v[slot] = ev;
-          ctrl->pages[slot] = int((there & 1) | ((there >> 7) & 2) | ((there >> 14) & 4) | ((there >> 21) & 8)) | (whole ? 16 : 0);
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ctrl->e_full[slot]);
-        kb = kb_n;
-        vb = vb_n;
-        blk = blk_n;
-        blk_n = blk_2;
       }
     }
     // ---------------------------------------------------------------- MMA issuers, one per query tile (see attn_prefill.cu)
     constexpr uint32_t idesc_qk = p8_idesc(128, kP8Tile, 0), idesc_pv = p8_idesc(128, D, 1);
     const int t = warp - 12;
-    if (t < 2 && (t == 0 || two) && elect_one()) {
-      const P8Range tr = t == 0 ? tr0 : tr1;
-      const int a_lo = tr.lo - u_lo, a_hi = tr.hi - u_lo;
+    if (t < 2 && elect_one()) {
       const uint32_t q_lo = uint32_t(make_smem_desc_sw128(smem_u32(q_s + t * L::kTile), 0, 1024));
       const uint32_t kv_lo = uint32_t(make_smem_desc_sw128(smem_u32(kv_s), 0, 1024));
       const uint32_t p_lo = uint32_t(make_smem_desc_sw128(smem_u32(p_s + t * L::kP), 0, 1024));
       const uint64_t hk = uint64_t(uint32_t(make_smem_desc_sw128(0, 0, 1024) >> 32)) << 32;
       const uint32_t lbo_v = (uint32_t(kHalf) >> 4) << 16;
       const uint32_t s_tmem = tmem_base + kSCol + t * 128, o_tmem = tmem_base + kOCol + t * 128;
-      bool ok = p8_wait(&ctrl->q_full[t], 0, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
-      int seq = 0;
+      bool ok = true;
+      uint32_t item = 0, tiles = 0;                       // ring items, and tiles that this query tile attended to
+      uint32_t results = 0;                               // works in which it had any
+      int a_lo = 0, a_hi = 0, n_union = 0;
       auto do_k = [&](int x) {
         if (x >= n_union || !ok) return;
-        const int item = seq++, st = item % kStages;
-        ok = p8_wait(&ctrl->kv_full[st], uint32_t(item / kStages) & 1u, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
+        const uint32_t st = item % kStages, ph = item / kStages & 1u;
+        ++item;
+        ok = p8_wait(&ctrl->kv_full[st], ph, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
         if (!ok) return;
         if (x >= a_lo && x < a_hi) {
-          ok = p8_wait(&ctrl->s_empty[t], (uint32_t(x - a_lo) & 1u) ^ 1u, abort_flag, p.status, ERR_WAIT_TMEM_EMPTY);
+          ok = p8_wait(&ctrl->s_empty[t], (tiles + uint32_t(x - a_lo) & 1u) ^ 1u, abort_flag, p.status, ERR_WAIT_TMEM_EMPTY);
           if (!ok) return;
           tc_fence_after();
           const uint32_t kvd = kv_lo + uint32_t(st * L::kTile >> 4);
@@ -385,11 +503,14 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
       };
       auto do_v = [&](int x) {
         if (!ok) return;
-        const int item = seq++, st = item % kStages;
-        ok = p8_wait(&ctrl->kv_full[st], uint32_t(item / kStages) & 1u, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
+        const uint32_t st = item % kStages, ph = item / kStages & 1u;
+        ++item;
+        ok = p8_wait(&ctrl->kv_full[st], ph, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
         if (!ok) return;
         if (x >= a_lo && x < a_hi) {
-          ok = p8_wait(&ctrl->p_full[t], uint32_t(x - a_lo) & 1u, abort_flag, p.status, ERR_WAIT_SOFTMAX);
+          // O_t of the work before has been read
+          if (x == a_lo) ok = p8_wait(&ctrl->o_empty[t], (results & 1u) ^ 1u, abort_flag, p.status, ERR_WAIT_TMEM_EMPTY);
+          ok = ok && p8_wait(&ctrl->p_full[t], tiles + uint32_t(x - a_lo) & 1u, abort_flag, p.status, ERR_WAIT_SOFTMAX);
           if (!ok) return;
           tc_fence_after();
           const uint32_t kvd = kv_lo + uint32_t(st * L::kTile >> 4);
@@ -407,73 +528,62 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
         }
         umma_commit(&ctrl->kv_empty[st]);
       };
-      do_k(0);
+      uint32_t n_works = 0;
+      P8Work k;
 #pragma unroll 1
-      for (int u = 0; u < n_union && ok; ++u) {
-        do_k(u + 1);
-        do_v(u);
+      while (ok && p8_next(ctrl, n_works, k, true, p.status)) {
+        const P8Range tr = t == 0 ? k.tr0 : k.tr1;
+        n_union = k.n_union;
+        a_lo = a_hi = 0;
+        if (tr.hi > tr.lo) {
+          a_lo = tr.lo - k.u_lo;
+          a_hi = tr.hi - k.u_lo;
+          ok = p8_wait(&ctrl->q_full[t], results & 1u, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
+        }
+        do_k(0);
+#pragma unroll 1
+        for (int u = 0; u < n_union && ok; ++u) {
+          do_k(u + 1);
+          do_v(u);
+        }
+        tiles += a_hi - a_lo;
+        results += a_hi > a_lo;
       }
     }
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- softmax, one thread per row
     asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
-    const int t = (warp - 4) >> 2, quad = warp & 3;
-    const P8Range tr = t == 0 ? tr0 : tr1;
-    const int r = quad * 32 + lane, row = (qt * 2 + t) * kP8Tile + r;      // row of (token, head) pairs
-    const int token = row / p.group, head = kvh * p.group + row % p.group;
-    const long long q_row = (long long)p.q_start[b] + token;
-    const bool mine = r < tr.rows && q_row >= 0 && q_row < p.total_q;
+    const int t = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane;
     const uint32_t lane_off = uint32_t(quad * 32) << 16;
     const uint32_t s_addr = tmem_base + lane_off + kSCol + t * 128, o_addr = tmem_base + lane_off + kOCol + t * 128;
     uint8_t* my_p = p_s + t * L::kP + r * 128;
-    float raw_log2 = 0.f;                                                  // raw score -> exponent of two, without 2^K
-    if (tr.rows > 0) {
-      uint4 v[D / 8];
-      const uint4* src = reinterpret_cast<const uint4*>(p.q + (q_row * p.nq + head) * D);
-      float mx = 0.f;
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) v[i] = mine ? src[i] : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = unpack_bf16x2(w[j]);
-          mx = fmax3(mx, fabsf(f.x), fabsf(f.y));
-        }
-      }
-      const int e = max((__float_as_int(mx) >> 23) - 127, -100);
-      const float up = exp2_int(14 - e);
-      raw_log2 = p.scale_log2 * exp2_int(e - 14);
-      uint8_t* dst = q_s + t * L::kTile + r * 128;
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-        uint32_t h[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = unpack_bf16x2(w[j]);
-          h[j] = p8_pack_f16x2(f.x * up, f.y * up);
-        }
-        *reinterpret_cast<uint4*>(dst + (i >> 3) * kHalf + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-      }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&ctrl->q_full[t]);
-    }
-    const int n_tiles = tr.hi - tr.lo, n_other = t == 0 ? (two ? tr1.hi - tr1.lo : 0) : tr0.hi - tr0.lo;
-    const int q_pos = ctx - q_len + token, hi_pos = p.causal ? min(ctx - 1, q_pos) : ctx - 1;
-    const int lo_pos = nkb_first_visible(q_pos, p.window, p.chunk);
-    float m = -INFINITY, l = 0.f;
-    bool alive = true;
+    // a row of a work: (token, head of the group)
+    struct Row {
+      int tile_lo, n_tiles, lo_pos, hi_pos, head, x0;     // x0: walk position of its first tile
+      int paired;                                         // tiles whose exponentials the two query tiles take turns with
+      long long at;                                       // row of q and out (of heads), < 0: none
+      float raw_log2;                                     // raw score -> exponent of two, without 2^K
+      uint32_t tiles0;                                    // tiles of the works before
+    };
+    Row cur{}, next{};
+    bool have = false, alive = true;
+    uint32_t tiles_seen = 0, done = 0, pairs = 0;         // tiles of all works; this query tile's; paired ones
+    uint32_t n_works = 0;
+    bool last = false;                                    // no more works
+#pragma unroll 1
+    while (true) {
+      float m = -INFINITY, l = 0.f;
+      if (have) {
+        const int n_tiles = cur.n_tiles, hi_pos = cur.hi_pos, lo_pos = cur.lo_pos;
     for (int it = 0; it < n_tiles; ++it) {
-      const int x = tr.lo - u_lo + it, kv0 = (tr.lo + it) * kP8Tile;
-      bool ok = p8_wait(&ctrl->e_full[x % kP8Slots], uint32_t(x / kP8Slots) & 1u, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
-      ok = ok && p8_wait(&ctrl->s_full[t], uint32_t(it) & 1u, abort_flag, p.status, ERR_WAIT_TMEM_FULL);
+      const uint32_t x = cur.tiles0 + cur.x0 + it;
+      const int kv0 = (cur.tile_lo + it) * kP8Tile;
+      bool ok = p8_wait(&ctrl->e_full[x % kP8Slots], x / kP8Slots & 1u, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
+      ok = ok && p8_wait(&ctrl->s_full[t], done + it & 1u, abort_flag, p.status, ERR_WAIT_TMEM_FULL);
       if (!__all_sync(kAll, ok)) { alive = false; break; }
       const int e_k = *(volatile int*)&ctrl->e_k[x % kP8Slots], e_v = *(volatile int*)&ctrl->e_v[x % kP8Slots];
-      const float to_log2 = raw_log2 * exp2_int(e_k - int(kP8Lift)), add = float(e_v);
+      const float to_log2 = cur.raw_log2 * exp2_int(e_k - int(kP8Lift)), add = float(e_v);
       tc_fence_after();
       uint32_t v[kP8Tile];
 #pragma unroll
@@ -501,7 +611,7 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
       } else {
         const bool grow = mx > m + kP8Grow;
         if (__any_sync(kAll, grow)) {
-          ok = p8_wait(&ctrl->o_full[t], uint32_t(it - 1) & 1u, abort_flag, p.status, ERR_WAIT_TMEM_FULL);
+          ok = p8_wait(&ctrl->o_full[t], done + it - 1 & 1u, abort_flag, p.status, ERR_WAIT_TMEM_FULL);
           if (!__all_sync(kAll, ok)) { alive = false; break; }
           p_free = true;
           tc_fence_after();
@@ -526,12 +636,12 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum2[i] = make_float2(0.f, 0.f);
       if (!p_free) {
-        ok = p8_wait(&ctrl->o_full[t], uint32_t(it - 1) & 1u, abort_flag, p.status, ERR_WAIT_TMEM_FULL);
+        ok = p8_wait(&ctrl->o_full[t], done + it - 1 & 1u, abort_flag, p.status, ERR_WAIT_TMEM_FULL);
         if (!__all_sync(kAll, ok)) { alive = false; break; }
       }
-      // turns with the exponentials: tile 0 (it), tile 1 (it), tile 0 (it + 1), ...
-      if (t == 0 ? (it >= 1 && it - 1 < n_other) : (it < n_other)) {
-        ok = p8_wait(&ctrl->turn[t][quad], uint32_t(t == 0 ? it - 1 : it) & 1u, abort_flag, p.status, ERR_WAIT_SOFTMAX);
+      // turns with the exponentials, where both query tiles have one: tile 0 (it), tile 1 (it), tile 0 (it + 1), ..., over all works
+      if (it < cur.paired && (t == 1 || pairs + it > 0)) {
+        ok = p8_wait(&ctrl->turn[t][quad], pairs + it - (t == 0 ? 1 : 0) & 1u, abort_flag, p.status, ERR_WAIT_SOFTMAX);
         if (!__all_sync(kAll, ok)) { alive = false; break; }
       }
 #pragma unroll
@@ -551,7 +661,7 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
               make_uint4(pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ctrl->turn[1 - t][quad]);
+      if (lane == 0 && it < cur.paired) mbar_arrive(&ctrl->turn[1 - t][quad]);
       fence_proxy_async();
       tc_fence_before();
       __syncwarp();
@@ -559,50 +669,128 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
       const float2 s4 = fadd2(fadd2(sum2[0], sum2[1]), fadd2(sum2[2], sum2[3]));
       l = fmaf(s4.x + s4.y, exp2_int(-e_v), l);
     }
-    // ---- O / l
-    if (tr.rows > 0) {
-      bool have_o = false;
-      if (alive && n_tiles > 0) {
-        const bool ok = p8_wait(&ctrl->o_full[t], uint32_t(n_tiles - 1) & 1u, abort_flag, p.status, ERR_WAIT_TMEM_FULL);
-        have_o = __all_sync(kAll, ok);
-        if (have_o) tc_fence_after();
       }
-      float osc = exp2f(-kP8Lift);                        // what values are larger by
-      if (p.sinks) {
-        const float sk = p.sinks[mine ? head : 0] * 1.4426950408889634f, m2 = fmaxf(m, sk), keep = m == -INFINITY ? 0.f : exp2f(m - m2);
-        osc *= keep;
-        l = l * keep + exp2f(sk - m2 + kP8Lift);
-      }
-      const float inv = l == 0.f ? 0.f : osc / l;
-      __nv_bfloat16* dst = p.out + (q_row * p.nq + head) * D;
-      const bool store = mine && !*abort_flag;
+      // ---- queries of the next work, ahead of this one's result: the products of this one with Q have been read
+      bool more = false;
+      P8Work k;
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        if (have_o) {
-          tmem_ld_32x32(o_addr + c * 32, o);
-          tmem_ld_wait();
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0u;
+      while (alive && !last && !more) {
+        if (!p8_next(ctrl, n_works, k, false, p.status)) {
+          last = true;
+          break;
         }
-        if (store) {
+        const P8Range tr = t == 0 ? k.tr0 : k.tr1;
+        next.tiles0 = tiles_seen;
+        tiles_seen += k.n_union;
+        if (tr.rows == 0) continue;                       // (a work's second query tile may have none)
+        more = true;
+        const int row = k.row0 + t * kP8Tile + r, token = row / p.group;
+        const long long q_row = (long long)p.q_start[k.b] + token;
+        next.head = k.kvh * p.group + row % p.group;
+        next.at = r < tr.rows && q_row >= 0 && q_row < p.total_q ? q_row * p.nq + next.head : -1;
+        next.tile_lo = tr.lo;
+        next.x0 = tr.lo - k.u_lo;
+        next.n_tiles = tr.hi - tr.lo;
+        next.paired = k.paired();
+        const int q_pos = k.ctx - k.q_len + token;
+        next.hi_pos = p.causal ? min(k.ctx - 1, q_pos) : k.ctx - 1;
+        next.lo_pos = nkb_first_visible(q_pos, p.window, p.chunk);
+        uint4 v[D / 8];
+        const uint4* src = reinterpret_cast<const uint4*>(p.q + next.at * D);
+        float mx = 0.f;
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            uint4 w;
-            w.x = pack_bf16x2(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
-            w.y = pack_bf16x2(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
-            w.z = pack_bf16x2(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
-            w.w = pack_bf16x2(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
-            *reinterpret_cast<uint4*>(dst + c * 32 + i) = w;
+        for (int i = 0; i < D / 8; ++i) v[i] = next.at >= 0 ? src[i] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const uint32_t q4[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = unpack_bf16x2(q4[j]);
+            mx = fmax3(mx, fabsf(f.x), fabsf(f.y));
           }
         }
+        const int e = max((__float_as_int(mx) >> 23) - 127, -100);
+        const float up = exp2_int(14 - e);
+        next.raw_log2 = p.scale_log2 * exp2_int(e - 14);
+        uint8_t* dst = q_s + t * L::kTile + r * 128;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const uint32_t q4[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+          uint32_t h[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = unpack_bf16x2(q4[j]);
+            h[j] = p8_pack_f16x2(f.x * up, f.y * up);
+          }
+          *reinterpret_cast<uint4*>(dst + (i >> 3) * kHalf + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0 && next.n_tiles > 0) mbar_arrive(&ctrl->q_full[t]);
       }
+      // ---- O / l
+      if (have) {
+        bool have_o = false;
+        if (alive && cur.n_tiles > 0) {
+          const bool ok = p8_wait(&ctrl->o_full[t], done + cur.n_tiles - 1 & 1u, abort_flag, p.status, ERR_WAIT_TMEM_FULL);
+          have_o = __all_sync(kAll, ok);
+          alive = have_o;
+          if (have_o) tc_fence_after();
+        }
+        float osc = exp2f(-kP8Lift);                      // what values are larger by
+        if (p.sinks) {
+          const float sk = p.sinks[cur.head] * 1.4426950408889634f, m2 = fmaxf(m, sk), keep = m == -INFINITY ? 0.f : exp2f(m - m2);
+          osc *= keep;
+          l = l * keep + exp2f(sk - m2 + kP8Lift);
+        }
+        const float inv = l == 0.f ? 0.f : osc / l;
+        __nv_bfloat16* dst = p.out + cur.at * D;
+        const bool store = cur.at >= 0 && !*abort_flag;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          if (have_o) {
+            tmem_ld_32x32(o_addr + c * 32, o);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0u;
+          }
+          if (store) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              uint4 x;
+              x.x = pack_bf16x2(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
+              x.y = pack_bf16x2(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
+              x.z = pack_bf16x2(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
+              x.w = pack_bf16x2(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
+              *reinterpret_cast<uint4*>(dst + c * 32 + i) = x;
+            }
+          }
+        }
+        if (have_o) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctrl->o_empty[t]);
+        }
+        done += cur.n_tiles;
+        pairs += cur.paired;
+      }
+      if (!more || !alive) break;
+      cur = next;
+      have = true;
     }
   }
 
   if (*abort_flag) {
     for (int i = 0; i < 200; ++i) __nanosleep(1000);
+  }
+  if (threadIdx.x == 15 * 32) {                           // this warp has taken its last work
+    __threadfence();
+    if (atomicAdd(p.sched + 1, 1u) == gridDim.x - 1) {
+      p.sched[0] = 0u;
+      p.sched[1] = 0u;
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -613,7 +801,7 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
 }
 
 template <int D>
-static int launch_prefill_q8(const PrefillQ8Params& p, int batch, int max_q_len, cudaStream_t s) {
+static int launch_prefill_q8(const PrefillQ8Params& p, cudaStream_t s) {
   using L = PrefillQ8Smem<D>;
   static bool attr_set[64] = {false};
   int dev = 0;
@@ -626,20 +814,20 @@ static int launch_prefill_q8(const PrefillQ8Params& p, int batch, int max_q_len,
     if (cudaError_t e = cudaFuncSetAttribute(attn_q8_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes)) return int(e);
     attr_set[dev] = true;
   }
-  const long long tiles = ((long long)max_q_len * p.group + 2 * kP8Tile - 1) / (2 * kP8Tile);
-  if (tiles > 0x7fffffffll) return -2;
-  return launch_pdl(attn_q8_prefill_kernel<D>, dim3(unsigned(tiles), p.nkv, batch), dim3(kP8Threads), size_t(L::kBytes), s, p);
+  const long long works = (long long)p.q_blocks * p.nkv * p.batch;
+  return launch_pdl(attn_q8_prefill_kernel<D>, dim3(unsigned(works < num_sms() ? works : num_sms())), dim3(kP8Threads), size_t(L::kBytes), s, p);
 }
 
 }  // namespace nkb
 
 using namespace nkb;
 
+// sched: two words that are zero before the first call (a call leaves them at zero); not shared by calls that may run at the same time
 extern "C" int nkb_q8_attn_prefill(const void* q, const void* k_values, const void* k_scales, const void* v_values, const void* v_scales,
                                    const int* block_table, const int* q_start, const int* q_lens, const int* context_lens, void* out,
                                    int batch, int total_q, int max_q_len, int nq, int nkv, int head_dim, int num_blocks, int table_width,
                                    long long table_stride, float scale, int causal, int window, int chunk, const float* sinks,
-                                   void* stream) {
+                                   unsigned int* sched, void* stream) {
   if (batch <= 0 || total_q <= 0) return 0;
   if (batch > 65535 || nkv > 65535 || nkv < 1 || nq % nkv || max_q_len < 1) return -2;
   if (!status_word() && nkb_init() != 0) return -1;
@@ -651,12 +839,16 @@ extern "C" int nkb_q8_attn_prefill(const void* q, const void* k_values, const vo
   p.out = (__nv_bfloat16*)out;
   p.sinks = sinks;
   p.status = status_word();
+  p.sched = sched;
+  const long long blocks = ((long long)max_q_len * (nq / nkv) + 2 * kP8Tile - 1) / (2 * kP8Tile);
+  if (!sched || blocks * nkv * batch > 0x7fffffffll) return -2;
+  p.batch = batch; p.q_blocks = int(blocks);
   p.total_q = total_q; p.nq = nq; p.nkv = nkv; p.group = nq / nkv; p.num_blocks = num_blocks; p.table_width = table_width;
   p.causal = causal; p.window = window; p.chunk = chunk;
   p.table_stride = table_stride;
   p.scale_log2 = scale * 1.4426950408889634f;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (head_dim == 128) return launch_prefill_q8<128>(p, batch, max_q_len, s);
-  if (head_dim == 64) return launch_prefill_q8<64>(p, batch, max_q_len, s);
+  if (head_dim == 128) return launch_prefill_q8<128>(p, s);
+  if (head_dim == 64) return launch_prefill_q8<64>(p, s);
   return -2;
 }

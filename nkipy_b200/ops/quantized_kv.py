@@ -378,7 +378,7 @@ def flash_attn_prefill(q, k_cache, v_cache, block_table, q_start, q_lens, contex
         q.data_ptr(), k_cache.values.data_ptr(), k_cache.scales.data_ptr(), v_cache.values.data_ptr(), v_cache.scales.data_ptr(),
         block_table.data_ptr(), q_start.data_ptr(), q_lens.data_ptr(), context_lens.data_ptr(), out.data_ptr(), B, q.shape[0],
         int(max_q_len), nq, nkv, D, blocks, block_table.shape[1], block_table.stride(0), float(scale), 1 if causal else 0, int(window),
-        int(chunk), _p(sinks), _stream())
+        int(chunk), _p(sinks), _scratch(dev, COUNTERS).data_ptr(), _stream())
     _lib.check(rc, "nkb_q8_attn_prefill")
     _count_launch()
     return out

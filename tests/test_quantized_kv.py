@@ -341,6 +341,9 @@ PROMPTS = [
     (2, 1, 128, [(60, 150)], dict(chunk=70)),
     (1, 1, 64, [(0, 70), (0, 200)], dict(causal=False)),
     (2, 1, 128, [(0, 140), (33, 5)], dict(causal=False)),
+    (8, 4, 64, [(0, 70)] * 41 + [(129, 3), (0, 1)], {}),                     # more pieces than SMs
+    (6, 1, 128, [(3 * i, 1 + 11 * i) for i in range(24)], {}),               # of every length
+    (5, 1, 64, [(0, 60), (300, 60)], dict(window=1)),
 ]
 
 
@@ -364,6 +367,27 @@ def test_prompts(device, nq, nkv, dim, spans, masks):
     check_attention(out.view(-1, nq, dim), q.view(-1, nq, dim), k, v, table, list(zip(starts, new, contexts)), dim ** -0.5, nq, nq // nkv,
                     sinks, **masks)
     assert bool((out[total:] == 7.0).all())                                  # rows behind the last sequence
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prompts_with_tokens_ahead_of_the_first(device, dim):
+    """Contexts shorter than the new tokens, or empty: rows that see nothing are zero (with or without sinks), pieces without a tile lie
+    among others."""
+    g = torch.Generator().manual_seed(dim + 2)
+    nq, nkv = 4, 1
+    spans = [(70, 3), (90, 0), (200, 130), (1, 0), (150, -1), (65, 65), (300, 10)]
+    contexts = [c for _, c in spans]
+    table, blocks = shuffled_table(g, contexts)
+    k, v = pool(g, blocks, nkv, dim, device)
+    new = [n for n, _ in spans]
+    starts = [sum(new[:b]) for b in range(len(new))]
+    q = torch.randn((sum(new), nq * dim), generator=g).to(torch.bfloat16)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)        # noqa: E731
+    for sinks in (None, torch.randn((nq,), generator=g)):
+        out = ops.flash_attn_prefill(q.to(device), k, v, table.to(device), i32(starts), i32(new), i32(contexts), dim ** -0.5,
+                                     max_q_len=max(new), sinks=None if sinks is None else sinks.to(device))
+        check_attention(out.view(-1, nq, dim), q.view(-1, nq, dim), k, v, table, list(zip(starts, new, contexts)), dim ** -0.5, nq, nq, sinks)
 
 
 @pytest.mark.parametrize("device", DEVICES)
