@@ -32,7 +32,7 @@ get_config = _load("gpt_oss_config", os.path.join(HERE, "..", "config.py")).get_
 peagle_config = _load("peagle_config", os.path.join(HERE, "config.py"))
 
 from nkipy_b200.models.engine import GenerationEngine  # noqa: E402
-from nkipy_b200.models.runner import add_common_args, build_model, build_prompts, load_tokenizer  # noqa: E402
+from nkipy_b200.models.runner import add_common_args, build_model, build_prompts, kv_dtype, load_tokenizer  # noqa: E402
 from nkipy_b200.models.speculative import DrafterLM, SpeculativeEngine, random_drafter_weights  # noqa: E402
 from nkipy_b200.models.weights import load_shard  # noqa: E402
 from nkipy_b200.parallel.comm import TPGroup  # noqa: E402
@@ -56,7 +56,7 @@ def main():
     drafter = DrafterLM(ecfg, dw, tp.device)
     prompts = build_prompts(args, cfg, load_tokenizer(args.model))
     max_len = max(len(p) for p in prompts) + args.max_new_tokens + 64
-    spec = SpeculativeEngine(target, drafter, max_batch=len(prompts), max_seq_len=max_len)
+    spec = SpeculativeEngine(target, drafter, max_batch=len(prompts), max_seq_len=max_len, kv_dtype=kv_dtype(args))
     spec.generate([p[:16] for p in prompts], 4)                    # warm-up
     spec.stats.__init__()
     out = spec.generate(prompts, args.max_new_tokens)
@@ -67,7 +67,7 @@ def main():
     print(f"Mean acceptance length: {s.mean_acceptance:.2f} (K={spec.K})")
     print(f"Decode tokens/sec: {n / max(s.decode_s, 1e-9):.2f}  (draft {s.draft_s:.3f}s, verify {s.verify_s:.3f}s)")
     eng = GenerationEngine(target, max_batch=len(prompts), max_seq_len=max_len,
-                           use_cuda_graph=tp.device.type == "cuda" and not args.no_graph)
+                           use_cuda_graph=tp.device.type == "cuda" and not args.no_graph, kv_dtype=kv_dtype(args))
     eng.generate([p[:16] for p in prompts], 4)
     eng.stats.__init__()
     t0 = time.perf_counter()

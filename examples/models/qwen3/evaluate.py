@@ -23,7 +23,7 @@ from config import get_config  # noqa: E402
 
 from nkipy_b200.models.engine import GenerationEngine  # noqa: E402
 from nkipy_b200.models.reference import EagerTransformer  # noqa: E402
-from nkipy_b200.models.runner import add_common_args, build_prompts, load_tokenizer  # noqa: E402
+from nkipy_b200.models.runner import add_common_args, build_prompts, kv_dtype, load_tokenizer  # noqa: E402
 from nkipy_b200.models.transformer import TransformerLM  # noqa: E402
 from nkipy_b200.models.weights import load_shard, random_weights  # noqa: E402
 from nkipy_b200.parallel.comm import TPGroup  # noqa: E402
@@ -38,7 +38,7 @@ def evaluate(cfg, args):
     prompts = build_prompts(args, cfg, load_tokenizer(args.model))
     n = args.max_new_tokens
     eng = GenerationEngine(model, max_batch=len(prompts), max_seq_len=len(prompts[0]) + n + 64,
-                           use_cuda_graph=dev.type == "cuda" and not args.no_graph)
+                           use_cuda_graph=dev.type == "cuda" and not args.no_graph, kv_dtype=kv_dtype(args))
     eng.generate([p[:8] for p in prompts], 2)
     eng.stats.__init__()
     t0 = time.perf_counter()

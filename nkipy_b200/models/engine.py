@@ -127,7 +127,8 @@ class GenerationEngine:
 
     def __init__(self, model: TransformerLM, max_batch: int, max_seq_len: int, num_blocks: Optional[int] = None,
                  prefill_chunk_tokens: int = 16384, use_cuda_graph: Optional[bool] = None,
-                 enable_prefix_sharing: bool = True):
+                 enable_prefix_sharing: bool = True, kv_dtype: Optional[torch.dtype] = None):
+        """kv_dtype torch.float8_e4m3fn: keys and values in 8 bits (default: as the model computes)."""
         self.model = model
         self.device = model.device
         self.max_batch = max_batch
@@ -135,7 +136,8 @@ class GenerationEngine:
         blocks_per_seq = (max_seq_len + BLOCK_SIZE - 1) // BLOCK_SIZE
         if num_blocks is None:
             num_blocks = max_batch * blocks_per_seq + 8
-        self.cache: PagedKVCache = model.new_cache(num_blocks, max_batch, max_seq_len, enable_prefix_sharing)
+        self.cache: PagedKVCache = model.new_cache(num_blocks, max_batch, max_seq_len, enable_prefix_sharing,
+                                                  kv_dtype=kv_dtype)
         self.prefill_chunk_tokens = prefill_chunk_tokens
         self.use_cuda_graph = (self.device.type == "cuda") if use_cuda_graph is None else use_cuda_graph
         dev = self.device

@@ -300,7 +300,9 @@ class HybridLM:
 
     # ------------------------------------------------------------------ cache
     def new_cache(self, num_blocks: int, max_batch: int, max_seq_len: int,
-                  enable_prefix_sharing: bool = True) -> PagedKVCache:
+                  enable_prefix_sharing: bool = True, kv_dtype: Optional[torch.dtype] = None) -> PagedKVCache:
+        if kv_dtype not in (None, self.dtype):
+            raise ValueError(f"a model described layer by layer keeps keys and values as {self.dtype}, not {kv_dtype}")
         max_blocks = (max_seq_len + self.cfg.block_size - 1) // self.cfg.block_size
         self._extend_rope(max_blocks * self.cfg.block_size)
         entries = [e for i, _ in self.runs for e in self.layers[i].mixer.entries()]

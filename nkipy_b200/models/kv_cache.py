@@ -14,6 +14,10 @@ Layers may also differ: `PagedKVCache.for_layers` takes one `KVLayer` (keys and
 values of any sizes, paged) or `StateLayer` (a fixed-size recurrent state per
 batch row, fp32) per layer.  A state belongs to a whole sequence, not to a block
 of tokens, so a cache with state layers never shares prefixes.
+
+``dtype=torch.float8_e4m3fn`` keeps keys and values in 8 bits (`ops.QuantizedPages`
+in the place of every pool): half the bytes of bf16, and half of what a decode
+step reads of the cache.
 """
 
 from __future__ import annotations
@@ -24,6 +28,9 @@ from typing import Dict, List, Optional, Sequence, Tuple, Union
 
 import numpy as np
 import torch
+
+from ..ops.quantized_kv import DIMS as QUANTIZED_DIMS
+from ..ops.quantized_kv import QuantizedPages
 
 BLOCK_SIZE = 32
 
@@ -200,9 +207,14 @@ class PagedKVCache:
         self.max_blocks_per_seq = max_blocks_per_seq
         self.device = torch.device(device)
         self.has_state = any(isinstance(l, StateLayer) for l in layers)
-        # zero-filled: masked positions are multiplied by probability 0 and must be finite
-        pool = lambda heads, dim: torch.zeros((num_blocks, heads, BLOCK_SIZE, dim), dtype=dtype, device=device)
+        self.quantized = dtype is torch.float8_e4m3fn
+        self.scratch = None                  # workspace of decode attention that belongs to this cache (quantised pages)
         kv = [isinstance(l, KVLayer) for l in layers]
+        if self.quantized and not all(on and l.k_dim == l.v_dim and l.k_dim in QUANTIZED_DIMS for on, l in zip(kv, layers)):
+            raise ValueError("a cache in 8 bits wants keys and values of 64 or 128 columns in every layer")
+        # zero-filled: masked positions are multiplied by probability 0 and must be finite
+        pool = lambda heads, dim: (QuantizedPages.new(num_blocks, heads, dim, device) if self.quantized else
+                                   torch.zeros((num_blocks, heads, BLOCK_SIZE, dim), dtype=dtype, device=device))
         self.k = [pool(l.kv_heads, l.k_dim) if on else None for l, on in zip(layers, kv)]
         self.v = [pool(l.kv_heads, l.v_dim) if on else None for l, on in zip(layers, kv)]
         self.state = [None if on else torch.zeros((max_batch, *l.shape), dtype=torch.float32, device=device)
@@ -217,7 +229,7 @@ class PagedKVCache:
         self._next_id = 0
 
     def bytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in (*self.k, *self.v, *self.state) if t is not None)
+        return sum(t.nbytes for t in (*self.k, *self.v, *self.state) if t is not None)
 
     # -- admission / growth / release
     def open_sequence(self) -> SequenceState:

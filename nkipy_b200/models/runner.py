@@ -38,8 +38,14 @@ def add_common_args(ap: argparse.ArgumentParser) -> None:
     ap.add_argument("--top-p", type=float, default=1.0)
     ap.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16",
                     help="float32: true 32-bit, for the models that have it")
+    ap.add_argument("--kv-dtype", choices=["auto", "bfloat16", "e4m3"], default="auto",
+                    help="keys and values in the cache; e4m3: 8 bits, for the models that have it; auto: as the model computes")
     ap.add_argument("--tiny", action="store_true",
                     help="shrink the model (hidden 256, vocabulary 2048, <= 8 experts) for quick functional runs")
+
+
+def kv_dtype(args) -> Optional[torch.dtype]:
+    return {"auto": None, "bfloat16": torch.bfloat16, "e4m3": torch.float8_e4m3fn}[args.kv_dtype]
 
 
 def load_tokenizer(path: Optional[str]):
@@ -117,7 +123,7 @@ def run_generation(cfg: ModelConfig, args, model=None, tp: Optional[TPGroup] = N
     prompts = build_prompts(args, model.cfg, tokenizer)
     max_len = min(args.max_seq_len, max(len(p) for p in prompts) + args.max_new_tokens + 64)
     eng = GenerationEngine(model, max_batch=len(prompts), max_seq_len=max_len,
-                           use_cuda_graph=not args.no_graph and tp.device.type == "cuda")
+                           use_cuda_graph=not args.no_graph and tp.device.type == "cuda", kv_dtype=kv_dtype(args))
     eng.generate([p[:8] for p in prompts], 2)            # warm-up (graph capture, autotuned splits)
     eng.stats.__init__()
     tp.barrier()

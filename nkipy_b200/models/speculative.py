@@ -154,7 +154,9 @@ class SpeculativeEngine:
     """Target engine state + drafter + the accept loop (examples/models/gpt_oss/peagle/speculate.py:236-459)."""
 
     def __init__(self, target: TransformerLM, drafter: DrafterLM, max_batch: int, max_seq_len: int,
-                 num_draft_tokens: Optional[int] = None, num_blocks: Optional[int] = None):
+                 num_draft_tokens: Optional[int] = None, num_blocks: Optional[int] = None,
+                 kv_dtype: Optional[torch.dtype] = None):
+        """kv_dtype: of the target's keys and values (the drafter's stay bf16)."""
         if target.tp.world_size != 1:
             raise NotImplementedError("speculative decoding runs the target on one rank here")
         self.target, self.drafter = target, drafter
@@ -166,7 +168,7 @@ class SpeculativeEngine:
         blocks_per_seq = (max_seq_len + slack + BLOCK_SIZE - 1) // BLOCK_SIZE
         if num_blocks is None:
             num_blocks = max_batch * blocks_per_seq + 1
-        self.cache = target.new_cache(num_blocks, max_batch, max_seq_len + slack, enable_prefix_sharing=False)
+        self.cache = target.new_cache(num_blocks, max_batch, max_seq_len + slack, enable_prefix_sharing=False, kv_dtype=kv_dtype)
         self.dcache = drafter.new_cache(self.cache)
         self.taps = tap_layers(target.cfg.num_layers)
         self.stats = SpecStats()

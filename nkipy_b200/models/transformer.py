@@ -132,10 +132,16 @@ class TransformerLM:
 
     # ------------------------------------------------------------------ cache
     def new_cache(self, num_blocks: int, max_batch: int, max_seq_len: int,
-                  enable_prefix_sharing: bool = True) -> PagedKVCache:
+                  enable_prefix_sharing: bool = True, kv_dtype: Optional[torch.dtype] = None) -> PagedKVCache:
+        """kv_dtype torch.float8_e4m3fn: keys and values in 8 bits."""
+        if kv_dtype not in (None, torch.bfloat16, torch.float8_e4m3fn):
+            raise ValueError(f"keys and values are kept as bfloat16 or float8_e4m3fn, not {kv_dtype}")
         max_blocks = (max_seq_len + self.cfg.block_size - 1) // self.cfg.block_size
-        return PagedKVCache(self.cfg.num_layers, self.nkv, self.d, num_blocks, max_batch, max_blocks, self.device,
-                            enable_prefix_sharing=enable_prefix_sharing)
+        cache = PagedKVCache(self.cfg.num_layers, self.nkv, self.d, num_blocks, max_batch, max_blocks, self.device,
+                             dtype=kv_dtype or torch.bfloat16, enable_prefix_sharing=enable_prefix_sharing)
+        if cache.quantized:
+            cache.scratch = ops.quantized_kv.decode_scratch(cache.k[0], self.nq, max_batch, max_blocks)
+        return cache
 
     def weight_bytes(self) -> int:
         n = self.tok_embedding.numel() + self.lm_head.numel()
@@ -221,10 +227,11 @@ class TransformerLM:
             resid, normed = inputs
         taps = [] if return_hidden else None
         T = normed.shape[0]
-        if self._persistent_layers(T, normed):
+        if self._persistent_layers(T, normed) and not cache.quantized:
             return self._decode_step_persistent(resid, normed, positions, slots, cache, block_table, context_lens,
                                                 q_len, taps)
-        cluster = self.cluster_gemm and T <= 128 and normed.is_cuda and self.d in (64, 128)
+        # (the projections that append by themselves write bf16)
+        cluster = self.cluster_gemm and T <= 128 and normed.is_cuda and self.d in (64, 128) and not cache.quantized
         for i, lw in enumerate(self.layers):
             if cluster:
                 # QKV projection, QK-norm, RoPE and the cache append in one launch
@@ -243,14 +250,14 @@ class TransformerLM:
                     attn = ops.rope_attn_decode(qkv, positions, slots, self.rope, cache.k[i], cache.v[i], block_table,
                                                 context_lens, self.scale, self.nq, self.nkv, bias=lw.qkv_bias,
                                                 q_norm_w=lw.q_norm, k_norm_w=lw.k_norm, norm_eps=cfg.rms_eps,
-                                                window=cfg.window_for_layer(i), sinks=lw.sinks)
+                                                window=cfg.window_for_layer(i), sinks=lw.sinks, scratch=cache.scratch)
                 else:
                     q = ops.rope_kv_append(qkv, positions, slots, self.rope, cache.k[i], cache.v[i], self.nq,
                                            self.nkv, self.d, bias=lw.qkv_bias, q_norm_w=lw.q_norm,
                                            k_norm_w=lw.k_norm, norm_eps=cfg.rms_eps)
             if q is not None:
-                attn = ops.paged_attn_decode(q, cache.k[i], cache.v[i], block_table, context_lens, self.scale,
-                                             q_len=q_len, window=cfg.window_for_layer(i), sinks=lw.sinks)
+                attn = ops.paged_attn_decode(q, cache.k[i], cache.v[i], block_table, context_lens, self.scale, q_len=q_len,
+                                             window=cfg.window_for_layer(i), sinks=lw.sinks, scratch=cache.scratch)
             split_o = self._csplits(lw.o, T) if cluster else self.split_o
             resid, normed = self._row_parallel_reduce(attn, lw.o, split_o, resid, lw.post_norm, lw.o_bias)
             nxt = self.layers[i + 1].input_norm if i + 1 < len(self.layers) else self.final_norm

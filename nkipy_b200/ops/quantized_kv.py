@@ -269,6 +269,17 @@ def _pick_splits(ctas: int, max_pages: int, sms: int = 148) -> int:
     return 1 if ctas >= sms else max(min(sms // ctas, max(max_pages // 8, 1), 16), 1)
 
 
+def decode_scratch(pages: QuantizedPages, nq: int, max_batch: int, max_pages: int) -> Optional[torch.Tensor]:
+    """Scratch for every decode attention of up to max_batch sequences of max_pages pages, for a caller that keeps its own: steps that
+    are captured into a graph share it, one behind another.  None on the CPU."""
+    if not pages.is_cuda:
+        return None
+    nkv, D = pages.shape[1], pages.shape[3]
+    L = _lib.lib()
+    floats = max(L.nkb_q8_attn_decode_scratch_floats(b, nkv, D, nq // nkv, _pick_splits(b * nkv, max_pages)) for b in range(1, max_batch + 1))
+    return torch.zeros((max(int(floats), COUNTERS),), dtype=torch.float32, device=pages.device)
+
+
 # --------------------------------------------------------------------------- operators
 def rope_kv_append(qkv, positions, slots, cos_sin, k_cache, v_cache, nq, nkv, head_dim, *, bias=None, q_norm_w=None, k_norm_w=None,
                    norm_eps=1e-6, q_out=None) -> torch.Tensor:
