@@ -129,25 +129,60 @@ __global__ void __launch_bounds__(256) append_q8_kernel(const AppendQ8Params p) 
   if (lane == 0) (is_k ? p.k_scales : p.v_scales)[row] = uint8_t(fine ? 127 + e : 255);
 }
 
+// a * c - d * s from 32-bit numbers, rounded to odd like round_to_odd of the same in 64 bits: products and their difference with what each
+// rounding leaves (a product's rest is one multiply-add; the difference's by Knuth's two-sum).  Finite where the inputs are.
+__device__ __forceinline__ float turn_to_odd(float a, float c, float d, float s) {
+  // (intrinsics: the compiler must not merge these)
+  const float p = __fmul_rn(a, c), pe = __fmaf_rn(a, c, -p), q = __fmul_rn(d, s), qe = __fmaf_rn(d, s, -q);
+  const float x = __fsub_rn(p, q), v = __fsub_rn(x, p);
+  const float rest = __fadd_rn(__fsub_rn(__fsub_rn(p, __fsub_rn(x, v)), __fadd_rn(q, v)), __fsub_rn(pe, qe));
+  const float top = fminf(fmaxf(x == 0.f ? rest : x, -3.402823466e38f), 3.402823466e38f);
+  int bits = __float_as_int(top);
+  if (rest != 0.f && x != 0.f) {
+    if ((rest < 0.f) != (top < 0.f)) --bits;       // the sum lies nearer zero: the number before
+    bits |= 1;
+  }
+  return __int_as_float(bits);
+}
+
 // The same in pieces of sixteen bytes: D / 16 lanes share a head, each with eight elements of its first half and the eight that turn with
-// them.  Every pointer on 16 bytes, split_stride a multiple of four.
+// them.  A warp takes 512 / D heads of a token at a time, `run` times, the next ones' inputs on their way.  Every pointer on 16 bytes, split_stride a multiple of four.
+//
+// Bound by memory from some thousand tokens on, and next by what goes through L1: cos and sin are twice the bytes of a head's input, so a run
+// loads them once.  Then come instructions: 64-bit arithmetic and conversions run at a fraction of the 32-bit
+// rate, so keys of a bf16 projection without norm and bias turn in pairs of 32-bit numbers, and such values need no sum at all.
 template <int D, bool PARTIALS>
-__global__ void __launch_bounds__(256, PARTIALS ? 2 : 4) append8_q8_kernel(const AppendQ8Params p) {
-  constexpr int L = D / 16;
-  constexpr uint32_t kAll = 0xffffffffu;
-  const int heads = p.nq + 2 * p.nkv;
-  const long long units = (long long)p.tokens * heads, unit = (blockIdx.x * (long long)blockDim.x + threadIdx.x) / L;
+__global__ void __launch_bounds__(256, PARTIALS ? 2 : 3) append8_q8_kernel(const AppendQ8Params p, int run) {
+  constexpr int L = D / 16, kHeads = 32 / L;
+  const int heads = p.nq + 2 * p.nkv, runs = (heads + kHeads * run - 1) / (kHeads * run);
   const int i0 = (threadIdx.x % L) * 8;
+  const uint32_t mine = ((1u << L) - 1u) << ((threadIdx.x & 31) / L * L);      // the lanes of this head
   griddep_wait();
   griddep_launch();
-  // a warp's lanes leave together or stay for the sums: units past the end repeat the last one and store nothing
-  const bool on = unit < units;
-  const long long u = on ? unit : units - 1;
-  const int t = int(u / heads), h = int(u % heads);
-  const bool is_q = h < p.nq, is_k = !is_q && h < p.nq + p.nkv;
-  const long long base = (long long)t * heads * D + (long long)h * D + i0;
-  auto get8 = [](const __nv_bfloat16* src, float* o) {
-    const uint4 r = *reinterpret_cast<const uint4*>(src);
+  const uint32_t unit = blockIdx.x * 8 + threadIdx.x / 32;
+  const int t = int(unit / uint32_t(runs)), first = int(unit - uint32_t(t) * runs) * run * kHeads, h1 = min(first + run * kHeads, heads);
+  const int h0 = first + (threadIdx.x & 31) / L;
+  if (t >= p.tokens) return;
+  uint4 raw[2], raw_n[2];
+  auto load = [&](int h, uint4 (&r)[2]) {
+    if (!PARTIALS && h < h1) {
+      const __nv_bfloat16* src = p.qkv + ((long long)t * heads + h) * D + i0;
+      r[0] = *reinterpret_cast<const uint4*>(src);
+      r[1] = *reinterpret_cast<const uint4*>(src + D / 2);
+    }
+  };
+  load(h0, raw_n);
+  const long long slot = p.slots && h1 > p.nq ? p.slots[t] : -1;
+  float c[8], sn[8];
+  if (p.cos_sin && h0 < p.nq + p.nkv) {
+    const float* cs = p.cos_sin + (long long)min(max(p.positions[t], 0), p.max_pos - 1) * D + i0;  // [cos(d/2) | sin(d/2)]
+#pragma unroll
+    for (int j = 0; j < 8; j += 4) {
+      *reinterpret_cast<float4*>(c + j) = *reinterpret_cast<const float4*>(cs + j);
+      *reinterpret_cast<float4*>(sn + j) = *reinterpret_cast<const float4*>(cs + D / 2 + j);
+    }
+  }
+  auto floats = [](const uint4& r, float* o) {
     const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -156,135 +191,143 @@ __global__ void __launch_bounds__(256, PARTIALS ? 2 : 4) append8_q8_kernel(const
       o[2 * e + 1] = f.y;
     }
   };
-  float x[16];                           // queries, and what goes to the pages; at first bf16 inputs, exactly
-  double y[PARTIALS ? 16 : 1];           // sums of partials
-  if constexpr (PARTIALS) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) y[j] = 0.;
-#pragma unroll 2
-    for (int s = 0; s < p.splits; ++s) {
-#pragma unroll
-      for (int j = 0; j < 16; j += 4) {
-        const float4 v = *reinterpret_cast<const float4*>(p.partials + s * p.split_stride + base + (j < 8 ? j : D / 2 + j - 8));
-        y[j] += double(v.x);
-        y[j + 1] += double(v.y);
-        y[j + 2] += double(v.z);
-        y[j + 3] += double(v.w);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 16; ++j) x[j] = float(y[j]);
-  } else {
-    get8(p.qkv + base, x);
-    get8(p.qkv + base + D / 2, x + 8);
-  }
-  const auto at = [&](int j) { return i0 + (j < 8 ? j : D / 2 + j - 8); };
-  // the input with its bias in 64 bits
-  const auto in64 = [&](int j) {
-    double v;
-    if constexpr (PARTIALS) v = y[j];
-    else v = double(x[j]);
-    return p.bias ? v + double(__bfloat162float(p.bias[h * D + at(j)])) : v;
+  auto get16 = [&](const __nv_bfloat16* src, float* o) {         // this lane's elements of a head's row
+    floats(*reinterpret_cast<const uint4*>(src + i0), o);
+    floats(*reinterpret_cast<const uint4*>(src + D / 2 + i0), o + 8);
   };
-  const __nv_bfloat16* nw = is_q ? p.q_norm_w : (is_k ? p.k_norm_w : nullptr);
-  const float* cs = nullptr;             // [cos(d/2) | sin(d/2)]
-  if ((is_q || is_k) && p.cos_sin) cs = p.cos_sin + (long long)min(max(p.positions[t], 0), p.max_pos - 1) * D + i0;
-  if (is_q && p.bias) {
-    float b[16];
-    get8(p.bias + h * D + i0, b);
-    get8(p.bias + h * D + D / 2 + i0, b + 8);
+  const auto at = [&](int j) { return i0 + (j < 8 ? j : D / 2 + j - 8); };
+#pragma unroll 1
+  for (int h = h0; h < h1; h += kHeads) {
+    raw[0] = raw_n[0];
+    raw[1] = raw_n[1];
+    load(h + kHeads, raw_n);
+    const long long row0 = ((long long)t * heads + h) * D + i0;
+    const bool is_q = h < p.nq, is_k = !is_q && h < p.nq + p.nkv, turn = p.cos_sin && h < p.nq + p.nkv;
+    float x[16];                         // queries, and what goes to the pages; at first bf16 inputs, exactly
+    double y[PARTIALS ? 16 : 1];         // sums of partials
+    if constexpr (PARTIALS) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) x[j] += b[j];
-  }
-  double inv = 1.;
-  if (p.q_norm_w || p.k_norm_w) {
-    double ss = 0.;
+      for (int j = 0; j < 16; ++j) y[j] = 0.;
+#pragma unroll 2
+      for (int s = 0; s < p.splits; ++s) {
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(p.partials + s * p.split_stride + row0 + (j < 8 ? j : D / 2 + j - 8));
+          y[j] += double(v.x);
+          y[j + 1] += double(v.y);
+          y[j + 2] += double(v.z);
+          y[j + 3] += double(v.w);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = float(y[j]);
+    } else {
+      floats(raw[0], x);
+      floats(raw[1], x + 8);
+    }
+    // the input with its bias in 64 bits
+    const auto in64 = [&](int j) {
+      double v;
+      if constexpr (PARTIALS) v = y[j];
+      else v = double(x[j]);
+      return p.bias ? v + double(__bfloat162float(p.bias[h * D + at(j)])) : v;
+    };
+    const __nv_bfloat16* nw = is_q ? p.q_norm_w : (is_k ? p.k_norm_w : nullptr);
+    double inv = 1.;
     if (is_q) {
-      float s = 0.f;
+      if (p.bias) {
+        float b[16];
+        get16(p.bias + h * D, b);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) s += x[j] * x[j];
-      ss = double(s);
+        for (int j = 0; j < 16; ++j) x[j] += b[j];
+      }
+      if (nw) {
+        float ss = 0.f, w[16];
+        get16(nw, w);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) ss += x[j] * x[j];
+#pragma unroll
+        for (int m = L / 2; m > 0; m >>= 1) ss += __shfl_xor_sync(mine, ss, m);
+        const float f = 1.f / sqrtf(ss / float(D) + float(p.eps));
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = x[j] * f * w[j];
+      }
+      if (turn) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float a = x[j], d = x[8 + j];
+          x[j] = a * c[j] - d * sn[j];
+          x[8 + j] = d * c[j] + a * sn[j];
+        }
+      }
+      __nv_bfloat16* dst = p.q_out + ((long long)t * p.nq + h) * D + i0;
+      *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+      *reinterpret_cast<uint4*>(dst + D / 2) =
+          make_uint4(pack_bf16x2(x[8], x[9]), pack_bf16x2(x[10], x[11]), pack_bf16x2(x[12], x[13]), pack_bf16x2(x[14], x[15]));
+      continue;
+    }
+    bool fine = true;
+    if (PARTIALS || p.bias || nw) {
+      if (nw) {
+        double ss = 0.;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const double v = in64(j);
+          ss += v * v;
+        }
+#pragma unroll
+        for (int m = L / 2; m > 0; m >>= 1) ss += __shfl_xor_sync(mine, ss, m);
+        inv = 1. / sqrt(ss / double(D) + p.eps);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        double a = in64(j), d = in64(8 + j);
+        if (nw) {
+          a = a * inv * double(__bfloat162float(nw[at(j)]));
+          d = d * inv * double(__bfloat162float(nw[at(8 + j)]));
+        }
+        if (is_k && turn) {
+          const double co = c[j], si = sn[j], a0 = a;
+          a = a0 * co - d * si;
+          d = d * co + a0 * si;
+        }
+        x[j] = round_to_odd(a);
+        x[8 + j] = round_to_odd(d);
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) fine = fine && isfinite(x[j]);
     } else {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const double v = in64(j);
-        ss += v * v;
-      }
-    }
+      for (int j = 0; j < 16; ++j) fine = fine && isfinite(x[j]);
+      if (is_k && turn) {
 #pragma unroll
-    for (int m = L / 2; m > 0; m >>= 1) ss += __shfl_xor_sync(kAll, ss, m);
-    if (nw) inv = 1. / sqrt(ss / double(D) + p.eps);
-  }
-  if (is_q) {
-    if (nw) {
-      float w[16];
-      get8(nw + i0, w);
-      get8(nw + D / 2 + i0, w + 8);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) x[j] = x[j] * float(inv) * w[j];
-    }
-    if (cs) {
-#pragma unroll
-      for (int j = 0; j < 8; j += 4) {
-        const float4 c4 = *reinterpret_cast<const float4*>(cs + j), s4 = *reinterpret_cast<const float4*>(cs + D / 2 + j);
-        const float c[4] = {c4.x, c4.y, c4.z, c4.w}, sn[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float a = x[j + k], d = x[8 + j + k];
-          x[j + k] = a * c[k] - d * sn[k];
-          x[8 + j + k] = d * c[k] + a * sn[k];
+        for (int j = 0; j < 8; ++j) {
+          const float a = x[j], d = x[8 + j];
+          fine = fine && isfinite(c[j]) && isfinite(sn[j]);
+          x[j] = turn_to_odd(a, c[j], d, sn[j]);
+          x[8 + j] = turn_to_odd(d, c[j], -a, sn[j]);
         }
       }
     }
-    if (!on) return;
-    __nv_bfloat16* dst = p.q_out + ((long long)t * p.nq + h) * D + i0;
-    *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
-    *reinterpret_cast<uint4*>(dst + D / 2) =
-        make_uint4(pack_bf16x2(x[8], x[9]), pack_bf16x2(x[10], x[11]), pack_bf16x2(x[12], x[13]), pack_bf16x2(x[14], x[15]));
-    return;
+    float amax = 0.f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(x[j]));
+#pragma unroll
+    for (int m = L / 2; m > 0; m >>= 1) amax = fmaxf(amax, __shfl_xor_sync(mine, amax, m));
+    fine = __all_sync(mine, fine);
+    if (slot < 0 || slot >= p.slots_end) continue;
+    const int e = q8_log2_scale(amax);
+    const float down = exp2_int(-e);
+    const long long row = (slot / kQ8Page * p.nkv + (is_k ? h - p.nq : h - p.nq - p.nkv)) * kQ8Page + slot % kQ8Page;
+    uint8_t* dst = (is_k ? p.k_values : p.v_values) + row * D + i0;
+    uint32_t v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      v[j] = fine ? pack_e4m3x2(x[4 * j] * down, x[4 * j + 1] * down) | uint32_t(pack_e4m3x2(x[4 * j + 2] * down, x[4 * j + 3] * down)) << 16 : 0u;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(v[0], v[1]);
+    *reinterpret_cast<uint2*>(dst + D / 2) = make_uint2(v[2], v[3]);
+    if (i0 == 0) (is_k ? p.k_scales : p.v_scales)[row] = uint8_t(fine ? 127 + e : 255);
   }
-  if (is_k || PARTIALS || p.bias) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      double a = in64(j), d = in64(8 + j);
-      if (nw) {
-        a = a * inv * double(__bfloat162float(nw[at(j)]));
-        d = d * inv * double(__bfloat162float(nw[at(8 + j)]));
-      }
-      if (cs) {
-        const double c = cs[j], sn = cs[D / 2 + j], a0 = a;
-        a = a0 * c - d * sn;
-        d = d * c + a0 * sn;
-      }
-      x[j] = round_to_odd(a);
-      x[8 + j] = round_to_odd(d);
-    }
-  }
-  float amax = 0.f;
-  bool fine = true;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    fine = fine && isfinite(x[j]);
-    amax = fmaxf(amax, fabsf(x[j]));
-  }
-  // the lanes of this head (those of queries have left)
-  const uint32_t mine = ((1u << L) - 1u) << ((threadIdx.x & 31) / L * L);
-#pragma unroll
-  for (int m = L / 2; m > 0; m >>= 1) amax = fmaxf(amax, __shfl_xor_sync(mine, amax, m));
-  fine = __all_sync(mine, fine);
-  const long long slot = p.slots ? p.slots[t] : -1;
-  if (!on || slot < 0 || slot >= p.slots_end) return;
-  const int e = q8_log2_scale(amax);
-  const float down = exp2_int(-e);
-  const long long row = (slot / kQ8Page * p.nkv + (is_k ? h - p.nq : h - p.nq - p.nkv)) * kQ8Page + slot % kQ8Page;
-  uint8_t* dst = (is_k ? p.k_values : p.v_values) + row * D + i0;
-  uint32_t v[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    v[j] = fine ? pack_e4m3x2(x[4 * j] * down, x[4 * j + 1] * down) | uint32_t(pack_e4m3x2(x[4 * j + 2] * down, x[4 * j + 3] * down)) << 16 : 0u;
-  *reinterpret_cast<uint2*>(dst) = make_uint2(v[0], v[1]);
-  *reinterpret_cast<uint2*>(dst + D / 2) = make_uint2(v[2], v[3]);
-  if (i0 == 0) (is_k ? p.k_scales : p.v_scales)[row] = uint8_t(fine ? 127 + e : 255);
 }
 
 }  // namespace nkb
@@ -296,6 +339,7 @@ extern "C" int nkb_q8_append(const void* qkv_bf16, const float* qkv_partials, in
                              double eps, void* q_out, void* k_values, void* k_scales, void* v_values, void* v_scales, int tokens, int nq,
                              int nkv, int head_dim, int max_pos, int num_blocks, void* stream) {
   if (tokens <= 0) return 0;
+  if (!status_word() && nkb_init() != 0) return -1;
   AppendQ8Params p{};
   p.qkv = (const __nv_bfloat16*)qkv_bf16;
   p.partials = qkv_partials;
@@ -319,13 +363,21 @@ extern "C" int nkb_q8_append(const void* qkv_bf16, const float* qkv_partials, in
   for (const void* a : {qkv_bf16, (const void*)qkv_partials, bias, (const void*)cos_sin, q_norm_w, k_norm_w, (const void*)q_out,
                         (const void*)k_values, (const void*)v_values})
     at |= reinterpret_cast<uintptr_t>(a);
-  const bool pieces = tokens >= 256 && (at & 15) == 0 && (!qkv_partials || (split_stride & 3) == 0);
+  // A few tokens are bound by latency and keep a warp per head: 64 of them from partial sums 3.3 us and 4.1 in pieces, 128 5.7 and 5.5, 255 from
+  // bf16 4.3 and 3.05.
+  const bool pieces = tokens >= (qkv_partials ? 128 : 64) && (at & 15) == 0 && (!qkv_partials || (split_stride & 3) == 0);
   const long long heads = (long long)tokens * (nq + 2 * nkv);
   if (heads > 0x7fffffffll) return -2;
-  const dim3 blocks(unsigned(pieces ? (heads * (head_dim / 16) + 255) / 256 : (heads + 7) / 8));
+  // runs so long that all warps are resident at once
+  const int steps = (nq + 2 * nkv + 512 / head_dim - 1) / (512 / head_dim);
+  const long long resident = num_sms() * (qkv_partials ? 16 : 24), need = ((long long)tokens * steps + resident - 1) / resident;
+  const long long run = need > steps ? steps : need;
+  const long long blocks = ((pieces ? tokens * ((steps + run - 1) / run) : heads) + 7) / 8;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-#define NKB_APPEND(D) \
-  return launch_pdl(pieces ? (qkv_partials ? append8_q8_kernel<D, true> : append8_q8_kernel<D, false>) : append_q8_kernel<D>, blocks, dim3(256), 0, s, p)
+  const dim3 grid = dim3(unsigned(blocks));
+#define NKB_APPEND(D)                                                                                                                 \
+  return pieces ? launch_pdl(qkv_partials ? append8_q8_kernel<D, true> : append8_q8_kernel<D, false>, grid, dim3(256), 0, s, p, int(run)) \
+                : launch_pdl(append_q8_kernel<D>, grid, dim3(256), 0, s, p)
   if (head_dim == 128) NKB_APPEND(128);
   if (head_dim == 64) NKB_APPEND(64);
 #undef NKB_APPEND
