@@ -167,6 +167,11 @@ int nkb_q8_attn_decode(const void* q, const void* k_values, const void* k_scales
                        const int* block_table, const int* context_lens, void* out, float* scratch, int batch, int q_len, int nq, int nkv,
                        int head_dim, int num_blocks, int table_width, long long table_stride, float scale, int window, int chunk,
                        const float* sinks, int num_splits, void* stream);
+int nkb_q8_step(const float* qkv_partials, int splits, long long split_stride, const void* bias, const int* positions, const int* slots,
+                const float* cos_sin, const void* q_norm_w, const void* k_norm_w, double eps, void* queries, void* k_values, void* k_scales,
+                void* v_values, void* v_scales, const int* block_table, const int* context_lens, void* out, float* scratch, int batch,
+                int nq, int nkv, int head_dim, int max_pos, int num_blocks, int table_width, long long table_stride, float scale, int window,
+                const float* sinks, int num_splits, void* stream);
 int nkb_decode_advance(int* context_lens, const int* block_table, int* positions, int* slots, int batch, int q_len,
                        int max_blocks, int block_size, void* stream);
 // Positions and cache slots of the tokens of a packed step (sequences one behind another without gaps, each with its row of the table).

@@ -44,6 +44,9 @@ struct DecodeQ8Params {
   int* status;
   int batch, q_len, nq, nkv, group, table_width, window, chunk;
   int units;
+  // The kernel before writes queries and the newest token's page (at position context - 1) and nothing else that is read here: the other pages
+  // are fetched without waiting for it.
+  int early;
   long long table_stride;
   float scale_log2;
   __device__ __forceinline__ int context(int b) const { return min(context_lens[b], table_width * kPage); }
@@ -106,10 +109,12 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
     tma_prefetch_desc(&tmVS);
   }
   __syncthreads();
-  griddep_wait();
-  griddep_launch();
+  if (!p.early) {
+    griddep_wait();
+    griddep_launch();
+  }
   PagePlan plan{int(blockIdx.z), 0, 1, 0x3fffffff};
-  if (p.units && !plan_pages<false>(p, blockIdx.x, 2 * W, lane, plan)) return;
+  if (p.units && !plan_pages<false>(p, blockIdx.x, 2 * W, lane, plan)) return;     // (a grid waits for the one before until its last CTA ends)
   const int b = plan.b, split = plan.split, ctx = p.context(b);
   int page_lo, kept;
   const int npages = pages_of<false>(p, ctx, page_lo, kept);
@@ -137,9 +142,17 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
     const int pg = p0 + warp + s * W;
     blks[s] = pg < p1 ? table[pg] : 0;
   }
+  const int late = p.early ? (ctx - 1) / kPage : -1;      // the page that has to wait
 #pragma unroll
   for (int s = 0; s < kQ8Stages; ++s)
-    if (p0 + warp + s * W < p1) issue(blks[s], s);
+    if (p0 + warp + s * W < p1 && p0 + warp + s * W != late) issue(blks[s], s);
+  if (p.early) {
+    griddep_wait();
+    griddep_launch();
+#pragma unroll
+    for (int s = 0; s < kQ8Stages; ++s)
+      if (p0 + warp + s * W < p1 && p0 + warp + s * W == late) issue(blks[s], s);
+  }
 
   // ---- query fragments (the first pages are on their way): lane (g, t) has columns 16 ks + 4 t ... of row g, as the keys come.
   // rs: raw score -> exponent of two, without the key's factor, of rows 2 t and 2 t + 1
@@ -503,12 +516,10 @@ extern "C" long long nkb_q8_attn_decode_scratch_floats(int batch, int nkv, int h
   return kQ8Counters + (long long)plan_units(batch, nkv, group, num_splits) * nkv * (16 * head_dim + 32);
 }
 
-// At most 16 query rows per kv head (q_len * nq / nkv).  num_splits > 1: scratch as large as the function above says, its first kQ8Counters
-// words zero before the first call (a call leaves them at zero).
-extern "C" int nkb_q8_attn_decode(const void* q, const void* k_values, const void* k_scales, const void* v_values, const void* v_scales,
-                                  const int* block_table, const int* context_lens, void* out, float* scratch, int batch, int q_len, int nq,
-                                  int nkv, int head_dim, int num_blocks, int table_width, long long table_stride, float scale, int window,
-                                  int chunk, const float* sinks, int num_splits, void* stream) {
+static int attn_q8_decode(const void* q, const void* k_values, const void* k_scales, const void* v_values, const void* v_scales,
+                          const int* block_table, const int* context_lens, void* out, float* scratch, int batch, int q_len, int nq, int nkv,
+                          int head_dim, int num_blocks, int table_width, long long table_stride, float scale, int window, int chunk,
+                          const float* sinks, int num_splits, int early, void* stream) {
   if (batch <= 0) return 0;
   if (nkv < 1 || nq % nkv || q_len * (nq / nkv) > 16 || nkv > 65535 || batch > 65535) return -2;
   if (num_splits > 1 && (!scratch || (long long)batch * nkv > kQ8Counters)) return -2;
@@ -522,7 +533,7 @@ extern "C" int nkb_q8_attn_decode(const void* q, const void* k_values, const voi
   p.sinks = sinks;
   p.status = status_word();
   p.batch = batch; p.q_len = q_len; p.nq = nq; p.nkv = nkv; p.group = nq / nkv; p.table_width = table_width;
-  p.window = window; p.chunk = chunk;
+  p.window = window; p.chunk = chunk; p.early = early;
   p.units = plan_units(batch, nkv, p.group, num_splits);
   p.table_stride = table_stride;
   p.scale_log2 = scale * 1.4426950408889634f;
@@ -533,4 +544,31 @@ extern "C" int nkb_q8_attn_decode(const void* q, const void* k_values, const voi
   if (head_dim == 128) return eight ? dispatch_decode_q8<128, 1>(m, p, s) : dispatch_decode_q8<128, 2>(m, p, s);
   if (head_dim == 64) return eight ? dispatch_decode_q8<64, 1>(m, p, s) : dispatch_decode_q8<64, 2>(m, p, s);
   return -2;
+}
+
+// At most 16 query rows per kv head (q_len * nq / nkv).  num_splits > 1: scratch as large as the function above says, its first kQ8Counters
+// words zero before the first call (a call leaves them at zero).
+extern "C" int nkb_q8_attn_decode(const void* q, const void* k_values, const void* k_scales, const void* v_values, const void* v_scales,
+                                  const int* block_table, const int* context_lens, void* out, float* scratch, int batch, int q_len, int nq,
+                                  int nkv, int head_dim, int num_blocks, int table_width, long long table_stride, float scale, int window,
+                                  int chunk, const float* sinks, int num_splits, void* stream) {
+  return attn_q8_decode(q, k_values, k_scales, v_values, v_scales, block_table, context_lens, out, scratch, batch, q_len, nq, nkv, head_dim,
+                        num_blocks, table_width, table_stride, scale, window, chunk, sinks, num_splits, 0, stream);
+}
+
+// One new token per sequence, from split-K partials [splits][batch][(nq + 2 nkv) * head_dim]: nkb_q8_append and, behind it, attention that
+// fetches all pages but the new token's while the append runs.  slots[b]: the place of position context_lens[b] - 1 (negative: none).
+// queries: batch * nq * head_dim bf16 values for the rotated queries.
+extern "C" int nkb_q8_step(const float* qkv_partials, int splits, long long split_stride, const void* bias, const int* positions,
+                           const int* slots, const float* cos_sin, const void* q_norm_w, const void* k_norm_w, double eps, void* queries,
+                           void* k_values, void* k_scales, void* v_values, void* v_scales, const int* block_table, const int* context_lens,
+                           void* out, float* scratch, int batch, int nq, int nkv, int head_dim, int max_pos, int num_blocks,
+                           int table_width, long long table_stride, float scale, int window, const float* sinks, int num_splits,
+                           void* stream) {
+  if (nkv < 1 || nq % nkv || nq / nkv > 16) return -2;
+  if (int rc = nkb_q8_append(nullptr, qkv_partials, splits, split_stride, bias, positions, slots, cos_sin, q_norm_w, k_norm_w, eps, queries,
+                             k_values, k_scales, v_values, v_scales, batch, nq, nkv, head_dim, max_pos, num_blocks, stream))
+    return rc;
+  return attn_q8_decode(queries, k_values, k_scales, v_values, v_scales, block_table, context_lens, out, scratch, batch, 1, nq, nkv, head_dim,
+                        num_blocks, table_width, table_stride, scale, window, 0, sinks, num_splits, pdl_enabled() ? 1 : 0, stream);
 }

@@ -194,6 +194,8 @@ _SIGNATURES = {
     ),
     "nkb_q8_append": (c_int, [_P, _P, c_int, c_longlong, _P, _P, _P, _P, _P, _P, c_double, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int,
                               c_int, c_int, _P]),
+    "nkb_q8_step": (c_int, [_P, c_int, c_longlong, _P, _P, _P, _P, _P, _P, c_double, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int,
+                            c_int, c_int, c_int, c_int, c_longlong, c_float, c_int, _P, c_int, _P]),
     "nkb_q8_attn_prefill": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                                    c_longlong, c_float, c_int, c_int, c_int, _P, _P, _P]),
     "nkb_q8_attn_decode_scratch_floats": (c_longlong, [c_int, c_int, c_int, c_int, c_int]),

@@ -33,7 +33,7 @@ DIMS = (64, 128)
 class QuantizedPages:
     """Keys or values of one layer: e4m3 `values` [blocks, kv heads, 32, dim] and power-of-two `scales` [blocks, kv heads, 32]
     (torch.float8_e8m0fnu), both contiguous and on one device."""
-    __slots__ = ("values", "scales", "shape", "device", "is_cuda")
+    __slots__ = ("values", "scales", "shape", "device", "is_cuda", "at")
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor):
         if values.dtype is not torch.float8_e4m3fn or scales.dtype is not torch.float8_e8m0fnu:
@@ -44,7 +44,8 @@ class QuantizedPages:
             raise ValueError("QuantizedPages has heads of 64 or 128 columns")
         if not values.is_contiguous() or not scales.is_contiguous() or values.device != scales.device:
             raise ValueError("QuantizedPages wants contiguous tensors on one device")
-        if (values.data_ptr() | scales.data_ptr()) & 15:
+        self.at = v, s = values.data_ptr(), scales.data_ptr()
+        if (v | s) & 15:
             raise ValueError("QuantizedPages wants tensors that start on 16 bytes")
         self.values, self.scales = values, scales
         self.shape, self.device, self.is_cuda = values.shape, values.device, values.is_cuda
@@ -269,6 +270,19 @@ def _pick_splits(ctas: int, max_pages: int, sms: int = 148) -> int:
     return 1 if ctas >= sms else max(min(sms // ctas, max(max_pages // 8, 1), 16), 1)
 
 
+def _splits(num_splits: int, scratch, B: int, nkv: int, D: int, group: int, max_pages: int, device):
+    """(parts of a sequence, scratch for their results)."""
+    if num_splits <= 0:
+        num_splits = _pick_splits(B * nkv, max_pages)
+    if num_splits > 1:
+        need = _lib.lib().nkb_q8_attn_decode_scratch_floats(B, nkv, D, group, num_splits)
+        if scratch is None:
+            scratch = _scratch(device, need)
+        elif scratch.dtype is not torch.float32 or scratch.numel() < need or scratch.device != device or not scratch.is_contiguous():
+            raise ValueError(f"scratch wants {need} contiguous fp32 values on {device}, the first {COUNTERS} zero before the first call")
+    return num_splits, scratch
+
+
 def decode_scratch(pages: QuantizedPages, nq: int, max_batch: int, max_pages: int) -> Optional[torch.Tensor]:
     """Scratch for every decode attention of up to max_batch sequences of max_pages pages, for a caller that keeps its own: steps that
     are captured into a graph share it, one behind another.  None on the CPU."""
@@ -295,9 +309,10 @@ def rope_kv_append(qkv, positions, slots, cos_sin, k_cache, v_cache, nq, nkv, he
     at = qkv.data_ptr()
     rc = _lib.lib().nkb_q8_append(
         None if partial else at, at if partial else None, splits, stride, _p(bias), _p(positions), _p(slots), _p(cos_sin), _p(q_norm_w),
-        _p(k_norm_w), float(norm_eps), q_out.data_ptr(), k_cache.values.data_ptr(), k_cache.scales.data_ptr(), v_cache.values.data_ptr(),
-        v_cache.scales.data_ptr(), T, nq, nkv, head_dim, 0 if cos_sin is None else cos_sin.shape[0], blocks, _stream())
-    _lib.check(rc, "nkb_q8_append")
+        _p(k_norm_w), norm_eps, q_out.data_ptr(), *k_cache.at, *v_cache.at, T, nq, nkv, head_dim,
+        0 if cos_sin is None else cos_sin.shape[0], blocks, _stream())
+    if rc:
+        _lib.check(rc, "nkb_q8_append")
     _count_launch()
     return q_out
 
@@ -328,20 +343,12 @@ def paged_attn_decode(q, k_cache, v_cache, block_table, context_lens, scale, *, 
         q_start = torch.arange(0, B * q_len, q_len, device=dev, dtype=torch.int32)
         return flash_attn_prefill(q, k_cache, v_cache, block_table, q_start, torch.full_like(q_start, q_len), context_lens, scale,
                                   max_q_len=q_len, window=window, chunk=chunk, sinks=sinks, out=out)
-    L = _lib.lib()
-    if num_splits <= 0:
-        num_splits = _pick_splits(B * nkv, block_table.shape[1])
-    if num_splits > 1:
-        need = L.nkb_q8_attn_decode_scratch_floats(B, nkv, D, group, num_splits)
-        if scratch is None:
-            scratch = _scratch(dev, need)
-        elif scratch.dtype is not torch.float32 or scratch.numel() < need or scratch.device != dev or not scratch.is_contiguous():
-            raise ValueError(f"scratch wants {need} contiguous fp32 values on {dev}, the first {COUNTERS} zero before the first call")
-    rc = L.nkb_q8_attn_decode(
-        q.data_ptr(), k_cache.values.data_ptr(), k_cache.scales.data_ptr(), v_cache.values.data_ptr(), v_cache.scales.data_ptr(),
-        block_table.data_ptr(), context_lens.data_ptr(), out.data_ptr(), _p(scratch), B, q_len, nq, nkv, D, blocks,
-        block_table.shape[1], block_table.stride(0), float(scale), int(window), int(chunk), _p(sinks), num_splits, _stream())
-    _lib.check(rc, "nkb_q8_attn_decode")
+    num_splits, scratch = _splits(num_splits, scratch, B, nkv, D, group, block_table.shape[1], dev)
+    rc = _lib.lib().nkb_q8_attn_decode(
+        q.data_ptr(), *k_cache.at, *v_cache.at, block_table.data_ptr(), context_lens.data_ptr(), out.data_ptr(), _p(scratch), B, q_len, nq,
+        nkv, D, blocks, block_table.shape[1], block_table.stride(0), scale, window, chunk, _p(sinks), num_splits, _stream())
+    if rc:
+        _lib.check(rc, "nkb_q8_attn_decode")
     _count_launch()
     return out
 
@@ -349,15 +356,34 @@ def paged_attn_decode(q, k_cache, v_cache, block_table, context_lens, scale, *, 
 def rope_attn_decode(qkv_partials, positions, slots, cos_sin, k_cache, v_cache, block_table, context_lens, scale, nq, nkv, *, bias=None,
                      q_norm_w=None, k_norm_w=None, norm_eps=1e-6, window=0, sinks=None, num_splits=0, scratch=None,
                      out=None) -> torch.Tensor:
-    """`ops.rope_attn_decode` over quantised pages.  The new token takes part as it is kept, in 8 bits, so that a step has the
-    result of `rope_kv_append` and `paged_attn_decode`."""
-    _pair(k_cache, v_cache)
+    """`ops.rope_attn_decode` over quantised pages: `rope_kv_append`, and attention that fetches the older pages meanwhile.  The new token
+    takes part as it is kept, in 8 bits.  slots[b] is the place of sequence b's position context_lens[b] - 1, or negative."""
+    blocks, _, D = _pair(k_cache, v_cache)
     if qkv_partials.dtype is not torch.float32 or qkv_partials.shape[-2] != block_table.shape[0]:
         raise ValueError("rope_attn_decode wants fp32 partials [S, B, W], one token per sequence")
-    q = rope_kv_append(qkv_partials, positions, slots, cos_sin, k_cache, v_cache, nq, nkv, k_cache.shape[3], bias=bias, q_norm_w=q_norm_w,
-                       k_norm_w=k_norm_w, norm_eps=norm_eps)
-    return paged_attn_decode(q, k_cache, v_cache, block_table, context_lens, scale, window=window, sinks=sinks, num_splits=num_splits,
-                             scratch=scratch, out=out)
+    dev = k_cache.device
+    B = _check_table(block_table, context_lens, dev)
+    group = nq // nkv if nkv > 0 else 0
+    if not k_cache.is_cuda or group > 16 or not B:
+        q = rope_kv_append(qkv_partials, positions, slots, cos_sin, k_cache, v_cache, nq, nkv, D, bias=bias, q_norm_w=q_norm_w,
+                           k_norm_w=k_norm_w, norm_eps=norm_eps)
+        return paged_attn_decode(q, k_cache, v_cache, block_table, context_lens, scale, window=window, sinks=sinks, num_splits=num_splits,
+                                 scratch=scratch, out=out)
+    _check_qkv(qkv_partials, positions, slots, cos_sin, k_cache, nq, nkv, D, bias, q_norm_w, k_norm_w)
+    _check_masks(None, window, 0, sinks, nq, dev)
+    out = _result(out, (B, nq * D), dev)
+    _check_device(k_cache)
+    num_splits, scratch = _splits(num_splits, scratch, B, nkv, D, group, block_table.shape[1], dev)
+    splits, stride = (qkv_partials.shape[0], qkv_partials.stride(0)) if qkv_partials.dim() == 3 else (1, 0)
+    rc = _lib.lib().nkb_q8_step(
+        qkv_partials.data_ptr(), splits, stride, _p(bias), _p(positions), _p(slots), _p(cos_sin), _p(q_norm_w), _p(k_norm_w), norm_eps,
+        torch.empty_like(out).data_ptr(), *k_cache.at, *v_cache.at, block_table.data_ptr(), context_lens.data_ptr(), out.data_ptr(), _p(scratch),
+        B, nq, nkv, D, 0 if cos_sin is None else cos_sin.shape[0], blocks, block_table.shape[1], block_table.stride(0), scale, window,
+        _p(sinks), num_splits, _stream())
+    if rc:
+        _lib.check(rc, "nkb_q8_step")
+    _count_launch(2)
+    return out
 
 
 def flash_attn_prefill(q, k_cache, v_cache, block_table, q_start, q_lens, context_lens, scale, *, max_q_len, causal=True, window=0,
@@ -386,11 +412,11 @@ def flash_attn_prefill(q, k_cache, v_cache, block_table, q_start, q_lens, contex
                                              sinks)
         return out
     rc = _lib.lib().nkb_q8_attn_prefill(
-        q.data_ptr(), k_cache.values.data_ptr(), k_cache.scales.data_ptr(), v_cache.values.data_ptr(), v_cache.scales.data_ptr(),
-        block_table.data_ptr(), q_start.data_ptr(), q_lens.data_ptr(), context_lens.data_ptr(), out.data_ptr(), B, q.shape[0],
-        int(max_q_len), nq, nkv, D, blocks, block_table.shape[1], block_table.stride(0), float(scale), 1 if causal else 0, int(window),
-        int(chunk), _p(sinks), _scratch(dev, COUNTERS).data_ptr(), _stream())
-    _lib.check(rc, "nkb_q8_attn_prefill")
+        q.data_ptr(), *k_cache.at, *v_cache.at, block_table.data_ptr(), q_start.data_ptr(), q_lens.data_ptr(), context_lens.data_ptr(),
+        out.data_ptr(), B, q.shape[0], max_q_len, nq, nkv, D, blocks, block_table.shape[1], block_table.stride(0), scale,
+        1 if causal else 0, window, chunk, _p(sinks), _scratch(dev, COUNTERS).data_ptr(), _stream())
+    if rc:
+        _lib.check(rc, "nkb_q8_attn_prefill")
     _count_launch()
     return out
 
