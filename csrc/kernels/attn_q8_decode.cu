@@ -45,7 +45,8 @@ struct DecodeQ8Params {
   int batch, q_len, nq, nkv, group, table_width, window, chunk;
   int units;
   // The kernel before writes queries and the newest token's page (at position context - 1) and nothing else that is read here: the other pages
-  // are fetched without waiting for it.
+  // are fetched without waiting for it.  Append and attention, us: 64 sequences of 1024 29.2 -> 28.2, 7 of 3500 to 7000 27.5 -> 24.9, 128 of 512
+  // on 4 heads 21.1 -> 19.1, one of 203 7.1 -> 6.4.
   int early;
   long long table_stride;
   float scale_log2;
@@ -115,11 +116,30 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
   }
   PagePlan plan{int(blockIdx.z), 0, 1, 0x3fffffff};
   if (p.units && !plan_pages<false>(p, blockIdx.x, 2 * W, lane, plan)) return;     // (a grid waits for the one before until its last CTA ends)
-  const int b = plan.b, split = plan.split, ctx = p.context(b);
+  const int b = plan.b, split = plan.split;
+  // what does not depend on the context's length is on its way beside it
+  uint2 q_raw[NT][D / 16];
+  auto load_q = [&]() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = nt * 8 + g;
+      const __nv_bfloat16* src = p.q + (((long long)b * p.q_len + r / p.group) * p.nq + kvh * p.group + r % p.group) * D + 4 * t;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) q_raw[nt][ks] = r < rows ? *reinterpret_cast<const uint2*>(src + 16 * ks) : make_uint2(0u, 0u);
+    }
+  };
+  const int* table = p.block_table + b * p.table_stride;
+  const bool from_start = !p.units && p.window == 0 && p.chunk == 0;     // this CTA's pages begin with the first
+  int blks[kQ8Stages];
+  if (from_start) {
+#pragma unroll
+    for (int s = 0; s < kQ8Stages; ++s) blks[s] = table[min(warp + s * W, p.table_width - 1)];
+  }
+  if (!p.early) load_q();
+  const int ctx = p.context(b);
   int page_lo, kept;
   const int npages = pages_of<false>(p, ctx, page_lo, kept);
   const int p0 = page_lo + split * (plan.splits > 1 ? plan.per : 0), p1 = min(page_lo + npages, p0 + plan.per);
-  const int* table = p.block_table + b * p.table_stride;
 
   uint8_t* my_ring = smem + warp * kQ8Stages * L::kStage;
   uint8_t* my_scales = smem + L::kScaleAt + warp * kQ8Stages * L::kScales;
@@ -136,11 +156,9 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
       tma_load_3d_as(my_scales + stage * L::kScales + 128, &tmVS, bar, 0, kvh, blk, policy);
     }
   };
-  int blks[kQ8Stages];
+  if (!from_start) {
 #pragma unroll
-  for (int s = 0; s < kQ8Stages; ++s) {
-    const int pg = p0 + warp + s * W;
-    blks[s] = pg < p1 ? table[pg] : 0;
+    for (int s = 0; s < kQ8Stages; ++s) blks[s] = p0 + warp + s * W < p1 ? table[p0 + warp + s * W] : 0;
   }
   const int late = p.early ? (ctx - 1) / kPage : -1;      // the page that has to wait
 #pragma unroll
@@ -152,6 +170,7 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
 #pragma unroll
     for (int s = 0; s < kQ8Stages; ++s)
       if (p0 + warp + s * W < p1 && p0 + warp + s * W == late) issue(blks[s], s);
+    load_q();
   }
 
   // ---- query fragments (the first pages are on their way): lane (g, t) has columns 16 ks + 4 t ... of row g, as the keys come.
@@ -161,13 +180,10 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
   int pos[NT][2], low[NT][2];            // last and first visible position
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int r = nt * 8 + g;
-    const __nv_bfloat16* src = p.q + (((long long)b * p.q_len + r / p.group) * p.nq + kvh * p.group + r % p.group) * D + 4 * t;
-    uint2 v[D / 16];
+    const uint2(&v)[D / 16] = q_raw[nt];
     float mx = 0.f;
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
-      v[ks] = r < rows ? *reinterpret_cast<const uint2*>(src + 16 * ks) : make_uint2(0u, 0u);
       const float2 x = unpack_bf16x2(v[ks].x), y = unpack_bf16x2(v[ks].y);
       mx = fmaxf(fmaxf(fmaxf(mx, fabsf(x.x)), fmaxf(fabsf(x.y), fabsf(y.x))), fabsf(y.y));
     }
