@@ -157,11 +157,12 @@ int nkb_q8_append(const void* qkv_bf16, const float* qkv_partials, int splits, l
                   const int* positions, const int* slots, const float* cos_sin, const void* q_norm_w, const void* k_norm_w, double eps,
                   void* q_out, void* k_values, void* k_scales, void* v_values, void* v_scales, int tokens, int nq, int nkv, int head_dim,
                   int max_pos, int num_blocks, void* stream);
+long long nkb_q8_attn_prefill_scratch_floats(int batch, int max_q_len, int nq, int nkv, int head_dim, int table_width);
 int nkb_q8_attn_prefill(const void* q, const void* k_values, const void* k_scales, const void* v_values, const void* v_scales,
                        const int* block_table, const int* q_start, const int* q_lens, const int* context_lens, void* out, int batch,
                        int total_q, int max_q_len, int nq, int nkv, int head_dim, int num_blocks, int table_width, long long table_stride,
                        float scale, int causal, int window, int chunk, const float* sinks,
-                       unsigned int* sched, void* stream);
+                       float* scratch, void* stream);
 long long nkb_q8_attn_decode_scratch_floats(int batch, int nkv, int head_dim, int group, int num_splits);
 int nkb_q8_attn_decode(const void* q, const void* k_values, const void* k_scales, const void* v_values, const void* v_scales,
                        const int* block_table, const int* context_lens, void* out, float* scratch, int batch, int q_len, int nq, int nkv,

@@ -51,6 +51,8 @@ struct PrefillQ8Params {
   long long table_stride;
   float scale_log2;
   unsigned int* sched;                   // [0] works taken, [1] CTAs done; zero between calls
+  int parts;                             // of a block's tiles, each a work of its own
+  float* partials;                       // their results: [block][part][256 rows of D columns, then maxima, then sums]
 };
 
 // Piece of work of a CTA: 256 rows of a sequence's kv head
@@ -58,12 +60,14 @@ struct P8Range {                         // tiles [lo, hi) that a query tile att
   int lo, hi, rows;
 };
 struct P8Work {
-  int b, kvh, q_len, ctx, row0;          // b < 0: none
+  int b, kvh, q_len, ctx, row0, q_start; // b < 0: none
+  int block, part;
   int u_lo, n_union;                     // tiles that either query tile attends to
   P8Range tr0, tr1;
   // tiles whose exponentials the two take turns with
   __device__ __forceinline__ int paired() const { return tr1.rows > 0 ? min(tr0.hi - tr0.lo, tr1.hi - tr1.lo) : 0; }
 };
+constexpr int kP8Counters = 16384;       // words ahead of the partial results (the scratch of decode attention has as many)
 constexpr int kP8Works = 3;              // works ahead of their use
 constexpr int kP8Readers = 15;           // warps 0 to 14 read them
 
@@ -109,11 +113,14 @@ __device__ __forceinline__ P8Range p8_range(const PrefillQ8Params& p, int row0, 
   return r;
 }
 // Rows row0 .. of sequence b and kv head kvh; false: there are none
-__device__ __forceinline__ bool p8_work(const PrefillQ8Params& p, int b, int kvh, int row0, P8Work& o) {
+__device__ __forceinline__ bool p8_work(const PrefillQ8Params& p, int b, int kvh, int row0, int part, P8Work& o) {
   o.b = b;
   o.kvh = kvh;
   o.row0 = row0;
+  o.part = part;
+  o.block = (row0 / (2 * kP8Tile) * p.batch + b) * p.nkv + kvh;
   o.q_len = p.q_lens[b];
+  o.q_start = p.q_start[b];
   o.ctx = min(p.context_lens[b], p.table_width * kQ8Page);
   if (row0 >= (long long)o.q_len * p.group) return false;
   const int all_rows = o.q_len * p.group;
@@ -121,6 +128,15 @@ __device__ __forceinline__ bool p8_work(const PrefillQ8Params& p, int b, int kvh
   o.tr1 = p8_range(p, row0 + kP8Tile, all_rows, o.q_len, o.ctx);
   o.u_lo = o.tr0.lo;
   o.n_union = (o.tr1.rows > 0 ? max(o.tr0.hi, o.tr1.hi) : o.tr0.hi) - o.u_lo;
+  if (p.parts > 1) {
+    const int lo = o.u_lo + o.n_union * part / p.parts, hi = o.u_lo + o.n_union * (part + 1) / p.parts;
+    for (P8Range* r : {&o.tr0, &o.tr1}) {
+      r->lo = max(r->lo, lo);
+      r->hi = max(min(r->hi, hi), r->lo);
+    }
+    o.u_lo = lo;
+    o.n_union = hi - lo;
+  }
   return true;
 }
 // The next work for a warp or (one = true) a single thread; n counts them.  False: there are no more, or the wait has run out.
@@ -149,6 +165,17 @@ __device__ __forceinline__ int p8_block(const PrefillQ8Params& p, const P8Work& 
 // Ring items of a work in the order the issuers take them: K(0), then K(u + 1), V(u)
 __device__ __forceinline__ bool p8_is_v(int i, int items) { return i > 0 && ((i & 1) == 0 || i == items - 1); }
 __device__ __forceinline__ int p8_tile(int i, int items) { return i == 0 ? 0 : ((i & 1) == 0 ? i / 2 - 1 : min((i + 1) / 2, items / 2 - 1)); }
+
+// What a row's sum of weighted values is multiplied by, from the exponent m of its weights and their sum (values are larger by 2^lift)
+__device__ __forceinline__ float p8_inverse(const PrefillQ8Params& p, int head, float m, float l) {
+  float scale = exp2f(-kP8Lift);
+  if (p.sinks) {
+    const float sk = p.sinks[head] * 1.4426950408889634f, m2 = fmaxf(m, sk), keep = m == -INFINITY ? 0.f : exp2f(m - m2);
+    scale *= keep;
+    l = l * keep + exp2f(sk - m2 + kP8Lift);
+  }
+  return l == 0.f ? 0.f : scale / l;
+}
 
 template <int D>
 struct PrefillQ8Smem {
@@ -332,26 +359,27 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 15) {
       // -------------------------------------------------------------- pages: lanes 0 to 3 a page of the item each
-      // and the works, taken from a counter of the grid: the last rows of all sequences first, those with the longest contexts ahead
-      const int across = p.nkv * p.batch;
+      // and the works: a CTA's first has its number, the others come from a counter of the grid.  The last rows of all sequences first, those
+      // with the longest contexts ahead.
+      const int across = p.nkv * p.batch * p.parts;
       int order = lane;                                   // (up to 32 sequences) the sequence of rank `lane`
-      if (p.batch <= 32) {
+      if (p.batch > 1 && p.batch <= 32) {
         const int ctx = lane < p.batch ? p.context_lens[lane] : INT_MIN;
         int rank = 0;
-        for (int j = 0; j < 32; ++j) {
+        for (int j = 0; j < p.batch; ++j) {
           const int c = __shfl_sync(kAll, ctx, j);
           rank += c > ctx || (c == ctx && j < lane);
         }
-        for (int j = 0; j < 32; ++j)
+        for (int j = 0; j < p.batch; ++j)
           if (__shfl_sync(kAll, rank, j) == lane) order = j;
       }
       auto take = [&]() {
         unsigned int w = 0;
-        if (lane == 0) w = atomicAdd(p.sched, 1u);
+        if (lane == 0) w = gridDim.x + atomicAdd(p.sched, 1u);
         return w;
       };
       uint32_t item0 = 0, n_works = 0;
-      unsigned int taken = take();
+      unsigned int taken = blockIdx.x;
       bool alive = true;
       P8Work k;
 #pragma unroll 1
@@ -360,12 +388,15 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
         k.b = -1;
         k.n_union = 0;
         if (level < unsigned(p.q_blocks)) {
-          const int rest = int(w % across), b = rest / p.nkv;
-          if (!p8_work(p, p.batch <= 32 ? __shfl_sync(kAll, order, b & 31) : b, rest % p.nkv, (p.q_blocks - 1 - int(level)) * 2 * kP8Tile, k)) {
+          const int rest = int(w % across), head = rest / p.parts, b = head / p.nkv;
+          if (!p8_work(p, p.batch <= 32 ? __shfl_sync(kAll, order, b & 31) : b, head % p.nkv, (p.q_blocks - 1 - int(level)) * 2 * kP8Tile,
+                       rest % p.parts, k)) {
             taken = take();
             continue;
           }
         }
+        const int items = 2 * k.n_union;
+        int blk = items > 0 && lane < 4 ? p8_block(p, k, 0, lane) : -1;
         const bool free_slot = p8_wait(&ctrl->w_empty[n_works % kP8Works], (n_works / kP8Works & 1u) ^ 1u, abort_flag, p.status, ERR_WAIT_SMEM_EMPTY);
         if (!__all_sync(kAll, free_slot)) break;
         if (lane == 0) {
@@ -375,8 +406,6 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
         __syncwarp();
         ++n_works;
         if (k.b < 0) break;
-        const int items = 2 * k.n_union;
-        int blk = lane < 4 ? p8_block(p, k, 0, lane) : -1;
 #pragma unroll 1
         for (int i = 0; i < items; ++i, ++item0) {
           if (i == max(items - 3, 0)) taken = take();     // late, so that works go to who is free, and early enough to be there
@@ -562,6 +591,7 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
     struct Row {
       int tile_lo, n_tiles, lo_pos, hi_pos, head, x0;     // x0: walk position of its first tile
       int paired;                                         // tiles whose exponentials the two query tiles take turns with
+      int block, part;
       long long at;                                       // row of q and out (of heads), < 0: none
       float raw_log2;                                     // raw score -> exponent of two, without 2^K
       uint32_t tiles0;                                    // tiles of the works before
@@ -685,13 +715,15 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
         if (tr.rows == 0) continue;                       // (a work's second query tile may have none)
         more = true;
         const int row = k.row0 + t * kP8Tile + r, token = row / p.group;
-        const long long q_row = (long long)p.q_start[k.b] + token;
+        const long long q_row = (long long)k.q_start + token;
         next.head = k.kvh * p.group + row % p.group;
         next.at = r < tr.rows && q_row >= 0 && q_row < p.total_q ? q_row * p.nq + next.head : -1;
         next.tile_lo = tr.lo;
         next.x0 = tr.lo - k.u_lo;
         next.n_tiles = tr.hi - tr.lo;
         next.paired = k.paired();
+        next.block = k.block;
+        next.part = k.part;
         const int q_pos = k.ctx - k.q_len + token;
         next.hi_pos = p.causal ? min(k.ctx - 1, q_pos) : k.ctx - 1;
         next.lo_pos = nkb_first_visible(q_pos, p.window, p.chunk);
@@ -737,41 +769,44 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
           alive = have_o;
           if (have_o) tc_fence_after();
         }
-        float osc = exp2f(-kP8Lift);                      // what values are larger by
-        if (p.sinks) {
-          const float sk = p.sinks[cur.head] * 1.4426950408889634f, m2 = fmaxf(m, sk), keep = m == -INFINITY ? 0.f : exp2f(m - m2);
-          osc *= keep;
-          l = l * keep + exp2f(sk - m2 + kP8Lift);
-        }
-        const float inv = l == 0.f ? 0.f : osc / l;
-        __nv_bfloat16* dst = p.out + cur.at * D;
+        const bool whole = p.parts == 1;
+        const float inv = whole ? p8_inverse(p, cur.head, m, l) : 0.f;
         const bool store = cur.at >= 0 && !*abort_flag;
+        constexpr long long kPart = 2 * kP8Tile * (D + 2);
+        float* first = p.partials + (long long)cur.block * p.parts * kPart;
+        float* mine = first + cur.part * kPart + (t * kP8Tile + r) * D;
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
+          float o[32];
           if (have_o) {
-            tmem_ld_32x32(o_addr + c * 32, o);
+            tmem_ld_32x32(o_addr + c * 32, reinterpret_cast<uint32_t(&)[32]>(o));
             tmem_ld_wait();
           } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = 0u;
+            for (int i = 0; i < 32; ++i) o[i] = 0.f;
           }
-          if (store) {
+          if (whole) {
+            if (store) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              uint4 x;
-              x.x = pack_bf16x2(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
-              x.y = pack_bf16x2(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
-              x.z = pack_bf16x2(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
-              x.w = pack_bf16x2(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
-              *reinterpret_cast<uint4*>(dst + c * 32 + i) = x;
+              for (int i = 0; i < 32; i += 8)
+                *reinterpret_cast<uint4*>(p.out + cur.at * D + c * 32 + i) =
+                    make_uint4(pack_bf16x2(o[i] * inv, o[i + 1] * inv), pack_bf16x2(o[i + 2] * inv, o[i + 3] * inv),
+                               pack_bf16x2(o[i + 4] * inv, o[i + 5] * inv), pack_bf16x2(o[i + 6] * inv, o[i + 7] * inv));
             }
+          } else if (have_o) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(mine + c * 32 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
           }
         }
         if (have_o) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&ctrl->o_empty[t]);
+        }
+        if (!whole) {
+          float* tail = first + cur.part * kPart + 2 * kP8Tile * D + t * kP8Tile + r;
+          tail[0] = have_o ? m : -INFINITY;
+          tail[2 * kP8Tile] = have_o ? l : 0.f;
         }
         done += cur.n_tiles;
         pairs += cur.paired;
@@ -800,6 +835,46 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
   }
 }
 
+// Puts the parts of divided blocks together: a warp per row, D / 32 columns a lane
+template <int D>
+__global__ void __launch_bounds__(256) attn_q8_join_kernel(const PrefillQ8Params p) {
+  constexpr int N = D / 32, kAhead = 4;
+  constexpr long long kPart = 2 * kP8Tile * (D + 2);
+  griddep_wait();
+  griddep_launch();
+  const int lane = threadIdx.x & 31, block = blockIdx.y, r = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int head_of = block % p.nkv, b = block / p.nkv % p.batch, row = block / (p.nkv * p.batch) * 2 * kP8Tile + r;
+  const int q_len = p.q_lens[b], token = row / p.group, head = head_of * p.group + row % p.group;
+  const long long q_row = (long long)p.q_start[b] + token;
+  if (token >= q_len || q_row < 0 || q_row >= p.total_q) return;
+  const float* first = p.partials + (long long)block * p.parts * kPart;
+  // lane = part
+  const float mine = lane < p.parts ? __ldcg(first + lane * kPart + 2 * kP8Tile * D + r) : -INFINITY;
+  const float sum = lane < p.parts ? __ldcg(first + lane * kPart + 2 * kP8Tile * (D + 1) + r) : 0.f;
+  const float m = warp_max(mine), weight = mine == m ? 1.f : exp2f(mine - m);
+  const uint32_t there = __ballot_sync(0xffffffffu, mine != -INFINITY || sum != 0.f);      // the others had no tile, or saw nothing
+  const float inv = p8_inverse(p, head, m, warp_sum(sum * weight));
+  float o[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) o[i] = 0.f;
+  for (int s0 = 0; s0 < p.parts; s0 += kAhead) {
+    float x[kAhead][N];
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[s][i] = there >> (s0 + s) & 1 ? __ldcg(first + (s0 + s) * kPart + r * D + i * 32 + lane) : 0.f;
+    }
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) {
+      const float w = __shfl_sync(0xffffffffu, weight, s0 + s);
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[i] = there >> (s0 + s) & 1 ? fmaf(w, x[s][i], o[i]) : o[i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) p.out[(q_row * p.nq + head) * D + i * 32 + lane] = __float2bfloat16(o[i] * inv);
+}
+
 template <int D>
 static int launch_prefill_q8(const PrefillQ8Params& p, cudaStream_t s) {
   using L = PrefillQ8Smem<D>;
@@ -814,20 +889,40 @@ static int launch_prefill_q8(const PrefillQ8Params& p, cudaStream_t s) {
     if (cudaError_t e = cudaFuncSetAttribute(attn_q8_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes)) return int(e);
     attr_set[dev] = true;
   }
-  const long long works = (long long)p.q_blocks * p.nkv * p.batch;
-  return launch_pdl(attn_q8_prefill_kernel<D>, dim3(unsigned(works < num_sms() ? works : num_sms())), dim3(kP8Threads), size_t(L::kBytes), s, p);
+  const long long works = (long long)p.q_blocks * p.nkv * p.batch * p.parts;
+  if (int rc = launch_pdl(attn_q8_prefill_kernel<D>, dim3(unsigned(works < num_sms() ? works : num_sms())), dim3(kP8Threads), size_t(L::kBytes), s, p))
+    return rc;
+  return p.parts == 1 ? 0 : launch_pdl(attn_q8_join_kernel<D>, dim3(2 * kP8Tile / 8, unsigned(works / p.parts)), dim3(256), 0, s, p);
 }
 
 }  // namespace nkb
 
 using namespace nkb;
 
-// sched: two words that are zero before the first call (a call leaves them at zero); not shared by calls that may run at the same time
+// How many works a block's tiles are divided into: where there are fewer blocks than half the SMs, and more than a few tiles that they may see
+static int p8_parts(long long blocks, int table_width) {
+  const long long fit = blocks > 0 ? num_sms() / blocks : 1, tiles = (table_width + 3) / 4;
+  const long long parts = fit < tiles / 4 ? fit : tiles / 4;
+  return int(parts < 2 ? 1 : (parts > 16 ? 16 : parts));
+}
+static long long p8_blocks(int batch, int max_q_len, int nq, int nkv) {
+  return ((long long)max_q_len * (nq / nkv) + 2 * kP8Tile - 1) / (2 * kP8Tile) * nkv * batch;
+}
+
+extern "C" long long nkb_q8_attn_prefill_scratch_floats(int batch, int max_q_len, int nq, int nkv, int head_dim, int table_width) {
+  if (batch <= 0 || nkv < 1 || max_q_len < 1 || (!status_word() && nkb_init() != 0)) return 0;
+  const long long blocks = p8_blocks(batch, max_q_len, nq, nkv);
+  const int parts = p8_parts(blocks, table_width);
+  return kP8Counters + (parts > 1 ? blocks * parts * 2 * kP8Tile * (head_dim + 2) : 0);
+}
+
+// scratch: as large as the function above says; its first kP8Counters words are zero before the first call (a call leaves them at zero); not
+// shared by calls that may run at the same time
 extern "C" int nkb_q8_attn_prefill(const void* q, const void* k_values, const void* k_scales, const void* v_values, const void* v_scales,
                                    const int* block_table, const int* q_start, const int* q_lens, const int* context_lens, void* out,
                                    int batch, int total_q, int max_q_len, int nq, int nkv, int head_dim, int num_blocks, int table_width,
                                    long long table_stride, float scale, int causal, int window, int chunk, const float* sinks,
-                                   unsigned int* sched, void* stream) {
+                                   float* scratch, void* stream) {
   if (batch <= 0 || total_q <= 0) return 0;
   if (batch > 65535 || nkv > 65535 || nkv < 1 || nq % nkv || max_q_len < 1) return -2;
   if (!status_word() && nkb_init() != 0) return -1;
@@ -839,10 +934,12 @@ extern "C" int nkb_q8_attn_prefill(const void* q, const void* k_values, const vo
   p.out = (__nv_bfloat16*)out;
   p.sinks = sinks;
   p.status = status_word();
-  p.sched = sched;
-  const long long blocks = ((long long)max_q_len * (nq / nkv) + 2 * kP8Tile - 1) / (2 * kP8Tile);
-  if (!sched || blocks * nkv * batch > 0x7fffffffll) return -2;
-  p.batch = batch; p.q_blocks = int(blocks);
+  const long long blocks = p8_blocks(batch, max_q_len, nq, nkv);
+  p.parts = p8_parts(blocks, table_width);
+  if (!scratch || blocks * p.parts > 0x7fffffffll) return -2;
+  p.sched = reinterpret_cast<unsigned int*>(scratch);
+  p.partials = scratch + kP8Counters;
+  p.batch = batch; p.q_blocks = int(blocks / ((long long)nkv * batch));
   p.total_q = total_q; p.nq = nq; p.nkv = nkv; p.group = nq / nkv; p.num_blocks = num_blocks; p.table_width = table_width;
   p.causal = causal; p.window = window; p.chunk = chunk;
   p.table_stride = table_stride;

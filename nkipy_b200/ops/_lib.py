@@ -198,6 +198,7 @@ _SIGNATURES = {
                             c_int, c_int, c_int, c_int, c_longlong, c_float, c_int, _P, c_int, _P]),
     "nkb_q8_attn_prefill": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                                    c_longlong, c_float, c_int, c_int, c_int, _P, _P, _P]),
+    "nkb_q8_attn_prefill_scratch_floats": (c_longlong, [c_int, c_int, c_int, c_int, c_int, c_int]),
     "nkb_q8_attn_decode_scratch_floats": (c_longlong, [c_int, c_int, c_int, c_int, c_int]),
     "nkb_q8_attn_decode": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_longlong,
                                    c_float, c_int, c_int, _P, c_int, _P]),

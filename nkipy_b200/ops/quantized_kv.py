@@ -246,7 +246,7 @@ def _p(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-COUNTERS = 16384                     # words of the scratch of decode attention that count arrivals
+COUNTERS = 16384                     # words of the scratch of attention that count
 _SCRATCH = {}
 
 
@@ -411,13 +411,16 @@ def flash_attn_prefill(q, k_cache, v_cache, block_table, q_start, q_lens, contex
                 res[at:at + n] = _ref_attend(qf[at:at + n], k_cache, v_cache, block_table[b], ctx, scale, ctx - n, causal, window, chunk,
                                              sinks)
         return out
-    rc = _lib.lib().nkb_q8_attn_prefill(
+    L, width = _lib.lib(), block_table.shape[1]
+    floats = L.nkb_q8_attn_prefill_scratch_floats(B, max_q_len, nq, nkv, D, width)
+    scratch = _scratch(dev, floats)
+    rc = L.nkb_q8_attn_prefill(
         q.data_ptr(), *k_cache.at, *v_cache.at, block_table.data_ptr(), q_start.data_ptr(), q_lens.data_ptr(), context_lens.data_ptr(),
-        out.data_ptr(), B, q.shape[0], max_q_len, nq, nkv, D, blocks, block_table.shape[1], block_table.stride(0), scale,
-        1 if causal else 0, window, chunk, _p(sinks), _scratch(dev, COUNTERS).data_ptr(), _stream())
+        out.data_ptr(), B, q.shape[0], max_q_len, nq, nkv, D, blocks, width, block_table.stride(0), scale, 1 if causal else 0, window, chunk,
+        _p(sinks), scratch.data_ptr(), _stream())
     if rc:
         _lib.check(rc, "nkb_q8_attn_prefill")
-    _count_launch()
+    _count_launch(2 if floats > COUNTERS else 1)        # parts of blocks are joined by a second one
     return out
 
 

@@ -344,6 +344,10 @@ PROMPTS = [
     (8, 4, 64, [(0, 70)] * 41 + [(129, 3), (0, 1)], {}),                     # more pieces than SMs
     (6, 1, 128, [(3 * i, 1 + 11 * i) for i in range(24)], {}),               # of every length
     (5, 1, 64, [(0, 60), (300, 60)], dict(window=1)),
+    (8, 1, 64, [(2100, 5), (0, 3), (1300, 20)], {}),                         # few rows over long contexts, divided among works
+    (4, 2, 128, [(3000, 2), (40, 1)], dict(sinks=True)),
+    (2, 1, 128, [(2500, 33), (1, 300)], dict(window=700)),
+    (2, 1, 64, [(1600, 4)], dict(causal=False)),
 ]
 
 
