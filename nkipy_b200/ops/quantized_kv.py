@@ -33,22 +33,28 @@ DIMS = (64, 128)
 class QuantizedPages:
     """Keys or values of one layer: e4m3 `values` [blocks, kv heads, 32, dim] and power-of-two `scales` [blocks, kv heads, 32]
     (torch.float8_e8m0fnu), both contiguous and on one device."""
-    __slots__ = ("values", "scales", "shape", "device", "is_cuda", "at")
+    __slots__ = ("values", "scales", "shape", "device", "index", "at")
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor):
         if values.dtype is not torch.float8_e4m3fn or scales.dtype is not torch.float8_e8m0fnu:
             raise TypeError("QuantizedPages wants float8_e4m3fn values and float8_e8m0fnu scales")
-        if values.dim() != 4 or values.shape[2] != PAGE or scales.shape != values.shape[:3]:
+        shape = values.shape
+        if len(shape) != 4 or shape[2] != PAGE or scales.shape != shape[:3]:
             raise ValueError("QuantizedPages wants values [blocks, kv heads, 32, dim] and scales [blocks, kv heads, 32]")
-        if values.shape[3] not in DIMS:
+        if shape[3] not in DIMS:
             raise ValueError("QuantizedPages has heads of 64 or 128 columns")
-        if not values.is_contiguous() or not scales.is_contiguous() or values.device != scales.device:
+        index = values.get_device()
+        if not values.is_contiguous() or not scales.is_contiguous() or scales.get_device() != index:
             raise ValueError("QuantizedPages wants contiguous tensors on one device")
         self.at = v, s = values.data_ptr(), scales.data_ptr()
         if (v | s) & 15:
             raise ValueError("QuantizedPages wants tensors that start on 16 bytes")
-        self.values, self.scales = values, scales
-        self.shape, self.device, self.is_cuda = values.shape, values.device, values.is_cuda
+        # shape as of a cache tensor; index: of the CUDA device, -1: the CPU; at: where the tensors start
+        self.values, self.scales, self.shape, self.index, self.device = values, scales, shape, index, values.device
+
+    @property
+    def is_cuda(self) -> bool:
+        return self.index >= 0
 
     @classmethod
     def new(cls, num_blocks: int, kv_heads: int, dim: int, device="cpu") -> "QuantizedPages":
@@ -155,90 +161,116 @@ def _ref_attend(q, k_pages, v_pages, table_row, ctx, scale, pos0, causal, window
 
 
 # --------------------------------------------------------------------------- checks of arguments
+# (a call has a few microseconds on the host: each check is one line that passes, and the reason is looked for when it does not)
 def _pair(k_cache, v_cache) -> Tuple[int, int, int]:
     """(blocks, kv heads, dim) of a layer's pages."""
     if type(k_cache) is not QuantizedPages or type(v_cache) is not QuantizedPages:
         raise TypeError("keys and values are both QuantizedPages, or neither is")
-    if k_cache.shape != v_cache.shape or k_cache.device != v_cache.device:
+    if k_cache.shape != v_cache.shape or k_cache.index != v_cache.index:
         raise ValueError("keys and values want pages of one shape on one device")
-    return k_cache.shape[0], k_cache.shape[1], k_cache.shape[3]
+    blocks, nkv, _, dim = k_cache.shape
+    return blocks, nkv, dim
 
 
-def _want(t: Optional[torch.Tensor], name: str, dtype, shape, device, optional: bool = False) -> None:
-    if t is None:
-        if not optional:
-            raise ValueError(f"{name} is missing")
+def _want(t: torch.Tensor, name: str, dtype, shape, index: int) -> None:
+    """A contiguous tensor of this type and shape on device `index` (-1: the CPU)."""
+    if t.dtype is dtype and t.shape == shape and t.get_device() == index and t.is_contiguous():
         return
     if t.dtype is not dtype:
         raise TypeError(f"{name} wants {dtype}, not {t.dtype}")
     if t.shape != shape:
         raise ValueError(f"{name} has the shape {tuple(t.shape)}, not {tuple(shape)}")
-    if t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name} wants to be contiguous and on {device}")
+    raise ValueError(f"{name} wants to be contiguous and on the pages' device")
 
 
-def _check_device(pages: QuantizedPages) -> bool:
+def _want_rows(t: torch.Tensor, name: str, shape, index: int) -> int:
+    """Address of bf16 rows that kernels read or write in pieces of sixteen bytes."""
+    _want(t, name, torch.bfloat16, shape, index)
+    at = t.data_ptr()
+    if at & 15 and index >= 0:
+        raise ValueError(f"{name} wants to start on 16 bytes")
+    return at
+
+
+def _on_gpu(index: int) -> bool:
     """Whether the kernels run (CUDA); they are launched on the current device's current stream."""
-    if not pages.is_cuda:
+    if index < 0:
         return False
-    if pages.device.index != torch._C._cuda_getDevice():
+    if index != torch._C._cuda_getDevice():
         raise ValueError("the pages are on another device than the current one")
-    _lib.ensure_init()
+    if not _lib._initialised:
+        _lib.ensure_init()
     return True
 
 
-def _check_heads(nq: int, nkv: int) -> None:
+def _check_heads(nq: int, nkv: int) -> int:
     if nq < 1 or nkv < 1 or nq % nkv:
         raise ValueError("query heads are a multiple of the kv heads")
+    return nq // nkv
 
 
-def _check_table(block_table, context_lens, device) -> int:
+def _check_table(block_table, context_lens, index: int) -> Tuple[int, int]:
+    """(sequences, blocks of a row)"""
     if block_table.dim() != 2 or block_table.shape[1] < 1:
         raise ValueError("block_table wants [sequences, blocks]")
     if block_table.dtype is not torch.int32:
         raise TypeError(f"block_table wants torch.int32, not {block_table.dtype}")
-    if block_table.device != device or block_table.stride(1) != 1:
-        raise ValueError(f"block_table wants neighbouring columns and to be on {device}")
-    B = block_table.shape[0]
-    _want(context_lens, "context_lens", torch.int32, (B,), device)
-    return B
+    if block_table.get_device() != index or block_table.stride(1) != 1:
+        raise ValueError("block_table wants neighbouring columns and to be on the pages' device")
+    B, width = block_table.shape
+    _want(context_lens, "context_lens", torch.int32, (B,), index)
+    return B, width
 
 
-def _check_qkv(qkv, positions, slots, cos_sin, k_cache, nq, nkv, head_dim, bias, q_norm_w, k_norm_w) -> int:
-    dev, T, W = k_cache.device, qkv.shape[-2], (nq + 2 * nkv) * head_dim
+def _check_qkv(qkv, positions, slots, cos_sin, k_cache, nq, nkv, head_dim, bias, q_norm_w, k_norm_w) -> Tuple[int, int, int, int]:
+    """(tokens, partial sums, elements between them, rows of cos_sin)"""
+    index, shape = k_cache.index, qkv.shape
     _check_heads(nq, nkv)
     if nkv != k_cache.shape[1] or head_dim != k_cache.shape[3]:
         raise ValueError("the pages have other kv heads than the projection")
-    if qkv.dtype not in (torch.float32, torch.bfloat16) or qkv.dim() not in ((2, 3) if qkv.dtype is torch.float32 else (2,)):
+    W = (nq + 2 * nkv) * head_dim
+    parts, stride = 1, 0
+    if len(shape) == 3 and qkv.dtype is torch.float32:
+        parts, stride = shape[0], qkv.stride(0)
+    elif len(shape) != 2 or qkv.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError("qkv is bf16 [T, W] or fp32 partial sums [S, T, W]")
-    if qkv.shape[-1] != W or qkv.shape[0] < 1 <= T:
-        raise ValueError(f"qkv has {qkv.shape[-1]} columns, not {W}")
-    if qkv.device != dev or qkv.stride(-1) != 1 or qkv.stride(-2) != W:
-        raise ValueError(f"qkv wants rows that follow one another, on {dev}")
-    _want(positions, "positions", torch.int32, (T,), dev, optional=cos_sin is None)
-    _want(slots, "slots", torch.int32, (T,), dev, optional=True)
+    T = shape[-2]
+    if shape[-1] != W or parts < 1:
+        raise ValueError(f"qkv has the shape {tuple(shape)}, not [..., {W}]")
+    if qkv.get_device() != index or qkv.stride(-1) != 1 or qkv.stride(-2) != W:
+        raise ValueError("qkv wants rows that follow one another, on the pages' device")
+    rows = 0
     if cos_sin is not None:
-        _want(cos_sin, "cos_sin", torch.float32, (cos_sin.shape[0], head_dim), dev)
-        if not cos_sin.shape[0]:
-            raise ValueError("cos_sin has no rows")
-    _want(bias, "bias", torch.bfloat16, (W,), dev, optional=True)
-    _want(q_norm_w, "q_norm_w", torch.bfloat16, (head_dim,), dev, optional=True)
-    _want(k_norm_w, "k_norm_w", torch.bfloat16, (head_dim,), dev, optional=True)
-    return T
+        rows = cos_sin.shape[0]
+        _want(cos_sin, "cos_sin", torch.float32, (rows, head_dim), index)
+        if not rows or positions is None:
+            raise ValueError("a rotation wants positions and rows of cos and sin")
+    if positions is not None:
+        _want(positions, "positions", torch.int32, (T,), index)
+    if slots is not None:
+        _want(slots, "slots", torch.int32, (T,), index)
+    if bias is not None:
+        _want(bias, "bias", torch.bfloat16, (W,), index)
+    if q_norm_w is not None:
+        _want(q_norm_w, "q_norm_w", torch.bfloat16, (head_dim,), index)
+    if k_norm_w is not None:
+        _want(k_norm_w, "k_norm_w", torch.bfloat16, (head_dim,), index)
+    return T, parts, stride, rows
 
 
-def _check_masks(mods, window: int, chunk: int, sinks, nq: int, device) -> None:
+def _check_masks(mods, window: int, chunk: int, sinks, nq: int, index: int) -> None:
     if mods:
         raise ValueError("attention over QuantizedPages takes no score modifications")
     if window < 0 or chunk < 0:
         raise ValueError("window and chunk are not negative")
-    _want(sinks, "sinks", torch.float32, (nq,), device, optional=True)
+    if sinks is not None:
+        _want(sinks, "sinks", torch.float32, (nq,), index)
 
 
-def _result(out: Optional[torch.Tensor], shape, device) -> torch.Tensor:
+def _result(out: Optional[torch.Tensor], shape, pages: QuantizedPages) -> torch.Tensor:
     if out is None:
-        return torch.empty(shape, dtype=torch.bfloat16, device=device)
-    _want(out, "out", torch.bfloat16, shape, device)
+        return torch.empty(shape, dtype=torch.bfloat16, device=pages.device)
+    _want_rows(out, "out", shape, pages.index)
     return out
 
 
@@ -271,16 +303,19 @@ def _pick_splits(ctas: int, max_pages: int, sms: int = 148) -> int:
 
 
 def _splits(num_splits: int, scratch, B: int, nkv: int, D: int, group: int, max_pages: int, device):
-    """(parts of a sequence, scratch for their results)."""
+    """(parts of a sequence, address of scratch for their results)."""
     if num_splits <= 0:
         num_splits = _pick_splits(B * nkv, max_pages)
-    if num_splits > 1:
-        need = _lib.lib().nkb_q8_attn_decode_scratch_floats(B, nkv, D, group, num_splits)
-        if scratch is None:
-            scratch = _scratch(device, need)
-        elif scratch.dtype is not torch.float32 or scratch.numel() < need or scratch.device != device or not scratch.is_contiguous():
-            raise ValueError(f"scratch wants {need} contiguous fp32 values on {device}, the first {COUNTERS} zero before the first call")
-    return num_splits, scratch
+    if num_splits <= 1:
+        return 1, None
+    need = _lib.lib().nkb_q8_attn_decode_scratch_floats(B, nkv, D, group, num_splits)
+    if scratch is None:
+        scratch = _scratch(device, need)
+    elif (scratch.dtype is not torch.float32 or scratch.numel() < need or scratch.device != device or not scratch.is_contiguous()
+          or scratch.data_ptr() & 15):
+        raise ValueError(f"scratch wants {need} contiguous fp32 values on {device} from 16 bytes on, the first {COUNTERS} zero before "
+                         "the first call")
+    return num_splits, scratch.data_ptr()
 
 
 def decode_scratch(pages: QuantizedPages, nq: int, max_batch: int, max_pages: int) -> Optional[torch.Tensor]:
@@ -300,17 +335,14 @@ def rope_kv_append(qkv, positions, slots, cos_sin, k_cache, v_cache, nq, nkv, he
     """`ops.rope_kv_append` onto quantised pages: norms and rotations are rounded once, at the end.  A slot that is negative or
     outside the pages stores nothing; two tokens of a call have different slots."""
     blocks = _pair(k_cache, v_cache)[0]
-    T = _check_qkv(qkv, positions, slots, cos_sin, k_cache, nq, nkv, head_dim, bias, q_norm_w, k_norm_w)
-    q_out = _result(q_out, (T, nq * head_dim), k_cache.device)
-    if not _check_device(k_cache):
+    T, parts, stride, rows = _check_qkv(qkv, positions, slots, cos_sin, k_cache, nq, nkv, head_dim, bias, q_norm_w, k_norm_w)
+    q_out = _result(q_out, (T, nq * head_dim), k_cache)
+    if not _on_gpu(k_cache.index):
         return _ref_append(qkv, positions, slots, cos_sin, k_cache, v_cache, nq, nkv, head_dim, bias, q_norm_w, k_norm_w, norm_eps, q_out)
-    partial = qkv.dtype is torch.float32
-    splits, stride = (qkv.shape[0], qkv.stride(0)) if qkv.dim() == 3 else (1, 0)
-    at = qkv.data_ptr()
+    partial, at = qkv.dtype is torch.float32, qkv.data_ptr()
     rc = _lib.lib().nkb_q8_append(
-        None if partial else at, at if partial else None, splits, stride, _p(bias), _p(positions), _p(slots), _p(cos_sin), _p(q_norm_w),
-        _p(k_norm_w), norm_eps, q_out.data_ptr(), *k_cache.at, *v_cache.at, T, nq, nkv, head_dim,
-        0 if cos_sin is None else cos_sin.shape[0], blocks, _stream())
+        None if partial else at, at if partial else None, parts, stride, _p(bias), _p(positions), _p(slots), _p(cos_sin), _p(q_norm_w),
+        _p(k_norm_w), norm_eps, q_out.data_ptr(), *k_cache.at, *v_cache.at, T, nq, nkv, head_dim, rows, blocks, _stream())
     if rc:
         _lib.check(rc, "nkb_q8_append")
     _count_launch()
@@ -321,32 +353,31 @@ def paged_attn_decode(q, k_cache, v_cache, block_table, context_lens, scale, *, 
                       num_splits=0, scratch=None, out=None) -> torch.Tensor:
     """`ops.paged_attn_decode` over quantised pages."""
     blocks, nkv, D = _pair(k_cache, v_cache)
-    dev = k_cache.device
-    B = _check_table(block_table, context_lens, dev)
+    index = k_cache.index
+    B, width = _check_table(block_table, context_lens, index)
     nq = q.shape[-1] // D
-    _check_heads(nq, nkv)
-    _check_masks(mods, window, chunk, sinks, nq, dev)
+    group = _check_heads(nq, nkv)
+    _check_masks(mods, window, chunk, sinks, nq, index)
     if q_len < 1:
         raise ValueError("q_len is at least one")
-    _want(q, "q", torch.bfloat16, (B * q_len, nq * D), dev)
-    out = _result(out, q.shape, dev)
+    q_at = _want_rows(q, "q", (B * q_len, nq * D), index)
+    out = _result(out, q.shape, k_cache)
     if not B:
         return out
-    if not _check_device(k_cache):
+    if not _on_gpu(index):
         qf, res = q.float().reshape(B, q_len, nq, D), out.view(B, q_len, nq, D)
         for b in range(B):
-            ctx = min(int(context_lens[b]), block_table.shape[1] * PAGE)
+            ctx = min(int(context_lens[b]), width * PAGE)
             res[b] = _ref_attend(qf[b], k_cache, v_cache, block_table[b], ctx, scale, ctx - q_len, True, window, chunk, sinks)
         return out
-    group = nq // nkv
     if q_len * group > 16:          # more rows than a fragment of the decode kernel has
-        q_start = torch.arange(0, B * q_len, q_len, device=dev, dtype=torch.int32)
+        q_start = torch.arange(0, B * q_len, q_len, device=k_cache.device, dtype=torch.int32)
         return flash_attn_prefill(q, k_cache, v_cache, block_table, q_start, torch.full_like(q_start, q_len), context_lens, scale,
                                   max_q_len=q_len, window=window, chunk=chunk, sinks=sinks, out=out)
-    num_splits, scratch = _splits(num_splits, scratch, B, nkv, D, group, block_table.shape[1], dev)
+    num_splits, scratch = _splits(num_splits, scratch, B, nkv, D, group, width, k_cache.device)
     rc = _lib.lib().nkb_q8_attn_decode(
-        q.data_ptr(), *k_cache.at, *v_cache.at, block_table.data_ptr(), context_lens.data_ptr(), out.data_ptr(), _p(scratch), B, q_len, nq,
-        nkv, D, blocks, block_table.shape[1], block_table.stride(0), scale, window, chunk, _p(sinks), num_splits, _stream())
+        q_at, *k_cache.at, *v_cache.at, block_table.data_ptr(), context_lens.data_ptr(), out.data_ptr(), scratch, B, q_len, nq, nkv, D,
+        blocks, width, block_table.stride(0), scale, window, chunk, _p(sinks), num_splits, _stream())
     if rc:
         _lib.check(rc, "nkb_q8_attn_decode")
     _count_launch()
@@ -359,27 +390,24 @@ def rope_attn_decode(qkv_partials, positions, slots, cos_sin, k_cache, v_cache, 
     """`ops.rope_attn_decode` over quantised pages: `rope_kv_append`, and attention that fetches the older pages meanwhile.  The new token
     takes part as it is kept, in 8 bits.  slots[b] is the place of sequence b's position context_lens[b] - 1, or negative."""
     blocks, _, D = _pair(k_cache, v_cache)
-    if qkv_partials.dtype is not torch.float32 or qkv_partials.shape[-2] != block_table.shape[0]:
+    index = k_cache.index
+    B, width = _check_table(block_table, context_lens, index)
+    if qkv_partials.dtype is not torch.float32 or qkv_partials.shape[-2] != B:
         raise ValueError("rope_attn_decode wants fp32 partials [S, B, W], one token per sequence")
-    dev = k_cache.device
-    B = _check_table(block_table, context_lens, dev)
-    group = nq // nkv if nkv > 0 else 0
-    if not k_cache.is_cuda or group > 16 or not B:
+    if index < 0 or not B or nkv < 1 or nq // nkv > 16:
         q = rope_kv_append(qkv_partials, positions, slots, cos_sin, k_cache, v_cache, nq, nkv, D, bias=bias, q_norm_w=q_norm_w,
                            k_norm_w=k_norm_w, norm_eps=norm_eps)
         return paged_attn_decode(q, k_cache, v_cache, block_table, context_lens, scale, window=window, sinks=sinks, num_splits=num_splits,
                                  scratch=scratch, out=out)
-    _check_qkv(qkv_partials, positions, slots, cos_sin, k_cache, nq, nkv, D, bias, q_norm_w, k_norm_w)
-    _check_masks(None, window, 0, sinks, nq, dev)
-    out = _result(out, (B, nq * D), dev)
-    _check_device(k_cache)
-    num_splits, scratch = _splits(num_splits, scratch, B, nkv, D, group, block_table.shape[1], dev)
-    splits, stride = (qkv_partials.shape[0], qkv_partials.stride(0)) if qkv_partials.dim() == 3 else (1, 0)
+    _, parts, stride, rows = _check_qkv(qkv_partials, positions, slots, cos_sin, k_cache, nq, nkv, D, bias, q_norm_w, k_norm_w)
+    _check_masks(None, window, 0, sinks, nq, index)
+    out = _result(out, (B, nq * D), k_cache)
+    _on_gpu(index)
+    num_splits, scratch = _splits(num_splits, scratch, B, nkv, D, nq // nkv, width, k_cache.device)
     rc = _lib.lib().nkb_q8_step(
-        qkv_partials.data_ptr(), splits, stride, _p(bias), _p(positions), _p(slots), _p(cos_sin), _p(q_norm_w), _p(k_norm_w), norm_eps,
-        torch.empty_like(out).data_ptr(), *k_cache.at, *v_cache.at, block_table.data_ptr(), context_lens.data_ptr(), out.data_ptr(), _p(scratch),
-        B, nq, nkv, D, 0 if cos_sin is None else cos_sin.shape[0], blocks, block_table.shape[1], block_table.stride(0), scale, window,
-        _p(sinks), num_splits, _stream())
+        qkv_partials.data_ptr(), parts, stride, _p(bias), _p(positions), _p(slots), _p(cos_sin), _p(q_norm_w), _p(k_norm_w), norm_eps,
+        torch.empty_like(out).data_ptr(), *k_cache.at, *v_cache.at, block_table.data_ptr(), context_lens.data_ptr(), out.data_ptr(), scratch,
+        B, nq, nkv, D, rows, blocks, width, block_table.stride(0), scale, window, _p(sinks), num_splits, _stream())
     if rc:
         _lib.check(rc, "nkb_q8_step")
     _count_launch(2)
@@ -390,34 +418,33 @@ def flash_attn_prefill(q, k_cache, v_cache, block_table, q_start, q_lens, contex
                        chunk=0, sinks=None, mods=None, out=None) -> torch.Tensor:
     """`ops.flash_attn_prefill` over quantised pages.  Rows of q that belong to no sequence are left as they are in `out`."""
     blocks, nkv, D = _pair(k_cache, v_cache)
-    dev = k_cache.device
-    B = _check_table(block_table, context_lens, dev)
-    nq = q.shape[-1] // D
+    index = k_cache.index
+    B, width = _check_table(block_table, context_lens, index)
+    nq, total = q.shape[-1] // D, q.shape[0]
     _check_heads(nq, nkv)
-    _check_masks(mods, window, chunk, sinks, nq, dev)
-    _want(q, "q", torch.bfloat16, (q.shape[0], nq * D), dev)
-    _want(q_start, "q_start", torch.int32, (B,), dev)
-    _want(q_lens, "q_lens", torch.int32, (B,), dev)
-    out = _result(out, q.shape, dev)
-    if not B or not q.shape[0]:
+    _check_masks(mods, window, chunk, sinks, nq, index)
+    q_at = _want_rows(q, "q", (total, nq * D), index)
+    _want(q_start, "q_start", torch.int32, (B,), index)
+    _want(q_lens, "q_lens", torch.int32, (B,), index)
+    out = _result(out, q.shape, k_cache)
+    if not B or not total:
         return out
     if max_q_len < 1:
         raise ValueError("max_q_len is at least one")
-    if not _check_device(k_cache):
+    if not _on_gpu(index):
         qf, res = q.float().reshape(-1, nq, D), out.view(-1, nq, D)
         for b in range(B):
-            n, at, ctx = int(q_lens[b]), int(q_start[b]), min(int(context_lens[b]), block_table.shape[1] * PAGE)
+            n, at, ctx = int(q_lens[b]), int(q_start[b]), min(int(context_lens[b]), width * PAGE)
             if n > 0:
                 res[at:at + n] = _ref_attend(qf[at:at + n], k_cache, v_cache, block_table[b], ctx, scale, ctx - n, causal, window, chunk,
                                              sinks)
         return out
-    L, width = _lib.lib(), block_table.shape[1]
+    L = _lib.lib()
     floats = L.nkb_q8_attn_prefill_scratch_floats(B, max_q_len, nq, nkv, D, width)
-    scratch = _scratch(dev, floats)
     rc = L.nkb_q8_attn_prefill(
-        q.data_ptr(), *k_cache.at, *v_cache.at, block_table.data_ptr(), q_start.data_ptr(), q_lens.data_ptr(), context_lens.data_ptr(),
-        out.data_ptr(), B, q.shape[0], max_q_len, nq, nkv, D, blocks, width, block_table.stride(0), scale, 1 if causal else 0, window, chunk,
-        _p(sinks), scratch.data_ptr(), _stream())
+        q_at, *k_cache.at, *v_cache.at, block_table.data_ptr(), q_start.data_ptr(), q_lens.data_ptr(), context_lens.data_ptr(),
+        out.data_ptr(), B, total, max_q_len, nq, nkv, D, blocks, width, block_table.stride(0), scale, 1 if causal else 0, window, chunk,
+        _p(sinks), _scratch(k_cache.device, floats).data_ptr(), _stream())
     if rc:
         _lib.check(rc, "nkb_q8_attn_prefill")
     _count_launch(2 if floats > COUNTERS else 1)        # parts of blocks are joined by a second one

@@ -462,6 +462,7 @@ def test_pages_are_checked():
 
 @pytest.mark.parametrize("device", DEVICES)
 def test_refusals(device):
+    shifted = lambda t: torch.empty((t.numel() + 1,), dtype=t.dtype, device=device)[1:].view(t.shape)        # noqa: E731
     k, v = (ops.QuantizedPages.new(4, 2, 64, device) for _ in range(2))
     i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)        # noqa: E731
     q = torch.zeros((2, 4 * 64), dtype=torch.bfloat16, device=device)
@@ -473,12 +474,14 @@ def test_refusals(device):
                     (dict(t=table.long()), TypeError), (dict(n=lens.long()), TypeError), (dict(n=lens[:1]), ValueError),
                     (dict(t=table[0]), ValueError), (dict(window=-1), ValueError), (dict(chunk=-2), ValueError), (dict(q_len=0), ValueError),
                     (dict(mods=ops.ScoreMods(softcap=3.0)), ValueError), (dict(sinks=torch.zeros((3,), device=device)), ValueError),
-                    (dict(out=torch.empty_like(q, dtype=torch.float32)), TypeError), (dict(out=q[:1]), ValueError)]:
+                    (dict(out=torch.empty_like(q, dtype=torch.float32)), TypeError), (dict(out=q[:1]), ValueError),
+                    *([] if device == "cpu" else [(dict(q=shifted(q)), ValueError), (dict(out=shifted(q)), ValueError),
+                                                  (dict(num_splits=2, scratch=torch.zeros((8,), device=device)), ValueError)])]:
         with pytest.raises(err):
             decode(**kw)
     prompt = lambda s=i32([0, 1]), n=i32([1, 1]), c=lens, **kw: ops.flash_attn_prefill(       # noqa: E731
         q, k, v, table, s, n, c, 0.1, **{"max_q_len": 1, **kw})
-    for kw, err in [(dict(s=i32([0])), ValueError), (dict(n=lens.float()), TypeError), (dict(max_q_len=0), ValueError),
+    for kw, err in [(dict(s=i32([0])), ValueError), (dict(n=lens.float()), TypeError), (dict(max_q_len=0), ValueError), (dict(out=q.float()), TypeError),
                     (dict(mods=ops.ScoreMods(keep_first=3)), ValueError)]:
         with pytest.raises(err):
             prompt(**kw)
