@@ -11,6 +11,7 @@
 #include "linear_attn.h"
 #include "post_residual.h"
 #include "proj_src.h"
+#include "q8_args.h"
 
 namespace nkb {
 int encode_tmap_bf16_2d(CUtensorMap* m, const void* ptr, uint64_t inner, uint64_t outer, uint64_t ld_elems,
@@ -152,27 +153,13 @@ int nkb_rope_kv_append(const void* qkv_bf16, const float* qkv_partials, int spli
                        const void* q_norm_w, const void* k_norm_w, float norm_eps, void* q_out, void* k_cache,
                        void* v_cache, int tokens, int nq, int nkv, int head_dim, int max_pos, int block_size,
                        void* stream);
-// Cache in 8 bits (kv_quant.cuh): pages [block][kv head][32 tokens][D] e4m3, scales [block][kv head][32 tokens].
-int nkb_q8_append(const void* qkv_bf16, const float* qkv_partials, int splits, long long split_stride, const void* bias,
-                  const int* positions, const int* slots, const float* cos_sin, const void* q_norm_w, const void* k_norm_w, double eps,
-                  void* q_out, void* k_values, void* k_scales, void* v_values, void* v_scales, int tokens, int nq, int nkv, int head_dim,
-                  int max_pos, int num_blocks, void* stream);
-long long nkb_q8_attn_prefill_scratch_floats(int batch, int max_q_len, int nq, int nkv, int head_dim, int table_width);
-int nkb_q8_attn_prefill(const void* q, const void* k_values, const void* k_scales, const void* v_values, const void* v_scales,
-                       const int* block_table, const int* q_start, const int* q_lens, const int* context_lens, void* out, int batch,
-                       int total_q, int max_q_len, int nq, int nkv, int head_dim, int num_blocks, int table_width, long long table_stride,
-                       float scale, int causal, int window, int chunk, const float* sinks,
-                       float* scratch, void* stream);
+// Cache in 8 bits (kv_quant.cuh, q8_args.h): pages [block][kv head][32 tokens][D] e4m3, scales [block][kv head][32 tokens].
+int nkb_q8_append(const NkbQ8Append* arg);
 long long nkb_q8_attn_decode_scratch_floats(int batch, int nkv, int head_dim, int group, int num_splits);
-int nkb_q8_attn_decode(const void* q, const void* k_values, const void* k_scales, const void* v_values, const void* v_scales,
-                       const int* block_table, const int* context_lens, void* out, float* scratch, int batch, int q_len, int nq, int nkv,
-                       int head_dim, int num_blocks, int table_width, long long table_stride, float scale, int window, int chunk,
-                       const float* sinks, int num_splits, void* stream);
-int nkb_q8_step(const float* qkv_partials, int splits, long long split_stride, const void* bias, const int* positions, const int* slots,
-                const float* cos_sin, const void* q_norm_w, const void* k_norm_w, double eps, void* queries, void* k_values, void* k_scales,
-                void* v_values, void* v_scales, const int* block_table, const int* context_lens, void* out, float* scratch, int batch,
-                int nq, int nkv, int head_dim, int max_pos, int num_blocks, int table_width, long long table_stride, float scale, int window,
-                const float* sinks, int num_splits, void* stream);
+int nkb_q8_attn_decode(const NkbQ8Attn* arg);
+int nkb_q8_step(const NkbQ8Append* append, const NkbQ8Attn* attn);
+long long nkb_q8_attn_prefill_scratch_floats(int batch, int max_q_len, int nq, int nkv, int head_dim, int table_width);
+int nkb_q8_attn_prefill(const NkbQ8Attn* arg);
 int nkb_decode_advance(int* context_lens, const int* block_table, int* positions, int* slots, int batch, int q_len,
                        int max_blocks, int block_size, void* stream);
 // Positions and cache slots of the tokens of a packed step (sequences one behind another without gaps, each with its row of the table).

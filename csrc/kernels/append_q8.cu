@@ -334,38 +334,40 @@ __global__ void __launch_bounds__(256, PARTIALS ? 2 : 3) append8_q8_kernel(const
 
 using namespace nkb;
 
-extern "C" int nkb_q8_append(const void* qkv_bf16, const float* qkv_partials, int splits, long long split_stride, const void* bias,
-                             const int* positions, const int* slots, const float* cos_sin, const void* q_norm_w, const void* k_norm_w,
-                             double eps, void* q_out, void* k_values, void* k_scales, void* v_values, void* v_scales, int tokens, int nq,
-                             int nkv, int head_dim, int max_pos, int num_blocks, void* stream) {
+extern "C" int nkb_q8_append(const NkbQ8Append* arg) {
+  const NkbQ8Append& g = *arg;
+  const int tokens = g.tokens, nq = g.nq, nkv = g.nkv, head_dim = g.head_dim;
+  const void* qkv_bf16 = g.qkv;
+  const float* qkv_partials = g.partials;
   if (tokens <= 0) return 0;
+  if (nq < 1 || nkv < 1 || (!qkv_bf16 && (!qkv_partials || g.splits < 1)) || (g.cos_sin && (!g.positions || g.max_pos < 1))) return -2;
   if (!status_word() && nkb_init() != 0) return -1;
   AppendQ8Params p{};
   p.qkv = (const __nv_bfloat16*)qkv_bf16;
   p.partials = qkv_partials;
-  p.splits = splits;
-  p.split_stride = split_stride;
-  p.bias = (const __nv_bfloat16*)bias;
-  p.positions = positions;
-  p.slots = slots;
-  p.cos_sin = cos_sin;
-  p.q_norm_w = (const __nv_bfloat16*)q_norm_w;
-  p.k_norm_w = (const __nv_bfloat16*)k_norm_w;
-  p.eps = eps;
-  p.q_out = (__nv_bfloat16*)q_out;
-  p.k_values = (uint8_t*)k_values;
-  p.k_scales = (uint8_t*)k_scales;
-  p.v_values = (uint8_t*)v_values;
-  p.v_scales = (uint8_t*)v_scales;
-  p.tokens = tokens; p.nq = nq; p.nkv = nkv; p.max_pos = max_pos;
-  p.slots_end = (long long)num_blocks * kQ8Page;
+  p.splits = g.splits;
+  p.split_stride = g.split_stride;
+  p.bias = (const __nv_bfloat16*)g.bias;
+  p.positions = g.positions;
+  p.slots = g.slots;
+  p.cos_sin = g.cos_sin;
+  p.q_norm_w = (const __nv_bfloat16*)g.q_norm_w;
+  p.k_norm_w = (const __nv_bfloat16*)g.k_norm_w;
+  p.eps = g.eps;
+  p.q_out = (__nv_bfloat16*)g.q_out;
+  p.k_values = (uint8_t*)g.k_values;
+  p.k_scales = (uint8_t*)g.k_scales;
+  p.v_values = (uint8_t*)g.v_values;
+  p.v_scales = (uint8_t*)g.v_scales;
+  p.tokens = tokens; p.nq = nq; p.nkv = nkv; p.max_pos = g.max_pos;
+  p.slots_end = (long long)g.num_blocks * kQ8Page;
   uintptr_t at = 0;
-  for (const void* a : {qkv_bf16, (const void*)qkv_partials, bias, (const void*)cos_sin, q_norm_w, k_norm_w, (const void*)q_out,
-                        (const void*)k_values, (const void*)v_values})
+  for (const void* a : {qkv_bf16, (const void*)qkv_partials, g.bias, (const void*)g.cos_sin, g.q_norm_w, g.k_norm_w, (const void*)g.q_out,
+                        (const void*)g.k_values, (const void*)g.v_values})
     at |= reinterpret_cast<uintptr_t>(a);
   // A few tokens are bound by latency and keep a warp per head: 64 of them from partial sums 3.3 us and 4.1 in pieces, 128 5.7 and 5.5, 255 from
   // bf16 4.3 and 3.05.
-  const bool pieces = tokens >= (qkv_partials ? 128 : 64) && (at & 15) == 0 && (!qkv_partials || (split_stride & 3) == 0);
+  const bool pieces = tokens >= (qkv_partials ? 128 : 64) && (at & 15) == 0 && (!qkv_partials || (g.split_stride & 3) == 0);
   const long long heads = (long long)tokens * (nq + 2 * nkv);
   if (heads > 0x7fffffffll) return -2;
   // runs so long that all warps are resident at once
@@ -373,7 +375,7 @@ extern "C" int nkb_q8_append(const void* qkv_bf16, const float* qkv_partials, in
   const long long resident = num_sms() * (qkv_partials ? 16 : 24), need = ((long long)tokens * steps + resident - 1) / resident;
   const long long run = need > steps ? steps : need;
   const long long blocks = ((pieces ? tokens * ((steps + run - 1) / run) : heads) + 7) / 8;
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(g.stream);
   const dim3 grid = dim3(unsigned(blocks));
 #define NKB_APPEND(D)                                                                                                                 \
   return pieces ? launch_pdl(qkv_partials ? append8_q8_kernel<D, true> : append8_q8_kernel<D, false>, grid, dim3(256), 0, s, p, int(run)) \

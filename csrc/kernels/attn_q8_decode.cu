@@ -29,7 +29,6 @@ constexpr int kQ8Stages = 3;
 // warps whose rings an SM holds
 template <int D>
 constexpr int kQ8SmWarps = 1024 / D;
-constexpr int kQ8Counters = 16384;     // the scratch starts with as many arrival counters
 constexpr float kQ8Lift = 6.f;         // log2 of the weight at M; t may grow by kQ8Grow above M before M follows: f16 ends at 2^16
 constexpr float kQ8Grow = 8.f;
 
@@ -532,59 +531,41 @@ extern "C" long long nkb_q8_attn_decode_scratch_floats(int batch, int nkv, int h
   return kQ8Counters + (long long)plan_units(batch, nkv, group, num_splits) * nkv * (16 * head_dim + 32);
 }
 
-static int attn_q8_decode(const void* q, const void* k_values, const void* k_scales, const void* v_values, const void* v_scales,
-                          const int* block_table, const int* context_lens, void* out, float* scratch, int batch, int q_len, int nq, int nkv,
-                          int head_dim, int num_blocks, int table_width, long long table_stride, float scale, int window, int chunk,
-                          const float* sinks, int num_splits, int early, void* stream) {
-  if (batch <= 0) return 0;
-  if (nkv < 1 || nq % nkv || q_len * (nq / nkv) > 16 || nkv > 65535 || batch > 65535) return -2;
-  if (num_splits > 1 && (!scratch || (long long)batch * nkv > kQ8Counters)) return -2;
+static int attn_q8_decode(const NkbQ8Attn& g, int early) {
+  if (g.batch <= 0) return 0;
+  const int group = g.nkv > 0 ? g.nq / g.nkv : 0;
+  if (group < 1 || g.nq % g.nkv || g.q_len < 1 || (long long)g.q_len * group > 16 || g.nkv > 65535 || g.batch > 65535) return -2;
+  if (g.num_splits > 1 && (!g.scratch || (long long)g.batch * g.nkv > kQ8Counters)) return -2;
   if (!status_word() && nkb_init() != 0) return -1;
   DecodeQ8Params p{};
-  p.q = (const __nv_bfloat16*)q;
-  p.block_table = block_table; p.context_lens = context_lens;
-  p.out = (__nv_bfloat16*)out;
-  p.scratch = num_splits > 1 ? scratch + kQ8Counters : nullptr;
-  p.counters = reinterpret_cast<unsigned int*>(scratch);
-  p.sinks = sinks;
+  p.q = (const __nv_bfloat16*)g.q;
+  p.block_table = g.block_table; p.context_lens = g.context_lens;
+  p.out = (__nv_bfloat16*)g.out;
+  p.scratch = g.num_splits > 1 ? g.scratch + kQ8Counters : nullptr;
+  p.counters = reinterpret_cast<unsigned int*>(g.scratch);
+  p.sinks = g.sinks;
   p.status = status_word();
-  p.batch = batch; p.q_len = q_len; p.nq = nq; p.nkv = nkv; p.group = nq / nkv; p.table_width = table_width;
-  p.window = window; p.chunk = chunk; p.early = early;
-  p.units = plan_units(batch, nkv, p.group, num_splits);
-  p.table_stride = table_stride;
-  p.scale_log2 = scale * 1.4426950408889634f;
+  p.batch = g.batch; p.q_len = g.q_len; p.nq = g.nq; p.nkv = g.nkv; p.group = group; p.table_width = g.table_width;
+  p.window = g.window; p.chunk = g.chunk; p.early = early;
+  p.units = plan_units(g.batch, g.nkv, group, g.num_splits);
+  p.table_stride = g.table_stride;
+  p.scale_log2 = g.scale * 1.4426950408889634f;
   CUtensorMap m[4];
-  if (int rc = q8_maps(m, {k_values, v_values, k_scales, v_scales}, head_dim, nkv, num_blocks)) return rc;
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const bool eight = q_len * p.group <= 8;
-  if (head_dim == 128) return eight ? dispatch_decode_q8<128, 1>(m, p, s) : dispatch_decode_q8<128, 2>(m, p, s);
-  if (head_dim == 64) return eight ? dispatch_decode_q8<64, 1>(m, p, s) : dispatch_decode_q8<64, 2>(m, p, s);
+  if (int rc = q8_maps(m, {g.k_values, g.v_values, g.k_scales, g.v_scales}, g.head_dim, g.nkv, g.num_blocks)) return rc;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(g.stream);
+  const bool eight = g.q_len * group <= 8;
+  if (g.head_dim == 128) return eight ? dispatch_decode_q8<128, 1>(m, p, s) : dispatch_decode_q8<128, 2>(m, p, s);
+  if (g.head_dim == 64) return eight ? dispatch_decode_q8<64, 1>(m, p, s) : dispatch_decode_q8<64, 2>(m, p, s);
   return -2;
 }
 
-// At most 16 query rows per kv head (q_len * nq / nkv).  num_splits > 1: scratch as large as the function above says, its first kQ8Counters
-// words zero before the first call (a call leaves them at zero).
-extern "C" int nkb_q8_attn_decode(const void* q, const void* k_values, const void* k_scales, const void* v_values, const void* v_scales,
-                                  const int* block_table, const int* context_lens, void* out, float* scratch, int batch, int q_len, int nq,
-                                  int nkv, int head_dim, int num_blocks, int table_width, long long table_stride, float scale, int window,
-                                  int chunk, const float* sinks, int num_splits, void* stream) {
-  return attn_q8_decode(q, k_values, k_scales, v_values, v_scales, block_table, context_lens, out, scratch, batch, q_len, nq, nkv, head_dim,
-                        num_blocks, table_width, table_stride, scale, window, chunk, sinks, num_splits, 0, stream);
-}
+// At most 16 query rows per kv head (q_len * nq / nkv).  num_splits > 1: parts of a sequence on average, with scratch.
+extern "C" int nkb_q8_attn_decode(const NkbQ8Attn* arg) { return attn_q8_decode(*arg, 0); }
 
-// One new token per sequence, from split-K partials [splits][batch][(nq + 2 nkv) * head_dim]: nkb_q8_append and, behind it, attention that
-// fetches all pages but the new token's while the append runs.  slots[b]: the place of position context_lens[b] - 1 (negative: none).
-// queries: batch * nq * head_dim bf16 values for the rotated queries.
-extern "C" int nkb_q8_step(const float* qkv_partials, int splits, long long split_stride, const void* bias, const int* positions,
-                           const int* slots, const float* cos_sin, const void* q_norm_w, const void* k_norm_w, double eps, void* queries,
-                           void* k_values, void* k_scales, void* v_values, void* v_scales, const int* block_table, const int* context_lens,
-                           void* out, float* scratch, int batch, int nq, int nkv, int head_dim, int max_pos, int num_blocks,
-                           int table_width, long long table_stride, float scale, int window, const float* sinks, int num_splits,
-                           void* stream) {
-  if (nkv < 1 || nq % nkv || nq / nkv > 16) return -2;
-  if (int rc = nkb_q8_append(nullptr, qkv_partials, splits, split_stride, bias, positions, slots, cos_sin, q_norm_w, k_norm_w, eps, queries,
-                             k_values, k_scales, v_values, v_scales, batch, nq, nkv, head_dim, max_pos, num_blocks, stream))
-    return rc;
-  return attn_q8_decode(queries, k_values, k_scales, v_values, v_scales, block_table, context_lens, out, scratch, batch, 1, nq, nkv, head_dim,
-                        num_blocks, table_width, table_stride, scale, window, 0, sinks, num_splits, pdl_enabled() ? 1 : 0, stream);
+// One new token per sequence: append, and behind it attention of its queries, which fetches all pages but the new token's while the append
+// runs.  append.slots[b] is the place of position context_lens[b] - 1, or negative.
+extern "C" int nkb_q8_step(const NkbQ8Append* append, const NkbQ8Attn* attn) {
+  if (attn->nkv < 1 || attn->nq % attn->nkv || attn->nq / attn->nkv > 16 || attn->q_len != 1 || append->tokens != attn->batch) return -2;
+  if (int rc = nkb_q8_append(append)) return rc;
+  return attn_q8_decode(*attn, pdl_enabled() ? 1 : 0);
 }

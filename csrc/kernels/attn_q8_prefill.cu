@@ -67,7 +67,6 @@ struct P8Work {
   // tiles whose exponentials the two take turns with
   __device__ __forceinline__ int paired() const { return tr1.rows > 0 ? min(tr0.hi - tr0.lo, tr1.hi - tr1.lo) : 0; }
 };
-constexpr int kP8Counters = 16384;       // words ahead of the partial results (the scratch of decode attention has as many)
 constexpr int kP8Works = 3;              // works ahead of their use
 constexpr int kP8Readers = 15;           // warps 0 to 14 read them
 
@@ -913,39 +912,34 @@ extern "C" long long nkb_q8_attn_prefill_scratch_floats(int batch, int max_q_len
   if (batch <= 0 || nkv < 1 || max_q_len < 1 || (!status_word() && nkb_init() != 0)) return 0;
   const long long blocks = p8_blocks(batch, max_q_len, nq, nkv);
   const int parts = p8_parts(blocks, table_width);
-  return kP8Counters + (parts > 1 ? blocks * parts * 2 * kP8Tile * (head_dim + 2) : 0);
+  return kQ8Counters + (parts > 1 ? blocks * parts * 2 * kP8Tile * (head_dim + 2) : 0);
 }
 
-// scratch: as large as the function above says; its first kP8Counters words are zero before the first call (a call leaves them at zero); not
-// shared by calls that may run at the same time
-extern "C" int nkb_q8_attn_prefill(const void* q, const void* k_values, const void* k_scales, const void* v_values, const void* v_scales,
-                                   const int* block_table, const int* q_start, const int* q_lens, const int* context_lens, void* out,
-                                   int batch, int total_q, int max_q_len, int nq, int nkv, int head_dim, int num_blocks, int table_width,
-                                   long long table_stride, float scale, int causal, int window, int chunk, const float* sinks,
-                                   float* scratch, void* stream) {
-  if (batch <= 0 || total_q <= 0) return 0;
-  if (batch > 65535 || nkv > 65535 || nkv < 1 || nq % nkv || max_q_len < 1) return -2;
+extern "C" int nkb_q8_attn_prefill(const NkbQ8Attn* arg) {
+  const NkbQ8Attn& g = *arg;
+  if (g.batch <= 0 || g.total_q <= 0) return 0;
+  if (g.batch > 65535 || g.nkv > 65535 || g.nkv < 1 || g.nq < g.nkv || g.nq % g.nkv || g.q_len < 1) return -2;
   if (!status_word() && nkb_init() != 0) return -1;
   PrefillQ8Params p{};
-  p.q = (const __nv_bfloat16*)q;
-  p.k_values = (const uint8_t*)k_values; p.k_scales = (const uint8_t*)k_scales;
-  p.v_values = (const uint8_t*)v_values; p.v_scales = (const uint8_t*)v_scales;
-  p.block_table = block_table; p.q_start = q_start; p.q_lens = q_lens; p.context_lens = context_lens;
-  p.out = (__nv_bfloat16*)out;
-  p.sinks = sinks;
+  p.q = (const __nv_bfloat16*)g.q;
+  p.k_values = (const uint8_t*)g.k_values; p.k_scales = (const uint8_t*)g.k_scales;
+  p.v_values = (const uint8_t*)g.v_values; p.v_scales = (const uint8_t*)g.v_scales;
+  p.block_table = g.block_table; p.q_start = g.q_start; p.q_lens = g.q_lens; p.context_lens = g.context_lens;
+  p.out = (__nv_bfloat16*)g.out;
+  p.sinks = g.sinks;
   p.status = status_word();
-  const long long blocks = p8_blocks(batch, max_q_len, nq, nkv);
-  p.parts = p8_parts(blocks, table_width);
-  if (!scratch || blocks * p.parts > 0x7fffffffll) return -2;
-  p.sched = reinterpret_cast<unsigned int*>(scratch);
-  p.partials = scratch + kP8Counters;
-  p.batch = batch; p.q_blocks = int(blocks / ((long long)nkv * batch));
-  p.total_q = total_q; p.nq = nq; p.nkv = nkv; p.group = nq / nkv; p.num_blocks = num_blocks; p.table_width = table_width;
-  p.causal = causal; p.window = window; p.chunk = chunk;
-  p.table_stride = table_stride;
-  p.scale_log2 = scale * 1.4426950408889634f;
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (head_dim == 128) return launch_prefill_q8<128>(p, s);
-  if (head_dim == 64) return launch_prefill_q8<64>(p, s);
+  const long long blocks = p8_blocks(g.batch, g.q_len, g.nq, g.nkv);
+  p.parts = p8_parts(blocks, g.table_width);
+  if (!g.scratch || blocks * p.parts > 0x3fffffffll) return -2;
+  p.sched = reinterpret_cast<unsigned int*>(g.scratch);
+  p.partials = g.scratch + kQ8Counters;
+  p.batch = g.batch; p.q_blocks = int(blocks / ((long long)g.nkv * g.batch));
+  p.total_q = g.total_q; p.nq = g.nq; p.nkv = g.nkv; p.group = g.nq / g.nkv; p.num_blocks = g.num_blocks; p.table_width = g.table_width;
+  p.causal = g.causal; p.window = g.window; p.chunk = g.chunk;
+  p.table_stride = g.table_stride;
+  p.scale_log2 = g.scale * 1.4426950408889634f;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(g.stream);
+  if (g.head_dim == 128) return launch_prefill_q8<128>(p, s);
+  if (g.head_dim == 64) return launch_prefill_q8<64>(p, s);
   return -2;
 }

@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_double, c_float, c_int, c_longlong, c_ulonglong, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_longlong, c_ulonglong, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libnkipy_b200_kernels.so"
@@ -192,16 +192,13 @@ _SIGNATURES = {
         [_P, _P, c_int, c_longlong, _P, _P, _P, _P, _P, _P, c_float, _P, _P, _P, c_int, c_int, c_int, c_int, c_int,
          c_int, _P],
     ),
-    "nkb_q8_append": (c_int, [_P, _P, c_int, c_longlong, _P, _P, _P, _P, _P, _P, c_double, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int,
-                              c_int, c_int, _P]),
-    "nkb_q8_step": (c_int, [_P, c_int, c_longlong, _P, _P, _P, _P, _P, _P, c_double, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int,
-                            c_int, c_int, c_int, c_int, c_longlong, c_float, c_int, _P, c_int, _P]),
-    "nkb_q8_attn_prefill": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
-                                   c_longlong, c_float, c_int, c_int, c_int, _P, _P, _P]),
-    "nkb_q8_attn_prefill_scratch_floats": (c_longlong, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    # (packed arguments: csrc/kernels/q8_args.h)
+    "nkb_q8_append": (c_int, [c_char_p]),
+    "nkb_q8_step": (c_int, [c_char_p, c_char_p]),
+    "nkb_q8_attn_decode": (c_int, [c_char_p]),
+    "nkb_q8_attn_prefill": (c_int, [c_char_p]),
     "nkb_q8_attn_decode_scratch_floats": (c_longlong, [c_int, c_int, c_int, c_int, c_int]),
-    "nkb_q8_attn_decode": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_longlong,
-                                   c_float, c_int, c_int, _P, c_int, _P]),
+    "nkb_q8_attn_prefill_scratch_floats": (c_longlong, [c_int, c_int, c_int, c_int, c_int, c_int]),
     "nkb_decode_advance": (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, c_int, _P]),
     "nkb_packed_positions": (c_int, [_P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, _P]),
     "nkb_argmax": (c_int, [_P, c_int, _P, _P, c_int, c_int, c_longlong, _P]),
