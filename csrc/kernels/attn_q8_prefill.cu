@@ -210,6 +210,24 @@ __host__ __device__ constexpr uint32_t p8_idesc(int m, int n, int b_mn_major) {
   return (1u << 4) | (uint32_t(b_mn_major) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
 }
 
+// A warp's 32 rows in a swizzled tile, as it reads q and writes out: D / 8 lanes have a row's sixteen-byte pieces, kRows rows at a time.  (With
+// a thread to a row every access would touch 32 lines: 16 sequences of 1024 tokens took 192 us for 166.)
+template <int D>
+struct P8Rows {
+  static constexpr int kRows = 256 / D;
+  int lane, piece, row;
+  uint8_t* tile;
+  __device__ __forceinline__ P8Rows(uint8_t* tile, int lane) : lane(lane), piece(lane % (D / 8)), row(lane / (D / 8)), tile(tile) {}
+  // the piece of row `first` + row
+  __device__ __forceinline__ uint4* wide(int first) const {
+    return reinterpret_cast<uint4*>(tile + (piece >> 3) * kP8Tile * 128 + (first + row) * 128 + (((piece ^ (first + row)) & 7) << 4));
+  }
+  // piece i of row `lane`
+  __device__ __forceinline__ uint4* own(int i) const {
+    return reinterpret_cast<uint4*>(tile + (i >> 3) * kP8Tile * 128 + lane * 128 + (((i ^ lane) & 7) << 4));
+  }
+};
+
 template <int D>
 __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const PrefillQ8Params p) {
   using L = PrefillQ8Smem<D>;
@@ -726,11 +744,19 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
         const int q_pos = k.ctx - k.q_len + token;
         next.hi_pos = p.causal ? min(k.ctx - 1, q_pos) : k.ctx - 1;
         next.lo_pos = nkb_first_visible(q_pos, p.window, p.chunk);
+        const P8Rows<D> rows(q_s + t * L::kTile + quad * 32 * 128, lane);
         uint4 v[D / 8];
-        const uint4* src = reinterpret_cast<const uint4*>(p.q + next.at * D);
         float mx = 0.f;
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) v[i] = next.at >= 0 ? src[i] : make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < D / 8; ++i) {
+          const long long at = __shfl_sync(kAll, next.at, i * rows.kRows + rows.row);
+          v[i] = at >= 0 ? reinterpret_cast<const uint4*>(p.q + at * D)[rows.piece] : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) *rows.wide(i * rows.kRows) = v[i];
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) v[i] = *rows.own(i);
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
           const uint32_t q4[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
@@ -743,7 +769,6 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
         const int e = max((__float_as_int(mx) >> 23) - 127, -100);
         const float up = exp2_int(14 - e);
         next.raw_log2 = p.scale_log2 * exp2_int(e - 14);
-        uint8_t* dst = q_s + t * L::kTile + r * 128;
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
           const uint32_t q4[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
@@ -753,7 +778,7 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
             const float2 f = unpack_bf16x2(q4[j]);
             h[j] = p8_pack_f16x2(f.x * up, f.y * up);
           }
-          *reinterpret_cast<uint4*>(dst + (i >> 3) * kHalf + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+          *rows.own(i) = make_uint4(h[0], h[1], h[2], h[3]);
         }
         fence_proxy_async();
         __syncwarp();
@@ -769,8 +794,13 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
           if (have_o) tc_fence_after();
         }
         const bool whole = p.parts == 1;
+        // the weights are behind their last product.  The lane goes through an empty asm, since addresses that are computed ahead of the loop
+        // over tiles take registers there (267 us for 251 at 64 columns).
+        int lane_o = lane;
+        asm volatile("" : "+r"(lane_o));
+        const P8Rows<D> rows(p_s + t * L::kP + quad * 32 * 128, lane_o);
         const float inv = whole ? p8_inverse(p, cur.head, m, l) : 0.f;
-        const bool store = cur.at >= 0 && !*abort_flag;
+        const bool store = !*abort_flag;
         constexpr long long kPart = 2 * kP8Tile * (D + 2);
         float* first = p.partials + (long long)cur.block * p.parts * kPart;
         float* mine = first + cur.part * kPart + (t * kP8Tile + r) * D;
@@ -785,13 +815,11 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
             for (int i = 0; i < 32; ++i) o[i] = 0.f;
           }
           if (whole) {
-            if (store) {
 #pragma unroll
-              for (int i = 0; i < 32; i += 8)
-                *reinterpret_cast<uint4*>(p.out + cur.at * D + c * 32 + i) =
-                    make_uint4(pack_bf16x2(o[i] * inv, o[i + 1] * inv), pack_bf16x2(o[i + 2] * inv, o[i + 3] * inv),
-                               pack_bf16x2(o[i + 4] * inv, o[i + 5] * inv), pack_bf16x2(o[i + 6] * inv, o[i + 7] * inv));
-            }
+            for (int i = 0; i < 4; ++i)
+              *rows.own(c * 4 + i) =
+                  make_uint4(pack_bf16x2(o[8 * i] * inv, o[8 * i + 1] * inv), pack_bf16x2(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
+                             pack_bf16x2(o[8 * i + 4] * inv, o[8 * i + 5] * inv), pack_bf16x2(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
           } else if (have_o) {
 #pragma unroll
             for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(mine + c * 32 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
@@ -801,6 +829,16 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&ctrl->o_empty[t]);
+        }
+        if (whole) {
+          __syncwarp();
+#pragma unroll 4
+          for (int j = 0; j < 32; j += rows.kRows) {
+            const long long at = __shfl_sync(kAll, cur.at, j + rows.row);
+            const uint4 x = *rows.wide(j);
+            if (at >= 0 && store) reinterpret_cast<uint4*>(p.out + at * D)[rows.piece] = x;
+          }
+          __syncwarp();
         }
         if (!whole) {
           float* tail = first + cur.part * kPart + 2 * kP8Tile * D + t * kP8Tile + r;
