@@ -21,7 +21,7 @@
 // f16 as they are loaded, each row scaled below 2^15 by a power of two.
 //
 // 128 exponentials per row bound the loop (2048 cycles per 256 x 128 scores, as many as its MMAs at 128 columns), so conversion has warps
-// of its own, with the registers that the softmax leaves: 72 and 184 a thread.
+// of its own, with the registers that the softmax leaves: 64 and 192 a thread.
 #include "api.h"
 #include "kv_quant.cuh"
 #include "attn_maps.h"
@@ -33,7 +33,7 @@ namespace nkb {
 
 constexpr int kP8Tile = 128;             // query rows of an MMA tile, tokens of a K or V tile
 constexpr int kP8Threads = 512;
-constexpr int kP8Regs = 128;             // a thread's registers at launch; 2 * 128 * (72 + 184) is all of them
+constexpr int kP8Regs = 128;             // a thread's registers at launch; 2 * 128 * (64 + 192) is all of them
 constexpr int kP8Slots = 8;              // tiles whose scales are kept
 constexpr int kP8Lead = 4;               // tiles that warp 14 is ahead of the conversion of V at most
 constexpr float kP8Grow = 8.f;           // log2 of the growth of a row's maximum that makes O follow
@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
 
   if (warp < 4) {
     // ---------------------------------------------------------------- conversion
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     constexpr int kRows = 512 / D, kSteps = kQ8Page / kRows;       // tokens per sixteen-byte load of the warp, loads per page
     constexpr int kLanes = D / 16;                                 // lanes that share a token
     const int piece = lane % kLanes, row_of = lane / kLanes;
@@ -301,79 +301,79 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
     P8Work k;
 #pragma unroll 1
     while (alive && p8_next(ctrl, n_works, k, false, p.status)) {
-    int vis_lo, vis_hi;
-    p8_seen(p, k, vis_lo, vis_hi);
-    const int items = 2 * k.n_union;
+      int vis_lo, vis_hi;
+      p8_seen(p, k, vis_lo, vis_hi);
+      const int items = 2 * k.n_union;
 #pragma unroll 1
-    for (int i = 0; i < items; ++i) {
-      const bool v_item = p8_is_v(i, items);
-      const int x = p8_tile(i, items), st = (item0 + i) % kStages, slot = (tiles0 + x) % kP8Slots;
-      const uint32_t ph = (item0 + i) / kStages & 1u;
-      bool ok = v_item || p8_wait(&ctrl->e_full[slot], (tiles0 + x) / kP8Slots & 1u, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
-      ok = ok && p8_wait(&ctrl->raw_full[st], ph, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
-      ok = ok && p8_wait(&ctrl->kv_empty[st], ph ^ 1u, abort_flag, p.status, ERR_WAIT_SMEM_EMPTY);
-      if (!__all_sync(kAll, ok)) {
-        alive = false;
-        break;
-      }
-      // factor of token `lane` of the page
-      const int pages = ctrl->pages[slot], byte = ctrl->bytes[slot][v_item][warp * kQ8Page + lane];
-      const bool whole = pages & 16;
-      uint32_t fac = f16x2_pow2(q8_log2_of(byte) - (v_item ? ctrl->e_v[slot] : ctrl->e_k[slot]) + int(kP8Lift));
-      const int tok0 = (k.u_lo + x) * kP8Tile + warp * kQ8Page;
-      if (!whole) {
-        // NaN, K's or V's, is one of the scores: a row that does not see the token must not meet it in a product
-        const bool none = byte == 255 || ctrl->bytes[slot][!v_item][warp * kQ8Page + lane] == 255;
-        if (none) fac = v_item ? 0u : 0x7fff7fffu;
-        if (tok0 + lane < vis_lo || tok0 + lane >= vis_hi) fac = 0u;
-      }
-      const int lo = vis_lo - tok0 - row_of, hi = (pages >> warp) & 1 ? vis_hi - tok0 - row_of : -kQ8Page;
-      const uint8_t* from = from0 + st * 4 * L::kPageBytes;
-      const uint32_t to = to0 + st * L::kTile;
-      // four loads at a time, then their stores (a load behind a store would wait for it)
-      constexpr int kAhead = 4;
-#pragma unroll
-      for (int j0 = 0; j0 < kSteps; j0 += kAhead) {
-        uint2 ra[kAhead], rc[kAhead];
-        uint32_t f[kAhead];
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-          const uint8_t* at = from + (j0 + j) * 512;
-          ra[j] = *reinterpret_cast<const uint2*>(at);
-          rc[j] = *reinterpret_cast<const uint2*>(odd ? at - 8 : at + 8);
+      for (int i = 0; i < items; ++i) {
+        const bool v_item = p8_is_v(i, items);
+        const int x = p8_tile(i, items), st = (item0 + i) % kStages, slot = (tiles0 + x) % kP8Slots;
+        const uint32_t ph = (item0 + i) / kStages & 1u;
+        bool ok = v_item || p8_wait(&ctrl->e_full[slot], (tiles0 + x) / kP8Slots & 1u, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
+        ok = ok && p8_wait(&ctrl->raw_full[st], ph, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
+        ok = ok && p8_wait(&ctrl->kv_empty[st], ph ^ 1u, abort_flag, p.status, ERR_WAIT_SMEM_EMPTY);
+        if (!__all_sync(kAll, ok)) {
+          alive = false;
+          break;
         }
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j) f[j] = __shfl_sync(kAll, fac, (j0 + j) * kRows + row_of);
-        if (!whole) {                                              // what no row sees may be anything
-#pragma unroll
-          for (int j = 0; j < kAhead; ++j)
-            if ((j0 + j) * kRows < lo || (j0 + j) * kRows >= hi) ra[j] = rc[j] = make_uint2(0u, 0u);
+        // factor of token `lane` of the page
+        const int pages = ctrl->pages[slot], byte = ctrl->bytes[slot][v_item][warp * kQ8Page + lane];
+        const bool whole = pages & 16;
+        uint32_t fac = f16x2_pow2(q8_log2_of(byte) - (v_item ? ctrl->e_v[slot] : ctrl->e_k[slot]) + int(kP8Lift));
+        const int tok0 = (k.u_lo + x) * kP8Tile + warp * kQ8Page;
+        if (!whole) {
+          // NaN, K's or V's, is one of the scores: a row that does not see the token must not meet it in a product
+          const bool none = byte == 255 || ctrl->bytes[slot][!v_item][warp * kQ8Page + lane] == 255;
+          if (none) fac = v_item ? 0u : 0x7fff7fffu;
+          if (tok0 + lane < vis_lo || tok0 + lane >= vis_hi) fac = 0u;
         }
+        const int lo = vis_lo - tok0 - row_of, hi = (pages >> warp) & 1 ? vis_hi - tok0 - row_of : -kQ8Page;
+        const uint8_t* from = from0 + st * 4 * L::kPageBytes;
+        const uint32_t to = to0 + st * L::kTile;
+        // four loads at a time, then their stores (a load behind a store would wait for it)
+        constexpr int kAhead = 4;
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-          const uint4 a = make_uint4(hmul2(e4m3x2_to_f16x2(uint16_t(ra[j].x)), f[j]), hmul2(e4m3x2_to_f16x2(uint16_t(ra[j].x >> 16)), f[j]),
-                                     hmul2(e4m3x2_to_f16x2(uint16_t(ra[j].y)), f[j]), hmul2(e4m3x2_to_f16x2(uint16_t(ra[j].y >> 16)), f[j]));
-          const uint4 c = make_uint4(hmul2(e4m3x2_to_f16x2(uint16_t(rc[j].x)), f[j]), hmul2(e4m3x2_to_f16x2(uint16_t(rc[j].x >> 16)), f[j]),
-                                     hmul2(e4m3x2_to_f16x2(uint16_t(rc[j].y)), f[j]), hmul2(e4m3x2_to_f16x2(uint16_t(rc[j].y >> 16)), f[j]));
-          // rows four on: bit 2 of the swizzle
-          const uint32_t at = (to ^ (kRows == 4 && (j & 1) ? 64u : 0u)) + (j0 + j) * kRows * 128;
-          st_shared_16(at, a);
-          st_shared_16(at ^ 16u, c);
+        for (int j0 = 0; j0 < kSteps; j0 += kAhead) {
+          uint2 ra[kAhead], rc[kAhead];
+          uint32_t f[kAhead];
+#pragma unroll
+          for (int j = 0; j < kAhead; ++j) {
+            const uint8_t* at = from + (j0 + j) * 512;
+            ra[j] = *reinterpret_cast<const uint2*>(at);
+            rc[j] = *reinterpret_cast<const uint2*>(odd ? at - 8 : at + 8);
+          }
+#pragma unroll
+          for (int j = 0; j < kAhead; ++j) f[j] = __shfl_sync(kAll, fac, (j0 + j) * kRows + row_of);
+          if (!whole) {                                              // what no row sees may be anything
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j)
+              if ((j0 + j) * kRows < lo || (j0 + j) * kRows >= hi) ra[j] = rc[j] = make_uint2(0u, 0u);
+          }
+#pragma unroll
+          for (int j = 0; j < kAhead; ++j) {
+            const uint4 a = make_uint4(hmul2(e4m3x2_to_f16x2(uint16_t(ra[j].x)), f[j]), hmul2(e4m3x2_to_f16x2(uint16_t(ra[j].x >> 16)), f[j]),
+                                       hmul2(e4m3x2_to_f16x2(uint16_t(ra[j].y)), f[j]), hmul2(e4m3x2_to_f16x2(uint16_t(ra[j].y >> 16)), f[j]));
+            const uint4 c = make_uint4(hmul2(e4m3x2_to_f16x2(uint16_t(rc[j].x)), f[j]), hmul2(e4m3x2_to_f16x2(uint16_t(rc[j].x >> 16)), f[j]),
+                                       hmul2(e4m3x2_to_f16x2(uint16_t(rc[j].y)), f[j]), hmul2(e4m3x2_to_f16x2(uint16_t(rc[j].y >> 16)), f[j]));
+            // rows four on: bit 2 of the swizzle
+            const uint32_t at = (to ^ (kRows == 4 && (j & 1) ? 64u : 0u)) + (j0 + j) * kRows * 128;
+            st_shared_16(at, a);
+            st_shared_16(at ^ 16u, c);
+          }
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&ctrl->kv_full[st]);
+          mbar_arrive(&ctrl->raw_empty[st]);
+          if (v_item) mbar_arrive(&ctrl->e_empty[slot]);
         }
       }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&ctrl->kv_full[st]);
-        mbar_arrive(&ctrl->raw_empty[st]);
-        if (v_item) mbar_arrive(&ctrl->e_empty[slot]);
-      }
-    }
-    item0 += items;
-    tiles0 += k.n_union;
+      item0 += items;
+      tiles0 += k.n_union;
     }
   } else if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == 15) {
       // -------------------------------------------------------------- pages: lanes 0 to 3 a page of the item each
       // and the works: a CTA's first has its number, the others come from a counter of the grid.  The last rows of all sequences first, those
@@ -599,11 +599,12 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- softmax, one thread per row
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     const int t = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane;
     const uint32_t lane_off = uint32_t(quad * 32) << 16;
     const uint32_t s_addr = tmem_base + lane_off + kSCol + t * 128, o_addr = tmem_base + lane_off + kOCol + t * 128;
     uint8_t* my_p = p_s + t * L::kP + r * 128;
+    const P8Rows<D> q_rows(q_s + t * L::kTile + quad * 32 * 128, lane);
     // a row of a work: (token, head of the group)
     struct Row {
       int tile_lo, n_tiles, lo_pos, hi_pos, head, x0;     // x0: walk position of its first tile
@@ -623,99 +624,99 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
       float m = -INFINITY, l = 0.f;
       if (have) {
         const int n_tiles = cur.n_tiles, hi_pos = cur.hi_pos, lo_pos = cur.lo_pos;
-    for (int it = 0; it < n_tiles; ++it) {
-      const uint32_t x = cur.tiles0 + cur.x0 + it;
-      const int kv0 = (cur.tile_lo + it) * kP8Tile;
-      bool ok = p8_wait(&ctrl->e_full[x % kP8Slots], x / kP8Slots & 1u, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
-      ok = ok && p8_wait(&ctrl->s_full[t], done + it & 1u, abort_flag, p.status, ERR_WAIT_TMEM_FULL);
-      if (!__all_sync(kAll, ok)) { alive = false; break; }
-      const int e_k = *(volatile int*)&ctrl->e_k[x % kP8Slots], e_v = *(volatile int*)&ctrl->e_v[x % kP8Slots];
-      const float to_log2 = cur.raw_log2 * exp2_int(e_k - int(kP8Lift)), add = float(e_v);
-      tc_fence_after();
-      uint32_t v[kP8Tile];
-#pragma unroll
-      for (int c = 0; c < kP8Tile / 32; ++c) tmem_ld_32x32(s_addr + c * 32, reinterpret_cast<uint32_t(&)[32]>(v[c * 32]));
-      tmem_ld_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&ctrl->s_empty[t]);      // the scores (and the tile's exponents) are in registers
-      const bool edge = kv0 + kP8Tile - 1 > hi_pos || kv0 < lo_pos;
-      if (__any_sync(kAll, edge)) {
-        const int hi_rel = hi_pos - kv0, lo_rel = lo_pos - kv0;
-#pragma unroll
-        for (int i = 0; i < kP8Tile; ++i)
-          if (i > hi_rel || i < lo_rel) v[i] = 0xff800000u;
-      }
-      float mx4[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) mx4[i] = fmaxf(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-#pragma unroll
-      for (int i = 8; i < kP8Tile; i += 2) mx4[(i >> 1) & 3] = fmax3(mx4[(i >> 1) & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-      const float mx = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), to_log2, add);
-      bool p_free = it == 0;
-      if (it == 0) {
-        m = mx;
-      } else {
-        const bool grow = mx > m + kP8Grow;
-        if (__any_sync(kAll, grow)) {
-          ok = p8_wait(&ctrl->o_full[t], done + it - 1 & 1u, abort_flag, p.status, ERR_WAIT_TMEM_FULL);
+        for (int it = 0; it < n_tiles; ++it) {
+          const uint32_t x = cur.tiles0 + cur.x0 + it;
+          const int kv0 = (cur.tile_lo + it) * kP8Tile;
+          bool ok = p8_wait(&ctrl->e_full[x % kP8Slots], x / kP8Slots & 1u, abort_flag, p.status, ERR_WAIT_SMEM_FULL);
+          ok = ok && p8_wait(&ctrl->s_full[t], done + it & 1u, abort_flag, p.status, ERR_WAIT_TMEM_FULL);
           if (!__all_sync(kAll, ok)) { alive = false; break; }
-          p_free = true;
+          const int e_k = *(volatile int*)&ctrl->e_k[x % kP8Slots], e_v = *(volatile int*)&ctrl->e_v[x % kP8Slots];
+          const float to_log2 = cur.raw_log2 * exp2_int(e_k - int(kP8Lift)), add = float(e_v);
           tc_fence_after();
-          const float alpha = grow ? exp2f(m - mx) : 1.f;
-#pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld_32x32(o_addr + c * 32, o);
-            tmem_ld_wait();
+          uint32_t v[kP8Tile];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-            tmem_st_32x32(o_addr + c * 32, o);
+          for (int c = 0; c < kP8Tile / 32; ++c) tmem_ld_32x32(s_addr + c * 32, reinterpret_cast<uint32_t(&)[32]>(v[c * 32]));
+          tmem_ld_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctrl->s_empty[t]);      // the scores (and the tile's exponents) are in registers
+          const bool edge = kv0 + kP8Tile - 1 > hi_pos || kv0 < lo_pos;
+          if (__any_sync(kAll, edge)) {
+            const int hi_rel = hi_pos - kv0, lo_rel = lo_pos - kv0;
+#pragma unroll
+            for (int i = 0; i < kP8Tile; ++i)
+              if (i > hi_rel || i < lo_rel) v[i] = 0xff800000u;
           }
-          tmem_st_wait();
-          l *= alpha;
-          if (grow) m = mx;
+          float mx4[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx4[i] = fmaxf(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+#pragma unroll
+          for (int i = 8; i < kP8Tile; i += 2) mx4[(i >> 1) & 3] = fmax3(mx4[(i >> 1) & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+          const float mx = fmaf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), to_log2, add);
+          bool p_free = it == 0;
+          if (it == 0) {
+            m = mx;
+          } else {
+            const bool grow = mx > m + kP8Grow;
+            if (__any_sync(kAll, grow)) {
+              ok = p8_wait(&ctrl->o_full[t], done + it - 1 & 1u, abort_flag, p.status, ERR_WAIT_TMEM_FULL);
+              if (!__all_sync(kAll, ok)) { alive = false; break; }
+              p_free = true;
+              tc_fence_after();
+              const float alpha = grow ? exp2f(m - mx) : 1.f;
+#pragma unroll 1
+              for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld_32x32(o_addr + c * 32, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                tmem_st_32x32(o_addr + c * 32, o);
+              }
+              tmem_st_wait();
+              l *= alpha;
+              if (grow) m = mx;
+            }
+          }
+          const float less = add + kP8Lift - (m == -INFINITY ? 0.f : m);
+          const float2 sc2 = make_float2(to_log2, to_log2), nb2 = make_float2(less, less);
+          float2 sum2[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum2[i] = make_float2(0.f, 0.f);
+          if (!p_free) {
+            ok = p8_wait(&ctrl->o_full[t], done + it - 1 & 1u, abort_flag, p.status, ERR_WAIT_TMEM_FULL);
+            if (!__all_sync(kAll, ok)) { alive = false; break; }
+          }
+          // turns with the exponentials, where both query tiles have one: tile 0 (it), tile 1 (it), tile 0 (it + 1), ..., over all works
+          if (it < cur.paired && (t == 1 || pairs + it > 0)) {
+            ok = p8_wait(&ctrl->turn[t][quad], pairs + it - (t == 0 ? 1 : 0) & 1u, abort_flag, p.status, ERR_WAIT_SOFTMAX);
+            if (!__all_sync(kAll, ok)) { alive = false; break; }
+          }
+#pragma unroll
+          for (int c = 0; c < kP8Tile / 32; ++c) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int k = c * 32 + 2 * i;
+              const float2 y = ffma2(make_float2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), sc2, nb2);
+              const float2 e = make_float2(exp2f(y.x), exp2f(y.y));
+              sum2[i & 3] = fadd2(sum2[i & 3], e);
+              pk[i] = p8_pack_f16x2(e.x, e.y);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              *reinterpret_cast<uint4*>(my_p + (c >> 1) * kHalf + ((((c & 1) * 4 + q) ^ (r & 7)) << 4)) =
+                  make_uint4(pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
+          }
+          __syncwarp();
+          if (lane == 0 && it < cur.paired) mbar_arrive(&ctrl->turn[1 - t][quad]);
+          fence_proxy_async();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctrl->p_full[t]);
+          const float2 s4 = fadd2(fadd2(sum2[0], sum2[1]), fadd2(sum2[2], sum2[3]));
+          l = fmaf(s4.x + s4.y, exp2_int(-e_v), l);
         }
-      }
-      const float less = add + kP8Lift - (m == -INFINITY ? 0.f : m);
-      const float2 sc2 = make_float2(to_log2, to_log2), nb2 = make_float2(less, less);
-      float2 sum2[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sum2[i] = make_float2(0.f, 0.f);
-      if (!p_free) {
-        ok = p8_wait(&ctrl->o_full[t], done + it - 1 & 1u, abort_flag, p.status, ERR_WAIT_TMEM_FULL);
-        if (!__all_sync(kAll, ok)) { alive = false; break; }
-      }
-      // turns with the exponentials, where both query tiles have one: tile 0 (it), tile 1 (it), tile 0 (it + 1), ..., over all works
-      if (it < cur.paired && (t == 1 || pairs + it > 0)) {
-        ok = p8_wait(&ctrl->turn[t][quad], pairs + it - (t == 0 ? 1 : 0) & 1u, abort_flag, p.status, ERR_WAIT_SOFTMAX);
-        if (!__all_sync(kAll, ok)) { alive = false; break; }
-      }
-#pragma unroll
-      for (int c = 0; c < kP8Tile / 32; ++c) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int k = c * 32 + 2 * i;
-          const float2 y = ffma2(make_float2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), sc2, nb2);
-          const float2 e = make_float2(exp2f(y.x), exp2f(y.y));
-          sum2[i & 3] = fadd2(sum2[i & 3], e);
-          pk[i] = p8_pack_f16x2(e.x, e.y);
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<uint4*>(my_p + (c >> 1) * kHalf + ((((c & 1) * 4 + q) ^ (r & 7)) << 4)) =
-              make_uint4(pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
-      }
-      __syncwarp();
-      if (lane == 0 && it < cur.paired) mbar_arrive(&ctrl->turn[1 - t][quad]);
-      fence_proxy_async();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&ctrl->p_full[t]);
-      const float2 s4 = fadd2(fadd2(sum2[0], sum2[1]), fadd2(sum2[2], sum2[3]));
-      l = fmaf(s4.x + s4.y, exp2_int(-e_v), l);
-    }
       }
       // ---- queries of the next work, ahead of this one's result: the products of this one with Q have been read
       bool more = false;
@@ -744,19 +745,18 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
         const int q_pos = k.ctx - k.q_len + token;
         next.hi_pos = p.causal ? min(k.ctx - 1, q_pos) : k.ctx - 1;
         next.lo_pos = nkb_first_visible(q_pos, p.window, p.chunk);
-        const P8Rows<D> rows(q_s + t * L::kTile + quad * 32 * 128, lane);
         uint4 v[D / 8];
         float mx = 0.f;
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
-          const long long at = __shfl_sync(kAll, next.at, i * rows.kRows + rows.row);
-          v[i] = at >= 0 ? reinterpret_cast<const uint4*>(p.q + at * D)[rows.piece] : make_uint4(0u, 0u, 0u, 0u);
+          const long long at = __shfl_sync(kAll, next.at, i * q_rows.kRows + q_rows.row);
+          v[i] = at >= 0 ? reinterpret_cast<const uint4*>(p.q + at * D)[q_rows.piece] : make_uint4(0u, 0u, 0u, 0u);
         }
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) *rows.wide(i * rows.kRows) = v[i];
+        for (int i = 0; i < D / 8; ++i) *q_rows.wide(i * q_rows.kRows) = v[i];
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) v[i] = *rows.own(i);
+        for (int i = 0; i < D / 8; ++i) v[i] = *q_rows.own(i);
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
           const uint32_t q4[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
@@ -778,7 +778,7 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
             const float2 f = unpack_bf16x2(q4[j]);
             h[j] = p8_pack_f16x2(f.x * up, f.y * up);
           }
-          *rows.own(i) = make_uint4(h[0], h[1], h[2], h[3]);
+          *q_rows.own(i) = make_uint4(h[0], h[1], h[2], h[3]);
         }
         fence_proxy_async();
         __syncwarp();
