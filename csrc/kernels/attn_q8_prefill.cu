@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
     // the other way round, so that all banks are used
     const int odd = NH == 2 ? piece >> 2 : 0;
     const uint32_t to0 = smem_u32(kv_s) + (piece >> 2) * kHalf + (warp * kQ8Page + row_of) * 128 + ((((piece & 3) * 2 + odd) ^ row_of) << 4);
-    const uint8_t* from0 = raw_s + warp * L::kPageBytes + lane * 16 + odd * 8;
+    const uint8_t* from0 = raw_s + warp * L::kPageBytes + lane * 16;
     uint32_t item0 = 0, tiles0 = 0;                                // ring items and tiles of the works before
     uint32_t n_works = 0;
     bool alive = true;
@@ -339,8 +339,9 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
 #pragma unroll
           for (int j = 0; j < kAhead; ++j) {
             const uint8_t* at = from + (j0 + j) * 512;
-            ra[j] = *reinterpret_cast<const uint2*>(at);
-            rc[j] = *reinterpret_cast<const uint2*>(odd ? at - 8 : at + 8);
+            const uint4 both = *reinterpret_cast<const uint4*>(at);
+            ra[j] = odd ? make_uint2(both.z, both.w) : make_uint2(both.x, both.y);
+            rc[j] = odd ? make_uint2(both.x, both.y) : make_uint2(both.z, both.w);
           }
 #pragma unroll
           for (int j = 0; j < kAhead; ++j) f[j] = __shfl_sync(kAll, fac, (j0 + j) * kRows + row_of);
