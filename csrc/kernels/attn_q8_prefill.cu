@@ -12,10 +12,11 @@
 //   warp 14      reads the scales of the tiles to come and finds K and V
 //   warp 15      fetches the pages, by bulk copies
 //
-// f16 holds an e4m3 value times 2^-22 and up exactly or nearly (from 2^6 down, behind the tile's largest), so the products see what is
-// kept.  A tile's exponents are two numbers that enter where one number did before: 2^K in the multiplier of the scores, V in the exponent
-// of the weights, 2^-V where the weights are summed.  Nothing is added per score.  There is no MMA of 16-bit queries with e4m3 keys, and keys
-// in two parts on the 8-bit MMA would double the products.
+// An e4m3 value is a multiple of 2^-9 and f16's steps end at 2^-24: with the tile's largest scale brought to 2^6, f16 holds the values of
+// tokens down to 2^-21 of that scale exactly, and is off by 2^-25 at most (2^-38 of the largest value) below.  A tile's exponents are two
+// numbers that enter where one number did before: 2^K in the multiplier of the scores, V in the exponent of the weights, 2^-V where the
+// weights are summed.  Nothing is added per score.  There is no MMA of 16-bit queries with e4m3 keys, and keys in two parts on the 8-bit MMA
+// would double the products.
 //
 // Rows of a query tile are (token, head of the group): short prompts fill tiles, and a tile's rows end close to one another.  Queries become
 // f16 as they are loaded, each row scaled below 2^15 by a power of two.

@@ -64,7 +64,7 @@ class _TimedLib:
                   "nkb_embedding", "nkb_rope", "nkb_decode_advance", "nkb_sample", "nkb_router", "nkb_paged_attn_decode",
                   "nkb_flash", "nkb_ag_gemm", "nkb_decode_gemm", "nkb_lmhead", "nkb_gated", "nkb_hgrn2", "nkb_maps",
                   "nkb_linattn", "nkb_low_rank", "nkb_token_mix", "nkb_gate_heads", "nkb_row_norm",
-                  "nkb_latent", "nkb_softcap", "nkb_post", "nkb_short_conv", "nkb_head_rec")
+                  "nkb_latent", "nkb_softcap", "nkb_post", "nkb_short_conv", "nkb_head_rec", "nkb_q8")
 
     def __init__(self, real):
         object.__setattr__(self, "_real", real)

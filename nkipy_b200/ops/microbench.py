@@ -21,7 +21,7 @@ import torch
 
 from . import (add_rmsnorm, decode_linear, flash_attn_prefill, grouped_linear, linear, moe_combine, moe_dispatch,
                paged_attn_decode, router_topk)
-from . import microbench_mixers, microbench_sandwich
+from . import microbench_mixers, microbench_quantized, microbench_sandwich
 
 _FALLBACK = {"hbm_gbs": 6650.0, "bf16_tflops": 1590.0}
 
@@ -400,7 +400,7 @@ CASES = {
     "add-rmsnorm": case_addnorm,
 }
 CASES.update({name: (lambda a, fn=fn: fn(a, _time, _sets_for))
-              for name, fn in {**microbench_mixers.CASES, **microbench_sandwich.CASES}.items()})
+              for name, fn in {**microbench_mixers.CASES, **microbench_sandwich.CASES, **microbench_quantized.CASES}.items()})
 
 
 def main(argv=None):
@@ -411,13 +411,13 @@ def main(argv=None):
     ap.add_argument("--no-graph", action="store_true", help="launch eagerly instead of replaying a CUDA graph")
     ap.add_argument("--sets", type=int, default=8, help="upper bound of rotating operand sets")
     ap.add_argument("--splits", type=int, default=0, help="override the split-K factor of the gemm-decode-* cases")
-    ap.add_argument("--kv-splits", type=int, default=0, help="split-KV factor of attn-decode (0 = heuristic)")
+    ap.add_argument("--kv-splits", type=int, default=0, help="split-KV factor of attn-decode and quantized-attn-decode (0 = heuristic)")
     ap.add_argument("--tokens", type=int, default=0, help="override the token count of the gemm-decode-* cases")
     ap.add_argument("--impl", default="splitk", choices=["fixup", "cluster", "splitk"],
                     help="gemm-decode-*: fixup / cluster = split-K summed inside the kernel (last-arriver fix-up / "
                          "CTA clusters), splitk = fp32 partials left to the next kernel")
-    ap.add_argument("--batch", type=int, default=0, help="attn-prefill: sequences (default 8)")
-    ap.add_argument("--seq", type=int, default=0, help="attn-prefill: tokens per sequence, a multiple of 32 (default 2048)")
+    ap.add_argument("--batch", type=int, default=0, help="attn-prefill, quantized-attn-prefill: sequences (default 8)")
+    ap.add_argument("--seq", type=int, default=0, help="the same: tokens per sequence, a multiple of 32 (default 2048)")
     ap.add_argument("--tp", type=int, default=1, help="gemm-decode-*: per-rank shard of an N-way tensor-parallel layer")
     args = ap.parse_args(argv)
     if not torch.cuda.is_available():

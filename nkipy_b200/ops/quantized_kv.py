@@ -284,6 +284,7 @@ def _p(t: Optional[torch.Tensor]) -> int:
 _APPEND, _ATTN = struct.Struct("14Pqd8i"), struct.Struct("13Pq12ifi")
 
 
+MAX_SPLITS = 1024
 COUNTERS = 16384                     # words of the scratch of attention that count
 _SCRATCH = {}
 
@@ -309,11 +310,12 @@ def _pick_splits(ctas: int, max_pages: int, sms: int = 148) -> int:
 
 
 def _splits(num_splits: int, scratch, B: int, nkv: int, D: int, group: int, max_pages: int, device):
-    """(parts of a sequence, address of scratch for their results)."""
+    """(parts of a sequence, scratch for their results or None).  The caller holds the scratch until the launch: a graph's own is free for
+    another tensor of the call otherwise."""
     if num_splits <= 0:
         num_splits = _pick_splits(B * nkv, max_pages)
     if num_splits <= 1:
-        return 1, 0
+        return 1, None
     need = _lib.lib().nkb_q8_attn_decode_scratch_floats(B, nkv, D, group, num_splits)
     if scratch is None:
         scratch = _scratch(device, need)
@@ -321,7 +323,7 @@ def _splits(num_splits: int, scratch, B: int, nkv: int, D: int, group: int, max_
           or scratch.data_ptr() & 15):
         raise ValueError(f"scratch wants {need} contiguous fp32 values on {device} from 16 bytes on, the first {COUNTERS} zero before "
                          "the first call")
-    return num_splits, scratch.data_ptr()
+    return num_splits, scratch
 
 
 def decode_scratch(pages: QuantizedPages, nq: int, max_batch: int, max_pages: int) -> Optional[torch.Tensor]:
@@ -367,8 +369,8 @@ def paged_attn_decode(q, k_cache, v_cache, block_table, context_lens, scale, *, 
     nq = q.shape[-1] // D
     group = _check_heads(nq, nkv)
     _check_masks(mods, window, chunk, sinks, nq, index)
-    if q_len < 1:
-        raise ValueError("q_len is at least one")
+    if q_len < 1 or num_splits > MAX_SPLITS:
+        raise ValueError(f"q_len is at least one, num_splits at most {MAX_SPLITS}")
     q_at = _want_rows(q, "q", (B * q_len, nq * D), index)
     out = _result(out, q, index)
     if not B:
@@ -385,7 +387,7 @@ def paged_attn_decode(q, k_cache, v_cache, block_table, context_lens, scale, *, 
                                   max_q_len=q_len, window=window, chunk=chunk, sinks=sinks, out=out)
     num_splits, scratch = _splits(num_splits, scratch, B, nkv, D, group, width, k_cache.device)
     rc = _lib.lib().nkb_q8_attn_decode(_ATTN.pack(
-        q_at, *k_cache.at, *v_cache.at, block_table.data_ptr(), 0, 0, context_lens.data_ptr(), out.data_ptr(), _p(sinks), scratch, _stream(),
+        q_at, *k_cache.at, *v_cache.at, block_table.data_ptr(), 0, 0, context_lens.data_ptr(), out.data_ptr(), _p(sinks), _p(scratch), _stream(),
         block_table.stride(0), B, B * q_len, q_len, nq, nkv, D, blocks, width, 1, window, chunk, num_splits, scale, 0))
     if rc:
         _lib.check(rc, "nkb_q8_attn_decode")
@@ -397,7 +399,8 @@ def rope_attn_decode(qkv_partials, positions, slots, cos_sin, k_cache, v_cache, 
                      q_norm_w=None, k_norm_w=None, norm_eps=1e-6, window=0, sinks=None, num_splits=0, scratch=None,
                      out=None) -> torch.Tensor:
     """`ops.rope_attn_decode` over quantised pages: `rope_kv_append`, and attention that fetches the older pages meanwhile.  The new token
-    takes part as it is kept, in 8 bits.  slots[b] is the place of sequence b's position context_lens[b] - 1, or negative."""
+    takes part as it is kept, in 8 bits.  slots[b] is the place of sequence b's position context_lens[b] - 1, which no other sequence of the
+    call sees, or negative."""
     blocks, _, D = _pair(k_cache, v_cache)
     index = k_cache.index
     B, width = _check_table(block_table, context_lens, index)
@@ -410,17 +413,20 @@ def rope_attn_decode(qkv_partials, positions, slots, cos_sin, k_cache, v_cache, 
                                  scratch=scratch, out=out)
     _, parts, stride, rows = _check_qkv(qkv_partials, positions, slots, cos_sin, k_cache, nq, nkv, D, bias, q_norm_w, k_norm_w)
     _check_masks(None, window, 0, sinks, nq, index)
+    if num_splits > MAX_SPLITS:
+        raise ValueError(f"num_splits is at most {MAX_SPLITS}")
     if out is None:
         out = torch.empty((B, nq * D), dtype=torch.bfloat16, device=k_cache.device)
     else:
         _want_rows(out, "out", (B, nq * D), index)
     _on_gpu(index)
     num_splits, scratch = _splits(num_splits, scratch, B, nkv, D, nq // nkv, width, k_cache.device)
-    q, stream, pages = torch.empty_like(out).data_ptr(), _stream(), (*k_cache.at, *v_cache.at)
+    q = torch.empty_like(out)
+    q_at, stream, pages = q.data_ptr(), _stream(), (*k_cache.at, *v_cache.at)
     rc = _lib.lib().nkb_q8_step(
-        _APPEND.pack(0, qkv_partials.data_ptr(), _p(bias), _p(positions), _p(slots), _p(cos_sin), _p(q_norm_w), _p(k_norm_w), q, *pages, stream,
+        _APPEND.pack(0, qkv_partials.data_ptr(), _p(bias), _p(positions), _p(slots), _p(cos_sin), _p(q_norm_w), _p(k_norm_w), q_at, *pages, stream,
                      stride, norm_eps, parts, B, nq, nkv, D, rows, blocks, 0),
-        _ATTN.pack(q, *pages, block_table.data_ptr(), 0, 0, context_lens.data_ptr(), out.data_ptr(), _p(sinks), scratch, stream,
+        _ATTN.pack(q_at, *pages, block_table.data_ptr(), 0, 0, context_lens.data_ptr(), out.data_ptr(), _p(sinks), _p(scratch), stream,
                    block_table.stride(0), B, B, 1, nq, nkv, D, blocks, width, 1, window, 0, num_splits, scale, 0))
     if rc:
         _lib.check(rc, "nkb_q8_step")
@@ -455,9 +461,10 @@ def flash_attn_prefill(q, k_cache, v_cache, block_table, q_start, q_lens, contex
         return out
     L = _lib.lib()
     floats = L.nkb_q8_attn_prefill_scratch_floats(B, max_q_len, nq, nkv, D, width)
+    scratch = _scratch(k_cache.device, floats)
     rc = L.nkb_q8_attn_prefill(_ATTN.pack(
         q_at, *k_cache.at, *v_cache.at, block_table.data_ptr(), q_start.data_ptr(), q_lens.data_ptr(), context_lens.data_ptr(), out.data_ptr(),
-        _p(sinks), _scratch(k_cache.device, floats).data_ptr(), _stream(), block_table.stride(0), B, total, max_q_len, nq, nkv, D, blocks,
+        _p(sinks), scratch.data_ptr(), _stream(), block_table.stride(0), B, total, max_q_len, nq, nkv, D, blocks,
         width, 1 if causal else 0, window, chunk, 1, scale, 0))
     if rc:
         _lib.check(rc, "nkb_q8_attn_prefill")

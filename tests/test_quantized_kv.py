@@ -442,6 +442,170 @@ def test_step_is_append_and_attention(device, nq, nkv, dim, splits, norm, bias, 
                     nq // nkv, None if sinks is None else sinks.cpu(), **masks)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_values_that_are_not_finite_stay_with_their_head_and_token(device):
+    """From the projection through the pages to attention: what is not finite reaches the rows that see it, and no others."""
+    g = torch.Generator().manual_seed(77)
+    nq, nkv, dim, n = 4, 2, 64, 40
+    k, v = pool(g, 3, nkv, dim, device)
+    table, slots = torch.tensor([[2, 0]], dtype=torch.int32), torch.cat([torch.arange(64, 96), torch.arange(8)]).int()
+    x = torch.randn((n, (nq + 2 * nkv) * dim), generator=g).to(torch.bfloat16)
+    head = x.view(n, nq + 2 * nkv, dim)
+    head[30, nq, 5], head[35, nq + nkv + 1, 63], head[20, 1, 7] = math.inf, math.nan, math.nan      # K of head 0, V of head 1, a query
+    cs, i32 = rope_table(dim, n), lambda t: torch.tensor(t, dtype=torch.int32, device=device)       # noqa: E731
+    q = ops.rope_kv_append(x.to(device), torch.arange(n, dtype=torch.int32).to(device), slots.to(device), cs.to(device), k, v, nq, nkv, dim)
+    out = ops.flash_attn_prefill(q, k, v, table.to(device), i32([0]), i32([n]), i32([n]), 0.125, max_q_len=n).view(n, nq, dim).cpu()
+    lost = torch.zeros((n, nq), dtype=torch.bool)
+    lost[30:, :2], lost[35:, 2:], lost[20, 1] = True, True, True
+    assert torch.equal(out.isnan().any(-1), lost) and torch.equal(out.isnan().all(-1), lost)
+    last = ops.paged_attn_decode(q[-1:], k, v, table.to(device), i32([n]), 0.125, window=5).view(nq, dim).cpu()
+    assert bool(last[:2].isfinite().all()) and bool(last[2:].isnan().all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_tables_that_are_part_of_larger_ones(device):
+    g = torch.Generator().manual_seed(78)
+    nq, nkv, dim, contexts = 4, 2, 64, [70, 1, 600]
+    table, blocks = shuffled_table(g, contexts)
+    k, v = pool(g, blocks, nkv, dim, device)
+    wide = torch.full((5, table.shape[1] + 7), -9, dtype=torch.int32)
+    wide[1:4, 3:3 + table.shape[1]] = table
+    part = wide.to(device)[1:4, 3:3 + table.shape[1]]
+    q = torch.randn((3, nq * dim), generator=g).to(torch.bfloat16)
+    lens, one = torch.tensor(contexts, dtype=torch.int32, device=device), torch.ones(3, dtype=torch.int32, device=device)
+    spans = [(b, 1, c) for b, c in enumerate(contexts)]
+    for out in (ops.paged_attn_decode(q.to(device), k, v, part, lens, 0.125), ops.paged_attn_decode(q.to(device), k, v, part, lens, 0.125, num_splits=3),
+                ops.flash_attn_prefill(q.to(device), k, v, part, torch.arange(3, dtype=torch.int32, device=device), one, lens, 0.125, max_q_len=1)):
+        check_attention(out.view(3, nq, dim), q.view(3, nq, dim), k, v, table, spans, 0.125, nq, nq // nkv)
+    # one row for all sequences
+    same = table[2:].to(device).expand(3, -1)
+    out = ops.paged_attn_decode(q.to(device), k, v, same, lens, 0.125)
+    check_attention(out.view(3, nq, dim), q.view(3, nq, dim), k, v, table[2:].expand(3, -1), spans, 0.125, nq, nq // nkv)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_packed_steps(device):
+    """Single tokens first, then prompts, then rows of padding."""
+    g = torch.Generator().manual_seed(79)
+    nq, nkv, dim = 4, 2, 128
+    spans = [(0, 1, 40), (1, 1, 333), (2, 1, 1), (3, 50, 50), (53, 20, 90)]
+    table, blocks = shuffled_table(g, [c for *_, c in spans])
+    k, v = pool(g, blocks, nkv, dim, device)
+    q = torch.randn((80, nq * dim), generator=g).to(torch.bfloat16)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)        # noqa: E731
+    out = ops.packed_attention(q.to(device), k, v, table.to(device), i32([s for s, *_ in spans]), i32([n for _, n, _ in spans]),
+                               i32([c for *_, c in spans]), dim ** -0.5, max_q_len=50, singles=3)
+    check_attention(out.view(80, nq, dim), q.view(80, nq, dim), k, v, table, spans, dim ** -0.5, nq, nq // nkv)
+
+
+class Work:
+    """Appended tokens, a step, decode attention in parts and prompts in parts, over pages of their own."""
+
+    def __init__(self, seed):
+        g = torch.Generator().manual_seed(seed)
+        self.nq, self.nkv, self.dim, contexts = 4, 2, 128, [900, 33, 2000]
+        self.contexts = contexts
+        table, blocks = shuffled_table(g, contexts)
+        self.k, self.v = pool(g, blocks, self.nkv, self.dim, "cuda")
+        W = (self.nq + 2 * self.nkv) * self.dim
+        self.parts, self.rows = torch.randn((3, 3, W), generator=g).cuda(), torch.randn((20, W), generator=g).to(torch.bfloat16).cuda()
+        pos = torch.tensor(contexts) - 1
+        self.slots = torch.tensor([int(table[b, p // PAGE]) * PAGE + p % PAGE for b, p in enumerate(pos.tolist())], dtype=torch.int32).cuda()
+        back = torch.arange(pos[2] - 19, pos[2] + 1)
+        self.long = (table[2, back // PAGE].long() * PAGE + back % PAGE).int().cuda()
+        self.pos, self.back, self.table = pos.int().cuda(), back.int().cuda(), table.cuda()
+        self.lens, self.cs = torch.tensor(contexts, dtype=torch.int32).cuda(), rope_table(self.dim, 2000).cuda()
+        self.at = [torch.tensor([x], dtype=torch.int32).cuda() for x in (0, 20, 2000)]
+
+    def run(self):
+        heads = self.nq, self.nkv
+        a = ops.rope_attn_decode(self.parts, self.pos, self.slots, self.cs, self.k, self.v, self.table, self.lens, 0.1, *heads, num_splits=4)
+        q = ops.rope_kv_append(self.rows, self.back, self.long, self.cs, self.k, self.v, *heads, self.dim)
+        b = ops.paged_attn_decode(q[:3], self.k, self.v, self.table, self.lens, 0.1, num_splits=5)
+        c = ops.flash_attn_prefill(q, self.k, self.v, self.table[2:], *self.at, 0.1, max_q_len=20)
+        return a, b, c
+
+    def change(self, other):
+        """The other's inputs in this one's tensors."""
+        self.parts.copy_(other.parts)
+        self.rows.copy_(other.rows)
+
+
+@pytest.mark.gpu
+def test_captured_and_on_several_streams():
+    """Graphs replayed beside one another and beside eager calls: the results are those of calls one after another, bit by bit."""
+    works = [Work(s) for s in range(4)]
+    [w.run() for w in works]
+    want = [[t.clone() for t in w.run()] for w in works]                     # (a second run stores the same bytes)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for w in works[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(w.run())
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in works]
+    got = [[] for _ in works]
+    for _ in range(10):
+        for i, (w, st) in enumerate(zip(works, streams)):
+            with torch.cuda.stream(st):
+                if i < 2:
+                    graphs[i].replay()
+                    got[i].append([t.clone() for t in outs[i]])
+                else:
+                    got[i].append(w.run())
+    torch.cuda.synchronize()
+    for rounds, w in zip(got, want):
+        for one in rounds:
+            assert all(torch.equal(a, b) for a, b in zip(one, w))
+    works[0].change(works[1])                                                # a replayed graph reads what is there then
+    graphs[0].replay()
+    graphs[0].replay()                                                       # (the tokens that the first one appended take part in its step)
+    torch.cuda.synchronize()
+    now = [t.clone() for t in outs[0]]
+    assert all(torch.equal(a, b) for a, b in zip(now, works[0].run())) and not torch.equal(now[0], want[0][0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_pools_beyond_32_bits(dim):
+    """Blocks whose bytes lie behind 2^32."""
+    g = torch.Generator().manual_seed(80 + dim)
+    nkv, nq, n = 8, 16, 130
+    blocks = (1 << 32) // (nkv * PAGE * dim) + 50
+    empty = lambda *shape: torch.empty(shape, dtype=torch.uint8, device="cuda")       # noqa: E731
+    k, v = (ops.QuantizedPages(empty(blocks, nkv, PAGE, dim).view(F8), empty(blocks, nkv, PAGE).view(E8)) for _ in range(2))
+    used = torch.tensor([blocks - 1, 0, blocks - 20, blocks - 3, 7], dtype=torch.int32)       # the last ones, and the first ones between them
+    pos = torch.arange(n, dtype=torch.int32)
+    slots = used[pos.long() // PAGE] * PAGE + pos % PAGE
+    x = torch.randn((n, (nq + 2 * nkv) * dim), generator=g).to(torch.bfloat16)
+    q = ops.rope_kv_append(x.cuda(), pos.cuda(), slots.cuda(), rope_table(dim, n).cuda(), k, v, nq, nkv, dim)
+    small = tuple(ops.QuantizedPages(p.values.view(torch.uint8)[used.cuda().long()].view(F8), p.scales.view(torch.uint8)[used.cuda().long()].view(E8))
+                  for p in (k, v))
+    i32 = lambda t: torch.tensor(t, dtype=torch.int32).cuda()                # noqa: E731
+    out = ops.flash_attn_prefill(q, k, v, used[None].cuda(), i32([0]), i32([n]), i32([n]), 0.1, max_q_len=n)
+    check_attention(out.view(n, nq, dim), q.view(n, nq, dim), *small, torch.arange(5)[None], [(0, n, n)], 0.1, nq, 2)
+    last = ops.paged_attn_decode(q[-1:], k, v, used[None].cuda(), i32([n]), 0.1, num_splits=2)
+    check_attention(last.view(1, nq, dim), q[-1:].view(1, nq, dim), *small, torch.arange(5)[None], [(0, 1, n)], 0.1, nq, 2)
+    step = ops.rope_attn_decode(x[None, -1:].float().cuda(), pos[-1:].cuda(), slots[-1:].cuda(), rope_table(dim, n).cuda(),
+                                k, v, used[None].cuda(), i32([n]), 0.1, nq, nkv)
+    check_attention(step.view(1, nq, dim), q[-1:].view(1, nq, dim), *small, torch.arange(5)[None], [(0, 1, n)], 0.1, nq, 2)
+
+
+@pytest.mark.gpu
+def test_kernels_are_counted():
+    w = Work(9)
+    w.run()
+    heads, n = (w.nq, w.nkv), []
+    for f in (lambda: ops.rope_kv_append(w.rows, w.back, w.long, w.cs, w.k, w.v, *heads, w.dim),
+              lambda: ops.rope_attn_decode(w.parts, w.pos, w.slots, w.cs, w.k, w.v, w.table, w.lens, 0.1, *heads),
+              lambda: ops.paged_attn_decode(w.parts[0, :, :w.nq * w.dim].bfloat16().contiguous(), w.k, w.v, w.table, w.lens, 0.1)):
+        before = ops.launch_count()
+        f()
+        n.append(ops.launch_count() - before)
+    assert n == [1, 2, 1]
+
+
 # ------------------------------------------------------------------------------------------------ refusals
 def test_pages_are_checked():
     good = ops.QuantizedPages.new(2, 1, 64)
@@ -498,3 +662,32 @@ def test_refusals(device):
             append(**kw)
     with pytest.raises(ValueError):
         ops.rope_attn_decode(qkv, i32([0, 1]), i32([0, 1]), cs, k, v, table, lens, 0.1, 4, 2)
+
+
+def test_parts_of_a_sequence_are_bounded():
+    pages = ops.QuantizedPages.new(2, 1, 64)
+    with pytest.raises(ValueError):
+        ops.paged_attn_decode(torch.zeros((1, 64), dtype=torch.bfloat16), pages, pages, torch.zeros((1, 1), dtype=torch.int32),
+                              torch.ones(1, dtype=torch.int32), 0.1, num_splits=100000)
+
+
+@pytest.mark.gpu
+def test_tensors_of_another_device_are_refused(monkeypatch):
+    w = Work(3)
+    q = torch.zeros((3, w.nq * w.dim), dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        ops.paged_attn_decode(q, w.k, w.v, w.table, w.lens, 0.1)
+    with pytest.raises(ValueError):
+        ops.paged_attn_decode(q.cuda(), w.k, w.v, w.table.cpu(), w.lens, 0.1)
+    with pytest.raises(ValueError):
+        ops.rope_kv_append(w.rows.cpu(), w.back, w.long, w.cs, w.k, w.v, w.nq, w.nkv, w.dim)
+    with pytest.raises(ValueError):
+        ops.flash_attn_prefill(q.cuda(), w.k, w.v, w.table, w.lens.cpu(), w.lens, w.lens, 0.1, max_q_len=1)
+    cpu = ops.QuantizedPages(w.v.values.cpu(), w.v.scales.cpu())
+    with pytest.raises(ValueError):
+        ops.paged_attn_decode(q.cuda(), w.k, cpu, w.table, w.lens, 0.1)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 1)              # the pages' device is not the current one
+    for call in (lambda: ops.paged_attn_decode(q.cuda(), w.k, w.v, w.table, w.lens, 0.1), w.run,
+                 lambda: ops.flash_attn_prefill(q.cuda(), w.k, w.v, w.table, w.lens, w.lens, w.lens, 0.1, max_q_len=1)):
+        with pytest.raises(ValueError):
+            call()
