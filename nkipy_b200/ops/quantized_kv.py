@@ -19,6 +19,7 @@ them (its cache is dense and bf16, examples/models/qwen3/qwen3.py:52-71).
 
 from __future__ import annotations
 
+import functools
 import struct
 from typing import Optional, Tuple
 
@@ -304,6 +305,16 @@ def _scratch(device: torch.device, floats: int) -> torch.Tensor:
     return buf
 
 
+@functools.lru_cache(maxsize=4096)
+def _decode_floats(B: int, nkv: int, D: int, group: int, num_splits: int) -> int:
+    return _lib.lib().nkb_q8_attn_decode_scratch_floats(B, nkv, D, group, num_splits)
+
+
+@functools.lru_cache(maxsize=4096)
+def _prefill_floats(B: int, max_q_len: int, nq: int, nkv: int, D: int, width: int) -> int:
+    return _lib.lib().nkb_q8_attn_prefill_scratch_floats(B, max_q_len, nq, nkv, D, width)
+
+
 def _pick_splits(ctas: int, max_pages: int, sms: int = 148) -> int:
     """Parts that decode attention makes of a sequence on average."""
     return 1 if ctas >= sms else max(min(sms // ctas, max(max_pages // 8, 1), 16), 1)
@@ -316,7 +327,7 @@ def _splits(num_splits: int, scratch, B: int, nkv: int, D: int, group: int, max_
         num_splits = _pick_splits(B * nkv, max_pages)
     if num_splits <= 1:
         return 1, None
-    need = _lib.lib().nkb_q8_attn_decode_scratch_floats(B, nkv, D, group, num_splits)
+    need = _decode_floats(B, nkv, D, group, num_splits)
     if scratch is None:
         scratch = _scratch(device, need)
     elif (scratch.dtype is not torch.float32 or scratch.numel() < need or scratch.device != device or not scratch.is_contiguous()
@@ -332,9 +343,8 @@ def decode_scratch(pages: QuantizedPages, nq: int, max_batch: int, max_pages: in
     if not pages.is_cuda:
         return None
     nkv, D = pages.shape[1], pages.shape[3]
-    L = _lib.lib()
-    floats = max(L.nkb_q8_attn_decode_scratch_floats(b, nkv, D, nq // nkv, _pick_splits(b * nkv, max_pages)) for b in range(1, max_batch + 1))
-    return torch.zeros((max(int(floats), COUNTERS),), dtype=torch.float32, device=pages.device)
+    floats = max(_decode_floats(b, nkv, D, nq // nkv, _pick_splits(b * nkv, max_pages)) for b in range(1, max_batch + 1))
+    return torch.zeros((max(floats, COUNTERS),), dtype=torch.float32, device=pages.device)
 
 
 # --------------------------------------------------------------------------- operators
@@ -345,7 +355,7 @@ def rope_kv_append(qkv, positions, slots, cos_sin, k_cache, v_cache, nq, nkv, he
     blocks = _pair(k_cache, v_cache)[0]
     T, parts, stride, rows = _check_qkv(qkv, positions, slots, cos_sin, k_cache, nq, nkv, head_dim, bias, q_norm_w, k_norm_w)
     if q_out is None:
-        q_out = torch.empty((T, nq * head_dim), dtype=torch.bfloat16, device=k_cache.device)
+        q_out = qkv.new_empty((T, nq * head_dim), dtype=torch.bfloat16)
     else:
         _want_rows(q_out, "q_out", (T, nq * head_dim), k_cache.index)
     if not _on_gpu(k_cache.index):
@@ -416,7 +426,7 @@ def rope_attn_decode(qkv_partials, positions, slots, cos_sin, k_cache, v_cache, 
     if num_splits > MAX_SPLITS:
         raise ValueError(f"num_splits is at most {MAX_SPLITS}")
     if out is None:
-        out = torch.empty((B, nq * D), dtype=torch.bfloat16, device=k_cache.device)
+        out = qkv_partials.new_empty((B, nq * D), dtype=torch.bfloat16)
     else:
         _want_rows(out, "out", (B, nq * D), index)
     _on_gpu(index)
@@ -459,10 +469,9 @@ def flash_attn_prefill(q, k_cache, v_cache, block_table, q_start, q_lens, contex
                 res[at:at + n] = _ref_attend(qf[at:at + n], k_cache, v_cache, block_table[b], ctx, scale, ctx - n, causal, window, chunk,
                                              sinks)
         return out
-    L = _lib.lib()
-    floats = L.nkb_q8_attn_prefill_scratch_floats(B, max_q_len, nq, nkv, D, width)
+    floats = _prefill_floats(B, max_q_len, nq, nkv, D, width)
     scratch = _scratch(k_cache.device, floats)
-    rc = L.nkb_q8_attn_prefill(_ATTN.pack(
+    rc = _lib.lib().nkb_q8_attn_prefill(_ATTN.pack(
         q_at, *k_cache.at, *v_cache.at, block_table.data_ptr(), q_start.data_ptr(), q_lens.data_ptr(), context_lens.data_ptr(), out.data_ptr(),
         _p(sinks), scratch.data_ptr(), _stream(), block_table.stride(0), B, total, max_q_len, nq, nkv, D, blocks,
         width, 1 if causal else 0, window, chunk, 1, scale, 0))
