@@ -33,7 +33,7 @@ constexpr float kQ8Lift = 6.f;         // log2 of the weight at M; t may grow by
 constexpr float kQ8Grow = 8.f;
 
 struct DecodeQ8Params {
-  const __nv_bfloat16* q;
+  const __nv_bfloat16* q;              // may be out: all warps have read their queries before a result of their sequence and kv head is written
   const int *block_table, *context_lens;
   __nv_bfloat16* out;
   float* scratch;

@@ -431,12 +431,12 @@ def rope_attn_decode(qkv_partials, positions, slots, cos_sin, k_cache, v_cache, 
         _want_rows(out, "out", (B, nq * D), index)
     _on_gpu(index)
     num_splits, scratch = _splits(num_splits, scratch, B, nkv, D, nq // nkv, width, k_cache.device)
-    q = torch.empty_like(out)
-    q_at, stream, pages = q.data_ptr(), _stream(), (*k_cache.at, *v_cache.at)
+    # the queries lie where their results come: who writes a result has read, or waited for those who read, its queries
+    q_at, stream, pages = out.data_ptr(), _stream(), (*k_cache.at, *v_cache.at)
     rc = _lib.lib().nkb_q8_step(
         _APPEND.pack(0, qkv_partials.data_ptr(), _p(bias), _p(positions), _p(slots), _p(cos_sin), _p(q_norm_w), _p(k_norm_w), q_at, *pages, stream,
                      stride, norm_eps, parts, B, nq, nkv, D, rows, blocks, 0),
-        _ATTN.pack(q_at, *pages, block_table.data_ptr(), 0, 0, context_lens.data_ptr(), out.data_ptr(), _p(sinks), _p(scratch), stream,
+        _ATTN.pack(q_at, *pages, block_table.data_ptr(), 0, 0, context_lens.data_ptr(), q_at, _p(sinks), _p(scratch), stream,
                    block_table.stride(0), B, B, 1, nq, nkv, D, blocks, width, 1, window, 0, num_splits, scale, 0))
     if rc:
         _lib.check(rc, "nkb_q8_step")
