@@ -49,8 +49,8 @@ class QuantizedPages:
         if not values.is_contiguous() or not scales.is_contiguous() or scales.get_device() != index:
             raise ValueError("QuantizedPages wants contiguous tensors on one device")
         self.at = v, s = values.data_ptr(), scales.data_ptr()
-        if (v | s) & 15:
-            raise ValueError("QuantizedPages wants tensors that start on 16 bytes")
+        if (v | s) & 15 or not v:
+            raise ValueError("QuantizedPages wants tensors that start on 16 bytes, of a block and a head at least")
         # shape as of a cache tensor; index: of the CUDA device, -1: the CPU; at: where the tensors start
         self.values, self.scales, self.shape, self.index, self.device = values, scales, shape, index, values.device
 

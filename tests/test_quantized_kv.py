@@ -664,6 +664,13 @@ def test_refusals(device):
         ops.rope_attn_decode(qkv, i32([0, 1]), i32([0, 1]), cs, k, v, table, lens, 0.1, 4, 2)
 
 
+@pytest.mark.parametrize("blocks,heads", [(0, 1), (1, 0)])
+@pytest.mark.parametrize("device", DEVICES)
+def test_pools_have_a_page(device, blocks, heads):
+    with pytest.raises(ValueError):
+        ops.QuantizedPages.new(blocks, heads, 64, device)
+
+
 def test_parts_of_a_sequence_are_bounded():
     pages = ops.QuantizedPages.new(2, 1, 64)
     with pytest.raises(ValueError):
