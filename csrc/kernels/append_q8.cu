@@ -3,6 +3,9 @@
 // rope_kv_append (elementwise.cu) for a quantised cache.
 //
 // Keys and values are computed in 64 bits, so that their one rounding to e4m3 does not depend on the order of operations.
+//
+// Measured with 32 heads of 128 on 8: one token from 8 partial sums 3.1 us (latency), 16384 tokens from bf16 75.3 us (58.1 at the copy
+// bandwidth of 6.56 TB/s; 80 for bf16 pages), 390 of 32 heads on 4 with norms 6.2 us (1.2; a chain of latencies, two square roots in it).
 #include "api.h"
 #include "kv_quant.cuh"
 
@@ -146,7 +149,8 @@ __device__ __forceinline__ float turn_to_odd(float a, float c, float d, float s)
 }
 
 // The same in pieces of sixteen bytes: D / 16 lanes share a head, each with eight elements of its first half and the eight that turn with
-// them.  A warp takes 512 / D heads of a token at a time, `run` times, the next ones' inputs on their way.  Every pointer on 16 bytes, split_stride a multiple of four.
+// them.  A warp takes 512 / D heads of a token at a time, `run` times, the next ones' inputs on their way.  Every pointer on 16 bytes,
+// split_stride a multiple of four.
 //
 // Bound by memory from some thousand tokens on, and next by what goes through L1: cos and sin are twice the bytes of a head's input, so a run
 // loads them once.  Then come instructions: 64-bit arithmetic and conversions run at a fraction of the 32-bit

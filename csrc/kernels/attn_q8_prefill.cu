@@ -21,8 +21,14 @@
 // Rows of a query tile are (token, head of the group): short prompts fill tiles, and a tile's rows end close to one another.  Queries become
 // f16 as they are loaded, each row scaled below 2^15 by a power of two.
 //
-// 128 exponentials per row bound the loop (2048 cycles per 256 x 128 scores, as many as its MMAs at 128 columns), so conversion has warps
-// of its own, with the registers that the softmax leaves: 64 and 192 a thread.
+// 128 exponentials per row want 2048 cycles per 256 x 128 scores, as many as its MMAs at 128 columns, so conversion has warps of its own, with
+// the registers that the softmax leaves: 64 and 192 a thread.  What the loop takes is some 4500 cycles: the two softmax warps of a scheduler
+// and a converting one wait for each other's issue slots, and shared memory, which MMAs, weights, conversion and copies share, is busy for
+// 3500 of them.  Weights in tensor memory spare a fifth of those bytes; at 128 columns there is room for them only where the scores are, whose
+// next product then waits for theirs: 2 sequences of 8000 856 us for 801.
+//
+// Measured, beside the MMAs at 1658 TFLOP/s and bf16 pages: 32 heads of 128 on 8, 16 prompts of 1024 166 us (52, 197), 2 of 8000 801 (494, 764),
+// one of 77 11.0 (0.2, 6.8; a fixed part of some 8 us); 64 heads of 64 on 8, 3 portions of up to 500 behind 4000 to 8000 tokens 249 (81, 259).
 #include "api.h"
 #include "kv_quant.cuh"
 #include "attn_maps.h"

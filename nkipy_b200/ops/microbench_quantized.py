@@ -4,7 +4,7 @@ from __future__ import annotations
 import torch
 
 from . import QuantizedPages, flash_attn_prefill, paged_attn_decode, rope_attn_decode, rope_kv_append
-from .quantized_kv import PAGE
+from .quantized_kv import PAGE, quantize_rows
 
 NQ, NKV, D = 32, 8, 128
 TOKEN = 2 * NKV * (D + 1)                # bytes of a token's keys and values
@@ -19,13 +19,9 @@ def _rows(*shape):
 
 
 def _pools(blocks, sets):
-    """Pages of random values: bytes below 0x7f, no NaN among them."""
-    pools = [(QuantizedPages.new(blocks, NKV, D, "cuda"), QuantizedPages.new(blocks, NKV, D, "cuda")) for _ in range(sets)]
-    for pair in pools:
-        for pages in pair:
-            pages.values.view(torch.uint8).random_(0, 0x7f)
-            pages.scales.view(torch.uint8).random_(120, 124)
-    return pools
+    """Pages of normal values."""
+    pages = lambda: QuantizedPages(*quantize_rows(torch.randn(blocks, NKV, PAGE, D, device="cuda")))       # noqa: E731
+    return [(pages(), pages()) for _ in range(sets)]
 
 
 def _batch(B, ctx):
