@@ -41,9 +41,12 @@ class QuantizedPages:
         if values.dtype is not torch.float8_e4m3fn or scales.dtype is not torch.float8_e8m0fnu:
             raise TypeError("QuantizedPages wants float8_e4m3fn values and float8_e8m0fnu scales")
         shape = values.shape
-        if len(shape) != 4 or shape[2] != PAGE or scales.shape != shape[:3]:
+        if len(shape) != 4:
+            raise ValueError("QuantizedPages wants values [blocks, kv heads, 32, dim]")
+        blocks, heads, page, dim = shape
+        if page != PAGE or scales.shape != (blocks, heads, PAGE):
             raise ValueError("QuantizedPages wants values [blocks, kv heads, 32, dim] and scales [blocks, kv heads, 32]")
-        if shape[3] not in DIMS:
+        if dim not in DIMS:
             raise ValueError("QuantizedPages has heads of 64 or 128 columns")
         index = values.get_device()
         if not values.is_contiguous() or not scales.is_contiguous() or scales.get_device() != index:
@@ -211,17 +214,19 @@ def _check_heads(nq: int, nkv: int) -> int:
     return nq // nkv
 
 
-def _check_table(block_table, context_lens, index: int) -> Tuple[int, int]:
-    """(sequences, blocks of a row)"""
-    if block_table.dim() != 2 or block_table.shape[1] < 1:
+def _check_table(block_table, context_lens, index: int) -> Tuple[int, int, int]:
+    """(sequences, blocks of a row, entries from one row to the next)"""
+    shape = block_table.shape
+    if len(shape) != 2 or shape[1] < 1:
         raise ValueError("block_table wants [sequences, blocks]")
     if block_table.dtype is not torch.int32:
         raise TypeError(f"block_table wants torch.int32, not {block_table.dtype}")
-    if block_table.get_device() != index or block_table.stride(1) != 1:
+    B, width = shape
+    step, column = (width, 1) if block_table.is_contiguous() else block_table.stride()
+    if block_table.get_device() != index or (column != 1 and width > 1):
         raise ValueError("block_table wants neighbouring columns and to be on the pages' device")
-    B, width = block_table.shape
     _want(context_lens, "context_lens", torch.int32, (B,), index)
-    return B, width
+    return B, width, step
 
 
 def _check_qkv(qkv, positions, slots, cos_sin, k_cache, nq, nkv, head_dim, bias, q_norm_w, k_norm_w) -> Tuple[int, int, int, int]:
@@ -231,16 +236,21 @@ def _check_qkv(qkv, positions, slots, cos_sin, k_cache, nq, nkv, head_dim, bias,
     if nkv != k_cache.shape[1] or head_dim != k_cache.shape[3]:
         raise ValueError("the pages have other kv heads than the projection")
     W = (nq + 2 * nkv) * head_dim
-    parts, stride = 1, 0
+    parts = 1
     if len(shape) == 3 and qkv.dtype is torch.float32:
-        parts, stride = shape[0], qkv.stride(0)
+        parts = shape[0]
     elif len(shape) != 2 or qkv.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError("qkv is bf16 [T, W] or fp32 partial sums [S, T, W]")
     T = shape[-2]
     if shape[-1] != W or parts < 1:
         raise ValueError(f"qkv has the shape {tuple(shape)}, not [..., {W}]")
-    if qkv.get_device() != index or qkv.stride(-1) != 1 or qkv.stride(-2) != W:
-        raise ValueError("qkv wants rows that follow one another, on the pages' device")
+    stride = T * W
+    if not qkv.is_contiguous():                                   # partial sums may lie apart
+        stride = qkv.stride(0)
+        if len(shape) == 2 or qkv.stride(-1) != 1 or (T > 1 and qkv.stride(-2) != W):
+            raise ValueError("qkv wants rows that follow one another")
+    if qkv.get_device() != index:
+        raise ValueError("qkv wants to be on the pages' device")
     rows = 0
     if cos_sin is not None:
         rows = cos_sin.shape[0]
@@ -294,7 +304,7 @@ def _scratch(device: torch.device, floats: int) -> torch.Tensor:
     """Partial results of divided sequences, behind arrival counters that are zero between calls: one per device and stream.  A graph
     that is captured gets its own, cleared whenever it runs: it may run beside other graphs, and ahead of the call that would have
     cleared a shared one."""
-    if torch.cuda.is_current_stream_capturing():
+    if torch._C._cuda_isCurrentStreamCapturing():
         buf = torch.empty((floats,), dtype=torch.float32, device=device)
         buf[:COUNTERS].zero_()
         return buf
@@ -375,7 +385,7 @@ def paged_attn_decode(q, k_cache, v_cache, block_table, context_lens, scale, *, 
     """`ops.paged_attn_decode` over quantised pages."""
     blocks, nkv, D = _pair(k_cache, v_cache)
     index = k_cache.index
-    B, width = _check_table(block_table, context_lens, index)
+    B, width, table_step = _check_table(block_table, context_lens, index)
     nq = q.shape[-1] // D
     group = _check_heads(nq, nkv)
     _check_masks(mods, window, chunk, sinks, nq, index)
@@ -398,7 +408,7 @@ def paged_attn_decode(q, k_cache, v_cache, block_table, context_lens, scale, *, 
     num_splits, scratch = _splits(num_splits, scratch, B, nkv, D, group, width, k_cache.device)
     rc = _lib.lib().nkb_q8_attn_decode(_ATTN.pack(
         q_at, *k_cache.at, *v_cache.at, block_table.data_ptr(), 0, 0, context_lens.data_ptr(), out.data_ptr(), _p(sinks), _p(scratch), _stream(),
-        block_table.stride(0), B, B * q_len, q_len, nq, nkv, D, blocks, width, 1, window, chunk, num_splits, scale, 0))
+        table_step, B, B * q_len, q_len, nq, nkv, D, blocks, width, 1, window, chunk, num_splits, scale, 0))
     if rc:
         _lib.check(rc, "nkb_q8_attn_decode")
     _count_launch()
@@ -413,7 +423,7 @@ def rope_attn_decode(qkv_partials, positions, slots, cos_sin, k_cache, v_cache, 
     call sees, or negative."""
     blocks, _, D = _pair(k_cache, v_cache)
     index = k_cache.index
-    B, width = _check_table(block_table, context_lens, index)
+    B, width, table_step = _check_table(block_table, context_lens, index)
     if qkv_partials.dtype is not torch.float32 or qkv_partials.shape[-2] != B:
         raise ValueError("rope_attn_decode wants fp32 partials [S, B, W], one token per sequence")
     if index < 0 or not B or nkv < 1 or nq // nkv > 16:
@@ -437,7 +447,7 @@ def rope_attn_decode(qkv_partials, positions, slots, cos_sin, k_cache, v_cache, 
         _APPEND.pack(0, qkv_partials.data_ptr(), _p(bias), _p(positions), _p(slots), _p(cos_sin), _p(q_norm_w), _p(k_norm_w), q_at, *pages, stream,
                      stride, norm_eps, parts, B, nq, nkv, D, rows, blocks, 0),
         _ATTN.pack(q_at, *pages, block_table.data_ptr(), 0, 0, context_lens.data_ptr(), q_at, _p(sinks), _p(scratch), stream,
-                   block_table.stride(0), B, B, 1, nq, nkv, D, blocks, width, 1, window, 0, num_splits, scale, 0))
+                   table_step, B, B, 1, nq, nkv, D, blocks, width, 1, window, 0, num_splits, scale, 0))
     if rc:
         _lib.check(rc, "nkb_q8_step")
     _count_launch(2)
@@ -449,7 +459,7 @@ def flash_attn_prefill(q, k_cache, v_cache, block_table, q_start, q_lens, contex
     """`ops.flash_attn_prefill` over quantised pages.  Rows of q that belong to no sequence are left as they are in `out`."""
     blocks, nkv, D = _pair(k_cache, v_cache)
     index = k_cache.index
-    B, width = _check_table(block_table, context_lens, index)
+    B, width, table_step = _check_table(block_table, context_lens, index)
     nq, total = q.shape[-1] // D, q.shape[0]
     _check_heads(nq, nkv)
     _check_masks(mods, window, chunk, sinks, nq, index)
@@ -473,7 +483,7 @@ def flash_attn_prefill(q, k_cache, v_cache, block_table, q_start, q_lens, contex
     scratch = _scratch(k_cache.device, floats)
     rc = _lib.lib().nkb_q8_attn_prefill(_ATTN.pack(
         q_at, *k_cache.at, *v_cache.at, block_table.data_ptr(), q_start.data_ptr(), q_lens.data_ptr(), context_lens.data_ptr(), out.data_ptr(),
-        _p(sinks), scratch.data_ptr(), _stream(), block_table.stride(0), B, total, max_q_len, nq, nkv, D, blocks,
+        _p(sinks), scratch.data_ptr(), _stream(), table_step, B, total, max_q_len, nq, nkv, D, blocks,
         width, 1 if causal else 0, window, chunk, 1, scale, 0))
     if rc:
         _lib.check(rc, "nkb_q8_attn_prefill")

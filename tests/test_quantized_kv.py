@@ -664,6 +664,25 @@ def test_refusals(device):
         ops.rope_attn_decode(qkv, i32([0, 1]), i32([0, 1]), cs, k, v, table, lens, 0.1, 4, 2)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("T", [1, 3])
+def test_partial_sums_that_lie_apart(device, T):
+    """Slices of a larger buffer: partial sums further apart than their rows; rows apart are refused."""
+    g = torch.Generator().manual_seed(90)
+    nq, nkv, dim, W = 2, 1, 64, 4 * 64
+    whole = torch.randn((3, T + 2, W), generator=g).to(device)
+    at = torch.arange(T, dtype=torch.int32, device=device)
+    one, two = (tuple(ops.QuantizedPages.new(1, nkv, dim, device) for _ in range(2)) for _ in range(2))
+    cs = rope_table(dim, T).to(device)
+    a = ops.rope_kv_append(whole[:, 1:1 + T], at, at, cs, *one, nq, nkv, dim)
+    b = ops.rope_kv_append(whole[:, 1:1 + T].contiguous(), at, at, cs, *two, nq, nkv, dim)
+    assert torch.equal(a, b) and all(torch.equal(x.values.view(torch.uint8), y.values.view(torch.uint8)) for x, y in zip(one, two))
+    for bad in (torch.zeros((3, T, 2 * W), device=device)[..., ::2], torch.zeros((3, 2, 2 * W), device=device)[:, :, :W],
+                torch.zeros((2, 2 * W), dtype=torch.bfloat16, device=device)[:, :W]):
+        with pytest.raises(ValueError):
+            ops.rope_kv_append(bad, at[:1].expand(bad.shape[-2]).contiguous(), None, None, *one, nq, nkv, dim)
+
+
 @pytest.mark.parametrize("blocks,heads", [(0, 1), (1, 0)])
 @pytest.mark.parametrize("device", DEVICES)
 def test_pools_have_a_page(device, blocks, heads):
