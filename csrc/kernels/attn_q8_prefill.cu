@@ -22,7 +22,7 @@
 // f16 as they are loaded, each row scaled below 2^15 by a power of two.
 //
 // 128 exponentials per row want 2048 cycles per 256 x 128 scores, as many as its MMAs at 128 columns, so conversion has warps of its own, with
-// the registers that the softmax leaves: 64 and 192 a thread.  What the loop takes is some 4500 cycles: the two softmax warps of a scheduler
+// the registers that the softmax leaves: 56 and 200 a thread.  What the loop takes is some 4500 cycles: the two softmax warps of a scheduler
 // and a converting one wait for each other's issue slots, and shared memory, which MMAs, weights, conversion and copies share, is busy for
 // 3500 of them.  Weights in tensor memory spare a fifth of those bytes; at 128 columns there is room for them only where the scores are, whose
 // next product then waits for theirs: 2 sequences of 8000 856 us for 801.
@@ -40,7 +40,7 @@ namespace nkb {
 
 constexpr int kP8Tile = 128;             // query rows of an MMA tile, tokens of a K or V tile
 constexpr int kP8Threads = 512;
-constexpr int kP8Regs = 128;             // a thread's registers at launch; 2 * 128 * (64 + 192) is all of them
+constexpr int kP8Regs = 128;             // a thread's registers at launch; 2 * 128 * (56 + 200) is all of them
 constexpr int kP8Slots = 8;              // tiles whose scales are kept
 constexpr int kP8Lead = 4;               // tiles that warp 14 is ahead of the conversion of V at most
 constexpr float kP8Grow = 8.f;           // log2 of the growth of a row's maximum that makes O follow
@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
 
   if (warp < 4) {
     // ---------------------------------------------------------------- conversion
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     constexpr int kRows = 512 / D, kSteps = kQ8Page / kRows;       // tokens per sixteen-byte load of the warp, loads per page
     constexpr int kLanes = D / 16;                                 // lanes that share a token
     const int piece = lane % kLanes, row_of = lane / kLanes;
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
       tiles0 += k.n_union;
     }
   } else if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 15) {
       // -------------------------------------------------------------- pages: lanes 0 to 3 a page of the item each
       // and the works: a CTA's first has its number, the others come from a counter of the grid.  The last rows of all sequences first, those
@@ -607,7 +607,7 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- softmax, one thread per row
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     const int t = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane;
     const uint32_t lane_off = uint32_t(quad * 32) << 16;
     const uint32_t s_addr = tmem_base + lane_off + kSCol + t * 128, o_addr = tmem_base + lane_off + kOCol + t * 128;
@@ -659,7 +659,10 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
 #pragma unroll
           for (int c = kFirst / 32; c < kP8Tile / 32; ++c) tmem_ld_32x32(s_addr + c * 32, reinterpret_cast<uint32_t(&)[32]>(v[c * 32]));
           const bool edge = __any_sync(kAll, kv0 + kP8Tile - 1 > hi_pos || kv0 < lo_pos);
-          if (!edge) largest(0, kFirst);
+          if (!edge) {
+            largest(0, kFirst);
+            asm volatile("" : "+f"(mx4[0]), "+f"(mx4[1]), "+f"(mx4[2]), "+f"(mx4[3]));
+          }
           tmem_ld_wait();
           tc_fence_before();
           __syncwarp();
