@@ -22,13 +22,15 @@
 // f16 as they are loaded, each row scaled below 2^15 by a power of two.
 //
 // 128 exponentials per row want 2048 cycles per 256 x 128 scores, as many as its MMAs at 128 columns, so conversion has warps of its own, with
-// the registers that the softmax leaves: 56 and 200 a thread.  What the loop takes is some 4500 cycles: the two softmax warps of a scheduler
-// and a converting one wait for each other's issue slots, and shared memory, which MMAs, weights, conversion and copies share, is busy for
-// 3500 of them.  Weights in tensor memory spare a fifth of those bytes; at 128 columns there is room for them only where the scores are, whose
-// next product then waits for theirs: 2 sequences of 8000 856 us for 801.
+// the registers that the softmax leaves: 56 and 200 a thread (64 and 192: 2 sequences of 8000 753 us, 741 here).  What the loop takes is some
+// 4000 cycles.  Two softmax warps and a converting one share a scheduler's issue slots: exponentials on the multiply-add units, which spare
+// the special-function unit and take more instructions, made it slower (an eighth of them 793 us).  Shared memory, which MMAs, weights,
+// conversion and copies share, is busy for 3500 cycles.  Weights in tensor memory would spare a fifth of those bytes; at 128 columns there is
+// room for them only where the scores are, whose next product then waits for theirs (856 us, where it was 801), or with one place for the scores
+// of both query tiles, which then wait for each other (781 for 741).
 //
-// Measured, beside the MMAs at 1658 TFLOP/s and bf16 pages: 32 heads of 128 on 8, 16 prompts of 1024 166 us (52, 197), 2 of 8000 801 (494, 764),
-// one of 77 11.0 (0.2, 6.8; a fixed part of some 8 us); 64 heads of 64 on 8, 3 portions of up to 500 behind 4000 to 8000 tokens 249 (81, 259).
+// Measured, beside the MMAs at 1658 TFLOP/s and bf16 pages: 32 heads of 128 on 8, 16 prompts of 1024 157 us (52, 197), 2 of 8000 741 (494, 764),
+// one of 77 10.8 (0.2, 6.8; a fixed part of some 8 us); 64 heads of 64 on 8, 3 portions of up to 500 behind 4000 to 8000 tokens 241 (81, 259).
 #include "api.h"
 #include "kv_quant.cuh"
 #include "attn_maps.h"
@@ -704,7 +706,7 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
           const float less = add + kP8Lift - (m == -INFINITY ? 0.f : m);
           const float2 sc2 = make_float2(to_log2, to_log2), nb2 = make_float2(less, less);
           // The other query tile's turn comes ahead of this one's end: while its exponentials start, this one's last weights are stored and published.
-          // At the end, us: 16 prompts of 1024 165 (158 here), 2 of 8000 797 (753); 64 columns 249 at the end and 245 here, 254 one quarter earlier.
+          // A quarter later, us: 16 prompts of 1024 165 (157 here), 2 of 8000 786 (741); a quarter earlier 159 and 747, and 247 for 241 at 64 columns.
           constexpr int kHand = NH == 2 ? 2 : 3;
           float2 sum2[4];
 #pragma unroll
