@@ -4,7 +4,7 @@
 //
 // Keys and values are computed in 64 bits, so that their one rounding to e4m3 does not depend on the order of operations.
 //
-// Measured with 32 heads of 128 on 8: one token from 8 partial sums 3.1 us (latency), 16384 tokens from bf16 75.3 us (58.1 at the copy
+// Measured with 32 heads of 128 on 8: one token from 8 partial sums 3.1 us (latency), 16384 tokens from bf16 76.1 us (58.1 at the copy
 // bandwidth of 6.56 TB/s; 80 for bf16 pages), 390 of 32 heads on 4 with norms 6.2 us (1.2; a chain of latencies, two square roots in it).
 #include "api.h"
 #include "kv_quant.cuh"
@@ -133,16 +133,20 @@ __global__ void __launch_bounds__(256) append_q8_kernel(const AppendQ8Params p) 
 }
 
 // a * c - d * s from 32-bit numbers, rounded to odd like round_to_odd of the same in 64 bits: products and their difference with what each
-// rounding leaves (a product's rest is one multiply-add; the difference's by Knuth's two-sum).  Finite where the inputs are.
+// rounding leaves (a product's rest is one multiply-add; the difference's by Knuth's two-sum).  What the products leave may be more than a
+// step of their difference, so it is added before the rounding to odd (Dekker's sum, whose rest is wrong only where the products cancel, and
+// the result becomes zero beside the head's other half).  Finite where the inputs are.
 __device__ __forceinline__ float turn_to_odd(float a, float c, float d, float s) {
+  constexpr float kMost = 3.402823466e38f;
   // (intrinsics: the compiler must not merge these)
   const float p = __fmul_rn(a, c), pe = __fmaf_rn(a, c, -p), q = __fmul_rn(d, s), qe = __fmaf_rn(d, s, -q);
   const float x = __fsub_rn(p, q), v = __fsub_rn(x, p);
   const float rest = __fadd_rn(__fsub_rn(__fsub_rn(p, __fsub_rn(x, v)), __fadd_rn(q, v)), __fsub_rn(pe, qe));
-  const float top = fminf(fmaxf(x == 0.f ? rest : x, -3.402823466e38f), 3.402823466e38f);
+  const float y = __fadd_rn(x, rest), least = __fsub_rn(rest, __fsub_rn(y, x));
+  const float top = fminf(fmaxf(fabsf(x) <= kMost ? y : x, -kMost), kMost);
   int bits = __float_as_int(top);
-  if (rest != 0.f && x != 0.f) {
-    if ((rest < 0.f) != (top < 0.f)) --bits;       // the sum lies nearer zero: the number before
+  if (least != 0.f && top != 0.f) {
+    if ((least < 0.f) != (top < 0.f)) --bits;      // the sum lies nearer zero: the number before
     bits |= 1;
   }
   return __int_as_float(bits);

@@ -218,6 +218,31 @@ def test_append_rounds_ties_and_ends_of_the_range(device):
             assert torch.equal(gs[at // PAGE, 0, at % PAGE].nan_to_num(-1), scales.nan_to_num(-1))
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("T", [1, 200])
+def test_append_rounds_rotations_beside_a_tie(device, T):
+    """Rotations that 32 bits put on the other side of the middle between two values of e4m3: the products' roundings move their difference
+    by more than one of its steps."""
+    g = torch.Generator().manual_seed(33)
+    dim, h, n = 64, 32, 3000000
+    a, d = ((1 + torch.randint(0, 128, (2, n), generator=g) / 128) * (1 - 2 * torch.randint(0, 2, (2, n), generator=g))).unbind(0)
+    a = 2 * a
+    c, tie = 0.5 + 0.5 * torch.rand(n, generator=g), 1 + (1 + 2 * torch.randint(0, 8, (n,), generator=g)) / 16
+    s = ((a.double() * c.double() - tie) / d.double()).float()
+    exact, rough = a.double() * c.double() - d.double() * s.double(), a * c - d * s      # (products of 8 and 24 bits: exact)
+    odd = (((rough > tie) & (exact < tie)) | ((rough < tie) & (exact > tie))) & (s.abs() < 1)
+    a, c, d, s, exact = (t[odd][:T * h].view(T, h) for t in (a, c, d, s, exact))
+    k, v = (ops.QuantizedPages.new(-(-T // PAGE), 1, dim, device) for _ in range(2))
+    x = torch.zeros((T, 3, dim))
+    x[:, 1] = torch.cat([a, d], -1)
+    at = torch.arange(T, dtype=torch.int32, device=device)
+    ops.rope_kv_append(x.view(T, -1).to(torch.bfloat16).to(device), at, at, torch.cat([c, s], -1).to(device), k, v, 1, 1, dim)
+    turned = torch.cat([exact, d.double() * c.double() + a.double() * s.double()], -1)
+    want, scale = oracle_quantize(turned)
+    assert torch.equal(k.values.view(-1, dim)[:T].cpu().double(), want)
+    assert torch.equal(k.scales.view(-1)[:T].cpu().float().double(), scale)
+
+
 def test_dequantize_gives_what_is_stored():
     g = torch.Generator().manual_seed(3)
     k, _ = pool(g, 3, 2, 64, "cpu")
