@@ -400,6 +400,28 @@ def test_prompts(device, nq, nkv, dim, spans, masks):
 
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("spans", [[(0, 5)], [(0, 1), (700, 9), (1400, 3), (50, 60)], [(383, 1), (384, 1), (511, 2)]])
+def test_prompts_with_room_in_their_tables(device, dim, spans):
+    """Tables as wide as the longest sequence may become: what is divided goes by what a sequence has."""
+    g = torch.Generator().manual_seed(dim + len(spans))
+    nq, nkv = 4, 2
+    contexts, new = [a + n for a, n in spans], [n for _, n in spans]
+    table, blocks = shuffled_table(g, contexts)
+    k, v = pool(g, blocks, nkv, dim, device)
+    wide = torch.zeros((len(spans), 512), dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    q, sinks = torch.randn((sum(new), nq * dim), generator=g).to(torch.bfloat16), torch.randn((nq,), generator=g)
+    starts = [sum(new[:b]) for b in range(len(new))]
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)        # noqa: E731
+    for window in (0, 600):
+        out = ops.flash_attn_prefill(q.to(device), k, v, wide.to(device), i32(starts), i32(new), i32(contexts), dim ** -0.5, max_q_len=max(new),
+                                     sinks=sinks.to(device), window=window)
+        check_attention(out.view(-1, nq, dim), q.view(-1, nq, dim), k, v, table, list(zip(starts, new, contexts)), dim ** -0.5, nq, 2, sinks,
+                        window=window)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dim", [64, 128])
 def test_prompts_with_tokens_ahead_of_the_first(device, dim):
     """Contexts shorter than the new tokens, or empty: rows that see nothing are zero (with or without sinks), pieces without a tile lie
     among others."""
