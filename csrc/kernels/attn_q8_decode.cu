@@ -530,8 +530,10 @@ static int q8_maps(CUtensorMap (&m)[4], const void* const (&at)[4], int dim, int
 
 using namespace nkb;
 
+// Needs the device (the plan rounds up to waves of its SMs); negative: there is none.
 extern "C" long long nkb_q8_attn_decode_scratch_floats(int batch, int nkv, int head_dim, int group, int num_splits) {
   if (num_splits <= 1) return 0;
+  if (batch < 1 || nkv < 1 || group < 1 || (!status_word() && nkb_init() != 0)) return -1;
   return kQ8Counters + (long long)plan_units(batch, nkv, group, num_splits) * nkv * (16 * head_dim + 32);
 }
 
@@ -541,6 +543,7 @@ static int attn_q8_decode(const NkbQ8Attn& g, int early) {
   if (group < 1 || g.nq % g.nkv || g.q_len < 1 || (long long)g.q_len * group > 16 || g.nkv > 65535 || g.batch > 65535) return -2;
   if (g.num_splits > 1 && (!g.scratch || (long long)g.batch * g.nkv > kQ8Counters)) return -2;
   if (!status_word() && nkb_init() != 0) return -1;
+  if (g.num_splits > 1 && g.scratch_floats < nkb_q8_attn_decode_scratch_floats(g.batch, g.nkv, g.head_dim, group, g.num_splits)) return -2;
   DecodeQ8Params p{};
   p.q = (const __nv_bfloat16*)g.q;
   p.block_table = g.block_table; p.context_lens = g.context_lens;

@@ -990,8 +990,9 @@ static long long p8_blocks(int batch, int max_q_len, int nq, int nkv) {
   return ((long long)max_q_len * (nq / nkv) + 2 * kP8Tile - 1) / (2 * kP8Tile) * nkv * batch;
 }
 
+// Negative: there is no device.
 extern "C" long long nkb_q8_attn_prefill_scratch_floats(int batch, int max_q_len, int nq, int nkv, int head_dim, int table_width) {
-  if (batch <= 0 || nkv < 1 || max_q_len < 1 || (!status_word() && nkb_init() != 0)) return 0;
+  if (batch <= 0 || nkv < 1 || nq < nkv || max_q_len < 1 || (!status_word() && nkb_init() != 0)) return -1;
   const long long blocks = p8_blocks(batch, max_q_len, nq, nkv);
   const int parts = p8_parts(blocks, table_width);
   return kQ8Counters + (parts > 1 ? kP8Counts + blocks * parts * 2 * kP8Tile * (head_dim + 2) : 0);
@@ -1013,6 +1014,7 @@ extern "C" int nkb_q8_attn_prefill(const NkbQ8Attn* arg) {
   const long long blocks = p8_blocks(g.batch, g.q_len, g.nq, g.nkv);
   p.parts = p8_parts(blocks, g.table_width);
   if (!g.scratch || blocks * p.parts > 0x3fffffffll) return -2;
+  if (g.scratch_floats < nkb_q8_attn_prefill_scratch_floats(g.batch, g.q_len, g.nq, g.nkv, g.head_dim, g.table_width)) return -2;
   p.sched = reinterpret_cast<unsigned int*>(g.scratch);
   p.counts = reinterpret_cast<int*>(g.scratch + kQ8Counters);
   p.partials = g.scratch + kQ8Counters + kP8Counts;

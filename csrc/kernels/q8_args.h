@@ -33,6 +33,7 @@ struct NkbQ8Attn {
   float* scratch;
   void* stream;
   long long table_stride;
+  long long scratch_floats;              // what there is of it; a call that wants more is refused
   int batch, total_q, q_len;             // q_len: new tokens of every sequence (prompts: at most)
   int nq, nkv, head_dim, num_blocks, table_width, causal, window, chunk, num_splits;
   float scale;

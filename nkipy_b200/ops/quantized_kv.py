@@ -291,8 +291,12 @@ def _p(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def _floats(scratch: Optional[torch.Tensor]) -> int:
+    return 0 if scratch is None else scratch.numel()
+
+
 # NkbQ8Append and NkbQ8Attn of csrc/kernels/q8_args.h: packed, a call takes a quarter of the time that as many arguments do
-_APPEND, _ATTN = struct.Struct("14Pqd8i"), struct.Struct("13Pq12ifi")
+_APPEND, _ATTN = struct.Struct("14Pqd8i"), struct.Struct("13P2q12ifi")
 
 
 MAX_SPLITS = 1024
@@ -315,14 +319,23 @@ def _scratch(device: torch.device, floats: int) -> torch.Tensor:
     return buf
 
 
+# (sizes go by the device's SMs, which the library knows once it is initialised)
 @functools.lru_cache(maxsize=4096)
 def _decode_floats(B: int, nkv: int, D: int, group: int, num_splits: int) -> int:
-    return _lib.lib().nkb_q8_attn_decode_scratch_floats(B, nkv, D, group, num_splits)
+    _lib.ensure_init()
+    floats = _lib.lib().nkb_q8_attn_decode_scratch_floats(B, nkv, D, group, num_splits)
+    if floats < 0:
+        raise _lib.KernelLibraryError(f"nkb_q8_attn_decode_scratch_floats failed with code {floats}")
+    return floats
 
 
 @functools.lru_cache(maxsize=4096)
 def _prefill_floats(B: int, max_q_len: int, nq: int, nkv: int, D: int, width: int) -> int:
-    return _lib.lib().nkb_q8_attn_prefill_scratch_floats(B, max_q_len, nq, nkv, D, width)
+    _lib.ensure_init()
+    floats = _lib.lib().nkb_q8_attn_prefill_scratch_floats(B, max_q_len, nq, nkv, D, width)
+    if floats < 0:
+        raise _lib.KernelLibraryError(f"nkb_q8_attn_prefill_scratch_floats failed with code {floats}")
+    return floats
 
 
 def _pick_splits(ctas: int, max_pages: int, sms: int = 148) -> int:
@@ -408,7 +421,7 @@ def paged_attn_decode(q, k_cache, v_cache, block_table, context_lens, scale, *, 
     num_splits, scratch = _splits(num_splits, scratch, B, nkv, D, group, width, k_cache.device)
     rc = _lib.lib().nkb_q8_attn_decode(_ATTN.pack(
         q_at, *k_cache.at, *v_cache.at, block_table.data_ptr(), 0, 0, context_lens.data_ptr(), out.data_ptr(), _p(sinks), _p(scratch), _stream(),
-        table_step, B, B * q_len, q_len, nq, nkv, D, blocks, width, 1, window, chunk, num_splits, scale, 0))
+        table_step, _floats(scratch), B, B * q_len, q_len, nq, nkv, D, blocks, width, 1, window, chunk, num_splits, scale, 0))
     if rc:
         _lib.check(rc, "nkb_q8_attn_decode")
     _count_launch()
@@ -447,7 +460,7 @@ def rope_attn_decode(qkv_partials, positions, slots, cos_sin, k_cache, v_cache, 
         _APPEND.pack(0, qkv_partials.data_ptr(), _p(bias), _p(positions), _p(slots), _p(cos_sin), _p(q_norm_w), _p(k_norm_w), q_at, *pages, stream,
                      stride, norm_eps, parts, B, nq, nkv, D, rows, blocks, 0),
         _ATTN.pack(q_at, *pages, block_table.data_ptr(), 0, 0, context_lens.data_ptr(), q_at, _p(sinks), _p(scratch), stream,
-                   table_step, B, B, 1, nq, nkv, D, blocks, width, 1, window, 0, num_splits, scale, 0))
+                   table_step, _floats(scratch), B, B, 1, nq, nkv, D, blocks, width, 1, window, 0, num_splits, scale, 0))
     if rc:
         _lib.check(rc, "nkb_q8_step")
     _count_launch(2)
@@ -483,7 +496,7 @@ def flash_attn_prefill(q, k_cache, v_cache, block_table, q_start, q_lens, contex
     scratch = _scratch(k_cache.device, floats)
     rc = _lib.lib().nkb_q8_attn_prefill(_ATTN.pack(
         q_at, *k_cache.at, *v_cache.at, block_table.data_ptr(), q_start.data_ptr(), q_lens.data_ptr(), context_lens.data_ptr(), out.data_ptr(),
-        _p(sinks), scratch.data_ptr(), _stream(), table_step, B, total, max_q_len, nq, nkv, D, blocks,
+        _p(sinks), scratch.data_ptr(), _stream(), table_step, scratch.numel(), B, total, max_q_len, nq, nkv, D, blocks,
         width, 1 if causal else 0, window, chunk, 1, scale, 0))
     if rc:
         _lib.check(rc, "nkb_q8_attn_prefill")
