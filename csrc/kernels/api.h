@@ -78,6 +78,8 @@ int nkb_gemm_bf16(const void* A, const void* B, void* out, int rows, int cols, i
                   int gate_off, const void* bias, int bias_on_rows, const void* residual, int block_n, int max_ctas,
                   int weights_operand, int ctas_per_sm, int act, float act_a, float act_b, void* stream);
 int nkb_gemm_effective_splits(int k, int splits);
+int nkb_query_turn(int t, int lo0, int hi0, int lo1, int hi1, int tile);   // query_turns.h, on the host
+int nkb_query_turns_from_first(int lo0, int hi0, int lo1, int hi1);
 int nkb_gemm_ring_stages(int block_n, int ctas_per_sm, int gated, int push);
 int nkb_gemm_bf16_2cta(const void* A, const void* B, void* out, int m, int n, int k, long long lda, long long ldb,
                        long long ldo, const void* bias, const void* residual, int gated, int gate_off, int act,

@@ -49,6 +49,7 @@
 // of examples/models/qwen3_embedding/kernels/attention.py.
 #include "common.cuh"
 #include "attn_maps.h"
+#include "query_turns.h"
 #include "api.h"
 #include <math.h>
 
@@ -384,8 +385,11 @@ flash_attn_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
     const uint32_t o_addr = tmem_base + lane_off + kOCol + t * 128;
     uint8_t* my_p = p_s + t * kPBytes + r * 128;
     const int n_tiles = (tr.rows > 0 ? kept : 0) + tr.hi - tr.lo;
-    // KV tiles of the other query tile
-    const int n_other = t == 0 ? (two ? kept + tr1.hi - tr1.lo : 0) : kept + tr0.hi - tr0.lo;
+    const NkbTurns shared = nkb_turns(t, tr0.lo, tr0.hi, two ? tr1.lo : 0, two ? tr1.hi : 0);
+    const int turn_from = shared.first - tr.lo;      // a tile less its turn (kept ones aside)
+    const uint32_t turns = shared.count;
+    const int wait_from = turn_from + 1 - t;
+    const uint32_t wait_n = max(shared.count - 1 + t, 0);
     float m = -INFINITY, l = 0.f;
     int hi_pos = ctx - 1;
     if (p.causal) hi_pos = min(hi_pos, q_pos);
@@ -566,9 +570,23 @@ flash_attn_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
       // as long as the rest of an iteration takes; left alone the two tiles fall into step (they share the K/V
       // ring), both compute exponentials at half speed and then both wait.  Alternating lets one tile use the unit
       // at full speed while the other loads its scores, takes the maximum and publishes P.
-      // Order: tile 0 (it), tile 1 (it), tile 0 (it + 1), ...; a tile that has run out of KV tiles is not waited for.
-      if (t == 0 ? (it >= 1 && it - 1 < n_other) : (it < n_other)) {
-        ok = pf_wait(&ctrl->turn[t][quad], uint32_t(t == 0 ? it - 1 : it) & 1u, abort_flag, p.status, ERR_WAIT_SOFTMAX);
+      // query_turns.h says at which KV tiles; the kept ones come first.  (Two ranges of `it` in registers: the header's own form in this loop
+      // took 16 prompts of 1024 tokens from 248 to 255 us.)
+      uint32_t turn;                       // the other tile's that this one waits for
+      bool waits, turned;
+      if constexpr (MODS) {
+        const bool early = it < kept;
+        const int at = early ? it : it - turn_from;
+        turned = early ? two : uint32_t(at - kept) < turns;
+        waits = turned && at >= 1 - t;
+        turn = at - 1 + t;
+      } else {
+        turned = uint32_t(it - turn_from) < turns;
+        turn = it - wait_from;
+        waits = turn < wait_n;
+      }
+      if (waits) {
+        ok = pf_wait(&ctrl->turn[t][quad], turn & 1u, abort_flag, p.status, ERR_WAIT_SOFTMAX);
         if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
       }
 #pragma unroll
@@ -578,7 +596,7 @@ flash_attn_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
         store_chunk(c, pk);
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ctrl->turn[1 - t][quad]);
+      if (lane == 0 && turned) mbar_arrive(&ctrl->turn[1 - t][quad]);
       fence_proxy_async();
       tc_fence_before();
       __syncwarp();
@@ -673,6 +691,12 @@ static int launch_prefill(const CUtensorMap& tq, const CUtensorMap& tk, const CU
 }  // namespace nkb
 
 using namespace nkb;
+
+// query_turns.h on the host: the turn of query tile t at a key tile, and how many there are from each one's first
+extern "C" int nkb_query_turn(int t, int lo0, int hi0, int lo1, int hi1, int tile) {
+  return nkb_turn_at(nkb_turns(t, lo0, hi0, lo1, hi1), tile);
+}
+extern "C" int nkb_query_turns_from_first(int lo0, int hi0, int lo1, int hi1) { return nkb_turns_from_first(lo0, hi0, lo1, hi1); }
 
 extern "C" int nkb_flash_attn_prefill(const void* q, const void* k_cache, const void* v_cache, const int* block_table,
                                       const int* q_start, const int* q_lens, const int* context_lens, void* out,

@@ -34,6 +34,7 @@
 #include "api.h"
 #include "kv_quant.cuh"
 #include "attn_maps.h"
+#include "query_turns.h"
 #include <cuda_fp16.h>
 #include <limits.h>
 #include <math.h>
@@ -74,8 +75,8 @@ struct P8Work {
   int block, part;                       // part: its number, and << 8 how many there are
   int u_lo, n_union;                     // tiles that either query tile attends to
   P8Range tr0, tr1;
-  // tiles whose exponentials the two take turns with
-  __device__ __forceinline__ int paired() const { return tr1.rows > 0 ? min(tr0.hi - tr0.lo, tr1.hi - tr1.lo) : 0; }
+  // tiles, from each one's first, whose exponentials the two take turns with
+  __device__ __forceinline__ int paired() const { return tr1.rows > 0 ? nkb_turns_from_first(tr0.lo, tr0.hi, tr1.lo, tr1.hi) : 0; }
 };
 constexpr int kP8Least = 4;              // tiles that are divided, one or more to a part
 constexpr int kP8Works = 3;              // works ahead of their use

@@ -1,5 +1,6 @@
 """Keys and values in 8 bits at their edges: scratch, queries and scales of unusual sizes, masks that part two query tiles, bytes that nobody sees."""
 
+import math
 import subprocess
 import sys
 
@@ -9,7 +10,7 @@ import torch
 from nkipy_b200 import ops
 from nkipy_b200.ops import _lib
 from nkipy_b200.ops import quantized_kv as Q
-from tests.test_quantized_kv import pool, shuffled_table
+from tests.test_quantized_kv import DEVICES, cached, pool, shuffled_table
 
 
 # ------------------------------------------------------------------------------------------------ scratch
@@ -94,3 +95,80 @@ def test_kernels_refuse_scratch_that_is_too_small(monkeypatch):
     with pytest.raises(_lib.KernelLibraryError):
         ops.flash_attn_prefill(q, k, v, table.cuda(), i32(0), i32(1), i32(900), 0.1, max_q_len=1)
     assert not bool(small.any())
+
+
+# ------------------------------------------------------------------------------------------------ attention, all rows of a sequence at once
+def attend(q, k, v, scale, pos0, causal=True, window=0, chunk=0, sink=None, weights=2.0 ** -11, lost=2.0 ** -30):
+    """One query head's rows q [n, dim] at positions pos0 on, over k, v [tokens, dim], in 64 bits: (results, tolerances).
+
+    As `test_quantized_kv.oracle_attend` has it: 2^-8 of the result for its rounding to bf16; of every weight `weights` for its own rounding
+    (f16: 2^-11, bf16: 2^-8), 2^-19 for exponential and sum, and twice what 2^-19 of the largest sum |q k| moves it by; `lost` of the largest
+    value that the row sees, for every token that it sees, for weights that end above nothing."""
+    pos, at = pos0 + torch.arange(q.shape[0])[:, None], torch.arange(k.shape[0])
+    seen = at <= pos if causal else torch.ones((q.shape[0], k.shape[0]), dtype=torch.bool)
+    if window:
+        seen = seen & (at > pos - window)
+    if chunk:
+        seen = seen & (at >= pos - pos % chunk)
+    s = (q @ k.T * scale).masked_fill(~seen, -math.inf)
+    top = s.amax(-1, keepdim=True)
+    if sink is not None:
+        top = top.clamp(min=sink)
+    top = torch.where(top == -math.inf, 0.0, top)
+    p = torch.exp(s - top)
+    total = p.sum(-1, keepdim=True) + (0.0 if sink is None else torch.exp(sink - top))
+    p = torch.where(total > 0, p / total, 0.0)
+    o = p @ v
+    moved = 2.0 ** -19 * (q.abs() @ k.abs().T).masked_fill(~seen, 0.0).amax(-1, keepdim=True) * scale
+    largest = v.abs().amax(-1).expand(seen.shape).masked_fill(~seen, 0.0).amax(-1, keepdim=True)
+    return o, 2.0 ** -8 * o.abs() + (p @ v.abs()) * (weights + 2.0 ** -19 + 2 * moved) + seen.sum(-1, keepdim=True) * lost * largest + 1e-30
+
+
+def check_rows(out, q, k, v, spans, scale, group, sinks=None, **masks):
+    """out, q [tokens, heads, dim]; k, v: a sequence's rows [context, kv heads, dim] each; spans: (first row, new tokens, context)."""
+    out, q = out.cpu().double(), q.cpu().double()
+    for b, (row, n, ctx) in enumerate(spans):
+        for h in range(q.shape[1]):
+            want, tol = attend(q[row:row + n, h], k[b][:, h // group].double(), v[b][:, h // group].double(), scale, ctx - n,
+                               sink=None if sinks is None else float(sinks[h]), **masks)
+            err = (out[row:row + n, h] - want).abs()
+            assert bool((err <= tol).all()), (b, h, float((err / tol).nan_to_num(math.inf).max()))
+
+
+def i32(x, device):
+    return torch.tensor(x, dtype=torch.int32, device=device)
+
+
+# ------------------------------------------------------------------------------------------------ masks that part two query tiles
+CHUNKS = [
+    # nq, nkv, (cached, new) per sequence, masks
+    (1, 1, [(200, 700)], dict(chunk=512)),                                   # the second 128 rows of a pair begin four key tiles later
+    (2, 2, [(0, 1500), (77, 300)], dict(chunk=1100)),
+    (4, 1, [(900, 300)], dict(chunk=1000)),
+    (1, 1, [(100, 800)], dict(chunk=512, window=300)),
+    (1, 1, [(130, 700)], dict(chunk=400, causal=False)),
+    (2, 1, [(1500, 40), (0, 200)], dict(chunk=700)),
+]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("nq,nkv,spans,masks", CHUNKS)
+def test_chunks_that_begin_between_query_tiles(device, dim, bits, nq, nkv, spans, masks):
+    g = torch.Generator().manual_seed(dim + nq)
+    contexts, new = [a + n for a, n in spans], [n for _, n in spans]
+    table, blocks = shuffled_table(g, contexts)
+    q = torch.randn((sum(new), nq * dim), generator=g).to(torch.bfloat16)
+    if bits == 8:
+        pages = pool(g, blocks, nkv, dim, device)
+        k, v = ([cached(p, table[b], c) for b, c in enumerate(contexts)] for p in pages)
+    else:
+        pages = [torch.randn((blocks, nkv, 32, dim), generator=g).to(torch.bfloat16) for _ in range(2)]
+        k, v = ([p[table[b, :-(-c // 32)].long()].transpose(1, 2).reshape(-1, nkv, dim)[:c] for b, c in enumerate(contexts)] for p in pages)
+        pages = [p.to(device) for p in pages]
+    starts = [sum(new[:b]) for b in range(len(new))]
+    out = ops.flash_attn_prefill(q.to(device), *pages, table.to(device), i32(starts, device), i32(new, device), i32(contexts, device),
+                                 dim ** -0.5, max_q_len=max(new), **masks)
+    check_rows(out.view(-1, nq, dim), q.view(-1, nq, dim), k, v, list(zip(starts, new, contexts)), dim ** -0.5, nq // nkv,
+               **masks, weights=2.0 ** -11 if bits == 8 else 2.0 ** -8)
