@@ -36,6 +36,7 @@
 #include "attn_maps.h"
 #include "query_turns.h"
 #include <cuda_fp16.h>
+#include <float.h>
 #include <limits.h>
 #include <math.h>
 
@@ -649,7 +650,8 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
           ok = ok && p8_wait(&ctrl->s_full[t], done + it & 1u, abort_flag, p.status, ERR_WAIT_TMEM_FULL);
           if (!__all_sync(kAll, ok)) { alive = false; break; }
           const int e_k = *(volatile int*)&ctrl->e_k[x % kP8Slots], e_v = *(volatile int*)&ctrl->e_v[x % kP8Slots];
-          const float to_log2 = cur.raw_log2 * exp2_int(e_k - int(kP8Lift)), add = float(e_v);
+          // not zero, for rows of zeros or next to it: masked scores are -infinity
+          const float to_log2 = fmaxf(cur.raw_log2 * exp2_int(e_k - int(kP8Lift)), FLT_MIN), add = float(e_v);
           tc_fence_after();
           uint32_t v[kP8Tile];
           constexpr int kFirst = 64;                          // scores whose maximum is taken while the others come

@@ -10,7 +10,7 @@ import torch
 from nkipy_b200 import ops
 from nkipy_b200.ops import _lib
 from nkipy_b200.ops import quantized_kv as Q
-from tests.test_quantized_kv import DEVICES, cached, pool, shuffled_table
+from tests.test_quantized_kv import DEVICES, cached, fill, pool, shuffled_table
 
 
 # ------------------------------------------------------------------------------------------------ scratch
@@ -172,3 +172,61 @@ def test_chunks_that_begin_between_query_tiles(device, dim, bits, nq, nkv, spans
                                  dim ** -0.5, max_q_len=max(new), **masks)
     check_rows(out.view(-1, nq, dim), q.view(-1, nq, dim), k, v, list(zip(starts, new, contexts)), dim ** -0.5, nq // nkv,
                **masks, weights=2.0 ** -11 if bits == 8 else 2.0 ** -8)
+
+
+# ------------------------------------------------------------------------------------------------ queries and keys of unusual sizes
+def prompt(q, pages, table, spans, scale, device, **masks):
+    """Rows [tokens, heads, dim] of `spans` (first row, new tokens, context)."""
+    n, heads, dim = q.shape
+    out = ops.flash_attn_prefill(q.reshape(n, heads * dim).to(device), *pages, table.to(device), *(i32([s[j] for s in spans], device) for j in (0, 1, 2)),
+                                 scale, max_q_len=max(s[1] for s in spans), **{m: x.to(device) if m == "sinks" else x for m, x in masks.items()})
+    return out.view(n, heads, dim)
+
+
+def rows_of(pages, table, spans):
+    """Keys and values of every sequence, [context, kv heads, dim] in 64 bits."""
+    return ([cached(p, table[b], ctx) for b, (_, _, ctx) in enumerate(spans)] for p in pages)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("sinks", [False, True])
+@pytest.mark.parametrize("nq,nkv,spans,masks", [
+    (4, 2, [(0, 200, 200), (200, 33, 350), (233, 1, 77)], {}),
+    (2, 1, [(0, 140, 300)], dict(window=50)),
+    (8, 1, [(0, 5, 2100), (5, 3, 1000)], {}),                               # divided among works
+    (4, 4, [(70 * i, 70, 70) for i in range(40)], {}),
+    (4, 1, [(0, 130, 260)], dict(chunk=100)),
+])
+def test_queries_that_are_zero_or_tiny(device, dim, sinks, nq, nkv, spans, masks):
+    """Rows of zeros see the mean of their values, rows next to zero the same within the tolerance."""
+    g = torch.Generator().manual_seed(dim + nq)
+    table, blocks = shuffled_table(g, [c for _, _, c in spans])
+    pages = pool(g, blocks, nkv, dim, device)
+    q = torch.randn((sum(n for _, n, _ in spans), nq, dim), generator=g).to(torch.bfloat16)
+    size = torch.randint(0, 4, q.shape[:2], generator=g)
+    q = torch.where(size[..., None] == 0, q, q * torch.tensor([0.0, 0.0, 1e-20, 1e-38])[size][..., None]).to(torch.bfloat16)
+    q[:, -1] = 0.0                                                          # a head of zeros
+    s = torch.randn((nq,), generator=g) if sinks else None
+    out = prompt(q, pages, table, spans, dim ** -0.5, device, **masks, **({"sinks": s} if sinks else {}))
+    check_rows(out, q, *rows_of(pages, table, spans), spans, dim ** -0.5, nq // nkv, s, **masks)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("keys", [0.0, 2.0 ** -60, 2.0 ** -30, 2.0 ** 60])
+def test_keys_that_are_zero_or_far_from_one(device, dim, keys):
+    g = torch.Generator().manual_seed(dim)
+    spans, nq = [(0, 150, 250), (150, 5, 1500)], 2
+    table, blocks = shuffled_table(g, [c for _, _, c in spans])
+    k, v = pool(g, blocks, 1, dim, device)
+    fill(k, torch.randn((blocks, 1, 32, dim), generator=g, dtype=torch.float64) * keys)
+    for size in (0.0, 1e-30, 2.0 ** -60, 1.0):
+        if size * keys > 2.0 ** 10:
+            continue
+        q = (torch.randn((155, nq, dim), generator=g) * size).to(torch.bfloat16)
+        for scale in (dim ** -0.5, 1e-6):
+            out = prompt(q, (k, v), table, spans, scale, device)
+            check_rows(out, q, *rows_of((k, v), table, spans), spans, scale, nq)
+            one = ops.paged_attn_decode(q[149:151].reshape(2, -1).to(device), k, v, table.to(device), i32([250, 1500], device), scale)
+            check_rows(one.view(2, nq, dim), q[149:151], *rows_of((k, v), table, spans), [(0, 1, 250), (1, 1, 1500)], scale, nq)
