@@ -807,8 +807,8 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
           }
         }
         const int e = max((__float_as_int(mx) >> 23) - 127, -100);
-        const float up = exp2_int(14 - e);
-        next.raw_log2 = p.scale_log2 * exp2_int(e - 14);
+        const float up = copysignf(exp2_int(14 - e), p.scale_log2);       // the largest score has the largest exponent so
+        next.raw_log2 = fabsf(p.scale_log2) * exp2_int(e - 14);
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
           const uint32_t q4[4] = {v[i].x, v[i].y, v[i].z, v[i].w};

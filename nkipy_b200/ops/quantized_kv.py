@@ -20,6 +20,7 @@ them (its cache is dense and bf16, examples/models/qwen3/qwen3.py:52-71).
 from __future__ import annotations
 
 import functools
+import math
 import struct
 from typing import Optional, Tuple
 
@@ -270,9 +271,11 @@ def _check_qkv(qkv, positions, slots, cos_sin, k_cache, nq, nkv, head_dim, bias,
     return T, parts, stride, rows
 
 
-def _check_masks(mods, window: int, chunk: int, sinks, nq: int, index: int) -> None:
+def _check_masks(mods, scale: float, window: int, chunk: int, sinks, nq: int, index: int) -> None:
     if mods:
         raise ValueError("attention over QuantizedPages takes no score modifications")
+    if not math.isfinite(scale):
+        raise ValueError("scale is a finite number")
     if window < 0 or chunk < 0:
         raise ValueError("window and chunk are not negative")
     if sinks is not None:
@@ -401,7 +404,7 @@ def paged_attn_decode(q, k_cache, v_cache, block_table, context_lens, scale, *, 
     B, width, table_step = _check_table(block_table, context_lens, index)
     nq = q.shape[-1] // D
     group = _check_heads(nq, nkv)
-    _check_masks(mods, window, chunk, sinks, nq, index)
+    _check_masks(mods, scale, window, chunk, sinks, nq, index)
     if q_len < 1 or num_splits > MAX_SPLITS:
         raise ValueError(f"q_len is at least one, num_splits at most {MAX_SPLITS}")
     q_at = _want_rows(q, "q", (B * q_len, nq * D), index)
@@ -445,7 +448,7 @@ def rope_attn_decode(qkv_partials, positions, slots, cos_sin, k_cache, v_cache, 
         return paged_attn_decode(q, k_cache, v_cache, block_table, context_lens, scale, window=window, sinks=sinks, num_splits=num_splits,
                                  scratch=scratch, out=out)
     _, parts, stride, rows = _check_qkv(qkv_partials, positions, slots, cos_sin, k_cache, nq, nkv, D, bias, q_norm_w, k_norm_w)
-    _check_masks(None, window, 0, sinks, nq, index)
+    _check_masks(None, scale, window, 0, sinks, nq, index)
     if num_splits > MAX_SPLITS:
         raise ValueError(f"num_splits is at most {MAX_SPLITS}")
     if out is None:
@@ -475,7 +478,7 @@ def flash_attn_prefill(q, k_cache, v_cache, block_table, q_start, q_lens, contex
     B, width, table_step = _check_table(block_table, context_lens, index)
     nq, total = q.shape[-1] // D, q.shape[0]
     _check_heads(nq, nkv)
-    _check_masks(mods, window, chunk, sinks, nq, index)
+    _check_masks(mods, scale, window, chunk, sinks, nq, index)
     q_at = _want_rows(q, "q", (total, nq * D), index)
     _want(q_start, "q_start", torch.int32, (B,), index)
     _want(q_lens, "q_lens", torch.int32, (B,), index)

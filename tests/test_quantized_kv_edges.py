@@ -119,7 +119,7 @@ def attend(q, k, v, scale, pos0, causal=True, window=0, chunk=0, sink=None, weig
     total = p.sum(-1, keepdim=True) + (0.0 if sink is None else torch.exp(sink - top))
     p = torch.where(total > 0, p / total, 0.0)
     o = p @ v
-    moved = 2.0 ** -19 * (q.abs() @ k.abs().T).masked_fill(~seen, 0.0).amax(-1, keepdim=True) * scale
+    moved = 2.0 ** -19 * (q.abs() @ k.abs().T).masked_fill(~seen, 0.0).amax(-1, keepdim=True) * abs(scale)
     largest = v.abs().amax(-1).expand(seen.shape).masked_fill(~seen, 0.0).amax(-1, keepdim=True)
     return o, 2.0 ** -8 * o.abs() + (p @ v.abs()) * (weights + 2.0 ** -19 + 2 * moved) + seen.sum(-1, keepdim=True) * lost * largest + 1e-30
 
@@ -230,3 +230,32 @@ def test_keys_that_are_zero_or_far_from_one(device, dim, keys):
             check_rows(out, q, *rows_of((k, v), table, spans), spans, scale, nq)
             one = ops.paged_attn_decode(q[149:151].reshape(2, -1).to(device), k, v, table.to(device), i32([250, 1500], device), scale)
             check_rows(one.view(2, nq, dim), q[149:151], *rows_of((k, v), table, spans), [(0, 1, 250), (1, 1, 1500)], scale, nq)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("scale", [-1.0, -0.05, 0.0, 1e-30, -1e-40])
+def test_scales_of_scores(device, dim, scale):
+    g = torch.Generator().manual_seed(dim)
+    spans, nq = [(0, 150, 250), (150, 5, 1500)], 2
+    table, blocks = shuffled_table(g, [c for _, _, c in spans])
+    pages = pool(g, blocks, 1, dim, device)
+    q = torch.randn((155, nq, dim), generator=g).to(torch.bfloat16)
+    check_rows(prompt(q, pages, table, spans, scale, device), q, *rows_of(pages, table, spans), spans, scale, nq)
+    one = ops.paged_attn_decode(q[149:151].reshape(2, -1).to(device), *pages, table.to(device), i32([250, 1500], device), scale)
+    check_rows(one.view(2, nq, dim), q[149:151], *rows_of(pages, table, spans), [(0, 1, 250), (1, 1, 1500)], scale, nq)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_scales_that_are_not_finite_are_refused(device):
+    g = torch.Generator().manual_seed(0)
+    table, blocks = shuffled_table(g, [40])
+    pages, q = pool(g, blocks, 1, 64, device), torch.zeros((1, 1, 64), dtype=torch.bfloat16)
+    for scale in (math.nan, math.inf, -math.inf):
+        with pytest.raises(ValueError):
+            prompt(q, pages, table, [(0, 1, 40)], scale, device)
+        with pytest.raises(ValueError):
+            ops.paged_attn_decode(q[0].to(device), *pages, table.to(device), i32([40], device), scale)
+        with pytest.raises(ValueError):
+            ops.rope_attn_decode(torch.zeros((1, 1, 3 * 64), device=device), i32([39], device), i32([-1], device), None, *pages, table.to(device),
+                                 i32([40], device), scale, 1, 1)
