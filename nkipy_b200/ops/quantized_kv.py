@@ -2,7 +2,7 @@
 
 A page of 32 tokens of one kv head is e4m3 values ``[32, dim]`` and one power of two per token.  A head's row x is kept as
 ``e4m3(x / 2^e)`` (nearest, ties to even) and e, the smallest whole number with ``max|x| <= 448 * 2^e``, between -64 and 64: rows
-beyond 448 * 2^64 saturate, and what is below 2^-74 becomes zero.  A row that holds a value which is not finite stands for NaN as a whole
+beyond 448 * 2^64 saturate, and what is below 2^-74 becomes zero.  Powers that no row has stand for the nearest that one may have.  A row that holds a value which is not finite stands for NaN as a whole
 (scale NaN, values 0), so that a NaN in a masked place has no way into a sum.
 
 One scale per token and head, because tokens are appended one at a time: a scale that several tokens shared would have to be
@@ -78,6 +78,7 @@ class QuantizedPages:
         v, s = self.values.view(torch.uint8), self.scales.view(torch.uint8)
         if blocks is not None:
             v, s = v[blocks], s[blocks]
+        s = torch.where(s == 255, s, s.clamp(127 + LOG2_MIN, 127 + LOG2_MAX))
         return v.view(torch.float8_e4m3fn).float() * s.view(torch.float8_e8m0fnu).float()[..., None]
 
 

@@ -259,3 +259,22 @@ def test_scales_that_are_not_finite_are_refused(device):
         with pytest.raises(ValueError):
             ops.rope_attn_decode(torch.zeros((1, 1, 3 * 64), device=device), i32([39], device), i32([-1], device), None, *pages, table.to(device),
                                  i32([40], device), scale, 1, 1)
+
+
+# ------------------------------------------------------------------------------------------------ scale bytes that no row has
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("byte,stands_for", [(0, 63), (1, 63), (62, 63), (192, 191), (254, 191)])
+def test_scales_outside_the_range_stand_for_its_ends(device, byte, stands_for):
+    g = torch.Generator().manual_seed(byte)
+    dim, nq, spans = 64, 2, [(0, 1, 40)]
+    table, blocks = shuffled_table(g, [40])
+    k, v = pool(g, blocks, 1, dim, device)
+    v.scales.view(torch.uint8)[...] = byte
+    want = v.values.float() * 2.0 ** (stands_for - 127)
+    assert torch.equal(v.dequantize(), want) and torch.equal(v.dequantize(torch.tensor([1], device=device)), want[1:2])
+    keys, _ = rows_of((k, v), table, spans)
+    values = [want.cpu()[table[0].long()].transpose(1, 2).reshape(-1, 1, dim)[:40]]
+    q = torch.randn((1, nq, dim), generator=g).to(torch.bfloat16)
+    for out in (prompt(q, (k, v), table, spans, 0.125, device),
+                ops.paged_attn_decode(q.view(1, -1).to(device), k, v, table.to(device), i32([40], device), 0.125).view(1, nq, dim)):
+        check_rows(out, q, keys, values, spans, 0.125, nq)
