@@ -209,6 +209,7 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
     }
   }
   const int all_hi = ctx - p.q_len, all_lo = nkb_first_visible(ctx - 1, p.window, p.chunk);      // what every row sees
+  const int any_lo = nkb_first_visible(ctx - p.q_len, p.window, p.chunk);                        // and what one does, up to ctx
 
   // lane (g, t): rows 2 t, 2 t + 1 of columns 16 c + 2 g, 16 c + 2 g + 1
   float o[NT][D / 16][4], m[NT][2], l[NT][2];
@@ -298,6 +299,20 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
           for (int e = 0; e < 4; ++e) {
             const int tok = tok0 + mt * 16 + (e >> 1) * 8 + g;
             if (tok > pos[nt][e & 1] || tok < low[nt][e & 1]) s[mt][nt][e] = -INFINITY;
+          }
+        }
+      }
+      // what no row sees may be anything: a lane's values are of tokens 2 t and 2 t + 1 of each eight
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int tok = tok0 + mt * 16 + h * 8 + 2 * t;
+          const uint32_t keep = (tok >= any_lo && tok < ctx ? 0xffffu : 0u) | (tok + 1 >= any_lo && tok + 1 < ctx ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int c2 = 0; c2 < D / 32; ++c2) {
+            vr[mt][c2][h] &= keep;
+            vr[mt][c2][2 + h] &= keep;
           }
         }
       }

@@ -2,8 +2,10 @@
 
 A page of 32 tokens of one kv head is e4m3 values ``[32, dim]`` and one power of two per token.  A head's row x is kept as
 ``e4m3(x / 2^e)`` (nearest, ties to even) and e, the smallest whole number with ``max|x| <= 448 * 2^e``, between -64 and 64: rows
-beyond 448 * 2^64 saturate, and what is below 2^-74 becomes zero.  Powers that no row has stand for the nearest that one may have.  A row that holds a value which is not finite stands for NaN as a whole
-(scale NaN, values 0), so that a NaN in a masked place has no way into a sum.
+beyond 448 * 2^64 saturate, and what is below 2^-74 becomes zero.  A row that holds a value which is not finite stands for NaN as a whole
+(scale NaN, values 0), so that a NaN in a masked place has no way into a sum.  Scale bytes that no row has stand for the nearest that
+one may have.  What no query of a call sees, behind a context or before a window, may be any bytes; what one of them sees has no e4m3
+NaN among its values.
 
 One scale per token and head, because tokens are appended one at a time: a scale that several tokens shared would have to be
 guessed, or change what is stored already.  A power of two, because e4m3 is a floating type: another factor would keep no more

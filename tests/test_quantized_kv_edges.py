@@ -278,3 +278,41 @@ def test_scales_outside_the_range_stand_for_its_ends(device, byte, stands_for):
     for out in (prompt(q, (k, v), table, spans, 0.125, device),
                 ops.paged_attn_decode(q.view(1, -1).to(device), k, v, table.to(device), i32([40], device), 0.125).view(1, nq, dim)):
         check_rows(out, q, keys, values, spans, 0.125, nq)
+
+
+# ------------------------------------------------------------------------------------------------ bytes that nobody sees
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("byte", [0x7f, 0xff, 0x7e])
+@pytest.mark.parametrize("q_len,masks", [(1, {}), (1, dict(window=45)), (3, {}), (4, dict(window=40)), (2, dict(chunk=48))])
+def test_bytes_that_nobody_sees(device, dim, byte, q_len, masks):
+    """Behind a context, before a window and in other blocks: e4m3's NaN or largest number, with any scale."""
+    g = torch.Generator().manual_seed(dim + byte + q_len)
+    nq, nkv, contexts = 4, 2, [37, 150, 64, 700, q_len]
+    table, blocks = shuffled_table(g, contexts, extra=2)
+    pages = pool(g, blocks, nkv, dim, device)
+    spans = [(b * q_len, q_len, c) for b, c in enumerate(contexts)]
+    k, v = rows_of(pages, table, spans)
+    seen = torch.zeros((blocks, 32), dtype=torch.bool)
+    for b, c in enumerate(contexts):
+        first = c - q_len
+        lo = max(first - masks.get("window", c) + 1, first - first % masks["chunk"] if "chunk" in masks else 0, 0)
+        for j in range(lo, c):
+            seen[table[b, j // 32], j % 32] = True
+    for p in pages:
+        values, scales = p.values.view(torch.uint8).cpu(), p.scales.view(torch.uint8).cpu()
+        values[~seen[:, None].expand(scales.shape)] = byte
+        scales[~seen[:, None].expand(scales.shape)] = torch.randint(0, 256, (int((~seen).sum()) * nkv,), generator=g).to(torch.uint8)
+        p.values.view(torch.uint8).copy_(values)
+        p.scales.view(torch.uint8).copy_(scales)
+    q = torch.randn((len(contexts) * q_len, nq, dim), generator=g).to(torch.bfloat16)
+    for splits in (1, 4):
+        out = ops.paged_attn_decode(q.view(q.shape[0], -1).to(device), *pages, table.to(device), i32(contexts, device), 0.1, q_len=q_len,
+                                    num_splits=splits, **masks)
+        check_rows(out.view(q.shape), q, k, v, spans, 0.1, 2, **masks)
+    check_rows(prompt(q, pages, table, spans, 0.1, device, **masks), q, k, v, spans, 0.1, 2, **masks)
+    if q_len == 1 and "chunk" not in masks:                                  # the step: nothing appended, queries as they are
+        qkv = torch.cat([q.float().view(5, -1), torch.zeros((5, 2 * nkv * dim))], -1)[None].to(device)
+        out = ops.rope_attn_decode(qkv, i32([0] * 5, device), i32([-1] * 5, device), None, *pages, table.to(device), i32(contexts, device), 0.1, nq,
+                                   nkv, **masks)
+        check_rows(out.view(q.shape), q, k, v, spans, 0.1, 2, **masks)
