@@ -4,7 +4,10 @@
 //
 // with 2^{k_j} and 2^{v_j} the powers of two that token j's key and value are kept with.  The sums run over t_j = s_j + v_j: weights
 // 2^{t_j - M}, M near the largest t so far, multiply the values as they are kept, and 2^{-v_j} takes a weight back to the denominator.  So
-// values of any size meet weights that f16 holds: a weight below 2^-30 of the largest contribution is all that rounds to nothing.
+// values of any size meet weights that f16 holds: a weight below 2^-30 of the largest contribution is all that rounds to nothing.  In the
+// denominator a token counts by its score alone: where v_j is so small that 2^{t_j - M} may be below the least normal number while the
+// token still counts (a row of zeros beside values of 2^40 or more), it gets an exponential of its own, and factors of the denominator go
+// on in two steps.
 //
 // The op is bound by the bytes of the pages, half of a bf16 cache's, and next by what a warp does per page.  Four bytes are two
 // conversions to f16 (exact; e4m3 has no matrix instruction with 16-bit queries).  Keys and columns of values are the 16-row side of the
@@ -34,6 +37,7 @@ constexpr int kQ8Stages = 3;
 template <int D>
 constexpr int kQ8SmWarps = 1024 / D;
 constexpr float kQ8Lift = 6.f;         // log2 of the weight at M; t may grow by kQ8Grow above M before M follows: f16 ends at 2^16
+constexpr int kQ8Tiny = -40;            // log2 of a value's scale: 2^-126 (f32) 2^40 is 2^-28 of the least that a token at M adds
 constexpr float kQ8Grow = 8.f;
 
 struct DecodeQ8Params {
@@ -325,7 +329,7 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) grow = grow || mx[nt][0] > m[nt][0] + kQ8Grow || mx[nt][1] > m[nt][1] + kQ8Grow;
     // M follows the largest t when that has grown by more than kQ8Grow
-    if (__any_sync(kAll, grow)) {
+    if (__any_sync(kAll, grow || v_log2 < kQ8Tiny)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float keep[2];
@@ -335,14 +339,31 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
           x = fmaxf(x, __shfl_xor_sync(kAll, x, 4));
           x = fmaxf(x, __shfl_xor_sync(kAll, x, 8));
           x = fmaxf(fmaxf(x, __shfl_xor_sync(kAll, x, 16)), m[nt][i]);
-          keep[i] = m[nt][i] == x ? 1.f : exp2f(m[nt][i] - x);
+          const float root = m[nt][i] == x ? 1.f : exp2f(0.5f * (m[nt][i] - x));
+          keep[i] = root * root;
           m[nt][i] = x;
-          l[nt][i] *= keep[i];
+          l[nt][i] = l[nt][i] * root * root;
         }
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) {
           o[nt][c][0] *= keep[0]; o[nt][c][1] *= keep[1];
           o[nt][c][2] *= keep[0]; o[nt][c][3] *= keep[1];
+        }
+      }
+      if (__any_sync(kAll, v_log2 < kQ8Tiny)) {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int ve = __shfl_sync(kAll, v_log2, mt * 16 + h * 8 + g);
+            if (ve >= kQ8Tiny) continue;
+            back[mt][h] = 0.f;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+              for (int i = 0; i < 2; ++i) l[nt][i] += exp2f(s[mt][nt][2 * h + i] - (m[nt][i] == -INFINITY ? 0.f : m[nt][i]) + (kQ8Lift - float(ve)));
+            }
+          }
         }
       }
     }
@@ -438,10 +459,10 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
     for (int w = 0; w < W; ++w) mf = fmaxf(mf, mm[w * 16 + r]);
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      const float mw = mm[w * 16 + r], sc = mw == -INFINITY && mf != -INFINITY ? 0.f : exp2f(mw == mf ? 0.f : mw - mf);
+      const float mw = mm[w * 16 + r], root = mw == -INFINITY && mf != -INFINITY ? 0.f : exp2f(mw == mf ? 0.f : 0.5f * (mw - mf)), sc = root * root;
       const float4 x = *reinterpret_cast<const float4*>(mo + (w * 16 + r) * L::kPitch + d);
       acc.x += sc * x.x; acc.y += sc * x.y; acc.z += sc * x.z; acc.w += sc * x.w;
-      l += sc * ml[w * 16 + r];
+      l += root * ml[w * 16 + r] * root;
     }
     if (plan.splits == 1) {
       finish(r, d, mf, l, acc);
@@ -487,16 +508,16 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
       float mn = mf;
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) mn = fmaxf(mn, ms[i]);
-      const float keep = mf == mn ? 1.f : exp2f(mf - mn);
+      const float kept = mf == mn ? 1.f : exp2f(0.5f * (mf - mn)), keep = kept * kept;
       acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
-      l *= keep;
+      l = l * kept * kept;
       mf = mn;
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         if (s0 + i >= plan.splits) break;
-        const float sc = ms[i] == mn ? 1.f : exp2f(ms[i] - mn);
+        const float root = ms[i] == mn ? 1.f : exp2f(0.5f * (ms[i] - mn)), sc = root * root;
         acc.x += sc * x[i].x; acc.y += sc * x[i].y; acc.z += sc * x[i].z; acc.w += sc * x[i].w;
-        l += sc * ls[i];
+        l += root * ls[i] * root;
       }
     }
     finish(r, d, mf, l, acc);

@@ -316,3 +316,43 @@ def test_bytes_that_nobody_sees(device, dim, byte, q_len, masks):
         out = ops.rope_attn_decode(qkv, i32([0] * 5, device), i32([-1] * 5, device), None, *pages, table.to(device), i32(contexts, device), 0.1, nq,
                                    nkv, **masks)
         check_rows(out.view(q.shape), q, k, v, spans, 0.1, 2, **masks)
+
+
+# ------------------------------------------------------------------------------------------------ values of very different sizes
+def stored_rows(g, pages, table, spans, sizes):
+    """Random rows in the pages, the sequences' tokens times their sizes (one tensor of them per sequence)."""
+    rows = torch.randn(pages.values.shape, generator=g, dtype=torch.float64)
+    for b, (_, _, ctx) in enumerate(spans):
+        at = torch.arange(ctx)
+        rows[table[b, at // 32].long(), :, at % 32] *= sizes[b][:, None, None]
+    fill(pages, rows)
+
+
+def zeros_and_large(g, dim, large, places, device):
+    """Pages of three sequences whose values are zero or large, by thirds or halves of their tokens; (pages, table, contexts)."""
+    contexts = [700, 900, 64]
+    table, blocks = shuffled_table(g, contexts)
+    k, v = (ops.QuantizedPages.new(blocks, 1, dim, device) for _ in range(2))
+    spans = [(0, 0, c) for c in contexts]
+    stored_rows(g, k, table, spans, [torch.full((c,), 0.5, dtype=torch.float64) for c in contexts])
+    stored_rows(g, v, table, spans, [torch.tensor(places)[torch.arange(c) * len(places) // c].double() * large for c in contexts])
+    return (k, v), table, contexts
+
+
+LARGE = [2.0 ** 40, 2.0 ** 60, 2.0 ** 70]
+PLACES = [[0.0, 1.0], [1.0, 0.0], [0.0, 1.0, 0.0]]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("large", LARGE)
+@pytest.mark.parametrize("places", PLACES)
+def test_rows_of_zeros_count_beside_large_values(device, dim, large, places):
+    """Tokens whose values are zero, and with them their scales the smallest, take their part of the denominator."""
+    g = torch.Generator().manual_seed(dim)
+    pages, table, contexts = zeros_and_large(g, dim, large, places, device)
+    q = torch.randn((3, 2, dim), generator=g).to(torch.bfloat16)
+    spans = [(b, 1, c) for b, c in enumerate(contexts)]
+    for splits in (1, 4):
+        out = ops.paged_attn_decode(q.view(3, -1).to(device), *pages, table.to(device), i32(contexts, device), 0.3, num_splits=splits)
+        check_rows(out.view(q.shape), q, *rows_of(pages, table, spans), spans, 0.3, 2)
