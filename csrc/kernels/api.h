@@ -161,6 +161,7 @@ long long nkb_q8_attn_decode_scratch_floats(int batch, int nkv, int head_dim, in
 int nkb_q8_attn_decode(const NkbQ8Attn* arg);
 int nkb_q8_step(const NkbQ8Append* append, const NkbQ8Attn* attn);
 long long nkb_q8_attn_prefill_scratch_floats(int batch, int max_q_len, int nq, int nkv, int head_dim, int table_width);
+int nkb_q8_attn_prefill_launches(int batch, int max_q_len, int nq, int nkv, int table_width);
 int nkb_q8_attn_prefill(const NkbQ8Attn* arg);
 int nkb_decode_advance(int* context_lens, const int* block_table, int* positions, int* slots, int batch, int q_len,
                        int max_blocks, int block_size, void* stream);

@@ -49,6 +49,10 @@ constexpr int kP8Slots = 8;              // tiles whose scales are kept
 constexpr int kP8Lead = 4;               // tiles that warp 14 is ahead of the conversion of V at most
 constexpr float kP8Grow = 8.f;           // log2 of the growth of a row's maximum that makes O follow
 constexpr float kP8Lift = 6.f;           // log2 of a weight at the maximum, and of a value at the tile's largest scale
+// log2 of what a tile's scales may lie above all that a row sees: keys then keep 2^-23 of the row's largest, and weights, whose exponent V is
+// part of, 2^-22 of the largest contribution
+constexpr int kP8MoreK = 16, kP8MoreV = 8;
+constexpr int kP8Apart = 92;             // log2 of V of one tile over that of another: what is below 2^-126 is 2^-34 of the denominator then
 
 struct PrefillQ8Params {
   const __nv_bfloat16* q;
@@ -65,6 +69,7 @@ struct PrefillQ8Params {
   int parts;                             // of a block's tiles at most, each a work of its own
   int* counts;                           // [block] how many there are
   float* partials;                       // their results: [block][part][256 rows of D columns, then maxima, then sums]
+  int* again;                            // [block][part] the work that this CTA looks at again behind this one (see p8_again)
 };
 
 // Piece of work of a CTA: 256 rows of a sequence's kv head
@@ -97,6 +102,9 @@ struct PrefillQ8Ctrl {
   uint8_t bytes[kP8Slots][2][kP8Tile];   // scales of K and of V
   uint32_t tmem_base;
   int abort;
+  // (behind the others, whose places matter: with these two among them 16 prompts of 1024 tokens took 228 us for 224)
+  int again;                             // the first work to look at again, < 0: none
+  uint64_t done;                         // softmax warps and warp 14 have done all works
 };
 
 // Bounded barrier wait of a few instructions: the kernel has two dozen of them beside its unrolled loops, and a call would not allow the
@@ -246,6 +254,192 @@ struct P8Rows {
   }
 };
 
+// ---- rows whose tiles hold scales far above all that they see
+// A tile's scales K and V are the largest of its tokens, which some row sees and another does not.  To a row that sees only far smaller
+// ones f16 has little of them left, and weights below a maximum that V is part of.  So warp 14 marks works where that may be: where a
+// tile that not all rows see has scales far above its smallest and above those of the tiles that all rows see, or where V of the tiles lies so far
+// apart that the denominator may lose a tile.  When a CTA has no more works, the four converting warps look at the rows of those once more
+// and compute those that it concerns by 32-bit products, token by token (some 1000 instructions of a warp per row and page), in the
+// place of the first result.  Nothing of this is in the loop over tiles; what warp 14 notes costs a percent (16 prompts of 1024 220 -> 222 us,
+// 4 x 2000 of 64 columns with a window of 128 68.4 -> 70.1; noted by the converting warps 226 and 70.5).
+
+__device__ __forceinline__ int p8_page_block(const PrefillQ8Params& p, int b, int page) {
+  const int blk = p.block_table[b * p.table_stride + page];
+  return blk >= 0 && blk < p.num_blocks ? blk : -1;
+}
+
+// Largest scales (bytes) of a tile: of what the work sees, and of what this lane's row sees of it, [lo, hi]
+struct P8Largest {
+  int k_tile, v_tile, k_row, v_row;
+};
+__device__ __forceinline__ void p8_largest(const PrefillQ8Params& p, const P8Work& k, int tile, int vis_lo, int vis_hi, int lo, int hi, P8Largest& o) {
+#pragma unroll 1
+  for (int pg = 0; pg < 4; ++pg) {
+    const int page = tile * 4 + pg;
+    if (page * kQ8Page >= k.ctx) break;
+    const int blk = p8_page_block(p, k.b, page);
+    const long long at = ((long long)blk * p.nkv + k.kvh) * kQ8Page;
+#pragma unroll 1
+    for (int j = 0; j < kQ8Page; j += 4) {
+      const uint32_t kb = blk >= 0 ? *reinterpret_cast<const uint32_t*>(p.k_scales + at + j) : 0x7f7f7f7fu;
+      const uint32_t vb = blk >= 0 ? *reinterpret_cast<const uint32_t*>(p.v_scales + at + j) : 0x7f7f7f7fu;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int tok = page * kQ8Page + j + i, kx = (kb >> (8 * i)) & 255, vx = (vb >> (8 * i)) & 255;
+        if (tok >= vis_lo && tok < vis_hi && kx != 255 && vx != 255) {
+          o.k_tile = max(o.k_tile, kx);
+          o.v_tile = max(o.v_tile, vx);
+          if (tok >= lo && tok <= hi) {
+            o.k_row = max(o.k_row, kx);
+            o.v_row = max(o.v_row, vx);
+          }
+        }
+      }
+    }
+  }
+}
+
+// One row (`at`, of heads) by a warp, over positions [lo, hi].  A whole result goes to its place; that of a part to `part`, with its maximum
+// and sum at `tail`.
+template <int D>
+__device__ __forceinline__ void p8_row(const PrefillQ8Params& p, const P8Work& k, long long at, int head, int lo, int hi, float* part, float* tail,
+                                       int lane) {
+  constexpr int N = D / 32;
+  constexpr uint32_t kAll = 0xffffffffu;
+  const __nv_bfloat16* q = p.q + at * D;
+  float mx = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) mx = fmaxf(mx, fabsf(__bfloat162float(q[lane * N + i])));
+  mx = warp_max(mx);
+  const int e = max((__float_as_int(mx) >> 23) - 127, -100);
+  const float up = exp2_int(14 - e), rs = p.scale_log2 * exp2_int(e - 14);
+  float m = -INFINITY, l = 0.f, o[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) o[i] = 0.f;
+#pragma unroll 1
+  for (int page = lo >> 5; page <= hi >> 5; ++page) {
+    const int blk = p8_page_block(p, k.b, page), tok = page * kQ8Page + lane;
+    const long long first = ((long long)max(blk, 0) * p.nkv + k.kvh) * kQ8Page;
+    const int kb = blk >= 0 ? p.k_scales[first + lane] : 127, vb = blk >= 0 ? p.v_scales[first + lane] : 127;
+    float dot = 0.f;
+    if (blk >= 0) {
+      const uint4* key = reinterpret_cast<const uint4*>(p.k_values + (first + lane) * D);
+#pragma unroll 1
+      for (int c = 0; c < D / 16; ++c) {
+        const uint4 x4 = key[c];
+        const uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint2 q4 = *reinterpret_cast<const uint2*>(q + c * 16 + j * 4);
+          const float2 q0 = unpack_bf16x2(q4.x), q1 = unpack_bf16x2(q4.y);
+          const uint32_t h0 = e4m3x2_to_f16x2(uint16_t(x[j])), h1 = e4m3x2_to_f16x2(uint16_t(x[j] >> 16));
+          const float2 k0 = __half22float2(*reinterpret_cast<const __half2*>(&h0)), k1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+          dot = fmaf(q0.x * up, k0.x, fmaf(q0.y * up, k0.y, fmaf(q1.x * up, k1.x, fmaf(q1.y * up, k1.y, dot))));
+        }
+      }
+    }
+    float s = dot * rs * q8_factor_of(kb);
+    if (vb == 255) s = __int_as_float(0x7fc00000);
+    const bool seen = tok >= lo && tok <= hi;
+    if (!seen) s = -INFINITY;
+    const float top = fmaxf(m, warp_max(s));
+    const float keep = m == top ? 1.f : exp2f(m - top), w = exp2f(s - (top == -INFINITY ? 0.f : top) + kP8Lift);
+    m = top;
+    l = l * keep + w;
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] *= keep;
+    // (NaN goes on; what is not seen may be anything)
+    const float to_o = seen ? w * exp2_int(q8_log2_of(vb) + int(kP8Lift)) : 0.f;
+    if (blk < 0) continue;
+#pragma unroll 4
+    for (int j = 0; j < kQ8Page; ++j) {
+      const float wj = __shfl_sync(kAll, to_o, j);
+      const uint8_t* value = p.v_values + (first + j) * D + lane * N;
+      uint32_t x;
+      if constexpr (N == 4) x = *reinterpret_cast<const uint32_t*>(value);
+      else x = *reinterpret_cast<const uint16_t*>(value);
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        const uint32_t h = e4m3x2_to_f16x2(uint16_t(x >> (8 * i)));
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h));
+        o[i] = wj == 0.f ? o[i] : fmaf(wj, v.x, o[i]);
+        o[i + 1] = wj == 0.f ? o[i + 1] : fmaf(wj, v.y, o[i + 1]);
+      }
+    }
+  }
+  l = warp_sum(l);
+  if (part) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) part[lane * N + i] = o[i];
+    if (lane == 0) {
+      tail[0] = m;
+      tail[2 * kP8Tile] = l;
+    }
+  } else {
+    const float inv = p8_inverse(p, head, m, l);
+    uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + at * D) + lane * (N / 2);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) dst[i / 2] = pack_bf16x2(o[i] * inv, o[i + 1] * inv);
+  }
+}
+
+// The works from `head` on; a warp has 64 of a work's rows.
+template <int D>
+__device__ __forceinline__ void p8_again(const PrefillQ8Params& p, int head, int warp, int lane) {
+  constexpr uint32_t kAll = 0xffffffffu;
+  constexpr long long kPart = 2 * kP8Tile * (D + 2);
+#pragma unroll 1
+  while (head >= 0) {
+    const int id = head >> 1, block = id / p.parts;
+    const bool apart = head & 1;
+    head = *(volatile const int*)(p.again + id);
+    P8Work k;
+    if (!p8_work(p, block / p.nkv % p.batch, block % p.nkv, block / (p.nkv * p.batch) * 2 * kP8Tile, id % p.parts, k)) return;
+    const int t = warp >> 1;
+    const P8Range tr = t == 0 ? k.tr0 : k.tr1;
+    int vis_lo, vis_hi;
+    p8_seen(p, k, vis_lo, vis_hi);
+#pragma unroll 1
+    for (int r0 = (warp & 1) * 64; r0 < (warp & 1) * 64 + 64 && r0 < tr.rows; r0 += 32) {
+      const int r = r0 + lane, row = k.row0 + t * kP8Tile + r, token = row / p.group, q_pos = k.ctx - k.q_len + token;
+      const long long q_row = (long long)k.q_start + token;
+      const int hi = min(p.causal ? min(k.ctx - 1, q_pos) : k.ctx - 1, tr.hi * kP8Tile - 1);
+      const int lo = max(nkb_first_visible(q_pos, p.window, p.chunk), tr.lo * kP8Tile);
+      const bool there = r < tr.rows && q_row >= 0 && q_row < p.total_q && lo <= hi;
+      bool concerned = there && apart;
+      if (!apart) {
+        // the tiles at the ends of what the row sees, and the whole one before its last
+        P8Largest most{0, 0, 0, 0};
+        const int first = __reduce_min_sync(kAll, there ? lo >> 7 : INT_MAX), last = __reduce_max_sync(kAll, there ? hi >> 7 : -1);
+        for (int tile = first; tile <= last; ++tile) {
+          const bool mine = there && (tile == lo >> 7 || tile == hi >> 7 || (tile == (hi >> 7) - 1 && tile >= lo >> 7));
+          if (!__any_sync(kAll, mine)) continue;
+          P8Largest one = most;
+          p8_largest(p, k, tile, vis_lo, vis_hi, lo, hi, one);
+          if (mine) most = one;
+        }
+        concerned = there && (q8_log2_of(most.k_tile) - q8_log2_of(most.k_row) > kP8MoreK || q8_log2_of(most.v_tile) - q8_log2_of(most.v_row) > kP8MoreV);
+      }
+      uint32_t todo = __ballot_sync(kAll, concerned);
+#pragma unroll 1
+      while (todo) {
+        const int j = __ffs(todo) - 1;
+        todo &= todo - 1;
+        const int one = __shfl_sync(kAll, row, j), one_token = one / p.group, one_head = k.kvh * p.group + one % p.group;
+        const long long at = ((long long)k.q_start + one_token) * p.nq + one_head;
+        float *part = nullptr, *tail = nullptr;
+        if (k.part >> 8 > 1) {
+          float* mine = p.partials + ((long long)k.block * p.parts + (k.part & 255)) * kPart;
+          const int in_pair = t * kP8Tile + r0 + j;
+          part = mine + in_pair * D;
+          tail = mine + 2 * kP8Tile * D + in_pair;
+        }
+        p8_row<D>(p, k, at, one_head, __shfl_sync(kAll, lo, j), __shfl_sync(kAll, hi, j), part, tail, lane);
+      }
+    }
+  }
+}
+
 template <int D>
 __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const PrefillQ8Params p) {
   using L = PrefillQ8Smem<D>;
@@ -286,7 +480,9 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
       mbar_init(&ctrl->o_empty[i], 4);
       for (int q = 0; q < 4; ++q) mbar_init(&ctrl->turn[i][q], 1);
     }
+    mbar_init(&ctrl->done, 9);
     ctrl->abort = 0;
+    ctrl->again = -1;
     mbar_fence_init();
     fence_proxy_async();
   }
@@ -391,6 +587,8 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
       item0 += items;
       tiles0 += k.n_union;
     }
+    alive = p8_wait(&ctrl->done, 0, abort_flag, p.status, ERR_WAIT_SOFTMAX);
+    if (__all_sync(kAll, alive) && !*abort_flag) p8_again<D>(p, ctrl->again, warp, lane);
   } else if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 15) {
@@ -479,6 +677,13 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
         };
         int vis_lo, vis_hi;
         p8_seen(p, k, vis_lo, vis_hi);
+        // tokens [all_lo, all_hi) are seen by all rows, whose positions are less than 256 apart
+        const int all_hi = p.causal ? vis_hi - 2 * kP8Tile : vis_hi, all_lo = p.chunk > 0 ? INT_MAX : (p.window > 0 ? vis_lo + 2 * kP8Tile : 0);
+        // for p8_again: largest scales of tiles that all rows see, and of others; this lane's least of the others; V's ends
+        constexpr int kNone = 1000;
+        int in_k = -kNone, in_v = -kNone, at_k = -2 * kNone, at_v = -2 * kNone;
+        uint32_t k_low = 0x00ff00ffu, v_low = 0x00ff00ffu;
+        int v_most = -kNone, v_least = kNone;
         int blk = p8_block(p, k, 0, lane >> 3), blk_n = p8_block(p, k, 1, lane >> 3);
         uint32_t kb = scales_of(p.k_scales, blk), vb = scales_of(p.v_scales, blk);
 #pragma unroll 1
@@ -495,7 +700,7 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
               break;
             }
           }
-          uint32_t k4 = kb, v4 = vb;
+          uint32_t k4 = kb, v4 = vb, k_up = kb, v_up = vb;
           bool all = blk >= 0;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -503,6 +708,8 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
             if (tok >= vis_hi || tok < vis_lo || ((kb >> (8 * j)) & 255) == 255 || ((vb >> (8 * j)) & 255) == 255) {
               k4 &= ~(255u << (8 * j));                   // such a token has no say in the tile's scale
               v4 &= ~(255u << (8 * j));
+              k_up |= 255u << (8 * j);
+              v_up |= 255u << (8 * j);
               all = false;
             }
           }
@@ -520,12 +727,34 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(&ctrl->e_full[slot]);
+          v_most = max(v_most, ev);
+          v_least = min(v_least, ev);
+          if (tile0 >= all_lo && tile0 + kP8Tile <= all_hi) {
+            in_k = max(in_k, ek);
+            in_v = max(in_v, ev);
+          } else {
+            at_k = max(at_k, ek);
+            at_v = max(at_v, ev);
+            k_low = __vminu2(__vminu2(k_low, k_up & 0x00ff00ffu), (k_up >> 8) & 0x00ff00ffu);
+            v_low = __vminu2(__vminu2(v_low, v_up & 0x00ff00ffu), (v_up >> 8) & 0x00ff00ffu);
+          }
           kb = kb_n;
           vb = vb_n;
           blk = blk_n;
           blk_n = blk_2;
         }
+        // (a lane's own least tokens: where there are any so small, some lane has them)
+        const int k_least = q8_log2_of(int(min(k_low & 0xffffu, k_low >> 16))), v_least_at = q8_log2_of(int(min(v_low & 0xffffu, v_low >> 16)));
+        const bool apart = v_most - v_least > kP8Apart;
+        const bool again = apart || at_k > max(in_k, k_least) + kP8MoreK || at_v > max(in_v, v_least_at) + kP8MoreV;
+        if (__any_sync(kAll, again) && lane == 0) {
+          const int id = k.block * p.parts + (k.part & 255);
+          p.again[id] = ctrl->again;
+          ctrl->again = 2 * id + (apart ? 1 : 0);
+        }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctrl->done);
     }
     // ---------------------------------------------------------------- MMA issuers, one per query tile (see attn_prefill.cu)
     constexpr uint32_t idesc_qk = p8_idesc(128, kP8Tile, 0), idesc_pv = p8_idesc(128, D, 1);
@@ -893,6 +1122,8 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
       cur = next;
       have = true;
     }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&ctrl->done);
   }
 
   if (*abort_flag) {
@@ -936,8 +1167,10 @@ __global__ void __launch_bounds__(256) attn_q8_join_kernel(const PrefillQ8Params
     sum = 0.f;
   }
   const float m = warp_max(mine), weight = mine == m ? 1.f : exp2f(mine - m);
+  // (a part of small values counts in the denominator where its weight may be below the least normal number)
+  const float counts = mine - m < -60.f && sum > 0.f ? exp2f(mine - m + log2f(sum)) : sum * weight;
   const uint32_t there = __ballot_sync(0xffffffffu, mine != -INFINITY || sum != 0.f);      // the others had no tile, or saw nothing
-  const float inv = p8_inverse(p, head, m, warp_sum(sum * weight));
+  const float inv = p8_inverse(p, head, m, warp_sum(counts));
   float o[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) o[i] = 0.f;
@@ -993,12 +1226,19 @@ static long long p8_blocks(int batch, int max_q_len, int nq, int nkv) {
   return ((long long)max_q_len * (nq / nkv) + 2 * kP8Tile - 1) / (2 * kP8Tile) * nkv * batch;
 }
 
+static long long p8_again_ints(long long works) { return (works + 3) / 4 * 4; }
+
 // Negative: there is no device.
 extern "C" long long nkb_q8_attn_prefill_scratch_floats(int batch, int max_q_len, int nq, int nkv, int head_dim, int table_width) {
   if (batch <= 0 || nkv < 1 || nq < nkv || max_q_len < 1 || (!status_word() && nkb_init() != 0)) return -1;
   const long long blocks = p8_blocks(batch, max_q_len, nq, nkv);
   const int parts = p8_parts(blocks, table_width);
-  return kQ8Counters + (parts > 1 ? kP8Counts + blocks * parts * 2 * kP8Tile * (head_dim + 2) : 0);
+  return kQ8Counters + p8_again_ints(blocks * parts) + (parts > 1 ? kP8Counts + blocks * parts * 2 * kP8Tile * (head_dim + 2) : 0);
+}
+// 2 where parts of blocks are joined, else 1
+extern "C" int nkb_q8_attn_prefill_launches(int batch, int max_q_len, int nq, int nkv, int table_width) {
+  if (batch <= 0 || nkv < 1 || nq < nkv || max_q_len < 1 || (!status_word() && nkb_init() != 0)) return -1;
+  return p8_parts(p8_blocks(batch, max_q_len, nq, nkv), table_width) > 1 ? 2 : 1;
 }
 
 extern "C" int nkb_q8_attn_prefill(const NkbQ8Attn* arg) {
@@ -1019,8 +1259,9 @@ extern "C" int nkb_q8_attn_prefill(const NkbQ8Attn* arg) {
   if (!g.scratch || blocks * p.parts > 0x3fffffffll) return -2;
   if (g.scratch_floats < nkb_q8_attn_prefill_scratch_floats(g.batch, g.q_len, g.nq, g.nkv, g.head_dim, g.table_width)) return -2;
   p.sched = reinterpret_cast<unsigned int*>(g.scratch);
-  p.counts = reinterpret_cast<int*>(g.scratch + kQ8Counters);
-  p.partials = g.scratch + kQ8Counters + kP8Counts;
+  p.again = reinterpret_cast<int*>(g.scratch + kQ8Counters);
+  p.counts = p.again + p8_again_ints(blocks * p.parts);
+  p.partials = reinterpret_cast<float*>(p.counts + kP8Counts);
   p.batch = g.batch; p.q_blocks = int(blocks / ((long long)g.nkv * g.batch));
   p.total_q = g.total_q; p.nq = g.nq; p.nkv = g.nkv; p.group = g.nq / g.nkv; p.num_blocks = g.num_blocks; p.table_width = g.table_width;
   p.causal = g.causal; p.window = g.window; p.chunk = g.chunk;

@@ -200,6 +200,7 @@ _SIGNATURES = {
     "nkb_q8_attn_decode": (c_int, [c_char_p]),
     "nkb_q8_attn_prefill": (c_int, [c_char_p]),
     "nkb_q8_attn_decode_scratch_floats": (c_longlong, [c_int, c_int, c_int, c_int, c_int]),
+    "nkb_q8_attn_prefill_launches": (c_int, [c_int, c_int, c_int, c_int, c_int]),
     "nkb_q8_attn_prefill_scratch_floats": (c_longlong, [c_int, c_int, c_int, c_int, c_int, c_int]),
     "nkb_decode_advance": (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, c_int, _P]),
     "nkb_packed_positions": (c_int, [_P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, _P]),

@@ -344,6 +344,12 @@ def _prefill_floats(B: int, max_q_len: int, nq: int, nkv: int, D: int, width: in
     return floats
 
 
+@functools.lru_cache(maxsize=4096)
+def _prefill_launches(B: int, max_q_len: int, nq: int, nkv: int, width: int) -> int:
+    """Parts of blocks are joined by a second one."""
+    return _lib.lib().nkb_q8_attn_prefill_launches(B, max_q_len, nq, nkv, width)
+
+
 def _pick_splits(ctas: int, max_pages: int, sms: int = 148) -> int:
     """Parts that decode attention makes of a sequence on average."""
     return 1 if ctas >= sms else max(min(sms // ctas, max(max_pages // 8, 1), 16), 1)
@@ -506,7 +512,7 @@ def flash_attn_prefill(q, k_cache, v_cache, block_table, q_start, q_lens, contex
         width, 1 if causal else 0, window, chunk, 1, scale, 0))
     if rc:
         _lib.check(rc, "nkb_q8_attn_prefill")
-    _count_launch(2 if floats > COUNTERS else 1)        # parts of blocks are joined by a second one
+    _count_launch(_prefill_launches(B, max_q_len, nq, nkv, width))
     return out
 
 

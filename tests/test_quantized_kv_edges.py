@@ -110,6 +110,8 @@ def attend(q, k, v, scale, pos0, causal=True, window=0, chunk=0, sink=None, weig
         seen = seen & (at > pos - window)
     if chunk:
         seen = seen & (at >= pos - pos % chunk)
+    lost_rows = (seen & (k.isnan() | v.isnan()).any(-1)).any(-1)              # tokens that stand for NaN take the rows that see them along
+    k, v = k.nan_to_num(0.0), v.nan_to_num(0.0)
     s = (q @ k.T * scale).masked_fill(~seen, -math.inf)
     top = s.amax(-1, keepdim=True)
     if sink is not None:
@@ -118,10 +120,10 @@ def attend(q, k, v, scale, pos0, causal=True, window=0, chunk=0, sink=None, weig
     p = torch.exp(s - top)
     total = p.sum(-1, keepdim=True) + (0.0 if sink is None else torch.exp(sink - top))
     p = torch.where(total > 0, p / total, 0.0)
-    o = p @ v
+    o = (p @ v).masked_fill(lost_rows[:, None], math.nan)
     moved = 2.0 ** -19 * (q.abs() @ k.abs().T).masked_fill(~seen, 0.0).amax(-1, keepdim=True) * abs(scale)
     largest = v.abs().amax(-1).expand(seen.shape).masked_fill(~seen, 0.0).amax(-1, keepdim=True)
-    return o, 2.0 ** -8 * o.abs() + (p @ v.abs()) * (weights + 2.0 ** -19 + 2 * moved) + seen.sum(-1, keepdim=True) * lost * largest + 1e-30
+    return o, 2.0 ** -8 * o.abs().nan_to_num(0.0) + (p @ v.abs()) * (weights + 2.0 ** -19 + 2 * moved) + seen.sum(-1, keepdim=True) * lost * largest + 1e-30
 
 
 def check_rows(out, q, k, v, spans, scale, group, sinks=None, **masks):
@@ -131,8 +133,10 @@ def check_rows(out, q, k, v, spans, scale, group, sinks=None, **masks):
         for h in range(q.shape[1]):
             want, tol = attend(q[row:row + n, h], k[b][:, h // group].double(), v[b][:, h // group].double(), scale, ctx - n,
                                sink=None if sinks is None else float(sinks[h]), **masks)
-            err = (out[row:row + n, h] - want).abs()
-            assert bool((err <= tol).all()), (b, h, float((err / tol).nan_to_num(math.inf).max()))
+            got = out[row:row + n, h]
+            assert torch.equal(got.isnan(), want.isnan()), (b, h)
+            err = (got - want).abs().nan_to_num(0.0)
+            assert bool((err <= tol).all()), (b, h, float((err / tol).max()))
 
 
 def i32(x, device):
@@ -356,3 +360,115 @@ def test_rows_of_zeros_count_beside_large_values(device, dim, large, places):
     for splits in (1, 4):
         out = ops.paged_attn_decode(q.view(3, -1).to(device), *pages, table.to(device), i32(contexts, device), 0.3, num_splits=splits)
         check_rows(out.view(q.shape), q, *rows_of(pages, table, spans), spans, 0.3, 2)
+
+
+# ------------------------------------------------------------------------------------------------ sizes far apart within a prompt
+# The 128 tokens of a tile are brought to its largest scale, which may be that of a token that a row does not see.  What that may cost a row is
+# 2^-30 of its largest value for a token, as elsewhere, times 2^8 by which the tile's scale may be above what the row sees.
+FAR = 2.0 ** -22
+
+
+FAR_SPANS = [
+    # nq, nkv, spans, masks
+    (4, 2, [(0, 200, 200), (200, 33, 350), (233, 1, 77)], {}),
+    (1, 1, [(0, 300, 700)], dict(window=150)),
+    (2, 1, [(0, 140, 300)], dict(window=50)),
+    (8, 1, [(0, 5, 2100), (5, 3, 1000)], {}),                               # divided among works
+    (16, 4, [(0, 9, 1200)], dict(window=700)),
+    (4, 4, [(70 * i, 70, 70) for i in range(40)], {}),
+    (2, 1, [(0, 150, 300)], dict(chunk=100)),
+    (2, 1, [(0, 40, 300)], dict(causal=False, window=130)),
+]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("sinks", [False, True])
+@pytest.mark.parametrize("nq,nkv,spans,masks", FAR_SPANS)
+def test_prompts_with_sizes_far_apart(device, dim, sinks, nq, nkv, spans, masks):
+    """Values of 2^-40 to 2^40 and keys of 2^-30 to 1 beside one another, some tokens zero."""
+    g = torch.Generator().manual_seed(dim + nq + len(spans))
+    table, blocks = shuffled_table(g, [c for _, _, c in spans])
+    k, v = (ops.QuantizedPages.new(blocks, nkv, dim, device) for _ in range(2))
+    sizes = lambda lo, hi: [2.0 ** torch.randint(lo, hi + 1, (c,), generator=g).double() * (torch.rand((c,), generator=g) > 0.1)       # noqa: E731
+                            for _, _, c in spans]
+    stored_rows(g, k, table, spans, sizes(-30, 0))
+    stored_rows(g, v, table, spans, sizes(-40, 40))
+    q = torch.randn((sum(n for _, n, _ in spans), nq, dim), generator=g).to(torch.bfloat16)
+    s = torch.randn((nq,), generator=g) if sinks else None
+    out = prompt(q, (k, v), table, spans, dim ** -0.5, device, **masks, **({"sinks": s} if sinks else {}))
+    check_rows(out, q, *rows_of((k, v), table, spans), spans, dim ** -0.5, nq // nkv, s, **masks, lost=FAR)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("what", ["keys", "values", "both"])
+@pytest.mark.parametrize("up", [2.0 ** 9, 2.0 ** 30, 2.0 ** 60])
+def test_large_tokens_beside_what_a_row_sees(device, dim, what, up):
+    """Tokens that are far larger than the others: rows ahead of them, and behind the window that shows them, do not notice."""
+    g = torch.Generator().manual_seed(dim)
+    nq, nkv = 4, 2
+    spans, masks = [(0, 290, 290), (290, 100, 600), (390, 1, 129)], dict(window=200)
+    table, blocks = shuffled_table(g, [c for _, _, c in spans])
+    k, v = pool(g, blocks, nkv, dim, device)
+    q = torch.randn((391, nq, dim), generator=g).to(torch.bfloat16)
+    plain = rows_of((k, v), table, spans)
+    want = [[attend(q[r:r + n, h].double(), ks[:, h // 2], vs[:, h // 2], 0.1, c - n, lost=FAR, **masks) for h in range(nq)]
+            for (r, n, c), ks, vs in zip(spans, *plain)]
+    large = [[200, 255, 256], [310, 599], [128]]                             # positions
+    for pages, name in ((k, "keys"), (v, "values")):
+        if what in (name, "both"):
+            scales = pages.scales.view(torch.uint8).cpu()
+            for b, at in enumerate(large):
+                for j in at:
+                    scales[table[b, j // 32], :, j % 32] += int(math.log2(up))
+            pages.scales.view(torch.uint8).copy_(scales.clamp(max=190))
+    out = prompt(q, (k, v), table, spans, 0.1, device, **masks).cpu().double()
+    check = 0
+    for b, (r, n, c) in enumerate(spans):
+        pos = c - n + torch.arange(n)
+        free = torch.ones(n, dtype=torch.bool)
+        for j in large[b]:
+            free &= (pos < j) | (pos >= j + 200)
+        check += int(free.sum())
+        for h in range(nq):
+            o, tol = want[b][h]
+            assert bool(((out[r:r + n, h] - o).abs() <= tol)[free].all()), (b, h)
+    assert check == 289
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("large", LARGE)
+@pytest.mark.parametrize("places", PLACES)
+@pytest.mark.parametrize("new", [[3, 150, 5], [3, 4, 5]])                   # the second: divided among works
+def test_rows_of_zeros_count_beside_large_values_of_prompts(device, dim, large, places, new):
+    g = torch.Generator().manual_seed(dim)
+    pages, table, contexts = zeros_and_large(g, dim, large, places, device)
+    spans = [(sum(new[:b]), n, c) for b, (n, c) in enumerate(zip(new, contexts))]
+    q = torch.randn((sum(new), 2, dim), generator=g).to(torch.bfloat16)
+    check_rows(prompt(q, pages, table, spans, 0.3, device), q, *rows_of(pages, table, spans), spans, 0.3, 2, lost=FAR)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("spans,masks", [([(0, 200, 500), (200, 30, 90), (230, 9, 7)], {}), ([(0, 4, 1500), (4, 5, 700)], dict(window=300))])
+def test_sizes_far_apart_beside_what_is_lost(device, dim, spans, masks):
+    """Tokens that stand for NaN, blocks outside the pool, contexts shorter than the new tokens, rows behind the last sequence."""
+    g = torch.Generator().manual_seed(dim)
+    table, blocks = shuffled_table(g, [c for _, _, c in spans])
+    k, v = (ops.QuantizedPages.new(blocks, 1, dim, device) for _ in range(2))
+    for pages, up in ((k, 20), (v, 40)):
+        stored_rows(g, pages, table, spans, [2.0 ** torch.randint(-up, 1, (c,), generator=g).double() for _, _, c in spans])
+        lost = torch.rand((blocks, 1, 32), generator=g) < 0.004
+        raw = pages.scales.view(torch.uint8).cpu().masked_fill(lost, 255)
+        pages.scales.view(torch.uint8).copy_(raw)
+        values = pages.values.view(torch.uint8).cpu().masked_fill(lost[..., None], 0)
+        pages.values.view(torch.uint8).copy_(values)
+    table[0, 2], table[1, -1] = -1, blocks + 5
+    total = sum(n for _, n, _ in spans)
+    q = torch.randn((total + 2, 2, dim), generator=g).to(torch.bfloat16)
+    out = torch.full((total + 2, 2 * dim), 7.0, dtype=torch.bfloat16, device=device)
+    got = prompt(q, (k, v), table, spans, 0.2, device, out=out, **masks)
+    check_rows(got, q, *rows_of((k, v), table, spans), spans, 0.2, 2, **masks, lost=FAR)
+    assert bool((out[total:] == 7.0).all())
