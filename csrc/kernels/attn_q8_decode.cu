@@ -441,8 +441,9 @@ attn_q8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_cons
     const int head = kvh * p.group + r % p.group;
     if (p.sinks) {
       const float sk = p.sinks[head] * 1.4426950408889634f, m2 = fmaxf(mf, sk), sc = mf == -INFINITY ? 0.f : exp2f(mf - m2);
+      const float add = sk == -INFINITY ? 0.f : exp2f(sk - m2 + kQ8Lift);
       acc.x *= sc; acc.y *= sc; acc.z *= sc; acc.w *= sc;
-      l = l * sc + exp2f(sk - m2 + kQ8Lift);
+      l = l * sc + add;
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     uint2 v;

@@ -197,7 +197,7 @@ __device__ __forceinline__ float p8_inverse(const PrefillQ8Params& p, int head, 
   if (p.sinks) {
     const float sk = p.sinks[head] * 1.4426950408889634f, m2 = fmaxf(m, sk), keep = m == -INFINITY ? 0.f : exp2f(m - m2);
     scale *= keep;
-    l = l * keep + exp2f(sk - m2 + kP8Lift);
+    l = l * keep + (sk == -INFINITY ? 0.f : exp2f(sk - m2 + kP8Lift));      // (no sink, and nothing seen: the sum stays zero)
   }
   return l == 0.f ? 0.f : scale / l;
 }

@@ -105,6 +105,8 @@ def attend(q, k, v, scale, pos0, causal=True, window=0, chunk=0, sink=None, weig
     (f16: 2^-11, bf16: 2^-8), 2^-19 for exponential and sum, and twice what 2^-19 of the largest sum |q k| moves it by; `lost` of the largest
     value that the row sees, for every token that it sees, for weights that end above nothing."""
     pos, at = pos0 + torch.arange(q.shape[0])[:, None], torch.arange(k.shape[0])
+    if not len(k):
+        return torch.zeros_like(q), torch.zeros_like(q)
     seen = at <= pos if causal else torch.ones((q.shape[0], k.shape[0]), dtype=torch.bool)
     if window:
         seen = seen & (at > pos - window)
@@ -472,3 +474,28 @@ def test_sizes_far_apart_beside_what_is_lost(device, dim, spans, masks):
     got = prompt(q, (k, v), table, spans, 0.2, device, out=out, **masks)
     check_rows(got, q, *rows_of((k, v), table, spans), spans, 0.2, 2, **masks, lost=FAR)
     assert bool((out[total:] == 7.0).all())
+
+
+# ------------------------------------------------------------------------------------------------ sinks
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_sinks_of_minus_infinity_are_none(device, dim):
+    """Also where a row sees nothing: its result is zero."""
+    g = torch.Generator().manual_seed(dim)
+    nq, contexts = 4, [40, 0, 700, -1, 3]
+    table, blocks = shuffled_table(g, contexts)
+    pages = pool(g, blocks, 2, dim, device)
+    sinks = torch.tensor([-math.inf, 0.5, -math.inf, torch.finfo(torch.float32).min])
+    q = torch.randn((5, nq, dim), generator=g).to(torch.bfloat16)
+    spans = [(b, 1, max(c, 0)) for b, c in enumerate(contexts)]
+    lens, some = i32(contexts, device), sinks.to(device)
+    for splits in (1, 4):
+        out = ops.paged_attn_decode(q.view(5, -1).to(device), *pages, table.to(device), lens, 0.3, sinks=some, num_splits=splits)
+        check_rows(out.view(q.shape), q, *rows_of(pages, table, spans), spans, 0.3, 2, sinks)
+    spans = [(0, 3, 40), (3, 9, 4), (12, 5, 0), (17, 2, 900)]
+    table, blocks = shuffled_table(g, [c for _, _, c in spans])
+    pages = pool(g, blocks, 2, dim, device)
+    q = torch.randn((19, nq, dim), generator=g).to(torch.bfloat16)
+    for window in (0, 2):
+        out = prompt(q, pages, table, spans, 0.3, device, sinks=sinks, window=window)
+        check_rows(out, q, *rows_of(pages, table, spans), spans, 0.3, 2, sinks, window=window)
