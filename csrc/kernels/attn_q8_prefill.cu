@@ -278,11 +278,11 @@ __device__ __forceinline__ void p8_largest(const PrefillQ8Params& p, const P8Wor
     const int page = tile * 4 + pg;
     if (page * kQ8Page >= k.ctx) break;
     const int blk = p8_page_block(p, k.b, page);
+    if (blk < 0) continue;
     const long long at = ((long long)blk * p.nkv + k.kvh) * kQ8Page;
 #pragma unroll 1
     for (int j = 0; j < kQ8Page; j += 4) {
-      const uint32_t kb = blk >= 0 ? *reinterpret_cast<const uint32_t*>(p.k_scales + at + j) : 0x7f7f7f7fu;
-      const uint32_t vb = blk >= 0 ? *reinterpret_cast<const uint32_t*>(p.v_scales + at + j) : 0x7f7f7f7fu;
+      const uint32_t kb = *reinterpret_cast<const uint32_t*>(p.k_scales + at + j), vb = *reinterpret_cast<const uint32_t*>(p.v_scales + at + j);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int tok = page * kQ8Page + j + i, kx = (kb >> (8 * i)) & 255, vx = (vb >> (8 * i)) & 255;
@@ -673,7 +673,8 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
 #pragma unroll 1
       while (alive && p8_next(ctrl, n_works, k, false, p.status)) {
         auto scales_of = [&](const uint8_t* at, int blk) {
-          return blk >= 0 ? *reinterpret_cast<const uint32_t*>(at + ((long long)blk * p.nkv + k.kvh) * kQ8Page + (lane & 7) * 4) : 0x7f7f7f7fu;
+          // (a page that is not there has no say in the tile's scale)
+          return blk >= 0 ? *reinterpret_cast<const uint32_t*>(at + ((long long)blk * p.nkv + k.kvh) * kQ8Page + (lane & 7) * 4) : 0u;
         };
         int vis_lo, vis_hi;
         p8_seen(p, k, vis_lo, vis_hi);
@@ -700,7 +701,7 @@ __global__ void __launch_bounds__(kP8Threads, 1) attn_q8_prefill_kernel(const Pr
               break;
             }
           }
-          uint32_t k4 = kb, v4 = vb, k_up = kb, v_up = vb;
+          uint32_t k4 = kb, v4 = vb, k_up = blk >= 0 ? kb : 0xffffffffu, v_up = blk >= 0 ? vb : 0xffffffffu;
           bool all = blk >= 0;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {

@@ -499,3 +499,21 @@ def test_sinks_of_minus_infinity_are_none(device, dim):
     for window in (0, 2):
         out = prompt(q, pages, table, spans, 0.3, device, sinks=sinks, window=window)
         check_rows(out, q, *rows_of(pages, table, spans), spans, 0.3, 2, sinks, window=window)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("spans,lost", [([(0, 100, 100), (100, 33, 33)], [1, 0]), ([(0, 5, 1500), (5, 3, 700)], [46, 3])])
+def test_blocks_outside_the_pool_beside_small_rows(device, dim, spans, lost):
+    """Zeros that stand for such a block have no say in the scale of the tile that it is in."""
+    g = torch.Generator().manual_seed(dim)
+    table, blocks = shuffled_table(g, [c for _, _, c in spans])
+    pages = [ops.QuantizedPages.new(blocks, 1, dim, device) for _ in range(2)]
+    for p in pages:
+        stored_rows(g, p, table, spans, [torch.full((c,), 2.0 ** -40, dtype=torch.float64) for _, _, c in spans])
+    table[0, lost[0]], table[1, lost[1]] = -1, blocks + 5
+    q = (torch.randn((sum(n for _, n, _ in spans), 2, dim), generator=g) * 2.0 ** 37).to(torch.bfloat16)
+    check_rows(prompt(q, pages, table, spans, 0.3, device), q, *rows_of(pages, table, spans), spans, 0.3, 2)
+    lens, last = i32([c for _, _, c in spans], device), torch.stack([q[r + n - 1] for r, n, _ in spans])
+    out = ops.paged_attn_decode(last.reshape(2, -1).to(device), *pages, table.to(device), lens, 0.3)
+    check_rows(out.view(last.shape), last, *rows_of(pages, table, spans), [(b, 1, c) for b, (_, _, c) in enumerate(spans)], 0.3, 2)
