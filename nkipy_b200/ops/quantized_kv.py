@@ -504,6 +504,9 @@ def flash_attn_prefill(q, k_cache, v_cache, block_table, q_start, q_lens, contex
                 res[at:at + n] = _ref_attend(qf[at:at + n], k_cache, v_cache, block_table[b], ctx, scale, ctx - n, causal, window, chunk,
                                              sinks)
         return out
+    if abs(out.data_ptr() - q_at) < 2 * q.numel():      # (queries may be read again behind their results)
+        q = q.clone()
+        q_at = q.data_ptr()
     floats = _prefill_floats(B, max_q_len, nq, nkv, D, width)
     scratch = _scratch(k_cache.device, floats)
     rc = _lib.lib().nkb_q8_attn_prefill(_ATTN.pack(

@@ -517,3 +517,26 @@ def test_blocks_outside_the_pool_beside_small_rows(device, dim, spans, lost):
     lens, last = i32([c for _, _, c in spans], device), torch.stack([q[r + n - 1] for r, n, _ in spans])
     out = ops.paged_attn_decode(last.reshape(2, -1).to(device), *pages, table.to(device), lens, 0.3)
     check_rows(out.view(last.shape), last, *rows_of(pages, table, spans), [(b, 1, c) for b, (_, _, c) in enumerate(spans)], 0.3, 2)
+
+
+# ------------------------------------------------------------------------------------------------ results in the place of queries
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("spans,q_len", [([(0, 200, 260), (200, 40, 40)], 0), ([(0, 4, 1500), (4, 4, 700)], 4)])
+def test_results_in_the_place_of_queries(device, spans, q_len):
+    g = torch.Generator().manual_seed(len(spans))
+    nq, nkv, dim = 8, 1, 64
+    table, blocks = shuffled_table(g, [c for _, _, c in spans])
+    k, v = (ops.QuantizedPages.new(blocks, nkv, dim, device) for _ in range(2))
+    stored_rows(g, k, table, spans, [2.0 ** torch.randint(-30, 1, (c,), generator=g).double() for _, _, c in spans])
+    stored_rows(g, v, table, spans, [2.0 ** torch.randint(-40, 41, (c,), generator=g).double() for _, _, c in spans])
+    q = torch.randn((sum(n for _, n, _ in spans), nq, dim), generator=g).to(torch.bfloat16)
+    both = q.reshape(q.shape[0], -1).to(device).clone()
+    want = prompt(q, (k, v), table, spans, 0.125, device)
+    lens = i32([c for _, _, c in spans], device)
+    if q_len:                                                               # decode of more than sixteen rows goes the prompts' way
+        ops.paged_attn_decode(both, k, v, table.to(device), lens, 0.125, q_len=q_len, out=both)
+    else:
+        ops.flash_attn_prefill(both, k, v, table.to(device), *(i32([s[j] for s in spans], device) for j in (0, 1)), lens, 0.125,
+                               max_q_len=max(n for _, n, _ in spans), out=both)
+    assert torch.equal(both.view(q.shape), want)
+    check_rows(both.view(q.shape), q, *rows_of((k, v), table, spans), spans, 0.125, nq, lost=FAR)
