@@ -49,9 +49,10 @@ constexpr int kP8Slots = 8;              // tiles whose scales are kept
 constexpr int kP8Lead = 4;               // tiles that warp 14 is ahead of the conversion of V at most
 constexpr float kP8Grow = 8.f;           // log2 of the growth of a row's maximum that makes O follow
 constexpr float kP8Lift = 6.f;           // log2 of a weight at the maximum, and of a value at the tile's largest scale
-// log2 of what a tile's scales may lie above all that a row sees: keys then keep 2^-23 of the row's largest, and weights, whose exponent V is
-// part of, 2^-22 of the largest contribution
-constexpr int kP8MoreK = 16, kP8MoreV = 8;
+// log2 of what a tile's scales may lie above all that a row sees.  A key's elements are then off by 2^-20 of the row's largest at most (2^-25 of
+// what is 2^6 at scale K; the largest is 224 or more at its own), and weights, whose exponent V is part of, by 2^-18 of the largest contribution
+// (2^-25 of 2^6, by 2^12, and half of that).
+constexpr int kP8MoreK = 18, kP8MoreV = 12;
 constexpr int kP8Apart = 92;             // log2 of V of one tile over that of another: what is below 2^-126 is 2^-34 of the denominator then
 
 struct PrefillQ8Params {
@@ -259,43 +260,55 @@ struct P8Rows {
 // ones f16 has little of them left, and weights below a maximum that V is part of.  So warp 14 marks works where that may be: where a
 // tile that not all rows see has scales far above its smallest and above those of the tiles that all rows see, or where V of the tiles lies so far
 // apart that the denominator may lose a tile.  When a CTA has no more works, the four converting warps look at the rows of those once more
-// and compute those that it concerns by 32-bit products, token by token (some 1000 instructions of a warp per row and page), in the
-// place of the first result.  Nothing of this is in the loop over tiles; what warp 14 notes costs a percent (16 prompts of 1024 220 -> 222 us,
-// 4 x 2000 of 64 columns with a window of 128 68.4 -> 70.1; noted by the converting warps 226 and 70.5).
+// and compute those that it concerns by 32-bit products, token by token (some 2 us of a warp per row and page, most of it latency), in the
+// place of the first result.  Nothing of this is in the loop over tiles; what warp 14 notes costs a percent (16 prompts of 1024 157.3 -> 159.5
+// us, 4 x 2000 of 64 columns with a window of 128 68.4 -> 70.1; noted by the converting warps half as much again).  16 prompts of 1024 with
+// a first value of 2^-10 164 us, with a first key and value of zero 191.
 
 __device__ __forceinline__ int p8_page_block(const PrefillQ8Params& p, int b, int page) {
   const int blk = p.block_table[b * p.table_stride + page];
   return blk >= 0 && blk < p.num_blocks ? blk : -1;
 }
 
-// Largest scales (bytes) of a tile: of what the work sees, and of what this lane's row sees of it, [lo, hi]
+// Largest scales (bytes) of a tile: of what the work sees, and of what this lane's row sees of it, [lo, hi].  Lanes have four tokens each.
 struct P8Largest {
   int k_tile, v_tile, k_row, v_row;
 };
-__device__ __forceinline__ void p8_largest(const PrefillQ8Params& p, const P8Work& k, int tile, int vis_lo, int vis_hi, int lo, int hi, P8Largest& o) {
-#pragma unroll 1
-  for (int pg = 0; pg < 4; ++pg) {
-    const int page = tile * 4 + pg;
-    if (page * kQ8Page >= k.ctx) break;
-    const int blk = p8_page_block(p, k.b, page);
-    if (blk < 0) continue;
-    const long long at = ((long long)blk * p.nkv + k.kvh) * kQ8Page;
-#pragma unroll 1
-    for (int j = 0; j < kQ8Page; j += 4) {
-      const uint32_t kb = *reinterpret_cast<const uint32_t*>(p.k_scales + at + j), vb = *reinterpret_cast<const uint32_t*>(p.v_scales + at + j);
+__device__ __forceinline__ int p8_top_byte(uint32_t pairs) { return int(max(pairs & 0xffffu, pairs >> 16)); }
+__device__ __forceinline__ void p8_largest(const PrefillQ8Params& p, const P8Work& k, int tile, int vis_lo, int vis_hi, int lo, int hi, int lane,
+                                           bool mine, P8Largest& o) {
+  constexpr uint32_t kAll = 0xffffffffu, kEven = 0x00ff00ffu;
+  const int page = tile * 4 + (lane >> 3), tok0 = tile * kP8Tile + lane * 4;
+  const int blk = page * kQ8Page < k.ctx ? p8_page_block(p, k.b, page) : -1;
+  uint32_t kb = 0u, vb = 0u;
+  if (blk >= 0) {
+    const long long at = ((long long)blk * p.nkv + k.kvh) * kQ8Page + (lane & 7) * 4;
+    kb = *reinterpret_cast<const uint32_t*>(p.k_scales + at);
+    vb = *reinterpret_cast<const uint32_t*>(p.v_scales + at);
+  }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int tok = page * kQ8Page + j + i, kx = (kb >> (8 * i)) & 255, vx = (vb >> (8 * i)) & 255;
-        if (tok >= vis_lo && tok < vis_hi && kx != 255 && vx != 255) {
-          o.k_tile = max(o.k_tile, kx);
-          o.v_tile = max(o.v_tile, vx);
-          if (tok >= lo && tok <= hi) {
-            o.k_row = max(o.k_row, kx);
-            o.v_row = max(o.v_row, vx);
-          }
-        }
-      }
+  for (int j = 0; j < 4; ++j) {
+    if (tok0 + j < vis_lo || tok0 + j >= vis_hi || ((kb >> (8 * j)) & 255) == 255 || ((vb >> (8 * j)) & 255) == 255) {
+      kb &= ~(255u << (8 * j));
+      vb &= ~(255u << (8 * j));
     }
+  }
+  const int k_top = __reduce_max_sync(kAll, p8_top_byte(__vmaxu2(kb & kEven, (kb >> 8) & kEven)));
+  const int v_top = __reduce_max_sync(kAll, p8_top_byte(__vmaxu2(vb & kEven, (vb >> 8) & kEven)));
+  uint32_t k_row = 0u, v_row = 0u;
+#pragma unroll 4
+  for (int i = 0; i < 32; ++i) {
+    const int from = min(max(lo - (tile * kP8Tile + 4 * i), 0), 4), end = min(max(hi + 1 - (tile * kP8Tile + 4 * i), 0), 4);
+    const uint32_t seen = end > from ? (0xffffffffu >> (8 * (4 - end + from))) << (8 * from) : 0u;
+    const uint32_t kw = __shfl_sync(kAll, kb, i) & seen, vw = __shfl_sync(kAll, vb, i) & seen;
+    k_row = __vmaxu2(__vmaxu2(k_row, kw & kEven), (kw >> 8) & kEven);
+    v_row = __vmaxu2(__vmaxu2(v_row, vw & kEven), (vw >> 8) & kEven);
+  }
+  if (mine) {
+    o.k_tile = max(o.k_tile, k_top);
+    o.v_tile = max(o.v_tile, v_top);
+    o.k_row = max(o.k_row, p8_top_byte(k_row));
+    o.v_row = max(o.v_row, p8_top_byte(v_row));
   }
 }
 
@@ -316,28 +329,42 @@ __device__ __forceinline__ void p8_row(const PrefillQ8Params& p, const P8Work& k
   float m = -INFINITY, l = 0.f, o[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) o[i] = 0.f;
+  const int last = hi >> 5;
+  int blk_n = p8_page_block(p, k.b, lo >> 5);
+  const auto scale_of = [&](const uint8_t* scales, int blk) {
+    return blk >= 0 ? scales[((long long)blk * p.nkv + k.kvh) * kQ8Page + lane] : 127;
+  };
+  int kb_n = scale_of(p.k_scales, blk_n), vb_n = scale_of(p.v_scales, blk_n);
 #pragma unroll 1
-  for (int page = lo >> 5; page <= hi >> 5; ++page) {
-    const int blk = p8_page_block(p, k.b, page), tok = page * kQ8Page + lane;
+  for (int page = lo >> 5; page <= last; ++page) {
+    const int blk = blk_n, kb = kb_n, vb = vb_n, tok = page * kQ8Page + lane;
     const long long first = ((long long)max(blk, 0) * p.nkv + k.kvh) * kQ8Page;
-    const int kb = blk >= 0 ? p.k_scales[first + lane] : 127, vb = blk >= 0 ? p.v_scales[first + lane] : 127;
+    blk_n = page < last ? p8_page_block(p, k.b, page + 1) : -1;
     float dot = 0.f;
     if (blk >= 0) {
       const uint4* key = reinterpret_cast<const uint4*>(p.k_values + (first + lane) * D);
+      constexpr int kAhead = 4;
 #pragma unroll 1
-      for (int c = 0; c < D / 16; ++c) {
-        const uint4 x4 = key[c];
-        const uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w};
+      for (int c = 0; c < D / 16; c += kAhead) {
+        uint4 x4[kAhead];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint2 q4 = *reinterpret_cast<const uint2*>(q + c * 16 + j * 4);
-          const float2 q0 = unpack_bf16x2(q4.x), q1 = unpack_bf16x2(q4.y);
-          const uint32_t h0 = e4m3x2_to_f16x2(uint16_t(x[j])), h1 = e4m3x2_to_f16x2(uint16_t(x[j] >> 16));
-          const float2 k0 = __half22float2(*reinterpret_cast<const __half2*>(&h0)), k1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-          dot = fmaf(q0.x * up, k0.x, fmaf(q0.y * up, k0.y, fmaf(q1.x * up, k1.x, fmaf(q1.y * up, k1.y, dot))));
+        for (int i = 0; i < kAhead; ++i) x4[i] = key[c + i];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const uint32_t x[4] = {x4[i].x, x4[i].y, x4[i].z, x4[i].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint2 q4 = *reinterpret_cast<const uint2*>(q + (c + i) * 16 + j * 4);
+            const float2 q0 = unpack_bf16x2(q4.x), q1 = unpack_bf16x2(q4.y);
+            const uint32_t h0 = e4m3x2_to_f16x2(uint16_t(x[j])), h1 = e4m3x2_to_f16x2(uint16_t(x[j] >> 16));
+            const float2 k0 = __half22float2(*reinterpret_cast<const __half2*>(&h0)), k1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+            dot = fmaf(q0.x * up, k0.x, fmaf(q0.y * up, k0.y, fmaf(q1.x * up, k1.x, fmaf(q1.y * up, k1.y, dot))));
+          }
         }
       }
     }
+    kb_n = scale_of(p.k_scales, blk_n);
+    vb_n = scale_of(p.v_scales, blk_n);
     float s = dot * rs * q8_factor_of(kb);
     if (vb == 255) s = __int_as_float(0x7fc00000);
     const bool seen = tok >= lo && tok <= hi;
@@ -351,19 +378,26 @@ __device__ __forceinline__ void p8_row(const PrefillQ8Params& p, const P8Work& k
     // (NaN goes on; what is not seen may be anything)
     const float to_o = seen ? w * exp2_int(q8_log2_of(vb) + int(kP8Lift)) : 0.f;
     if (blk < 0) continue;
-#pragma unroll 4
-    for (int j = 0; j < kQ8Page; ++j) {
-      const float wj = __shfl_sync(kAll, to_o, j);
-      const uint8_t* value = p.v_values + (first + j) * D + lane * N;
-      uint32_t x;
-      if constexpr (N == 4) x = *reinterpret_cast<const uint32_t*>(value);
-      else x = *reinterpret_cast<const uint16_t*>(value);
+    const uint8_t* value = p.v_values + first * D + lane * N;
+    constexpr int kRows = 16;
+#pragma unroll 1
+    for (int j0 = 0; j0 < kQ8Page; j0 += kRows) {
+      uint32_t x[kRows];
 #pragma unroll
-      for (int i = 0; i < N; i += 2) {
-        const uint32_t h = e4m3x2_to_f16x2(uint16_t(x >> (8 * i)));
-        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h));
-        o[i] = wj == 0.f ? o[i] : fmaf(wj, v.x, o[i]);
-        o[i + 1] = wj == 0.f ? o[i + 1] : fmaf(wj, v.y, o[i + 1]);
+      for (int j = 0; j < kRows; ++j) {
+        if constexpr (N == 4) x[j] = *reinterpret_cast<const uint32_t*>(value + (j0 + j) * D);
+        else x[j] = *reinterpret_cast<const uint16_t*>(value + (j0 + j) * D);
+      }
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {
+        const float wj = __shfl_sync(kAll, to_o, j0 + j);
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+          const uint32_t h = e4m3x2_to_f16x2(uint16_t(x[j] >> (8 * i)));
+          const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h));
+          o[i] = wj == 0.f ? o[i] : fmaf(wj, v.x, o[i]);
+          o[i + 1] = wj == 0.f ? o[i + 1] : fmaf(wj, v.y, o[i + 1]);
+        }
       }
     }
   }
@@ -383,7 +417,7 @@ __device__ __forceinline__ void p8_row(const PrefillQ8Params& p, const P8Work& k
   }
 }
 
-// The works from `head` on; a warp has 64 of a work's rows.
+// The works from `head` on; a warp has every fourth of a work's rows.
 template <int D>
 __device__ __forceinline__ void p8_again(const PrefillQ8Params& p, int head, int warp, int lane) {
   constexpr uint32_t kAll = 0xffffffffu;
@@ -395,13 +429,12 @@ __device__ __forceinline__ void p8_again(const PrefillQ8Params& p, int head, int
     head = *(volatile const int*)(p.again + id);
     P8Work k;
     if (!p8_work(p, block / p.nkv % p.batch, block % p.nkv, block / (p.nkv * p.batch) * 2 * kP8Tile, id % p.parts, k)) return;
-    const int t = warp >> 1;
-    const P8Range tr = t == 0 ? k.tr0 : k.tr1;
     int vis_lo, vis_hi;
     p8_seen(p, k, vis_lo, vis_hi);
 #pragma unroll 1
-    for (int r0 = (warp & 1) * 64; r0 < (warp & 1) * 64 + 64 && r0 < tr.rows; r0 += 32) {
-      const int r = r0 + lane, row = k.row0 + t * kP8Tile + r, token = row / p.group, q_pos = k.ctx - k.q_len + token;
+    for (int t = 0; t < 2; ++t) {
+      const P8Range tr = t == 0 ? k.tr0 : k.tr1;
+      const int r = lane * 4 + warp, row = k.row0 + t * kP8Tile + r, token = row / p.group, q_pos = k.ctx - k.q_len + token;
       const long long q_row = (long long)k.q_start + token;
       const int hi = min(p.causal ? min(k.ctx - 1, q_pos) : k.ctx - 1, tr.hi * kP8Tile - 1);
       const int lo = max(nkb_first_visible(q_pos, p.window, p.chunk), tr.lo * kP8Tile);
@@ -414,9 +447,7 @@ __device__ __forceinline__ void p8_again(const PrefillQ8Params& p, int head, int
         for (int tile = first; tile <= last; ++tile) {
           const bool mine = there && (tile == lo >> 7 || tile == hi >> 7 || (tile == (hi >> 7) - 1 && tile >= lo >> 7));
           if (!__any_sync(kAll, mine)) continue;
-          P8Largest one = most;
-          p8_largest(p, k, tile, vis_lo, vis_hi, lo, hi, one);
-          if (mine) most = one;
+          p8_largest(p, k, tile, vis_lo, vis_hi, lo, hi, lane, mine, most);
         }
         concerned = there && (q8_log2_of(most.k_tile) - q8_log2_of(most.k_row) > kP8MoreK || q8_log2_of(most.v_tile) - q8_log2_of(most.v_row) > kP8MoreV);
       }
@@ -430,7 +461,7 @@ __device__ __forceinline__ void p8_again(const PrefillQ8Params& p, int head, int
         float *part = nullptr, *tail = nullptr;
         if (k.part >> 8 > 1) {
           float* mine = p.partials + ((long long)k.block * p.parts + (k.part & 255)) * kPart;
-          const int in_pair = t * kP8Tile + r0 + j;
+          const int in_pair = t * kP8Tile + j * 4 + warp;
           part = mine + in_pair * D;
           tail = mine + 2 * kP8Tile * D + in_pair;
         }
