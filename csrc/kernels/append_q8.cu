@@ -5,7 +5,7 @@
 // Keys and values are computed in 64 bits, so that their one rounding to e4m3 does not depend on the order of operations.
 //
 // Measured with 32 heads of 128 on 8: one token from 8 partial sums 3.1 us (latency), 16384 tokens from bf16 76.1 us (58.1 at the copy
-// bandwidth of 6.56 TB/s; 80 for bf16 pages), 390 of 32 heads on 4 with norms 6.2 us (1.2; a chain of latencies, two square roots in it).
+// bandwidth of 6.56 TB/s; 80 for bf16 pages), 390 of 32 heads on 4 with norms 5.2 us (1.2; a chain of latencies, two square roots in it).
 #include "api.h"
 #include "kv_quant.cuh"
 

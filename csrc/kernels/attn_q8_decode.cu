@@ -20,9 +20,9 @@
 // The grid, the page plan and the merge are those of decode attention over bf16 pages (attn_decode.cu); a page is half as large, so
 // an SM holds the rings of twice as many warps.
 //
-// Measured, beside the bytes at the copy bandwidth (6.56 TB/s) and bf16 pages: 32 heads of 128 on 8, 64 sequences of 1024 24.4 us (21.0, 46.0), 7 of
-// 3500 to 7000 23.0 (15.6, 36.7; its CTAs' ends and the merge), one of 203 4.0 (latency); 64 heads of 64 on 8 with two new tokens, 37 of 1000 to
-// 2000 18.6 (9.1, 27.4): sixteen rows, half the bytes per conversion, and issue slots at half use.
+// Measured, beside the bytes at the copy bandwidth (6.56 TB/s) and bf16 pages: 32 heads of 128 on 8, 64 sequences of 1024 24.8 us (21.0, 46.0), 7 of
+// 3500 to 7000 23.4 (15.6, 36.7; its CTAs' ends and the merge), one of 203 4.2 (latency); 64 heads of 64 on 8 with two new tokens, 37 of 1000 to
+// 2000 18.7 (9.1, 27.4): sixteen rows, half the bytes per conversion, and issue slots at half use.
 #include "api.h"
 #include "kv_quant.cuh"
 #include "mma_frag.cuh"

@@ -29,8 +29,8 @@
 // room for them only where the scores are, whose next product then waits for theirs (856 us, where it was 801), or with one place for the scores
 // of both query tiles, which then wait for each other (781 for 741).
 //
-// Measured, beside the MMAs at 1658 TFLOP/s and bf16 pages: 32 heads of 128 on 8, 16 prompts of 1024 157 us (52, 197), 2 of 8000 741 (494, 764),
-// one of 77 10.8 (0.2, 6.8; a fixed part of some 8 us); 64 heads of 64 on 8, 3 portions of up to 500 behind 4000 to 8000 tokens 241 (81, 259).
+// Measured, beside the MMAs at 1658 TFLOP/s and bf16 pages: 32 heads of 128 on 8, 16 prompts of 1024 160 us (52, 195), 2 of 8000 737 (494, 785),
+// one of 77 11.2 (0.2, 6.7; a fixed part of some 8 us); 64 heads of 64 on 8, 3 portions of up to 500 behind 4000 to 8000 tokens 241 (81, 258).
 #include "api.h"
 #include "kv_quant.cuh"
 #include "attn_maps.h"

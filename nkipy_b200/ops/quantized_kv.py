@@ -481,7 +481,8 @@ def rope_attn_decode(qkv_partials, positions, slots, cos_sin, k_cache, v_cache, 
 
 def flash_attn_prefill(q, k_cache, v_cache, block_table, q_start, q_lens, context_lens, scale, *, max_q_len, causal=True, window=0,
                        chunk=0, sinks=None, mods=None, out=None) -> torch.Tensor:
-    """`ops.flash_attn_prefill` over quantised pages.  Rows of q that belong to no sequence are left as they are in `out`."""
+    """`ops.flash_attn_prefill` over quantised pages.  Rows of q that belong to no sequence are left as they are in `out`, which may be q.  What a
+    row does not see costs it no more than 2^-18 of its largest value for a token and 2^-20 of its largest key, whatever its size."""
     blocks, nkv, D = _pair(k_cache, v_cache)
     index = k_cache.index
     B, width, table_step = _check_table(block_table, context_lens, index)
