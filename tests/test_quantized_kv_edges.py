@@ -98,7 +98,7 @@ def test_kernels_refuse_scratch_that_is_too_small(monkeypatch):
 
 
 # ------------------------------------------------------------------------------------------------ attention, all rows of a sequence at once
-def attend(q, k, v, scale, pos0, causal=True, window=0, chunk=0, sink=None, weights=2.0 ** -11, lost=2.0 ** -30):
+def attend(q, k, v, scale, pos0, causal=True, window=0, chunk=0, sink=None, weights=2.0 ** -11, lost=2.0 ** -30, keep_first=0, softcap=0.0):
     """One query head's rows q [n, dim] at positions pos0 on, over k, v [tokens, dim], in 64 bits: (results, tolerances).
 
     As `test_quantized_kv.oracle_attend` has it: 2^-8 of the result for its rounding to bf16; of every weight `weights` for its own rounding
@@ -112,9 +112,12 @@ def attend(q, k, v, scale, pos0, causal=True, window=0, chunk=0, sink=None, weig
         seen = seen & (at > pos - window)
     if chunk:
         seen = seen & (at >= pos - pos % chunk)
+    if keep_first:
+        seen = seen | ((at < keep_first) & (at <= pos))
     lost_rows = (seen & (k.isnan() | v.isnan()).any(-1)).any(-1)              # tokens that stand for NaN take the rows that see them along
     k, v = k.nan_to_num(0.0), v.nan_to_num(0.0)
-    s = (q @ k.T * scale).masked_fill(~seen, -math.inf)
+    s = q @ k.T * scale
+    s = (softcap * torch.tanh(s / softcap) if softcap else s).masked_fill(~seen, -math.inf)
     top = s.amax(-1, keepdim=True)
     if sink is not None:
         top = top.clamp(min=sink)
@@ -543,3 +546,21 @@ def test_results_in_the_place_of_queries(device, spans, q_len):
                                max_q_len=max(n for _, n, _ in spans), out=both)
     assert torch.equal(both.view(q.shape), want)
     check_rows(both.view(q.shape), q, *rows_of((k, v), table, spans), spans, 0.125, nq, lost=FAR)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("spans,masks,mods", [
+    ([(0, 700, 900)], dict(chunk=512), dict(softcap=20.0)), ([(0, 900, 900), (900, 200, 1300)], dict(chunk=700), dict(softcap=20.0)),
+    ([(0, 600, 1100)], dict(window=300), dict(softcap=20.0, keep_first=70)), ([(0, 400, 900)], dict(window=64), dict(keep_first=130)),
+    ([(0, 500, 500)], dict(window=128), dict(softcap=20.0))])
+def test_modified_scores_over_16_bit_pages_with_masks_that_part_query_tiles(device, dim, spans, masks, mods):
+    """Capped scores and kept first tokens take turns by key tiles of 64, the kept ones ahead (see test_query_turns.py)."""
+    g = torch.Generator().manual_seed(dim)
+    table, blocks = shuffled_table(g, [c for _, _, c in spans])
+    pages = [torch.randn((blocks, 1, 32, dim), generator=g).to(torch.bfloat16) for _ in range(2)]
+    k, v = ([p[table[b, :-(-c // 32)].long()].transpose(1, 2).reshape(-1, 1, dim)[:c] for b, (_, _, c) in enumerate(spans)] for p in pages)
+    q = torch.randn((sum(n for _, n, _ in spans), 2, dim), generator=g).to(torch.bfloat16)
+    out = prompt(q, [p.to(device) for p in pages], table, spans, dim ** -0.5, device, mods=ops.ScoreMods(**mods), **masks)
+    # (a capped score comes from a polynomial or an exponential of the special-function unit: 2^-19 of the cap, as weights have it)
+    check_rows(out, q, k, v, spans, dim ** -0.5, 2, weights=2.0 ** -8 + 2.0 ** -19 * mods.get("softcap", 0.0), **masks, **mods)
