@@ -4,8 +4,8 @@
 //
 // Keys and values are computed in 64 bits, so that their one rounding to e4m3 does not depend on the order of operations.
 //
-// Measured with 32 heads of 128 on 8: one token from 8 partial sums 3.1 us (latency), 16384 tokens from bf16 76.1 us (58.1 at the copy
-// bandwidth of 6.56 TB/s; 80 for bf16 pages), 390 of 32 heads on 4 with norms 5.2 us (1.2; a chain of latencies, two square roots in it).
+// Measured with 32 heads of 128 on 8: one token from 8 partial sums 3.1 us (latency), 16384 tokens from bf16 77.3 us (58.1 at the copy
+// bandwidth of 6.56 TB/s; 80 for bf16 pages), 390 of 32 heads on 4 with norms 5.4 us (1.2; a chain of latencies, two square roots in it).
 #include "api.h"
 #include "kv_quant.cuh"
 
@@ -256,7 +256,15 @@ __global__ void __launch_bounds__(256, PARTIALS ? 2 : 3) append8_q8_kernel(const
         for (int j = 0; j < 16; ++j) ss += x[j] * x[j];
 #pragma unroll
         for (int m = L / 2; m > 0; m >>= 1) ss += __shfl_xor_sync(mine, ss, m);
-        const float f = 1.f / sqrtf(ss / float(D) + float(p.eps));
+        float f = 1.f / sqrtf(ss / float(D) + float(p.eps));
+        if (!(ss > 1e-30f && ss <= 1e38f)) {       // squares beyond 32 bits (a head's lanes agree)
+          double wide = 0.;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) wide += double(x[j]) * double(x[j]);
+#pragma unroll
+          for (int m = L / 2; m > 0; m >>= 1) wide += __shfl_xor_sync(mine, wide, m);
+          f = float(1. / sqrt(wide / double(D) + p.eps));
+        }
 #pragma unroll
         for (int j = 0; j < 16; ++j) x[j] = x[j] * f * w[j];
       }

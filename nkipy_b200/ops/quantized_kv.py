@@ -120,7 +120,7 @@ def _ref_append(qkv, positions, slots, cos_sin, k_pages, v_pages, nq, nkv, dim, 
             t = torch.cat([t[..., :h] * cs[..., :h] - t[..., h:] * cs[..., h:], t[..., h:] * cs[..., :h] + t[..., :h] * cs[..., h:]], -1)
         return t
 
-    q_out.copy_(turn(x[:, :nq].float(), q_norm_w).reshape(q_out.shape))
+    q_out.copy_(turn(x[:, :nq], q_norm_w).reshape(q_out.shape))
     if slots is not None:
         at = slots.long()
         on = (at >= 0) & (at < k_pages.shape[0] * PAGE)

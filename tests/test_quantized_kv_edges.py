@@ -10,7 +10,7 @@ import torch
 from nkipy_b200 import ops
 from nkipy_b200.ops import _lib
 from nkipy_b200.ops import quantized_kv as Q
-from tests.test_quantized_kv import DEVICES, cached, fill, pool, shuffled_table
+from tests.test_quantized_kv import DEVICES, cached, fill, oracle_quantize, oracle_turn, pool, rope_table, shuffled_table, stored
 
 
 # ------------------------------------------------------------------------------------------------ scratch
@@ -564,3 +564,28 @@ def test_modified_scores_over_16_bit_pages_with_masks_that_part_query_tiles(devi
     out = prompt(q, [p.to(device) for p in pages], table, spans, dim ** -0.5, device, mods=ops.ScoreMods(**mods), **masks)
     # (a capped score comes from a polynomial or an exponential of the special-function unit: 2^-19 of the cap, as weights have it)
     check_rows(out, q, k, v, spans, dim ** -0.5, 2, weights=2.0 ** -8 + 2.0 ** -19 * mods.get("softcap", 0.0), **masks, **mods)
+
+
+# ------------------------------------------------------------------------------------------------ norms of rows of any size
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("T,splits", [(3, 0), (3, 2), (70, 0), (200, 0), (200, 3)])
+@pytest.mark.parametrize("eps", [1e-6, 1e-60])
+def test_norms_of_rows_whose_squares_leave_32_bits(device, dim, T, splits, eps):
+    """Queries and keys of 1e-25 to 1e25, however many tokens a call has."""
+    g = torch.Generator().manual_seed(dim + T)
+    nq, nkv, size = 3, 1, 10.0 ** torch.tensor([-25.0, 0.0, 18.0, 25.0])
+    x = torch.randn((T, nq + 2 * nkv, dim), generator=g) * size[torch.randint(0, 4, (T, nq + 2 * nkv, 1), generator=g)]
+    x = torch.stack([x * 0.25 for _ in range(splits)]) if splits else x.to(torch.bfloat16)
+    w = [(1 + 0.3 * torch.randn((dim,), generator=g)).to(torch.bfloat16) for _ in range(2)]
+    cs, pos = rope_table(dim, 300), torch.arange(T, dtype=torch.int32)
+    k, v = (ops.QuantizedPages.new(-(-T // 32), nkv, dim, device) for _ in range(2))
+    q = ops.rope_kv_append(x.reshape(*x.shape[:-2], -1).to(device), pos.to(device), pos.to(device), cs.to(device), k, v, nq, nkv, dim,
+                           q_norm_w=w[0].to(device), k_norm_w=w[1].to(device), norm_eps=eps).cpu().double().view(T, nq, dim)
+    y = x.double().sum(0) if splits else x.double()
+    want = oracle_turn(y[:, :nq], cs[:T], w[0], eps)
+    # rounded to bf16; a dozen roundings of 32 bits of at most twice the head's largest
+    assert bool(((q - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -18 * want.abs().amax(-1, keepdim=True)).all())
+    values, scales = oracle_quantize(oracle_turn(y[:, nq:nq + nkv], cs[:T], w[1], eps))
+    got, s = stored(k)
+    assert torch.equal(got[pos.long() // 32, :, pos.long() % 32], values) and torch.equal(s[pos.long() // 32, :, pos.long() % 32], scales)
