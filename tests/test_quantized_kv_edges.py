@@ -589,3 +589,33 @@ def test_norms_of_rows_whose_squares_leave_32_bits(device, dim, T, splits, eps):
     values, scales = oracle_quantize(oracle_turn(y[:, nq:nq + nkv], cs[:T], w[1], eps))
     got, s = stored(k)
     assert torch.equal(got[pos.long() // 32, :, pos.long() % 32], values) and torch.equal(s[pos.long() // 32, :, pos.long() % 32], scales)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("spans", [[(0, 150, 250), (150, 90, 90)], [(0, 4, 1500), (4, 5, 700)]])
+def test_rows_computed_once_more_beside_other_calls(spans):
+    """Captured, replayed beside eager calls on another stream, and after other prompts: the same bits."""
+    g = torch.Generator().manual_seed(7)
+    table, blocks = shuffled_table(g, [c for _, _, c in spans])
+    works = []
+    for _ in range(2):
+        k, v = (ops.QuantizedPages.new(blocks, 2, 128, "cuda") for _ in range(2))
+        stored_rows(g, k, table, spans, [2.0 ** torch.randint(-30, 1, (c,), generator=g).double() for _, _, c in spans])
+        stored_rows(g, v, table, spans, [2.0 ** torch.randint(-40, 41, (c,), generator=g).double() for _, _, c in spans])
+        q = torch.randn((sum(n for _, n, _ in spans), 4 * 128), generator=g).to(torch.bfloat16).cuda()
+        at = [i32([s[j] for s in spans], "cuda") for j in (0, 1, 2)]
+        works.append(lambda q=q, k=k, v=v, t=table.cuda(), at=at: ops.flash_attn_prefill(q, k, v, t, *at, 0.1, max_q_len=max(s[1] for s in spans)))
+    want = [w().clone() for w in works]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = works[0]()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(10):
+        with torch.cuda.stream(streams[0]):
+            graph.replay()
+            got[0].append(out.clone())
+        with torch.cuda.stream(streams[1]):
+            got[1].append(works[1]().clone())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, w) for outs, w in zip(got, want) for a in outs)
