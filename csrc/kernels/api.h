@@ -7,11 +7,13 @@
 #include <stdint.h>
 #include "attn_maps.h"
 #include "head_recurrence.h"
+#include "i8_args.h"
 #include "latent_attn.h"
 #include "linear_attn.h"
 #include "post_residual.h"
 #include "proj_src.h"
 #include "q8_args.h"
+#include "rules_args.h"
 
 namespace nkb {
 int encode_tmap_bf16_2d(CUtensorMap* m, const void* ptr, uint64_t inner, uint64_t outer, uint64_t ld_elems,
@@ -77,6 +79,11 @@ int nkb_gemm_bf16(const void* A, const void* B, void* out, int rows, int cols, i
                   long long ldo, int transpose_out, int out_fp32, int splits, long long split_stride, int gated,
                   int gate_off, const void* bias, int bias_on_rows, const void* residual, int block_n, int max_ctas,
                   int weights_operand, int ctas_per_sm, int act, float act_a, float act_b, void* stream);
+// rows and weights in 8-bit whole numbers, rules on logits: packed arguments of i8_args.h and rules_args.h
+int nkb_quant_rows(const void* args);
+int nkb_gemm_i8(const void* args);
+int nkb_gemm_i8_splits(int k, int splits);
+int nkb_logit_rules(const void* args);
 int nkb_gemm_effective_splits(int k, int splits);
 int nkb_query_turn(int t, int lo0, int hi0, int lo1, int hi1, int tile);   // query_turns.h, on the host
 int nkb_query_turns_from_first(int lo0, int hi0, int lo1, int hi1);

@@ -37,6 +37,7 @@ __all__ = [
     "Decay", "linear_attention", "low_rank", "token_mix",
     "Act", "ScoreMods", "HeadRecurrence", "ShortConv", "head_recurrence", "gated_group_norm", "short_conv",
     "QuantizedPages",
+    "QuantizedRows", "QuantizedWeight", "quantize_rows", "LogitRules", "apply_rules", "pack_mask",
     "KernelLibraryError", "device_status", "raise_on_device_error", "native_available", "launch_count",
     "reset_launch_count",
 ]
@@ -206,7 +207,13 @@ def linear(
     weights_static: w is not written by the kernels launched just before this one, so its
            tiles may be fetched before the preceding kernel has finished (set False when w is
            itself a fresh activation).  Whole products of 512 rows or more on CTA pairs wait in any case.
+
+    A `QuantizedWeight` in the place of w: a product in 8 bits, of `QuantizedRows` or of rows that it brings into 8 bits (without
+    out_act; swap, max_ctas and ctas_per_sm choose among bf16 kernels only).
     """
+    if type(w) is QuantizedWeight or type(x) is QuantizedRows:
+        return quantized_linear.linear(x, w, bias=bias, residual=residual, out=out, splits=splits, gated=gated, weights_static=weights_static,
+                                       act=act, fp32_out=fp32_out, out_act=out_act)
     M, K = x.shape
     N = w.shape[0] // 2 if gated else w.shape[0]
     if w.shape[1] != K:
@@ -461,8 +468,13 @@ def reduce_partials(partials: torch.Tensor, residual: Optional[torch.Tensor] = N
 
 
 # --------------------------------------------------------------------------- norms
-def rmsnorm(x: torch.Tensor, w: torch.Tensor, eps: float, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Row-wise RMSNorm with fp32 statistics; x [..., H] bf16."""
+def rmsnorm(x: torch.Tensor, w: torch.Tensor, eps: float, out: Optional[torch.Tensor] = None,
+            quantize: bool = False) -> Union[torch.Tensor, "QuantizedRows"]:
+    """Row-wise RMSNorm with fp32 statistics; x [..., H] bf16.  quantize: `QuantizedRows` [rows, H] in the place of bf16 ones."""
+    if quantize:
+        if out is not None:
+            raise ValueError("quantised rows take no out")
+        return quantized_linear.add_rmsnorm(x, w, eps=eps)[1]
     H = x.shape[-1]
     rows = x.numel() // H
     if out is None:
@@ -492,10 +504,16 @@ def add_rmsnorm(
     eps: float = 1e-6,
     hidden: Optional[int] = None,
     rows: Optional[int] = None,
-) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+    quantize: bool = False,
+) -> Tuple[Optional[torch.Tensor], Union[torch.Tensor, "QuantizedRows", None]]:
     """Fused ``h = sum(partials) + x + bias + residual_in``; ``residual_out = h``;
     ``normed_out = rmsnorm(h) * w``.  Any of x / partials / bias / residual_in may
-    be None; w None skips the norm.  Returns (residual_out, normed_out)."""
+    be None; w None skips the norm.  Returns (residual_out, normed_out); quantize: `QuantizedRows` in the place of normed_out."""
+    if quantize:
+        if normed_out is not None:
+            raise ValueError("quantised rows take no normed_out")
+        return quantized_linear.add_rmsnorm(x, w, residual_in=residual_in, partials=partials, bias=bias, residual_out=residual_out, eps=eps,
+                                            hidden=hidden, rows=rows)
     ref = x if x is not None else partials
     if hidden is None:
         hidden = ref.shape[-1]
@@ -570,9 +588,13 @@ def _silu_mul_partials(parts, out, limit, alpha, bias):
 
 
 def silu_mul(gate_up: torch.Tensor, out: Optional[torch.Tensor] = None, limit: float = 0.0,
-             alpha: float = 1.702, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+             alpha: float = 1.702, bias: Optional[torch.Tensor] = None, quantize: bool = False) -> Union[torch.Tensor, "QuantizedRows"]:
     """SwiGLU gate over ``[T, 2I]`` (gate | up) -> ``[T, I]``; limit > 0 selects the
-    clamped gpt-oss form ``(up + 1) * gate * sigmoid(alpha * gate)``."""
+    clamped gpt-oss form ``(up + 1) * gate * sigmoid(alpha * gate)``.  quantize: `QuantizedRows` in the place of bf16 ones."""
+    if quantize:
+        if out is not None:
+            raise ValueError("quantised rows take no out")
+        return quantized_linear.silu_mul(gate_up, limit, alpha, bias)
     if gate_up.dtype == torch.float32:
         return _silu_mul_partials(gate_up, out, limit, alpha, bias)
     T, two_i = gate_up.shape
@@ -766,8 +788,13 @@ def packed_positions(q_start: torch.Tensor, q_lens: torch.Tensor, context_lens: 
 
 # --------------------------------------------------------------------------- sampling / routing
 def argmax(logits: torch.Tensor, out_ids: Optional[torch.Tensor] = None,
-           out_vals: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Row-wise argmax (first occurrence) of bf16/fp32 ``[B, V]`` logits -> int32 ids."""
+           out_vals: Optional[torch.Tensor] = None, rules: Optional["LogitRules"] = None) -> torch.Tensor:
+    """Row-wise argmax (first occurrence) of bf16/fp32 ``[B, V]`` logits -> int32 ids.  rules: of what they leave of the logits, -1 where
+    that is nothing (without out_vals)."""
+    if rules is not None:
+        if out_vals is not None:
+            raise ValueError("argmax under rules has no out_vals")
+        return logit_rules.argmax(logits, rules, out_ids)
     B, V = logits.shape
     if out_ids is None:
         out_ids = torch.empty((B,), dtype=torch.int32, device=logits.device)
@@ -1461,6 +1488,10 @@ from .latent_attention import (LatentSpec, latent_append, latent_attention, late
 from .linear_attention import Decay, linear_attention, low_rank, token_mix  # noqa: E402,F401
 from . import quantized_kv  # noqa: E402
 from .quantized_kv import QuantizedPages  # noqa: E402
+from . import quantized_linear  # noqa: E402
+from .quantized_linear import QuantizedRows, QuantizedWeight, quantize_rows  # noqa: E402
+from . import logit_rules  # noqa: E402
+from .logit_rules import LogitRules, apply_rules, pack_mask  # noqa: E402
 from .head_recurrence import (HeadRecurrence, ShortConv, gated_group_norm, head_recurrence,  # noqa: E402,F401
                               short_conv)
 

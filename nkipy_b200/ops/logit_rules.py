@@ -1,0 +1,197 @@
+"""Rules on logits ahead of the choice of a token: penalties for repeated tokens, biases and masks.
+
+They are reached through `apply_rules`, which gives the logits that are left, and `argmax` with rules, which chooses the most likely token
+without writing them.  A row's tokens are its state: the list of ids that a scheduler keeps anyway, into which a call writes the
+newest.  No file of the reference corresponds to these (it decodes greedily, examples/models/qwen3/kernels/sampling.py:113-147).
+"""
+
+from __future__ import annotations
+
+import struct
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import _lib
+from . import _count_launch, _stream
+from .quantized_linear import _on_gpu
+
+_ARGS = struct.Struct("15P5q6i")          # NkbLogitRules of csrc/kernels/rules_args.h
+
+
+@dataclass
+class LogitRules:
+    """What is done to the logits [rows, vocab] of a step, in 64 bits and rounded once, in this order:
+
+    tokens int32 [rows, width], lens int32 [rows]: the ids of every row so far, the newest included (lens beyond the width count as the
+        width; a length below one: no tokens).  ids int32 [rows]: the newest, which the call writes to tokens[b, lens[b] - 1]; None: it
+        is there already.  prompt_lens int32 [rows]: how many of them are the prompt's; None: none.  Ids outside the vocabulary count for
+        nothing.
+    repetition fp32 [rows], above zero: a token that is among the row's is divided by it where its logit is above zero, and multiplied
+        elsewhere.
+    frequency, presence fp32 [rows]: taken off a token that is among the answer's, as often as it is there, and once.
+    bias_ids int32 [rows, n], bias_values fp32 [rows, n]: added to single tokens; several for one token add up.  Negative ids: none.
+    mask int32 [masks, words]: bit t % 32 of word t // 32 says whether token t may come (zero: its logit becomes minus infinity).
+        mask_rows int32 [rows]: a row's mask, outside of them: none; None: row b has mask b.
+
+    All on the logits' device.  Rows of the matrices may lie apart; the vectors are contiguous."""
+    tokens: Optional[torch.Tensor] = None
+    lens: Optional[torch.Tensor] = None
+    prompt_lens: Optional[torch.Tensor] = None
+    ids: Optional[torch.Tensor] = None
+    repetition: Optional[torch.Tensor] = None
+    frequency: Optional[torch.Tensor] = None
+    presence: Optional[torch.Tensor] = None
+    bias_ids: Optional[torch.Tensor] = None
+    bias_values: Optional[torch.Tensor] = None
+    mask: Optional[torch.Tensor] = None
+    mask_rows: Optional[torch.Tensor] = None
+
+
+def mask_words(vocab: int) -> int:
+    """Words of a mask."""
+    return -(-vocab // 32)
+
+
+def pack_mask(allowed: torch.Tensor) -> torch.Tensor:
+    """bool [masks, vocab] (or [vocab]) as the words of `LogitRules.mask`."""
+    vocab = allowed.shape[-1]
+    bits = torch.zeros((*allowed.shape[:-1], mask_words(vocab) * 32), dtype=torch.int64, device=allowed.device)
+    bits[..., :vocab] = allowed
+    words = (bits.unflatten(-1, (-1, 32)) << torch.arange(32, device=allowed.device)).sum(-1)
+    return torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32)
+
+
+def _vector(t, name, dtype, rows, index):
+    if t is None:
+        return 0
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} wants {dtype}, not {t.dtype}")
+    if t.shape != (rows,) or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name} wants to be contiguous [{rows}], on the logits' device")
+    return t.data_ptr()
+
+
+def _matrix(t, name, dtype, rows, index):
+    """(address, elements from one row to the next); rows None: any number."""
+    if t is None:
+        return 0, 0
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} wants {dtype}, not {t.dtype}")
+    if t.dim() != 2 or (rows is not None and t.shape[0] != rows) or t.get_device() != index or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name} wants rows of neighbouring numbers, one for each of the logits', on their device")
+    return t.data_ptr(), t.stride(0)
+
+
+def _packed(logits, rules: LogitRules, out, out_ids) -> bytes:
+    if not isinstance(rules, LogitRules):
+        raise TypeError("rules are LogitRules")
+    if logits.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"rules want bf16 or fp32 logits, not {logits.dtype}")
+    if logits.dim() != 2 or logits.shape[1] < 1 or logits.shape[0] > 65535 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("rules want logits [rows, vocab], of 65535 rows at most, with neighbouring columns")
+    B, V = logits.shape
+    index = logits.get_device()
+    out_at, out_ld = _matrix(out, "out", logits.dtype, B, index)
+    if out is not None and (out.shape != logits.shape or (B > 1 and out_ld < V)):
+        raise ValueError("out wants the logits' shape")
+    if out is not None and out_at == logits.data_ptr() and B > 1 and out_ld != logits.stride(0):
+        raise ValueError("rows of out that lie over the logits want to be the same ones")
+    r, i32, f32 = rules, torch.int32, torch.float32
+    tokens, tokens_ld = _matrix(r.tokens, "tokens", i32, B, index)
+    if r.tokens is None:
+        if r.lens is not None or r.ids is not None or r.prompt_lens is not None:
+            raise ValueError("lens, prompt_lens and ids belong to tokens")
+        if r.repetition is not None or r.frequency is not None or r.presence is not None:
+            raise ValueError("penalties want the rows' tokens")
+    elif r.lens is None:
+        raise ValueError("tokens want lens")
+    if (r.bias_ids is None) != (r.bias_values is None):
+        raise ValueError("biases want ids and values")
+    bias_ids, bias_ld = _matrix(r.bias_ids, "bias_ids", i32, B, index)
+    bias_values, values_ld = _matrix(r.bias_values, "bias_values", f32, B, index)
+    if r.bias_ids is not None and (r.bias_ids.shape != r.bias_values.shape or (B > 1 and bias_ld != values_ld)):
+        raise ValueError("biases want as many values as ids, laid out the same")
+    mask, mask_ld = _matrix(r.mask, "mask", i32, None if r.mask_rows is not None else B, index)
+    if r.mask is not None and r.mask.shape[1] < mask_words(V):
+        raise ValueError(f"mask wants {mask_words(V)} words for a vocabulary of {V}")
+    if r.mask is None and r.mask_rows is not None:
+        raise ValueError("mask_rows belong to masks")
+    return _ARGS.pack(
+        logits.data_ptr(), out_at, _vector(out_ids, "out_ids", i32, B, index), tokens, _vector(r.lens, "lens", i32, B, index),
+        _vector(r.prompt_lens, "prompt_lens", i32, B, index), _vector(r.ids, "ids", i32, B, index),
+        _vector(r.repetition, "repetition", f32, B, index), _vector(r.frequency, "frequency", f32, B, index),
+        _vector(r.presence, "presence", f32, B, index), bias_ids, bias_values, mask, _vector(r.mask_rows, "mask_rows", i32, B, index),
+        _stream() if index >= 0 else 0, logits.stride(0), out_ld, tokens_ld, bias_ld, mask_ld, B, V, r.tokens.shape[1] if tokens else 0,
+        r.bias_ids.shape[1] if bias_ids else 0, r.mask.shape[0] if mask else 0, logits.dtype is torch.float32)
+
+
+def _reference(logits, r: LogitRules) -> torch.Tensor:
+    """fp32 logits under the rules; writes the newest tokens."""
+    y = logits.double().clone()
+    B, V = y.shape
+    for b in range(B):
+        row = y[b]
+        if r.tokens is not None:
+            n = min(int(r.lens[b]), r.tokens.shape[1])
+            if n > 0:
+                if r.ids is not None:
+                    r.tokens[b, n - 1] = r.ids[b]
+                ids = r.tokens[b, :n].long()
+                inside = (ids >= 0) & (ids < V)
+                seen = torch.bincount(ids[inside], minlength=V) > 0
+                answer = torch.arange(n) >= (int(r.prompt_lens[b]) if r.prompt_lens is not None else 0)
+                times = torch.bincount(ids[inside & answer], minlength=V).double()
+                rep, freq, pres = (d if t is None else float(t[b]) for t, d in ((r.repetition, 1.0), (r.frequency, 0.0), (r.presence, 0.0)))
+                hit = row[seen]
+                hit = torch.where(hit > 0, hit / rep, hit * rep) - freq * times[seen]
+                row[seen] = torch.where(times[seen] > 0, hit - pres, hit)
+        if r.bias_ids is not None:
+            total = {}
+            for t, v in zip(r.bias_ids[b].tolist(), r.bias_values[b].double().tolist()):
+                if 0 <= t < V:
+                    total[t] = total.get(t, 0.0) + v
+            for t, v in total.items():
+                row[t] += v
+        m = -1 if r.mask is None else (b if r.mask_rows is None else int(r.mask_rows[b]))
+        if r.mask is not None and 0 <= m < r.mask.shape[0]:
+            t = torch.arange(V)
+            row[((r.mask[m][t // 32] >> (t % 32)) & 1) == 0] = float("-inf")
+    return y.float()
+
+
+def apply_rules(logits: torch.Tensor, rules: LogitRules, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The logits [rows, vocab] (bf16 or fp32) under the rules, in their type.  out: where they go; the logits themselves, whose
+    untouched pieces are not even read then, or apart from them."""
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    args = _packed(logits, rules, out, None)
+    if not logits.shape[0]:
+        return out
+    if not _on_gpu(logits.get_device()):
+        return out.copy_(_reference(logits, rules))
+    rc = _lib.lib().nkb_logit_rules(args)
+    if rc:
+        _lib.check(rc, "nkb_logit_rules")
+    _count_launch()
+    return out
+
+
+def argmax(logits: torch.Tensor, rules: LogitRules, out_ids: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """int32 [rows]: the first of the largest values that the rules leave, as 32 bits hold them; -1 where none is above minus infinity."""
+    if out_ids is None:
+        out_ids = torch.empty((logits.shape[0],), dtype=torch.int32, device=logits.device)
+    args = _packed(logits, rules, None, out_ids)
+    if not logits.shape[0]:
+        return out_ids
+    if not _on_gpu(logits.get_device()):
+        y = _reference(logits, rules).nan_to_num(nan=float("-inf"), posinf=float("inf"), neginf=float("-inf"))
+        top, at = y.max(-1)
+        first = torch.where(y == top[:, None], torch.arange(y.shape[1]), y.shape[1]).amin(-1)
+        return out_ids.copy_(torch.where(top == float("-inf"), -1, first))
+    rc = _lib.lib().nkb_logit_rules(args)
+    if rc:
+        _lib.check(rc, "nkb_logit_rules")
+    _count_launch()
+    return out_ids

@@ -1,0 +1,341 @@
+"""Products of rows and weights in 8-bit whole numbers.
+
+A row x, of activations or of a weight, is held as ``q``, the whole numbers nearest to ``127 x / max|x|`` (ties to the even one), and one
+factor ``scale = max|x| / 127``: x is about ``q * scale``, off by half a scale at most.  A row with a value that is not finite has the
+scale NaN and zeros, a row of zeros the scale 0.
+
+A factor for every token and every output channel, because both leave the sum over k: ``y = (sum_k q_x q_w) * scale_x * scale_w``, whose
+sum is exact.  The numbers of a row are decided exactly too (quant_rows.cu), so a row has the same numbers whichever kernel, or the
+reference on the CPU, made them.  Behind a norm they come from the products h * w of the residual stream and the norm's weights, which
+are exact; the norm's factor is one for the row and goes into its scale.
+
+    QuantizedRows     rows of activations: `quantize_rows`, or `rmsnorm`, `add_rmsnorm` and `silu_mul` with quantize=True
+    QuantizedWeight   a weight, which `linear` takes in the place of a bf16 one
+
+No file of the reference corresponds to these (its products are bf16, examples/models/qwen3/kernels/transformer_layer.py:16-120).
+"""
+
+from __future__ import annotations
+
+import struct
+from typing import Optional
+
+import torch
+
+from . import _lib
+from . import _count_launch, _stream, mixers
+
+MAX_K = 133144                       # 127 * 127 * k stays below 2^31
+_FORMS = {"bf16": 0, "f32": 1, "norm": 2, "gate_bf16": 3, "gate_f32": 4}
+# NkbQuantRows and NkbGemmI8 of csrc/kernels/i8_args.h
+_ROWS, _GEMM = struct.Struct("9P3q4i3fi"), struct.Struct("8P4q8i")
+
+
+class _Quantized:
+    """int8 `values` [rows, k] and fp32 `scale` [rows] on one device.  Rows start on 16 bytes: values that do not lie so are copied."""
+    __slots__ = ("values", "scale", "shape", "index", "device", "ld", "at")
+
+    def __init__(self, values: torch.Tensor, scale: torch.Tensor):
+        if values.dtype is not torch.int8 or scale.dtype is not torch.float32:
+            raise TypeError(f"{type(self).__name__} wants int8 values and fp32 scales")
+        shape = values.shape
+        if len(shape) != 2 or scale.shape != shape[:1] or not 1 <= shape[1] <= MAX_K:
+            raise ValueError(f"{type(self).__name__} wants values [rows, k] of at most {MAX_K} columns and scales [rows]")
+        index = values.get_device()
+        if scale.get_device() != index or (shape[0] > 1 and scale.stride(0) != 1):
+            raise ValueError(f"{type(self).__name__} wants scales that follow one another, on the values' device")
+        ld, column = values.stride()
+        if (column != 1 and shape[1] > 1) or ld < shape[1] or ld & 15 or values.data_ptr() & 15:
+            values = _padded(shape[0], shape[1], values.device).copy_(values)
+            ld = values.stride(0)
+        # index: of the CUDA device, -1: the CPU; ld: numbers from one row to the next; at: where values and scales start
+        self.values, self.scale, self.shape, self.index, self.device, self.ld = values, scale, shape, index, values.device, ld
+        self.at = values.data_ptr(), scale.data_ptr()
+
+    @property
+    def is_cuda(self) -> bool:
+        return self.index >= 0
+
+    @property
+    def nbytes(self) -> int:
+        return self.values.numel() + 4 * self.scale.numel()
+
+    def dequantize(self) -> torch.Tensor:
+        """The values that the rows stand for, fp32 [rows, k]."""
+        return self.values.float() * self.scale[:, None]
+
+
+class QuantizedRows(_Quantized):
+    """Rows of activations [tokens, k] in 8 bits."""
+    __slots__ = ()
+
+
+class QuantizedWeight(_Quantized):
+    """A weight [n, k] in 8 bits with a scale for every output channel; for a gated product [2 n, k], gate rows and then up rows.
+
+    Weights may be fetched while the kernel before the product still runs (`linear`, weights_static): a program that writes the
+    values of an existing one says weights_static=False in the product behind that."""
+    __slots__ = ()
+
+    @classmethod
+    def of(cls, w: torch.Tensor) -> "QuantizedWeight":
+        """From bf16 or fp32 [n, k]."""
+        r = quantize_rows(w)
+        return cls(r.values, r.scale)
+
+
+def _padded(rows: int, k: int, device) -> torch.Tensor:
+    """int8 [rows, k] whose rows start on 16 bytes."""
+    ld = (k + 15) // 16 * 16
+    t = torch.empty((rows, ld), dtype=torch.int8, device=device)
+    if ld == k:
+        return t
+    t[:, k:].zero_()
+    return t[:, :k]
+
+
+def _want(t: torch.Tensor, name: str, dtypes, shape, index: int) -> None:
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} wants {' or '.join(map(str, dtypes))}, not {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name} has the shape {tuple(t.shape)}, not {tuple(shape)}")
+    if t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name} wants to be contiguous and on the others' device")
+
+
+def _on_gpu(index: int) -> bool:
+    """Whether the kernels run (CUDA); they are launched on the current device's current stream."""
+    if index < 0:
+        return False
+    if index != torch._C._cuda_getDevice():
+        raise ValueError("the tensors are on another device than the current one")
+    if not _lib._initialised:
+        _lib.ensure_init()
+    return True
+
+
+_BF16, _BF16_F32 = (torch.bfloat16,), (torch.bfloat16, torch.float32)
+
+
+# --------------------------------------------------------------------------- rows
+def _numbers(x: torch.Tensor):
+    """(whole numbers, largest magnitude) of rows in 64 bits; zeros and NaN where a row is not finite in 32."""
+    fine = x.float().isfinite().all(-1, keepdim=True)
+    top = torch.where(fine, x, 0.0).abs().amax(-1, keepdim=True)
+    q = torch.round(127 * (x / top))
+    return torch.where(fine & (top > 0), q, 0.0).to(torch.int8), torch.where(fine, top, torch.nan).squeeze(-1)
+
+
+def _new_rows(rows: int, width: int, device):
+    """(buffer whose rows end on 16 bytes, scales); the kernel writes the buffer's last columns too."""
+    return (torch.empty((rows, (width + 15) // 16 * 16), dtype=torch.int8, device=device),
+            torch.empty((rows,), dtype=torch.float32, device=device))
+
+
+def _rows_of(buffer: torch.Tensor, scale: torch.Tensor, width: int) -> QuantizedRows:
+    return QuantizedRows(buffer if buffer.shape[1] == width else buffer[:, :width], scale)
+
+
+def _launch_rows(form, rows, width, device, x=0, partials=0, bias=None, residual=None, w=None, residual_out=None, x_ld=0, split_stride=0,
+                 splits=0, eps=0.0, limit=0.0, alpha=0.0) -> QuantizedRows:
+    buffer, scale = _new_rows(rows, width, device)
+    p = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    rc = _lib.lib().nkb_quant_rows(_ROWS.pack(
+        x, partials, p(bias), p(residual), p(w), p(residual_out), buffer.data_ptr(), scale.data_ptr(), _stream(), x_ld, buffer.shape[1],
+        split_stride, _FORMS[form], rows, width, splits, eps, limit, alpha, 0))
+    if rc:
+        _lib.check(rc, "nkb_quant_rows")
+    _count_launch()
+    return _rows_of(buffer, scale, width)
+
+
+def quantize_rows(x: torch.Tensor) -> QuantizedRows:
+    """bf16 or fp32 rows [rows, k] (they may lie apart) in 8 bits."""
+    if x.dtype not in _BF16_F32:
+        raise TypeError(f"quantize_rows wants bf16 or fp32, not {x.dtype}")
+    if x.dim() != 2 or not 1 <= x.shape[1] <= MAX_K:
+        raise ValueError(f"quantize_rows wants [rows, k] of at most {MAX_K} columns")
+    rows, width = x.shape
+    ld, column = x.stride()
+    if column != 1 and width > 1:
+        raise ValueError("quantize_rows wants neighbouring columns")
+    if not _on_gpu(x.get_device()):
+        q, top = _numbers(x.double())
+        return QuantizedRows(q, (top / 127).float())
+    return _launch_rows("bf16" if x.dtype is torch.bfloat16 else "f32", rows, width, x.device, x=x.data_ptr(), x_ld=ld)
+
+
+def add_rmsnorm(x, w, *, residual_in=None, partials=None, bias=None, residual_out=None, eps=1e-6, hidden=None, rows=None):
+    """`ops.add_rmsnorm` whose normed rows are brought into 8 bits.  The residual stream, the sum rounded to bf16, is what the norm sees,
+    whether it is wanted or not; sums of more than two addends are taken in 64 bits."""
+    ref = x if x is not None else partials
+    if ref is None or w is None:
+        raise ValueError("quantised rows come from x or partial sums, and from a norm")
+    index, hidden = ref.get_device(), ref.shape[-1] if hidden is None else hidden
+    if not 1 <= hidden <= MAX_K:
+        raise ValueError(f"quantised rows have at most {MAX_K} columns")
+    if rows is None:
+        rows = x.numel() // hidden if x is not None else partials.shape[-2]
+    splits, stride = 0, 0
+    if partials is not None:
+        if partials.dtype is not torch.float32:
+            raise TypeError("partials must be fp32")
+        splits = partials.shape[0] if partials.dim() == 3 else 1
+        stride = partials.stride(0) if partials.dim() == 3 else 0
+        one = partials[0] if partials.dim() == 3 and splits else partials
+        if not splits or one.shape != (rows, hidden) or partials.get_device() != index or not one.is_contiguous():
+            raise ValueError("partials wants [splits, rows, hidden] with neighbouring rows, on the others' device")
+    for t, name in ((x, "x"), (residual_in, "residual_in"), (residual_out, "residual_out")):
+        if t is not None and t.numel() != rows * hidden:
+            raise ValueError(f"{name} wants {rows} rows of {hidden}")
+        if t is not None:
+            _want(t, name, _BF16, t.shape, index)
+    _want(w, "w", _BF16, (hidden,), index)
+    if bias is not None:
+        _want(bias, "bias", _BF16, (hidden,), index)
+    if residual_out is None and (residual_in is not None or partials is not None):
+        residual_out = torch.empty((rows, hidden), dtype=torch.bfloat16, device=ref.device)
+    if not _on_gpu(index):
+        h = torch.zeros((rows, hidden), dtype=torch.float64)
+        if partials is not None:
+            h = h + (partials.double().sum(0) if partials.dim() == 3 else partials.double())
+        for t in (x, bias, residual_in):
+            if t is not None:
+                h = h + t.double().reshape(-1, hidden)
+        h = h.to(torch.bfloat16)
+        if residual_out is not None:
+            residual_out.copy_(h.reshape(residual_out.shape))
+        q, top = _numbers(h.double() * w.double())
+        scale = (top / 127).float() * torch.rsqrt(h.float().square().mean(-1) + eps)
+        return residual_out, QuantizedRows(q, scale)
+    return residual_out, _launch_rows("norm", rows, hidden, ref.device, x=0 if x is None else x.data_ptr(),
+                                      partials=0 if partials is None else partials.data_ptr(), bias=bias, residual=residual_in, w=w,
+                                      residual_out=residual_out, x_ld=hidden, split_stride=stride, splits=splits, eps=eps)
+
+
+def silu_mul(gate_up, limit: float = 0.0, alpha: float = 1.702, bias=None) -> QuantizedRows:
+    """`ops.silu_mul` whose rows are brought into 8 bits; bf16 [T, 2 I], or fp32 (partial sums) [S, T, 2 I]."""
+    if gate_up.dtype not in _BF16_F32:
+        raise TypeError(f"silu_mul wants bf16 or fp32, not {gate_up.dtype}")
+    index, f32 = gate_up.get_device(), gate_up.dtype is torch.float32
+    if gate_up.dim() != 2 and not (f32 and gate_up.dim() == 3 and gate_up.shape[0]):
+        raise ValueError("silu_mul wants [T, 2 I], or fp32 partial sums [S, T, 2 I]")
+    rows, two = gate_up.shape[-2:]
+    width = two // 2
+    if two % 2 or not 1 <= width <= MAX_K:
+        raise ValueError(f"silu_mul wants gate and up of at most {MAX_K} columns")
+    if gate_up.stride(-1) != 1:
+        raise ValueError("silu_mul wants neighbouring columns")
+    if bias is not None:
+        _want(bias, "bias", _BF16, (two,), index)
+    if not _on_gpu(index):
+        v = gate_up.double() if gate_up.dim() == 2 else gate_up.double().sum(0)
+        if bias is not None:
+            v = v + bias.double()
+        g, u = v[:, :width], v[:, width:]
+        if limit > 0:
+            g, u = g.clamp(max=limit), u.clamp(-limit, limit)
+            y = (u + 1) * g / (1 + torch.exp(-alpha * g))
+        else:
+            y = g / (1 + torch.exp(-g)) * u
+        q, top = _numbers(y)
+        return QuantizedRows(q, (top / 127).float())
+    parts = gate_up.shape[0] if gate_up.dim() == 3 else 1
+    return _launch_rows("gate_f32" if f32 else "gate_bf16", rows, width, gate_up.device, x=0 if f32 else gate_up.data_ptr(),
+                        partials=gate_up.data_ptr() if f32 else 0, bias=bias, x_ld=gate_up.stride(-2),
+                        split_stride=gate_up.stride(0) if gate_up.dim() == 3 else 0, splits=parts if f32 else 0, limit=limit, alpha=alpha)
+
+
+# --------------------------------------------------------------------------- products
+def effective_splits(k: int, splits: int) -> int:
+    """Partial sums that a product asked for `splits` of them really has: whole slabs of 128 k, none of them empty."""
+    slabs = -(-k // 128)
+    return -(-slabs // -(-slabs // max(1, min(splits, slabs))))
+
+
+def linear(x, w: QuantizedWeight, *, bias=None, residual=None, out=None, splits: int = 1, gated: bool = False, weights_static: bool = True,
+           act: str = "silu", fp32_out: bool = False, out_act=None) -> torch.Tensor:
+    """`ops.linear` with a weight in 8 bits; x: `QuantizedRows`, or bf16 or fp32 rows, which are brought into 8 bits first.
+
+    The sum is exact; it is rounded to 32 bits and multiplied by both scales, and the result is rounded once more, to bf16, at the
+    end.  Rows of other types than bf16 and fp32 are refused, and so is out_act."""
+    if type(w) is not QuantizedWeight:
+        raise TypeError("rows in 8 bits want a QuantizedWeight")
+    if out_act is not None:
+        raise ValueError("products in 8 bits have no out_act")
+    N = w.shape[0] // 2 if gated else w.shape[0]
+    if gated and (w.shape[0] % 2 or act not in ("silu", "gelu_tanh")):
+        raise ValueError("a gated product wants gate and up rows, and silu or gelu_tanh")
+    if not isinstance(x, QuantizedRows):
+        if x.dim() != 2 or x.shape[1] != w.shape[1]:
+            raise ValueError(f"shape mismatch: x {tuple(x.shape)} w {tuple(w.shape)}")
+        x = quantize_rows(x)
+    M, K = x.shape
+    index = w.index
+    if K != w.shape[1]:
+        raise ValueError(f"shape mismatch: x {tuple(x.shape)} w {tuple(w.shape)}")
+    if x.index != index:
+        raise ValueError("rows and weight want to be on one device")
+    if gated and (bias is not None or residual is not None or fp32_out or splits > 1):
+        raise ValueError("a gated product has no bias, residual, fp32_out or splits")
+    if splits > 1 and residual is not None:
+        raise ValueError("partial sums have no residual")
+    dtype = torch.float32 if fp32_out or splits > 1 else torch.bfloat16
+    parts = effective_splits(K, splits) if splits > 1 else 0
+    if bias is not None:
+        _want(bias, "bias", _BF16, (N,), index)
+    if out is None:
+        out = torch.empty((parts, M, N) if parts else (M, N), dtype=dtype, device=w.device)
+    elif parts:
+        if out.dtype is not dtype or not out.is_contiguous() or out.get_device() != index or out.numel() < parts * M * N:
+            raise ValueError("split-K output must be fp32 with room for [S, M, N]")
+        out = out.view(-1)[:parts * M * N].view(parts, M, N)
+    else:
+        if out.dtype is not dtype:
+            raise TypeError(f"out wants {dtype}, not {out.dtype}")
+        if out.shape != (M, N) or out.get_device() != index or (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
+            raise ValueError("out wants [M, N] with neighbouring columns, on the weight's device")
+    ldo = max(out.stride(-2), N)
+    if residual is not None:
+        if residual.dtype is not torch.bfloat16:
+            raise TypeError(f"residual wants torch.bfloat16, not {residual.dtype}")
+        if residual.shape != (M, N) or residual.get_device() != index:
+            raise ValueError("residual wants [M, N] on the weight's device")
+        if residual.stride() != out.stride():
+            residual = residual.contiguous() if ldo == N else torch.empty_strided((M, N), (ldo, 1), dtype=residual.dtype,
+                                                                                  device=residual.device).copy_(residual)
+    if not M or not w.shape[0]:
+        return out
+    if not _on_gpu(index):
+        return _reference(x, w, bias, residual, out, parts, gated, act, N)
+    rc = _lib.lib().nkb_gemm_i8(_GEMM.pack(
+        x.at[0], w.at[0], x.at[1], w.at[1], 0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(),
+        out.data_ptr(), _stream(), x.ld, w.ld, ldo, out.stride(0) if parts else 0, M, N, K, gated, mixers.ACTIVATIONS[act][0] if gated else 0,
+        dtype is torch.float32, parts, weights_static))
+    if rc:
+        _lib.check(rc, "nkb_gemm_i8")
+    _count_launch()
+    return out
+
+
+def _reference(x, w, bias, residual, out, parts, gated, act, N):
+    q, v = x.values.double(), w.values.double()
+
+    def part(a, b):
+        return (q[:, a:b] @ v[:, a:b].T).float() * x.scale[:, None] * w.scale
+
+    if parts:
+        step = -(-(-(-x.shape[1] // 128)) // parts) * 128
+        for s in range(parts):
+            out[s] = part(s * step, (s + 1) * step)
+        if bias is not None:
+            out[0] += bias.float()
+        return out
+    y = part(0, x.shape[1])
+    if gated:
+        y = mixers.ACTIVATIONS[act][1](y[:, :N]) * y[:, N:]
+    if bias is not None:
+        y = y + bias.float()
+    if residual is not None:
+        y = y + residual.float()
+    return out.copy_(y)
