@@ -7,37 +7,79 @@
 //   mask bit zero:                       l = -inf
 // Most tokens are named by none: they pass as they are, and in place they are not even read.
 //
-// A slice of the vocabulary per CTA.  Its counts lie in shared memory, one word per token (bit 31: seen, bit 30: has a bias, below: times in the answer), filled
-// from the row's whole list of tokens, so there is no state to keep beside that list, no hashing, and no limit on its length; whole numbers, so the
-// order of the counting changes nothing.  Then one pass over the slice's logits.  The most likely token of a row's slices is found by the CTAs of a cluster
-// through distributed shared memory: no workspace that calls could share, and ties go to the lowest index.
+// A slice of the vocabulary per CTA.  Its counts lie in shared memory, half a word per token (highest bit: seen in the prompt, next: has a bias, below:
+// times in the answer; a whole word where a list may be longer than 14 bits), filled from the row's whole list of tokens, so there is no state to
+// keep beside that list, no hashing, and no limit on its length; whole numbers, so the order of the counting changes nothing.  Then one pass over the
+// slice's logits, whose first loads are on their way while the counting goes on.  The counting also puts every token that the rules name on a list, which the
+// whole CTA works off: named tokens lie close together (a text has its frequent ones), and 64-bit divisions in the pass itself would be one thread's, one
+// after another.  The most likely token of a row's slices is found by the CTAs of a cluster through distributed shared
+// memory: no workspace that calls could share, and ties go to the lowest index.
 #include "api.h"
 #include "common.cuh"
 #include "rules_args.h"
+#include <type_traits>
 
 namespace nkb {
 
-constexpr uint32_t kSeen = 0x80000000u, kBiased = 0x40000000u, kTimes = 0x3fffffffu;
-constexpr int kSliceMost = 24576;       // tokens whose counts are held at a time (96 KB)
 constexpr int kRuleThreads = 512;
+constexpr int kCountBytes = 96 * 1024;  // counts of the tokens that a CTA holds at a time: two CTAs per SM
+constexpr int kListMost = 2048;         // named tokens on the list
+constexpr int kPer = 8;                 // tokens of a piece
+
+template <bool WIDE>
+struct Counts {
+  static constexpr uint32_t kSeen = WIDE ? 0x80000000u : 0x8000u, kBiased = kSeen >> 1, kTimes = kBiased - 1;
+  static constexpr int kTokens = kCountBytes / (WIDE ? 4 : 2);
+  uint32_t* w;
+  // (both say whether the token had not been named before: one of all threads is told so)
+  __device__ __forceinline__ bool add(int t, uint32_t v) const {
+    if (WIDE) return atomicAdd(w + t, v) == 0u;
+    return ((atomicAdd(w + (t >> 1), v << (16 * (t & 1))) >> (16 * (t & 1))) & 0xffffu) == 0u;
+  }
+  __device__ __forceinline__ bool mark(int t, uint32_t v) const {
+    if (WIDE) return atomicOr(w + t, v) == 0u;
+    return ((atomicOr(w + (t >> 1), v << (16 * (t & 1))) >> (16 * (t & 1))) & 0xffffu) == 0u;
+  }
+  __device__ __forceinline__ uint32_t get(int t) const { return WIDE ? w[t] : (w[t >> 1] >> (16 * (t & 1))) & 0xffffu; }
+  // which tokens of a piece are named
+  __device__ __forceinline__ uint32_t named(int piece) const {
+    uint32_t b = 0;
+    if constexpr (WIDE) {
+      const uint4 x = reinterpret_cast<const uint4*>(w)[2 * piece], y = reinterpret_cast<const uint4*>(w)[2 * piece + 1];
+      const uint32_t c[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) b |= (c[j] ? 1u : 0u) << j;
+    } else {
+      const uint4 x = reinterpret_cast<const uint4*>(w)[piece];
+      if ((x.x | x.y | x.z | x.w) == 0u) return 0u;
+      const uint32_t c[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b |= ((c[j] & 0xffffu) ? 1u << (2 * j) : 0u) | ((c[j] >> 16) ? 2u << (2 * j) : 0u);
+    }
+    return b;
+  }
+};
 
 struct RuleRow {
-  double rep, freq, pres;
+  float rep, freq, pres;
   const int* bias_ids;
   const float* bias_values;
   int biases;
 };
 
+template <bool WIDE>
 __device__ __noinline__ float ruled(const RuleRow& r, float l0, uint32_t c, int token) {
+  using C = Counts<WIDE>;
   double l = l0;
-  if (c & kSeen) {
-    l = l > 0.0 ? l / r.rep : l * r.rep;
-    const uint32_t n = c & kTimes;
-    l -= r.freq * double(n);
-    if (n) l -= r.pres;
+  const uint32_t n = c & C::kTimes;
+  if (n || (c & C::kSeen)) {
+    if (r.rep != 1.f) l = l > 0.0 ? l / double(r.rep) : l * double(r.rep);
+    l -= double(r.freq) * double(n);
+    if (n) l -= double(r.pres);
   }
-  if (c & kBiased) {
+  if (c & C::kBiased) {
     double sum = 0.0;
+#pragma unroll 8
     for (int i = 0; i < r.biases; ++i)
       if (r.bias_ids[i] == token) sum += double(r.bias_values[i]);
     l += sum;
@@ -49,139 +91,249 @@ template <bool F32>
 __device__ __forceinline__ float rule_logit(const void* p, long long i) {
   return F32 ? reinterpret_cast<const float*>(p)[i] : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
 }
+template <bool F32>
+__device__ __forceinline__ void rule_store(void* p, long long i, float v) {
+  if constexpr (F32) reinterpret_cast<float*>(p)[i] = v;
+  else reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16(v);
+}
 
-// Grid: x = slices of a row (a cluster where ids are wanted), y strides over the rows.
-template <bool F32, bool VEC>
-__global__ void __launch_bounds__(kRuleThreads) logit_rules_kernel(const NkbLogitRules a, int slice) {
-  extern __shared__ __align__(16) uint32_t counts[];
+// Logits of a whole piece as they lie in memory, on sixteen bytes.
+template <bool F32>
+struct Piece {
+  static constexpr int kWords = F32 ? 2 : 1;
+  uint4 r[kWords];
+  __device__ __forceinline__ void load(const uint8_t* p) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) r[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  __device__ __forceinline__ float value(int j) const {
+    const uint32_t w[8] = {r[0].x, r[0].y, r[0].z, r[0].w, r[F32].x, r[F32].y, r[F32].z, r[F32].w};
+    return F32 ? __uint_as_float(w[j]) : __uint_as_float(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
+  }
+  // minus infinity where `left` has no bit
+  __device__ __forceinline__ Piece masked(uint32_t left) const {
+    Piece o = *this;
+    uint32_t w[8] = {r[0].x, r[0].y, r[0].z, r[0].w, r[F32].x, r[F32].y, r[F32].z, r[F32].w};
+    if constexpr (F32) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) w[j] = (left >> j) & 1u ? w[j] : 0xff800000u;
+      o.r[F32] = make_uint4(w[4], w[5], w[6], w[7]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t keep = ((((left >> (2 * e)) & 3u) * 0x8001u) & 0x10001u) * 0xffffu;       // two bits, sixteen times each
+        w[e] = (w[e] & keep) | (0xff80ff80u & ~keep);
+      }
+    }
+    o.r[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    return o;
+  }
+  __device__ __forceinline__ void store(uint8_t* p) const {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) reinterpret_cast<uint4*>(p)[i] = r[i];
+  }
+  // The largest number; a NaN loses against every number.
+  __device__ __forceinline__ float largest() const {
+    if constexpr (F32) {
+      return fmaxf(fmaxf(fmaxf(value(0), value(1)), fmaxf(value(2), value(3))), fmaxf(fmaxf(value(4), value(5)), fmaxf(value(6), value(7))));
+    } else {
+      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r[0]);
+      const float2 f = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+      return fmaxf(f.x, f.y);
+    }
+  }
+};
+
+// Grid: x = slices of a row (a cluster where ids are wanted), y: rows.  Either out or out_ids.
+template <bool F32, bool VEC, bool WIDE>
+__global__ void __launch_bounds__(kRuleThreads, 2) logit_rules_kernel(const NkbLogitRules a, int slice) {
+  using C = Counts<WIDE>;
+  extern __shared__ __align__(16) uint32_t words[];
+  __shared__ int s_list[kListMost];
+  __shared__ int s_n;
   __shared__ float s_best[kRuleThreads / 32];
   __shared__ int s_at[kRuleThreads / 32];
-  __shared__ int2 s_mine;               // best of this CTA's slice: bits of the value, token
-  constexpr int kPer = 8;               // tokens of a piece
-  constexpr int kBytes = F32 ? 4 : 2;
-  griddep_wait();
-  griddep_launch();
+  __shared__ int2 s_slices[8];          // in the cluster's first CTA: best of every slice, bits of the value and token
+  constexpr int kBytes = F32 ? 4 : 2, kAhead = F32 ? 4 : 8;       // pieces of a thread on their way: 128 bytes
+  const C counts{words};
   const int row = blockIdx.y, tid = threadIdx.x;
   const int first = blockIdx.x * slice, last = min(a.vocab, first + slice);
-  const int len = a.tokens ? min(a.lens[row], a.width) : 0;
-  const int prompt = a.prompts && a.tokens ? a.prompts[row] : 0;
+  const uint8_t* in = reinterpret_cast<const uint8_t*>(a.logits) + (long long)row * a.ld * kBytes;
+  uint8_t* out = reinterpret_cast<uint8_t*>(a.out) + (a.out ? (long long)row * a.out_ld * kBytes : 0);
+  const bool ids = a.out_ids != nullptr, in_place = !ids && out == in;
+  const bool joined = ids && gridDim.x > 1;
+  if (joined) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");       // (waited for before the first access to another CTA)
+  griddep_wait();
+  griddep_launch();
+
+  // VEC: whole pieces of sixteen-byte words; what is left of a slice, and everything where rows do not start on sixteen bytes, token by token
+  constexpr int kPiece = kPer * kBytes;
+  Piece<F32> x[VEC ? kAhead : 1];
+  auto load = [&](int lo, int pieces, int p0) {
+    if (!VEC || in_place) return;
+    const uint8_t* p = in + (long long)lo * kBytes + (p0 + tid) * kPiece;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (p0 + tid + i * kRuleThreads < pieces) x[VEC ? i : 0].load(p + i * (kRuleThreads * kPiece));
+  };
+  load(first, (min(last, first + C::kTokens) - first) / kPer, 0);
+
   int* tokens = a.tokens ? a.tokens + row * a.tokens_ld : nullptr;
+  // the first tokens of the list, too, whose length is not known yet
+  const bool token16 = (reinterpret_cast<uintptr_t>(tokens) & 15) == 0;
+  const bool early = tokens && token16 && 4 * tid + 4 <= a.width;
+  int4 ahead = make_int4(-1, -1, -1, -1);
+  if (early) ahead = *reinterpret_cast<const int4*>(tokens + 4 * tid);
+  const int len = a.tokens ? min(a.lens[row], a.width) : 0;
   const bool fresh = a.ids && len > 0;
   const int newest = fresh ? a.ids[row] : 0;
   if (fresh && blockIdx.x == 0 && tid == 0) tokens[len - 1] = newest;      // (the others take it from ids)
   RuleRow r;
-  r.rep = a.repetition ? double(a.repetition[row]) : 1.0;
-  r.freq = a.frequency ? double(a.frequency[row]) : 0.0;
-  r.pres = a.presence ? double(a.presence[row]) : 0.0;
+  r.rep = a.repetition ? a.repetition[row] : 1.f;
+  r.freq = a.frequency ? a.frequency[row] : 0.f;
+  r.pres = a.presence ? a.presence[row] : 0.f;
   r.bias_ids = a.bias_ids + row * a.bias_ld;
   r.bias_values = a.bias_values + row * a.bias_ld;
   r.biases = a.biases;
-  const bool counted = len > 0 && (r.rep != 1.0 || r.freq != 0.0 || r.pres != 0.0);
+  const bool counted = len > 0 && (r.rep != 1.f || r.freq != 0.f || r.pres != 0.f);
+  const int prompt = a.prompts && counted ? a.prompts[row] : 0;
   const int mrow = a.mask_rows ? a.mask_rows[row] : row;
   const int* mask = a.mask && mrow >= 0 && mrow < a.mask_count ? a.mask + mrow * a.mask_ld : nullptr;
-  const uint8_t* in = reinterpret_cast<const uint8_t*>(a.logits) + (long long)row * a.ld * kBytes;
-  uint8_t* out = reinterpret_cast<uint8_t*>(a.out) + (a.out ? (long long)row * a.out_ld * kBytes : 0);
-  const bool in_place = a.out && out == in;
   const bool named = counted || a.biases > 0;
   float best = -INFINITY;
   int at = 0x7fffffff;
-
-  for (int lo = first; lo < last; lo += kSliceMost) {
-    const int hi = min(last, lo + kSliceMost);
-    if (named) {
-      for (int i = tid; i < (hi - lo + 3) / 4; i += kRuleThreads) reinterpret_cast<uint4*>(counts)[i] = make_uint4(0u, 0u, 0u, 0u);
-      __syncthreads();
-      if (counted) {
-        for (int i = tid; i < len; i += kRuleThreads) {
-          const int t = (fresh && i == len - 1 ? newest : tokens[i]) - lo;
-          if (t < 0 || t >= hi - lo) continue;
-          atomicOr(&counts[t], kSeen);
-          if (i >= prompt) atomicAdd(&counts[t], 1u);
-        }
-      }
-      for (int i = tid; i < a.biases; i += kRuleThreads) {
-        const int t = r.bias_ids[i] - lo;
-        if (t >= 0 && t < hi - lo) atomicOr(&counts[t], kBiased);
-      }
-      __syncthreads();
-    }
-    for (int p = tid; p < (hi - lo + kPer - 1) / kPer; p += kRuleThreads) {
-      const int t0 = lo + p * kPer, n = min(kPer, hi - t0);
-      uint32_t c[kPer];
-      uint32_t any = 0;
-      if (named) {
-        const uint4 c0 = reinterpret_cast<const uint4*>(counts)[2 * p], c1 = reinterpret_cast<const uint4*>(counts)[2 * p + 1];
-        c[0] = c0.x; c[1] = c0.y; c[2] = c0.z; c[3] = c0.w;
-        c[4] = c1.x; c[5] = c1.y; c[6] = c1.z; c[7] = c1.w;
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) any |= j < n ? c[j] : 0u;
-      }
-      const uint32_t left = mask ? (uint32_t(mask[t0 >> 5]) >> (t0 & 31)) & 255u : 255u;
-      if (in_place && !any && left == 255u && !a.out_ids) continue;
-      float l[kPer];
-      if (VEC && n == kPer) {
-        if constexpr (F32) {
-          const float4 x = reinterpret_cast<const float4*>(in + t0 * 4ll)[0], y = reinterpret_cast<const float4*>(in + t0 * 4ll)[1];
-          l[0] = x.x; l[1] = x.y; l[2] = x.z; l[3] = x.w;
-          l[4] = y.x; l[5] = y.y; l[6] = y.z; l[7] = y.w;
-        } else {
-          const uint4 x = *reinterpret_cast<const uint4*>(in + t0 * 2ll);
-          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 f = unpack_bf16x2(w[e]);
-            l[2 * e] = f.x;
-            l[2 * e + 1] = f.y;
-          }
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) l[j] = j < n ? rule_logit<F32>(in, t0 + j) : 0.f;
-      }
-      if (any) {
-#pragma unroll
-        for (int j = 0; j < kPer; ++j)
-          if (j < n && c[j]) l[j] = ruled(r, l[j], c[j], t0 + j);
-      }
-#pragma unroll
-      for (int j = 0; j < kPer; ++j)
-        if (!((left >> j) & 1u)) l[j] = -INFINITY;
-      if (a.out) {
-        if (VEC && n == kPer) {
-          if constexpr (F32) {
-            reinterpret_cast<float4*>(out + t0 * 4ll)[0] = make_float4(l[0], l[1], l[2], l[3]);
-            reinterpret_cast<float4*>(out + t0 * 4ll)[1] = make_float4(l[4], l[5], l[6], l[7]);
-          } else {
-            *reinterpret_cast<uint4*>(out + t0 * 2ll) = make_uint4(pack_bf16x2(l[0], l[1]), pack_bf16x2(l[2], l[3]), pack_bf16x2(l[4], l[5]),
-                                                                   pack_bf16x2(l[6], l[7]));
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < kPer; ++j)
-            if (j < n) {
-              if constexpr (F32) reinterpret_cast<float*>(out)[t0 + j] = l[j];
-              else reinterpret_cast<__nv_bfloat16*>(out)[t0 + j] = __float2bfloat16(l[j]);
-            }
-        }
-      }
-      if (a.out_ids) {
-#pragma unroll
-        for (int j = 0; j < kPer; ++j)
-          if (j < n && l[j] > best) {            // pieces of a thread come in ascending order; a NaN loses against every number
-            best = l[j];
-            at = t0 + j;
-          }
-      }
-    }
-    if (named) __syncthreads();
-  }
-  if (!a.out_ids) return;
   auto better = [&](float v, int i) {
     if (v > best || (v == best && i < at)) {
       best = v;
       at = i;
     }
   };
+
+  // The tokens on the list; one that ran over is left alone, and every token looked at.
+  auto named_tokens = [&](int lo, int hi) {
+    const bool listed = s_n <= kListMost;
+    const int n = listed ? s_n : hi - lo;
+    for (int e = tid; e < n; e += kRuleThreads) {
+      const int t = listed ? s_list[e] : lo + e;
+      const uint32_t c = counts.get(t - lo);
+      if (!c || (mask && !((uint32_t(mask[t >> 5]) >> (t & 31)) & 1u))) continue;
+      const float v = ruled<WIDE>(r, rule_logit<F32>(in, t), c, t);
+      if (ids) better(v, t);
+      else rule_store<F32>(out, t, v);
+    }
+  };
+
+  for (int lo = first; lo < last; lo += C::kTokens) {
+    const int hi = min(last, lo + C::kTokens), pieces = VEC ? (hi - lo) / kPer : 0;
+    if (lo > first) load(lo, pieces, 0);
+    if (named) {
+      for (int i = tid; i < (WIDE ? 2 : 1) * ((hi - lo + kPer - 1) / kPer); i += kRuleThreads) reinterpret_cast<uint4*>(words)[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (tid == 0) s_n = 0;
+      __syncthreads();
+      // who names a token first puts it on the list; places for a whole warp at once: one counter that many lanes add to takes them one after another
+      auto list = [&](bool first_time, int t) {
+        const uint32_t lanes = __ballot_sync(0xffffffffu, first_time);
+        if (lanes == 0u) return;
+        int base = 0;
+        if ((tid & 31) == 0) base = atomicAdd(&s_n, __popc(lanes));
+        const int e = __shfl_sync(0xffffffffu, base, 0) + __popc(lanes & ((1u << (tid & 31)) - 1u));
+        if (first_time && e < kListMost) s_list[e] = t;
+      };
+      auto count = [&](int t, int i) {
+        if (fresh && i == len - 1) t = newest;
+        bool first_time = false;
+        if (i < len && t >= lo && t < hi) first_time = i >= prompt ? counts.add(t - lo, 1u) : counts.mark(t - lo, C::kSeen);
+        list(first_time, t);
+      };
+      if (counted) {
+        const int most = (len + 127) & ~127;           // whole warps
+        for (int i = 4 * tid; i < most; i += 4 * kRuleThreads) {
+          int4 t = make_int4(-1, -1, -1, -1);
+          if (early && i == 4 * tid) {
+            t = ahead;
+          } else if (token16 && i + 4 <= a.width) {
+            t = *reinterpret_cast<const int4*>(tokens + i);
+          } else {
+            if (i < len) t.x = tokens[i];
+            if (i + 1 < len) t.y = tokens[i + 1];
+            if (i + 2 < len) t.z = tokens[i + 2];
+            if (i + 3 < len) t.w = tokens[i + 3];
+          }
+          count(t.x, i);
+          count(t.y, i + 1);
+          count(t.z, i + 2);
+          count(t.w, i + 3);
+        }
+      }
+      for (int i = tid; i < ((a.biases + 31) & ~31); i += kRuleThreads) {
+        const int t = i < a.biases ? r.bias_ids[i] : -1;
+        list(t >= lo && t < hi && counts.mark(t - lo, C::kBiased), t);
+      }
+      __syncthreads();
+      if (ids) named_tokens(lo, hi);
+    }
+    const uint8_t* mask8 = reinterpret_cast<const uint8_t*>(mask) + (lo >> 3);           // (slices begin at whole words)
+    float top = -INFINITY;                  // of this thread's pieces, which come in ascending order
+    int top_piece = -1;
+    for (int p0 = 0; p0 < pieces; p0 += kAhead * kRuleThreads) {
+      uint32_t left[VEC ? kAhead : 1];
+#pragma unroll
+      for (int i = 0; i < (VEC ? kAhead : 0); ++i) {
+        const int p = p0 + i * kRuleThreads + tid;
+        left[i] = mask && p < pieces ? mask8[p] : 255u;
+      }
+      uint8_t* to = out + (long long)lo * kBytes + (p0 + tid) * kPiece;
+#pragma unroll
+      for (int i = 0; i < (VEC ? kAhead : 0); ++i) {
+        const int p = p0 + i * kRuleThreads + tid;
+        if (p >= pieces) continue;
+        if (ids) {
+          const uint32_t plain = named ? left[i] & ~counts.named(p) : left[i];
+          const float m = plain == 255u ? x[i].largest() : x[i].masked(plain).largest();
+          if (m > top) {
+            top = m;
+            top_piece = p;
+          }
+        } else if (!in_place) {
+          if (left[i] == 255u) x[i].store(to + i * (kRuleThreads * kPiece));
+          else x[i].masked(left[i]).store(to + i * (kRuleThreads * kPiece));
+        } else if (left[i] != 255u) {
+          Piece<F32> y;
+          y.load(to + i * (kRuleThreads * kPiece));
+          y.masked(left[i]).store(to + i * (kRuleThreads * kPiece));
+        }
+      }
+      if (p0 + kAhead * kRuleThreads < pieces) load(lo, pieces, p0 + kAhead * kRuleThreads);
+    }
+    if (top_piece >= 0) {
+      // which of the piece's tokens it was
+      Piece<F32> y;
+      y.load(in + ((long long)lo + top_piece * kPer) * kBytes);
+      uint32_t plain = mask ? mask8[top_piece] : 255u;
+      if (named) plain &= ~counts.named(top_piece);
+      int j = kPer;
+#pragma unroll
+      for (int i = kPer - 1; i >= 0; --i)
+        if (((plain >> i) & 1u) && y.value(i) == top) j = i;
+      better(top, lo + top_piece * kPer + j);
+    }
+    for (int t = lo + pieces * kPer + tid; t < hi; t += kRuleThreads) {
+      const bool allowed = !mask || ((uint32_t(mask[t >> 5]) >> (t & 31)) & 1u);
+      if (ids) {
+        if (allowed && !(named && counts.get(t - lo))) better(rule_logit<F32>(in, t), t);
+      } else if (!allowed) {
+        rule_store<F32>(out, t, -INFINITY);
+      } else if (!in_place) {
+        rule_store<F32>(out, t, rule_logit<F32>(in, t));
+      }
+    }
+    if (named) {
+      __syncthreads();
+      if (!ids) named_tokens(lo, hi);        // over what the pass has written
+      __syncthreads();
+    }
+  }
+  if (!ids) return;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float v = __shfl_xor_sync(0xffffffffu, best, o);
@@ -193,44 +345,54 @@ __global__ void __launch_bounds__(kRuleThreads) logit_rules_kernel(const NkbLogi
     s_at[tid >> 5] = at;
   }
   __syncthreads();
+  if (joined) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   if (tid == 0) {
     for (int w = 1; w < kRuleThreads / 32; ++w) better(s_best[w], s_at[w]);
-    s_mine = make_int2(__float_as_int(best), at);
+    if (joined)
+      asm volatile("st.shared::cluster.v2.s32 [%0], {%1, %2};" ::"r"(map_to_cta(&s_slices[blockIdx.x], 0)), "r"(__float_as_int(best)), "r"(at)
+                   : "memory");
   }
-  if (gridDim.x > 1) {
-    cluster_sync_all();
-    if (blockIdx.x == 0 && tid == 0)
-      for (unsigned c = 1; c < gridDim.x; ++c) {
-        int v, i;
-        asm volatile("ld.shared::cluster.v2.s32 {%0, %1}, [%2];" : "=r"(v), "=r"(i) : "r"(map_to_cta(&s_mine, c)) : "memory");
-        better(__int_as_float(v), i);
-      }
-    cluster_sync_all();               // shared memory stays until it has been read
+  if (joined) {
+    // the first CTA's shared memory has every slice's best once all have arrived; the others have nothing that anyone reads, and may leave
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    if (blockIdx.x != 0) return;
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (tid == 0)
+      for (unsigned c = 1; c < gridDim.x; ++c) better(__int_as_float(s_slices[c].x), s_slices[c].y);
   }
   if (blockIdx.x == 0 && tid == 0) a.out_ids[row] = best == -INFINITY ? -1 : at;
 }
 
-template <bool F32, bool VEC>
+template <bool F32, bool VEC, bool WIDE>
 static int launch_rules(const NkbLogitRules& a) {
-  // slices: a cluster of up to eight where ids are wanted, otherwise as many as give every SM some two CTAs
-  int slices = (2 * num_sms() + a.rows - 1) / a.rows;
-  if (a.out_ids && slices > 8) slices = 8;
-  int fewest = (a.vocab + kSliceMost - 1) / kSliceMost;         // (a slice that has more runs in several turns)
-  if (a.out_ids && fewest > 8) fewest = 8;
-  if (slices < fewest) slices = fewest;
-  int slice = ((a.vocab + slices - 1) / slices + 511) / 512 * 512;
+  // Slices of a row: as few rounds of two CTAs per SM as may be, a round's time being some 3 us for every turn of counting and its logits at
+  // an SM's share of the memory's rate; at most eight where a cluster joins them.
+  const int slots = 2 * num_sms(), most = a.out_ids ? 8 : slots;
+  constexpr int kStep = 512;
+  int slices = 1;
+  double best = 0.0;
+  for (int s = 1; s <= most && (s == 1 || a.vocab > (s - 1) * kStep); ++s) {
+    const double each = (double(a.vocab) + s - 1) / s;
+    const double turns = double(int(each / Counts<WIDE>::kTokens) + 1), rounds = double(((long long)a.rows * s + slots - 1) / slots);
+    const double us = rounds * (3.0 * turns + each * (F32 ? 4 : 2) * (a.out ? 2 : 1) / 22e3);
+    if (s == 1 || us < best) {
+      best = us;
+      slices = s;
+    }
+  }
+  const int slice = ((a.vocab + slices - 1) / slices + kStep - 1) / kStep * kStep;
   slices = (a.vocab + slice - 1) / slice;
-  const int smem = (slice < kSliceMost ? slice : kSliceMost) * 4;
+  const int bytes = slice * (WIDE ? 4 : 2), smem = bytes < kCountBytes ? bytes : kCountBytes;
   constexpr int kMaxDev = 64;
   static bool ready[kMaxDev] = {false};
   int dev = -1;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDev) return -1;
   if (!ready[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(logit_rules_kernel<F32, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSliceMost * 4);
+    const cudaError_t e = cudaFuncSetAttribute(logit_rules_kernel<F32, VEC, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kCountBytes);
     if (e != cudaSuccess) return int(e);
     ready[dev] = true;
   }
-  return launch_pdl_cluster(logit_rules_kernel<F32, VEC>, dim3(unsigned(slices), unsigned(a.rows)), dim3(kRuleThreads), size_t(smem),
+  return launch_pdl_cluster(logit_rules_kernel<F32, VEC, WIDE>, dim3(unsigned(slices), unsigned(a.rows)), dim3(kRuleThreads), size_t(smem),
                             reinterpret_cast<cudaStream_t>(a.stream), a.out_ids ? slices : 1, a, slice);
 }
 
@@ -244,8 +406,16 @@ extern "C" int nkb_logit_rules(const void* packed) {
   if (a.rows <= 0) return 0;
   if (a.vocab <= 0 || a.rows > 65535 || (!a.out && !a.out_ids) || a.biases < 0 || a.width < 0) return -2;
   if (a.tokens && !a.lens) return -2;
+  if (a.out && a.out_ids) return -2;
   const uintptr_t at = reinterpret_cast<uintptr_t>(a.logits) | reinterpret_cast<uintptr_t>(a.out);
   const bool vec = (at & 15) == 0 && ((a.ld | (a.out ? a.out_ld : 0)) & (a.fp32 ? 3 : 7)) == 0;
-  if (a.fp32) return vec ? launch_rules<true, true>(a) : launch_rules<true, false>(a);
-  return vec ? launch_rules<false, true>(a) : launch_rules<false, false>(a);
+  const bool wide = a.width > int(Counts<false>::kTimes);
+  auto go = [&](auto f32, auto v) {
+    constexpr bool F = decltype(f32)::value, V = decltype(v)::value;
+    return wide ? launch_rules<F, V, true>(a) : launch_rules<F, V, false>(a);
+  };
+  using T = std::true_type;
+  using N = std::false_type;
+  if (a.fp32) return vec ? go(T{}, T{}) : go(T{}, N{});
+  return vec ? go(N{}, T{}) : go(N{}, N{});
 }

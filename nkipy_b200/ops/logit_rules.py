@@ -66,11 +66,12 @@ def pack_mask(allowed: torch.Tensor) -> torch.Tensor:
 def _vector(t, name, dtype, rows, index):
     if t is None:
         return 0
+    if t.dtype is dtype and t.shape == (rows,) and t.get_device() == index and t.is_contiguous():
+        return t.data_ptr()
     if t.dtype is not dtype:
         raise TypeError(f"{name} wants {dtype}, not {t.dtype}")
     if t.shape != (rows,) or t.get_device() != index or not t.is_contiguous():
         raise ValueError(f"{name} wants to be contiguous [{rows}], on the logits' device")
-    return t.data_ptr()
 
 
 def _matrix(t, name, dtype, rows, index):
@@ -165,7 +166,7 @@ def apply_rules(logits: torch.Tensor, rules: LogitRules, out: Optional[torch.Ten
     """The logits [rows, vocab] (bf16 or fp32) under the rules, in their type.  out: where they go; the logits themselves, whose
     untouched pieces are not even read then, or apart from them."""
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        out = torch.empty_strided(logits.shape, (logits.shape[-1], 1), dtype=logits.dtype, device=logits.device) if logits.dim() == 2 else logits
     args = _packed(logits, rules, out, None)
     if not logits.shape[0]:
         return out
@@ -181,7 +182,7 @@ def apply_rules(logits: torch.Tensor, rules: LogitRules, out: Optional[torch.Ten
 def argmax(logits: torch.Tensor, rules: LogitRules, out_ids: Optional[torch.Tensor] = None) -> torch.Tensor:
     """int32 [rows]: the first of the largest values that the rules leave, as 32 bits hold them; -1 where none is above minus infinity."""
     if out_ids is None:
-        out_ids = torch.empty((logits.shape[0],), dtype=torch.int32, device=logits.device)
+        out_ids = torch.empty_strided((logits.shape[0],), (1,), dtype=torch.int32, device=logits.device)
     args = _packed(logits, rules, None, out_ids)
     if not logits.shape[0]:
         return out_ids

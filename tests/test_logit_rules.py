@@ -155,6 +155,16 @@ def test_many_rows_over_several_turns():
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("width,V,spread", [(4500, 5000, 1), (9001, 3001, 1), (20000, 700, 1), (20000, 40000, 30)])
+def test_long_lists(device, width, V, spread):
+    """More named tokens than a list holds, and more occurrences than half a word counts."""
+    r = make(width, 2, V, width=width, lens=[width, width - 3], biases=2, masks="rows" if spread == 1 else None)
+    g = torch.Generator().manual_seed(5)
+    r["tokens"] = (V * torch.rand((2, width), generator=g) ** spread).int().clamp(max=V - 1)
+    check(logits_of(width, 2, V, BF), r, device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_without_rules(device):
     x = logits_of(0, 3, 1000, BF)
     check(x, {}, device)
@@ -188,6 +198,17 @@ def test_ties_infinities_and_nan(device, dtype):
     x[3, 10] = 0
     allowed[3, 11] = False
     assert ops.argmax(x.to(device), rules=ops.LogitRules(mask=ops.pack_mask(allowed).to(device))).tolist()[3] == V - 1
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_ties_of_named_and_other_tokens(device):
+    """A bias lifts a token to a value that others have, on either side of it and in the same piece of eight."""
+    V = 100
+    for at, others, want in ((18, [21, 40], 18), (18, [17, 40], 17), (90, [5], 5), (0, [1], 0), (15, [16], 15), (16, [15], 15)):
+        x = torch.zeros((1, V))
+        x[0, others] = 2.0
+        rules = ops.LogitRules(bias_ids=torch.tensor([[at]]).int().to(device), bias_values=torch.tensor([[2.0]]).to(device))
+        assert ops.argmax(x.to(device), rules=rules).tolist() == [want]
 
 
 @pytest.mark.parametrize("device", DEVICES)
