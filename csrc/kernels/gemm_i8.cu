@@ -47,27 +47,37 @@ __host__ __device__ constexpr uint32_t make_idesc_i8(int m, int n) {
 
 __device__ __forceinline__ int4 ld_cluster_v4(uint32_t addr) {
   int4 v;
-  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
   return v;
 }
 
-struct I8Args {               // <= 128 bytes (see GemmArgs)
-  int m, n, k;                // tokens, features
-  int kb_total, stages;
-  int splits, kb_per_split;
-  int gate_off;               // row offset of the up half of w
-  int act;
-  int fp32;
-  int join;                   // swap: the CTAs of a cluster (as many as splits) join their sums; otherwise splits leave partial sums
-  int static_w;
-  int tiles_m, tiles_n, tile_n, group_m;   // pairs
-  long long ldo, split_stride;
+// (Argument blocks: small ones, see GemmArgs.)
+struct I8Out {                // what the epilogues write
+  int m, n;                   // tokens, features; the up half of w and its scales begin at n
+  int act, fp32;
+  long long ldo;
   void* out;
   const float *sx, *sw;
   const __nv_bfloat16 *bias, *residual;
+};
+struct I8SwapArgs {
+  I8Out o;
+  int kb_total, kb_per_split, splits, stages;
+  int join;                   // the CTAs of a cluster (as many as splits) join their sums; otherwise splits leave partial sums
+  int static_w;
+  long long split_stride;
   int* status;
 };
-static_assert(sizeof(I8Args) <= 128, "I8Args grew past the fast kernel-parameter size");
+struct I8PairArgs {
+  I8Out o;
+  int kb_total, stages;
+  int tiles_m, tiles_n, tile_n, group_m;
+  int splits, kb_per_split;   // more than one: partial sums in 32 bits, split s at o.out + s * split_stride
+  int static_w, gated;
+  long long split_stride;
+  int* status;
+};
+static_assert(sizeof(I8SwapArgs) <= 112 && sizeof(I8PairArgs) <= 128, "argument blocks grew past the fast kernel-parameter size");
 
 __device__ __forceinline__ float gate_act(float g, int act) { return act ? gelu_tanh_f(g) : silu_f(g); }
 
@@ -80,27 +90,50 @@ struct I8Ctrl {
   int abort;
 };
 
-// Four finished features (whole sums s, up half u) of one token, from feature f on.
+// Scales and bias of the four features from f on (those past the last one read its); they stay with a thread for all of its tokens.
 template <bool GATED>
-__device__ __forceinline__ void i8_store4(const I8Args& a, int split, int tok, int f, const int4& s, const int4& u) {
+struct Features4 {
+  float sw[4], su[4], bias[4];
+  __device__ __forceinline__ Features4(const I8Out& a, bool first, int f) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int fj = min(f + j, a.n - 1);
+      sw[j] = __ldg(a.sw + fj);
+      su[j] = GATED ? __ldg(a.sw + a.n + fj) : 0.f;
+      bias[j] = !GATED && a.bias && first ? __bfloat162float(a.bias[fj]) : 0.f;
+    }
+  }
+};
+
+// Four finished features (whole sums s, up half u) of one token, from feature f on; at: where the results begin.
+template <bool GATED>
+__device__ __forceinline__ void i8_store4(const I8Out& a, const Features4<GATED>& w, long long at, int tok, int f, const int4& s, const int4& u) {
   const float sx = a.sx[tok];
   const int sv[4] = {s.x, s.y, s.z, s.w}, uv[4] = {u.x, u.y, u.z, u.w};
   float y[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int fj = min(f + j, a.n - 1);
-    y[j] = float(sv[j]) * sx * a.sw[fj];
-    if constexpr (GATED) y[j] = gate_act(y[j], a.act) * (float(uv[j]) * sx * a.sw[a.gate_off + fj]);
-    if (!GATED && a.bias && split == 0) y[j] += __bfloat162float(a.bias[fj]);
+    y[j] = float(sv[j]) * sx * w.sw[j];
+    if constexpr (GATED) y[j] = gate_act(y[j], a.act) * (float(uv[j]) * sx * w.su[j]);
+    else if (a.bias) y[j] += w.bias[j];
   }
-  const long long at = (long long)tok * a.ldo + f;
+  at += (long long)tok * a.ldo + f;
+  const bool whole = f + 4 <= a.n;
   if (!GATED && a.residual) {
+    const __nv_bfloat16* r = a.residual + at;
+    if (whole && (reinterpret_cast<uintptr_t>(r) & 7) == 0) {
+      const uint2 v = *reinterpret_cast<const uint2*>(r);
+      const float2 lo = unpack_bf16x2(v.x), hi = unpack_bf16x2(v.y);
+      y[0] += lo.x; y[1] += lo.y; y[2] += hi.x; y[3] += hi.y;
+    } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] += __bfloat162float(a.residual[at + min(j, a.n - 1 - f)]);
+      for (int j = 0; j < 4; ++j)
+        if (f + j < a.n) y[j] += __bfloat162float(r[j]);
+    }
   }
   if (a.fp32) {
-    float* o = reinterpret_cast<float*>(a.out) + split * a.split_stride + at;
-    if (f + 4 <= a.n && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
+    float* o = reinterpret_cast<float*>(a.out) + at;
+    if (whole && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
       *reinterpret_cast<float4*>(o) = make_float4(y[0], y[1], y[2], y[3]);
     } else {
 #pragma unroll
@@ -109,7 +142,7 @@ __device__ __forceinline__ void i8_store4(const I8Args& a, int split, int tok, i
     }
   } else {
     __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(a.out) + at;
-    if (f + 4 <= a.n && (reinterpret_cast<uintptr_t>(o) & 7) == 0) {
+    if (whole && (reinterpret_cast<uintptr_t>(o) & 7) == 0) {
       *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
     } else {
 #pragma unroll
@@ -122,7 +155,7 @@ __device__ __forceinline__ void i8_store4(const I8Args& a, int split, int tok, i
 // Grid: x = feature tiles * splits (the splits of a tile follow one another; joined ones are a cluster), y = token tiles of BN.
 template <int BN, bool GATED>
 __global__ void __launch_bounds__(128)
-i8_swap_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const I8Args args) {
+i8_swap_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const I8SwapArgs args) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ I8Ctrl ctrl;
@@ -163,7 +196,7 @@ i8_swap_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ 
       auto load_w = [&](int stage, int kb) {
         uint8_t* p = tiles + stage * kStage;
         tma_load_2d(p, &tmW, &ctrl.full[stage], kb * kI8Slab, f0);
-        if (GATED) tma_load_2d(p + kI8ATile, &tmW, &ctrl.full[stage], kb * kI8Slab, args.gate_off + f0);
+        if (GATED) tma_load_2d(p + kI8ATile, &tmW, &ctrl.full[stage], kb * kI8Slab, args.o.n + f0);
       };
       auto load_x = [&](int stage, int kb) {
         tma_load_2d(tiles + stage * kStage + kW * kI8ATile, &tmX, &ctrl.full[stage], kb * kI8Slab, tok0);
@@ -193,17 +226,19 @@ i8_swap_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ 
     if (elect_one()) {
       int stage = 0;
       uint32_t phase = 0;
+      const uint64_t d_tiles = make_smem_desc_sw128(smem_u32(tiles), 0, 1024);
+      const uint64_t d_hi = d_tiles & 0xffffffff00000000ull;
+      const uint32_t w_lo0 = uint32_t(d_tiles);
       bool ok = true;
-      for (int i = 0; i < slabs && ok; ++i) {
+      for (int kb = kb0; kb < kb1; ++kb) {
         ok = mbar_wait(&ctrl.full[stage], phase, abort_flag, args.status, ERR_WAIT_SMEM_FULL);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t w = smem_u32(tiles + stage * kStage);
-        const uint64_t dw = make_smem_desc_sw128(w, 0, 1024), du = make_smem_desc_sw128(w + kI8ATile, 0, 1024);
-        const uint64_t dx = make_smem_desc_sw128(w + kW * kI8ATile, 0, 1024);
+        const uint32_t w_lo = w_lo0 + uint32_t(stage) * uint32_t(kStage >> 4);
+        const uint64_t dw = d_hi | w_lo, du = d_hi | (w_lo + uint32_t(kI8ATile >> 4)), dx = d_hi | (w_lo + uint32_t(kW * kI8ATile >> 4));
 #pragma unroll
         for (int k = 0; k < 4; ++k) {          // 32 numbers per instruction
-          const uint32_t acc = (i > 0 || k > 0) ? 1u : 0u;
+          const uint32_t acc = (kb > kb0 || k > 0) ? 1u : 0u;
           umma_i8(tmem_base, dw + uint64_t(2 * k), dx + uint64_t(2 * k), idesc, acc);
           if (GATED) umma_i8(tmem_base + BN, du + uint64_t(2 * k), dx + uint64_t(2 * k), idesc, acc);
         }
@@ -236,29 +271,41 @@ i8_swap_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ 
   ok = __syncthreads_and(ok);
   if (joined > 1) cluster_sync_all();            // (a CTA that gave up takes part too)
   if (ok) {
-    const int toks = min(BN, args.m - tok0), groups = toks * 32;         // pieces of four features
-    const int share = (groups + joined - 1) / joined, rank = joined > 1 ? split : 0;
-    const int g1 = min(groups, (rank + 1) * share);
-    for (int g = rank * share + threadIdx.x; g < g1; g += 128) {
-      const int t = g >> 5, f = (g & 31) * 4;
-      if (f0 + f >= args.n) continue;
-      int4 s, u = make_int4(0, 0, 0, 0);
-      const int* p = stg + t * 128 + f;
-      if (joined > 1) {
-        s = make_int4(0, 0, 0, 0);
-        for (int r = 0; r < joined; ++r) {
-          const int4 v = ld_cluster_v4(map_to_cta(p, r));
-          s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
-          if (GATED) {
-            const int4 q = ld_cluster_v4(map_to_cta(p + BN * 128, r));
-            u.x += q.x; u.y += q.y; u.z += q.z; u.w += q.w;
-          }
+    // A lane has four features, a warp goes from token to token; the CTAs of a cluster share the tokens, or the features of fewer tokens than CTAs.
+    const int toks = min(BN, args.o.m - tok0), rank = joined > 1 ? split : 0, f = lane * 4;
+    const bool by_token = toks >= joined;
+    const bool mine = f0 + f < args.o.n && (by_token || lane / (32 / joined) == rank);
+    const int step = by_token ? 4 * joined : 4, first_tok = by_token ? warp * joined + rank : warp;
+    if (mine) {
+      const Features4<GATED> w(args.o, args.join || split == 0, f0 + f);
+      const long long at = args.join ? 0 : split * args.split_stride;
+      for (int t = first_tok; t < toks; t += step) {
+        const int* p = stg + t * 128 + f;
+        int4 s, u = make_int4(0, 0, 0, 0);
+        if (joined > 1) {
+          int4 v[8], q[GATED ? 8 : 1];
+#pragma unroll
+          for (int r = 0; r < 8; ++r)
+            if (r < joined) {
+              v[r] = ld_cluster_v4(map_to_cta(p, r));
+              if (GATED) q[r] = ld_cluster_v4(map_to_cta(p + BN * 128, r));
+            }
+          s = v[0];
+          if (GATED) u = q[0];
+#pragma unroll
+          for (int r = 1; r < 8; ++r)
+            if (r < joined) {
+              s.x += v[r].x; s.y += v[r].y; s.z += v[r].z; s.w += v[r].w;
+              if (GATED) {
+                u.x += q[r].x; u.y += q[r].y; u.z += q[r].z; u.w += q[r].w;
+              }
+            }
+        } else {
+          s = *reinterpret_cast<const int4*>(p);
+          if (GATED) u = *reinterpret_cast<const int4*>(p + BN * 128);
         }
-      } else {
-        s = *reinterpret_cast<const int4*>(p);
-        if (GATED) u = *reinterpret_cast<const int4*>(p + BN * 128);
+        i8_store4<GATED>(args.o, w, at, tok0 + t, f0 + f, s, u);
       }
-      i8_store4<GATED>(args, args.join ? 0 : split, tok0 + t, f0 + f, s, u);
     }
   }
   if (joined > 1) cluster_sync_all();            // shared memory stays until every CTA of the cluster has read it
@@ -278,51 +325,42 @@ constexpr int kPairTileN = 256;
 constexpr int kPairStage = 2 * kI8ATile;
 
 struct WorkI8 {
-  int tm, tn;
+  int tm, tn, sp, kb0, kb1;
 };
-// group_m row tiles share a sweep over the column tiles so that tiles of both operands are read again from L2
-__device__ __forceinline__ WorkI8 i8_work(const I8Args& a, int t) {
+// group_m row tiles share a sweep over the column tiles, so that both operands are read again from L2; the splits of a tile follow one another.
+//
+// The slabs' bounds come from the split even where there is one.  With a loop from zero to a kernel argument nvcc 12.9 no longer keeps the operands of the
+// MMAs in uniform registers: an MMA then takes 65 cycles to issue and not 16, and 200 tokens by 4096 x 14336 40 us and not 25.
+__device__ __forceinline__ WorkI8 i8_work(const I8PairArgs& a, int w) {
+  WorkI8 o;
+  o.sp = w % a.splits;
+  const int t = w / a.splits;
   const int per_group = a.group_m * a.tiles_n;
   const int gr = t / per_group, first = gr * a.group_m;
   const int gsz = min(a.tiles_m - first, a.group_m), in = t - gr * per_group;
-  return {first + in % gsz, in / gsz};
+  o.tm = first + in % gsz;
+  o.tn = in / gsz;
+  o.kb0 = o.sp * a.kb_per_split;
+  o.kb1 = min(a.kb_total, o.kb0 + a.kb_per_split);
+  return o;
 }
 
-// 32 finished columns of a row from column c on, cols_end at most; y in fp32.
+// 32 finished columns of a row from column c on, cols_end at most; at: where the results begin.
 template <bool GATED>
-__device__ __forceinline__ void i8_store_row(const I8Args& a, int row, int c, int cols_end, float (&y)[32]) {
-  const long long at = (long long)row * a.ldo + c;
-  const bool whole = c + 32 <= cols_end;
-  if (!GATED && a.bias) {
+__device__ __forceinline__ void i8_store_row(const I8Out& a, bool first, long long at, int row, int c, int cols_end, float (&y)[32]) {
+  at += (long long)row * a.ldo + c;
+  if (!GATED && a.bias && first) {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
-      if (whole || c + j < cols_end) y[j] += __bfloat162float(a.bias[c + j]);
+      if (c + j < cols_end) y[j] += __bfloat162float(__ldg(a.bias + c + j));
   }
-  if (a.fp32) {
-    float* o = reinterpret_cast<float*>(a.out) + at;
-    if (!GATED && a.residual) {
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (whole || c + j < cols_end) y[j] += __bfloat162float(a.residual[at + j]);
-    }
-    if (whole && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        reinterpret_cast<float4*>(o)[j] = make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (c + j < cols_end) o[j] = y[j];
-    }
-    return;
-  }
-  __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(a.out) + at;
-  const bool r16 = !GATED && a.residual && (reinterpret_cast<uintptr_t>(a.residual + at) & 15) == 0;
-  if (whole && (reinterpret_cast<uintptr_t>(o) & 15) == 0 && (GATED || !a.residual || r16)) {
+  if (!GATED && a.residual) {
+    const __nv_bfloat16* r = a.residual + at;
+    const bool r16 = (reinterpret_cast<uintptr_t>(r) & 15) == 0;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      if (!GATED && a.residual) {
-        const uint4 rr = reinterpret_cast<const uint4*>(a.residual + at)[q];
+      if (r16 && c + 8 * q + 8 <= cols_end) {
+        const uint4 rr = reinterpret_cast<const uint4*>(r)[q];
         const uint32_t rw[4] = {rr.x, rr.y, rr.z, rr.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -330,40 +368,63 @@ __device__ __forceinline__ void i8_store_row(const I8Args& a, int row, int c, in
           y[8 * q + 2 * e] += f.x;
           y[8 * q + 2 * e + 1] += f.y;
         }
+      } else {
+#pragma unroll
+        for (int j = 8 * q; j < 8 * q + 8; ++j)
+          if (c + j < cols_end) y[j] += __bfloat162float(r[j]);
       }
+    }
+  }
+  if (a.fp32) {
+    float* o = reinterpret_cast<float*>(a.out) + at;
+    const bool o16 = (reinterpret_cast<uintptr_t>(o) & 15) == 0;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      if (o16 && c + 4 * q + 4 <= cols_end) {
+        reinterpret_cast<float4*>(o)[q] = make_float4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
+      } else {
+#pragma unroll
+        for (int j = 4 * q; j < 4 * q + 4; ++j)
+          if (c + j < cols_end) o[j] = y[j];
+      }
+    }
+    return;
+  }
+  __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(a.out) + at;
+  const bool o16 = (reinterpret_cast<uintptr_t>(o) & 15) == 0;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if (o16 && c + 8 * q + 8 <= cols_end) {
       reinterpret_cast<uint4*>(o)[q] = make_uint4(pack_bf16x2(y[8 * q], y[8 * q + 1]), pack_bf16x2(y[8 * q + 2], y[8 * q + 3]),
                                                   pack_bf16x2(y[8 * q + 4], y[8 * q + 5]), pack_bf16x2(y[8 * q + 6], y[8 * q + 7]));
-    }
-  } else {
+    } else {
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (c + j < cols_end) {
-        if (!GATED && a.residual) y[j] += __bfloat162float(a.residual[at + j]);
-        o[j] = __float2bfloat16(y[j]);
-      }
+      for (int j = 8 * q; j < 8 * q + 8; ++j)
+        if (c + j < cols_end) o[j] = __float2bfloat16(y[j]);
+    }
   }
 }
 
-// y[j] = v[j] * sx * sw[c + j]; columns from cols_end on read the last scale.
+// y[j] = v[j] * sx * sw[c + j]; columns from cols_end on may get anything.
 __device__ __forceinline__ void i8_scale_row(const uint32_t (&v)[32], float sx, const float* sw, int c, int cols_end, float (&y)[32]) {
-  if (c + 32 <= cols_end && (reinterpret_cast<uintptr_t>(sw + c) & 15) == 0) {
+  const bool s16 = (reinterpret_cast<uintptr_t>(sw + c) & 15) == 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float4 s = __ldg(reinterpret_cast<const float4*>(sw + c) + j);
-      y[4 * j] = float(int(v[4 * j])) * sx * s.x;
-      y[4 * j + 1] = float(int(v[4 * j + 1])) * sx * s.y;
-      y[4 * j + 2] = float(int(v[4 * j + 2])) * sx * s.z;
-      y[4 * j + 3] = float(int(v[4 * j + 3])) * sx * s.w;
+  for (int q = 0; q < 8; ++q) {
+    float s[4];
+    if (s16 && c + 4 * q + 4 <= cols_end) {
+      const float4 f = __ldg(reinterpret_cast<const float4*>(sw + c) + q);
+      s[0] = f.x; s[1] = f.y; s[2] = f.z; s[3] = f.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[j] = __ldg(sw + min(c + 4 * q + j, cols_end - 1));
     }
-  } else {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) y[j] = float(int(v[j])) * sx * __ldg(sw + min(c + j, cols_end - 1));
+    for (int j = 0; j < 4; ++j) y[4 * q + j] = float(int(v[4 * q + j])) * sx * s[j];
   }
 }
 
 template <bool GATED>
-__global__ void __launch_bounds__(kGemmThreads, 1)
-i8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const I8Args args) {
+__device__ __forceinline__ void i8_pair_body(const CUtensorMap& tmX, const CUtensorMap& tmW, const I8PairArgs& args) {
   extern __shared__ uint8_t smem_raw[];
   // identical layout in both CTAs: [control 1 KB][ring]
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -373,8 +434,8 @@ i8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
   const int lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();        // 0 = issues the MMAs
   const int stages = args.stages;
-  constexpr uint32_t tmem_cols = 2 * kPairTileN;
-  const int tile_n = args.tile_n, half_n = tile_n / 2;     // half_n: rows of w per CTA
+  constexpr uint32_t tmem_cols = 2 * kPairTileN;     // two accumulators of 256 columns
+  const int tile_n = args.tile_n, half_n = tile_n / 2;     // half_n: rows of B per CTA
   const uint32_t stage_tx = 2u * uint32_t(kI8ATile + half_n * kI8Slab);
 
   if (threadIdx.x == 0) {
@@ -402,23 +463,27 @@ i8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
   tc_fence_after();
   const uint32_t tmem_base = ctrl->tmem_base;
   volatile int* abort_flag = &ctrl->abort;
+
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
-  const int total = args.tiles_m * args.tiles_n;
+  const int total_work = args.tiles_m * args.tiles_n * args.splits;
   griddep_launch();
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (both CTAs)
-    auto w_row_of = [&](int tn) {
-      return GATED ? int(rank) * args.gate_off + tn * half_n : tn * tile_n + int(rank) * half_n;
+    auto b_row_of = [&](const WorkI8& t) {
+      return args.gated ? int(rank) * args.o.n + t.tn * half_n : t.tn * tile_n + int(rank) * half_n;
     };
+    // Weight tiles do not depend on the preceding kernel: the first fill of the ring takes them before the wait.  (The second
+    // CTA's bytes may arrive before the first one has announced them: a barrier's phase ends only with the announcement.)
     int pre = 0;
-    if (args.static_w && pair < total) {
+    if (args.static_w && pair < total_work) {
       const WorkI8 t = i8_work(args, pair);
-      pre = min(stages, args.kb_total);
+      pre = min(stages, t.kb1 - t.kb0);
       if (lane == 0)
         for (int i = 0; i < pre; ++i) {
           if (rank == 0) mbar_expect_tx(&ctrl->full[i], stage_tx);
-          tma_load_2d_pair(tiles + i * kPairStage + kI8ATile, &tmW, map_to_cta(&ctrl->full[i], 0), i * kI8Slab, w_row_of(t.tn));
+          tma_load_2d_pair(tiles + i * kPairStage + kI8ATile, &tmW, map_to_cta(&ctrl->full[i], 0), (t.kb0 + i) * kI8Slab,
+                           b_row_of(t));
         }
       __syncwarp();
     }
@@ -426,19 +491,23 @@ i8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
     int stage = 0;
     uint32_t phase = 0;
     bool alive = true;
-    for (int w = pair; w < total && alive; w += npairs) {
+    for (int w = pair; w < total_work && alive; w += npairs) {
       const WorkI8 t = i8_work(args, w);
-      const int x_row = t.tm * 256 + int(rank) * 128, w_row = w_row_of(t.tn);
-      for (int kb = 0; kb < args.kb_total; ++kb) {
+      const int a_row = t.tm * 256 + int(rank) * 128;
+      const int b_row = b_row_of(t);
+      for (int kb = t.kb0; kb < t.kb1; ++kb) {
         bool ok = mbar_wait(&ctrl->empty[stage], phase ^ 1u, abort_flag, args.status, ERR_WAIT_SMEM_EMPTY);
         if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
         if (lane == 0) {
           const uint32_t full0 = map_to_cta(&ctrl->full[stage], 0);
-          uint8_t* p = tiles + stage * kPairStage;
-          const bool ahead = w == pair && kb < pre;
+          uint8_t* a_ptr = tiles + stage * kPairStage;
+          // the first CTA announces the bytes of both CTAs; the second only lets its loads complete there
+          // (its loads of this phase cannot start before the barrier entered the phase: they wait for the
+          // stage to be released, which follows the previous phase's completion)
+          const bool ahead = w == pair && kb - t.kb0 < pre;
           if (rank == 0 && !ahead) mbar_expect_tx(&ctrl->full[stage], stage_tx);
-          tma_load_2d_pair(p, &tmX, full0, kb * kI8Slab, x_row);
-          if (!ahead) tma_load_2d_pair(p + kI8ATile, &tmW, full0, kb * kI8Slab, w_row);
+          tma_load_2d_pair(a_ptr, &tmX, full0, kb * kI8Slab, a_row);
+          if (!ahead) tma_load_2d_pair(a_ptr + kI8ATile, &tmW, full0, kb * kI8Slab, b_row);
         }
         __syncwarp();
         if (++stage == stages) { stage = 0; phase ^= 1u; }
@@ -446,6 +515,8 @@ i8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
     }
   } else if (warp == 1 && rank == 0) {
     // ------------------------------------------------------------------ MMA issuer (first CTA of the pair)
+    // One elected thread runs the whole loop alone: the tensor pipe queues only a few MMAs, so warp votes,
+    // reconvergence and descriptor arithmetic between two k-blocks are time in which it drains.
     const uint32_t idesc = make_idesc_i8(256, tile_n);
     if (elect_one()) {
       int stage = 0;
@@ -457,11 +528,12 @@ i8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
       const uint32_t a_lo0 = uint32_t(d_tiles);
       const uint32_t empty0 = map_to_cta(&ctrl->empty[0], 0), empty1 = map_to_cta(&ctrl->empty[0], 1);
       bool ok = true;
-      for (int w = pair; w < total && ok; w += npairs) {
+      for (int w = pair; w < total_work && ok; w += npairs) {
         ok = mbar_wait(&ctrl->tempty[acc], acc_phase ^ 1u, abort_flag, args.status, ERR_WAIT_TMEM_EMPTY);
         if (!ok) break;
         const uint32_t d0 = tmem_base + uint32_t(acc * kPairTileN);
-        for (int kb = 0; kb < args.kb_total; ++kb) {
+        const WorkI8 t = i8_work(args, w);
+        for (int kb = t.kb0; kb < t.kb1; ++kb) {
           ok = mbar_wait(&ctrl->full[stage], phase, abort_flag, args.status, ERR_WAIT_SMEM_FULL);
           if (!ok) break;
           tc_fence_after();
@@ -469,7 +541,7 @@ i8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
           const uint64_t da = d_hi | a_lo, db = d_hi | (a_lo + uint32_t(kI8ATile >> 4));
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            umma_i8_pair(d0, da + uint64_t(k * 2), db + uint64_t(k * 2), idesc, (kb > 0 || k > 0) ? 1u : 0u);
+            umma_i8_pair(d0, da + uint64_t(k * 2), db + uint64_t(k * 2), idesc, (kb > t.kb0 || k > 0) ? 1u : 0u);
           umma_commit_pair(empty0 + uint32_t(stage) * 8u);
           umma_commit_pair(empty1 + uint32_t(stage) * 8u);
           if (++stage == stages) { stage = 0; phase ^= 1u; }
@@ -488,16 +560,16 @@ i8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
     griddep_wait();
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int w = pair; w < total; w += npairs) {
+    for (int w = pair; w < total_work; w += npairs) {
       const WorkI8 t = i8_work(args, w);
       const int row = t.tm * 256 + int(rank) * 128 + quad * 32 + lane;
-      const float sx = args.sx[min(row, args.m - 1)];
+      const float sx = args.o.sx[min(row, args.o.m - 1)];
       bool ok = mbar_wait(&ctrl->tfull[acc], acc_phase, abort_flag, args.status, ERR_WAIT_TMEM_FULL);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
       const uint32_t t0 = tmem_base + (uint32_t(quad * 32) << 16) + uint32_t(acc * kPairTileN);
       const int width = GATED ? half_n : tile_n;
-      const int col0 = t.tn * width, cols_end = min(args.n, col0 + width);
+      const int col0 = t.tn * width, cols_end = min(args.o.n, col0 + width);
 #pragma unroll 1
       for (int c = 0; c < width; c += 32) {
         float y[32];
@@ -509,9 +581,9 @@ i8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
           tmem_ld_wait();
           if (col0 + c < cols_end) {
             float up[32];
-            i8_scale_row(v, sx, args.sw, col0 + c, cols_end, y);
-            i8_scale_row(u, sx, args.sw + args.gate_off, col0 + c, cols_end, up);
-            if (args.act) {
+            i8_scale_row(v, sx, args.o.sw, col0 + c, cols_end, y);
+            i8_scale_row(u, sx, args.o.sw + args.o.n, col0 + c, cols_end, up);
+            if (args.o.act) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) y[j] = gelu_tanh_f(y[j]) * up[j];
             } else {
@@ -521,14 +593,14 @@ i8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
           }
         } else {
           tmem_ld_wait();
-          if (col0 + c < cols_end) i8_scale_row(v, sx, args.sw, col0 + c, cols_end, y);
+          if (col0 + c < cols_end) i8_scale_row(v, sx, args.o.sw, col0 + c, cols_end, y);
         }
         if (c + 32 >= width) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(map_to_cta(&ctrl->tempty[acc], 0));
         }
-        if (row < args.m && col0 + c < cols_end) i8_store_row<GATED>(args, row, col0 + c, cols_end, y);
+        if (row < args.o.m && col0 + c < cols_end) i8_store_row<GATED>(args.o, t.sp == 0, t.sp * args.split_stride, row, col0 + c, cols_end, y);
       }
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1u;
@@ -547,6 +619,12 @@ i8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
   }
 }
 
+template <bool GATED>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+i8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const I8PairArgs args) {
+  i8_pair_body<GATED>(tmX, tmW, args);
+}
+
 constexpr int kMaxDev = 64;
 
 static int i8_maps(const NkbGemmI8& g, CUtensorMap* x, uint32_t x_box, CUtensorMap* w, uint32_t w_box) {
@@ -557,10 +635,13 @@ static int i8_maps(const NkbGemmI8& g, CUtensorMap* x, uint32_t x_box, CUtensorM
 }
 
 template <int BN, bool GATED>
-static int launch_swap(const NkbGemmI8& g, I8Args a, int join) {
+static int launch_swap(const NkbGemmI8& g, I8SwapArgs a) {
   constexpr int kW = GATED ? 2 : 1, kStage = kW * kI8ATile + BN * kI8Slab, kStaging = kW * BN * 128 * 4;
-  // two CTAs per SM at least where the staging leaves room
-  int stages = (110 * 1024) / kStage;
+  // Two CTAs per SM where a round is all there is; where tiles come in several rounds, four (three of 128 tokens, whose sums are staged in 64 KB), whose
+  // starts and ends lie under one another's loads.  Vocabulary of 128256 x 4096, us: 64 tokens 106 with two per SM and 96 with four, one token 81 and 78.
+  const long long ctas = (long long)((g.n + 127) / 128) * a.splits * ((g.m + BN - 1) / BN);
+  const int ring = ctas <= 2 * num_sms() ? 110 : (BN == 128 ? 75 : 56);
+  int stages = (ring * 1024) / kStage;
   stages = stages > a.kb_per_split ? a.kb_per_split : stages;
   stages = stages < 1 ? 1 : (stages > kMaxStages ? kMaxStages : stages);
   a.stages = stages;
@@ -577,25 +658,69 @@ static int launch_swap(const NkbGemmI8& g, I8Args a, int join) {
   if (i8_maps(g, &tx, BN, &tw, 128)) return -4;
   const dim3 grid(unsigned((g.n + 127) / 128 * a.splits), unsigned((g.m + BN - 1) / BN));
   return launch_pdl_cluster(i8_swap_kernel<BN, GATED>, grid, dim3(128), size_t(smem), reinterpret_cast<cudaStream_t>(g.stream),
-                            join ? a.splits : 1, tw, tx, a);
+                            a.join ? a.splits : 1, tw, tx, a);
+}
+
+// k divided into whole slabs, none of them empty: at most `want` parts.
+template <typename A>
+static void divide(A& a, int want) {
+  want = want < 1 ? 1 : (want > a.kb_total ? a.kb_total : want);
+  a.kb_per_split = (a.kb_total + want - 1) / want;
+  a.splits = (a.kb_total + a.kb_per_split - 1) / a.kb_per_split;
+}
+
+// CTA pairs that can be resident at once on the current device; negative: an error.
+template <bool GATED>
+static int resident_pairs(int dev, cudaLaunchConfig_t cfg) {
+  static int known[kMaxDev] = {0};
+  if (known[dev] == 0) {
+    if (cudaFuncSetAttribute(i8_pair_kernel<GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448) != cudaSuccess) return -1;
+    int n = 0;
+    cfg.gridDim = dim3(2 * (num_sms() / 2));
+    cfg.numAttrs = 1;
+    known[dev] = cudaOccupancyMaxActiveClusters(&n, i8_pair_kernel<GATED>, &cfg) == cudaSuccess && n > 0 ? n : num_sms() / 4;
+  }
+  return known[dev];
+}
+
+// Columns of a tile.  A pair takes its tiles one after another, so a narrower tile wins where it makes the rounds come out even.  us per slab of a tile
+// (measured, 200 tokens by 4096 x 14336): at 256 columns both operands' 32 KB per CTA and slab are what L2 gives an SM (52 bytes per clock), narrower
+// ones wait for the MMAs' and loads' latencies.  414 tokens by 2 x 14336 x 4096, us: 48.6 at 256, 47.1 at 192, 42 at 160, 52.7 at 128; 200 by 4096 x 4096
+// 17.5 at 256, 12.0 at 128, 11.2 at 64; 2048 by 4096 x 14336 79.8 at 256, 92 at 128.
+static int pair_width(int tiles_m, int splits, int slabs, int columns, int pairs, float* us_out) {
+  static const struct { int width; float us; } kSlab[] = {{256, 0.326f}, {224, 0.287f}, {192, 0.250f}, {160, 0.224f}, {128, 0.207f}, {96, 0.200f}, {64, 0.192f}};
+  int best = 256;
+  float best_us = 0.f;
+  for (const auto& t : kSlab) {
+    const long long tiles = (long long)tiles_m * ((columns + t.width - 1) / t.width) * splits;
+    const float us = float((tiles + pairs - 1) / pairs) * float(slabs) * t.us + 4.f + 0.012f * float(t.width);
+    if (t.width == 256 || us < 0.97f * best_us) {
+      best = t.width;
+      best_us = us;
+    }
+  }
+  if (us_out) *us_out = best_us;
+  return best;
 }
 
 template <bool GATED>
-static int launch_i8_pairs(const NkbGemmI8& g, I8Args a, int tile_n) {
-  a.tile_n = tile_n;
-  a.tiles_m = (g.m + 255) / 256;
-  a.tiles_n = GATED ? (g.n + tile_n / 2 - 1) / (tile_n / 2) : (g.n + tile_n - 1) / tile_n;
+static int launch_i8_pairs(const NkbGemmI8& g, const I8Out& o) {
+  I8PairArgs a{};
+  a.o = o;
+  a.kb_total = (g.k + kI8Slab - 1) / kI8Slab;
+  a.static_w = g.static_w;
+  a.gated = GATED;
   a.group_m = 16;
+  a.split_stride = g.split_stride;
+  divide(a, g.splits);
+  a.status = status_word();
+  a.tiles_m = (g.m + 255) / 256;
   a.stages = (232448 - 2048) / kPairStage;
-  const int smem = a.stages * kPairStage + 2048;
-  CUtensorMap tx, tw;
-  if (i8_maps(g, &tx, 128, &tw, uint32_t(tile_n / 2))) return -4;
   int dev = -1;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDev) return -1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2 * (num_sms() / 2));
   cfg.blockDim = dim3(kGemmThreads);
-  cfg.dynamicSmemBytes = size_t(smem);
+  cfg.dynamicSmemBytes = size_t(a.stages * kPairStage + 2048);
   cfg.stream = reinterpret_cast<cudaStream_t>(g.stream);
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -605,59 +730,67 @@ static int launch_i8_pairs(const NkbGemmI8& g, I8Args a, int tile_n) {
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  static int resident[kMaxDev] = {0};
-  if (resident[dev] == 0) {
-    const cudaError_t e = cudaFuncSetAttribute(i8_pair_kernel<GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
-    if (e != cudaSuccess) return int(e);
-    int n = 0;
-    resident[dev] = cudaOccupancyMaxActiveClusters(&n, i8_pair_kernel<GATED>, &cfg) == cudaSuccess && n > 0 ? n : num_sms() / 4;
-  }
-  const int total = a.tiles_m * a.tiles_n;
-  cfg.gridDim = dim3(2 * unsigned(resident[dev] < total ? resident[dev] : total));
+  const int pairs = resident_pairs<GATED>(dev, cfg);
+  if (pairs < 0) return -1;
+  const int columns = (GATED ? 2 : 1) * g.n;
+  a.tile_n = pair_width(a.tiles_m, a.splits, a.kb_per_split, columns, pairs, nullptr);
+  a.tiles_n = (columns + a.tile_n - 1) / a.tile_n;
+  if (GATED) a.tiles_n = (g.n + a.tile_n / 2 - 1) / (a.tile_n / 2);
+  CUtensorMap tx, tw;
+  if (i8_maps(g, &tx, 128, &tw, uint32_t(a.tile_n / 2))) return -4;
+  const int total = a.tiles_m * a.tiles_n * a.splits;
+  cfg.gridDim = dim3(2 * unsigned(pairs < total ? pairs : total));
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
   return int(cudaLaunchKernelEx(&cfg, i8_pair_kernel<GATED>, tx, tw, a));
 }
 
-// k divided into whole slabs, none of them empty: at most `want` parts.
-static void divide(I8Args& a, int want) {
-  want = want < 1 ? 1 : (want > a.kb_total ? a.kb_total : want);
-  a.kb_per_split = (a.kb_total + want - 1) / want;
-  a.splits = (a.kb_total + a.kb_per_split - 1) / a.kb_per_split;
-}
-
-// CTAs of a cluster that share a tile's k in the swap kernel: doubled while the grid stays within two CTAs per SM and each keeps four slabs.
+// CTAs of a cluster that share a tile's k in the swap kernel: doubled while the grid stays within two CTAs per SM and each keeps two slabs.
 static int pick_join(int tiles, int kb) {
   int s = 1;
-  while (s < 8 && tiles * s * 2 <= 2 * num_sms() && kb / (s * 2) >= 4) s *= 2;
+  while (s < 8 && tiles * s * 2 <= 2 * num_sms() && kb / (s * 2) >= 2) s *= 2;
   return s;
 }
 
+// Whether pairs take a whole product of more than 32 tokens: the times of both kernels by their models.  That of the swap kernel is a start, an end with its
+// staging (6 us at 64 tokens, 8.3 at 128), and 0.33 us per slab and CTA of an SM.  Swap and pairs, us: 64 tokens by 6144 x 4096 9.9 and 12.0, by 4096 x
+// 14336 14.9 and 25.5, by 2 x 14336 x 4096 30.8 and 32.9, by 2048 x 768 7.5 and 4.8; 128 by 6144 x 4096 13.1 and 12.8, by 4096 x 14336 17.9 and 25.7, by 128256
+// x 4096 121 and 99; 256 by 1500 x 8000 12.3 and 19.9, by 6144 x 4096 19.0 and 13.3.
+static bool pairs_first(const NkbGemmI8& g, int bn, int tiles, int splits) {
+  const int slabs = (g.k + kI8Slab - 1) / kI8Slab, weights = g.gated ? 2 : 1;
+  const long long per_sm = ((long long)tiles * splits + num_sms() - 1) / num_sms();
+  const float swap_us = (bn <= 64 ? 6.f : 8.3f) + 0.33f * float(per_sm) * float((slabs + splits - 1) / splits) * float(weights);
+  float pair_us = 0.f;
+  pair_width((g.m + 255) / 256, 1, slabs, weights * g.n, num_sms() / 2, &pair_us);
+  return pair_us < swap_us;
+}
+
 template <bool GATED>
-static int launch_i8(const NkbGemmI8& g, const I8Args& a0) {
-  I8Args a = a0;
-  if (g.m > 128 && g.splits == 0) {
-    divide(a, 1);
-    return launch_i8_pairs<GATED>(g, a, 256);
-  }
+static int launch_i8(const NkbGemmI8& g, const I8Out& o) {
   const int bn = g.m <= 16 ? 16 : (g.m <= 32 ? 32 : (g.m <= 64 || GATED ? 64 : 128));
-  const int tiles = (g.n + 127) / 128 * ((g.m + bn - 1) / bn);
-  int join = 0;
+  const long long tiles = (long long)((g.n + 127) / 128) * ((g.m + bn - 1) / bn);
+  I8SwapArgs a{};
+  a.o = o;
+  a.kb_total = (g.k + kI8Slab - 1) / kI8Slab;
+  a.split_stride = g.split_stride;
+  a.static_w = g.static_w;
+  a.status = status_word();
   if (g.splits > 0) {
+    if (g.m > 128) return launch_i8_pairs<GATED>(g, o);
     divide(a, g.splits);
   } else {
+    if (tiles > 64 * num_sms()) return launch_i8_pairs<GATED>(g, o);
     // (a cluster wants as many CTAs as it is launched with, and a power of two of them)
-    for (int s = pick_join(tiles, a.kb_total);; s /= 2) {
+    for (int s = pick_join(int(tiles), a.kb_total);; s /= 2) {
       divide(a, s);
       if (a.splits == s) break;
     }
-    join = a.splits > 1;
+    a.join = a.splits > 1;
+    if (g.m > 32 && pairs_first(g, bn, int(tiles), a.splits)) return launch_i8_pairs<GATED>(g, o);
   }
-  a.join = join;
-  if (bn == 16) return launch_swap<16, GATED>(g, a, join);
-  if (bn == 32) return launch_swap<32, GATED>(g, a, join);
-  if (bn == 64) return launch_swap<64, GATED>(g, a, join);
-  if constexpr (!GATED) return launch_swap<128, GATED>(g, a, join);
+  if (bn == 16) return launch_swap<16, GATED>(g, a);
+  if (bn == 32) return launch_swap<32, GATED>(g, a);
+  if (bn == 64) return launch_swap<64, GATED>(g, a);
+  if constexpr (!GATED) return launch_swap<128, GATED>(g, a);
   return -2;
 }
 
@@ -667,7 +800,7 @@ using namespace nkb;
 
 // Splits that a product asked for `splits` of them really has.
 extern "C" int nkb_gemm_i8_splits(int k, int splits) {
-  I8Args a{};
+  I8SwapArgs a{};
   a.kb_total = (k + kI8Slab - 1) / kI8Slab;
   divide(a, splits);
   return a.splits;
@@ -682,20 +815,25 @@ extern "C" int nkb_gemm_i8(const void* packed) {
   if (g.gated && (g.bias || g.residual || g.fp32 || g.splits)) return -2;
   if (g.splits < 0 || (g.splits > 0 && (!g.fp32 || g.residual))) return -2;
   if ((g.n + 127) / 128 > 0x7fffffff / 1024 || (g.m + 15) / 16 > 65535 * 8) return -2;
-  I8Args a{};
-  a.m = g.m; a.n = g.n; a.k = g.k;
-  a.kb_total = (g.k + kI8Slab - 1) / kI8Slab;
-  a.gate_off = g.n;
-  a.act = g.act;
-  a.fp32 = g.fp32;
-  a.static_w = g.static_w;
-  a.ldo = g.ldo;
-  a.split_stride = g.split_stride;
-  a.out = g.out;
-  a.sx = g.x_scale;
-  a.sw = g.w_scale;
-  a.bias = reinterpret_cast<const __nv_bfloat16*>(g.bias);
-  a.residual = reinterpret_cast<const __nv_bfloat16*>(g.residual);
-  a.status = status_word();
-  return g.gated ? launch_i8<true>(g, a) : launch_i8<false>(g, a);
+  I8Out o{};
+  o.m = g.m;
+  o.n = g.n;
+  o.act = g.act;
+  o.fp32 = g.fp32;
+  o.ldo = g.ldo;
+  o.out = g.out;
+  o.sx = g.x_scale;
+  o.sw = g.w_scale;
+  o.bias = reinterpret_cast<const __nv_bfloat16*>(g.bias);
+  o.residual = reinterpret_cast<const __nv_bfloat16*>(g.residual);
+  return g.gated ? launch_i8<true>(g, o) : launch_i8<false>(g, o);
+}
+
+// Rows brought into 8 bits (null: they are), and their product.
+extern "C" int nkb_linear_i8(const void* rows, const void* gemm) {
+  if (rows) {
+    const int rc = nkb_quant_rows(rows);
+    if (rc) return rc;
+  }
+  return nkb_gemm_i8(gemm);
 }

@@ -11,16 +11,30 @@
 //
 // The numbers are thus the same for every order of the sums and every launch shape, and equal those of the CPU.
 //
-// Layout: a block per row, eight neighbouring columns per thread and turn, kept in registers between the pass for the maximum and the one that
-// writes; rows too wide for the registers are computed twice.
+// Layout: a CTA per row, or a cluster where there are few and long ones, whose parts meet through distributed shared memory; eight neighbouring
+// columns per thread and turn, kept in registers between the pass for the maximum and the one that writes; rows too wide for them are
+// computed twice.
 #include "api.h"
 #include "common.cuh"
 #include "i8_args.h"
 
 namespace nkb {
 
-constexpr float kHalfNear = 1.f / 2048;      // of m: distance from a half below which a gated value is worked out in 64 bits
+// Distance from a whole number beyond which a number is decided exactly: half, less the error of 127 x / m in 32 bits (two roundings, some
+// 2^-16 at 127); for gated rows less 127 times the 2^-20 of a gated value in 32 bits.
+constexpr float kNearHalf = 0.5f - 1.f / (1 << 15), kNearHalfGated = 0.5f - 1.f / 4096;
 constexpr float kGateSmall = 1.f / (1 << 20);   // rows with a smaller maximum are gated in 64 bits: their 32-bit errors are not small beside it
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
 
 __device__ __forceinline__ double gate64(double g, double u, float limit, float alpha) {
   if (limit > 0.f) {
@@ -31,85 +45,177 @@ __device__ __forceinline__ double gate64(double g, double u, float limit, float 
   return g / (1.0 + exp(-g)) * u;
 }
 
-// 8 columns from `c` on of a bf16 row; columns past the width read as zeros.  VEC: rows start on 16 bytes.
+// 8 columns from `c` on of a row, as they lie in memory; columns past the width read as zeros.  VEC: rows start on 16 bytes.  (Through the read-only
+// path: a thread's loads may then go ahead of its stores, which in place follow the loads of the same columns.)
 template <bool VEC>
-__device__ __forceinline__ void load8_bf16(const __nv_bfloat16* row, int c, int width, float (&v)[8]) {
-  if (VEC && c + 8 <= width) {
-    const uint4 r = *reinterpret_cast<const uint4*>(row + c);
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+__device__ __forceinline__ uint4 fetch8_bf16(const void* row, int c, int width) {
+  if (VEC && c + 8 <= width) return __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(row) + c));
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 f = unpack_bf16x2(w[e]);
-      v[2 * e] = f.x;
-      v[2 * e + 1] = f.y;
-    }
+  for (int j = 0; j < 8; ++j)
+    if (c + j < width) w[j >> 1] |= uint32_t(__ldg(reinterpret_cast<const uint16_t*>(row) + c + j)) << (16 * (j & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <bool VEC>
+__device__ __forceinline__ void fetch8_f32(const float* row, int c, int width, uint4 (&r)[2]) {
+  if (VEC && c + 8 <= width) {
+    r[0] = __ldg(reinterpret_cast<const uint4*>(row + c));
+    r[1] = __ldg(reinterpret_cast<const uint4*>(row + c) + 1);
     return;
   }
+  uint32_t w[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = c + j < width ? __bfloat162float(row[c + j]) : 0.f;
+  for (int j = 0; j < 8; ++j) w[j] = c + j < width ? __ldg(reinterpret_cast<const uint32_t*>(row) + c + j) : 0u;
+  r[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  r[1] = make_uint4(w[4], w[5], w[6], w[7]);
+}
+__device__ __forceinline__ void values8_bf16(const uint4& r, float (&v)[8]) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float2 f = unpack_bf16x2(w[e]);
+    v[2 * e] = f.x;
+    v[2 * e + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void values8_f32(const uint4 (&r)[2], float (&v)[8]) {
+  const uint32_t w[8] = {r[0].x, r[0].y, r[0].z, r[0].w, r[1].x, r[1].y, r[1].z, r[1].w};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
+}
+template <bool VEC>
+__device__ __forceinline__ void load8_bf16(const void* row, int c, int width, float (&v)[8]) {
+  values8_bf16(fetch8_bf16<VEC>(row, c, width), v);
 }
 template <bool VEC>
 __device__ __forceinline__ void load8_f32(const float* row, int c, int width, float (&v)[8]) {
-  if (VEC && c + 8 <= width) {
-    const float4 a = reinterpret_cast<const float4*>(row + c)[0], b = reinterpret_cast<const float4*>(row + c)[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = c + j < width ? row[c + j] : 0.f;
+  uint4 r[2];
+  fetch8_f32<VEC>(row, c, width, r);
+  values8_f32(r, v);
 }
 
-// Gate and up of 8 columns, summed in 64 bits.
+// What 8 columns are made of, fetched ahead: bf16 and fp32 rows; norm: x, residual and the norm's weights; gate and up (of the first partial sum).
+template <int FORM>
+struct Raw8 {
+  static constexpr int kN = FORM == NKB_ROW_BF16 ? 1 : FORM == NKB_ROW_NORM ? 3 : FORM == NKB_ROW_GATE_F32 ? 4 : 2;
+  uint4 r[kN];
+};
 template <int FORM, bool VEC>
-__device__ __forceinline__ void load8_gate(const NkbQuantRows& a, long long row, int c, double (&g)[8], double (&u)[8]) {
-  float v[8];
+__device__ __forceinline__ void fetch8(const NkbQuantRows& a, long long row, int c, Raw8<FORM>& o, bool weights) {
+  const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+  const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x) + row * a.x_ld;
+  if constexpr (FORM == NKB_ROW_BF16) {
+    o.r[0] = fetch8_bf16<VEC>(x, c, a.width);
+  } else if constexpr (FORM == NKB_ROW_F32) {
+    fetch8_f32<VEC>(reinterpret_cast<const float*>(a.x) + row * a.x_ld, c, a.width, o.r);
+  } else if constexpr (FORM == NKB_ROW_NORM) {
+    o.r[0] = a.x ? fetch8_bf16<VEC>(x, c, a.width) : none;
+    o.r[1] = a.residual ? fetch8_bf16<VEC>(reinterpret_cast<const __nv_bfloat16*>(a.residual) + row * a.width, c, a.width) : none;
+    if (weights) o.r[2] = fetch8_bf16<VEC>(a.w, c, a.width);        // (a thread's columns are the same in every row)
+  } else if constexpr (FORM == NKB_ROW_GATE_BF16) {
+    o.r[0] = fetch8_bf16<VEC>(x, c, a.width);
+    o.r[1] = fetch8_bf16<VEC>(x + a.width, c, a.width);
+  } else {
+    const float* p = a.partials + row * a.x_ld;
+    uint4 g[2], u[2];
+    fetch8_f32<VEC>(p, c, a.width, g);
+    fetch8_f32<VEC>(p + a.width, c, a.width, u);
+    o.r[0] = g[0];
+    o.r[1] = g[1];
+    o.r[2] = u[0];
+    o.r[3] = u[1];
+  }
+}
+
+// Gate times up of one column in 64 bits.
+template <int FORM>
+__device__ __noinline__ double gate_exact(const NkbQuantRows& a, long long row, int c) {
+  double g = 0.0, u = 0.0;
   if constexpr (FORM == NKB_ROW_GATE_BF16) {
     const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x) + row * a.x_ld;
-    load8_bf16<VEC>(x, c, a.width, v);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) g[j] = v[j];
-    load8_bf16<VEC>(x + a.width, c, a.width, v);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) u[j] = v[j];
+    g = __bfloat162float(x[c]);
+    u = __bfloat162float(x[a.width + c]);
   } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) g[j] = u[j] = 0.0;
     for (int s = 0; s < a.splits; ++s) {
       const float* p = a.partials + s * a.split_stride + row * a.x_ld;
-      load8_f32<VEC>(p, c, a.width, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) g[j] += v[j];
-      load8_f32<VEC>(p + a.width, c, a.width, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) u[j] += v[j];
+      g += p[c];
+      u += p[a.width + c];
     }
   }
   if (a.bias) {
     const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(a.bias);
+    g += __bfloat162float(b[c]);
+    u += __bfloat162float(b[a.width + c]);
+  }
+  return gate64(g, u, a.limit, a.alpha);
+}
+
+// s + e += v, nothing lost: the rounding error of every addition of 32 bits is a number of 32 bits, kept in e.
+__device__ __forceinline__ void add_pair(float& s, float& e, float v) {
+  const float t = s + v, w = t - s;
+  e += (s - (t - w)) + (v - w);
+  s = t;
+}
+
+// Gate and up of 8 columns, each rounded once from its sum (up to the 2^-48 of pairs).
+template <int FORM, bool VEC>
+__device__ __forceinline__ void load8_gate(const NkbQuantRows& a, long long row, int c, const Raw8<FORM>& raw, float (&g)[8], float (&u)[8]) {
+  if constexpr (FORM == NKB_ROW_GATE_BF16) {
+    values8_bf16(raw.r[0], g);
+    values8_bf16(raw.r[1], u);
+    if (!a.bias) return;
+  } else {
+    const uint4 rg[2] = {raw.r[0], raw.r[1]}, ru[2] = {raw.r[2], raw.r[3]};
+    values8_f32(rg, g);
+    values8_f32(ru, u);
+    if (a.splits == 1 && !a.bias) return;
+  }
+  float ge[8], ue[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (c + j >= a.width) continue;
-      g[j] += __bfloat162float(b[c + j]);
-      u[j] += __bfloat162float(b[a.width + c + j]);
+  for (int j = 0; j < 8; ++j) ge[j] = ue[j] = 0.f;
+  if constexpr (FORM == NKB_ROW_GATE_F32) {
+    for (int s = 1; s < a.splits; ++s) {
+      const float* p = a.partials + s * a.split_stride + row * a.x_ld;
+      float v[8], w[8];
+      load8_f32<VEC>(p, c, a.width, v);
+      load8_f32<VEC>(p + a.width, c, a.width, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        add_pair(g[j], ge[j], v[j]);
+        add_pair(u[j], ue[j], w[j]);
+      }
     }
+  }
+  if (a.bias) {
+    const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(a.bias);
+    float v[8];
+    load8_bf16<VEC>(b, c, a.width, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) add_pair(g[j], ge[j], v[j]);
+    load8_bf16<VEC>(b + a.width, c, a.width, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) add_pair(u[j], ue[j], v[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    // (beside an infinite sum the errors are NaN)
+    g[j] = fabsf(g[j]) < INFINITY ? g[j] + ge[j] : g[j];
+    u[j] = fabsf(u[j]) < INFINITY ? u[j] + ue[j] : u[j];
   }
 }
 
 // What the 8 columns from c on are rounded from.  Norm: stores the residual stream, and adds its squares to ss.
 template <int FORM, bool VEC>
-__device__ __forceinline__ void load8(const NkbQuantRows& a, long long row, int c, float (&v)[8], float& ss, bool store) {
+__device__ __forceinline__ void load8(const NkbQuantRows& a, long long row, int c, const Raw8<FORM>& raw, float (&v)[8], float& ss) {
   if constexpr (FORM == NKB_ROW_BF16) {
-    load8_bf16<VEC>(reinterpret_cast<const __nv_bfloat16*>(a.x) + row * a.x_ld, c, a.width, v);
+    values8_bf16(raw.r[0], v);
   } else if constexpr (FORM == NKB_ROW_F32) {
-    load8_f32<VEC>(reinterpret_cast<const float*>(a.x) + row * a.x_ld, c, a.width, v);
+    values8_f32(raw.r, v);
   } else if constexpr (FORM == NKB_ROW_NORM) {
     float r[8], w[8], x[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) r[j] = x[j] = 0.f;
-    if (a.residual) load8_bf16<VEC>(reinterpret_cast<const __nv_bfloat16*>(a.residual) + row * a.width, c, a.width, r);
-    if (a.x) load8_bf16<VEC>(reinterpret_cast<const __nv_bfloat16*>(a.x) + row * a.x_ld, c, a.width, x);
-    load8_bf16<VEC>(reinterpret_cast<const __nv_bfloat16*>(a.w), c, a.width, w);
+    values8_bf16(raw.r[0], x);
+    values8_bf16(raw.r[1], r);
+    values8_bf16(raw.r[2], w);
     if (a.partials || a.bias) {
       // more than two addends: in 64 bits, so that the rounding to bf16 is the one of the sum
       double h[8];
@@ -132,13 +238,20 @@ __device__ __forceinline__ void load8(const NkbQuantRows& a, long long row, int 
     } else {
       // the sum of two bf16 numbers in 32 bits is never a tie of bf16 that the sum itself is not
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = __bfloat162float(__float2bfloat16(x[j] + r[j]));
+      for (int j = 0; j < 8; ++j) x[j] += r[j];
     }
-    if (store && a.residual_out) {
+    uint32_t h[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      h[e] = pack_bf16x2(x[2 * e], x[2 * e + 1]);
+      const float2 f = unpack_bf16x2(h[e]);
+      x[2 * e] = f.x;
+      x[2 * e + 1] = f.y;
+    }
+    if (a.residual_out) {
       __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(a.residual_out) + row * a.width + c;
       if (VEC && c + 8 <= a.width) {
-        *reinterpret_cast<uint4*>(o) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
-                                                  pack_bf16x2(x[6], x[7]));
+        *reinterpret_cast<uint4*>(o) = make_uint4(h[0], h[1], h[2], h[3]);
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -151,179 +264,329 @@ __device__ __forceinline__ void load8(const NkbQuantRows& a, long long row, int 
       v[j] = x[j] * w[j];
     }
   } else {
-    double g[8], u[8];
-    load8_gate<FORM, VEC>(a, row, c, g, u);
+    float g[8], u[8];
+    load8_gate<FORM, VEC>(a, row, c, raw, g, u);
+    if (a.limit > 0.f) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (a.limit > 0.f) {
-        v[j] = float(gate64(g[j], u[j], a.limit, a.alpha));
-      } else {
-        const float gf = float(g[j]);
-        v[j] = gf / (1.f + expf(-gf)) * float(u[j]);
+      for (int j = 0; j < 8; ++j) {
+        const float gl = min_nan(g[j], a.limit), ul = max_nan(min_nan(u[j], a.limit), -a.limit);
+        v[j] = __fdividef((ul + 1.f) * gl, 1.f + expf(-a.alpha * gl));
       }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = g[j] / (1.f + expf(-g[j])) * u[j];
+    }
+    // columns past the width read as zeros
+    if (c + 8 > a.width) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j >= a.width) v[j] = 0.f;
     }
   }
 }
 
-template <int FORM, bool VEC, int IT>
-__global__ void __launch_bounds__(1024) quant_rows_kernel(const NkbQuantRows a) {
-  constexpr bool kGate = FORM == NKB_ROW_GATE_BF16 || FORM == NKB_ROW_GATE_F32;
-  constexpr bool kKeep = IT > 0;
-  __shared__ uint32_t s_top[32];
-  __shared__ float s_ss[32];
-  __shared__ unsigned long long s_top64;
-  const long long row = blockIdx.x;
-  const int chunks = (a.width + 7) / 8, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) s_top64 = 0ull;
-  griddep_wait();
-  griddep_launch();
-  float v[kKeep ? IT : 1][8];
-  uint32_t top = 0;                       // bits of the largest magnitude: infinities and NaN lie above all numbers
-  float ss = 0.f;
-  if constexpr (kKeep) {
-#pragma unroll
-    for (int it = 0; it < IT; ++it) {
-      const int ch = threadIdx.x + it * blockDim.x;
-      if (ch >= chunks) break;
-      load8<FORM, VEC>(a, row, ch * 8, v[it], ss, true);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[it][j]) & 0x7fffffffu);
-    }
-  } else {
-    for (int ch = threadIdx.x; ch < chunks; ch += blockDim.x) {
-      load8<FORM, VEC>(a, row, ch * 8, v[0], ss, true);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[0][j]) & 0x7fffffffu);
-    }
-  }
-  top = __reduce_max_sync(0xffffffffu, top);
-  if constexpr (FORM == NKB_ROW_NORM) ss = warp_sum(ss);
-  if (lane == 0) {
-    s_top[warp] = top;
-    s_ss[warp] = ss;
-  }
-  __syncthreads();
-  const int warps = blockDim.x >> 5;
-  top = __reduce_max_sync(0xffffffffu, lane < warps ? s_top[lane] : 0u);
-  float m = __uint_as_float(top);
-  bool in64 = false;                      // gate: the whole row in 64 bits
-  double m64 = m;
-  if constexpr (kGate) {
-    in64 = a.limit > 0.f || m < kGateSmall;
-    if (top < 0x7f800000u) {
-      // the exact maximum, of the values that may be it
-      const float near = in64 ? 0.f : m * (1.f - 1.f / (1 << 18));
-      double best = 0.0;
-      for (int it = 0;; ++it) {
-        const int ch = threadIdx.x + it * blockDim.x;
-        if (ch >= chunks || (kKeep && it >= IT)) break;
-        float mine = 0.f;
-        if constexpr (kKeep) {
-#pragma unroll
-          for (int i = 0; i < IT; ++i)
-            if (i == it)
-#pragma unroll
-              for (int j = 0; j < 8; ++j) mine = fmaxf(mine, fabsf(v[i][j]));
-        } else {
-          float none = 0.f;
-          load8<FORM, VEC>(a, row, ch * 8, v[0], none, false);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) mine = fmaxf(mine, fabsf(v[0][j]));
-        }
-        if (mine >= near) {
-          double g[8], u[8];
-          load8_gate<FORM, VEC>(a, row, ch * 8, g, u);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) best = fmax(best, fabs(gate64(g[j], u[j], a.limit, a.alpha)));
-        }
-      }
-      if (best > 0.0) atomicMax(&s_top64, (unsigned long long)__double_as_longlong(best));
-      __syncthreads();
-      m64 = __longlong_as_double((long long)s_top64);
-      m = float(m64);
-    }
-  }
-  const bool fine = top < 0x7f800000u;
-  if (threadIdx.x == 0) {
-    float scale = kGate ? float(m64 / 127.0) : m / 127.f;
-    if constexpr (FORM == NKB_ROW_NORM) {
-      float total = 0.f;
-      for (int i = 0; i < warps; ++i) total += s_ss[i];
-      scale *= rsqrtf(total / float(a.width) + a.eps);
-    }
-    a.scale[row] = fine ? scale : __uint_as_float(0x7fffffffu);
-  }
+// The numbers of 8 columns by the exact comparison.  WIDE: x and m have 24 bits, the sides of the comparison 32.
+template <bool WIDE>
+__device__ __noinline__ uint2 exact8(const float (&x)[8], float m) {
   // a power of two that keeps 254 |x| and 127 / m inside the range of 32 bits
   const float f = m < 1e-18f ? 1.1805916207174113e21f : (m > 1e18f ? 8.470329472543003e-22f : 1.f);
   const float mf = m * f, inv = mf > 0.f ? 127.f / mf : 0.f;
+  uint32_t packed[2] = {0u, 0u};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float ax = fabsf(x[j]) * f, k = floorf(ax * inv);
+    bool up;
+    if constexpr (WIDE) {
+      const double l = 254.0 * double(ax), r = (2.0 * double(k) + 1.0) * double(mf);
+      up = l > r || (l == r && (int(k) & 1));
+    } else {
+      const float l = 254.f * ax, r = (2.f * k + 1.f) * mf;
+      up = l > r || (l == r && (int(k) & 1));
+    }
+    const int q = int(k) + (up ? 1 : 0);
+    packed[j >> 2] |= uint32_t((x[j] < 0.f ? -q : q) & 255) << (8 * (j & 3));
+  }
+  return make_uint2(packed[0], packed[1]);
+}
+
+// What a CTA of a cluster tells the others about its part of the row.
+struct RowPart {
+  unsigned long long top64;
+  uint32_t top;
+  float ss;
+};
+
+// Registers of a thread: as few as the chunks that it keeps and has on their way leave room for, since more warps hide more of the loads and barriers.
+constexpr int row_registers(int form, int it) {
+  if (it == 1) return form == NKB_ROW_GATE_F32 ? 128 : 64;
+  if (it == 2) return form <= NKB_ROW_NORM ? 72 : 128;
+  if (it == 4) return form == NKB_ROW_BF16 ? 64 : 128;
+  return 128;
+}
+
+// Grid: a CTA per row, or (CLUSTER) a cluster along x per row y.  IT: chunks of eight columns that a thread keeps, 0: none, they are read twice.
+template <int FORM, bool VEC, int IT, bool CLUSTER>
+__global__ void __maxnreg__(row_registers(FORM, IT)) quant_rows_kernel(const NkbQuantRows a) {
+  constexpr bool kGate = FORM == NKB_ROW_GATE_BF16 || FORM == NKB_ROW_GATE_F32;
+  constexpr bool kKeep = IT > 0;
+  __shared__ uint32_t s_top[2][16];
+  __shared__ float s_ss[2][16];
+  __shared__ unsigned long long s_top64[2];
+  __shared__ RowPart s_part;
+  const int all = (a.width + 7) / 8, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int each = CLUSTER ? (all + gridDim.x - 1) / gridDim.x : all;
+  const int chunk0 = CLUSTER ? blockIdx.x * each : 0, chunks = min(all, chunk0 + each);      // [chunk0, chunks)
+  if (threadIdx.x == 0) s_top64[0] = 0ull;
+  griddep_wait();
+  griddep_launch();
+  Raw8<FORM> raw[kKeep ? IT : 1];
+  auto fetch = [&](long long row, bool first) {
+#pragma unroll
+    for (int it = 0; it < (kKeep ? IT : 0); ++it) {
+      const int ch = chunk0 + threadIdx.x + it * blockDim.x;
+      if (ch < chunks) fetch8<FORM, VEC>(a, row, ch * 8, raw[it], first);
+    }
+  };
+  long long row = CLUSTER ? blockIdx.y : blockIdx.x;
+  fetch(row, true);
+  // (of the shared words one set is filled while the other may still be read: one barrier a row, two of gated ones)
+  for (int turn = 0; row < a.rows; row += CLUSTER ? a.rows : gridDim.x, turn ^= 1) {
+  float v[kKeep ? IT : 1][8];
+  float big = 0.f, ss = 0.f;              // largest magnitude, NaN if there is one
+  if constexpr (kKeep) {
+#pragma unroll
+    for (int it = 0; it < IT; ++it) {
+      const int ch = chunk0 + threadIdx.x + it * blockDim.x;
+      if (ch >= chunks) continue;
+      load8<FORM, VEC>(a, row, ch * 8, raw[it], v[it], ss);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) big = max_nan(big, fabsf(v[it][j]));
+    }
+    // the next row's loads are on their way while this one is finished
+    if (!CLUSTER && row + gridDim.x < a.rows) fetch(row + gridDim.x, false);
+  } else {
+    for (int ch = chunk0 + threadIdx.x; ch < chunks; ch += blockDim.x) {
+      fetch8<FORM, VEC>(a, row, ch * 8, raw[0], true);
+      load8<FORM, VEC>(a, row, ch * 8, raw[0], v[0], ss);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) big = max_nan(big, fabsf(v[0][j]));
+    }
+  }
+  // wide rows: the columns once more.  The residual stream may lie in the place of what it was made of.
+  NkbQuantRows again_a = a;
+  if (!kKeep && FORM == NKB_ROW_NORM && a.residual_out) {
+    again_a.x = a.residual_out;
+    again_a.x_ld = a.width;
+    again_a.residual = again_a.residual_out = nullptr;
+    again_a.partials = nullptr;
+    again_a.bias = nullptr;
+    again_a.splits = 0;
+  }
+  auto once_more = [&](int ch) {
+    float none = 0.f;
+    if constexpr (FORM == NKB_ROW_NORM) {
+      // (written by this thread: not through the read-only path)
+      const __nv_bfloat16* h = reinterpret_cast<const __nv_bfloat16*>(again_a.x) + row * again_a.x_ld;
+      if (a.residual_out) {
+        uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (ch * 8 + j < a.width)
+            w[j >> 1] |= uint32_t(*reinterpret_cast<const volatile uint16_t*>(h + ch * 8 + j)) << (16 * (j & 1));
+        raw[0].r[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        raw[0].r[1] = make_uint4(0u, 0u, 0u, 0u);
+        raw[0].r[2] = fetch8_bf16<VEC>(a.w, ch * 8, a.width);
+        load8<FORM, VEC>(again_a, row, ch * 8, raw[0], v[0], none);
+        return;
+      }
+    }
+    fetch8<FORM, VEC>(again_a, row, ch * 8, raw[0], true);
+    load8<FORM, VEC>(again_a, row, ch * 8, raw[0], v[0], none);
+  };
+  uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(big));      // infinities and NaN lie above all numbers
+  if constexpr (FORM == NKB_ROW_NORM) ss = warp_sum(ss);
+  if (lane == 0) {
+    s_top[turn][warp] = top;
+    s_ss[turn][warp] = ss;
+  }
+  __syncthreads();
+  if (kGate && threadIdx.x == 0) s_top64[turn ^ 1] = 0ull;
+  top = __reduce_max_sync(0xffffffffu, lane < warps ? s_top[turn][lane] : 0u);
+  if constexpr (FORM == NKB_ROW_NORM) ss = warp_sum(lane < warps ? s_ss[turn][lane] : 0.f);
+  auto small = [&](float m) { return m < kGateSmall || m < a.limit * a.limit / 16.f || m > 1e18f; };
+  double m64 = 0.0;
+  if constexpr (kGate) {
+    // the exact maximum of this CTA's columns, of the values that may be it
+    if (top < 0x7f800000u) {
+      const float mine = __uint_as_float(top), near = small(mine) ? 0.f : mine * (1.f - 1.f / (1 << 18));
+      double best = 0.0;
+#pragma unroll
+      for (int it = 0; it < (kKeep ? IT : 1 << 30); ++it) {
+        const int ch = chunk0 + threadIdx.x + it * blockDim.x;
+        if (ch >= chunks) break;
+        if constexpr (!kKeep) once_more(ch);
+        uint32_t some = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) some |= fabsf(v[kKeep ? it : 0][j]) >= near && ch * 8 + j < a.width ? 1u << j : 0u;
+#pragma unroll 1
+        for (; some; some &= some - 1u) best = fmax(best, fabs(gate_exact<FORM>(a, row, ch * 8 + __ffs(some) - 1)));
+      }
+      if (best > 0.0) atomicMax(&s_top64[turn], (unsigned long long)__double_as_longlong(best));
+    }
+    __syncthreads();
+    m64 = __longlong_as_double((long long)s_top64[turn]);
+  }
+  if constexpr (CLUSTER) {
+    if (threadIdx.x == 0) {
+      s_part.top = top;
+      s_part.ss = ss;
+      s_part.top64 = (unsigned long long)__double_as_longlong(m64);
+    }
+    cluster_sync_all();
+    uint32_t t = 0, f = 0;
+    if (lane < int(gridDim.x)) {
+      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(t) : "r"(map_to_cta(&s_part.top, lane)) : "memory");
+      if constexpr (FORM == NKB_ROW_NORM)
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(f) : "r"(map_to_cta(&s_part.ss, lane)) : "memory");
+    }
+    top = __reduce_max_sync(0xffffffffu, t);
+    if constexpr (FORM == NKB_ROW_NORM) ss = warp_sum(__uint_as_float(f));
+    if constexpr (kGate) {
+      unsigned long long o = 0;
+      if (lane < int(gridDim.x))
+        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(o) : "r"(map_to_cta(&s_part.top64, lane)) : "memory");
+      m64 = __longlong_as_double((long long)o);
+#pragma unroll
+      for (int i = 4; i > 0; i >>= 1) m64 = fmax(m64, __shfl_xor_sync(0xffffffffu, m64, i));
+      m64 = __shfl_sync(0xffffffffu, m64, 0);
+    }
+  }
+  const bool fine = top < 0x7f800000u;
+  const bool in64 = kGate && small(__uint_as_float(top));       // the whole row in 64 bits
+  const float m = kGate ? float(m64) : __uint_as_float(top);
+  if (threadIdx.x == 0 && (!CLUSTER || blockIdx.x == 0)) {
+    float scale = kGate ? float(m64 / 127.0) : m / 127.f;
+    if constexpr (FORM == NKB_ROW_NORM) scale *= rsqrtf(ss / float(a.width) + a.eps);
+    a.scale[row] = fine ? scale : __uint_as_float(0x7fffffffu);
+  }
+  // Rows whose m or 127 / m is at an end of the range: every number by the comparison, scaled by a power of two.
+  const bool odd = m < 1e-18f || m > 1e18f;
+  const float inv = odd ? 0.f : 127.f / m;
   uint8_t* out = reinterpret_cast<uint8_t*>(a.values) + row * a.q_ld;
   auto finish = [&](float (&x)[8], int ch) {
     uint32_t packed[2] = {0u, 0u};
-    uint32_t again = 0;                   // columns to be worked out in 64 bits
-    if (fine && !in64) {
+    if (fine) {
+      // 127 x / m + 1.5 * 2^23 rounds to the nearest whole number, whose lowest byte is then that of the sum
+      uint32_t t[8], again = 0;
+      float most = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float ax = fabsf(x[j]) * f;
-        float k = floorf(ax * inv);
-        const float l = 254.f * ax, r = (2.f * k + 1.f) * mf;
-        bool up = l > r || (l == r && (int(k) & 1));
-        if constexpr (FORM == NKB_ROW_F32) {
-          if (fabsf(l - r) <= kHalfNear * mf) {      // 24-bit numbers: the sides have 32 bits
-            const double l64 = 254.0 * double(ax), r64 = (2.0 * double(k) + 1.0) * double(mf);
-            up = l64 > r64 || (l64 == r64 && (int(k) & 1));
+        const float s = fmaf(x[j], inv, 12582912.f);
+        t[j] = __float_as_uint(s);
+        const float d = fabsf(fmaf(x[j], inv, 12582912.f - s));
+        most = fmaxf(most, d);
+        if constexpr (kGate) again |= d > kNearHalfGated ? 1u << j : 0u;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        packed[i] = __byte_perm(__byte_perm(t[4 * i], t[4 * i + 1], 0x0040), __byte_perm(t[4 * i + 2], t[4 * i + 3], 0x0040), 0x5410);
+      if constexpr (kGate) {
+        if (in64) again = m64 > 0.0 ? 255u : 0u;
+        if (again) {
+#pragma unroll 1
+          for (; again; again &= again - 1u) {
+            const int j = __ffs(again) - 1;
+            if (ch * 8 + j >= a.width) break;
+            const double y = gate_exact<FORM>(a, row, ch * 8 + j);
+            const uint32_t q = uint32_t(int(rint(127.0 * (y / m64))) & 255), at = 8 * (j & 3);
+            if (j < 4) packed[0] = (packed[0] & ~(255u << at)) | q << at;
+            else packed[1] = (packed[1] & ~(255u << at)) | q << at;
           }
         }
-        if constexpr (kGate) {
-          if (fabsf(l - r) <= kHalfNear * mf) again |= 1u << j;
-        }
-        const int q = int(k) + (up ? 1 : 0);
-        packed[j >> 2] |= uint32_t((x[j] < 0.f ? -q : q) & 255) << (8 * (j & 3));
-      }
-    }
-    if constexpr (kGate) {
-      if (fine && in64) again = m64 > 0.0 ? 255u : 0u;
-      if (again) {
-        double g[8], u[8];
-        load8_gate<FORM, VEC>(a, row, ch * 8, g, u);
+      } else if (most > kNearHalf || odd) {
+        // (copies: what a call may reach has to lie in memory)
+        float y[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (!((again >> j) & 1)) continue;
-          const double y = gate64(g[j], u[j], a.limit, a.alpha);
-          const int q = int(rint(127.0 * (y / m64)));
-          packed[j >> 2] = (packed[j >> 2] & ~(255u << (8 * (j & 3)))) | uint32_t(q & 255) << (8 * (j & 3));
-        }
+        for (int j = 0; j < 8; ++j) y[j] = x[j];
+        const uint2 p = exact8<FORM == NKB_ROW_F32>(y, m);
+        packed[0] = p.x;
+        packed[1] = p.y;
       }
     }
     *reinterpret_cast<uint2*>(out + ch * 8) = make_uint2(packed[0], packed[1]);
     // (rows end on sixteen bytes)
-    if (ch == chunks - 1 && (chunks & 1)) *reinterpret_cast<uint2*>(out + ch * 8 + 8) = make_uint2(0u, 0u);
+    if (ch == all - 1 && (all & 1)) *reinterpret_cast<uint2*>(out + ch * 8 + 8) = make_uint2(0u, 0u);
   };
   if constexpr (kKeep) {
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
-      const int ch = threadIdx.x + it * blockDim.x;
+      const int ch = chunk0 + threadIdx.x + it * blockDim.x;
       if (ch >= chunks) break;
       finish(v[it], ch);
     }
   } else {
-    for (int ch = threadIdx.x; ch < chunks; ch += blockDim.x) {
-      float none = 0.f;
-      load8<FORM, VEC>(a, row, ch * 8, v[0], none, false);
+    for (int ch = chunk0 + threadIdx.x; ch < chunks; ch += blockDim.x) {
+      once_more(ch);
       finish(v[0], ch);
     }
   }
+  }
+  if constexpr (CLUSTER) cluster_sync_all();        // shared memory stays until every CTA of the cluster has read it
+}
+
+// CTAs of a row: doubled while a row's part stays 1024 columns and all parts have room on the SMs, `per_sm` on each.
+static int row_ctas(int rows, int chunks, int per_sm) {
+  int c = 1;
+  while (c < 8 && chunks > 512 && (long long)rows * c * 2 <= per_sm * num_sms() && chunks / (2 * c) >= 128) c *= 2;
+  return c;
+}
+
+// Blocks of that many threads, IT chunks each, that an SM holds at once.
+template <int FORM, bool VEC, int IT>
+static int resident(unsigned threads) {
+  constexpr int kMaxDev = 64;
+  static int known[kMaxDev][17] = {};
+  int dev = -1, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDev) return 1;
+  int& k = known[dev][threads / 32];
+  if (k == 0) k = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, quant_rows_kernel<FORM, VEC, IT, false>, int(threads), 0) == cudaSuccess && n > 0 ? n : 1;
+  return k;
+}
+
+// Rows for several rounds: a block goes from row to row, its next row's loads on their way while it finishes one, as many blocks as the SMs hold.
+// Fewer rows than that: -5.
+template <int FORM, bool VEC, int IT>
+static int launch_many(const NkbQuantRows& a, int chunks) {
+  const unsigned threads = unsigned(((chunks + IT - 1) / IT + 31) / 32 * 32);
+  if (threads > 512) return -5;
+  const int blocks = num_sms() * resident<FORM, VEC, IT>(threads);
+  if (a.rows < 2 * blocks) return -5;
+  return launch_pdl(quant_rows_kernel<FORM, VEC, IT, false>, dim3(unsigned(blocks)), dim3(threads), 0, reinterpret_cast<cudaStream_t>(a.stream), a);
 }
 
 template <int FORM, bool VEC>
 static int launch_rows(const NkbQuantRows& a) {
   const int chunks = (a.width + 7) / 8;
-  auto go = [&](auto kernel, int threads) {
-    return launch_pdl(kernel, dim3(unsigned(a.rows)), dim3(unsigned(threads)), 0, reinterpret_cast<cudaStream_t>(a.stream), a);
-  };
-  auto warps = [](int n) { return (n + 31) / 32 * 32; };
-  if (chunks <= 1024) return go(quant_rows_kernel<FORM, VEC, 1>, warps(chunks));
-  if (chunks <= 2048) return go(quant_rows_kernel<FORM, VEC, 2>, warps((chunks + 1) / 2));
-  return go(quant_rows_kernel<FORM, VEC, 0>, 1024);
+  auto warps = [](int n) { return unsigned((n + 31) / 32 * 32); };
+  const cudaStream_t stream = reinterpret_cast<cudaStream_t>(a.stream);
+  if constexpr (VEC) {
+    const int c = row_ctas(a.rows, chunks, FORM == NKB_ROW_GATE_F32 ? 1 : 2);
+    if (c > 1) {
+      const int part = (chunks + c - 1) / c;
+      const dim3 grid(unsigned(c), unsigned(a.rows));
+      if (part <= 512) return launch_pdl_cluster(quant_rows_kernel<FORM, VEC, 1, true>, grid, dim3(warps(part)), 0, stream, c, a);
+      if (part <= 1024) return launch_pdl_cluster(quant_rows_kernel<FORM, VEC, 2, true>, grid, dim3(warps((part + 1) / 2)), 0, stream, c, a);
+    }
+  }
+  if (chunks > 32 && chunks <= 2048) {
+    constexpr int kFew = FORM == NKB_ROW_F32 || FORM == NKB_ROW_GATE_F32 ? 2 : 4;
+    int rc = kFew == 2 && chunks <= 1024 ? launch_many<FORM, VEC, kFew>(a, chunks) : launch_many<FORM, VEC, 4>(a, chunks);
+    if (rc != -5) return rc;
+  }
+  const dim3 grid(unsigned(a.rows));
+  if (chunks <= 512) return launch_pdl(quant_rows_kernel<FORM, VEC, 1, false>, grid, dim3(warps(chunks)), 0, stream, a);
+  if (chunks <= 2048) return launch_pdl(quant_rows_kernel<FORM, VEC, 4, false>, grid, dim3(warps((chunks + 3) / 4)), 0, stream, a);
+  return launch_pdl(quant_rows_kernel<FORM, VEC, 0, false>, grid, dim3(512), 0, stream, a);
 }
 
 }  // namespace nkb
@@ -332,6 +595,7 @@ using namespace nkb;
 
 extern "C" int nkb_quant_rows(const void* packed) {
   const NkbQuantRows& a = *reinterpret_cast<const NkbQuantRows*>(packed);
+  if (!status_word() && nkb_init() != 0) return -1;
   if (a.rows <= 0) return 0;
   if (a.width <= 0 || a.splits < 0 || a.q_ld < (a.width + 15) / 16 * 16 || (a.q_ld & 15)) return -2;
   uintptr_t at = reinterpret_cast<uintptr_t>(a.values);

@@ -26,7 +26,6 @@ from . import _lib
 from . import _count_launch, _stream, mixers
 
 MAX_K = 133144                       # 127 * 127 * k stays below 2^31
-_FORMS = {"bf16": 0, "f32": 1, "norm": 2, "gate_bf16": 3, "gate_f32": 4}
 # NkbQuantRows and NkbGemmI8 of csrc/kernels/i8_args.h
 _ROWS, _GEMM = struct.Struct("9P3q4i3fi"), struct.Struct("8P4q8i")
 
@@ -51,6 +50,14 @@ class _Quantized:
         # index: of the CUDA device, -1: the CPU; ld: numbers from one row to the next; at: where values and scales start
         self.values, self.scale, self.shape, self.index, self.device, self.ld = values, scale, shape, index, values.device, ld
         self.at = values.data_ptr(), scale.data_ptr()
+
+    @classmethod
+    def _made(cls, values: torch.Tensor, scale: torch.Tensor, ld: int, index: int):
+        """Of tensors that are known to lie as they should."""
+        self = cls.__new__(cls)
+        self.values, self.scale, self.shape, self.index, self.device, self.ld = values, scale, values.shape, index, values.device, ld
+        self.at = values.data_ptr(), scale.data_ptr()
+        return self
 
     @property
     def is_cuda(self) -> bool:
@@ -94,13 +101,15 @@ def _padded(rows: int, k: int, device) -> torch.Tensor:
     return t[:, :k]
 
 
-def _want(t: torch.Tensor, name: str, dtypes, shape, index: int) -> None:
-    if t.dtype not in dtypes:
-        raise TypeError(f"{name} wants {' or '.join(map(str, dtypes))}, not {t.dtype}")
+def _want(t: torch.Tensor, name: str, dtype, shape, index: int) -> int:
+    """Address of a contiguous tensor of this type and shape on device `index`."""
+    if t.dtype is dtype and t.shape == shape and t.get_device() == index and t.is_contiguous():
+        return t.data_ptr()
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} wants {dtype}, not {t.dtype}")
     if t.shape != shape:
         raise ValueError(f"{name} has the shape {tuple(t.shape)}, not {tuple(shape)}")
-    if t.get_device() != index or not t.is_contiguous():
-        raise ValueError(f"{name} wants to be contiguous and on the others' device")
+    raise ValueError(f"{name} wants to be contiguous and on the others' device")
 
 
 def _on_gpu(index: int) -> bool:
@@ -114,7 +123,7 @@ def _on_gpu(index: int) -> bool:
     return True
 
 
-_BF16, _BF16_F32 = (torch.bfloat16,), (torch.bfloat16, torch.float32)
+_BF16, _F32 = torch.bfloat16, torch.float32
 
 
 # --------------------------------------------------------------------------- rows
@@ -126,43 +135,43 @@ def _numbers(x: torch.Tensor):
     return torch.where(fine & (top > 0), q, 0.0).to(torch.int8), torch.where(fine, top, torch.nan).squeeze(-1)
 
 
-def _new_rows(rows: int, width: int, device):
-    """(buffer whose rows end on 16 bytes, scales); the kernel writes the buffer's last columns too."""
-    return (torch.empty((rows, (width + 15) // 16 * 16), dtype=torch.int8, device=device),
-            torch.empty((rows,), dtype=torch.float32, device=device))
-
-
-def _rows_of(buffer: torch.Tensor, scale: torch.Tensor, width: int) -> QuantizedRows:
-    return QuantizedRows(buffer if buffer.shape[1] == width else buffer[:, :width], scale)
-
-
-def _launch_rows(form, rows, width, device, x=0, partials=0, bias=None, residual=None, w=None, residual_out=None, x_ld=0, split_stride=0,
+def _launch_rows(form, rows, width, device, index, x=0, partials=0, bias=0, residual=0, w=0, residual_out=0, x_ld=0, split_stride=0,
                  splits=0, eps=0.0, limit=0.0, alpha=0.0) -> QuantizedRows:
-    buffer, scale = _new_rows(rows, width, device)
-    p = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    # (the kernel writes the columns up to the next sixteen, too)
+    ld = (width + 15) & -16
+    values = torch.empty_strided((rows, width), (ld, 1), dtype=torch.int8, device=device) if ld == width else \
+        torch.empty((rows, ld), dtype=torch.int8, device=device)[:, :width]
+    scale = torch.empty_strided((rows,), (1,), dtype=_F32, device=device)
     rc = _lib.lib().nkb_quant_rows(_ROWS.pack(
-        x, partials, p(bias), p(residual), p(w), p(residual_out), buffer.data_ptr(), scale.data_ptr(), _stream(), x_ld, buffer.shape[1],
-        split_stride, _FORMS[form], rows, width, splits, eps, limit, alpha, 0))
+        x, partials, bias, residual, w, residual_out, values.data_ptr(), scale.data_ptr(), _stream(), x_ld, ld, split_stride, form, rows,
+        width, splits, eps, limit, alpha, 0))
     if rc:
         _lib.check(rc, "nkb_quant_rows")
     _count_launch()
-    return _rows_of(buffer, scale, width)
+    return QuantizedRows._made(values, scale, ld, index)
+
+
+def _check_rows(x: torch.Tensor):
+    """(rows, columns, elements from one row to the next) of rows to be brought into 8 bits."""
+    if x.dtype is not _BF16 and x.dtype is not _F32:
+        raise TypeError(f"quantize_rows wants bf16 or fp32, not {x.dtype}")
+    shape = x.shape
+    if len(shape) != 2 or not 1 <= shape[1] <= MAX_K:
+        raise ValueError(f"quantize_rows wants [rows, k] of at most {MAX_K} columns")
+    ld, column = x.stride()
+    if column != 1 and shape[1] > 1:
+        raise ValueError("quantize_rows wants neighbouring columns")
+    return shape[0], shape[1], ld
 
 
 def quantize_rows(x: torch.Tensor) -> QuantizedRows:
     """bf16 or fp32 rows [rows, k] (they may lie apart) in 8 bits."""
-    if x.dtype not in _BF16_F32:
-        raise TypeError(f"quantize_rows wants bf16 or fp32, not {x.dtype}")
-    if x.dim() != 2 or not 1 <= x.shape[1] <= MAX_K:
-        raise ValueError(f"quantize_rows wants [rows, k] of at most {MAX_K} columns")
-    rows, width = x.shape
-    ld, column = x.stride()
-    if column != 1 and width > 1:
-        raise ValueError("quantize_rows wants neighbouring columns")
-    if not _on_gpu(x.get_device()):
+    rows, width, ld = _check_rows(x)
+    index = x.get_device()
+    if not _on_gpu(index):
         q, top = _numbers(x.double())
         return QuantizedRows(q, (top / 127).float())
-    return _launch_rows("bf16" if x.dtype is torch.bfloat16 else "f32", rows, width, x.device, x=x.data_ptr(), x_ld=ld)
+    return _launch_rows(0 if x.dtype is _BF16 else 1, rows, width, x.device, index, x=x.data_ptr(), x_ld=ld)
 
 
 def add_rmsnorm(x, w, *, residual_in=None, partials=None, bias=None, residual_out=None, eps=1e-6, hidden=None, rows=None):
@@ -176,25 +185,36 @@ def add_rmsnorm(x, w, *, residual_in=None, partials=None, bias=None, residual_ou
         raise ValueError(f"quantised rows have at most {MAX_K} columns")
     if rows is None:
         rows = x.numel() // hidden if x is not None else partials.shape[-2]
-    splits, stride = 0, 0
+    splits, stride, parts_at, n = 0, 0, 0, rows * hidden
     if partials is not None:
-        if partials.dtype is not torch.float32:
+        if partials.dtype is not _F32:
             raise TypeError("partials must be fp32")
         splits = partials.shape[0] if partials.dim() == 3 else 1
         stride = partials.stride(0) if partials.dim() == 3 else 0
         one = partials[0] if partials.dim() == 3 and splits else partials
         if not splits or one.shape != (rows, hidden) or partials.get_device() != index or not one.is_contiguous():
             raise ValueError("partials wants [splits, rows, hidden] with neighbouring rows, on the others' device")
-    for t, name in ((x, "x"), (residual_in, "residual_in"), (residual_out, "residual_out")):
-        if t is not None and t.numel() != rows * hidden:
-            raise ValueError(f"{name} wants {rows} rows of {hidden}")
-        if t is not None:
-            _want(t, name, _BF16, t.shape, index)
-    _want(w, "w", _BF16, (hidden,), index)
+        parts_at = partials.data_ptr()
+    x_at = residual_at = bias_at = 0
+    if x is not None:
+        if x.numel() != n:
+            raise ValueError(f"x wants {rows} rows of {hidden}")
+        x_at = _want(x, "x", _BF16, x.shape, index)
+    if residual_in is not None:
+        if residual_in.numel() != n:
+            raise ValueError(f"residual_in wants {rows} rows of {hidden}")
+        residual_at = _want(residual_in, "residual_in", _BF16, residual_in.shape, index)
+    w_at = _want(w, "w", _BF16, (hidden,), index)
     if bias is not None:
-        _want(bias, "bias", _BF16, (hidden,), index)
-    if residual_out is None and (residual_in is not None or partials is not None):
-        residual_out = torch.empty((rows, hidden), dtype=torch.bfloat16, device=ref.device)
+        bias_at = _want(bias, "bias", _BF16, (hidden,), index)
+    if residual_out is not None:
+        if residual_out.numel() != n:
+            raise ValueError(f"residual_out wants {rows} rows of {hidden}")
+        _want(residual_out, "residual_out", _BF16, residual_out.shape, index)
+    elif x is not None and residual_in is not None and len(x.shape) == 2:
+        residual_out = torch.empty_like(x)
+    elif residual_in is not None or partials is not None:
+        residual_out = torch.empty((rows, hidden), dtype=_BF16, device=ref.device)
     if not _on_gpu(index):
         h = torch.zeros((rows, hidden), dtype=torch.float64)
         if partials is not None:
@@ -208,14 +228,14 @@ def add_rmsnorm(x, w, *, residual_in=None, partials=None, bias=None, residual_ou
         q, top = _numbers(h.double() * w.double())
         scale = (top / 127).float() * torch.rsqrt(h.float().square().mean(-1) + eps)
         return residual_out, QuantizedRows(q, scale)
-    return residual_out, _launch_rows("norm", rows, hidden, ref.device, x=0 if x is None else x.data_ptr(),
-                                      partials=0 if partials is None else partials.data_ptr(), bias=bias, residual=residual_in, w=w,
-                                      residual_out=residual_out, x_ld=hidden, split_stride=stride, splits=splits, eps=eps)
+    return residual_out, _launch_rows(2, rows, hidden, ref.device, index, x=x_at, partials=parts_at, bias=bias_at, residual=residual_at, w=w_at,
+                                      residual_out=0 if residual_out is None else residual_out.data_ptr(), x_ld=hidden,
+                                      split_stride=stride, splits=splits, eps=eps)
 
 
 def silu_mul(gate_up, limit: float = 0.0, alpha: float = 1.702, bias=None) -> QuantizedRows:
     """`ops.silu_mul` whose rows are brought into 8 bits; bf16 [T, 2 I], or fp32 (partial sums) [S, T, 2 I]."""
-    if gate_up.dtype not in _BF16_F32:
+    if gate_up.dtype is not _BF16 and gate_up.dtype is not _F32:
         raise TypeError(f"silu_mul wants bf16 or fp32, not {gate_up.dtype}")
     index, f32 = gate_up.get_device(), gate_up.dtype is torch.float32
     if gate_up.dim() != 2 and not (f32 and gate_up.dim() == 3 and gate_up.shape[0]):
@@ -226,8 +246,7 @@ def silu_mul(gate_up, limit: float = 0.0, alpha: float = 1.702, bias=None) -> Qu
         raise ValueError(f"silu_mul wants gate and up of at most {MAX_K} columns")
     if gate_up.stride(-1) != 1:
         raise ValueError("silu_mul wants neighbouring columns")
-    if bias is not None:
-        _want(bias, "bias", _BF16, (two,), index)
+    bias_at = 0 if bias is None else _want(bias, "bias", _BF16, (two,), index)
     if not _on_gpu(index):
         v = gate_up.double() if gate_up.dim() == 2 else gate_up.double().sum(0)
         if bias is not None:
@@ -240,10 +259,10 @@ def silu_mul(gate_up, limit: float = 0.0, alpha: float = 1.702, bias=None) -> Qu
             y = g / (1 + torch.exp(-g)) * u
         q, top = _numbers(y)
         return QuantizedRows(q, (top / 127).float())
-    parts = gate_up.shape[0] if gate_up.dim() == 3 else 1
-    return _launch_rows("gate_f32" if f32 else "gate_bf16", rows, width, gate_up.device, x=0 if f32 else gate_up.data_ptr(),
-                        partials=gate_up.data_ptr() if f32 else 0, bias=bias, x_ld=gate_up.stride(-2),
-                        split_stride=gate_up.stride(0) if gate_up.dim() == 3 else 0, splits=parts if f32 else 0, limit=limit, alpha=alpha)
+    deep, at = gate_up.dim() == 3, gate_up.data_ptr()
+    return _launch_rows(4 if f32 else 3, rows, width, gate_up.device, index, x=0 if f32 else at, partials=at if f32 else 0, bias=bias_at,
+                        x_ld=gate_up.stride(-2), split_stride=gate_up.stride(0) if deep else 0,
+                        splits=(gate_up.shape[0] if deep else 1) if f32 else 0, limit=limit, alpha=alpha)
 
 
 # --------------------------------------------------------------------------- products
@@ -266,24 +285,25 @@ def linear(x, w: QuantizedWeight, *, bias=None, residual=None, out=None, splits:
     N = w.shape[0] // 2 if gated else w.shape[0]
     if gated and (w.shape[0] % 2 or act not in ("silu", "gelu_tanh")):
         raise ValueError("a gated product wants gate and up rows, and silu or gelu_tanh")
-    if not isinstance(x, QuantizedRows):
-        if x.dim() != 2 or x.shape[1] != w.shape[1]:
-            raise ValueError(f"shape mismatch: x {tuple(x.shape)} w {tuple(w.shape)}")
-        x = quantize_rows(x)
-    M, K = x.shape
     index = w.index
+    given = type(x) is QuantizedRows
+    if given:
+        M, K = x.shape
+        if x.index != index:
+            raise ValueError("rows and weight want to be on one device")
+    else:
+        M, K, x_ld = _check_rows(x)
+        if x.get_device() != index:
+            raise ValueError("rows and weight want to be on one device")
     if K != w.shape[1]:
         raise ValueError(f"shape mismatch: x {tuple(x.shape)} w {tuple(w.shape)}")
-    if x.index != index:
-        raise ValueError("rows and weight want to be on one device")
     if gated and (bias is not None or residual is not None or fp32_out or splits > 1):
         raise ValueError("a gated product has no bias, residual, fp32_out or splits")
     if splits > 1 and residual is not None:
         raise ValueError("partial sums have no residual")
-    dtype = torch.float32 if fp32_out or splits > 1 else torch.bfloat16
+    dtype = _F32 if fp32_out or splits > 1 else _BF16
     parts = effective_splits(K, splits) if splits > 1 else 0
-    if bias is not None:
-        _want(bias, "bias", _BF16, (N,), index)
+    bias_at = 0 if bias is None else _want(bias, "bias", _BF16, (N,), index)
     if out is None:
         out = torch.empty((parts, M, N) if parts else (M, N), dtype=dtype, device=w.device)
     elif parts:
@@ -295,7 +315,7 @@ def linear(x, w: QuantizedWeight, *, bias=None, residual=None, out=None, splits:
             raise TypeError(f"out wants {dtype}, not {out.dtype}")
         if out.shape != (M, N) or out.get_device() != index or (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
             raise ValueError("out wants [M, N] with neighbouring columns, on the weight's device")
-    ldo = max(out.stride(-2), N)
+    ldo = N if out.is_contiguous() else max(out.stride(-2), N)
     if residual is not None:
         if residual.dtype is not torch.bfloat16:
             raise TypeError(f"residual wants torch.bfloat16, not {residual.dtype}")
@@ -304,17 +324,26 @@ def linear(x, w: QuantizedWeight, *, bias=None, residual=None, out=None, splits:
         if residual.stride() != out.stride():
             residual = residual.contiguous() if ldo == N else torch.empty_strided((M, N), (ldo, 1), dtype=residual.dtype,
                                                                                   device=residual.device).copy_(residual)
-    if not M or not w.shape[0]:
+    if not M or not N:
         return out
     if not _on_gpu(index):
-        return _reference(x, w, bias, residual, out, parts, gated, act, N)
-    rc = _lib.lib().nkb_gemm_i8(_GEMM.pack(
-        x.at[0], w.at[0], x.at[1], w.at[1], 0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(),
-        out.data_ptr(), _stream(), x.ld, w.ld, ldo, out.stride(0) if parts else 0, M, N, K, gated, mixers.ACTIVATIONS[act][0] if gated else 0,
-        dtype is torch.float32, parts, weights_static))
+        return _reference(x if given else quantize_rows(x), w, bias, residual, out, parts, gated, act, N)
+    stream = _stream()
+    if given:
+        (q_at, scale_at), q_ld, rows = x.at, x.ld, None
+    else:
+        # numbers and scales in one piece of memory; both launches by one call
+        q_ld = (K + 15) & -16
+        buffer = torch.empty_strided((M * (q_ld + 4),), (1,), dtype=torch.int8, device=w.device)
+        q_at = buffer.data_ptr()
+        scale_at = q_at + M * q_ld
+        rows = _ROWS.pack(x.data_ptr(), 0, 0, 0, 0, 0, q_at, scale_at, stream, x_ld, q_ld, 0, 0 if x.dtype is _BF16 else 1, M, K, 0, 0.0, 0.0, 0.0, 0)
+    rc = _lib.lib().nkb_linear_i8(rows, _GEMM.pack(
+        q_at, w.at[0], scale_at, w.at[1], bias_at, 0 if residual is None else residual.data_ptr(), out.data_ptr(), stream, q_ld, w.ld, ldo,
+        out.stride(0) if parts else 0, M, N, K, gated, mixers.ACTIVATIONS[act][0] if gated else 0, dtype is _F32, parts, weights_static))
     if rc:
-        _lib.check(rc, "nkb_gemm_i8")
-    _count_launch()
+        _lib.check(rc, "nkb_linear_i8")
+    _count_launch(1 if given else 2)
     return out
 
 
