@@ -32,7 +32,8 @@ get_config = _load("gpt_oss_config", os.path.join(HERE, "..", "config.py")).get_
 peagle_config = _load("peagle_config", os.path.join(HERE, "config.py"))
 
 from nkipy_b200.models.engine import GenerationEngine  # noqa: E402
-from nkipy_b200.models.runner import add_common_args, build_model, build_prompts, kv_dtype, load_tokenizer  # noqa: E402
+from nkipy_b200.models.runner import (add_common_args, build_model, build_prompts, kv_dtype, load_tokenizer,  # noqa: E402
+                                      quantize_weights)
 from nkipy_b200.models.speculative import DrafterLM, SpeculativeEngine, random_drafter_weights  # noqa: E402
 from nkipy_b200.models.weights import load_shard  # noqa: E402
 from nkipy_b200.parallel.comm import TPGroup  # noqa: E402
@@ -47,6 +48,7 @@ def main():
     tp = TPGroup.from_env()
     cfg = get_config(args.model)
     target = build_model(cfg, args, tp)
+    quantize_weights(args, target)
     cfg = target.cfg
     ecfg = peagle_config.get_eagle_config(cfg, args.num_draft_tokens)
     if args.tiny:

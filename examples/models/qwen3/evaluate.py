@@ -23,7 +23,7 @@ from config import get_config  # noqa: E402
 
 from nkipy_b200.models.engine import GenerationEngine  # noqa: E402
 from nkipy_b200.models.reference import EagerTransformer  # noqa: E402
-from nkipy_b200.models.runner import add_common_args, build_prompts, kv_dtype, load_tokenizer  # noqa: E402
+from nkipy_b200.models.runner import add_common_args, build_prompts, kv_dtype, load_tokenizer, quantize_weights  # noqa: E402
 from nkipy_b200.models.transformer import TransformerLM  # noqa: E402
 from nkipy_b200.models.weights import load_shard, random_weights  # noqa: E402
 from nkipy_b200.parallel.comm import TPGroup  # noqa: E402
@@ -35,6 +35,7 @@ def evaluate(cfg, args):
     weights = (load_shard(args.checkpoint, tp.rank, device=dev) if args.checkpoint
                else random_weights(cfg, tp.rank, tp.world_size, device=dev, seed=args.seed, std=0.05))
     model = TransformerLM(cfg, weights, tp, device=dev)
+    quantize_weights(args, model)
     prompts = build_prompts(args, cfg, load_tokenizer(args.model))
     n = args.max_new_tokens
     eng = GenerationEngine(model, max_batch=len(prompts), max_seq_len=len(prompts[0]) + n + 64,

@@ -19,7 +19,7 @@ import os
 import struct
 import time
 from dataclasses import dataclass, field
-from typing import Dict, Iterable, List, Optional, Sequence
+from typing import Callable, Dict, Iterable, List, Optional, Sequence
 
 import numpy as np
 import torch
@@ -74,11 +74,92 @@ class StepEntry:
 
 @dataclass
 class Sampling:
-    """temperature <= 0: greedy; top_k 0 and top_p 1: unrestricted."""
+    """temperature <= 0: greedy; top_k 0 and top_p 1: unrestricted.
+
+    Rules on the logits ahead of either (`ops.LogitRules`): repetition, frequency and presence penalties, biases {token: value}, and
+    allowed(prompt, answer) -> the ids (or a bool [vocab]) that a sequence may go on with, None: any; where that is none, it ends."""
     temperature: float = 0.0
     top_k: int = 0
     top_p: float = 1.0
     seed: int = 0
+    repetition: float = 1.0
+    frequency: float = 0.0
+    presence: float = 0.0
+    biases: Optional[Dict[int, float]] = None
+    allowed: Optional[Callable] = None
+
+    def __post_init__(self):
+        if not self.repetition > 0 or self.repetition == float("inf"):
+            raise ValueError("the repetition penalty is a number above zero")
+        for v in (self.frequency, self.presence):
+            if not abs(v) < float("inf"):
+                raise ValueError("penalties are numbers")
+
+    @property
+    def ruled(self) -> bool:
+        return self.repetition != 1 or self.frequency != 0 or self.presence != 0 or bool(self.biases) or self.allowed is not None
+
+
+class StepRules:
+    """Rules of the sequences in a batch's rows: their tokens on the device, to which every choice adds one."""
+
+    def __init__(self, sampling: Sampling, vocab: int, rows: int, width: int, device):
+        self.sampling, self.vocab, self.device = sampling, vocab, device
+        n = len(sampling.biases or {})
+        if any(not 0 <= int(t) < vocab for t in sampling.biases or {}):
+            raise ValueError("biases are for tokens of the vocabulary")
+        whole = lambda v: torch.full((rows,), float(v), device=device)  # noqa: E731
+        zeros = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=device)  # noqa: E731
+        s = sampling
+        self.rules = ops.LogitRules(
+            tokens=zeros(rows, width), lens=zeros(rows), prompt_lens=zeros(rows), ids=zeros(rows), repetition=whole(s.repetition),
+            frequency=whole(s.frequency), presence=whole(s.presence),
+            bias_ids=torch.tensor([list(s.biases)] * rows, dtype=torch.int32, device=device) if n else None,
+            bias_values=torch.tensor([list(s.biases.values())] * rows, dtype=torch.float32, device=device) if n else None,
+            mask=zeros(rows, -(-vocab // 32)).fill_(-1) if s.allowed else None)
+
+    def start(self, rows: Sequence[int], prompts: Sequence[Sequence[int]]) -> None:
+        """Rows whose sequences have their prompts, and no answer."""
+        r = self.rules
+        for row, p in zip(rows, prompts):
+            r.tokens[row, :len(p)] = torch.tensor(list(p), dtype=torch.int32).to(self.device)
+            r.lens[row] = r.prompt_lens[row] = len(p)
+            r.ids[row] = int(p[-1])
+        self.allow(rows, prompts, [[]] * len(rows))
+
+    def allow(self, rows: Sequence[int], prompts: Sequence[Sequence[int]], answers: Sequence[Sequence[int]]) -> None:
+        """What the rows' sequences may go on with."""
+        if self.sampling.allowed is None:
+            return
+        bits = torch.zeros((len(rows), self.vocab), dtype=torch.bool)
+        for i, (p, a) in enumerate(zip(prompts, answers)):
+            ids = self.sampling.allowed(p, a)
+            if ids is None:
+                bits[i] = True
+            else:
+                bits[i, ids if torch.is_tensor(ids) else list(ids)] = True
+        at = torch.tensor(list(rows), device=self.device)
+        self.rules.mask.index_copy_(0, at, ops.pack_mask(bits).to(self.device))
+
+    def of_rows(self, rows: Sequence[int]) -> "ops.LogitRules":
+        """The rules of some rows, in their order (their tokens are there)."""
+        at, r = torch.tensor(list(rows), device=self.device), self.rules
+        pick = lambda t: None if t is None else t.index_select(0, at)  # noqa: E731
+        return ops.LogitRules(tokens=pick(r.tokens), lens=pick(r.lens), prompt_lens=pick(r.prompt_lens), repetition=pick(r.repetition),
+                              frequency=pick(r.frequency), presence=pick(r.presence), bias_ids=pick(r.bias_ids),
+                              bias_values=pick(r.bias_values), mask=pick(r.mask))
+
+    def choose(self, logits: torch.Tensor, rules: "ops.LogitRules", step: int, out_ids: Optional[torch.Tensor] = None) -> torch.Tensor:
+        s = self.sampling
+        if s.temperature <= 0:
+            return ops.argmax(logits, out_ids=out_ids, rules=rules)
+        left = ops.apply_rules(logits, rules)
+        if s.allowed is None:
+            return GenerationEngine._sample(left, s, step, out_ids)
+        # (there is no drawing from nothing)
+        none = ops.argmax(left, rules=ops.LogitRules()) < 0
+        ids = GenerationEngine._sample(left.masked_fill_(none[:, None], 0.0), s, step, out_ids)
+        return ids.masked_fill_(none, -1)
 
 
 def _token_arrays(entries: Sequence[StepEntry], lens: Sequence[int]) -> List[np.ndarray]:
@@ -224,9 +305,10 @@ class GenerationEngine:
         if batch:
             yield batch
 
-    def prefill(self, seqs: Sequence[SequenceState], sampling: Optional[Sampling] = None) -> torch.Tensor:
+    def prefill(self, seqs: Sequence[SequenceState], sampling: Optional[Sampling] = None,
+                rules: Optional[StepRules] = None) -> torch.Tensor:
         """Run the uncached part of the prompts (in portions of at most the token budget); returns the first
-        generated token of every sequence (int32, device) and records per-sequence TTFT."""
+        generated token of every sequence (int32, device) and records per-sequence TTFT.  rules: of the sequences' rows."""
         m, cache, dev = self.model, self.cache, self.device
         first = torch.zeros((len(seqs),), dtype=torch.int32, device=dev)
         t0 = time.perf_counter()
@@ -237,7 +319,10 @@ class GenerationEngine:
                 cache.mark_computed(batch[0][1], batch[0][3])
                 continue
             h = hidden.index_select(0, last)
-            tok_ids = m.greedy(h) if sampling is None else self._sample(m.logits(h), sampling, len(batch[0][1].tokens))
+            if rules is not None:
+                tok_ids = rules.choose(m.logits(h), rules.of_rows([s.slot for _, s, _, _ in batch]), len(batch[0][1].tokens))
+            else:
+                tok_ids = m.greedy(h) if sampling is None else self._sample(m.logits(h), sampling, len(batch[0][1].tokens))
             for j, (gi, _, _, _) in enumerate(batch):
                 first[gi:gi + 1].copy_(tok_ids[j:j + 1])
             if dev.type == "cuda":
@@ -329,14 +414,21 @@ class GenerationEngine:
         else:
             self._decode_body()
 
-    def step(self, ids_host: Optional[torch.Tensor] = None, sampling: Optional[Sampling] = None) -> torch.Tensor:
+    def step(self, ids_host: Optional[torch.Tensor] = None, sampling: Optional[Sampling] = None,
+             rules: Optional[StepRules] = None) -> torch.Tensor:
         """Public per-step API: token ids in pinned host memory -> device, one decode step,
         new ids back to pinned host memory (synchronises).  Without ids_host the ids already on
-        the device are used."""
+        the device are used.  rules: of the batch's rows; they choose the ids, and have the step's own as their newest."""
         if ids_host is not None:
             self.ids.copy_(ids_host, non_blocking=True)
+        if rules is not None:
+            rules.rules.ids.copy_(self.ids)
         self.decode_step_device()
-        if sampling is not None:
+        if rules is not None:
+            longest = max((s.num_computed for s in self.active.values()), default=0)
+            rules.rules.lens.copy_(self.context_lens)
+            rules.choose(self.step_logits, rules.rules, longest + 1, out_ids=self.ids)
+        elif sampling is not None:
             longest = max((s.num_computed for s in self.active.values()), default=0)
             self._sample(self.step_logits, sampling, longest + 1, out_ids=self.ids)
         self.out_host.copy_(self.ids, non_blocking=True)
@@ -467,14 +559,20 @@ class GenerationEngine:
                  sampling: Optional[Sampling] = None) -> List[List[int]]:
         """Generation for a batch of prompts, greedy unless `sampling` has a positive temperature; returns the new
         token ids per prompt."""
-        if sampling is not None and sampling.temperature <= 0:
+        ruled = sampling is not None and sampling.ruled
+        if sampling is not None and sampling.temperature <= 0 and not ruled:
             sampling = None
         if sampling is not None and self.model.tp.world_size > 1:
             raise NotImplementedError("sampling with a vocabulary split over ranks")
+        rules = StepRules(sampling, self.model.cfg.vocab_size, self.max_batch, self.max_seq_len + 1, self.device) if ruled else None
         seqs = self.add_requests(prompts)
-        self.prefill(seqs, sampling)
+        slots, prompts = [s.slot for s in seqs], [list(p) for p in prompts]
+        if rules is not None:
+            rules.start(slots, prompts)
+        self.prefill(seqs, sampling, rules)
         outs: List[List[int]] = [[s.tokens[-1]] for s in seqs]
-        finished = [eos_token_id is not None and o[0] == eos_token_id for o in outs]
+        # (-1: the rules have left nothing)
+        finished = [o[0] < 0 or (eos_token_id is not None and o[0] == eos_token_id) for o in outs]
         if max_new_tokens > 1:
             self.prepare_decode(max_new_tokens)
         t0 = time.perf_counter()
@@ -483,7 +581,10 @@ class GenerationEngine:
             if all(finished):
                 break
             ts = time.perf_counter()
-            host = self.step(sampling=sampling).clone()
+            if rules is not None:
+                on = [j for j in range(len(seqs)) if not finished[j]]
+                rules.allow([slots[j] for j in on], [prompts[j] for j in on], [outs[j] for j in on])
+            host = self.step(sampling=sampling, rules=rules).clone()
             self.stats.decode_step_ms.append((time.perf_counter() - ts) * 1e3)
             self.advance_host_state(1)
             steps += 1
@@ -493,12 +594,12 @@ class GenerationEngine:
                 tok = int(host[s.slot])
                 outs[j].append(tok)
                 s.tokens.append(tok)
-                if eos_token_id is not None and tok == eos_token_id:
+                if tok < 0 or (eos_token_id is not None and tok == eos_token_id):
                     finished[j] = True
         self.stats.decode_time_s += time.perf_counter() - t0
         self.stats.decode_tokens += steps * len(seqs)
         self.release(seqs)
-        return outs
+        return [o[:-1] if o[-1] < 0 else o for o in outs] if rules is not None else outs
 
     def release(self, seqs: Iterable[SequenceState]) -> None:
         seqs = list(seqs)

@@ -40,12 +40,30 @@ def add_common_args(ap: argparse.ArgumentParser) -> None:
                     help="float32: true 32-bit, for the models that have it")
     ap.add_argument("--kv-dtype", choices=["auto", "bfloat16", "e4m3"], default="auto",
                     help="keys and values in the cache; e4m3: 8 bits, for the models that have it; auto: as the model computes")
+    ap.add_argument("--weight-dtype", choices=["auto", "int8"], default="auto",
+                    help="weights of the products; int8: 8-bit whole numbers, for dense models on one GPU; auto: as the model computes")
+    ap.add_argument("--repetition-penalty", type=float, default=1.0, help="of tokens that the prompt or the answer has; 1: none")
+    ap.add_argument("--frequency-penalty", type=float, default=0.0, help="of tokens that the answer has, for each time")
+    ap.add_argument("--presence-penalty", type=float, default=0.0, help="of tokens that the answer has, once")
     ap.add_argument("--tiny", action="store_true",
                     help="shrink the model (hidden 256, vocabulary 2048, <= 8 experts) for quick functional runs")
 
 
 def kv_dtype(args) -> Optional[torch.dtype]:
     return {"auto": None, "bfloat16": torch.bfloat16, "e4m3": torch.float8_e4m3fn}[args.kv_dtype]
+
+
+def quantize_weights(args, model) -> None:
+    """Brings the model's weights into what the arguments ask for."""
+    if args.weight_dtype == "int8":
+        if not hasattr(model, "quantize_weights"):
+            raise ValueError("this model has no weights in 8 bits")
+        model.quantize_weights()
+
+
+def sampling_of(args) -> Sampling:
+    return Sampling(args.temperature, args.top_k, args.top_p, args.seed, args.repetition_penalty, args.frequency_penalty,
+                    args.presence_penalty)
 
 
 def load_tokenizer(path: Optional[str]):
@@ -120,6 +138,7 @@ def run_generation(cfg: ModelConfig, args, model=None, tp: Optional[TPGroup] = N
     tokenizer = load_tokenizer(args.model)
     if model is None:
         model = build_model(cfg, args, tp)
+    quantize_weights(args, model)
     prompts = build_prompts(args, model.cfg, tokenizer)
     max_len = min(args.max_seq_len, max(len(p) for p in prompts) + args.max_new_tokens + 64)
     eng = GenerationEngine(model, max_batch=len(prompts), max_seq_len=max_len,
@@ -129,7 +148,7 @@ def run_generation(cfg: ModelConfig, args, model=None, tp: Optional[TPGroup] = N
     tp.barrier()
     t0 = time.perf_counter()
     out = eng.generate(prompts, args.max_new_tokens,
-                       sampling=Sampling(args.temperature, args.top_k, args.top_p, args.seed))
+                       sampling=sampling_of(args))
     dt = time.perf_counter() - t0
     if tp.rank == 0:
         s = eng.stats.summary()

@@ -110,6 +110,7 @@ class TransformerLM:
             self.layers.append(lw)
         inv_freq, rope_scale = yarn_inv_freq(cfg)
         self.rope = ops.rope_table(cfg.head_dim, cfg.max_position, inv_freq=inv_freq, scaling=rope_scale, device=dev)
+        self.quantized = False                # weights in 8 bits (`quantize_weights`)
         self._moe = None
         if cfg.is_moe:
             from .moe import MoEBlock
@@ -130,6 +131,20 @@ class TransformerLM:
             if two_i // 256 < 100:          # fewer than ~100 fused gate/up tile pairs
                 self.split_gate_up = max(2, pick_splits(two_i, H))
 
+    def quantize_weights(self) -> "TransformerLM":
+        """Projections, feed-forward and head in 8-bit whole numbers with a scale for every output channel, which the products multiply
+        with activations in 8 bits; embeddings, norms and attention stay as they are.  Dense models on one rank."""
+        if self.cfg.is_moe or self.tp.world_size > 1 or self.force_fused:
+            raise ValueError("weights in 8 bits are for dense models on one rank")
+        if not self.quantized:
+            for lw in self.layers:
+                for name in ("qkv", "o", "gate_up", "down"):
+                    setattr(lw, name, ops.QuantizedWeight.of(getattr(lw, name)))
+            self.lm_head = ops.QuantizedWeight.of(self.lm_head)
+            self.quantized = True
+            self.cluster_gemm = self.fix_gemm = False          # (kernels of bf16 weights)
+        return self
+
     # ------------------------------------------------------------------ cache
     def new_cache(self, num_blocks: int, max_batch: int, max_seq_len: int,
                   enable_prefix_sharing: bool = True, kv_dtype: Optional[torch.dtype] = None) -> PagedKVCache:
@@ -144,13 +159,11 @@ class TransformerLM:
         return cache
 
     def weight_bytes(self) -> int:
-        n = self.tok_embedding.numel() + self.lm_head.numel()
-        for lw in self.layers:
-            for s in ("qkv", "o", "gate_up", "down", "router"):
-                t = getattr(lw, s)
-                if t is not None:
-                    n += t.numel()
-        return n * 2
+        def size(t):
+            return 0 if t is None else t.nbytes if isinstance(t, ops.QuantizedWeight) else 2 * t.numel()
+
+        return size(self.tok_embedding) + size(self.lm_head) + sum(
+            size(getattr(lw, s)) for lw in self.layers for s in ("qkv", "o", "gate_up", "down", "router"))
 
     # ------------------------------------------------------------------ FFN
     def _csplits(self, w: torch.Tensor, tokens: int, gated: bool = False) -> int:
@@ -165,8 +178,8 @@ class TransformerLM:
                 cache[key] = pick_cluster_splits(tiles, w.shape[1], tokens)
         return cache[key]
 
-    def _ffn_decode(self, lw: LayerWeights, normed: torch.Tensor, resid: torch.Tensor, next_norm: torch.Tensor):
-        """Returns (new residual, normed for the next block)."""
+    def _ffn_decode(self, lw: LayerWeights, normed: torch.Tensor, resid: torch.Tensor, next_norm: torch.Tensor, quantize: bool = False):
+        """Returns (new residual, normed for the next block, in 8 bits if `quantize`)."""
         cfg = self.cfg
         if cfg.is_moe:
             return self._moe.forward_add_rmsnorm(lw, normed, resid, next_norm)
@@ -181,13 +194,13 @@ class TransformerLM:
         elif self.split_gate_up > 1:
             # too few gate/up tile pairs to fill the SMs: split-K partials, gate applied by the reducer
             act = ops.silu_mul(ops.linear(normed, lw.gate_up, splits=self.split_gate_up), limit=cfg.swiglu_limit,
-                               alpha=cfg.swiglu_alpha)
+                               alpha=cfg.swiglu_alpha, quantize=self.quantized)
         else:
-            act = ops.silu_mul(ops.linear(normed, lw.gate_up), limit=cfg.swiglu_limit, alpha=cfg.swiglu_alpha)
-        return self._row_parallel_reduce(act, lw.down, self.split_down, resid, next_norm, None)
+            act = ops.silu_mul(ops.linear(normed, lw.gate_up), limit=cfg.swiglu_limit, alpha=cfg.swiglu_alpha, quantize=self.quantized)
+        return self._row_parallel_reduce(act, lw.down, self.split_down, resid, next_norm, None, quantize)
 
-    def _row_parallel_reduce(self, x, w, splits, resid, next_norm, bias):
-        """Row-parallel GEMM + sum over ranks + residual + next RMSNorm (decode-sized M)."""
+    def _row_parallel_reduce(self, x, w, splits, resid, next_norm, bias, quantize=False):
+        """Row-parallel GEMM + sum over ranks + residual + next RMSNorm (decode-sized M; in 8 bits if `quantize`)."""
         cfg = self.cfg
         if self.tp.world_size == 1 and not (self.force_fused and getattr(self.tp, "fused", None) is not None):
             if self.cluster_gemm and x.shape[0] <= 128 and x.is_cuda:
@@ -196,9 +209,9 @@ class TransformerLM:
             if splits > 1:
                 parts = ops.linear(x, w, splits=splits)
                 return ops.add_rmsnorm(None, next_norm, residual_in=resid, partials=parts, bias=bias,
-                                       eps=cfg.rms_eps)
+                                       eps=cfg.rms_eps, quantize=quantize)
             y = ops.linear(x, w)
-            return ops.add_rmsnorm(y, next_norm, residual_in=resid, bias=bias, eps=cfg.rms_eps)
+            return ops.add_rmsnorm(y, next_norm, residual_in=resid, bias=bias, eps=cfg.rms_eps, quantize=quantize)
         fused = getattr(self.tp, "fused", None)
         if fused is not None:
             return fused.gemm_allreduce_add_rmsnorm(x, w, resid, next_norm, bias, cfg.rms_eps, splits)
@@ -222,12 +235,12 @@ class TransformerLM:
         if inputs is None:
             x = ops.embedding(ids, self.tok_embedding)
             resid = x
-            normed = ops.rmsnorm(x, self.layers[0].input_norm, cfg.rms_eps)
+            normed = ops.rmsnorm(x, self.layers[0].input_norm, cfg.rms_eps, quantize=self.quantized)
         else:
             resid, normed = inputs
         taps = [] if return_hidden else None
         T = normed.shape[0]
-        if self._persistent_layers(T, normed) and not cache.quantized:
+        if self._persistent_layers(T, normed) and not cache.quantized and not self.quantized:
             return self._decode_step_persistent(resid, normed, positions, slots, cache, block_table, context_lens,
                                                 q_len, taps)
         # (the projections that append by themselves write bf16)
@@ -259,9 +272,10 @@ class TransformerLM:
                 attn = ops.paged_attn_decode(q, cache.k[i], cache.v[i], block_table, context_lens, self.scale, q_len=q_len,
                                              window=cfg.window_for_layer(i), sinks=lw.sinks, scratch=cache.scratch)
             split_o = self._csplits(lw.o, T) if cluster else self.split_o
-            resid, normed = self._row_parallel_reduce(attn, lw.o, split_o, resid, lw.post_norm, lw.o_bias)
-            nxt = self.layers[i + 1].input_norm if i + 1 < len(self.layers) else self.final_norm
-            resid, normed = self._ffn_decode(lw, normed, resid, nxt)
+            resid, normed = self._row_parallel_reduce(attn, lw.o, split_o, resid, lw.post_norm, lw.o_bias, self.quantized)
+            last = i + 1 == len(self.layers)
+            nxt = self.final_norm if last else self.layers[i + 1].input_norm
+            resid, normed = self._ffn_decode(lw, normed, resid, nxt, self.quantized and not last)
             if taps is not None:
                 taps.append(resid)
         if return_hidden:
@@ -420,13 +434,13 @@ class TransformerLM:
         if inputs is None:
             x = ops.embedding(ids, self.tok_embedding)
             resid = x
-            normed = ops.rmsnorm(x, self.layers[0].input_norm, cfg.rms_eps)
+            normed = ops.rmsnorm(x, self.layers[0].input_norm, cfg.rms_eps, quantize=self.quantized)
         else:
             resid, normed = inputs
         taps = [] if return_hidden else None
         singles = ops.leading_singles(spans)
         for i, lw in enumerate(self.layers):
-            swap, splits = ops.prefill_plan(normed.shape[0], lw.qkv.shape[0], lw.qkv.shape[1])
+            swap, splits = (False, 1) if self.quantized else ops.prefill_plan(normed.shape[0], lw.qkv.shape[0], lw.qkv.shape[1])
             qkv = ops.linear(normed, lw.qkv, swap=swap and splits > 1, splits=splits)
             q = ops.rope_kv_append(qkv, positions, slots, self.rope, cache.k[i], cache.v[i], self.nq, self.nkv,
                                    self.d, bias=lw.qkv_bias, q_norm_w=lw.q_norm, k_norm_w=lw.k_norm,
@@ -435,7 +449,7 @@ class TransformerLM:
                                         max_q_len=max_q_len, singles=singles, causal=cfg.causal,
                                         window=cfg.window_for_layer(i), sinks=lw.sinks)
             if tp1:
-                resid, normed = self._residual_linear(attn, lw.o, resid, lw.post_norm, lw.o_bias)
+                resid, normed = self._residual_linear(attn, lw.o, resid, lw.post_norm, lw.o_bias, self.quantized)
             else:
                 o = ops.linear(attn, lw.o, swap=False, bias=lw.o_bias)
                 self.tp.all_reduce(o)
@@ -450,9 +464,9 @@ class TransformerLM:
                     act = ops.linear(normed, lw.gate_up, gated=True, swap=normed.shape[0] <= 64)
                 else:
                     act = ops.silu_mul(ops.linear(normed, lw.gate_up, swap=False), limit=cfg.swiglu_limit,
-                                       alpha=cfg.swiglu_alpha)
+                                       alpha=cfg.swiglu_alpha, quantize=self.quantized)
                 if tp1:
-                    resid, normed = self._residual_linear(act, lw.down, resid, nxt)
+                    resid, normed = self._residual_linear(act, lw.down, resid, nxt, quantize=self.quantized and i + 1 < len(self.layers))
                 else:
                     dn = ops.linear(act, lw.down, swap=False)
                     self.tp.all_reduce(dn)
@@ -463,9 +477,13 @@ class TransformerLM:
             return normed, taps
         return normed
 
-    def _residual_linear(self, x, w, resid, next_norm, bias=None):
+    def _residual_linear(self, x, w, resid, next_norm, bias=None, quantize=False):
         """(resid + x w^T + bias, its norm) for a packed step on one rank: split-K partials summed by the norm kernel where a
-        step of that size splits (`ops.prefill_plan`), the residual in the epilogue otherwise."""
+        step of that size splits (`ops.prefill_plan`; whole products of weights in 8 bits divide k by themselves), the residual in the
+        epilogue otherwise.  quantize: the normed rows in 8 bits."""
+        if self.quantized:
+            resid = ops.linear(x, w, residual=resid, bias=bias)
+            return resid, ops.rmsnorm(resid, next_norm, self.cfg.rms_eps, quantize=quantize)
         swap, splits = ops.prefill_plan(x.shape[0], w.shape[0], x.shape[1])
         if splits > 1:
             return ops.add_rmsnorm(None, next_norm, residual_in=resid, partials=ops.linear(x, w, swap=swap, splits=splits),

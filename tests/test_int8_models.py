@@ -1,0 +1,210 @@
+"""Served models with weights in 8 bits, and generation under rules: the operators' calls of every step against plain implementations."""
+
+import pytest
+import torch
+
+from nkipy_b200 import ops
+from nkipy_b200.models import config as C
+from nkipy_b200.models.engine import GenerationEngine, Sampling, StepEntry
+from nkipy_b200.models.transformer import TransformerLM
+from nkipy_b200.models.weights import random_weights
+from tests.test_logit_rules import oracle, oracle_ids
+from tests.test_quantized_linear import DEVICES, check_product, check_rows, oracle_numbers, oracle_product
+
+E4M3 = torch.float8_e4m3fn
+KINDS = {
+    "llama": dict(hidden_size=256, head_dim=64, num_heads=8, num_kv_heads=2, intermediate_size=512, vocab_size=512, num_layers=2),
+    "qk-norm": dict(hidden_size=256, head_dim=128, num_heads=4, num_kv_heads=2, intermediate_size=512, vocab_size=512, num_layers=2,
+                    qk_norm=True),
+    "window": dict(hidden_size=256, head_dim=64, num_heads=8, num_kv_heads=1, intermediate_size=512, vocab_size=512, num_layers=2,
+                   attn_bias=True, attention_sinks=True, sliding_window=16),
+}
+
+
+def model_of(kind, device, quantize=True):
+    cfg = C.tiny(**KINDS[kind])
+    model = TransformerLM(cfg, random_weights(cfg, device=device, seed=1, std=0.05), device=device)
+    return model.quantize_weights() if quantize else model
+
+
+def ids(n, seed):
+    return torch.randint(0, 512, (n,), generator=torch.Generator().manual_seed(seed)).tolist()
+
+
+class Watched:
+    """Checks every product in 8 bits, and the rows behind every norm."""
+
+    def __init__(self, monkeypatch):
+        self.products = self.norms = 0
+        linear, norm = ops.quantized_linear.linear, ops.quantized_linear.add_rmsnorm
+
+        def checked_linear(x, w, **kw):
+            if type(x) is ops.QuantizedRows:
+                q, sx = x.values.cpu(), x.scale.cpu()
+            else:
+                q, top = oracle_numbers(x.cpu())
+                sx = (top / 127).float()
+            before = None if kw.get("residual") is None else kw["residual"].cpu().clone()
+            out = linear(x, w, **kw)
+            parts = out.dim() == 3
+            want, tol = oracle_product(q, sx, w.values.cpu(), w.scale.cpu(), gated=kw.get("gated", False), fp32=parts or kw.get("fp32_out", False),
+                                       bias=None if kw.get("bias") is None else kw["bias"].cpu(), residual=before)
+            # (partial sums: each is rounded to 32 bits, their sum of magnitudes is at most the sum over all of k)
+            mass = (q.double().abs() @ w.values.cpu().double().abs().T) * sx.double()[:, None] * w.scale.cpu().double()
+            check_product(out.double().sum(0) if parts else out, want, tol + (4 * 2.0 ** -24 * mass if parts else 0))
+            self.products += 1
+            return out
+
+        def checked_norm(x, w, **kw):
+            before = {k: v.cpu().double() for k, v in dict(kw, x=x).items() if torch.is_tensor(v) and k != "residual_out"}
+            h, rows = norm(x, w, **kw)
+            total = sum((before[k].reshape(rows.shape) for k in ("x", "residual_in") if k in before), torch.zeros(rows.shape, dtype=torch.float64))
+            if "partials" in before:
+                total = total + before["partials"].sum(0)
+            if "bias" in before:
+                total = total + before["bias"]
+            total = total.to(torch.bfloat16).double()
+            check_rows(rows, total * w.cpu().double(), 1 / torch.sqrt(total.square().mean(-1) + kw["eps"]), steps=64)
+            self.norms += 1
+            return h, rows
+
+        monkeypatch.setattr(ops.quantized_linear, "linear", checked_linear)
+        monkeypatch.setattr(ops.quantized_linear, "add_rmsnorm", checked_norm)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("kind", sorted(KINDS))
+def test_steps_of_a_scheduler(device, kind, monkeypatch):
+    model = model_of(kind, device)
+    engine = GenerationEngine(model, max_batch=4, max_seq_len=160, num_blocks=16, use_cuda_graph=False, enable_prefix_sharing=False)
+    seen = Watched(monkeypatch)
+    a, b = engine.open_request(), engine.open_request()
+    engine.run_step([StepEntry(a, ids(70, 1), [-1]), StepEntry(b, ids(5, 2))])
+    engine.run_step([StepEntry(a, ids(1, 3), [0]), StepEntry(b, ids(90, 4), [-1])])
+    logits = engine.run_step([StepEntry(b, ids(1, 5), [0]), StepEntry(a, ids(1, 6), [0])])
+    assert bool(logits.isfinite().all())
+    assert seen.products == 3 * (2 * 4 + 1) and seen.norms == 3 * 4
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_logits_are_near_those_of_bf16_weights(device):
+    """As far as 8 bits take them: every product adds an error of about 1 / (127 sqrt(12)) of its rows' and weights' largest numbers, some four
+    of their root mean squares, on both sides: 1.3 % of a result each; nine products in a chain, whose errors are independent, some 4 %."""
+    exact, model = model_of("llama", device, quantize=False), model_of("llama", device)
+    rows = []
+    for m in (exact, model):
+        engine = GenerationEngine(m, max_batch=1, max_seq_len=64, use_cuda_graph=False)
+        s = engine.open_request()
+        rows.append(engine.run_step([StepEntry(s, ids(40, 1), list(range(40)))]).float().cpu())
+    off = (rows[1] - rows[0]).norm() / rows[0].norm()
+    assert 0 < float(off) < 0.08
+    assert model.weight_bytes() < 0.75 * exact.weight_bytes()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", sorted(KINDS))
+@pytest.mark.parametrize("kv", [None, E4M3])
+def test_captured_steps_are_the_same(kind, kv):
+    model = model_of(kind, "cuda")
+    prompts = [ids(70, 1), ids(3, 2), ids(33, 3)]
+    outs = [GenerationEngine(model, max_batch=4, max_seq_len=160, use_cuda_graph=g, kv_dtype=kv).generate(prompts, 12) for g in (False, True)]
+    assert outs[0] == outs[1]
+
+
+def test_models_that_have_none():
+    cfg = C.tiny(num_experts=4, top_k=2, moe_intermediate_size=64) if "num_experts" in C.ModelConfig.__dataclass_fields__ else None
+    if cfg is not None and cfg.is_moe:
+        with pytest.raises(ValueError):
+            TransformerLM(cfg, random_weights(cfg, seed=1), device="cpu").quantize_weights()
+    model = model_of("llama", "cpu")
+    first = model.layers[0].qkv
+    assert model.quantize_weights() is model and model.layers[0].qkv is first
+
+
+# ------------------------------------------------------------------------------------------------ rules
+class Chosen:
+    """Follows every choice under rules by the oracle."""
+
+    def __init__(self, monkeypatch):
+        self.calls = 0
+        real = ops.logit_rules.argmax
+
+        def checked(logits, rules, out_ids=None):
+            r = {k: v.cpu().clone() for k, v in vars(rules).items() if v is not None}
+            got = real(logits, rules, out_ids)
+            want, tokens = oracle(logits.cpu(), r)
+            assert torch.equal(got.cpu(), oracle_ids(want))
+            assert torch.equal(rules.tokens.cpu(), tokens)
+            self.lens, self.tokens = r["lens"].tolist(), tokens
+            self.calls += 1
+            return got
+
+        monkeypatch.setattr(ops.logit_rules, "argmax", checked)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("quantize", [False, True])
+def test_generation_under_rules(device, quantize, monkeypatch):
+    model = model_of("llama", device, quantize)
+    engine = GenerationEngine(model, max_batch=4, max_seq_len=128, use_cuda_graph=device == "cuda")
+    prompts = [ids(40, 1), ids(5, 2), ids(33, 3)]
+    plain = engine.generate(prompts, 8)
+    assert engine.generate(prompts, 8, sampling=Sampling(presence=0.0)) == plain
+    seen = Chosen(monkeypatch)
+    out = engine.generate(prompts, 8, sampling=Sampling(repetition=1.3, frequency=0.4, presence=0.2, biases={7: 3.0, 9: -float("inf")}))
+    assert seen.calls == 8
+    assert seen.lens[:3] == [47, 12, 40]                                  # the last choice's: the prompt and seven of the answer
+    for row, (p, o) in enumerate(zip(prompts, out)):
+        assert seen.tokens[row, :len(p) + 7].tolist() == p + o[:7]
+        assert 9 not in o
+    # tokens that may not come again
+    out = engine.generate(prompts, 12, sampling=Sampling(presence=1e9))
+    assert all(len(set(o)) == 12 for o in out)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_generation_under_a_grammar(device):
+    """Even tokens and odd ones in turn; one sequence may go on with nothing after its third token."""
+    model = model_of("llama", device, False)
+    engine = GenerationEngine(model, max_batch=3, max_seq_len=96, use_cuda_graph=device == "cuda")
+    ends = ids(31, 2)
+    prompts = [ids(20, 1), ends]
+
+    def allowed(prompt, answer):
+        if prompt == ends and len(answer) == 3:
+            return []
+        if len(answer) == 5:
+            return None
+        return torch.arange(512) % 2 == len(answer) % 2 if len(answer) < 2 else range(len(answer) % 2, 512, 2)
+
+    for sampling in (Sampling(allowed=allowed), Sampling(temperature=0.9, top_k=50, seed=3, repetition=1.1, allowed=allowed)):
+        out = engine.generate(prompts, 7, sampling=sampling)
+        assert len(out[0]) == 7 and all(t % 2 == i % 2 for i, t in enumerate(out[0]) if i != 5)
+        assert len(out[1]) == 3 and all(t % 2 == i % 2 for i, t in enumerate(out[1]))
+
+
+def test_refusals_of_sampling():
+    for kw in (dict(repetition=0.0), dict(repetition=-1.0), dict(repetition=float("inf")), dict(repetition=float("nan")), dict(frequency=float("nan")),
+               dict(presence=float("inf"))):
+        with pytest.raises(ValueError):
+            Sampling(**kw)
+    engine = GenerationEngine(model_of("llama", "cpu", False), max_batch=1, max_seq_len=64)
+    for bad in (512, -1):
+        with pytest.raises(ValueError):
+            engine.generate([ids(4, 1)], 2, sampling=Sampling(biases={bad: 1.0}))
+
+
+def test_command_line(capsys):
+    import argparse
+
+    from nkipy_b200.models import runner
+
+    ap = argparse.ArgumentParser()
+    runner.add_common_args(ap)
+    args = ap.parse_args(["--tiny", "--layers", "2", "-n", "3", "--prompt-len", "20", "--weight-dtype", "int8", "--repetition-penalty", "1.2",
+                          "--frequency-penalty", "0.1", "--presence-penalty", "0.1"])
+    assert runner.sampling_of(args).ruled and not runner.sampling_of(ap.parse_args([])).ruled
+    assert runner.run_generation(C.llama3_8b(num_layers=2), args) == 0
+    assert "Generated 3 tokens" in capsys.readouterr().out
+    with pytest.raises(ValueError):
+        runner.quantize_weights(args, object())
