@@ -83,6 +83,7 @@ int nkb_gemm_bf16(const void* A, const void* B, void* out, int rows, int cols, i
 int nkb_quant_rows(const void* args);
 int nkb_gemm_i8(const void* args);
 int nkb_linear_i8(const void* rows, const void* gemm);
+int nkb_gemm_i8_few(const void* rows, const void* gemm);
 int nkb_gemm_i8_splits(int k, int splits);
 int nkb_logit_rules(const void* args);
 int nkb_gemm_effective_splits(int k, int splits);

@@ -15,21 +15,13 @@
 // columns per thread and turn, kept in registers between the pass for the maximum and the one that writes; rows too wide for them are
 // computed twice.
 #include "api.h"
-#include "common.cuh"
 #include "i8_args.h"
+#include "quant_rows.cuh"
 
 namespace nkb {
 
-// Distance from a whole number beyond which a number is decided exactly: half, less the error of 127 x / m in 32 bits (two roundings, some
-// 2^-16 at 127); for gated rows less 127 times the 2^-20 of a gated value in 32 bits.
-constexpr float kNearHalf = 0.5f - 1.f / (1 << 15), kNearHalfGated = 0.5f - 1.f / 4096;
 constexpr float kGateSmall = 1.f / (1 << 20);   // rows with a smaller maximum are gated in 64 bits: their 32-bit errors are not small beside it
 
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
 __device__ __forceinline__ float min_nan(float a, float b) {
   float d;
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
@@ -45,44 +37,6 @@ __device__ __forceinline__ double gate64(double g, double u, float limit, float 
   return g / (1.0 + exp(-g)) * u;
 }
 
-// 8 columns from `c` on of a row, as they lie in memory; columns past the width read as zeros.  VEC: rows start on 16 bytes.  (Through the read-only
-// path: a thread's loads may then go ahead of its stores, which in place follow the loads of the same columns.)
-template <bool VEC>
-__device__ __forceinline__ uint4 fetch8_bf16(const void* row, int c, int width) {
-  if (VEC && c + 8 <= width) return __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(row) + c));
-  uint32_t w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (c + j < width) w[j >> 1] |= uint32_t(__ldg(reinterpret_cast<const uint16_t*>(row) + c + j)) << (16 * (j & 1));
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-template <bool VEC>
-__device__ __forceinline__ void fetch8_f32(const float* row, int c, int width, uint4 (&r)[2]) {
-  if (VEC && c + 8 <= width) {
-    r[0] = __ldg(reinterpret_cast<const uint4*>(row + c));
-    r[1] = __ldg(reinterpret_cast<const uint4*>(row + c) + 1);
-    return;
-  }
-  uint32_t w[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) w[j] = c + j < width ? __ldg(reinterpret_cast<const uint32_t*>(row) + c + j) : 0u;
-  r[0] = make_uint4(w[0], w[1], w[2], w[3]);
-  r[1] = make_uint4(w[4], w[5], w[6], w[7]);
-}
-__device__ __forceinline__ void values8_bf16(const uint4& r, float (&v)[8]) {
-  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float2 f = unpack_bf16x2(w[e]);
-    v[2 * e] = f.x;
-    v[2 * e + 1] = f.y;
-  }
-}
-__device__ __forceinline__ void values8_f32(const uint4 (&r)[2], float (&v)[8]) {
-  const uint32_t w[8] = {r[0].x, r[0].y, r[0].z, r[0].w, r[1].x, r[1].y, r[1].z, r[1].w};
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
-}
 template <bool VEC>
 __device__ __forceinline__ void load8_bf16(const void* row, int c, int width, float (&v)[8]) {
   values8_bf16(fetch8_bf16<VEC>(row, c, width), v);
@@ -285,30 +239,6 @@ __device__ __forceinline__ void load8(const NkbQuantRows& a, long long row, int 
   }
 }
 
-// The numbers of 8 columns by the exact comparison.  WIDE: x and m have 24 bits, the sides of the comparison 32.
-template <bool WIDE>
-__device__ __noinline__ uint2 exact8(const float (&x)[8], float m) {
-  // a power of two that keeps 254 |x| and 127 / m inside the range of 32 bits
-  const float f = m < 1e-18f ? 1.1805916207174113e21f : (m > 1e18f ? 8.470329472543003e-22f : 1.f);
-  const float mf = m * f, inv = mf > 0.f ? 127.f / mf : 0.f;
-  uint32_t packed[2] = {0u, 0u};
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float ax = fabsf(x[j]) * f, k = floorf(ax * inv);
-    bool up;
-    if constexpr (WIDE) {
-      const double l = 254.0 * double(ax), r = (2.0 * double(k) + 1.0) * double(mf);
-      up = l > r || (l == r && (int(k) & 1));
-    } else {
-      const float l = 254.f * ax, r = (2.f * k + 1.f) * mf;
-      up = l > r || (l == r && (int(k) & 1));
-    }
-    const int q = int(k) + (up ? 1 : 0);
-    packed[j >> 2] |= uint32_t((x[j] < 0.f ? -q : q) & 255) << (8 * (j & 3));
-  }
-  return make_uint2(packed[0], packed[1]);
-}
-
 // What a CTA of a cluster tells the others about its part of the row.
 struct RowPart {
   unsigned long long top64;
@@ -470,47 +400,37 @@ __global__ void __maxnreg__(row_registers(FORM, IT)) quant_rows_kernel(const Nkb
     a.scale[row] = fine ? scale : __uint_as_float(0x7fffffffu);
   }
   // Rows whose m or 127 / m is at an end of the range: every number by the comparison, scaled by a power of two.
-  const bool odd = m < 1e-18f || m > 1e18f;
+  const bool odd = odd_row(m);
   const float inv = odd ? 0.f : 127.f / m;
   uint8_t* out = reinterpret_cast<uint8_t*>(a.values) + row * a.q_ld;
   auto finish = [&](float (&x)[8], int ch) {
     uint32_t packed[2] = {0u, 0u};
-    if (fine) {
-      // 127 x / m + 1.5 * 2^23 rounds to the nearest whole number, whose lowest byte is then that of the sum
-      uint32_t t[8], again = 0;
-      float most = 0.f;
+    if constexpr (!kGate) {
+      if (fine) {
+        const uint2 q = numbers8<FORM == NKB_ROW_F32>(x, m, inv, odd);
+        packed[0] = q.x;
+        packed[1] = q.y;
+      }
+    } else if (fine) {
+      uint32_t t[8], again = 0;           // as numbers8, and columns beside a half in 64 bits
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float s = fmaf(x[j], inv, 12582912.f);
         t[j] = __float_as_uint(s);
-        const float d = fabsf(fmaf(x[j], inv, 12582912.f - s));
-        most = fmaxf(most, d);
-        if constexpr (kGate) again |= d > kNearHalfGated ? 1u << j : 0u;
+        again |= fabsf(fmaf(x[j], inv, 12582912.f - s)) > kNearHalfGated ? 1u << j : 0u;
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         packed[i] = __byte_perm(__byte_perm(t[4 * i], t[4 * i + 1], 0x0040), __byte_perm(t[4 * i + 2], t[4 * i + 3], 0x0040), 0x5410);
-      if constexpr (kGate) {
-        if (in64) again = m64 > 0.0 ? 255u : 0u;
-        if (again) {
+      if (in64) again = m64 > 0.0 ? 255u : 0u;
 #pragma unroll 1
-          for (; again; again &= again - 1u) {
-            const int j = __ffs(again) - 1;
-            if (ch * 8 + j >= a.width) break;
-            const double y = gate_exact<FORM>(a, row, ch * 8 + j);
-            const uint32_t q = uint32_t(int(rint(127.0 * (y / m64))) & 255), at = 8 * (j & 3);
-            if (j < 4) packed[0] = (packed[0] & ~(255u << at)) | q << at;
-            else packed[1] = (packed[1] & ~(255u << at)) | q << at;
-          }
-        }
-      } else if (most > kNearHalf || odd) {
-        // (copies: what a call may reach has to lie in memory)
-        float y[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = x[j];
-        const uint2 p = exact8<FORM == NKB_ROW_F32>(y, m);
-        packed[0] = p.x;
-        packed[1] = p.y;
+      for (; again; again &= again - 1u) {
+        const int j = __ffs(again) - 1;
+        if (ch * 8 + j >= a.width) break;
+        const double y = gate_exact<FORM>(a, row, ch * 8 + j);
+        const uint32_t q = uint32_t(int(rint(127.0 * (y / m64))) & 255), at = 8 * (j & 3);
+        if (j < 4) packed[0] = (packed[0] & ~(255u << at)) | q << at;
+        else packed[1] = (packed[1] & ~(255u << at)) | q << at;
       }
     }
     *reinterpret_cast<uint2*>(out + ch * 8) = make_uint2(packed[0], packed[1]);

@@ -1,0 +1,101 @@
+// Rows brought into 8-bit whole numbers, device code of quant_rows.cu and gemm_i8_few.cu (compiled without fast math): quant_rows.cu has the mathematics.
+#pragma once
+#include "common.cuh"
+
+namespace nkb {
+
+// Distance from a whole number beyond which a number is decided exactly: half, less the error of 127 x / m in 32 bits (two roundings, some
+// 2^-16 at 127); for gated rows less 127 times the 2^-20 of a gated value in 32 bits.
+constexpr float kNearHalf = 0.5f - 1.f / (1 << 15), kNearHalfGated = 0.5f - 1.f / 4096;
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+// 8 columns from `c` on of a row, as they lie in memory; columns past the width read as zeros.  VEC: rows start on 16 bytes.  (Through the read-only
+// path: a thread's loads may then go ahead of its stores, which in place follow the loads of the same columns.)
+template <bool VEC>
+__device__ __forceinline__ uint4 fetch8_bf16(const void* row, int c, int width) {
+  if (VEC && c + 8 <= width) return __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(row) + c));
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (c + j < width) w[j >> 1] |= uint32_t(__ldg(reinterpret_cast<const uint16_t*>(row) + c + j)) << (16 * (j & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <bool VEC>
+__device__ __forceinline__ void fetch8_f32(const float* row, int c, int width, uint4 (&r)[2]) {
+  if (VEC && c + 8 <= width) {
+    r[0] = __ldg(reinterpret_cast<const uint4*>(row + c));
+    r[1] = __ldg(reinterpret_cast<const uint4*>(row + c) + 1);
+    return;
+  }
+  uint32_t w[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) w[j] = c + j < width ? __ldg(reinterpret_cast<const uint32_t*>(row) + c + j) : 0u;
+  r[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  r[1] = make_uint4(w[4], w[5], w[6], w[7]);
+}
+__device__ __forceinline__ void values8_bf16(const uint4& r, float (&v)[8]) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float2 f = unpack_bf16x2(w[e]);
+    v[2 * e] = f.x;
+    v[2 * e + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void values8_f32(const uint4 (&r)[2], float (&v)[8]) {
+  const uint32_t w[8] = {r[0].x, r[0].y, r[0].z, r[0].w, r[1].x, r[1].y, r[1].z, r[1].w};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
+}
+// The numbers of 8 columns by the exact comparison.  WIDE: x and m have 24 bits, the sides of the comparison 32.
+template <bool WIDE>
+__device__ __noinline__ uint2 exact8(const float (&x)[8], float m) {
+  // a power of two that keeps 254 |x| and 127 / m inside the range of 32 bits
+  const float f = m < 1e-18f ? 1.1805916207174113e21f : (m > 1e18f ? 8.470329472543003e-22f : 1.f);
+  const float mf = m * f, inv = mf > 0.f ? 127.f / mf : 0.f;
+  uint32_t packed[2] = {0u, 0u};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float ax = fabsf(x[j]) * f, k = floorf(ax * inv);
+    bool up;
+    if constexpr (WIDE) {
+      const double l = 254.0 * double(ax), r = (2.0 * double(k) + 1.0) * double(mf);
+      up = l > r || (l == r && (int(k) & 1));
+    } else {
+      const float l = 254.f * ax, r = (2.f * k + 1.f) * mf;
+      up = l > r || (l == r && (int(k) & 1));
+    }
+    const int q = int(k) + (up ? 1 : 0);
+    packed[j >> 2] |= uint32_t((x[j] < 0.f ? -q : q) & 255) << (8 * (j & 3));
+  }
+  return make_uint2(packed[0], packed[1]);
+}
+
+// The numbers nearest to 127 x / m of 8 columns; inv: 127 / m, or 0 for rows at an end of the range (`odd`), whose numbers are all decided exactly.
+// 127 x / m + 1.5 * 2^23 rounds to the nearest whole number, whose lowest byte is then that of the sum; beside a half the comparison decides.
+template <bool WIDE>
+__device__ __forceinline__ uint2 numbers8(const float (&x)[8], float m, float inv, bool odd) {
+  uint32_t t[8];
+  float most = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float s = fmaf(x[j], inv, 12582912.f);
+    t[j] = __float_as_uint(s);
+    most = fmaxf(most, fabsf(fmaf(x[j], inv, 12582912.f - s)));
+  }
+  if (most > kNearHalf || odd) {
+    // (copies: what a call may reach has to lie in memory)
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = x[j];
+    return exact8<WIDE>(y, m);
+  }
+  return make_uint2(__byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(t[4], t[5], 0x0040), __byte_perm(t[6], t[7], 0x0040), 0x5410));
+}
+__device__ __forceinline__ bool odd_row(float m) { return m < 1e-18f || m > 1e18f; }
+
+}  // namespace nkb

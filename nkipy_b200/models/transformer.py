@@ -199,6 +199,12 @@ class TransformerLM:
             act = ops.silu_mul(ops.linear(normed, lw.gate_up), limit=cfg.swiglu_limit, alpha=cfg.swiglu_alpha, quantize=self.quantized)
         return self._row_parallel_reduce(act, lw.down, self.split_down, resid, next_norm, None, quantize)
 
+    def _sums(self, x, w, splits):
+        """fp32 partial sums of a decode step's product; of few rows by weights in 8 bits, whose kernel finishes them, the results."""
+        if self.quantized and x.shape[0] <= ops.quantized_linear.FEW_ROWS:
+            return ops.linear(x, w, fp32_out=True)
+        return ops.linear(x, w, splits=splits)
+
     def _row_parallel_reduce(self, x, w, splits, resid, next_norm, bias, quantize=False):
         """Row-parallel GEMM + sum over ranks + residual + next RMSNorm (decode-sized M; in 8 bits if `quantize`)."""
         cfg = self.cfg
@@ -207,7 +213,7 @@ class TransformerLM:
                 h = ops.decode_linear(x, w, splits=splits, bias=bias, residual=resid)
                 return h, ops.rmsnorm(h, next_norm, cfg.rms_eps)
             if splits > 1:
-                parts = ops.linear(x, w, splits=splits)
+                parts = self._sums(x, w, splits)
                 return ops.add_rmsnorm(None, next_norm, residual_in=resid, partials=parts, bias=bias,
                                        eps=cfg.rms_eps, quantize=quantize)
             y = ops.linear(x, w)
@@ -253,7 +259,7 @@ class TransformerLM:
                                         q_norm_w=lw.q_norm, k_norm_w=lw.k_norm, norm_eps=cfg.rms_eps)
             else:
                 if self.split_qkv > 1:
-                    qkv = ops.linear(normed, lw.qkv, splits=self.split_qkv)
+                    qkv = self._sums(normed, lw.qkv, self.split_qkv)
                 else:
                     qkv = ops.linear(normed, lw.qkv)
                 if (ops.fused_rope_attn_enabled(self.tp.world_size) and q_len == 1 and qkv.dtype == torch.float32 and qkv.is_cuda

@@ -45,7 +45,7 @@ NVCC_FLAGS = [
 # files keep IEEE division and sqrt.
 NO_FAST_MATH = {"sampling.cu", "elementwise.cu", "decode_layer.cu", "gated_residual.cu", "recurrent.cu", "attn_maps.cu",
                 "gemm_simt.cu", "gemm_f32_split.cu", "linear_attn.cu", "latent_attn.cu", "head_recurrence.cu", "post_residual.cu",
-                "append_q8.cu", "quant_rows.cu", "logit_rules.cu"}
+                "append_q8.cu", "quant_rows.cu", "gemm_i8_few.cu", "logit_rules.cu"}
 
 
 # what a single-GPU decoder of models/hybrid.py launches

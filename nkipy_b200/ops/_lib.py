@@ -205,6 +205,7 @@ _SIGNATURES = {
     # (packed arguments: csrc/kernels/i8_args.h, rules_args.h)
     "nkb_quant_rows": (c_int, [c_char_p]),
     "nkb_linear_i8": (c_int, [c_char_p, c_char_p]),
+    "nkb_gemm_i8_few": (c_int, [c_char_p, c_char_p]),
     "nkb_gemm_i8_splits": (c_int, [c_int, c_int]),
     "nkb_logit_rules": (c_int, [c_char_p]),
     "nkb_decode_advance": (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, c_int, _P]),

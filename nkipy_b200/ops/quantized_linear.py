@@ -26,6 +26,7 @@ from . import _lib
 from . import _count_launch, _stream, mixers
 
 MAX_K = 133144                       # 127 * 127 * k stays below 2^31
+FEW_ROWS, FEW_BYTES = 2, 98304       # rows, and bytes of them in 8 bits, that the kernel for few tokens takes (gemm_i8_few.cu)
 # NkbQuantRows and NkbGemmI8 of csrc/kernels/i8_args.h
 _ROWS, _GEMM = struct.Struct("9P3q4i3fi"), struct.Struct("8P4q8i")
 
@@ -328,7 +329,20 @@ def linear(x, w: QuantizedWeight, *, bias=None, residual=None, out=None, splits:
         return out
     if not _on_gpu(index):
         return _reference(x if given else quantize_rows(x), w, bias, residual, out, parts, gated, act, N)
-    stream = _stream()
+    stream, form = _stream(), 0 if given or x.dtype is _BF16 else 1
+    more = (bias_at, 0 if residual is None else residual.data_ptr(), out.data_ptr(), stream)
+    ends = (w.ld, ldo, out.stride(0) if parts else 0, M, N, K, gated, mixers.ACTIVATIONS[act][0] if gated else 0, dtype is _F32, parts,
+            weights_static)
+    if M <= FEW_ROWS and not parts and M * ((K + 511) & -512) <= FEW_BYTES:
+        if given:
+            rows, at, q_ld = None, x.at, x.ld
+        else:
+            rows, at, q_ld = _ROWS.pack(x.data_ptr(), 0, 0, 0, 0, 0, 0, 0, stream, x_ld, 0, 0, form, M, K, 0, 0.0, 0.0, 0.0, 0), (0, 0), 0
+        rc = _lib.lib().nkb_gemm_i8_few(rows, _GEMM.pack(at[0], w.at[0], at[1], w.at[1], *more, q_ld, *ends))
+        if rc:
+            _lib.check(rc, "nkb_gemm_i8_few")
+        _count_launch()
+        return out
     if given:
         (q_at, scale_at), q_ld, rows = x.at, x.ld, None
     else:
@@ -337,10 +351,8 @@ def linear(x, w: QuantizedWeight, *, bias=None, residual=None, out=None, splits:
         buffer = torch.empty_strided((M * (q_ld + 4),), (1,), dtype=torch.int8, device=w.device)
         q_at = buffer.data_ptr()
         scale_at = q_at + M * q_ld
-        rows = _ROWS.pack(x.data_ptr(), 0, 0, 0, 0, 0, q_at, scale_at, stream, x_ld, q_ld, 0, 0 if x.dtype is _BF16 else 1, M, K, 0, 0.0, 0.0, 0.0, 0)
-    rc = _lib.lib().nkb_linear_i8(rows, _GEMM.pack(
-        q_at, w.at[0], scale_at, w.at[1], bias_at, 0 if residual is None else residual.data_ptr(), out.data_ptr(), stream, q_ld, w.ld, ldo,
-        out.stride(0) if parts else 0, M, N, K, gated, mixers.ACTIVATIONS[act][0] if gated else 0, dtype is _F32, parts, weights_static))
+        rows = _ROWS.pack(x.data_ptr(), 0, 0, 0, 0, 0, q_at, scale_at, stream, x_ld, q_ld, 0, form, M, K, 0, 0.0, 0.0, 0.0, 0)
+    rc = _lib.lib().nkb_linear_i8(rows, _GEMM.pack(q_at, w.at[0], scale_at, w.at[1], *more, q_ld, *ends))
     if rc:
         _lib.check(rc, "nkb_linear_i8")
     _count_launch(1 if given else 2)
