@@ -1,6 +1,6 @@
 // Products of rows and weights in 8-bit whole numbers: y[m, n] = sx[m] * sw[n] * sum_k x[m, k] w[n, k], both operands K-major.
 //
-// The sums are whole numbers of 32 bits (at most 127 * 127 * k, so k is up to 133144), exact whatever their order; the only roundings are
+// The sums are whole numbers of 32 bits (at most 128 * 128 * k, so k is up to 131071), exact whatever their order; the only roundings are
 // those of the epilogue: sum -> fp32, times sx, times sw, + bias, + residual, -> bf16.  So every variant below gives the same bits.
 //
 // Two kernels:
@@ -18,7 +18,7 @@ namespace nkb {
 
 constexpr int kI8Slab = 128;                       // bytes (numbers) of k per stage: one swizzled row
 constexpr int kI8ATile = 128 * kI8Slab;            // 16 KB
-constexpr int kI8MaxK = 133144;                    // 127 * 127 * k < 2^31
+constexpr int kI8MaxK = 131071;                    // 128 * 128 * k < 2^31
 
 __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(

@@ -24,7 +24,7 @@ struct NkbQuantRows {
   long long x_ld, q_ld, split_stride;
   int form, rows, width, splits;
   float eps, limit, alpha;      // limit > 0: (up + 1) * gate * sigmoid(alpha * gate) of clamped gate and up
-  int unused;
+  int late;                     // the kernel behind this one starts after its end: it may take the rows for weights, which it fetches ahead of its wait
 };
 
 // y = x w^T of whole numbers, times both scales.

@@ -2,7 +2,8 @@
 //
 // Mathematics.  The quotient is never formed.  With k = floor(127 |x| / m), wrong by one at most in 32 bits, |q| is k + 1 where
 // 254 |x| > (2 k + 1) m, or where both are equal and k is odd, and k elsewhere; that also mends a k that is wrong by one.  Both sides have at
-// most 24 bits where |x| and m have 16, so the comparison is exact in 32 bits for bf16 rows and for products of two bf16 numbers.
+// most 24 bits where |x| and m have 16, so the comparison is exact in 32 bits for bf16 rows and for products of two bf16 numbers.  The form that runs
+// (numbers8 in quant_rows.cuh) takes the nearest k by a rounding constant and looks at what is left of it, which is exact, too.
 //   norm   The norm's factor r = 1 / sqrt(mean(h^2) + eps) is the same for the whole row: 127 (r h w) / max|r h w| = 127 (h w) / max|h w|.  So the numbers
 //          come from the exact products h * w, and r enters the scale alone: no rounding of statistics can move a number to its neighbour.
 //   gate   silu(g) * u is not exact in 32 bits.  Numbers within 2^-11 of a half (one in a thousand) and candidates for the row's maximum are worked out
@@ -268,7 +269,7 @@ __global__ void __maxnreg__(row_registers(FORM, IT)) quant_rows_kernel(const Nkb
   const int chunk0 = CLUSTER ? blockIdx.x * each : 0, chunks = min(all, chunk0 + each);      // [chunk0, chunks)
   if (threadIdx.x == 0) s_top64[0] = 0ull;
   griddep_wait();
-  griddep_launch();
+  if (!a.late) griddep_launch();
   Raw8<FORM> raw[kKeep ? IT : 1];
   auto fetch = [&](long long row, bool first) {
 #pragma unroll
@@ -283,14 +284,22 @@ __global__ void __maxnreg__(row_registers(FORM, IT)) quant_rows_kernel(const Nkb
   for (int turn = 0; row < a.rows; row += CLUSTER ? a.rows : gridDim.x, turn ^= 1) {
   float v[kKeep ? IT : 1][8];
   float big = 0.f, ss = 0.f;              // largest magnitude, NaN if there is one
+  uint32_t big16 = 0;
   if constexpr (kKeep) {
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
       const int ch = chunk0 + threadIdx.x + it * blockDim.x;
       if (ch >= chunks) continue;
       load8<FORM, VEC>(a, row, ch * 8, raw[it], v[it], ss);
+      if constexpr (FORM == NKB_ROW_BF16) {
+        // magnitudes of bf16 are ordered as their bits are: two to a word
+        const uint4 w = raw[it].r[0];
+        big16 = __vimax3_s16x2(big16, w.x & 0x7fff7fffu, w.y & 0x7fff7fffu);
+        big16 = __vimax3_s16x2(big16, w.z & 0x7fff7fffu, w.w & 0x7fff7fffu);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) big = max_nan(big, fabsf(v[it][j]));
+        for (int j = 0; j < 8; ++j) big = max_nan(big, fabsf(v[it][j]));
+      }
     }
     // the next row's loads are on their way while this one is finished
     if (!CLUSTER && row + gridDim.x < a.rows) fetch(row + gridDim.x, false);
@@ -333,6 +342,7 @@ __global__ void __maxnreg__(row_registers(FORM, IT)) quant_rows_kernel(const Nkb
     fetch8<FORM, VEC>(again_a, row, ch * 8, raw[0], true);
     load8<FORM, VEC>(again_a, row, ch * 8, raw[0], v[0], none);
   };
+  if (kKeep && FORM == NKB_ROW_BF16) big = __uint_as_float(max(big16 << 16, big16 & 0xffff0000u));
   uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(big));      // infinities and NaN lie above all numbers
   if constexpr (FORM == NKB_ROW_NORM) ss = warp_sum(ss);
   if (lane == 0) {

@@ -4,9 +4,8 @@
 
 namespace nkb {
 
-// Distance from a whole number beyond which a number is decided exactly: half, less the error of 127 x / m in 32 bits (two roundings, some
-// 2^-16 at 127); for gated rows less 127 times the 2^-20 of a gated value in 32 bits.
-constexpr float kNearHalf = 0.5f - 1.f / (1 << 15), kNearHalfGated = 0.5f - 1.f / 4096;
+// Distance from a whole number beyond which a gated one is decided in 64 bits: half, less 127 times the 2^-20 of a gated value in 32 bits.
+constexpr float kNearHalfGated = 0.5f - 1.f / 4096;
 __device__ __forceinline__ float max_nan(float a, float b) {
   float d;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
@@ -74,24 +73,45 @@ __device__ __noinline__ uint2 exact8(const float (&x)[8], float m) {
   return make_uint2(packed[0], packed[1]);
 }
 
-// The numbers nearest to 127 x / m of 8 columns; inv: 127 / m, or 0 for rows at an end of the range (`odd`), whose numbers are all decided exactly.
-// 127 x / m + 1.5 * 2^23 rounds to the nearest whole number, whose lowest byte is then that of the sum; beside a half the comparison decides.
+// The numbers nearest to 127 x / m of 8 columns; inv: 127 / m.  odd: rows at an end of the range, by the comparison alone.
+// 127 x / m + 1.5 * 2^23 rounds to a whole number k, whose lowest byte is then that of the sum.  inv is rounded, so beside a half k may be a neighbour's;
+// what is left, r = 127 x - k m, says so: 127 x and k m have at most 24 bits, and r is exact.  Halves themselves are common (x = m / 2 is one: half a
+// percent of a normal row in bf16, three of ten warps' pieces), so they are mended in place.  WIDE: x and m have 24 bits; r in 64 where it is near m / 2.
 template <bool WIDE>
 __device__ __forceinline__ uint2 numbers8(const float (&x)[8], float m, float inv, bool odd) {
-  uint32_t t[8];
-  float most = 0.f;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float s = fmaf(x[j], inv, 12582912.f);
-    t[j] = __float_as_uint(s);
-    most = fmaxf(most, fabsf(fmaf(x[j], inv, 12582912.f - s)));
-  }
-  if (most > kNearHalf || odd) {
+  if (odd) {
     // (copies: what a call may reach has to lie in memory)
     float y[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[j] = x[j];
     return exact8<WIDE>(y, m);
+  }
+  uint32_t t[8];
+  float r[8], most = 0.f;
+  const float2 inv2 = make_float2(inv, inv), one = make_float2(12582912.f, 12582912.f), less = make_float2(-1.f, -1.f);
+  const float2 m2 = make_float2(m, m), top = make_float2(127.f, 127.f);
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {        // two columns an instruction
+    const float2 v = make_float2(x[j], x[j + 1]), s = ffma2(v, inv2, one), left = ffma2(ffma2(s, less, one), m2, fmul2(v, top));
+    t[j] = __float_as_uint(s.x);
+    t[j + 1] = __float_as_uint(s.y);
+    r[j] = left.x;
+    r[j + 1] = left.y;
+    most = fmax3(most, fabsf(left.x), fabsf(left.y));
+  }
+  if (2.f * most >= (WIDE ? m * (1.f - 1.f / 1024) : m)) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      bool over;
+      if constexpr (WIDE) {
+        const double k = double(__uint_as_float(t[j]) - 12582912.f), e = 2.0 * fabs(127.0 * double(x[j]) - k * double(m));
+        over = e > double(m) || (e == double(m) && (t[j] & 1u));
+      } else {
+        const float e = 2.f * fabsf(r[j]);
+        over = e > m || (e == m && (t[j] & 1u));
+      }
+      if (over) t[j] += r[j] > 0.f ? 1u : 0xffffffffu;
+    }
   }
   return make_uint2(__byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410),
                     __byte_perm(__byte_perm(t[4], t[5], 0x0040), __byte_perm(t[6], t[7], 0x0040), 0x5410));

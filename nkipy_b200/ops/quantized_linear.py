@@ -25,7 +25,7 @@ import torch
 from . import _lib
 from . import _count_launch, _stream, mixers
 
-MAX_K = 133144                       # 127 * 127 * k stays below 2^31
+MAX_K = 131071                       # 128 * 128 * k stays below 2^31
 FEW_ROWS, FEW_BYTES = 2, 98304       # rows, and bytes of them in 8 bits, that the kernel for few tokens takes (gemm_i8_few.cu)
 # NkbQuantRows and NkbGemmI8 of csrc/kernels/i8_args.h
 _ROWS, _GEMM = struct.Struct("9P3q4i3fi"), struct.Struct("8P4q8i")
@@ -137,7 +137,7 @@ def _numbers(x: torch.Tensor):
 
 
 def _launch_rows(form, rows, width, device, index, x=0, partials=0, bias=0, residual=0, w=0, residual_out=0, x_ld=0, split_stride=0,
-                 splits=0, eps=0.0, limit=0.0, alpha=0.0) -> QuantizedRows:
+                 splits=0, eps=0.0, limit=0.0, alpha=0.0, late=0) -> QuantizedRows:
     # (the kernel writes the columns up to the next sixteen, too)
     ld = (width + 15) & -16
     values = torch.empty_strided((rows, width), (ld, 1), dtype=torch.int8, device=device) if ld == width else \
@@ -145,7 +145,7 @@ def _launch_rows(form, rows, width, device, index, x=0, partials=0, bias=0, resi
     scale = torch.empty_strided((rows,), (1,), dtype=_F32, device=device)
     rc = _lib.lib().nkb_quant_rows(_ROWS.pack(
         x, partials, bias, residual, w, residual_out, values.data_ptr(), scale.data_ptr(), _stream(), x_ld, ld, split_stride, form, rows,
-        width, splits, eps, limit, alpha, 0))
+        width, splits, eps, limit, alpha, late))
     if rc:
         _lib.check(rc, "nkb_quant_rows")
     _count_launch()
@@ -172,7 +172,8 @@ def quantize_rows(x: torch.Tensor) -> QuantizedRows:
     if not _on_gpu(index):
         q, top = _numbers(x.double())
         return QuantizedRows(q, (top / 127).float())
-    return _launch_rows(0 if x.dtype is _BF16 else 1, rows, width, x.device, index, x=x.data_ptr(), x_ld=ld)
+    # (late: they may become a weight, which a product right behind fetches ahead of its wait)
+    return _launch_rows(0 if x.dtype is _BF16 else 1, rows, width, x.device, index, x=x.data_ptr(), x_ld=ld, late=1)
 
 
 def add_rmsnorm(x, w, *, residual_in=None, partials=None, bias=None, residual_out=None, eps=1e-6, hidden=None, rows=None):

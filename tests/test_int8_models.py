@@ -121,6 +121,20 @@ def test_models_that_have_none():
     assert model.quantize_weights() is model and model.layers[0].qkv is first
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_verified_drafts(device):
+    from nkipy_b200.models.speculative import DrafterLM, EagleConfig, SpeculativeEngine, random_drafter_weights
+
+    cfg = C.tiny(num_heads=4, num_kv_heads=2, head_dim=64, num_layers=4)
+    target = TransformerLM(cfg, random_weights(cfg, 0, 1, seed=5, std=0.05), device=device).quantize_weights()
+    ecfg = EagleConfig(hidden_size=cfg.hidden_size, target_hidden_size=cfg.hidden_size, num_heads=4, num_kv_heads=4, head_dim=64,
+                       intermediate_size=256, draft_vocab_size=cfg.vocab_size, vocab_size=cfg.vocab_size, num_draft_tokens=3, ptd_token_id=3)
+    drafter = DrafterLM(ecfg, random_drafter_weights(ecfg, seed=9, std=0.05), device)
+    spec = SpeculativeEngine(target, drafter, max_batch=2, max_seq_len=96)
+    out = spec.generate([ids(19, 1), ids(33, 2)], 6)
+    assert all(len(o) == 6 for o in out)
+
+
 # ------------------------------------------------------------------------------------------------ rules
 class Chosen:
     """Follows every choice under rules by the oracle."""

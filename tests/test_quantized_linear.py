@@ -481,3 +481,52 @@ def test_streams_beside_one_another():
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 64, 300])
+def test_weights_made_right_ahead_of_their_product(m):
+    """The product fetches weights ahead of its wait for the kernel before it, which is the one that makes them."""
+    g = draws(m)
+    x = ops.quantize_rows(rows_like_a_layers(g, m, 2048).cuda())
+    ws = [weight_like(g, 4096, 2048).cuda() for _ in range(4)]
+    want = []
+    for w in ws:
+        q = ops.QuantizedWeight.of(w)
+        torch.cuda.synchronize()
+        want.append(ops.linear(x, q))
+    junk = torch.full((4096 * 2048,), 99, dtype=torch.int8, device="cuda")
+    for _ in range(5):
+        for w, y in zip(ws, want):
+            del junk                                                 # (the new weight's memory has other numbers)
+            q = ops.QuantizedWeight.of(w)
+            got = ops.linear(x, q)
+            assert torch.equal(got, y)
+            del q
+            junk = torch.full((4096 * 2048,), 99, dtype=torch.int8, device="cuda")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_the_lowest_number(device):
+    """-128, which no row that was brought into 8 bits here has, counts as what it is."""
+    v = torch.randint(-128, 128, (70, 300), dtype=torch.int8, generator=draws(0))
+    v[:, ::3] = -128
+    x, w = ops.QuantizedRows(v, torch.rand(70)), ops.QuantizedWeight(v.flip(0), torch.rand(70))
+    for m in (1, 2, 40, 70):
+        rows = ops.QuantizedRows(x.values[:m].contiguous(), x.scale[:m])
+        want, tol = oracle_product(rows.values, rows.scale, w.values, w.scale, fp32=True)
+        check_product(ops.linear(there(rows, device), there(w, device), fp32_out=True), want, tol)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_normed_rows_in_the_place_of_the_stream(device):
+    """The residual stream may be written where it, or what is added, was; narrow rows and ones that are computed twice."""
+    for k in (64, 4096, 20000):
+        g = draws(k)
+        x, r = rows_like_a_layers(g, 3, k), rows_like_a_layers(g, 3, k)
+        w = torch.ones(k, dtype=BF)
+        want, rows = ops.add_rmsnorm(x.to(device), w.to(device), residual_in=r.to(device), quantize=True)
+        for place in (0, 1):
+            a, b = x.to(device, copy=True), r.to(device, copy=True)
+            h, q = ops.add_rmsnorm(a, w.to(device), residual_in=b, residual_out=(a, b)[place], quantize=True)
+            assert h is (a, b)[place] and torch.equal(h, want) and torch.equal(q.values, rows.values) and torch.equal(q.scale, rows.scale)
