@@ -20,7 +20,7 @@ from .quantized_linear import _on_gpu
 _ARGS = struct.Struct("15P5q6i")          # NkbLogitRules of csrc/kernels/rules_args.h
 
 
-@dataclass
+@dataclass(slots=True)
 class LogitRules:
     """What is done to the logits [rows, vocab] of a step, in 64 bits and rounded once, in this order:
 
@@ -63,15 +63,14 @@ def pack_mask(allowed: torch.Tensor) -> torch.Tensor:
     return torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32)
 
 
-def _vector(t, name, dtype, rows, index):
+def _vector(t, name, dtype, shape, index):
     if t is None:
         return 0
-    if t.dtype is dtype and t.shape == (rows,) and t.get_device() == index and t.is_contiguous():
+    if t.dtype is dtype and t.shape == shape and t.get_device() == index and t.is_contiguous():
         return t.data_ptr()
     if t.dtype is not dtype:
         raise TypeError(f"{name} wants {dtype}, not {t.dtype}")
-    if t.shape != (rows,) or t.get_device() != index or not t.is_contiguous():
-        raise ValueError(f"{name} wants to be contiguous [{rows}], on the logits' device")
+    raise ValueError(f"{name} wants to be contiguous {list(shape)}, on the logits' device")
 
 
 def _matrix(t, name, dtype, rows, index):
@@ -80,52 +79,68 @@ def _matrix(t, name, dtype, rows, index):
         return 0, 0
     if t.dtype is not dtype:
         raise TypeError(f"{name} wants {dtype}, not {t.dtype}")
-    if t.dim() != 2 or (rows is not None and t.shape[0] != rows) or t.get_device() != index or (t.shape[1] > 1 and t.stride(1) != 1):
+    shape = t.shape
+    if len(shape) != 2 or (rows is not None and shape[0] != rows) or t.get_device() != index:
         raise ValueError(f"{name} wants rows of neighbouring numbers, one for each of the logits', on their device")
-    return t.data_ptr(), t.stride(0)
+    ld, column = t.stride()
+    if column != 1 and shape[1] > 1:
+        raise ValueError(f"{name} wants rows of neighbouring numbers, one for each of the logits', on their device")
+    return t.data_ptr(), ld
 
 
 def _packed(logits, rules: LogitRules, out, out_ids) -> bytes:
     if not isinstance(rules, LogitRules):
         raise TypeError("rules are LogitRules")
-    if logits.dtype not in (torch.bfloat16, torch.float32):
+    f32 = logits.dtype is torch.float32
+    if not f32 and logits.dtype is not torch.bfloat16:
         raise TypeError(f"rules want bf16 or fp32 logits, not {logits.dtype}")
-    if logits.dim() != 2 or logits.shape[1] < 1 or logits.shape[0] > 65535 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+    shape = logits.shape
+    if len(shape) != 2 or shape[1] < 1 or shape[0] > 65535:
         raise ValueError("rules want logits [rows, vocab], of 65535 rows at most, with neighbouring columns")
-    B, V = logits.shape
-    index = logits.get_device()
+    (B, V), (ld, column), at, index, r, rows = shape, logits.stride(), logits.data_ptr(), logits.get_device(), rules, shape[:1]
+    if column != 1 and V > 1:
+        raise ValueError("rules want logits [rows, vocab], of 65535 rows at most, with neighbouring columns")
     out_at, out_ld = _matrix(out, "out", logits.dtype, B, index)
-    if out is not None and (out.shape != logits.shape or (B > 1 and out_ld < V)):
-        raise ValueError("out wants the logits' shape")
-    if out is not None and out_at == logits.data_ptr() and B > 1 and out_ld != logits.stride(0):
-        raise ValueError("rows of out that lie over the logits want to be the same ones")
-    r, i32, f32 = rules, torch.int32, torch.float32
-    tokens, tokens_ld = _matrix(r.tokens, "tokens", i32, B, index)
-    if r.tokens is None:
-        if r.lens is not None or r.ids is not None or r.prompt_lens is not None:
-            raise ValueError("lens, prompt_lens and ids belong to tokens")
-        if r.repetition is not None or r.frequency is not None or r.presence is not None:
-            raise ValueError("penalties want the rows' tokens")
-    elif r.lens is None:
-        raise ValueError("tokens want lens")
-    if (r.bias_ids is None) != (r.bias_values is None):
-        raise ValueError("biases want ids and values")
-    bias_ids, bias_ld = _matrix(r.bias_ids, "bias_ids", i32, B, index)
-    bias_values, values_ld = _matrix(r.bias_values, "bias_values", f32, B, index)
-    if r.bias_ids is not None and (r.bias_ids.shape != r.bias_values.shape or (B > 1 and bias_ld != values_ld)):
-        raise ValueError("biases want as many values as ids, laid out the same")
-    mask, mask_ld = _matrix(r.mask, "mask", i32, None if r.mask_rows is not None else B, index)
-    if r.mask is not None and r.mask.shape[1] < mask_words(V):
-        raise ValueError(f"mask wants {mask_words(V)} words for a vocabulary of {V}")
-    if r.mask is None and r.mask_rows is not None:
+    if out is not None:
+        if out.shape != shape or (B > 1 and out_ld < V):
+            raise ValueError("out wants the logits' shape")
+        if out_at == at and B > 1 and out_ld != ld:
+            raise ValueError("rows of out that lie over the logits want to be the same ones")
+    i32, number = torch.int32, torch.float32
+    tokens = tokens_ld = width = lens = prompts = ids = rep = freq = pres = bias_ids = bias_values = bias_ld = biases = mask = mask_ld = masks = 0
+    mask_rows = 0
+    if r.tokens is not None:
+        if r.lens is None:
+            raise ValueError("tokens want lens")
+        tokens, tokens_ld = _matrix(r.tokens, "tokens", i32, B, index)
+        width = r.tokens.shape[1]
+        lens, prompts = _vector(r.lens, "lens", i32, rows, index), _vector(r.prompt_lens, "prompt_lens", i32, rows, index)
+        ids = _vector(r.ids, "ids", i32, rows, index)
+        rep = _vector(r.repetition, "repetition", number, rows, index)
+        freq, pres = _vector(r.frequency, "frequency", number, rows, index), _vector(r.presence, "presence", number, rows, index)
+    elif r.lens is not None or r.ids is not None or r.prompt_lens is not None:
+        raise ValueError("lens, prompt_lens and ids belong to tokens")
+    elif r.repetition is not None or r.frequency is not None or r.presence is not None:
+        raise ValueError("penalties want the rows' tokens")
+    if r.bias_ids is not None or r.bias_values is not None:
+        if r.bias_ids is None or r.bias_values is None:
+            raise ValueError("biases want ids and values")
+        (bias_ids, bias_ld), (bias_values, values_ld) = (_matrix(r.bias_ids, "bias_ids", i32, B, index),
+                                                         _matrix(r.bias_values, "bias_values", number, B, index))
+        if r.bias_ids.shape != r.bias_values.shape or (B > 1 and bias_ld != values_ld):
+            raise ValueError("biases want as many values as ids, laid out the same")
+        biases = r.bias_ids.shape[1]
+    if r.mask is not None:
+        mask, mask_ld = _matrix(r.mask, "mask", i32, None if r.mask_rows is not None else B, index)
+        masks, words = r.mask.shape
+        if words < mask_words(V):
+            raise ValueError(f"mask wants {mask_words(V)} words for a vocabulary of {V}")
+        mask_rows = _vector(r.mask_rows, "mask_rows", i32, rows, index)
+    elif r.mask_rows is not None:
         raise ValueError("mask_rows belong to masks")
-    return _ARGS.pack(
-        logits.data_ptr(), out_at, _vector(out_ids, "out_ids", i32, B, index), tokens, _vector(r.lens, "lens", i32, B, index),
-        _vector(r.prompt_lens, "prompt_lens", i32, B, index), _vector(r.ids, "ids", i32, B, index),
-        _vector(r.repetition, "repetition", f32, B, index), _vector(r.frequency, "frequency", f32, B, index),
-        _vector(r.presence, "presence", f32, B, index), bias_ids, bias_values, mask, _vector(r.mask_rows, "mask_rows", i32, B, index),
-        _stream() if index >= 0 else 0, logits.stride(0), out_ld, tokens_ld, bias_ld, mask_ld, B, V, r.tokens.shape[1] if tokens else 0,
-        r.bias_ids.shape[1] if bias_ids else 0, r.mask.shape[0] if mask else 0, logits.dtype is torch.float32)
+    return _ARGS.pack(at, out_at, _vector(out_ids, "out_ids", i32, rows, index), tokens, lens, prompts, ids, rep, freq, pres, bias_ids,
+                      bias_values, mask, mask_rows, _stream() if index >= 0 else 0, ld, out_ld, tokens_ld, bias_ld, mask_ld, B, V, width,
+                      biases, masks, f32)
 
 
 def _reference(logits, r: LogitRules) -> torch.Tensor:

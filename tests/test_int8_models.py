@@ -144,7 +144,7 @@ class Chosen:
         real = ops.logit_rules.argmax
 
         def checked(logits, rules, out_ids=None):
-            r = {k: v.cpu().clone() for k, v in vars(rules).items() if v is not None}
+            r = {k: v.cpu().clone() for k, v in ((f, getattr(rules, f)) for f in rules.__dataclass_fields__) if v is not None}
             got = real(logits, rules, out_ids)
             want, tokens = oracle(logits.cpu(), r)
             assert torch.equal(got.cpu(), oracle_ids(want))
