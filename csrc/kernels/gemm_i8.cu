@@ -9,7 +9,6 @@
 //   swap   D[features, tokens] for few tokens: 128 features fill the M side, up to 128 tokens the narrow one.  One tile per CTA and several CTAs per SM, so
 //          that one's start and end lie under another's loads; k may be divided among the CTAs of a cluster, whose sums are joined through distributed
 //          shared memory, or left as partial sums.
-#include <stdlib.h>
 #include "api.h"
 #include "gemm_tcgen05.cuh"
 #include "i8_args.h"

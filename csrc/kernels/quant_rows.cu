@@ -12,7 +12,7 @@
 //
 // The numbers are thus the same for every order of the sums and every launch shape, and equal those of the CPU.
 //
-// Layout: a CTA per row, or a cluster where there are few and long ones, whose parts meet through distributed shared memory; eight neighbouring
+// Layout: a CTA per row, or a cluster where there are few and long gated ones, whose parts meet through distributed shared memory; eight neighbouring
 // columns per thread and turn, kept in registers between the pass for the maximum and the one that writes; rows too wide for them are
 // computed twice.
 #include "api.h"
@@ -244,7 +244,6 @@ __device__ __forceinline__ void load8(const NkbQuantRows& a, long long row, int 
 struct RowPart {
   unsigned long long top64;
   uint32_t top;
-  float ss;
 };
 
 // Registers of a thread: as few as the chunks that it keeps and has on their way leave room for, since more warps hide more of the loads and barriers.
@@ -255,11 +254,12 @@ constexpr int row_registers(int form, int it) {
   return 128;
 }
 
-// Grid: a CTA per row, or (CLUSTER) a cluster along x per row y.  IT: chunks of eight columns that a thread keeps, 0: none, they are read twice.
+// Grid: a CTA per row, or (CLUSTER, gated rows) a cluster along x per row y.  IT: chunks of eight columns that a thread keeps, 0: none, they are read twice.
 template <int FORM, bool VEC, int IT, bool CLUSTER>
 __global__ void __maxnreg__(row_registers(FORM, IT)) quant_rows_kernel(const NkbQuantRows a) {
   constexpr bool kGate = FORM == NKB_ROW_GATE_BF16 || FORM == NKB_ROW_GATE_F32;
   constexpr bool kKeep = IT > 0;
+  static_assert(!CLUSTER || kGate, "only gated rows are divided");
   __shared__ uint32_t s_top[2][16];
   __shared__ float s_ss[2][16];
   __shared__ unsigned long long s_top64[2];
@@ -379,27 +379,20 @@ __global__ void __maxnreg__(row_registers(FORM, IT)) quant_rows_kernel(const Nkb
   if constexpr (CLUSTER) {
     if (threadIdx.x == 0) {
       s_part.top = top;
-      s_part.ss = ss;
       s_part.top64 = (unsigned long long)__double_as_longlong(m64);
     }
     cluster_sync_all();
-    uint32_t t = 0, f = 0;
+    uint32_t t = 0;
+    unsigned long long o = 0;
     if (lane < int(gridDim.x)) {
       asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(t) : "r"(map_to_cta(&s_part.top, lane)) : "memory");
-      if constexpr (FORM == NKB_ROW_NORM)
-        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(f) : "r"(map_to_cta(&s_part.ss, lane)) : "memory");
+      asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(o) : "r"(map_to_cta(&s_part.top64, lane)) : "memory");
     }
     top = __reduce_max_sync(0xffffffffu, t);
-    if constexpr (FORM == NKB_ROW_NORM) ss = warp_sum(__uint_as_float(f));
-    if constexpr (kGate) {
-      unsigned long long o = 0;
-      if (lane < int(gridDim.x))
-        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(o) : "r"(map_to_cta(&s_part.top64, lane)) : "memory");
-      m64 = __longlong_as_double((long long)o);
+    m64 = __longlong_as_double((long long)o);
 #pragma unroll
-      for (int i = 4; i > 0; i >>= 1) m64 = fmax(m64, __shfl_xor_sync(0xffffffffu, m64, i));
-      m64 = __shfl_sync(0xffffffffu, m64, 0);
-    }
+    for (int i = 4; i > 0; i >>= 1) m64 = fmax(m64, __shfl_xor_sync(0xffffffffu, m64, i));
+    m64 = __shfl_sync(0xffffffffu, m64, 0);
   }
   const bool fine = top < 0x7f800000u;
   const bool in64 = kGate && small(__uint_as_float(top));       // the whole row in 64 bits
@@ -464,10 +457,12 @@ __global__ void __maxnreg__(row_registers(FORM, IT)) quant_rows_kernel(const Nkb
   if constexpr (CLUSTER) cluster_sync_all();        // shared memory stays until every CTA of the cluster has read it
 }
 
-// CTAs of a row: doubled while a row's part stays 1024 columns and all parts have room on the SMs, `per_sm` on each.
-static int row_ctas(int rows, int chunks, int per_sm) {
+// CTAs of a gated row: doubled while a row's part stays 1024 columns and all parts have an SM of their own.  Two partial sums of 2 x 14336, us, with 1, 2 and 4
+// CTAs: 64 rows 21.4, 13.0, 15.5; 16 rows 17.1, 10.9, 7.1 (8: 6.5).  Other rows have a few instructions a column, and the cluster's start and barriers cost more than
+// its parts gain: 64 behind a norm 5.2, 6.9, 5.9, as they are 3.7, 4.0, 4.1.
+static int row_ctas(int rows, int chunks) {
   int c = 1;
-  while (c < 8 && chunks > 512 && (long long)rows * c * 2 <= per_sm * num_sms() && chunks / (2 * c) >= 128) c *= 2;
+  while (c < 8 && chunks > 512 && (long long)rows * c * 2 <= num_sms() && chunks / (2 * c) >= 128) c *= 2;
   return c;
 }
 
@@ -499,8 +494,8 @@ static int launch_rows(const NkbQuantRows& a) {
   const int chunks = (a.width + 7) / 8;
   auto warps = [](int n) { return unsigned((n + 31) / 32 * 32); };
   const cudaStream_t stream = reinterpret_cast<cudaStream_t>(a.stream);
-  if constexpr (VEC) {
-    const int c = row_ctas(a.rows, chunks, FORM == NKB_ROW_GATE_F32 ? 1 : 2);
+  if constexpr (VEC && (FORM == NKB_ROW_GATE_BF16 || FORM == NKB_ROW_GATE_F32)) {
+    const int c = row_ctas(a.rows, chunks);
     if (c > 1) {
       const int part = (chunks + c - 1) / c;
       const dim3 grid(unsigned(c), unsigned(a.rows));
