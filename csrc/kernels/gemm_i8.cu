@@ -72,7 +72,8 @@ struct I8PairArgs {
   int kb_total, stages;
   int tiles_m, tiles_n, tile_n, group_m;
   int splits, kb_per_split;   // more than one: partial sums in 32 bits, split s at o.out + s * split_stride
-  int static_w, gated;
+  short static_w, gated;
+  int apart;                  // rows of results or of the residual do not start on sixteen bytes
   long long split_stride;
   int* status;
 };
@@ -322,6 +323,10 @@ i8_swap_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ 
 // ------------------------------------------------------------------------------------------------ pairs
 constexpr int kPairTileN = 256;
 constexpr int kPairStage = 2 * kI8ATile;
+constexpr int kPairStages = 7, kApartStages = 6;   // (without and with the epilogue's tiles)
+constexpr int kApartBytes = 4 * 32 * 33 * 4;       // a tile of 32 x 32 sums for each epilogue warp
+constexpr int kPairSmem = 2048 + kPairStages * kPairStage;
+static_assert(2048 + kApartStages * kPairStage + kApartBytes <= kPairSmem && kPairSmem <= 232448, "more than an SM's shared memory");
 
 struct WorkI8 {
   int tm, tn, sp, kb0, kb1;
@@ -402,6 +407,30 @@ __device__ __forceinline__ void i8_store_row(const I8Out& a, bool first, long lo
         if (c + j < cols_end) o[j] = __float2bfloat16(y[j]);
     }
   }
+}
+
+// The same of the warp's 32 rows from row0 on where they do not start on sixteen bytes: through shared memory, so that the lanes store neighbouring columns of
+// a row (848 tokens by 2 x 10726 x 100, whose rows start on four bytes: 118 us lane by lane, each with a row of its own).
+template <bool GATED>
+__device__ __forceinline__ void i8_store_rows(const I8Out& a, bool first, long long at, int row0, int c, int cols_end, const float (&y)[32], float* tile) {
+  const int lane = threadIdx.x & 31, col = c + lane;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) tile[lane * 33 + j] = y[j];
+  __syncwarp();
+  if (col < cols_end) {
+    const float bias = !GATED && a.bias && first ? __bfloat162float(__ldg(a.bias + col)) : 0.f;
+    const int rows = min(32, a.m - row0);
+    at += (long long)row0 * a.ldo + col;
+#pragma unroll 8
+    for (int r = 0; r < rows; ++r, at += a.ldo) {
+      float v = tile[r * 33 + lane];
+      if (!GATED && a.bias) v += bias;
+      if (!GATED && a.residual) v += __bfloat162float(a.residual[at]);
+      if (a.fp32) reinterpret_cast<float*>(a.out)[at] = v;
+      else reinterpret_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16(v);
+    }
+  }
+  __syncwarp();
 }
 
 // y[j] = v[j] * sx * sw[c + j]; columns from cols_end on may get anything.
@@ -556,6 +585,7 @@ __device__ __forceinline__ void i8_pair_body(const CUtensorMap& tmX, const CUten
   } else if (warp >= 2) {
     // ------------------------------------------------------------------ epilogue (warps 2..5, both CTAs)
     const int quad = warp & 3;
+    float* apart = reinterpret_cast<float*>(tiles + kApartStages * kPairStage) + quad * (32 * 33);
     griddep_wait();
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -599,7 +629,9 @@ __device__ __forceinline__ void i8_pair_body(const CUtensorMap& tmX, const CUten
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(map_to_cta(&ctrl->tempty[acc], 0));
         }
-        if (row < args.o.m && col0 + c < cols_end) i8_store_row<GATED>(args.o, t.sp == 0, t.sp * args.split_stride, row, col0 + c, cols_end, y);
+        if (col0 + c >= cols_end) continue;
+        if (args.apart) i8_store_rows<GATED>(args.o, t.sp == 0, t.sp * args.split_stride, row - lane, col0 + c, cols_end, y, apart);
+        else if (row < args.o.m) i8_store_row<GATED>(args.o, t.sp == 0, t.sp * args.split_stride, row, col0 + c, cols_end, y);
       }
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1u;
@@ -712,14 +744,17 @@ static int launch_i8_pairs(const NkbGemmI8& g, const I8Out& o) {
   a.group_m = 16;
   a.split_stride = g.split_stride;
   divide(a, g.splits);
+  const int size = g.fp32 ? 4 : 2;
+  a.apart = ((reinterpret_cast<uintptr_t>(g.out) | uintptr_t(g.ldo * size) | uintptr_t(g.split_stride * size)) & 15) != 0 ||
+            (g.residual && ((reinterpret_cast<uintptr_t>(g.residual) | uintptr_t(g.ldo * 2)) & 15) != 0);
   a.status = status_word();
   a.tiles_m = (g.m + 255) / 256;
-  a.stages = (232448 - 2048) / kPairStage;
+  a.stages = a.apart ? kApartStages : kPairStages;
   int dev = -1;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDev) return -1;
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kGemmThreads);
-  cfg.dynamicSmemBytes = size_t(a.stages * kPairStage + 2048);
+  cfg.dynamicSmemBytes = size_t(kPairSmem);
   cfg.stream = reinterpret_cast<cudaStream_t>(g.stream);
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;

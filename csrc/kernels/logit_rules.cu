@@ -24,6 +24,7 @@ namespace nkb {
 constexpr int kRuleThreads = 512;
 constexpr int kCountBytes = 96 * 1024;  // counts of the tokens that a CTA holds at a time: two CTAs per SM
 constexpr int kListMost = 2048;         // named tokens on the list
+constexpr int kBiasMost = 512;          // entries of a row that lie in shared memory; the ones behind are read where they are
 constexpr int kPer = 8;                 // tokens of a piece
 
 template <bool WIDE>
@@ -62,6 +63,8 @@ struct Counts {
 
 struct RuleRow {
   float rep, freq, pres;
+  const int4* near_ids;         // the first entries in shared memory, filled up with -1
+  const float* near_values;
   const int* bias_ids;
   const float* bias_values;
   int biases;
@@ -79,8 +82,17 @@ __device__ __noinline__ float ruled(const RuleRow& r, float l0, uint32_t c, int 
   }
   if (c & C::kBiased) {
     double sum = 0.0;
+    const int near = min(r.biases, kBiasMost);
+#pragma unroll 4
+    for (int i = 0; i < near; i += 4) {
+      const int4 id = r.near_ids[i >> 2];
+      if (id.x == token) sum += double(r.near_values[i]);
+      if (id.y == token) sum += double(r.near_values[i + 1]);
+      if (id.z == token) sum += double(r.near_values[i + 2]);
+      if (id.w == token) sum += double(r.near_values[i + 3]);
+    }
 #pragma unroll 8
-    for (int i = 0; i < r.biases; ++i)
+    for (int i = near; i < r.biases; ++i)
       if (r.bias_ids[i] == token) sum += double(r.bias_values[i]);
     l += sum;
   }
@@ -150,6 +162,8 @@ __global__ void __launch_bounds__(kRuleThreads, 2) logit_rules_kernel(const NkbL
   using C = Counts<WIDE>;
   extern __shared__ __align__(16) uint32_t words[];
   __shared__ int s_list[kListMost];
+  __shared__ __align__(16) int s_bias_ids[kBiasMost];
+  __shared__ float s_bias_values[kBiasMost];
   __shared__ int s_n;
   __shared__ float s_best[kRuleThreads / 32];
   __shared__ int s_at[kRuleThreads / 32];
@@ -195,6 +209,12 @@ __global__ void __launch_bounds__(kRuleThreads, 2) logit_rules_kernel(const NkbL
   r.bias_ids = a.bias_ids + row * a.bias_ld;
   r.bias_values = a.bias_values + row * a.bias_ld;
   r.biases = a.biases;
+  r.near_ids = reinterpret_cast<const int4*>(s_bias_ids);
+  r.near_values = s_bias_values;
+  for (int i = tid; i < min(kBiasMost, (a.biases + 3) & ~3); i += kRuleThreads) {        // (a barrier before they are read comes with the counts)
+    s_bias_ids[i] = i < a.biases ? r.bias_ids[i] : -1;
+    s_bias_values[i] = i < a.biases ? r.bias_values[i] : 0.f;
+  }
   const bool counted = len > 0 && (r.rep != 1.f || r.freq != 0.f || r.pres != 0.f);
   const int prompt = a.prompts && counted ? a.prompts[row] : 0;
   const int mrow = a.mask_rows ? a.mask_rows[row] : row;
@@ -317,14 +337,28 @@ __global__ void __launch_bounds__(kRuleThreads, 2) logit_rules_kernel(const NkbL
         if (((plain >> i) & 1u) && y.value(i) == top) j = i;
       better(top, lo + top_piece * kPer + j);
     }
-    for (int t = lo + pieces * kPer + tid; t < hi; t += kRuleThreads) {
-      const bool allowed = !mask || ((uint32_t(mask[t >> 5]) >> (t & 31)) & 1u);
-      if (ids) {
-        if (allowed && !(named && counts.get(t - lo))) better(rule_logit<F32>(in, t), t);
-      } else if (!allowed) {
-        rule_store<F32>(out, t, -INFINITY);
-      } else if (!in_place) {
-        rule_store<F32>(out, t, rule_logit<F32>(in, t));
+    constexpr int kSingles = VEC ? 1 : 8;       // tokens of a thread whose loads come together
+    for (int t0 = lo + pieces * kPer + tid; t0 < hi; t0 += kSingles * kRuleThreads) {
+      float l[kSingles];
+      uint32_t word[kSingles];
+#pragma unroll
+      for (int i = 0; i < kSingles; ++i) {
+        const int t = t0 + i * kRuleThreads;
+        l[i] = t < hi && !in_place ? rule_logit<F32>(in, t) : 0.f;
+        word[i] = t < hi && mask ? uint32_t(mask[t >> 5]) : ~0u;
+      }
+#pragma unroll
+      for (int i = 0; i < kSingles; ++i) {
+        const int t = t0 + i * kRuleThreads;
+        if (t >= hi) break;
+        const bool allowed = (word[i] >> (t & 31)) & 1u;
+        if (ids) {
+          if (allowed && !(named && counts.get(t - lo))) better(l[i], t);
+        } else if (!allowed) {
+          rule_store<F32>(out, t, -INFINITY);
+        } else if (!in_place) {
+          rule_store<F32>(out, t, l[i]);
+        }
       }
     }
     if (named) {

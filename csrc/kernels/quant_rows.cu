@@ -58,18 +58,35 @@ struct Raw8 {
 template <int FORM, bool VEC>
 __device__ __forceinline__ void fetch8(const NkbQuantRows& a, long long row, int c, Raw8<FORM>& o, bool weights) {
   const uint4 none = make_uint4(0u, 0u, 0u, 0u);
-  const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x) + row * a.x_ld;
-  if constexpr (FORM == NKB_ROW_BF16) {
+  const uint16_t* x = reinterpret_cast<const uint16_t*>(a.x) + row * a.x_ld;
+  const uint16_t* y = FORM == NKB_ROW_NORM ? reinterpret_cast<const uint16_t*>(a.residual) + row * a.width : x + a.width;       // up, or the stream
+  if constexpr (!VEC && (FORM == NKB_ROW_BF16 || FORM == NKB_ROW_NORM || FORM == NKB_ROW_GATE_BF16)) {
+    // All loads first.  Pieces are read where they have columns of the same tensor around them: the row's own, or the next and the last one's.
+    const int n = a.width - c;
+    const bool apart = a.x_ld >= a.width, next = row + 1 < a.rows;
+    const bool fx = a.x && n >= 8 && (c >= 8 || (apart && row > 0)) && (n >= 16 || (apart && next));
+    const bool fy = FORM == NKB_ROW_NORM ? a.residual && n >= 8 && (c >= 8 || row > 0) && (n >= 16 || next)
+                                         : FORM == NKB_ROW_GATE_BF16 && n >= 8 && (n >= 16 || (apart && next));
+    const bool fw = FORM == NKB_ROW_NORM && weights && c >= 8 && n >= 16;
+    const uint16_t* w = reinterpret_cast<const uint16_t*>(a.w);
+    const Pieces px = fetch_pieces(x + c, fx), py = fetch_pieces(y + c, fy), pw = fetch_pieces(w + c, fw);
+    o.r[0] = a.x ? from_pieces(px, x + c, fx, n) : none;
+    if constexpr (FORM == NKB_ROW_GATE_BF16) o.r[1] = from_pieces(py, y + c, fy, n);
+    if constexpr (FORM == NKB_ROW_NORM) {
+      o.r[1] = a.residual ? from_pieces(py, y + c, fy, n) : none;
+      if (weights) o.r[2] = from_pieces(pw, w + c, fw, n);        // (a thread's columns are the same in every row)
+    }
+  } else if constexpr (FORM == NKB_ROW_BF16) {
     o.r[0] = fetch8_bf16<VEC>(x, c, a.width);
   } else if constexpr (FORM == NKB_ROW_F32) {
     fetch8_f32<VEC>(reinterpret_cast<const float*>(a.x) + row * a.x_ld, c, a.width, o.r);
   } else if constexpr (FORM == NKB_ROW_NORM) {
     o.r[0] = a.x ? fetch8_bf16<VEC>(x, c, a.width) : none;
-    o.r[1] = a.residual ? fetch8_bf16<VEC>(reinterpret_cast<const __nv_bfloat16*>(a.residual) + row * a.width, c, a.width) : none;
-    if (weights) o.r[2] = fetch8_bf16<VEC>(a.w, c, a.width);        // (a thread's columns are the same in every row)
+    o.r[1] = a.residual ? fetch8_bf16<VEC>(y, c, a.width) : none;
+    if (weights) o.r[2] = fetch8_bf16<VEC>(a.w, c, a.width);
   } else if constexpr (FORM == NKB_ROW_GATE_BF16) {
     o.r[0] = fetch8_bf16<VEC>(x, c, a.width);
-    o.r[1] = fetch8_bf16<VEC>(x + a.width, c, a.width);
+    o.r[1] = fetch8_bf16<VEC>(y, c, a.width);
   } else {
     const float* p = a.partials + row * a.x_ld;
     uint4 g[2], u[2];
@@ -80,6 +97,13 @@ __device__ __forceinline__ void fetch8(const NkbQuantRows& a, long long row, int
     o.r[2] = u[0];
     o.r[3] = u[1];
   }
+}
+
+// Off by 2^-23 at most.
+__device__ __forceinline__ float reciprocal(float v) {
+  float d;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(d) : "f"(v));
+  return d;
 }
 
 // Gate times up of one column in 64 bits.
@@ -159,6 +183,38 @@ __device__ __forceinline__ void load8_gate(const NkbQuantRows& a, long long row,
   }
 }
 
+// 8 columns of a row of `width`, one more to the right in the next lane: rows that do not start on sixteen bytes are stored in pieces that do, which a lane makes
+// of its own columns and its neighbour's.  All lanes with columns come here together.
+__device__ __forceinline__ void store8_moved(__nv_bfloat16* row, int c, int width, const uint32_t (&h)[4]) {
+  const int lane = threadIdx.x & 31, n = min(32, (width + 7) / 8 - (c / 8 - lane));
+  const uint32_t mask = n >= 32 ? ~0u : (1u << n) - 1u;
+  __nv_bfloat16* o = row + c;
+  const uint32_t over = uint32_t(reinterpret_cast<uintptr_t>(o)) & 15u;        // (the same in all lanes)
+  int from = 0, to = 8;             // columns that are stored one by one
+  if (over == 0) {
+    if (c + 8 <= width) {
+      *reinterpret_cast<uint4*>(o) = make_uint4(h[0], h[1], h[2], h[3]);
+      return;
+    }
+  } else {
+    uint32_t v[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] = h[j];
+      v[4 + j] = __shfl_down_sync(mask, h[j], 1);
+    }
+    const int skip = int(16u - over) / 2;
+    if (lane > 0 && c + 8 <= width) from = skip;
+    if (lane + 1 < n && c + 16 <= width) {
+      *reinterpret_cast<uint4*>(o + skip) = moved(v, 16u - over);
+      to = skip;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j >= from && j < to && c + j < width) reinterpret_cast<uint16_t*>(o)[j] = uint16_t(h[j >> 1] >> (16 * (j & 1)));
+}
+
 // What the 8 columns from c on are rounded from.  Norm: stores the residual stream, and adds its squares to ss.
 template <int FORM, bool VEC>
 __device__ __forceinline__ void load8(const NkbQuantRows& a, long long row, int c, const Raw8<FORM>& raw, float (&v)[8], float& ss) {
@@ -204,13 +260,15 @@ __device__ __forceinline__ void load8(const NkbQuantRows& a, long long row, int 
       x[2 * e + 1] = f.y;
     }
     if (a.residual_out) {
-      __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(a.residual_out) + row * a.width + c;
-      if (VEC && c + 8 <= a.width) {
-        *reinterpret_cast<uint4*>(o) = make_uint4(h[0], h[1], h[2], h[3]);
+      __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(a.residual_out) + row * a.width;
+      if constexpr (!VEC) {
+        store8_moved(o, c, a.width, h);
+      } else if (c + 8 <= a.width) {
+        *reinterpret_cast<uint4*>(o + c) = make_uint4(h[0], h[1], h[2], h[3]);
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (c + j < a.width) o[j] = __float2bfloat16(x[j]);
+          if (c + j < a.width) o[c + j] = __float2bfloat16(x[j]);
       }
     }
 #pragma unroll
@@ -229,7 +287,7 @@ __device__ __forceinline__ void load8(const NkbQuantRows& a, long long row, int 
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = g[j] / (1.f + expf(-g[j])) * u[j];
+      for (int j = 0; j < 8; ++j) v[j] = g[j] * reciprocal(1.f + expf(-g[j])) * u[j];
     }
     // columns past the width read as zeros
     if (c + 8 > a.width) {
@@ -249,7 +307,7 @@ struct RowPart {
 // Registers of a thread: as few as the chunks that it keeps and has on their way leave room for, since more warps hide more of the loads and barriers.
 constexpr int row_registers(int form, int it) {
   if (it == 1) return form == NKB_ROW_GATE_F32 ? 128 : 64;
-  if (it == 2) return form <= NKB_ROW_NORM ? 72 : 128;
+  if (it == 2) return form == NKB_ROW_GATE_F32 ? 128 : 72;
   if (it == 4) return form == NKB_ROW_BF16 ? 64 : 128;
   return 128;
 }
@@ -324,7 +382,7 @@ __global__ void __maxnreg__(row_registers(FORM, IT)) quant_rows_kernel(const Nkb
   auto once_more = [&](int ch) {
     float none = 0.f;
     if constexpr (FORM == NKB_ROW_NORM) {
-      // (written by this thread: not through the read-only path)
+      // (written by this block before its barrier: not through the read-only path)
       const __nv_bfloat16* h = reinterpret_cast<const __nv_bfloat16*>(again_a.x) + row * again_a.x_ld;
       if (a.residual_out) {
         uint32_t w[4] = {0u, 0u, 0u, 0u};
@@ -402,6 +460,7 @@ __global__ void __maxnreg__(row_registers(FORM, IT)) quant_rows_kernel(const Nkb
     if constexpr (FORM == NKB_ROW_NORM) scale *= rsqrtf(ss / float(a.width) + a.eps);
     a.scale[row] = fine ? scale : __uint_as_float(0x7fffffffu);
   }
+  const float near_half = a.bias || a.limit > 0.f || a.splits > 1 ? kNearHalfGated : kNearHalfGatedOnce;
   // Rows whose m or 127 / m is at an end of the range: every number by the comparison, scaled by a power of two.
   const bool odd = odd_row(m);
   const float inv = odd ? 0.f : 127.f / m;
@@ -420,7 +479,7 @@ __global__ void __maxnreg__(row_registers(FORM, IT)) quant_rows_kernel(const Nkb
       for (int j = 0; j < 8; ++j) {
         const float s = fmaf(x[j], inv, 12582912.f);
         t[j] = __float_as_uint(s);
-        again |= fabsf(fmaf(x[j], inv, 12582912.f - s)) > kNearHalfGated ? 1u << j : 0u;
+        again |= fabsf(fmaf(x[j], inv, 12582912.f - s)) > near_half ? 1u << j : 0u;
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -503,8 +562,9 @@ static int launch_rows(const NkbQuantRows& a) {
       if (part <= 1024) return launch_pdl_cluster(quant_rows_kernel<FORM, VEC, 2, true>, grid, dim3(warps((part + 1) / 2)), 0, stream, c, a);
     }
   }
-  if (chunks > 32 && chunks <= 2048) {
-    constexpr int kFew = FORM == NKB_ROW_F32 || FORM == NKB_ROW_GATE_F32 ? 2 : 4;
+  // (not normed rows off sixteen bytes, which hold two pieces for each load: 15262 x 2557 184 us so, 114 in a block of its own each; gated 14565 x 930 54, 56)
+  if ((VEC || FORM != NKB_ROW_NORM) && chunks > 32 && chunks <= 2048) {
+    constexpr int kFew = FORM == NKB_ROW_BF16 || FORM == NKB_ROW_NORM ? 4 : 2;
     int rc = kFew == 2 && chunks <= 1024 ? launch_many<FORM, VEC, kFew>(a, chunks) : launch_many<FORM, VEC, 4>(a, chunks);
     if (rc != -5) return rc;
   }
@@ -529,7 +589,9 @@ extern "C" int nkb_quant_rows(const void* packed) {
     at |= reinterpret_cast<uintptr_t>(p);
   const bool gate = a.form == NKB_ROW_GATE_BF16 || a.form == NKB_ROW_GATE_F32;
   const bool rows_of_width = a.form == NKB_ROW_NORM || gate;
-  const bool vec = (at & 15) == 0 && (a.x_ld & 7) == 0 && (a.split_stride & 3) == 0 && (!rows_of_width || (a.width & 7) == 0);
+  // (of gated fp32 rows the up half starts on sixteen bytes with every fourth column already, a bias's with every eighth)
+  const int whole = a.form == NKB_ROW_GATE_F32 && !a.bias ? 3 : 7;
+  const bool vec = (at & 15) == 0 && (a.x_ld & whole) == 0 && (a.split_stride & 3) == 0 && (!rows_of_width || (a.width & whole) == 0);
   switch (a.form) {
     case NKB_ROW_BF16: return vec ? launch_rows<NKB_ROW_BF16, true>(a) : launch_rows<NKB_ROW_BF16, false>(a);
     case NKB_ROW_F32: return vec ? launch_rows<NKB_ROW_F32, true>(a) : launch_rows<NKB_ROW_F32, false>(a);

@@ -4,23 +4,53 @@
 
 namespace nkb {
 
-// Distance from a whole number beyond which a gated one is decided in 64 bits: half, less 127 times the 2^-20 of a gated value in 32 bits.
-constexpr float kNearHalfGated = 0.5f - 1.f / 4096;
+// Distance from a whole number beyond which a gated one is decided in 64 bits: half, less 127 times the error of a gated value in 32 bits.  That is 2^-20 where gate
+// and up are rounded sums (the exponential multiplies the gate's rounding by it), and below 2^-21 where both are given (the exponential, 1 +, the
+// quotient, the product); the row's largest and its quotient add 2^-23.
+constexpr float kNearHalfGated = 0.5f - 1.f / 4096, kNearHalfGatedOnce = 0.5f - 1.f / (1 << 13);
 __device__ __forceinline__ float max_nan(float a, float b) {
   float d;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
-// 8 columns from `c` on of a row, as they lie in memory; columns past the width read as zeros.  VEC: rows start on 16 bytes.  (Through the read-only
-// path: a thread's loads may then go ahead of its stores, which in place follow the loads of the same columns.)
-template <bool VEC>
-__device__ __forceinline__ uint4 fetch8_bf16(const void* row, int c, int width) {
-  if (VEC && c + 8 <= width) return __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(row) + c));
+// Bytes [by, by + 16) of 32; by: even, below 16.
+__device__ __forceinline__ uint4 moved(const uint32_t (&v)[8], uint32_t by) {
+  uint32_t u[7], t[5];
+#pragma unroll
+  for (int j = 0; j < 7; ++j) u[j] = by & 4u ? v[j + 1] : v[j];
+#pragma unroll
+  for (int j = 0; j < 5; ++j) t[j] = by & 8u ? u[j + 2] : u[j];
+  const uint32_t half = (by & 2u) * 8u;
+  return make_uint4(__funnelshift_r(t[0], t[1], half), __funnelshift_r(t[1], t[2], half), __funnelshift_r(t[2], t[3], half), __funnelshift_r(t[3], t[4], half));
+}
+// The two pieces of sixteen bytes that 8 columns from p on lie in, where `inside` says that both lie within the rows' memory.
+struct Pieces {
+  uint4 lo, hi;
+};
+__device__ __forceinline__ Pieces fetch_pieces(const uint16_t* p, bool inside) {
+  const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) & ~uintptr_t(15));
+  const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+  return {inside ? __ldg(q) : none, inside ? __ldg(q + 1) : none};
+}
+// 8 columns from `c` on of a row, as they lie in memory; columns past the width read as zeros.  VEC: rows start on 16 bytes; others column by column, or
+// from the pieces.  (Through the read-only path: a thread's loads may then go ahead of its stores, which in place follow the loads of the same columns.)
+__device__ __forceinline__ uint4 fetch8_each(const uint16_t* p, int columns) {
   uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
   for (int j = 0; j < 8; ++j)
-    if (c + j < width) w[j >> 1] |= uint32_t(__ldg(reinterpret_cast<const uint16_t*>(row) + c + j)) << (16 * (j & 1));
+    if (j < columns) w[j >> 1] |= uint32_t(__ldg(p + j)) << (16 * (j & 1));
   return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint4 from_pieces(const Pieces& t, const uint16_t* p, bool inside, int columns) {
+  if (!inside) return fetch8_each(p, columns);
+  const uint32_t v[8] = {t.lo.x, t.lo.y, t.lo.z, t.lo.w, t.hi.x, t.hi.y, t.hi.z, t.hi.w};
+  return moved(v, uint32_t(reinterpret_cast<uintptr_t>(p)) & 15u);
+}
+template <bool VEC>
+__device__ __forceinline__ uint4 fetch8_bf16(const void* row, int c, int width) {
+  const uint16_t* p = reinterpret_cast<const uint16_t*>(row) + c;
+  if (VEC && c + 8 <= width) return __ldg(reinterpret_cast<const uint4*>(p));
+  return fetch8_each(p, width - c);
 }
 template <bool VEC>
 __device__ __forceinline__ void fetch8_f32(const float* row, int c, int width, uint4 (&r)[2]) {

@@ -378,3 +378,23 @@ def test_from_the_last_layer_to_the_token(device, B, H, V):
     clear = ((top2[:, 0] - top2[:, 1]) > 1e-4) | (top2[:, 0] == -1e30)          # (nothing is left: -1)
     assert int(clear.sum()) >= B - 1
     assert torch.equal(ids.cpu()[clear], oracle_ids(want)[clear])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("biases,V", [(1, 50), (510, 3001), (512, 3008), (513, 700), (1500, 4003)])
+def test_many_biases(device, dtype, biases, V):
+    """As many as lie in shared memory, fewer and more; tokens with several; rows that start on sixteen bytes and others."""
+    check(logits_of(biases, 3, V, dtype), make(biases, 3, V, width=30, biases=biases, masks="rows"), device)
+    r = make(biases, 3, V, biases=biases)
+    r["bias_ids"][:, ::3] = 7
+    check(logits_of(biases, 3, V, dtype), r, device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_more_named_tokens_than_are_listed(device):
+    r = make(5, 2, 9000, width=4000)
+    g = torch.Generator().manual_seed(6)
+    r["tokens"] = torch.stack([torch.randperm(9000, generator=g)[:4000] for _ in range(2)]).int()
+    r["lens"] = torch.tensor([4000, 1100], dtype=torch.int32)
+    check(logits_of(5, 2, 9000, BF), r, device)

@@ -530,3 +530,73 @@ def test_normed_rows_in_the_place_of_the_stream(device):
             a, b = x.to(device, copy=True), r.to(device, copy=True)
             h, q = ops.add_rmsnorm(a, w.to(device), residual_in=b, residual_out=(a, b)[place], quantize=True)
             assert h is (a, b)[place] and torch.equal(h, want) and torch.equal(q.values, rows.values) and torch.equal(q.scale, rows.scale)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("offset", [0, 1, 2, 3, 4, 5, 6, 7, 9])
+def test_columns_that_start_anywhere(device, offset):
+    """Rows whose columns lie across pieces of sixteen bytes, whatever they are moved by, and rows that share their memory."""
+    g = draws(offset)
+    x = rows_like_a_layers(g, 5, 1030)
+    memory = torch.full((offset + 5 * 1030,), float("nan"), dtype=BF, device=device)[offset:].view(5, 1030)
+    memory.copy_(x)
+    for width in (1030 - offset, 1024, 17, 9):
+        check_rows(ops.quantize_rows(memory[:, :width]), x[:, :width], steps=1)
+        check_rows(ops.quantize_rows(memory[:, 1030 - width:]), x[:, 1030 - width:], steps=1)
+    check_rows(ops.quantize_rows(memory[2:3].expand(4, 1030)), x[2:3].expand(4, 1030), steps=1)
+    flat = x.reshape(-1)
+    check_rows(ops.quantize_rows(memory.reshape(-1).as_strided((40, 33), (7, 1), memory.storage_offset())), flat.as_strided((40, 33), (7, 1), 0), steps=1)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("m,n,k,gated", [(300, 1001, 96, False), (300, 1001, 96, True), (260, 2050, 130, False), (700, 333, 64, True), (513, 4100, 257, False)])
+@pytest.mark.parametrize("fp32,addends", [(False, False), (False, True), (True, False)])
+def test_products_into_rows_off_sixteen_bytes(device, m, n, k, gated, fp32, addends):
+    if gated and (fp32 or addends):
+        return
+    g = draws(m + n + k)
+    x, w = made(g, m, n, k, gated)
+    rows, weight = there(x, device), there(w, device)
+    bias = torch.randn((n,), generator=g).to(BF) if addends else None
+    residual = torch.randn((m, n), generator=g).to(BF) if addends else None
+    base = torch.full((m, n + 3), 7.0, dtype=F32 if fp32 else BF, device=device)
+    out = base[:, 1:n + 1]
+    kw = dict(gated=True) if gated else dict(fp32_out=fp32)
+    if addends:
+        kw.update(bias=bias.to(device), residual=residual.to(device))
+    want, tol = oracle_product(x.values, x.scale, w.values, w.scale, gated=gated, bias=bias, residual=residual, fp32=fp32)
+    for into in (None, out):
+        got = ops.linear(rows, weight, out=into, **kw)
+        assert into is None or got.data_ptr() == out.data_ptr()
+        check_product(got, want, tol)
+    assert bool((base[:, 0] == 7).all()) and bool((base[:, n + 1:] == 7).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,k", [(3, 1), (3, 9), (5, 23), (4, 257), (3, 263), (7, 1030), (5, 2557), (3, 9001), (2, 20003), (11000, 301), (6000, 2557)])
+@pytest.mark.parametrize("start", [0, 3])
+def test_normed_rows_of_odd_widths_in_place(t, k, start):
+    """The stream's rows start anywhere between pieces of sixteen bytes; what lies ahead of it and behind it stays."""
+    g = draws(t + k)
+    x, r = rows_like_a_layers(g, t, k), rows_like_a_layers(g, t, k)
+    w = (1 + 0.2 * torch.randn((k,), generator=g)).to(BF)
+    h, q = ops.add_rmsnorm(x, w, residual_in=r, eps=EPS, quantize=True)
+    for place in ("new", "x", "stream"):
+        memory = [torch.full((start + t * k + 5,), 7.0, dtype=BF, device="cuda") for _ in range(2)]
+        a, b = (m[start:start + t * k].view(t, k) for m in memory)
+        a.copy_(x), b.copy_(r)
+        got, rows = ops.add_rmsnorm(a, w.cuda(), residual_in=b, residual_out={"new": None, "x": a, "stream": b}[place], eps=EPS, quantize=True)
+        assert torch.equal(got.cpu(), h) and torch.equal(rows.values.cpu(), q.values)
+        assert bool(((rows.scale.cpu().double() - q.scale.double()).abs() <= 64 * U24 * q.scale.double()).all())
+        assert all(bool((m[:start] == 7).all()) and bool((m[start + t * k:] == 7).all()) for m in memory)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("t,k", [(5, 9), (3, 263), (9000, 301), (6000, 930), (6000, 928), (3000, 2557), (3000, 5000), (3, 17001)])
+def test_many_gated_rows(dtype, t, k):
+    g = draws(t + k)
+    x = (2 * torch.randn((t, 2 * k), generator=g)).to(dtype)
+    q, rows = ops.silu_mul(x, quantize=True), ops.silu_mul(x.cuda(), quantize=True)
+    assert torch.equal(rows.values.cpu(), q.values)
+    assert bool(((rows.scale.cpu().double() - q.scale.double()).abs() <= 2 * U24 * q.scale.double()).all())
