@@ -324,9 +324,12 @@ i8_swap_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ 
 constexpr int kPairTileN = 256;
 constexpr int kPairStage = 2 * kI8ATile;
 constexpr int kPairStages = 7, kApartStages = 6;   // (without and with the epilogue's tiles)
-constexpr int kApartBytes = 4 * 32 * 33 * 4;       // a tile of 32 x 32 sums for each epilogue warp
-constexpr int kPairSmem = 2048 + kPairStages * kPairStage;
-static_assert(2048 + kApartStages * kPairStage + kApartBytes <= kPairSmem && kPairSmem <= 232448, "more than an SM's shared memory");
+// Warps of the epilogue.  1024 tokens by 4096 x 4096, us, with four and eight at the widths 128, 192 and 256: 21.1 and 20.7, 24.5 and 22.6, 21.9 and 20.5;
+// 414 by 2 x 14336 x 4096 54.7 and 62.0, 50.0 and 53.7, 52.1 and 51.7; 4096 tokens by it 359 and 399, 314 and 333, 297 and 296.
+__host__ __device__ constexpr int pair_warps(bool gated) { return gated ? 4 : 8; }
+constexpr int kApartBytes = pair_warps(false) * 32 * 33 * 4;      // a tile of 32 x 32 sums for each
+constexpr int kPairSmem = 232448;
+static_assert(2048 + kApartStages * kPairStage + kApartBytes <= kPairSmem && 2048 + kPairStages * kPairStage <= kPairSmem, "more than an SM's shared memory");
 
 struct WorkI8 {
   int tm, tn, sp, kb0, kb1;
@@ -433,26 +436,38 @@ __device__ __forceinline__ void i8_store_rows(const I8Out& a, bool first, long l
   __syncwarp();
 }
 
-// y[j] = v[j] * sx * sw[c + j]; columns from cols_end on may get anything.
-__device__ __forceinline__ void i8_scale_row(const uint32_t (&v)[32], float sx, const float* sw, int c, int cols_end, float (&y)[32]) {
+// Scales of the columns from c on; those from cols_end on are another's.
+__device__ __forceinline__ void i8_scales(const float* sw, int c, int cols_end, float (&s)[32]) {
   const bool s16 = (reinterpret_cast<uintptr_t>(sw + c) & 15) == 0;
 #pragma unroll
   for (int q = 0; q < 8; ++q) {
-    float s[4];
     if (s16 && c + 4 * q + 4 <= cols_end) {
       const float4 f = __ldg(reinterpret_cast<const float4*>(sw + c) + q);
-      s[0] = f.x; s[1] = f.y; s[2] = f.z; s[3] = f.w;
+      s[4 * q] = f.x; s[4 * q + 1] = f.y; s[4 * q + 2] = f.z; s[4 * q + 3] = f.w;
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[j] = __ldg(sw + min(c + 4 * q + j, cols_end - 1));
+      for (int j = 4 * q; j < 4 * q + 4; ++j) s[j] = __ldg(sw + min(c + j, cols_end - 1));
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) y[4 * q + j] = float(int(v[4 * q + j])) * sx * s[j];
   }
+}
+// Two sums times their scales.
+__device__ __forceinline__ float2 i8_scaled(uint32_t a, uint32_t b, float2 sx, float sa, float sb) {
+  return fmul2(fmul2(make_float2(float(int(a)), float(int(b))), sx), make_float2(sa, sb));
+}
+// The SiLU of two gates times what they gate: with t = 2^(-g / ln 2), g u / (1 + t).
+__device__ __forceinline__ float2 silu_mul2(float2 g, float2 u) {
+  const float2 e = fmul2(g, make_float2(-1.4426950408889634f, -1.4426950408889634f));
+  float a, b;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(e.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(e.y));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(1.f + a));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(1.f + b));
+  return fmul2(fmul2(g, make_float2(a, b)), u);
 }
 
 template <bool GATED>
 __device__ __forceinline__ void i8_pair_body(const CUtensorMap& tmX, const CUtensorMap& tmW, const I8PairArgs& args) {
+  constexpr int W = pair_warps(GATED);
   extern __shared__ uint8_t smem_raw[];
   // identical layout in both CTAs: [control 1 KB][ring]
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -475,7 +490,7 @@ __device__ __forceinline__ void i8_pair_body(const CUtensorMap& tmX, const CUten
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ctrl->tfull[i], 1);
-      mbar_init(&ctrl->tempty[i], 8);
+      mbar_init(&ctrl->tempty[i], 2 * W);
     }
     ctrl->abort = 0;
     mbar_fence_init();
@@ -583,9 +598,9 @@ __device__ __forceinline__ void i8_pair_body(const CUtensorMap& tmX, const CUten
     }
     __syncwarp();
   } else if (warp >= 2) {
-    // ------------------------------------------------------------------ epilogue (warps 2..5, both CTAs)
-    const int quad = warp & 3;
-    float* apart = reinterpret_cast<float*>(tiles + kApartStages * kPairStage) + quad * (32 * 33);
+    // ------------------------------------------------------------------ epilogue (warps 2.., both CTAs): 32 rows, all 32 columns or every second
+    const int quad = warp & 3, part = (warp - 2) >> 2;
+    float* apart = reinterpret_cast<float*>(tiles + kApartStages * kPairStage) + (warp - 2) * (32 * 33);
     griddep_wait();
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -599,37 +614,50 @@ __device__ __forceinline__ void i8_pair_body(const CUtensorMap& tmX, const CUten
       const uint32_t t0 = tmem_base + (uint32_t(quad * 32) << 16) + uint32_t(acc * kPairTileN);
       const int width = GATED ? half_n : tile_n;
       const int col0 = t.tn * width, cols_end = min(args.o.n, col0 + width);
+      if (part * 32 >= width) {                    // nothing for this warp
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(map_to_cta(&ctrl->tempty[acc], 0));
+      }
 #pragma unroll 1
-      for (int c = 0; c < width; c += 32) {
-        float y[32];
+      for (int c = part * 32; c < width; c += 8 * W) {
+        const bool some = col0 + c < cols_end;
+        float y[32], s[32];
         uint32_t v[32];
         tmem_ld_32x32(t0 + c, v);
+        if (some) i8_scales(args.o.sw, col0 + c, cols_end, s);          // (while the sums are on their way)
+        const float2 sx2 = make_float2(sx, sx);
         if constexpr (GATED) {
           uint32_t u[32];
+          float su[32];
           tmem_ld_32x32(t0 + half_n + c, u);
+          if (some) i8_scales(args.o.sw + args.o.n, col0 + c, cols_end, su);
           tmem_ld_wait();
-          if (col0 + c < cols_end) {
-            float up[32];
-            i8_scale_row(v, sx, args.o.sw, col0 + c, cols_end, y);
-            i8_scale_row(u, sx, args.o.sw + args.o.n, col0 + c, cols_end, up);
-            if (args.o.act) {
+          if (some) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) y[j] = gelu_tanh_f(y[j]) * up[j];
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) y[j] = silu_f(y[j]) * up[j];
+            for (int j = 0; j < 32; j += 2) {
+              const float2 g = i8_scaled(v[j], v[j + 1], sx2, s[j], s[j + 1]), up = i8_scaled(u[j], u[j + 1], sx2, su[j], su[j + 1]);
+              const float2 r = args.o.act ? make_float2(gelu_tanh_f(g.x) * up.x, gelu_tanh_f(g.y) * up.y) : silu_mul2(g, up);
+              y[j] = r.x;
+              y[j + 1] = r.y;
             }
           }
         } else {
           tmem_ld_wait();
-          if (col0 + c < cols_end) i8_scale_row(v, sx, args.o.sw, col0 + c, cols_end, y);
+          if (some) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              const float2 r = i8_scaled(v[j], v[j + 1], sx2, s[j], s[j + 1]);
+              y[j] = r.x;
+              y[j + 1] = r.y;
+            }
+          }
         }
-        if (c + 32 >= width) {
+        if (c + 8 * W >= width) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(map_to_cta(&ctrl->tempty[acc], 0));
         }
-        if (col0 + c >= cols_end) continue;
+        if (!some) continue;
         if (args.apart) i8_store_rows<GATED>(args.o, t.sp == 0, t.sp * args.split_stride, row - lane, col0 + c, cols_end, y, apart);
         else if (row < args.o.m) i8_store_row<GATED>(args.o, t.sp == 0, t.sp * args.split_stride, row, col0 + c, cols_end, y);
       }
@@ -651,7 +679,7 @@ __device__ __forceinline__ void i8_pair_body(const CUtensorMap& tmX, const CUten
 }
 
 template <bool GATED>
-__global__ void __launch_bounds__(kGemmThreads, 1)
+__global__ void __launch_bounds__(64 + 32 * pair_warps(GATED), 1)
 i8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const I8PairArgs args) {
   i8_pair_body<GATED>(tmX, tmW, args);
 }
@@ -718,13 +746,15 @@ static int resident_pairs(int dev, cudaLaunchConfig_t cfg) {
 // (measured, 200 tokens by 4096 x 14336): at 256 columns both operands' 32 KB per CTA and slab are what L2 gives an SM (52 bytes per clock), narrower
 // ones wait for the MMAs' and loads' latencies.  414 tokens by 2 x 14336 x 4096, us: 48.6 at 256, 47.1 at 192, 42 at 160, 52.7 at 128; 200 by 4096 x 4096
 // 17.5 at 256, 12.0 at 128, 11.2 at 64; 2048 by 4096 x 14336 79.8 at 256, 92 at 128.
-static int pair_width(int tiles_m, int splits, int slabs, int columns, int pairs, float* us_out) {
+static int pair_width(int tiles_m, int splits, int slabs, int columns, bool gated, int pairs, float* us_out) {
   static const struct { int width; float us; } kSlab[] = {{256, 0.326f}, {224, 0.287f}, {192, 0.250f}, {160, 0.224f}, {128, 0.207f}, {96, 0.200f}, {64, 0.192f}};
   int best = 256;
   float best_us = 0.f;
   for (const auto& t : kSlab) {
     const long long tiles = (long long)tiles_m * ((columns + t.width - 1) / t.width) * splits;
-    const float us = float((tiles + pairs - 1) / pairs) * float(slabs) * t.us + 4.f + 0.012f * float(t.width);
+    // (a tile of few slabs takes as long as what comes behind its sums: 848 tokens by 2 x 10720 x 100 59 us at 64 columns, 37 at 256)
+    const float tile = fmaxf(float(slabs) * t.us, gated ? 0.8f + 1.6f * float(t.width / 64) : 0.7f + 0.95f * float((t.width + 63) / 64));
+    const float us = float((tiles + pairs - 1) / pairs) * tile + 4.f + 0.012f * float(t.width);
     if (t.width == 256 || us < 0.97f * best_us) {
       best = t.width;
       best_us = us;
@@ -753,7 +783,7 @@ static int launch_i8_pairs(const NkbGemmI8& g, const I8Out& o) {
   int dev = -1;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDev) return -1;
   cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(kGemmThreads);
+  cfg.blockDim = dim3(64 + 32 * pair_warps(GATED));
   cfg.dynamicSmemBytes = size_t(kPairSmem);
   cfg.stream = reinterpret_cast<cudaStream_t>(g.stream);
   cudaLaunchAttribute attr[2];
@@ -767,7 +797,7 @@ static int launch_i8_pairs(const NkbGemmI8& g, const I8Out& o) {
   const int pairs = resident_pairs<GATED>(dev, cfg);
   if (pairs < 0) return -1;
   const int columns = (GATED ? 2 : 1) * g.n;
-  a.tile_n = pair_width(a.tiles_m, a.splits, a.kb_per_split, columns, pairs, nullptr);
+  a.tile_n = pair_width(a.tiles_m, a.splits, a.kb_per_split, columns, GATED, pairs, nullptr);
   a.tiles_n = (columns + a.tile_n - 1) / a.tile_n;
   if (GATED) a.tiles_n = (g.n + a.tile_n / 2 - 1) / (a.tile_n / 2);
   CUtensorMap tx, tw;
@@ -794,7 +824,7 @@ static bool pairs_first(const NkbGemmI8& g, int bn, int tiles, int splits) {
   const long long per_sm = ((long long)tiles * splits + num_sms() - 1) / num_sms();
   const float swap_us = (bn <= 64 ? 6.f : 8.3f) + 0.33f * float(per_sm) * float((slabs + splits - 1) / splits) * float(weights);
   float pair_us = 0.f;
-  pair_width((g.m + 255) / 256, 1, slabs, weights * g.n, num_sms() / 2, &pair_us);
+  pair_width((g.m + 255) / 256, 1, slabs, weights * g.n, g.gated, num_sms() / 2, &pair_us);
   return pair_us < swap_us;
 }
 
