@@ -71,7 +71,7 @@ struct RuleRow {
 };
 
 template <bool WIDE>
-__device__ __noinline__ float ruled(const RuleRow& r, float l0, uint32_t c, int token) {
+__device__ __noinline__ float ruled(const RuleRow& r, float l0, uint32_t c, double bias) {
   using C = Counts<WIDE>;
   double l = l0;
   const uint32_t n = c & C::kTimes;
@@ -80,23 +80,35 @@ __device__ __noinline__ float ruled(const RuleRow& r, float l0, uint32_t c, int 
     l -= double(r.freq) * double(n);
     if (n) l -= double(r.pres);
   }
-  if (c & C::kBiased) {
-    double sum = 0.0;
-    const int near = min(r.biases, kBiasMost);
+  return float(l + bias);
+}
+
+// The sum of a token's biases, and through `first` whether entry `at` is the first of them.
+__device__ __noinline__ double bias_sum(const RuleRow& r, int at, int token, bool& first) {
+  double sum = 0.0;
+  int least = at;
+  const int near = min(r.biases, kBiasMost);
 #pragma unroll 4
-    for (int i = 0; i < near; i += 4) {
-      const int4 id = r.near_ids[i >> 2];
-      if (id.x == token) sum += double(r.near_values[i]);
-      if (id.y == token) sum += double(r.near_values[i + 1]);
-      if (id.z == token) sum += double(r.near_values[i + 2]);
-      if (id.w == token) sum += double(r.near_values[i + 3]);
+  for (int i = 0; i < near; i += 4) {         // (the same entries in every lane)
+    const int4 id = r.near_ids[i >> 2];
+    const bool e[4] = {id.x == token, id.y == token, id.z == token, id.w == token};
+    if (e[0] || e[1] || e[2] || e[3]) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (e[j]) {
+          least = min(least, i + j);
+          sum += double(r.near_values[i + j]);
+        }
     }
-#pragma unroll 8
-    for (int i = near; i < r.biases; ++i)
-      if (r.bias_ids[i] == token) sum += double(r.bias_values[i]);
-    l += sum;
   }
-  return float(l);
+#pragma unroll 8
+  for (int i = near; i < r.biases; ++i)
+    if (r.bias_ids[i] == token) {
+      least = min(least, i);
+      sum += double(r.bias_values[i]);
+    }
+  first = least == at;
+  return sum;
 }
 
 template <bool F32>
@@ -236,8 +248,19 @@ __global__ void __launch_bounds__(kRuleThreads, 2) logit_rules_kernel(const NkbL
     for (int e = tid; e < n; e += kRuleThreads) {
       const int t = listed ? s_list[e] : lo + e;
       const uint32_t c = counts.get(t - lo);
-      if (!c || (mask && !((uint32_t(mask[t >> 5]) >> (t & 31)) & 1u))) continue;
-      const float v = ruled<WIDE>(r, rule_logit<F32>(in, t), c, t);
+      if (!c || (c & C::kBiased) || (mask && !((uint32_t(mask[t >> 5]) >> (t & 31)) & 1u))) continue;
+      const float v = ruled<WIDE>(r, rule_logit<F32>(in, t), c, 0.0);
+      if (ids) better(v, t);
+      else rule_store<F32>(out, t, v);
+    }
+    // tokens with biases: the first entry of each
+    for (int e = tid; e < a.biases; e += kRuleThreads) {
+      const int t = e < kBiasMost ? s_bias_ids[e] : r.bias_ids[e];
+      if (t < lo || t >= hi || (mask && !((uint32_t(mask[t >> 5]) >> (t & 31)) & 1u))) continue;
+      bool first;
+      const double bias = bias_sum(r, e, t, first);
+      if (!first) continue;
+      const float v = ruled<WIDE>(r, rule_logit<F32>(in, t), counts.get(t - lo), bias);
       if (ids) better(v, t);
       else rule_store<F32>(out, t, v);
     }
@@ -285,9 +308,9 @@ __global__ void __launch_bounds__(kRuleThreads, 2) logit_rules_kernel(const NkbL
           count(t.w, i + 3);
         }
       }
-      for (int i = tid; i < ((a.biases + 31) & ~31); i += kRuleThreads) {
-        const int t = i < a.biases ? r.bias_ids[i] : -1;
-        list(t >= lo && t < hi && counts.mark(t - lo, C::kBiased), t);
+      for (int i = tid; i < a.biases; i += kRuleThreads) {
+        const int t = r.bias_ids[i];
+        if (t >= lo && t < hi) counts.mark(t - lo, C::kBiased);
       }
       __syncthreads();
       if (ids) named_tokens(lo, hi);
