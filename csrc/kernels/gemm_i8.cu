@@ -614,10 +614,7 @@ __device__ __forceinline__ void i8_pair_body(const CUtensorMap& tmX, const CUten
       const uint32_t t0 = tmem_base + (uint32_t(quad * 32) << 16) + uint32_t(acc * kPairTileN);
       const int width = GATED ? half_n : tile_n;
       const int col0 = t.tn * width, cols_end = min(args.o.n, col0 + width);
-      if (part * 32 >= width) {                    // nothing for this warp
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(map_to_cta(&ctrl->tempty[acc], 0));
-      }
+      // (tiles have at least 64 columns, so every warp has some)
 #pragma unroll 1
       for (int c = part * 32; c < width; c += 8 * W) {
         const bool some = col0 + c < cols_end;
@@ -744,7 +741,7 @@ static int resident_pairs(int dev, cudaLaunchConfig_t cfg) {
 
 // Columns of a tile.  A pair takes its tiles one after another, so a narrower tile wins where it makes the rounds come out even.  us per slab of a tile
 // (measured, 200 tokens by 4096 x 14336): at 256 columns both operands' 32 KB per CTA and slab are what L2 gives an SM (52 bytes per clock), narrower
-// ones wait for the MMAs' and loads' latencies.  414 tokens by 2 x 14336 x 4096, us: 48.6 at 256, 47.1 at 192, 42 at 160, 52.7 at 128; 200 by 4096 x 4096
+// ones wait for the MMAs' and loads' latencies.  414 tokens by 2 x 14336 x 4096, us: 52.1 at 256, 50.0 at 192, 49.5 at 160, 54.7 at 128; 200 by 4096 x 4096
 // 17.5 at 256, 12.0 at 128, 11.2 at 64; 2048 by 4096 x 14336 79.8 at 256, 92 at 128.
 static int pair_width(int tiles_m, int splits, int slabs, int columns, bool gated, int pairs, float* us_out) {
   static const struct { int width; float us; } kSlab[] = {{256, 0.326f}, {224, 0.287f}, {192, 0.250f}, {160, 0.224f}, {128, 0.207f}, {96, 0.200f}, {64, 0.192f}};

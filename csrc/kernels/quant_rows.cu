@@ -6,7 +6,7 @@
 // (numbers8 in quant_rows.cuh) takes the nearest k by a rounding constant and looks at what is left of it, which is exact, too.
 //   norm   The norm's factor r = 1 / sqrt(mean(h^2) + eps) is the same for the whole row: 127 (r h w) / max|r h w| = 127 (h w) / max|h w|.  So the numbers
 //          come from the exact products h * w, and r enters the scale alone: no rounding of statistics can move a number to its neighbour.
-//   gate   silu(g) * u is not exact in 32 bits.  Numbers within 2^-11 of a half (one in a thousand) and candidates for the row's maximum are worked out
+//   gate   silu(g) * u is not exact in 32 bits.  Numbers within 2^-12 of a half (one in two thousand; 2^-13 where gate and up are no sums) and candidates for the row's maximum are worked out
 //          once more in 64 bits; rows that are small altogether, and the clamped form, whose up + 1 may cancel, in 64 bits as a whole.
 // A row with a value that is not finite gets the scale NaN and zeros; a row of zeros the scale 0.
 //

@@ -116,6 +116,8 @@ def _packed(logits, rules: LogitRules, out, out_ids) -> bytes:
         width = r.tokens.shape[1]
         lens, prompts = _vector(r.lens, "lens", i32, rows, index), _vector(r.prompt_lens, "prompt_lens", i32, rows, index)
         ids = _vector(r.ids, "ids", i32, rows, index)
+        if ids and B > 1 and tokens_ld < width:
+            raise ValueError("rows of tokens that ids are written to want memory of their own")
         rep = _vector(r.repetition, "repetition", number, rows, index)
         freq, pres = _vector(r.frequency, "frequency", number, rows, index), _vector(r.presence, "presence", number, rows, index)
     elif r.lens is not None or r.ids is not None or r.prompt_lens is not None:

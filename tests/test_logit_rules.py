@@ -398,3 +398,13 @@ def test_more_named_tokens_than_are_listed(device):
     r["tokens"] = torch.stack([torch.randperm(9000, generator=g)[:4000] for _ in range(2)]).int()
     r["lens"] = torch.tensor([4000, 1100], dtype=torch.int32)
     check(logits_of(5, 2, 9000, BF), r, device)
+
+
+def test_rows_that_share_their_tokens():
+    """Read they may be; the newest tokens have no place of their own in them."""
+    tokens = torch.arange(6, dtype=torch.int32).expand(3, 6)
+    rules = dict(tokens=tokens, lens=torch.tensor([6, 2, 0], dtype=torch.int32), presence=torch.ones(3))
+    y = ops.apply_rules(torch.zeros((3, 8)), ops.LogitRules(**rules))
+    assert (y != 0).sum(-1).tolist() == [6, 2, 0]
+    with pytest.raises(ValueError):
+        ops.apply_rules(torch.zeros((3, 8)), ops.LogitRules(**rules, ids=torch.zeros(3, dtype=torch.int32)))
