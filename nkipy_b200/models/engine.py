@@ -136,8 +136,13 @@ class StepRules:
             ids = self.sampling.allowed(p, a)
             if ids is None:
                 bits[i] = True
-            else:
-                bits[i, ids if torch.is_tensor(ids) else list(ids)] = True
+                continue
+            ids = ids.cpu() if torch.is_tensor(ids) else torch.tensor(list(ids), dtype=torch.int64)
+            if ids.dtype is not torch.bool:
+                if ids.numel() and not 0 <= int(ids.min()) <= int(ids.max()) < self.vocab:
+                    raise ValueError("a sequence may go on with tokens of the vocabulary")
+                ids = ids.long()
+            bits[i, ids] = True
         at = torch.tensor(list(rows), device=self.device)
         self.rules.mask.index_copy_(0, at, ops.pack_mask(bits).to(self.device))
 
@@ -567,38 +572,41 @@ class GenerationEngine:
         rules = StepRules(sampling, self.model.cfg.vocab_size, self.max_batch, self.max_seq_len + 1, self.device) if ruled else None
         seqs = self.add_requests(prompts)
         slots, prompts = [s.slot for s in seqs], [list(p) for p in prompts]
-        if rules is not None:
-            rules.start(slots, prompts)
-        self.prefill(seqs, sampling, rules)
-        outs: List[List[int]] = [[s.tokens[-1]] for s in seqs]
-        # (-1: the rules have left nothing)
-        finished = [o[0] < 0 or (eos_token_id is not None and o[0] == eos_token_id) for o in outs]
-        if max_new_tokens > 1:
-            self.prepare_decode(max_new_tokens)
-        t0 = time.perf_counter()
-        steps = 0
-        for _ in range(max_new_tokens - 1):
-            if all(finished):
-                break
-            ts = time.perf_counter()
+        try:
             if rules is not None:
-                on = [j for j in range(len(seqs)) if not finished[j]]
-                rules.allow([slots[j] for j in on], [prompts[j] for j in on], [outs[j] for j in on])
-            host = self.step(sampling=sampling, rules=rules).clone()
-            self.stats.decode_step_ms.append((time.perf_counter() - ts) * 1e3)
-            self.advance_host_state(1)
-            steps += 1
-            for j, s in enumerate(seqs):
-                if finished[j]:
-                    continue
-                tok = int(host[s.slot])
-                outs[j].append(tok)
-                s.tokens.append(tok)
-                if tok < 0 or (eos_token_id is not None and tok == eos_token_id):
-                    finished[j] = True
-        self.stats.decode_time_s += time.perf_counter() - t0
-        self.stats.decode_tokens += steps * len(seqs)
-        self.release(seqs)
+                rules.start(slots, prompts)
+            self.prefill(seqs, sampling, rules)
+            outs: List[List[int]] = [[s.tokens[-1]] for s in seqs]
+            # (-1: the rules have left nothing)
+            finished = [o[0] < 0 or (eos_token_id is not None and o[0] == eos_token_id) for o in outs]
+            if max_new_tokens > 1:
+                self.prepare_decode(max_new_tokens)
+            t0 = time.perf_counter()
+            steps = 0
+            for _ in range(max_new_tokens - 1):
+                if all(finished):
+                    break
+                ts = time.perf_counter()
+                if rules is not None:
+                    on = [j for j in range(len(seqs)) if not finished[j]]
+                    rules.allow([slots[j] for j in on], [prompts[j] for j in on], [outs[j] for j in on])
+                host = self.step(sampling=sampling, rules=rules).clone()
+                self.stats.decode_step_ms.append((time.perf_counter() - ts) * 1e3)
+                self.advance_host_state(1)
+                steps += 1
+                for j, s in enumerate(seqs):
+                    if finished[j]:
+                        continue
+                    tok = int(host[s.slot])
+                    outs[j].append(tok)
+                    s.tokens.append(tok)
+                    if tok < 0 or (eos_token_id is not None and tok == eos_token_id):
+                        finished[j] = True
+            self.stats.decode_time_s += time.perf_counter() - t0
+            self.stats.decode_tokens += steps * len(seqs)
+        finally:
+            # (whatever `allowed` raises, the rows are free again)
+            self.release(seqs)
         return [o[:-1] if o[-1] < 0 else o for o in outs] if rules is not None else outs
 
     def release(self, seqs: Iterable[SequenceState]) -> None:

@@ -197,6 +197,25 @@ def test_generation_under_a_grammar(device):
         assert len(out[1]) == 3 and all(t % 2 == i % 2 for i, t in enumerate(out[1]))
 
 
+def test_rows_are_free_after_a_grammar_that_fails():
+    engine = GenerationEngine(model_of("llama", "cpu", False), max_batch=2, max_seq_len=64)
+    prompts = [ids(20, 1), ids(9, 2)]
+    plain = engine.generate(prompts, 4)
+
+    def raises(prompt, answer):
+        if len(answer) == 2:
+            raise KeyError("no such state")
+
+    for at in (0, 2):
+        for bad in ([-1], [512], torch.tensor([3, 512])):
+            with pytest.raises(ValueError):
+                engine.generate(prompts, 4, sampling=Sampling(allowed=lambda p, a: bad if len(a) == at else None))
+            assert not engine.active
+    with pytest.raises(KeyError):
+        engine.generate(prompts, 4, sampling=Sampling(allowed=raises))
+    assert not engine.active and engine.generate(prompts, 4) == plain
+
+
 def test_refusals_of_sampling():
     for kw in (dict(repetition=0.0), dict(repetition=-1.0), dict(repetition=float("inf")), dict(repetition=float("nan")), dict(frequency=float("nan")),
                dict(presence=float("inf"))):
