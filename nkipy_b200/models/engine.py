@@ -242,6 +242,7 @@ class GenerationEngine:
         self.active: Dict[int, SequenceState] = {}     # table row -> sequence
         self._opened: set = set()                      # rows whose length on the device may not be -1
         self._graph = None
+        self._weights = getattr(model, "weights_version", 0)      # the weights that graph and cached prefixes come from
         self.step_logits: Optional[torch.Tensor] = None   # logits of the last decode step [max_batch, V] (one rank)
         tp = model.tp
         if ((tp.world_size > 1 or getattr(model, "force_fused", False)) and dev.type == "cuda"
@@ -252,8 +253,23 @@ class GenerationEngine:
             tp.fused = FusedTP(tp, max_batch, model.cfg.hidden_size)
         self.stats = GenerationStats()
 
+    def _check_weights(self) -> None:
+        """Ahead of every use: where the model's weights have been replaced, the captured step reads memory that is no longer theirs, and the cache
+        holds keys and values that they did not make."""
+        version = getattr(self.model, "weights_version", 0)
+        if version == self._weights:
+            return
+        if any(s.num_computed for s in self.active.values()):
+            raise RuntimeError("the model's weights were replaced while sequences were open: release them first")
+        if self.device.type == "cuda":
+            torch.cuda.synchronize()
+        self._graph = None
+        self.cache.allocator.forget()
+        self._weights = version
+
     # ------------------------------------------------------------------ admission + prefill
     def add_requests(self, prompts: Sequence[Sequence[int]]) -> List[SequenceState]:
+        self._check_weights()
         seqs = [self.cache.add_sequence(p) for p in prompts]
         for s in seqs:
             self.active[s.slot] = s
@@ -314,6 +330,7 @@ class GenerationEngine:
                 rules: Optional[StepRules] = None) -> torch.Tensor:
         """Run the uncached part of the prompts (in portions of at most the token budget); returns the first
         generated token of every sequence (int32, device) and records per-sequence TTFT.  rules: of the sequences' rows."""
+        self._check_weights()
         m, cache, dev = self.model, self.cache, self.device
         first = torch.zeros((len(seqs),), dtype=torch.int32, device=dev)
         t0 = time.perf_counter()
@@ -414,6 +431,7 @@ class GenerationEngine:
     def decode_step_device(self) -> None:
         """One decode step whose input ids are already on the device (the previous step's
         output); nothing crosses PCIe."""
+        self._check_weights()
         if self.use_cuda_graph:
             self._graph.replay()
         else:
@@ -442,6 +460,7 @@ class GenerationEngine:
         return self.out_host
 
     def prepare_decode(self, steps: int, reserve: bool = True) -> None:
+        self._check_weights()
         if reserve:
             self._reserve(steps)
         if self.device.type == "cuda":
@@ -455,6 +474,7 @@ class GenerationEngine:
     # ------------------------------------------------------------------ steps of an external scheduler
     def open_request(self) -> SequenceState:
         """A sequence whose tokens arrive with `run_step`; `release` gives its blocks and row back."""
+        self._check_weights()
         s = self.cache.open_sequence()
         self.active[s.slot] = s
         return s
@@ -465,6 +485,7 @@ class GenerationEngine:
         wanted).  A step in which every sequence goes on by a single token is a decode step (the captured graph);
         any other mix of portions and single tokens is one packed batch.  Open sequences without an entry are left
         as they are."""
+        self._check_weights()
         if len({e.seq.slot for e in entries}) != len(entries):
             raise ValueError("a sequence may have one entry in a step")
         lens, places, decode, limit = [], [], self.model.tp.world_size == 1, self.max_seq_len

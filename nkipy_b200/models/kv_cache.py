@@ -136,6 +136,13 @@ class BlockAllocator:
                 self.by_hash[h] = b
             parent = h
 
+    def forget(self) -> None:
+        """No block is found by its tokens any more: what the blocks hold was computed by other weights."""
+        self.free.extend(self.evictable)
+        self.evictable.clear()
+        self.by_hash.clear()
+        self.hash_of = [None] * self.num_blocks
+
     def extend(self, blocks: List[int], new_len: int) -> int:
         """Grow a block list to cover new_len tokens; returns the number of blocks added."""
         need = (new_len + self.block_size - 1) // self.block_size - len(blocks)

@@ -111,6 +111,7 @@ class TransformerLM:
         inv_freq, rope_scale = yarn_inv_freq(cfg)
         self.rope = ops.rope_table(cfg.head_dim, cfg.max_position, inv_freq=inv_freq, scaling=rope_scale, device=dev)
         self.quantized = False                # weights in 8 bits (`quantize_weights`)
+        self.weights_version = 0              # counts replacements of the weights: engines compare it with what their graph and cache come from
         self._moe = None
         if cfg.is_moe:
             from .moe import MoEBlock
@@ -133,10 +134,14 @@ class TransformerLM:
 
     def quantize_weights(self) -> "TransformerLM":
         """Projections, feed-forward and head in 8-bit whole numbers with a scale for every output channel, which the products multiply
-        with activations in 8 bits; embeddings, norms and attention stay as they are.  Dense models on one rank."""
+        with activations in 8 bits; embeddings, norms and attention stay as they are.  Dense models on one rank.
+
+        The bf16 weights are let go.  A `GenerationEngine` that has run on them captures its decode step anew and forgets its cached prefixes, and wants
+        its open sequences released first; graphs that a program has captured itself hold the old weights' addresses and are not to be replayed."""
         if self.cfg.is_moe or self.tp.world_size > 1 or self.force_fused:
             raise ValueError("weights in 8 bits are for dense models on one rank")
         if not self.quantized:
+            self.weights_version += 1
             for lw in self.layers:
                 for name in ("qkv", "o", "gate_up", "down"):
                     setattr(lw, name, ops.QuantizedWeight.of(getattr(lw, name)))

@@ -241,3 +241,63 @@ def test_command_line(capsys):
     assert "Generated 3 tokens" in capsys.readouterr().out
     with pytest.raises(ValueError):
         runner.quantize_weights(args, object())
+
+
+# ------------------------------------------------------------------------------------------------ weights that are replaced under an engine
+@pytest.mark.parametrize("device", DEVICES)
+def test_an_engine_whose_models_weights_are_replaced(device):
+    """Neither the captured step nor the keys and values of the bf16 weights serve the quantised model."""
+    prompts = [ids(100, 1), ids(7, 2)]
+    model = model_of("llama", device, quantize=False)
+    engine = GenerationEngine(model, max_batch=2, max_seq_len=160)
+    engine.generate(prompts, 8)
+    cached, graph = engine.stats.cached_tokens, engine._graph
+    model.quantize_weights()
+    out = engine.generate(prompts, 8)
+    assert engine.stats.cached_tokens == cached and (device == "cpu" or engine._graph is not graph)
+    assert out == GenerationEngine(model_of("llama", device), max_batch=2, max_seq_len=160).generate(prompts, 8)
+    # the quantised model's own prefixes are found again, and every block is there
+    assert engine.generate(prompts, 8) == out and engine.stats.cached_tokens == cached + 96
+    assert engine.cache.allocator.num_free() == engine.cache.num_blocks
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_open_sequences_do_not_outlive_their_weights(device):
+    model = model_of("llama", device, quantize=False)
+    engine = GenerationEngine(model, max_batch=2, max_seq_len=96)
+    s, new = engine.open_request(), engine.open_request()
+    engine.run_step([StepEntry(s, ids(40, 1), [-1])])
+    engine.run_step([StepEntry(s, ids(1, 2), [-1])])
+    model.quantize_weights()
+    for call in (lambda: engine.run_step([StepEntry(s, ids(1, 3), [-1])]), lambda: engine.run_step([StepEntry(new, ids(4, 3), [-1])]),
+                 lambda: engine.add_requests([ids(5, 3)]), engine.open_request, lambda: engine.prepare_decode(1), engine.step,
+                 engine.decode_step_device):
+        with pytest.raises(RuntimeError, match="weights were replaced"):
+            call()
+    engine.release([s])
+    fresh = GenerationEngine(model, max_batch=2, max_seq_len=96)
+    other = fresh.open_request()
+    for tokens in (ids(40, 1), ids(1, 5)):             # (a sequence of which nothing was computed goes on)
+        a, b = engine.run_step([StepEntry(new, tokens, [-1])]), fresh.run_step([StepEntry(other, tokens, [-1])])
+        assert torch.equal(a, b)
+
+
+def test_blocks_are_forgotten():
+    from nkipy_b200.models.kv_cache import BlockAllocator
+
+    a = BlockAllocator(6)
+    tokens = list(range(70))
+    held, _ = a.admit(tokens)
+    a.publish(tokens, held, 70)
+    gone, cached = a.admit(tokens[:40])
+    assert cached == 32
+    a.release(gone)
+    a.release(held)
+    assert len(a.evictable) == 2
+    kept, _ = a.admit(tokens)
+    a.forget()
+    blocks, cached = a.admit(tokens)
+    assert cached == 0 and not set(blocks) & set(kept)
+    a.release(blocks)
+    a.publish(tokens, kept, 70)
+    assert a.admit(tokens[:40])[0][0] == kept[0]
