@@ -1,6 +1,6 @@
 // Rules on logits: penalties for repeated tokens, biases and masks; the logits that are left, or the most likely token.
 //
-// Mathematics, per row, for the tokens that the rules name, in 64 bits and rounded once:
+// Mathematics, per row, for the tokens that the rules name, in 64 bits and rounded once, to the logits' type, or to 32 bits where they are compared:
 //   seen (in the prompt or the answer):  l = l > 0 ? l / repetition : l * repetition
 //   n times among the answer's tokens:   l -= frequency * n;  l -= presence where n > 0
 //   biases:                              l += the sum of the token's entries, in their order
@@ -72,7 +72,7 @@ struct RuleRow {
 };
 
 template <bool WIDE>
-__device__ __noinline__ float ruled(const RuleRow& r, float l0, uint32_t c, double bias) {
+__device__ __noinline__ double ruled(const RuleRow& r, float l0, uint32_t c, double bias) {
   using C = Counts<WIDE>;
   double l = l0;
   const uint32_t n = c & C::kTimes;
@@ -81,7 +81,13 @@ __device__ __noinline__ float ruled(const RuleRow& r, float l0, uint32_t c, doub
     l -= double(r.freq) * double(n);
     if (n) l -= double(r.pres);
   }
-  return float(l + bias);
+  return l + bias;
+}
+// 64 bits on their way to bf16, rounded to odd: the rounding that follows is then the only one (to the nearest here, a value beside the middle of two bf16
+// numbers would become the middle, and 1 + 2^-8 + 2^-31 the lower one).
+__device__ __forceinline__ float to_odd(double l) {
+  const float f = __double2float_rz(l);
+  return double(f) == l ? f : __uint_as_float(__float_as_uint(f) | 1u);
 }
 
 // The sum of a token's biases, and through `first` whether entry `at` is the first of them.
@@ -250,9 +256,9 @@ __global__ void __launch_bounds__(kRuleThreads, 2) logit_rules_kernel(const NkbL
       const int t = listed ? s_list[e] : lo + e;
       const uint32_t c = counts.get(t - lo);
       if (!c || (c & C::kBiased) || (mask && !((uint32_t(mask[t >> 5]) >> (t & 31)) & 1u))) continue;
-      const float v = ruled<WIDE>(r, rule_logit<F32>(in, t), c, 0.0);
-      if (ids) better(v, t);
-      else rule_store<F32>(out, t, v);
+      const double l = ruled<WIDE>(r, rule_logit<F32>(in, t), c, 0.0);
+      if (ids) better(float(l), t);
+      else rule_store<F32>(out, t, F32 ? float(l) : to_odd(l));
     }
     // tokens with biases: the first entry of each
     for (int e = tid; e < a.biases; e += kRuleThreads) {
@@ -261,9 +267,9 @@ __global__ void __launch_bounds__(kRuleThreads, 2) logit_rules_kernel(const NkbL
       bool first;
       const double bias = bias_sum(r, e, t, first);
       if (!first) continue;
-      const float v = ruled<WIDE>(r, rule_logit<F32>(in, t), counts.get(t - lo), bias);
-      if (ids) better(v, t);
-      else rule_store<F32>(out, t, v);
+      const double l = ruled<WIDE>(r, rule_logit<F32>(in, t), counts.get(t - lo), bias);
+      if (ids) better(float(l), t);
+      else rule_store<F32>(out, t, F32 ? float(l) : to_odd(l));
     }
   };
 

@@ -15,14 +15,14 @@ import torch
 
 from . import _lib
 from . import _count_launch, _stream
-from .quantized_linear import _on_gpu
+from .quantized_linear import _on_gpu, to_bf16
 
 _ARGS = struct.Struct("15P5q6i")          # NkbLogitRules of csrc/kernels/rules_args.h
 
 
 @dataclass(slots=True)
 class LogitRules:
-    """What is done to the logits [rows, vocab] of a step, in 64 bits and rounded once, in this order:
+    """What is done to the logits [rows, vocab] of a step, in 64 bits and rounded once (`apply_rules` to their type, `argmax` to fp32), in this order:
 
     tokens int32 [rows, width], lens int32 [rows]: the ids of every row so far, the newest included (lens beyond the width count as the
         width; a length below one: no tokens).  ids int32 [rows]: the newest, which the call writes to tokens[b, lens[b] - 1]; None: it
@@ -146,7 +146,7 @@ def _packed(logits, rules: LogitRules, out, out_ids) -> bytes:
 
 
 def _reference(logits, r: LogitRules) -> torch.Tensor:
-    """fp32 logits under the rules; writes the newest tokens."""
+    """Logits under the rules in 64 bits; writes the newest tokens."""
     y = logits.double().clone()
     B, V = y.shape
     for b in range(B):
@@ -176,7 +176,7 @@ def _reference(logits, r: LogitRules) -> torch.Tensor:
         if r.mask is not None and 0 <= m < r.mask.shape[0]:
             t = torch.arange(V)
             row[((r.mask[m][t // 32] >> (t % 32)) & 1) == 0] = float("-inf")
-    return y.float()
+    return y
 
 
 def apply_rules(logits: torch.Tensor, rules: LogitRules, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -188,7 +188,8 @@ def apply_rules(logits: torch.Tensor, rules: LogitRules, out: Optional[torch.Ten
     if not logits.shape[0]:
         return out
     if not _on_gpu(logits.get_device()):
-        return out.copy_(_reference(logits, rules))
+        y = _reference(logits, rules)
+        return out.copy_(to_bf16(y) if out.dtype is torch.bfloat16 else y)
     rc = _lib.lib().nkb_logit_rules(args)
     if rc:
         _lib.check(rc, "nkb_logit_rules")
@@ -204,7 +205,7 @@ def argmax(logits: torch.Tensor, rules: LogitRules, out_ids: Optional[torch.Tens
     if not logits.shape[0]:
         return out_ids
     if not _on_gpu(logits.get_device()):
-        y = _reference(logits, rules).nan_to_num(nan=float("-inf"), posinf=float("inf"), neginf=float("-inf"))
+        y = _reference(logits, rules).float().nan_to_num(nan=float("-inf"), posinf=float("inf"), neginf=float("-inf"))
         top, at = y.max(-1)
         first = torch.where(y == top[:, None], torch.arange(y.shape[1]), y.shape[1]).amin(-1)
         return out_ids.copy_(torch.where(top == float("-inf"), -1, first))

@@ -127,6 +127,15 @@ def _on_gpu(index: int) -> bool:
 _BF16, _F32 = torch.bfloat16, torch.float32
 
 
+def to_bf16(y: torch.Tensor) -> torch.Tensor:
+    """Numbers in 64 bits rounded to bf16 once: on the way through 32 bits to odd, since to the nearest they may come to lie in the middle of two
+    bf16 numbers that they are not in the middle of."""
+    f = y.float()
+    d, bits = f.double(), f.view(torch.int32)
+    bits = torch.where((d == y) | y.isnan(), bits, (bits - (d.abs() > y.abs()).int()) | 1)
+    return bits.view(torch.float32).to(_BF16)
+
+
 # --------------------------------------------------------------------------- rows
 def _numbers(x: torch.Tensor):
     """(whole numbers, largest magnitude) of rows in 64 bits; zeros and NaN where a row is not finite in 32."""

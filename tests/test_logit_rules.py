@@ -408,3 +408,31 @@ def test_rows_that_share_their_tokens():
     assert (y != 0).sum(-1).tolist() == [6, 2, 0]
     with pytest.raises(ValueError):
         ops.apply_rules(torch.zeros((3, 8)), ops.LogitRules(**rules, ids=torch.zeros(3, dtype=torch.int32)))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_logits_are_rounded_once(device):
+    """Sums beside the middle of two bf16 numbers, which 32 bits hold as the middle itself; and the middle."""
+    middle, off = 2.0 ** -8, 2.0 ** -31
+    x = torch.ones((1, 24), dtype=BF)
+    x[0, 8:16], x[0, 16:] = -1.0, 1 + 2.0 ** -7
+    add = torch.tensor([[middle + off, middle - off, middle, 2 ** -7, -off, off, 0, -middle / 2,
+                         -middle - off, -middle + off, -middle, 0, -off, off, -2.0 ** -7, middle / 2,
+                         middle + off, middle - off, middle, -middle, -middle - off, -middle + off, off, -off]])
+    up, upper = 1 + 2.0 ** -7, 1 + 2.0 ** -6
+    want = [up, 1, 1, up, 1, 1, 1, 1, -up, -1, -1, -1, -1, -1, -up, -1,          # (1 - 2^-9 lies in the middle: to the even one)
+            upper, up, upper, 1, 1, up, up, up]
+    rules = ops.LogitRules(bias_ids=torch.arange(24).int()[None].to(device), bias_values=add.to(device))
+    for out in (None, x.to(device, copy=True)):
+        assert ops.apply_rules(x.to(device) if out is None else out, rules, out=out).tolist() == [want]
+    # penalties alike: 1 + 2^-8 + 2^-31 again; and numbers beyond the largest one
+    x = torch.tensor([[1.0, 3.3895e38, -3.3895e38]], dtype=BF)
+    rules = ops.LogitRules(tokens=torch.arange(3).int()[None].to(device), lens=torch.tensor([3]).int().to(device),
+                           frequency=torch.tensor([-(middle + off)]).to(device))
+    assert float(ops.apply_rules(x.to(device), rules)[0, 0]) == up
+    rules.frequency = torch.tensor([3e38]).to(device)
+    assert ops.apply_rules(x.to(device), rules).tolist()[0][2] == -INF
+    # the choice compares 32 bits
+    same = torch.ones((1, 2), dtype=BF)
+    rules = ops.LogitRules(bias_ids=torch.tensor([[0, 1]]).int().to(device), bias_values=torch.tensor([[middle, middle + off]]).to(device))
+    assert ops.argmax(same.to(device), rules=rules).tolist() == [0]
