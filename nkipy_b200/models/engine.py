@@ -403,19 +403,16 @@ class GenerationEngine:
     def _ensure_graph(self) -> None:
         if not self.use_cuda_graph or self._graph is not None:
             return
-        # warm up on a side stream (allocations, attribute setup, NCCL channels), restoring the
-        # state the warm-up step mutates, then capture
+        # warm up on a side stream (allocations, attribute setup, NCCL channels) without rows, then capture.  A row's length on the device may be behind what packed
+        # steps have computed, and the step would write over tokens in the cache; a recurrent state cannot take the same token twice
         saved = (self.ids.clone(), self.context_lens.clone())
-        if self.cache.has_state:
-            self.context_lens.fill_(-1)     # a recurrent state cannot take the same token twice: warm up without rows
         s = torch.cuda.Stream()
         s.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(s):
             for _ in range(2):
+                self.context_lens.fill_(-1)
                 self._decode_body()
                 self.ids.copy_(saved[0])
-                if not self.cache.has_state:
-                    self.context_lens.copy_(saved[1])
         torch.cuda.current_stream().wait_stream(s)
         torch.cuda.synchronize()
         before = ops.launch_count()
