@@ -1,7 +1,8 @@
 // Products of rows and weights in 8-bit whole numbers: y[m, n] = sx[m] * sw[n] * sum_k x[m, k] w[n, k], both operands K-major.
 //
 // The sums are whole numbers of 32 bits (at most 128 * 128 * k, so k is up to 131071), exact whatever their order; the only roundings are
-// those of the epilogue: sum -> fp32, times sx, times sw, + bias, + residual, -> bf16.  So every variant below gives the same bits.
+// those of the epilogue: sum -> fp32, times sx, times sw, gate, + bias, + residual, -> bf16, the same operations in every kernel (i8_epilogue.cuh).  So every
+// variant below, and the kernel for few tokens, gives a token the same bits, whatever else is in the step.
 //
 // Two kernels:
 //   pairs  D[tokens, features] on CTA pairs (tcgen05.mma.cta_group::2.kind::i8, tiles of 256 tokens by up to 256 features), for prompts;
@@ -12,6 +13,7 @@
 #include "api.h"
 #include "gemm_tcgen05.cuh"
 #include "i8_args.h"
+#include "i8_epilogue.cuh"
 
 namespace nkb {
 
@@ -79,8 +81,6 @@ struct I8PairArgs {
 };
 static_assert(sizeof(I8SwapArgs) <= 112 && sizeof(I8PairArgs) <= 128, "argument blocks grew past the fast kernel-parameter size");
 
-__device__ __forceinline__ float gate_act(float g, int act) { return act ? gelu_tanh_f(g) : silu_f(g); }
-
 // ------------------------------------------------------------------------------------------------ swap
 struct I8Ctrl {
   uint64_t full[kMaxStages];
@@ -113,9 +113,9 @@ __device__ __forceinline__ void i8_store4(const I8Out& a, const Features4<GATED>
   float y[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    y[j] = float(sv[j]) * sx * w.sw[j];
-    if constexpr (GATED) y[j] = gate_act(y[j], a.act) * (float(uv[j]) * sx * w.su[j]);
-    else if (a.bias) y[j] += w.bias[j];
+    y[j] = i8_scaled(sv[j], sx, w.sw[j]);
+    if constexpr (GATED) y[j] = i8_gated(y[j], i8_scaled(uv[j], sx, w.su[j]), a.act);
+    else if (a.bias) y[j] = add_rn(y[j], w.bias[j]);
   }
   at += (long long)tok * a.ldo + f;
   const bool whole = f + 4 <= a.n;
@@ -124,11 +124,11 @@ __device__ __forceinline__ void i8_store4(const I8Out& a, const Features4<GATED>
     if (whole && (reinterpret_cast<uintptr_t>(r) & 7) == 0) {
       const uint2 v = *reinterpret_cast<const uint2*>(r);
       const float2 lo = unpack_bf16x2(v.x), hi = unpack_bf16x2(v.y);
-      y[0] += lo.x; y[1] += lo.y; y[2] += hi.x; y[3] += hi.y;
+      y[0] = add_rn(y[0], lo.x); y[1] = add_rn(y[1], lo.y); y[2] = add_rn(y[2], hi.x); y[3] = add_rn(y[3], hi.y);
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (f + j < a.n) y[j] += __bfloat162float(r[j]);
+        if (f + j < a.n) y[j] = add_rn(y[j], __bfloat162float(r[j]));
     }
   }
   if (a.fp32) {
@@ -359,7 +359,7 @@ __device__ __forceinline__ void i8_store_row(const I8Out& a, bool first, long lo
   if (!GATED && a.bias && first) {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
-      if (c + j < cols_end) y[j] += __bfloat162float(__ldg(a.bias + c + j));
+      if (c + j < cols_end) y[j] = add_rn(y[j], __bfloat162float(__ldg(a.bias + c + j)));
   }
   if (!GATED && a.residual) {
     const __nv_bfloat16* r = a.residual + at;
@@ -372,13 +372,13 @@ __device__ __forceinline__ void i8_store_row(const I8Out& a, bool first, long lo
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float2 f = unpack_bf16x2(rw[e]);
-          y[8 * q + 2 * e] += f.x;
-          y[8 * q + 2 * e + 1] += f.y;
+          y[8 * q + 2 * e] = add_rn(y[8 * q + 2 * e], f.x);
+          y[8 * q + 2 * e + 1] = add_rn(y[8 * q + 2 * e + 1], f.y);
         }
       } else {
 #pragma unroll
         for (int j = 8 * q; j < 8 * q + 8; ++j)
-          if (c + j < cols_end) y[j] += __bfloat162float(r[j]);
+          if (c + j < cols_end) y[j] = add_rn(y[j], __bfloat162float(r[j]));
       }
     }
   }
@@ -427,8 +427,8 @@ __device__ __forceinline__ void i8_store_rows(const I8Out& a, bool first, long l
 #pragma unroll 8
     for (int r = 0; r < rows; ++r, at += a.ldo) {
       float v = tile[r * 33 + lane];
-      if (!GATED && a.bias) v += bias;
-      if (!GATED && a.residual) v += __bfloat162float(a.residual[at]);
+      if (!GATED && a.bias) v = add_rn(v, bias);
+      if (!GATED && a.residual) v = add_rn(v, __bfloat162float(a.residual[at]));
       if (a.fp32) reinterpret_cast<float*>(a.out)[at] = v;
       else reinterpret_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16(v);
     }
@@ -449,20 +449,6 @@ __device__ __forceinline__ void i8_scales(const float* sw, int c, int cols_end, 
       for (int j = 4 * q; j < 4 * q + 4; ++j) s[j] = __ldg(sw + min(c + j, cols_end - 1));
     }
   }
-}
-// Two sums times their scales.
-__device__ __forceinline__ float2 i8_scaled(uint32_t a, uint32_t b, float2 sx, float sa, float sb) {
-  return fmul2(fmul2(make_float2(float(int(a)), float(int(b))), sx), make_float2(sa, sb));
-}
-// The SiLU of two gates times what they gate: with t = 2^(-g / ln 2), g u / (1 + t).
-__device__ __forceinline__ float2 silu_mul2(float2 g, float2 u) {
-  const float2 e = fmul2(g, make_float2(-1.4426950408889634f, -1.4426950408889634f));
-  float a, b;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(e.x));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(e.y));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(1.f + a));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(1.f + b));
-  return fmul2(fmul2(g, make_float2(a, b)), u);
 }
 
 template <bool GATED>
@@ -632,8 +618,8 @@ __device__ __forceinline__ void i8_pair_body(const CUtensorMap& tmX, const CUten
           if (some) {
 #pragma unroll
             for (int j = 0; j < 32; j += 2) {
-              const float2 g = i8_scaled(v[j], v[j + 1], sx2, s[j], s[j + 1]), up = i8_scaled(u[j], u[j + 1], sx2, su[j], su[j + 1]);
-              const float2 r = args.o.act ? make_float2(gelu_tanh_f(g.x) * up.x, gelu_tanh_f(g.y) * up.y) : silu_mul2(g, up);
+              const float2 g = i8_scaled2(v[j], v[j + 1], sx2, s[j], s[j + 1]), up = i8_scaled2(u[j], u[j + 1], sx2, su[j], su[j + 1]);
+              const float2 r = i8_gated2(g, up, args.o.act);
               y[j] = r.x;
               y[j + 1] = r.y;
             }
@@ -643,7 +629,7 @@ __device__ __forceinline__ void i8_pair_body(const CUtensorMap& tmX, const CUten
           if (some) {
 #pragma unroll
             for (int j = 0; j < 32; j += 2) {
-              const float2 r = i8_scaled(v[j], v[j + 1], sx2, s[j], s[j + 1]);
+              const float2 r = i8_scaled2(v[j], v[j + 1], sx2, s[j], s[j + 1]);
               y[j] = r.x;
               y[j + 1] = r.y;
             }

@@ -6,14 +6,14 @@
 // the first weights' way from memory: a kernel, a launch and a buffer less.
 //
 // A warp per feature (gate and up: two), whose lanes read 16 bytes each, eight times ahead; sums over lanes by one integer reduction, so the order changes
-// nothing and the results are those of the other kernels, bit by bit (but for the gate's exponential, which is expf here).
+// nothing and the results are those of the other kernels, bit by bit (i8_epilogue.cuh).
 //
 // us, bf16 rows, here and on the tensor cores: one token by 6144 x 4096 6.7 and 9.4 (the bytes' floor 3.9), by 4096 x 4096 5.2 and 8.2, by 4096 x 14336 14.5 and
 // 17.0, by 2 x 14336 x 4096 22.4 and 26.7; two tokens 9.5 and 9.8, 6.5 and 8.5, 18.1 and 17.1, 24.4 and 26.9.  Three and four rows were slower in every CTA's own
 // way into 8 bits (four by 6144 x 4096 13.4 and 9.3), and in 8 bits already no faster (8.2 and 7.3).
 #include "api.h"
-#include "activations.cuh"
 #include "i8_args.h"
+#include "i8_epilogue.cuh"
 #include "quant_rows.cuh"
 
 namespace nkb {
@@ -163,14 +163,13 @@ __global__ void __launch_bounds__(kFewThreads, 2) i8_few_kernel(const FewArgs a)
         if (GATED) up = sum[GATED ? 1 : 0][m];
       }
     if (lane < M) {
-      float y = float(mine) * sx * __ldg(a.sw + n);
+      float y = i8_scaled(mine, sx, __ldg(a.sw + n));
       const long long at = lane * a.ldo + n;
       if constexpr (GATED) {
-        const float u = float(up) * sx * __ldg(a.sw + a.n + n);
-        y = apply_act(y, a.act ? ACT_GELU_TANH : ACT_SILU) * u;
+        y = i8_gated(y, i8_scaled(up, sx, __ldg(a.sw + a.n + n)), a.act);
       } else {
-        if (a.bias) y += __bfloat162float(a.bias[n]);
-        if (a.residual) y += __bfloat162float(a.residual[at]);
+        if (a.bias) y = add_rn(y, __bfloat162float(a.bias[n]));
+        if (a.residual) y = add_rn(y, __bfloat162float(a.residual[at]));
       }
       if (a.fp32) reinterpret_cast<float*>(a.out)[at] = y;
       else reinterpret_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16(y);

@@ -600,3 +600,37 @@ def test_many_gated_rows(dtype, t, k):
     q, rows = ops.silu_mul(x, quantize=True), ops.silu_mul(x.cuda(), quantize=True)
     assert torch.equal(rows.values.cpu(), q.values)
     assert bool(((rows.scale.cpu().double() - q.scale.double()).abs() <= 2 * U24 * q.scale.double()).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["plain", "bias", "residual", "fp32", "silu", "gelu_tanh", "parts"])
+@pytest.mark.parametrize("n,k,size", [(512, 1024, 1.0), (257, 700, 1.0), (512, 1024, 30.0), (300, 512, 1e-30)])
+def test_a_token_has_the_same_bits_in_every_batch(form, n, k, size):
+    """One and two tokens on the CUDA cores, few of them on narrow tiles with and without a cluster, prompts on pairs: the tokens that they share are the
+    same, for gates of tens too, and for scales that bring results below the normal numbers of 32 bits."""
+    g = draws(n + k)
+    rows = 700
+    gated = form in ("silu", "gelu_tanh")
+    x = ops.quantize_rows((size * rows_like_a_layers(g, rows, k).float()).to(BF).cuda())
+    w = weight_like(g, 2 * n if gated else n, k)
+    w = ops.QuantizedWeight.of((w.float() * (1e-8 if size < 1e-3 else 1.0)).to(BF).cuda())
+    bias = rows_like_a_layers(g, 1, n)[0].cuda() if form in ("bias", "residual", "parts") else None
+    residual = rows_like_a_layers(g, rows, n).cuda()
+    ys = {}
+    for m in (1, 2, 3, 16, 30, 64, 128, 300, 700):
+        kw = dict(gated=True, act=form) if gated else dict(bias=bias)
+        if form == "residual":
+            kw["residual"] = residual[:m]
+        if form in ("fp32", "parts"):
+            kw["fp32_out"] = True
+        if form == "parts":
+            kw["splits"] = 3
+        ys[m] = ops.linear(ops.QuantizedRows(x.values[:m], x.scale[:m]), w, **kw)
+    for m, y in ys.items():
+        assert torch.equal(y, ys[700][:, :m] if form == "parts" else ys[700][:m]), m
+    if form not in ("parts", "residual"):
+        # whole products, k in one piece: fp32 rows go the same way
+        bf = (size * rows_like_a_layers(draws(n + k), rows, k).float()).to(BF).cuda()
+        kw = dict(gated=True, act=form) if gated else dict(bias=bias, fp32_out=form == "fp32")
+        for m in (1, 2, 64):
+            assert torch.equal(ops.linear(bf[:m], w, **kw), ys[700][:m])
