@@ -264,6 +264,7 @@ def silu_mul(gate_up, limit: float = 0.0, alpha: float = 1.702, bias=None) -> Qu
             v = v + bias.double()
         g, u = v[:, :width], v[:, width:]
         if limit > 0:
+            limit, alpha = torch.tensor([limit, alpha], dtype=_F32).tolist()         # (as the kernel has them)
             g, u = g.clamp(max=limit), u.clamp(-limit, limit)
             y = (u + 1) * g / (1 + torch.exp(-alpha * g))
         else:

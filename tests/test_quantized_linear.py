@@ -634,3 +634,15 @@ def test_a_token_has_the_same_bits_in_every_batch(form, n, k, size):
         kw = dict(gated=True, act=form) if gated else dict(bias=bias, fp32_out=form == "fp32")
         for m in (1, 2, 64):
             assert torch.equal(ops.linear(bf[:m], w, **kw), ys[700][:m])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_the_clamped_gates_factors_have_32_bits(device):
+    """Columns whose number is another one where alpha has 64: the same on both devices."""
+    gate = torch.tensor([[7.0, float.fromhex("-0x1.1edd34p+1"), float.fromhex("-0x1.f4e338p+0"), float.fromhex("0x1.087114p+0")]])
+    up = torch.tensor([[7.0, float.fromhex("-0x1.63d0d8p+2"), float.fromhex("0x1.216e64p+1"), float.fromhex("0x1.c09ff8p+0")]])
+    alpha = float(torch.tensor(1.702))
+    y = (up.double() + 1) * gate.double() / (1 + torch.exp(-alpha * gate.double()))
+    rows = ops.silu_mul(torch.cat([gate, up], 1).to(device), limit=7.0, quantize=True)
+    check_rows(rows, y, steps=1)
+    assert rows.values.tolist() == [[127, 0, 0, 6]]
