@@ -233,7 +233,7 @@ def add_rmsnorm(x, w, *, residual_in=None, partials=None, bias=None, residual_ou
         for t in (x, bias, residual_in):
             if t is not None:
                 h = h + t.double().reshape(-1, hidden)
-        h = h.to(torch.bfloat16)
+        h = to_bf16(h)
         if residual_out is not None:
             residual_out.copy_(h.reshape(residual_out.shape))
         q, top = _numbers(h.double() * w.double())

@@ -646,3 +646,21 @@ def test_the_clamped_gates_factors_have_32_bits(device):
     rows = ops.silu_mul(torch.cat([gate, up], 1).to(device), limit=7.0, quantize=True)
     check_rows(rows, y, steps=1)
     assert rows.values.tolist() == [[127, 0, 0, 6]]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_the_stream_of_a_norm_is_rounded_once(device):
+    """Sums beside the middle of two bf16 numbers, which 32 bits hold as the middle itself."""
+    k, middle, off = 16, 2.0 ** -8, 2.0 ** -31
+    x = torch.ones((2, k), dtype=BF)
+    x[:, 8:] = -1
+    parts = torch.full((2, 2, k), off)
+    parts[0, :, :8], parts[0, :, 8:] = middle, -middle
+    parts[1, 1] = -off
+    w = torch.ones(k, dtype=BF)
+    h, rows = ops.add_rmsnorm(x.to(device), w.to(device), partials=parts.to(device), eps=EPS, quantize=True)
+    up = 1 + 2.0 ** -7
+    # above the middle: away from it, below: towards it; -1 - 2^-8 + 2^-31 is nearer to -1
+    want = torch.tensor([[up] * 8 + [-1.0] * 8, [1.0] * 8 + [-up] * 8])
+    assert torch.equal(h.cpu().float(), want)
+    check_rows(rows, want.double(), 1 / torch.sqrt(want.double().square().mean(-1) + EPS), steps=64)
