@@ -6,7 +6,7 @@
 // (numbers8 in quant_rows.cuh) takes the nearest k by a rounding constant and looks at what is left of it, which is exact, too.
 //   norm   The norm's factor r = 1 / sqrt(mean(h^2) + eps) is the same for the whole row: 127 (r h w) / max|r h w| = 127 (h w) / max|h w|.  So the numbers
 //          come from the exact products h * w, and r enters the scale alone: no rounding of statistics can move a number to its neighbour.
-//   gate   silu(g) * u is not exact in 32 bits.  Numbers within 2^-12 of a half (one in two thousand; 2^-13 where gate and up are no sums) and candidates for the row's maximum are worked out
+//   gate   silu(g) * u is not exact in 32 bits.  Columns whose gate is far below zero (kFar), numbers within 2^-12 of a half (one in two thousand; 2^-13 where gate and up are no sums) and candidates for the row's maximum are worked out
 //          once more in 64 bits; rows that are small altogether, and the clamped form, whose up + 1 may cancel, in 64 bits as a whole.
 // A row with a value that is not finite gets the scale NaN and zeros; a row of zeros the scale 0.
 //
@@ -26,6 +26,12 @@ constexpr float kGateSmall = 1.f / (1 << 20);   // rows with a smaller maximum a
 __device__ __forceinline__ float min_nan(float a, float b) {
   float d;
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+__device__ __forceinline__ float fmin3(float a, float b, float c) {
+  float d;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 
@@ -105,6 +111,15 @@ __device__ __forceinline__ float reciprocal(float v) {
   asm("rcp.approx.f32 %0, %1;" : "=f"(d) : "f"(v));
   return d;
 }
+
+// Whether gate and up are what memory has, and no rounded sums or clamped ones.
+__device__ __forceinline__ bool gates_given(const NkbQuantRows& a) { return !a.bias && a.limit <= 0.f && a.splits <= 1; }
+// Below these arguments of the sigmoid the 32-bit error of a gated value is not what numbers are decided by: the exponential multiplies the rounding of a sum by its
+// argument (at -20 the value is off by 28 * 2^-24, a number by 2^-12.2; at -88 by 96 * 2^-24, less than half of the margin for the row's maximum), and beyond -88 it
+// leaves the range of 32 bits.  A thread that has such a gate takes its columns in 64 bits.  Sums have some at times: only where gate times up is so large (kLift) that the
+// column is more than 2^-28.4, four tenths of a unit of any row that is not in 64 bits as a whole; otherwise its number is zero, however far off the value.
+constexpr float kFar = -20.f, kFarGiven = -80.f, kLift = 1.5f;
+__device__ __forceinline__ float far_edge(const NkbQuantRows& a) { return gates_given(a) ? kFarGiven : kFar; }
 
 // Gate times up of one column in 64 bits.
 template <int FORM>
@@ -215,9 +230,10 @@ __device__ __forceinline__ void store8_moved(__nv_bfloat16* row, int c, int widt
     if (j >= from && j < to && c + j < width) reinterpret_cast<uint16_t*>(o)[j] = uint16_t(h[j >> 1] >> (16 * (j & 1)));
 }
 
-// What the 8 columns from c on are rounded from.  Norm: stores the residual stream, and adds its squares to ss.
+// What the 8 columns from c on are rounded from.  Norm: stores the residual stream, and adds its squares to ss.  Gate: lowers least to the least argument of the
+// sigmoid (of sums: where up lifts it again).
 template <int FORM, bool VEC>
-__device__ __forceinline__ void load8(const NkbQuantRows& a, long long row, int c, const Raw8<FORM>& raw, float (&v)[8], float& ss) {
+__device__ __forceinline__ void load8(const NkbQuantRows& a, long long row, int c, const Raw8<FORM>& raw, float (&v)[8], float& ss, float& least) {
   if constexpr (FORM == NKB_ROW_BF16) {
     values8_bf16(raw.r[0], v);
   } else if constexpr (FORM == NKB_ROW_F32) {
@@ -277,17 +293,29 @@ __device__ __forceinline__ void load8(const NkbQuantRows& a, long long row, int 
       v[j] = x[j] * w[j];
     }
   } else {
-    float g[8], u[8];
+    float g[8], u[8], low = 0.f;
     load8_gate<FORM, VEC>(a, row, c, raw, g, u);
     if (a.limit > 0.f) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float gl = min_nan(g[j], a.limit), ul = max_nan(min_nan(u[j], a.limit), -a.limit);
-        v[j] = __fdividef((ul + 1.f) * gl, 1.f + expf(-a.alpha * gl));
+        g[j] = min_nan(g[j], a.limit);
+        u[j] = max_nan(min_nan(u[j], a.limit), -a.limit) + 1.f;
+        const float z = a.alpha * g[j];
+        low = fminf(low, z);
+        v[j] = __fdividef(g[j], 1.f + expf(-z)) * u[j];        // (in this order: the product of both may leave the range)
       }
     } else {
 #pragma unroll
+      for (int j = 0; j < 8; j += 2) low = fmin3(low, g[j], g[j + 1]);
+#pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = g[j] * reciprocal(1.f + expf(-g[j])) * u[j];
+    }
+    if constexpr (FORM == NKB_ROW_GATE_BF16) {
+      least = fminf(least, low);
+    } else if (low < far_edge(a)) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if ((a.limit > 0.f ? a.alpha * g[j] : g[j]) < far_edge(a) && fabsf(g[j] * u[j]) > kLift) least = -INFINITY;
     }
     // columns past the width read as zeros
     if (c + 8 > a.width) {
@@ -342,13 +370,14 @@ __global__ void __maxnreg__(row_registers(FORM, IT)) quant_rows_kernel(const Nkb
   for (int turn = 0; row < a.rows; row += CLUSTER ? a.rows : gridDim.x, turn ^= 1) {
   float v[kKeep ? IT : 1][8];
   float big = 0.f, ss = 0.f;              // largest magnitude, NaN if there is one
+  float least = 0.f;
   uint32_t big16 = 0;
   if constexpr (kKeep) {
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
       const int ch = chunk0 + threadIdx.x + it * blockDim.x;
       if (ch >= chunks) continue;
-      load8<FORM, VEC>(a, row, ch * 8, raw[it], v[it], ss);
+      load8<FORM, VEC>(a, row, ch * 8, raw[it], v[it], ss, least);
       if constexpr (FORM == NKB_ROW_BF16) {
         // magnitudes of bf16 are ordered as their bits are: two to a word
         const uint4 w = raw[it].r[0];
@@ -364,11 +393,12 @@ __global__ void __maxnreg__(row_registers(FORM, IT)) quant_rows_kernel(const Nkb
   } else {
     for (int ch = chunk0 + threadIdx.x; ch < chunks; ch += blockDim.x) {
       fetch8<FORM, VEC>(a, row, ch * 8, raw[0], true);
-      load8<FORM, VEC>(a, row, ch * 8, raw[0], v[0], ss);
+      load8<FORM, VEC>(a, row, ch * 8, raw[0], v[0], ss, least);
 #pragma unroll
       for (int j = 0; j < 8; ++j) big = max_nan(big, fabsf(v[0][j]));
     }
   }
+  const bool far = kGate && least < far_edge(a);        // this thread's columns are worked out in 64 bits
   // wide rows: the columns once more.  The residual stream may lie in the place of what it was made of.
   NkbQuantRows again_a = a;
   if (!kKeep && FORM == NKB_ROW_NORM && a.residual_out) {
@@ -393,12 +423,12 @@ __global__ void __maxnreg__(row_registers(FORM, IT)) quant_rows_kernel(const Nkb
         raw[0].r[0] = make_uint4(w[0], w[1], w[2], w[3]);
         raw[0].r[1] = make_uint4(0u, 0u, 0u, 0u);
         raw[0].r[2] = fetch8_bf16<VEC>(a.w, ch * 8, a.width);
-        load8<FORM, VEC>(again_a, row, ch * 8, raw[0], v[0], none);
+        load8<FORM, VEC>(again_a, row, ch * 8, raw[0], v[0], none, none);
         return;
       }
     }
     fetch8<FORM, VEC>(again_a, row, ch * 8, raw[0], true);
-    load8<FORM, VEC>(again_a, row, ch * 8, raw[0], v[0], none);
+    load8<FORM, VEC>(again_a, row, ch * 8, raw[0], v[0], none, none);
   };
   if (kKeep && FORM == NKB_ROW_BF16) big = __uint_as_float(max(big16 << 16, big16 & 0xffff0000u));
   uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(big));      // infinities and NaN lie above all numbers
@@ -416,7 +446,7 @@ __global__ void __maxnreg__(row_registers(FORM, IT)) quant_rows_kernel(const Nkb
   if constexpr (kGate) {
     // the exact maximum of this CTA's columns, of the values that may be it
     if (top < 0x7f800000u) {
-      const float mine = __uint_as_float(top), near = small(mine) ? 0.f : mine * (1.f - 1.f / (1 << 18));
+      const float mine = __uint_as_float(top), near = small(mine) ? 0.f : mine * (1.f - 1.f / (1 << 16));
       double best = 0.0;
 #pragma unroll
       for (int it = 0; it < (kKeep ? IT : 1 << 30); ++it) {
@@ -425,7 +455,7 @@ __global__ void __maxnreg__(row_registers(FORM, IT)) quant_rows_kernel(const Nkb
         if constexpr (!kKeep) once_more(ch);
         uint32_t some = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) some |= fabsf(v[kKeep ? it : 0][j]) >= near && ch * 8 + j < a.width ? 1u << j : 0u;
+        for (int j = 0; j < 8; ++j) some |= (far || fabsf(v[kKeep ? it : 0][j]) >= near) && ch * 8 + j < a.width ? 1u << j : 0u;
 #pragma unroll 1
         for (; some; some &= some - 1u) best = fmax(best, fabs(gate_exact<FORM>(a, row, ch * 8 + __ffs(some) - 1)));
       }
@@ -453,14 +483,14 @@ __global__ void __maxnreg__(row_registers(FORM, IT)) quant_rows_kernel(const Nkb
     m64 = __shfl_sync(0xffffffffu, m64, 0);
   }
   const bool fine = top < 0x7f800000u;
-  const bool in64 = kGate && small(__uint_as_float(top));       // the whole row in 64 bits
   const float m = kGate ? float(m64) : __uint_as_float(top);
+  const bool in64 = kGate && (small(__uint_as_float(top)) || m > 1e18f);       // the whole row in 64 bits
   if (threadIdx.x == 0 && (!CLUSTER || blockIdx.x == 0)) {
     float scale = kGate ? float(m64 / 127.0) : m / 127.f;
     if constexpr (FORM == NKB_ROW_NORM) scale *= rsqrtf(ss / float(a.width) + a.eps);
     a.scale[row] = fine ? scale : __uint_as_float(0x7fffffffu);
   }
-  const float near_half = a.bias || a.limit > 0.f || a.splits > 1 ? kNearHalfGated : kNearHalfGatedOnce;
+  const float near_half = gates_given(a) ? kNearHalfGatedOnce : kNearHalfGated;
   // Rows whose m or 127 / m is at an end of the range: every number by the comparison, scaled by a power of two.
   const bool odd = odd_row(m);
   const float inv = odd ? 0.f : 127.f / m;
@@ -484,7 +514,7 @@ __global__ void __maxnreg__(row_registers(FORM, IT)) quant_rows_kernel(const Nkb
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         packed[i] = __byte_perm(__byte_perm(t[4 * i], t[4 * i + 1], 0x0040), __byte_perm(t[4 * i + 2], t[4 * i + 3], 0x0040), 0x5410);
-      if (in64) again = m64 > 0.0 ? 255u : 0u;
+      if (in64 || far) again = m64 > 0.0 ? 255u : 0u;
 #pragma unroll 1
       for (; again; again &= again - 1u) {
         const int j = __ffs(again) - 1;

@@ -4,9 +4,10 @@
 
 namespace nkb {
 
-// Distance from a whole number beyond which a gated one is decided in 64 bits: half, less 127 times the error of a gated value in 32 bits.  That is 2^-20 where gate
-// and up are rounded sums (the exponential multiplies the gate's rounding by it), and below 2^-21 where both are given (the exponential, 1 +, the
-// quotient, the product); the row's largest and its quotient add 2^-23.
+// Distance from a whole number beyond which a gated one is decided in 64 bits: half, less 127 times the error of a gated value in 32 bits and that of its
+// quotient by the row's largest, 2 * 2^-24.  The value's is 28 * 2^-24 where gate and up are rounded sums (the exponential multiplies the gate's rounding by the gate, -20 at
+// the least: gates below are in 64 bits from the start, kFar in quant_rows.cu), and below 2^-21 where both are given (the exponential, 1 +, the quotient,
+// the product).
 constexpr float kNearHalfGated = 0.5f - 1.f / 4096, kNearHalfGatedOnce = 0.5f - 1.f / (1 << 13);
 __device__ __forceinline__ float max_nan(float a, float b) {
   float d;

@@ -664,3 +664,51 @@ def test_the_stream_of_a_norm_is_rounded_once(device):
     want = torch.tensor([[up] * 8 + [-1.0] * 8, [1.0] * 8 + [-up] * 8])
     assert torch.equal(h.cpu().float(), want)
     check_rows(rows, want.double(), 1 / torch.sqrt(want.double().square().mean(-1) + EPS), steps=64)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("t,k", [(24, 131000), (3, 24), (5, 1001), (64, 14336), (330, 928), (700, 2880)])
+def test_sums_of_gates_far_below_zero(device, t, k):
+    """Gates between -80 and -65, which ups of e^65 and more lift to numbers again: the exponential makes 80 roundings of the gate's one."""
+    g = draws(t + k)
+    x = torch.randn((2, t, 2 * k), generator=g)
+    gate = -65 - 15 * torch.rand((t, k), generator=g)
+    x[0, :, :k], x[1, :, :k] = gate, 0.1 * x[1, :, :k]
+    x[0, :, k:] *= torch.exp(-gate)
+    got = ops.silu_mul(x.to(device), quantize=True)
+    v = x.double().sum(0)
+    check_rows(got, v[:, :k] * torch.special.expit(v[:, :k]) * v[:, k:], steps=1)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("form", ["bf16", "f32", "parts"])
+@pytest.mark.parametrize("t,k", [(4, 24), (6, 999), (5, 2880), (64, 14336), (4, 20000), (1300, 300)])
+def test_gates_beyond_the_range_of_the_exponential(device, form, t, k):
+    """exp(88) is the last one that 32 bits hold: gates down to -100 and ups up to 1e38, ahead of the row's other columns, among them and alone."""
+    g = draws(t * k)
+    x = torch.randn((t, 2 * k), generator=g)
+    far = torch.rand((t, k), generator=g) < 0.1
+    far[0], far[1] = True, False
+    x[:, :k] = torch.where(far, -80 - 20 * torch.rand((t, k), generator=g), x[:, :k])
+    lift = torch.exp2(100 + 26 * torch.rand((t, k), generator=g))
+    x[:, k:] = torch.where(far, x[:, k:] * lift * torch.tensor([1.0, 1.0, 1e-4, 1e-12]).repeat(t)[:t, None], x[:, k:])
+    x[:, k:] = x[:, k:].clamp(-3e38, 3e38)
+    x = x.to(BF) if form == "bf16" else x
+    given = torch.stack([x, torch.zeros_like(x)]) if form == "parts" else x
+    got = ops.silu_mul(given.to(device), quantize=True)
+    v = x.double()
+    check_rows(got, v[:, :k] * torch.special.expit(v[:, :k]) * v[:, k:], steps=1)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_clamped_gates_whose_product_leaves_the_range(device, dtype):
+    """(up + 1) * gate is beyond 32 bits where the gate is -1e38; its sigmoid is zero.  A gate of minus infinity is not a number, here as elsewhere."""
+    x = torch.tensor([[-1e38, 3.0, -0.5, 2.0, 7.0, 5.0, -1.0, 3.0], [-1e38] * 4 + [7.0] * 4, [-float("inf"), 1, 1, 1, 7, 1, 1, 1], [-30, 1, -16, 2, 7, 1, 1, 1]]).to(dtype)
+    alpha = float(torch.tensor(1.702))
+    got = ops.silu_mul(x.to(device), limit=7.0, quantize=True)
+    v = x.double()
+    gate, up = v[:, :4].clamp(max=7), v[:, 4:].clamp(-7, 7)
+    y = (up + 1) * gate / (1 + torch.exp(-alpha * gate))
+    check_rows(got, y, steps=1)
+    assert got.scale.isnan().cpu().tolist() == [False, False, True, False]
