@@ -33,7 +33,7 @@ peagle_config = _load("peagle_config", os.path.join(HERE, "config.py"))
 
 from nkipy_b200.models.engine import GenerationEngine  # noqa: E402
 from nkipy_b200.models.runner import (add_common_args, build_model, build_prompts, kv_dtype, load_tokenizer,  # noqa: E402
-                                      quantize_weights)
+                                      quantize_weights, refuse_rules)
 from nkipy_b200.models.speculative import DrafterLM, SpeculativeEngine, random_drafter_weights  # noqa: E402
 from nkipy_b200.models.weights import load_shard  # noqa: E402
 from nkipy_b200.parallel.comm import TPGroup  # noqa: E402
@@ -45,6 +45,7 @@ def main():
     ap.add_argument("-k", "--num-draft-tokens", type=int, default=3)
     ap.add_argument("--draft-checkpoint", default=None, help="directory with the prepared drafter shard")
     args = ap.parse_args()
+    refuse_rules(args)
     tp = TPGroup.from_env()
     cfg = get_config(args.model)
     target = build_model(cfg, args, tp)

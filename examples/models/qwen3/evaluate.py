@@ -23,13 +23,15 @@ from config import get_config  # noqa: E402
 
 from nkipy_b200.models.engine import GenerationEngine  # noqa: E402
 from nkipy_b200.models.reference import EagerTransformer  # noqa: E402
-from nkipy_b200.models.runner import add_common_args, build_prompts, kv_dtype, load_tokenizer, quantize_weights  # noqa: E402
+from nkipy_b200.models.runner import (add_common_args, build_prompts, kv_dtype, load_tokenizer, quantize_weights,  # noqa: E402
+                                      refuse_rules)
 from nkipy_b200.models.transformer import TransformerLM  # noqa: E402
 from nkipy_b200.models.weights import load_shard, random_weights  # noqa: E402
 from nkipy_b200.parallel.comm import TPGroup  # noqa: E402
 
 
 def evaluate(cfg, args):
+    refuse_rules(args)
     tp = TPGroup.from_env()
     dev = tp.device
     weights = (load_shard(args.checkpoint, tp.rank, device=dev) if args.checkpoint

@@ -66,6 +66,12 @@ def sampling_of(args) -> Sampling:
                     args.presence_penalty)
 
 
+def refuse_rules(args) -> None:
+    """For commands that compare greedy answers: their engines do not choose under penalties."""
+    if sampling_of(args).ruled:
+        raise ValueError("this command generates without repetition, frequency and presence penalties")
+
+
 def load_tokenizer(path: Optional[str]):
     if not path:
         return None

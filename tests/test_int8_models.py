@@ -301,3 +301,16 @@ def test_blocks_are_forgotten():
     a.release(blocks)
     a.publish(tokens, kept, 70)
     assert a.admit(tokens[:40])[0][0] == kept[0]
+
+
+@pytest.mark.parametrize("script", ["qwen3/evaluate.py", "gpt_oss/peagle/speculate.py"])
+def test_commands_that_generate_without_rules_refuse_them(script):
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    for flag in ("--repetition-penalty", "--presence-penalty"):
+        r = subprocess.run([sys.executable, os.path.join(root, "examples", "models", script), "--layers", "1", flag, "1.5"], capture_output=True, text=True,
+                           cwd=root, env=dict(os.environ, PYTHONPATH=root), timeout=300)
+        assert r.returncode and "penalties" in r.stderr.splitlines()[-1]
