@@ -314,3 +314,81 @@ def test_commands_that_generate_without_rules_refuse_them(script):
         r = subprocess.run([sys.executable, os.path.join(root, "examples", "models", script), "--layers", "1", flag, "1.5"], capture_output=True, text=True,
                            cwd=root, env=dict(os.environ, PYTHONPATH=root), timeout=300)
         assert r.returncode and "penalties" in r.stderr.splitlines()[-1]
+
+
+# ------------------------------------------------------------------------------------------------ decode steps of one and two sequences
+class WatchedFew(Watched):
+    """Sums of few rows come to the norm as [rows, columns], without an axis of parts."""
+
+    def __init__(self, monkeypatch):
+        norm = ops.quantized_linear.add_rmsnorm
+        super().__init__(monkeypatch)
+        self.whole = 0
+
+        def checked_norm(x, w, **kw):
+            before = {k: v.cpu().double() for k, v in dict(kw, x=x).items() if torch.is_tensor(v) and k != "residual_out"}
+            h, rows = norm(x, w, **kw)
+            total = sum((before[k].reshape(rows.shape) for k in ("x", "residual_in") if k in before),
+                        torch.zeros(rows.shape, dtype=torch.float64))
+            if "partials" in before:
+                self.whole += before["partials"].dim() == 2
+                total = total + (before["partials"] if before["partials"].dim() == 2 else before["partials"].sum(0))
+            if "bias" in before:
+                total = total + before["bias"]
+            total = ops.quantized_linear.to_bf16(total)
+            if h is not None:
+                assert torch.equal(h.cpu().reshape(total.shape), total)
+            check_rows(rows, total.double() * w.cpu().double(), 1 / torch.sqrt(total.double().square().mean(-1) + kw["eps"]), steps=64)
+            self.norms += 1
+            return h, rows
+
+        monkeypatch.setattr(ops.quantized_linear, "add_rmsnorm", checked_norm)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("kind", sorted(KINDS))
+@pytest.mark.parametrize("kv", [None, E4M3])
+@pytest.mark.parametrize("batch", [1, 2, 4])
+def test_decode_steps_of_few_sequences(device, kind, kv, batch, monkeypatch):
+    """Every product and norm of decode steps with as many rows as the kernel for few tokens takes, and with more."""
+    model = model_of(kind, device)
+    engine = GenerationEngine(model, max_batch=batch, max_seq_len=96, use_cuda_graph=False, enable_prefix_sharing=False, kv_dtype=kv)
+    seqs = [engine.open_request() for _ in range(batch)]
+    engine.run_step([StepEntry(s, ids(30 + i, i), [-1]) for i, s in enumerate(seqs)])
+    seen = WatchedFew(monkeypatch)
+    for step in range(3):
+        logits = engine.run_step([StepEntry(s, ids(1, 10 * step + i), [0]) for i, s in enumerate(seqs)])
+        assert bool(logits.isfinite().all())
+    assert seen.products == 3 * (2 * 4 + 1) and seen.norms == 3 * 4
+    # (sums where k is divided: both layers' projection back, and the feed-forward's ahead of a norm in 8 bits)
+    assert seen.whole == (3 * (2 * (model.split_o > 1) + (model.split_down > 1)) if batch <= 2 else 0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("kind", sorted(KINDS))
+@pytest.mark.parametrize("kv", [None, E4M3])
+def test_a_sequence_decodes_alike_alone_and_beside_others(device, kind, kv):
+    """The logits of one sequence's decode steps with one, two and four rows: products have the same bits, sums of parts and attention are rounded elsewhere."""
+    model = model_of(kind, device)
+    logits = []
+    for batch in (1, 2, 4):
+        engine = GenerationEngine(model, max_batch=batch, max_seq_len=96, enable_prefix_sharing=False, kv_dtype=kv)
+        seqs = [engine.open_request() for _ in range(batch)]
+        engine.run_step([StepEntry(s, ids(30 + i, i)) for i, s in enumerate(seqs)])
+        logits.append(torch.stack([engine.run_step([StepEntry(s, ids(1, 10 * step + i), [0]) for i, s in enumerate(seqs)])[0].float().cpu()
+                                   for step in range(3)]))
+    # (a number of a row may go to its neighbour where a sum is rounded the other way: as far as 8 bits take the logits, 0.08, at the very most; another
+    # position, cache page or row is off by more than 1)
+    for other in logits[1:]:
+        assert float((other - logits[0]).norm() / logits[0].norm()) < 0.08
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", sorted(KINDS))
+@pytest.mark.parametrize("kv", [None, E4M3])
+@pytest.mark.parametrize("batch", [1, 2])
+def test_captured_steps_of_few_sequences_are_the_same(kind, kv, batch):
+    model = model_of(kind, "cuda")
+    prompts = [ids(70, 1), ids(3, 2)][:batch]
+    outs = [GenerationEngine(model, max_batch=batch, max_seq_len=160, use_cuda_graph=g, kv_dtype=kv).generate(prompts, 12) for g in (False, True)]
+    assert outs[0] == outs[1]
