@@ -94,6 +94,8 @@ class Sampling:
         for v in (self.frequency, self.presence):
             if not abs(v) < float("inf"):
                 raise ValueError("penalties are numbers")
+        if any(v != v for v in (self.biases or {}).values()):
+            raise ValueError("biases are numbers, or infinite")
 
     @property
     def ruled(self) -> bool:
@@ -105,6 +107,9 @@ class StepRules:
 
     def __init__(self, sampling: Sampling, vocab: int, rows: int, width: int, device):
         self.sampling, self.vocab, self.device = sampling, vocab, device
+        # rows may have a token that is certain, and none at all
+        self.lifted = any(v == float("inf") for v in (sampling.biases or {}).values())
+        self.may_end = sampling.allowed is not None or sum(v == -float("inf") for v in (sampling.biases or {}).values()) == vocab
         n = len(sampling.biases or {})
         if any(not 0 <= int(t) < vocab for t in sampling.biases or {}):
             raise ValueError("biases are for tokens of the vocabulary")
@@ -159,7 +164,9 @@ class StepRules:
         if s.temperature <= 0:
             return ops.argmax(logits, out_ids=out_ids, rules=rules)
         left = ops.apply_rules(logits, rules)
-        if s.allowed is None:
+        if self.lifted:
+            left.clamp_(max=1e30)          # (far above all others; divided by a temperature, and with another taken off, it stays a number)
+        if not self.may_end:
             return GenerationEngine._sample(left, s, step, out_ids)
         # (there is no drawing from nothing)
         none = ops.argmax(left, rules=ops.LogitRules()) < 0

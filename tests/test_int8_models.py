@@ -392,3 +392,22 @@ def test_captured_steps_of_few_sequences_are_the_same(kind, kv, batch):
     prompts = [ids(70, 1), ids(3, 2)][:batch]
     outs = [GenerationEngine(model, max_batch=batch, max_seq_len=160, use_cuda_graph=g, kv_dtype=kv).generate(prompts, 12) for g in (False, True)]
     assert outs[0] == outs[1]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_drawing_of_tokens_with_infinite_biases(device):
+    """A token that is certain, two of them, one that may not come all the same, and nothing to draw from."""
+    model = model_of("llama", device, False)
+    engine = GenerationEngine(model, max_batch=2, max_seq_len=64)
+    inf, prompts = float("inf"), [ids(9, 1), ids(20, 2)]
+    for temperature in (0.0, 0.7, 2.0):
+        warm = dict(temperature=temperature, seed=4)
+        assert engine.generate(prompts, 4, sampling=Sampling(biases={7: inf, 9: 3.0}, **warm)) == [[7] * 4] * 2
+        assert engine.generate(prompts, 4, sampling=Sampling(biases={7: inf}, top_k=5, top_p=0.9, **warm)) == [[7] * 4] * 2
+        two = [t for o in (engine.generate(prompts, 24, sampling=Sampling(biases={7: inf, 500: inf}, **warm))) for t in o]
+        assert set(two) == ({7, 500} if temperature else {7})
+        out = engine.generate(prompts, 3, sampling=Sampling(biases={7: inf}, allowed=lambda p, a: [3, 5], **warm))
+        assert {t for o in out for t in o} <= {3, 5}
+        assert engine.generate(prompts, 3, sampling=Sampling(biases={t: -inf for t in range(512)}, **warm)) == [[], []]
+    with pytest.raises(ValueError):
+        Sampling(biases={3: float("nan")})
