@@ -77,7 +77,7 @@ class Sampling:
     """temperature <= 0: greedy; top_k 0 and top_p 1: unrestricted.
 
     Rules on the logits ahead of either (`ops.LogitRules`): repetition, frequency and presence penalties, biases {token: value}, and
-    allowed(prompt, answer) -> the ids (or a bool [vocab]) that a sequence may go on with, None: any; where that is none, it ends."""
+    allowed(prompt, answer) -> the ids (or truth values [vocab]; tensors, arrays, lists, ids as any collection) that a sequence may go on with, None: any; where that is none, it ends."""
     temperature: float = 0.0
     top_k: int = 0
     top_p: float = 1.0
@@ -142,11 +142,14 @@ class StepRules:
             if ids is None:
                 bits[i] = True
                 continue
-            ids = ids.cpu() if torch.is_tensor(ids) else torch.tensor(list(ids), dtype=torch.int64)
-            if ids.dtype is not torch.bool:
-                if ids.numel() and not 0 <= int(ids.min()) <= int(ids.max()) < self.vocab:
+            ids = ids.cpu() if torch.is_tensor(ids) else torch.from_numpy(np.array(ids if isinstance(ids, (np.ndarray, list, tuple)) else list(ids)))
+            if ids.dtype is torch.bool:
+                if ids.shape != (self.vocab,):
+                    raise ValueError("truth values of tokens want one for each of the vocabulary")
+            else:
+                whole, ids = not ids.is_floating_point(), ids.long()
+                if ids.numel() and not (whole and 0 <= int(ids.min()) <= int(ids.max()) < self.vocab):
                     raise ValueError("a sequence may go on with tokens of the vocabulary")
-                ids = ids.long()
             bits[i, ids] = True
         at = torch.tensor(list(rows), device=self.device)
         self.rules.mask.index_copy_(0, at, ops.pack_mask(bits).to(self.device))

@@ -411,3 +411,28 @@ def test_drawing_of_tokens_with_infinite_biases(device):
         assert engine.generate(prompts, 3, sampling=Sampling(biases={t: -inf for t in range(512)}, **warm)) == [[], []]
     with pytest.raises(ValueError):
         Sampling(biases={3: float("nan")})
+
+
+def test_forms_of_what_a_grammar_allows():
+    """Ids and truth values as tensors, arrays, lists and other collections are the same masks; others are refused."""
+    import numpy as np
+
+    from nkipy_b200.models.engine import StepRules
+
+    mask = np.arange(70) % 3 == 1
+    some = np.flatnonzero(mask)
+    forms = [mask, mask.tolist(), tuple(mask), torch.from_numpy(mask), some, some.astype(np.int32), some.astype(np.uint16), some.tolist(), tuple(some), set(some.tolist()),
+             torch.from_numpy(some), torch.from_numpy(some).int(), range(1, 70, 3), (int(t) for t in some), {int(t): None for t in some}.keys()]
+    for form in forms:
+        rules = StepRules(Sampling(allowed=lambda p, a: form), 70, 2, 8, "cpu")
+        rules.allow([1], [[1]], [[]])
+        assert rules.rules.mask[0].tolist() == [-1] * 3
+        assert torch.equal(rules.rules.mask[1:], ops.pack_mask(torch.from_numpy(mask)[None])), type(form)
+    for none in ([], (), np.array([], dtype=np.int64), set(), torch.zeros(0), np.zeros(70, dtype=bool), iter([])):
+        rules = StepRules(Sampling(allowed=lambda p, a: none), 70, 2, 8, "cpu")
+        rules.allow([0], [[1]], [[]])
+        assert rules.rules.mask.tolist() == [[0] * 3, [-1] * 3]
+    for bad in (mask[:69], mask[None], [True] * 71, torch.ones(71, dtype=torch.bool), [1.5], np.array([2.0]), [70], {-1}, torch.tensor([3.0])):
+        rules = StepRules(Sampling(allowed=lambda p, a: bad), 70, 2, 8, "cpu")
+        with pytest.raises(ValueError):
+            rules.allow([0], [[1]], [[]])
