@@ -336,8 +336,8 @@ struct WorkI8 {
 };
 // group_m row tiles share a sweep over the column tiles, so that both operands are read again from L2; the splits of a tile follow one another.
 //
-// The slabs' bounds come from the split even where there is one.  With a loop from zero to a kernel argument nvcc 12.9 no longer keeps the operands of the
-// MMAs in uniform registers: an MMA then takes 65 cycles to issue and not 16, and 200 tokens by 4096 x 14336 40 us and not 25.
+// The slabs' bounds come from the split even where there is one.  With a loop from zero to a kernel argument (nvcc 12.9) an MMA takes 65 cycles to issue and not
+// 16, and 200 tokens by 4096 x 14336 40 us and not 25.
 __device__ __forceinline__ WorkI8 i8_work(const I8PairArgs& a, int w) {
   WorkI8 o;
   o.sp = w % a.splits;
@@ -726,9 +726,15 @@ static int resident_pairs(int dev, cudaLaunchConfig_t cfg) {
 }
 
 // Columns of a tile.  A pair takes its tiles one after another, so a narrower tile wins where it makes the rounds come out even.  us per slab of a tile
-// (measured, 200 tokens by 4096 x 14336): at 256 columns both operands' 32 KB per CTA and slab are what L2 gives an SM (52 bytes per clock), narrower
-// ones wait for the MMAs' and loads' latencies.  414 tokens by 2 x 14336 x 4096, us: 52.1 at 256, 50.0 at 192, 49.5 at 160, 54.7 at 128; 200 by 4096 x 4096
-// 17.5 at 256, 12.0 at 128, 11.2 at 64; 2048 by 4096 x 14336 79.8 at 256, 92 at 128.
+// (taken at 200 tokens by 4096 x 14336): at 256 columns both operands' 32 KB per CTA and slab are what L2 gives an SM (52 bytes per clock), narrower
+// ones wait for the MMAs' and loads' latencies.  us at every width; the rule's choice is within 3 % of the best one:
+//   columns                              256    224    192    160    128     96     64   chosen
+//    200 tokens by 14336 x 4096         20.4   19.6   22.6   22.2   20.7   24.8   29.2     19.6
+//    300 by 6144 x 4096                 18.4   17.3   15.7   19.6   18.9   18.2   22.3     15.7
+//    414 by 2 x 14336 x 4096            48.0   49.1   47.4   48.5   52.6   61.6   80.6     48.4
+//   1024 by 4096 x 4096                 18.3   20.3   20.5   19.6   18.8   23.4   27.5     18.2
+//   1024 by 2 x 14336 x 4096            86.1   88.7   87.9   93.4   97.2  115.5  148.7     88.8
+//   2048 by 4096 x 14336                78.6   90.2   85.0   81.8   92.1  106.4  137.1     79.0
 static int pair_width(int tiles_m, int splits, int slabs, int columns, bool gated, int pairs, float* us_out) {
   static const struct { int width; float us; } kSlab[] = {{256, 0.326f}, {224, 0.287f}, {192, 0.250f}, {160, 0.224f}, {128, 0.207f}, {96, 0.200f}, {64, 0.192f}};
   int best = 256;

@@ -5,9 +5,11 @@
 // most 24 bits where |x| and m have 16, so the comparison is exact in 32 bits for bf16 rows and for products of two bf16 numbers.  The form that runs
 // (numbers8 in quant_rows.cuh) takes the nearest k by a rounding constant and looks at what is left of it, which is exact, too.
 //   norm   The norm's factor r = 1 / sqrt(mean(h^2) + eps) is the same for the whole row: 127 (r h w) / max|r h w| = 127 (h w) / max|h w|.  So the numbers
-//          come from the exact products h * w, and r enters the scale alone: no rounding of statistics can move a number to its neighbour.
-//   gate   silu(g) * u is not exact in 32 bits.  Columns whose gate is far below zero (kFar), numbers within 2^-12 of a half (one in two thousand; 2^-13 where gate and up are no sums) and candidates for the row's maximum are worked out
-//          once more in 64 bits; rows that are small altogether, and the clamped form, whose up + 1 may cancel, in 64 bits as a whole.
+//          come from the exact products h * w, and r enters the scale alone: no rounding of statistics can move a number to its neighbour.  (Rows whose largest
+//          product is below 2^-125 have products that 32 bits round, and may have a number's neighbour.)
+//   gate   silu(g) * u is not exact in 32 bits.  Columns whose gate is far below zero (kFar), numbers within 2^-12 of a half (one in two thousand; 2^-13 where
+//          gate and up are no sums) and candidates for the row's maximum are worked out once more in 64 bits; rows that are small altogether, and the clamped
+//          form, whose up + 1 may cancel, in 64 bits as a whole.
 // A row with a value that is not finite gets the scale NaN and zeros; a row of zeros the scale 0.
 //
 // The numbers are thus the same for every order of the sums and every launch shape, and equal those of the CPU.
@@ -15,6 +17,9 @@
 // Layout: a CTA per row, or a cluster where there are few and long gated ones, whose parts meet through distributed shared memory; eight neighbouring
 // columns per thread and turn, kept in registers between the pass for the maximum and the one that writes; rows too wide for them are
 // computed twice.
+//
+// us in a graph (bytes at 6544 GB/s): bf16 rows as they are, 64 x 4096 1.7, 16384 x 4096 57 (31), 16384 x 14336 226 (108); fp32 4096 x 4096 14.4 (12.8),
+// 16384 x 4096 52 (51); a norm of one, two, four and eight sums of 64 x 4096 2.9, 3.2, 5.3, 7.6, of 128 x 4096 3.3, 4.2, 5.5, 7.9.
 #include "api.h"
 #include "i8_args.h"
 #include "quant_rows.cuh"

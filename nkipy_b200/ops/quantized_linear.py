@@ -7,7 +7,7 @@ scale NaN and zeros, a row of zeros the scale 0.
 A factor for every token and every output channel, because both leave the sum over k: ``y = (sum_k q_x q_w) * scale_x * scale_w``, whose
 sum is exact.  The numbers of a row are decided exactly too (quant_rows.cu), so a row has the same numbers whichever kernel, or the
 reference on the CPU, made them.  Behind a norm they come from the products h * w of the residual stream and the norm's weights, which
-are exact; the norm's factor is one for the row and goes into its scale.
+are exact (of rows whose largest product is 2^-125 or more); the norm's factor is one for the row and goes into its scale.
 
     QuantizedRows     rows of activations: `quantize_rows`, or `rmsnorm`, `add_rmsnorm` and `silu_mul` with quantize=True
     QuantizedWeight   a weight, which `linear` takes in the place of a bf16 one
