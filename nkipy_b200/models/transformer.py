@@ -142,10 +142,12 @@ class TransformerLM:
             raise ValueError("weights in 8 bits are for dense models on one rank")
         if not self.quantized:
             self.weights_version += 1
+            # (those that are, where a call before this one ran out of memory, stay)
+            of = lambda w: w if isinstance(w, ops.QuantizedWeight) else ops.QuantizedWeight.of(w)  # noqa: E731
             for lw in self.layers:
                 for name in ("qkv", "o", "gate_up", "down"):
-                    setattr(lw, name, ops.QuantizedWeight.of(getattr(lw, name)))
-            self.lm_head = ops.QuantizedWeight.of(self.lm_head)
+                    setattr(lw, name, of(getattr(lw, name)))
+            self.lm_head = of(self.lm_head)
             self.quantized = True
             self.cluster_gemm = self.fix_gemm = False          # (kernels of bf16 weights)
         return self

@@ -436,3 +436,24 @@ def test_forms_of_what_a_grammar_allows():
         rules = StepRules(Sampling(allowed=lambda p, a: bad), 70, 2, 8, "cpu")
         with pytest.raises(ValueError):
             rules.allow([0], [[1]], [[]])
+
+
+def test_quantising_goes_on_where_it_stopped(monkeypatch):
+    model, whole = model_of("llama", "cpu", quantize=False), model_of("llama", "cpu")
+    of, calls = ops.QuantizedWeight.of, []
+
+    def short_of_memory(w):
+        calls.append(w)
+        if len(calls) == 4:
+            raise torch.OutOfMemoryError("no more")
+        return of(w)
+
+    with monkeypatch.context() as m:
+        m.setattr(ops.QuantizedWeight, "of", short_of_memory)
+        with pytest.raises(torch.OutOfMemoryError):
+            model.quantize_weights()
+        assert not model.quantized
+        model.quantize_weights()
+    assert model.quantized and len(calls) == 4 * 2 + 1 + 1
+    outs = [GenerationEngine(m, max_batch=1, max_seq_len=64).generate([ids(9, 1)], 4) for m in (model, whole)]
+    assert outs[0] == outs[1]
